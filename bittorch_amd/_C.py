@@ -784,6 +784,75 @@ def rmsnorm(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6, store
     return out if rs is None else (*out, rs.reshape(x.shape[:-1]))
 
 
+def _add_rmsnorm_checks(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor]) -> int:
+    _check(x.dim() >= 1 and x.numel() > 0, "x is empty")
+    _check(x.dtype in _DT, "x must be float32, float16 or bfloat16")
+    K = x.shape[-1]
+    if residual is not None:
+        _check(residual.shape == x.shape, "residual shape doesn't match x")
+        _check(residual.dtype in (x.dtype, torch.float32), "residual must have x's dtype or be float32")
+        _check(residual.device == x.device, "All tensors must be CUDA")
+    if weight is not None:
+        _check(weight.dim() == 1 and weight.shape[0] == K, "weight must be 1D [K]")
+        _check(weight.dtype in (x.dtype, torch.float32), "weight must have x's dtype or be float32")
+        _check(weight.device == x.device, "All tensors must be CUDA")
+    _check(x.is_cuda, "All tensors must be CUDA")
+    return K
+
+
+def add_rmsnorm(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor] = None, eps: float = 1e-6, store: bool = True,
+                quantize: bool = False, operand_order: bool = False, return_rowsum: bool = False, return_rstd: bool = False):
+    """``s = x + residual`` and its RMSNorm in one pass: ``(s, y)``, with ``quantize`` ``(s, y, Q, s_x)`` or, ``store=False``,
+    ``(s, Q, s_x)``; ``return_rowsum`` and ``return_rstd`` append the rows' sums of ``Q`` and their reciprocal root mean squares.
+    ``s`` has the residual's dtype (``x``'s or fp32) and is ``x`` itself without a residual."""
+    K = _add_rmsnorm_checks(x, residual, weight)
+    _check(store or quantize, "nothing to compute: store and quantize are both False")
+    _check(quantize or not return_rowsum, "return_rowsum needs quantize=True")
+    x2 = _rows_2d(x, K)
+    r2 = None if residual is None else _rows_2d(residual, K)
+    w = None if weight is None else weight.contiguous()
+    B, dev, lead = x2.shape[0], x.device, x.shape[:-1]
+    s = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=dev)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev) if store else None
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev) if quantize else None
+    s_x = torch.empty(lead, dtype=torch.float32, device=dev) if quantize else None
+    rs = torch.empty(lead, dtype=torch.int32, device=dev) if return_rowsum else None
+    rstd = torch.empty((B,), dtype=torch.float32, device=dev) if return_rstd else None
+    with _on(x):
+        _status(_L.bt_add_rmsnorm(
+            x2.data_ptr(), x2.stride(0), _DT[x.dtype], _ptr(r2), 0 if r2 is None else r2.stride(0), 0 if r2 is None else _DT[r2.dtype],
+            _ptr(w), 0 if w is None else _DT[w.dtype], float(eps), B, K, None if residual is None else s.data_ptr(), _ptr(y), _ptr(rstd),
+            _ptr(q), _ptr(s_x), _ptr(rs), 1 if operand_order else 0, _stream(x)))
+    return tuple(t for t in (s, y, q, s_x, rs, rstd) if t is not None)
+
+
+def add_rmsnorm_backward(s: Tensor, rstd: Tensor, weight: Optional[Tensor], d_sum: Optional[Tensor], d_norm: Tensor,
+                         want_x: bool = True, want_residual: bool = True, want_weight: bool = True
+                         ) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """Gradients ``(x, residual, weight)`` of :func:`add_rmsnorm`'s ``s`` and ``y`` from the stored ``s`` and ``rstd``; those of
+    ``x`` and ``residual`` are one tensor where their dtypes are the same."""
+    K = _add_rmsnorm_checks(d_norm, s, weight)
+    _check(d_sum is None or (d_sum.shape == s.shape and d_sum.dtype == s.dtype and d_sum.device == s.device),
+           "the sum's gradient must match the sum")
+    B = s.numel() // K
+    _check(rstd.dtype == torch.float32 and rstd.numel() == B and rstd.device == s.device, "rstd must be fp32 [B]")
+    _check(not want_weight or weight is not None, "no weight to differentiate")
+    _check(want_x or want_residual or want_weight, "no gradient requested")
+    s, rstd, d_norm = s.contiguous(), rstd.contiguous(), d_norm.contiguous()
+    d_sum = None if d_sum is None else d_sum.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    dev, one = s.device, s.dtype == d_norm.dtype
+    dr = torch.empty(s.shape, dtype=s.dtype, device=dev) if want_residual or (one and want_x) else None
+    dx = torch.empty(s.shape, dtype=d_norm.dtype, device=dev) if want_x and not one else None
+    dw = torch.empty((K,), dtype=weight.dtype, device=dev) if want_weight else None
+    with _on(s):
+        ws = _workspace(_L.bt_add_rmsnorm_backward_workspace_bytes(B, K), dev) if want_weight else None
+        _status(_L.bt_add_rmsnorm_backward(
+            s.data_ptr(), _DT[s.dtype], rstd.data_ptr(), _ptr(weight), 0 if weight is None else _DT[weight.dtype], d_norm.data_ptr(),
+            _DT[d_norm.dtype], _ptr(d_sum), B, K, _ptr(dx), _ptr(dr), _ptr(dw), _ptr(ws), 0 if ws is None else ws.numel(), _stream(s)))
+    return (dr if one and want_x else dx), (dr if want_residual else None), dw
+
+
 def unpack_dequant(W_T: Tensor, in_features: int, scale: Optional[Tensor] = None,
                    out_dtype: torch.dtype = torch.float32) -> Tensor:
     """Dense ``[N, K]`` weights from packed ``W_T``: ``decode * scale[:, None]``

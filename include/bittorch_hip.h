@@ -49,8 +49,8 @@ typedef enum {
  * At present bt_ternary_linear_tensor_core_forward uses one (the int8 activations
  * and their row scales), bt_ternary_linear_packed_forward uses one for small
  * batches of fp32 activations (three bf16 planes), its fused and tiled forms also
- * one for a prologue that runs as its own kernel, and bt_linear_grad_weight and
- * bt_linear_grad_weight_16 one for partial sums; bt_ternary_gemm_i8 keeps the argument so that a kernel that needs
+ * one for a prologue that runs as its own kernel, and bt_linear_grad_weight,
+ * bt_linear_grad_weight_16 and bt_add_rmsnorm_backward one for partial sums; bt_ternary_gemm_i8 keeps the argument so that a kernel that needs
  * scratch can be introduced without an ABI change.
  */
 /* ABI version of the loaded library (BT_ABI_VERSION at build time). */
@@ -221,6 +221,28 @@ int bt_swiglu_rowsum(const void* gate, int64_t ld_gate, const void* up, int64_t 
                      int64_t K, void* H, int8_t* Q, float* s_x, int32_t* q_rowsum, int q_layout, void* stream);
 int bt_rmsnorm_rowsum(const void* X, int64_t ld_x, const void* weight, float eps, int dtype, int64_t B,
                       int64_t K, void* Y, int8_t* Q, float* s_x, int32_t* q_rowsum, int q_layout, void* stream);
+
+/*
+ * The residual connection and the norm behind it in one pass, and their gradient (no counterpart in the reference's Python/CUDA
+ * code; pre-norm block of its JS runtime, TernaryTransformer.ts:489-521):
+ *   sum = rd_r(X + residual),   Y = rd_x( (sum * r) * weight ),   r = 1/sqrt(float(sum_k double(sum)^2)/K + eps)
+ * i.e. bit for bit an addition followed by bt_rmsnorm of the stored sum; Q, s_x, q_rowsum (each optional, Y too as long as Q is
+ * given): Y quantized per row as bt_act_quant_i8 would.  residual (row stride ld_r) and sum [B,K] are of r_dtype: x_dtype or
+ * BT_F32; residual NULL: sum is X itself and is not written.  weight [K] of w_dtype (x_dtype or BT_F32) or NULL (ones).
+ * rstd (optional) [B]: the rows' r, for the gradient.
+ *   bt_add_rmsnorm_backward: for the gradients dSum (r_dtype, or NULL: zero) and dY (x_dtype) of the two outputs
+ *     d = dSum + r (dY weight - xhat mean_k(dY weight xhat)),  xhat = sum * r;  dWeight = sum over the rows of dY xhat
+ *   d goes to dX in x_dtype and to dResidual in r_dtype, where they are not NULL; dWeight [K] in w_dtype or NULL.  All of them
+ *   [B,K] contiguous; sums over rows are made in an order that depends on the shape alone.
+ *   workspace (with dWeight): at least bt_add_rmsnorm_backward_workspace_bytes(B,K) bytes.
+ */
+int bt_add_rmsnorm(const void* X, int64_t ld_x, int x_dtype, const void* residual, int64_t ld_r, int r_dtype, const void* weight,
+                   int w_dtype, float eps, int64_t B, int64_t K, void* sum, void* Y, float* rstd, int8_t* Q, float* s_x,
+                   int32_t* q_rowsum, int q_layout, void* stream);
+size_t bt_add_rmsnorm_backward_workspace_bytes(int64_t B, int64_t K);
+int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, const void* weight, int w_dtype, const void* dY,
+                            int x_dtype, const void* dSum, int64_t B, int64_t K, void* dX, void* dResidual, void* dWeight,
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Packed forward with an activation prologue (no counterpart in the reference's Python/CUDA code;
