@@ -853,6 +853,87 @@ def add_rmsnorm_backward(s: Tensor, rstd: Tensor, weight: Optional[Tensor], d_su
     return (dr if one and want_x else dx), (dr if want_residual else None), dw
 
 
+def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, up_bias: Optional[Tensor] = None,
+                  threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, rows: bool = False, back: bool = False):
+    """The operands of the gated pair, of two masters ``[F, K]`` quantized as :func:`ternary_quantize_pack` does: ``(W_pairs, W_back,
+    scale, bias)`` as ``bt_gated_weights`` makes them; ``rows``: ``W_rows [ceil(K/4), 2 F]`` in the first place; ``back``: with the copy
+    for the input's gradient (otherwise None)."""
+    _check(gate.dim() == 2 and gate.shape == up.shape and gate.dtype == up.dtype, "gate and up weights must match, 2D [F, K]")
+    _check(gate.numel() > 0, "weight is empty")
+    _check(not as_half or gate.dtype == torch.float32, "as_half takes fp32 weights")
+    F, K = gate.shape
+    for b in (gate_bias, up_bias):
+        _check(b is None or (b.dim() == 1 and b.shape[0] == F), "bias shape mismatch")
+    _check(_all_cuda(gate, up, gate_bias, up_bias), "All tensors must be CUDA")
+    dev, Kb = gate.device, (K + 3) // 4
+    wdt = _F32_AS_F16 if as_half else _dt(gate, "weight")
+    masters = [t.detach().contiguous() for t in (gate, up)]
+    biases = [None if b is None else b.detach() for b in (gate_bias, up_bias)]
+    if any(b is not None for b in biases):
+        bdt = next(b.dtype for b in biases if b is not None)
+        bdt = bdt if bdt in _DT and all(b is None or b.dtype == bdt for b in biases) else torch.float32
+        biases = [None if b is None else b.to(bdt).contiguous() for b in biases]
+    Fv = F if rows else (F + 15) // 16 * 16
+    packed = torch.empty((2, Kb, F), dtype=torch.uint8, device=dev)
+    scales = torch.empty((2, F if per_channel else 1), dtype=torch.float32, device=dev)
+    w = torch.empty((Kb, 2 * F) if rows else (_L.bt_tiled_weights_bytes(2 * Fv, K),), dtype=torch.uint8, device=dev)
+    w_back = torch.empty((_L.bt_tiled_weights_bytes(K, 2 * Fv),), dtype=torch.uint8, device=dev) if back and not rows else None
+    scale = torch.empty((2 * Fv + 1,), dtype=torch.float32, device=dev)
+    has_bias = any(b is not None for b in biases)
+    bias = torch.empty((2 * Fv,), dtype=torch.float32, device=dev) if has_bias else None
+    with _on(gate):
+        st = _stream(gate)
+        for i, m in enumerate(masters):
+            _status(_L.bt_quantize_pack(m.data_ptr(), wdt, F, K, float(threshold_factor), int(bool(per_channel)), packed[i].data_ptr(),
+                                        scales[i].data_ptr(), None, st))
+        _status(_L.bt_gated_weights(packed[0].data_ptr(), packed[1].data_ptr(), scales[0].data_ptr(), scales[1].data_ptr(),
+                                    scales.shape[1], _ptr(biases[0]), _ptr(biases[1]), _DT[bdt] if has_bias else 0, F, K,
+                                    None if rows else w.data_ptr(), _ptr(w_back), w.data_ptr() if rows else None, scale.data_ptr(),
+                                    _ptr(bias), st))
+    return w, w_back, scale, bias
+
+
+def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optional[Tensor], out_features: int,
+                          want_pre: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """``silu(gate) * up`` ``[B, F]`` of 16-bit rows ``[B, K]`` (K % 8 == 0, zeros behind a shorter weight row) on the operands of
+    :func:`gated_weights`, and with ``want_pre`` the two projections ``[B, 2 Fp]`` fp32 as :func:`gated_grad` reads them."""
+    _check(X.dim() == 2 and X.numel() > 0 and X.dtype in (torch.float16, torch.bfloat16), "X must be 2D fp16 or bf16")
+    B, K = X.shape
+    F, Fp = out_features, (out_features + 15) // 16 * 16
+    _check(W_pairs.dtype == torch.uint8 and W_pairs.dim() == 1 and W_pairs.is_contiguous()
+           and W_pairs.numel() == _L.bt_tiled_weights_bytes(2 * Fp, K), "W_pairs size doesn't match out_features x in_features")
+    _check(scale.dtype == torch.float32 and scale.numel() >= 2 * Fp and (bias is None or (bias.dtype == torch.float32 and bias.numel() >= 2 * Fp)),
+           "scale and bias must be fp32 with an entry for each padded feature")
+    _check(_all_cuda(X, W_pairs, scale, bias), "All tensors must be CUDA")
+    X, scale, bias = X.contiguous(), scale.contiguous(), None if bias is None else bias.contiguous()
+    h = torch.empty((B, F), dtype=X.dtype, device=X.device)
+    pre = torch.empty((B, 2 * Fp), dtype=torch.float32, device=X.device) if want_pre else None
+    with _on(X):
+        _status(_L.bt_ternary_gated_forward(X.data_ptr(), _DT[X.dtype], W_pairs.data_ptr(), scale.data_ptr(), _ptr(bias), h.data_ptr(),
+                                            _ptr(pre), B, F, K, _stream(X)))
+    return h, pre
+
+
+def gated_grad(dH: Tensor, pre: Tensor, scale: Optional[Tensor], bias_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Optional[Tensor]]:
+    """Gradient of ``silu(gate) * up`` in both projections, ``[B, 2 Fp]`` in 16 bits times their scales, or ``[B, 2 F]`` fp32 without
+    (``pre`` then is ``[gate | up]``); with ``bias_dtype`` also its sums over the rows ``[2 F]``, without scales."""
+    _check(dH.dim() == 2 and dH.numel() > 0 and dH.dtype in _DT, "dH must be 2D float32, float16 or bfloat16")
+    B, F = dH.shape
+    Fv = F if dH.dtype == torch.float32 else (F + 15) // 16 * 16
+    _check(pre.dtype == torch.float32 and pre.shape == (B, 2 * Fv) and pre.is_contiguous(), "the projections must be fp32 [B, 2 F]")
+    _check(dH.dtype == torch.float32 or (scale is not None and scale.dtype == torch.float32 and scale.numel() >= 2 * Fv and scale.is_contiguous()),
+           "scale must be fp32 with an entry for each padded feature")
+    _check(_all_cuda(dH, pre, scale), "All tensors must be CUDA")
+    dH = dH.contiguous()
+    G = torch.empty((B, 2 * Fv), dtype=dH.dtype, device=dH.device)
+    db = None if bias_dtype is None else torch.empty((2 * F,), dtype=bias_dtype, device=dH.device)
+    with _on(dH):
+        ws = None if db is None else _workspace(_L.bt_gated_grad_workspace_bytes(B, F), dH.device)
+        _status(_L.bt_gated_grad(dH.data_ptr(), _DT[dH.dtype], pre.data_ptr(), _ptr(scale), G.data_ptr(), _ptr(db),
+                                 0 if db is None else _DT[bias_dtype], B, F, _ptr(ws), 0 if ws is None else ws.numel(), _stream(dH)))
+    return G, db
+
+
 def unpack_dequant(W_T: Tensor, in_features: int, scale: Optional[Tensor] = None,
                    out_dtype: torch.dtype = torch.float32) -> Tensor:
     """Dense ``[N, K]`` weights from packed ``W_T``: ``decode * scale[:, None]``

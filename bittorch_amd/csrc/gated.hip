@@ -1,0 +1,338 @@
+// The gated pair of a feed-forward block in training, for gfx950:
+//
+//   g = a_g (x T_g^T) + b_g,   u = a_u (x T_u^T) + b_u,   h = silu(g) u = g u / (1 + exp(-g))
+//
+// with T = ternary(W), a = the rows' absolute maxima of two full-precision masters W [F, K] (straight-through gradient, as
+// bittorch/nn/ternary_linear_cuda.py:73-111; block structure of the JS runtime, js/src/models/TernaryTransformer.ts:366-423).
+// Its gradient, with sig = 1 / (1 + exp(-g)) and incoming dh:
+//
+//   dg = dh u sig (1 + g (1 - sig)),  du = dh g sig
+//   dx = (a_g dg) T_g + (a_u du) T_u,   dW_g = (a_g dg)^T x,  db_g = sum_rows dg,   likewise for up
+//
+// 16-bit rows: one product forms both projections and h in its output stage (gemm_f16.hip, OUT_GATED) on the tiled copy in pair
+// order.  One pass (gated_grad_kernel) makes G = [a_g dg | a_u du] of dh and the kept projections, rounded once to 16 bits as an operand
+// of the matrix cores; it serves both products behind it: dx = G [T_g; T_u] on a second tiled copy of the codes, in which the contraction
+// runs over the output features, by the forward's kernel, and dW = G^T x by the weight gradient's (grad_w16.hip).  a times dg, not
+// dg, is what is rounded, so that neither product has a scale of its own.
+// fp32 rows: the same steps on the fp32 kernels, G without the scales, which those kernels apply.
+//
+// Features are padded to Fp = F rounded up to 16 where the matrix cores read them: zero codes, scales and biases, zero columns of G.
+#include "row_vec.h"
+
+namespace bt {
+
+int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, float* pre, int64_t H, int64_t M,
+                          int64_t N, int64_t K, hipStream_t st);
+bool gemm_f16_supported(int64_t N, int64_t K, const void* X, const void* W_T, const void* Y, bool tiled);
+
+// ---- the two layers' packed weights as one operand ----------------------------------------------------------------------
+
+struct GatedWeightsParams {
+    const uint8_t* W[2];      // gate, up: packed [ceil(K / 4), F]
+    const float* a[2];        // their scales: F entries or one
+    const void* b[2];         // biases or null
+    int bias_dtype, one_scale;
+    int64_t F, Fv, K, Kb;     // Fv: features of a half in the outputs (F, or F padded)
+    uint8_t* pairs;           // forward: tiled copy in pair order of [gate | up], 2 Fv columns
+    uint8_t* back;            // backward: tiled copy of the transpose: K columns, contraction over 2 Fv
+    uint8_t* rows;            // or both as they lie, side by side: [Kb, 2 F]
+    float* scale;             // [2 Fv + 1], the last one 1 (the scale of products that have none)
+    float* bias;              // [2 Fv] or null
+    uint32_t n_pairs, n_back, n_rows;  // workgroups of each part, in this order; one more for the vectors
+    uint32_t steps, back_steps;        // 64-wide steps of the two tiled copies
+};
+
+// 16 packed bytes n .. n + 15 of a row of F, zeros past its end
+__device__ __forceinline__ u32x4 codes16(const uint8_t* row, int64_t n, int64_t F) {
+    if (n + 16 <= F) return *(const u32x4_a1*)(row + n);
+    u32x4 d = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+        if (n + e < F) d[e >> 2] |= (uint32_t)row[n + e] << (8 * (e & 3));
+    return d;
+}
+
+// Bound by the packed bytes, read once for each copy and written once; all parts in one launch.
+__global__ __launch_bounds__(256) void gated_weights_kernel(GatedWeightsParams p) {
+    constexpr int PITCH = 256 + 16;
+    __shared__ __attribute__((aligned(16))) uint8_t block[16 * PITCH];
+    uint32_t wg = blockIdx.x;
+    const int tid = threadIdx.x;
+    if (wg < p.n_pairs) {
+        // 16 packed rows (a step) of 256 features of one half, through LDS: retile_kernel with the order of the pairs
+        const uint32_t steps = p.steps, per_half = p.n_pairs / 2;
+        const int half = wg >= per_half;
+        wg -= half ? per_half : 0u;
+        const int64_t s = wg % steps, n0 = (int64_t)(wg / steps) * 256;
+        {
+            const int r = tid >> 4, c = 16 * (tid & 15);
+            const int64_t kb = 16 * s + r;
+            u32x4 d = {0u, 0u, 0u, 0u};
+            if (kb < p.Kb) d = codes16(p.W[half] + kb * p.F, n0 + c, p.F);
+            *(u32x4*)(block + r * PITCH + c) = d;
+        }
+        __syncthreads();
+        const int tile = tid >> 4, g = (tid >> 2) & 3, j = 4 * (tid & 3);
+        const int64_t t = (n0 >> 4) + tile;
+        if (16 * t >= p.Fv) return;
+        uint32_t row[4], out[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) row[r] = *(const uint32_t*)(block + (4 * g + r) * PITCH + 16 * tile + j);
+        transpose4x4_bytes(row[0], row[1], row[2], row[3], out);
+        ((uint4*)p.pairs)[((2 * t + half) * (int64_t)steps + s) * 16 + 4 * g + (j >> 2)] = make_uint4(out[0], out[1], out[2], out[3]);
+        return;
+    }
+    wg -= p.n_pairs;
+    if (wg < p.n_back) {
+        // A thread takes the codes of 16 features at four k: byte k / 4 of the packed rows, and turns them into four dwords of the copy,
+        // column k + c with the codes of feature n + 4 r + i at bits 8 r + 2 i.  A wave: the four bytes of a tile's 16 columns, four
+        // groups of 16 features, four steps: 256 consecutive bytes of each of four rows in, 1 KiB out.
+        const uint32_t per_tile = (p.back_steps + 15) / 16;
+        const int64_t S = p.back_steps, t = wg / per_tile, s = (int64_t)(wg % per_tile) * 16 + (tid >> 4);
+        const int g = (tid >> 2) & 3, q = tid & 3;
+        if (s >= S) return;
+        const int64_t kb = 4 * t + q, n = 64 * s + 16 * g;
+        u32x4 d = {0u, 0u, 0u, 0u};
+        if (kb < p.Kb && n < 2 * p.Fv) {
+            const int half = n >= p.Fv;
+            d = codes16(p.W[half] + kb * p.F, n - (half ? p.Fv : 0), p.F);
+        }
+        uint32_t out[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint32_t x = (d[r] >> (2 * c)) & 0x03030303u;
+                out[c] |= ((x | x >> 6 | x >> 12 | x >> 18) & 0xffu) << (8 * r);
+            }
+        ((uint4*)p.back)[(t * S + s) * 16 + 4 * g + q] = make_uint4(out[0], out[1], out[2], out[3]);
+        return;
+    }
+    wg -= p.n_back;
+    if (wg < p.n_rows) {
+        const int64_t i = ((int64_t)wg * 256 + tid) * 16, per_row = (p.F + 15) / 16 * 16;  // (one row of one half: per_row / 16 threads)
+        const int64_t kb = i / (2 * per_row), n2 = i - kb * 2 * per_row;
+        if (kb >= p.Kb) return;
+        const int half = n2 >= per_row;
+        const int64_t n = n2 - (half ? per_row : 0);
+        const uint8_t* src = p.W[half] + kb * p.F;
+        uint8_t* dst = p.rows + kb * 2 * p.F + (half ? p.F : 0);
+        if (n + 16 <= p.F) *(u32x4_a1*)(dst + n) = *(const u32x4_a1*)(src + n);
+        else
+            for (int e = 0; n + e < p.F; e++) dst[n + e] = src[n + e];
+        return;
+    }
+    for (int64_t n = tid; n < 2 * p.Fv; n += 256) {
+        const int half = n >= p.Fv;
+        const int64_t f = n - (half ? p.Fv : 0);
+        p.scale[n] = f < p.F ? p.a[half][p.one_scale ? 0 : f] : 0.0f;
+        if (p.bias) p.bias[n] = f < p.F && p.b[half] ? load_elem_rt(p.b[half], p.bias_dtype, f) : 0.0f;
+    }
+    if (tid == 0) p.scale[2 * p.Fv] = 1.0f;
+}
+
+// ---- gradient of silu(g) u ------------------------------------------------------------------------------------------------
+
+struct GatedGradParams {
+    const void* dH;       // [B, F]
+    const float* pre;     // 16-bit rows: [B, 2 Fp], column pairs of gate and up in turn; fp32 rows: [B, 2 F], gate | up
+    const float* scale;   // 16-bit rows: [2 Fp]
+    void* G;              // [B, 2 Fp] / [B, 2 F]
+    float* parts;         // [gridDim.y, 2 Fp] sums of dg | du, or null
+    int64_t B, rows;      // rows: of a workgroup
+    int F, Fp;
+};
+
+// dh, g, u -> dg, du
+template <int DT>
+__device__ __forceinline__ void gated_grad_value(float dh, float g, float u, float& dg, float& du) {
+    const float sig = DT == BT_F32 ? __fdiv_rn(1.0f, __fadd_rn(1.0f, exp_fixed(-g))) : sigmoid_fast(g);
+    dg = dh * u * (sig * __builtin_fmaf(g, 1.0f - sig, 1.0f));
+    du = dh * (g * sig);
+}
+
+// A thread takes eight features of a run of rows; the biases' sums stay in its registers.  Bound by memory: dh and both projections in, G
+// out once.  RAG: F is not a multiple of 8.
+template <int DT, bool RAG>
+__global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
+    const int k = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 8, F = p.F, Fp = p.Fp;
+    if (k >= Fp) return;
+    const int64_t first = (int64_t)blockIdx.y * p.rows, last = std::min(first + p.rows, p.B);
+    float ag[8], au[8], bg[8], bu[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        ag[e] = DT != BT_F32 ? p.scale[k + e] : 1.0f;
+        au[e] = DT != BT_F32 ? p.scale[Fp + k + e] : 1.0f;
+        bg[e] = bu[e] = 0.0f;
+    }
+#pragma unroll 2
+    for (int64_t row = first; row < last; row++) {
+        float dh[8], g[8], u[8];
+        const Raw8<DT> dh_in = load_raw8<DT>(p.dH, row * F + piece_at(k, F));
+        if constexpr (DT == BT_F32) {
+            const Raw8<DT> g_in = load_raw8<DT>(p.pre, row * 2 * F + piece_at(k, F)), u_in = load_raw8<DT>(p.pre, row * 2 * F + F + piece_at(k, F));
+            widen_piece<DT, RAG>(g_in, k, F, g);
+            widen_piece<DT, RAG>(u_in, k, F, u);
+        } else {
+            const v4f* at = (const v4f*)(p.pre + row * 2 * Fp + 2 * k);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const v4f v = at[q];
+                g[2 * q] = v[0]; g[2 * q + 1] = v[1];
+                u[2 * q] = v[2]; u[2 * q + 1] = v[3];
+            }
+        }
+        widen_piece<DT, RAG>(dh_in, k, F, dh);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float dg, du;
+            gated_grad_value<DT>(dh[e], g[e], u[e], dg, du);
+            bg[e] += dg;
+            bu[e] += du;
+            g[e] = DT != BT_F32 ? dg * ag[e] : dg;
+            u[e] = DT != BT_F32 ? du * au[e] : du;
+        }
+        if constexpr (DT == BT_F32) {
+            store_piece<DT, RAG>(p.G, row * 2 * F, k, F, g);
+            store_piece<DT, RAG>(p.G, row * 2 * F + F, k, F, u);
+        } else {
+            store8u<DT>(p.G, row * 2 * Fp + k, g);
+            store8u<DT>(p.G, row * 2 * Fp + Fp + k, u);
+        }
+    }
+    if (!p.parts) return;
+    float* out = p.parts + (int64_t)blockIdx.y * 2 * F;
+    store_piece<BT_F32, RAG>(out, 0, k, F, bg);
+    store_piece<BT_F32, RAG>(out, F, k, F, bu);
+}
+
+// F < 8: element by element
+template <int DT>
+__global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p) {
+    const int k = threadIdx.x, F = p.F, Fp = p.Fp;
+    if (k >= Fp) return;
+    const int64_t first = (int64_t)blockIdx.y * p.rows, last = std::min(first + p.rows, p.B);
+    const int at_g = DT == BT_F32 ? k : 4 * (k >> 1) + (k & 1), at_u = DT == BT_F32 ? F + k : at_g + 2;
+    float bg = 0.0f, bu = 0.0f;
+    for (int64_t row = first; row < last; row++) {
+        float dg = 0.0f, du = 0.0f;
+        if (k < F) gated_grad_value<DT>(load_elem<DT>(p.dH, row * F + k), p.pre[row * 2 * Fp + at_g], p.pre[row * 2 * Fp + at_u], dg, du);
+        bg += dg;
+        bu += du;
+        store_elem<DT>(p.G, row * 2 * Fp + k, DT != BT_F32 ? dg * p.scale[k] : dg);
+        store_elem<DT>(p.G, row * 2 * Fp + Fp + k, DT != BT_F32 ? du * p.scale[Fp + k] : du);
+    }
+    if (!p.parts || k >= F) return;
+    p.parts[(int64_t)blockIdx.y * 2 * F + k] = bg;
+    p.parts[(int64_t)blockIdx.y * 2 * F + F + k] = bu;
+}
+
+static int64_t padded(int64_t F) { return ceil_div(F, 16) * 16; }
+// Runs of rows of the gradient kernel: enough workgroups for the chip; 64 at most where each leaves sums behind
+static int64_t grad_runs(int64_t B, int64_t F, bool sums) {
+    const int64_t across = ceil_div(F, 2048), want = std::max<int64_t>(1, 8 * gemm_compute_units() / across);
+    return std::min<int64_t>(B, sums ? std::min<int64_t>(want, 64) : want);
+}
+
+template <int DT>
+static void launch_gated_grad(const GatedGradParams& p, int64_t runs, hipStream_t st) {
+    if (p.F < 8) {
+        hipLaunchKernelGGL(gated_grad_narrow_kernel<DT>, dim3(1, (unsigned)runs), dim3(64), 0, st, p);
+        return;
+    }
+    const dim3 grid((unsigned)ceil_div(p.Fp, 2048), (unsigned)runs);
+    if (p.F % 8 == 0) hipLaunchKernelGGL((gated_grad_kernel<DT, false>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((gated_grad_kernel<DT, true>), grid, dim3(256), 0, st, p);
+}
+
+}  // namespace bt
+
+using namespace bt;
+
+extern "C" int bt_gated_weights(const uint8_t* gate_T, const uint8_t* up_T, const float* gate_scale, const float* up_scale, int64_t scale_len,
+                                const void* gate_bias, const void* up_bias, int bias_dtype, int64_t F, int64_t K, uint8_t* W_pairs,
+                                uint8_t* W_back, uint8_t* W_rows, float* scale, float* bias, void* stream) {
+    const char* who = "bt_gated_weights";
+    if (!gate_T || !up_T || !gate_scale || !up_scale || !scale || F <= 0 || K <= 0 || (!W_pairs && !W_rows) || (W_rows && (W_pairs || W_back))) {
+        set_error("%s: null pointer or empty shape, or both the tiled copies and the rows asked for", who);
+        return BT_ERR_INVALID;
+    }
+    if ((scale_len != F && scale_len != 1) || ((gate_bias || up_bias) && (!bias || (bias_dtype != BT_F32 && bias_dtype != BT_F16 && bias_dtype != BT_BF16)))) {
+        set_error("%s: scale size doesn't match F, or a bias without room for it or of an unsupported dtype", who);
+        return BT_ERR_INVALID;
+    }
+    const int64_t Fp = padded(F);
+    if (F >= (1ll << 23) || K >= (1ll << 23) || bt_tiled_weights_bytes(2 * Fp, K) >= (1ull << 32) || bt_tiled_weights_bytes(K, 2 * Fp) >= (1ull << 32) ||
+        (((uintptr_t)W_pairs) | ((uintptr_t)W_back)) % 256 != 0) {
+        set_error("%s: F and K below 2^23, copies 256-byte aligned and below 4 GiB (F=%lld, K=%lld)", who, (long long)F, (long long)K);
+        return BT_ERR_INVALID;
+    }
+    GatedWeightsParams p = {};
+    p.W[0] = gate_T; p.W[1] = up_T; p.a[0] = gate_scale; p.a[1] = up_scale; p.b[0] = gate_bias; p.b[1] = up_bias;
+    p.bias_dtype = bias_dtype; p.one_scale = scale_len == 1 && F != 1;
+    p.F = F; p.Fv = W_rows ? F : Fp; p.K = K; p.Kb = ceil_div(K, 4);
+    p.pairs = W_pairs; p.back = W_back; p.rows = W_rows; p.scale = scale; p.bias = bias;
+    p.steps = (uint32_t)ceil_div(p.Kb, 16); p.back_steps = (uint32_t)ceil_div(2 * Fp, 64);
+    p.n_pairs = W_pairs ? (uint32_t)(2 * ceil_div(p.Kb, 16) * ceil_div(Fp, 256)) : 0;
+    p.n_back = W_back ? (uint32_t)(ceil_div(K, 16) * ceil_div(ceil_div(2 * Fp, 64), 16)) : 0;
+    p.n_rows = W_rows ? (uint32_t)ceil_div(p.Kb * 2 * ceil_div(F, 16), 256) : 0;
+    hipLaunchKernelGGL(gated_weights_kernel, dim3(p.n_pairs + p.n_back + p.n_rows + 1), dim3(256), 0, (hipStream_t)stream, p);
+    return check_launch(who);
+}
+
+extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
+                                        float* pre, int64_t B, int64_t F, int64_t K, void* stream) {
+    const char* who = "bt_ternary_gated_forward";
+    if (!X || !W_pairs || !scale || !H || B <= 0 || F <= 0 || K <= 0 || (x_dtype != BT_F16 && x_dtype != BT_BF16)) {
+        set_error("%s: null pointer, empty shape or bad dtype (fp16 and bf16 rows)", who);
+        return BT_ERR_INVALID;
+    }
+    const int64_t Fp = padded(F);
+    if (K % 8 != 0 || F >= (1ll << 23) || B >= (1ll << 31) || ((uintptr_t)W_pairs) % 256 != 0 || bt_tiled_weights_bytes(2 * Fp, K) >= (1ull << 32) ||
+        ((uintptr_t)pre) % 16 != 0 || !gemm_f16_supported(2 * Fp, K, X, W_pairs, H, true)) {
+        set_error("%s: K must be a multiple of 8, F and K below 2^23, buffers 16-byte and the weights 256-byte aligned (F=%lld, K=%lld)", who,
+                  (long long)F, (long long)K);
+        return BT_ERR_INVALID;
+    }
+    Epilogue epi = {};
+    epi.scale = scale; epi.scale_dtype = BT_F32;
+    epi.bias = bias; epi.bias_dtype = BT_F32;
+    return launch_gemm_f16_gated(x_dtype == BT_F16 ? MODE_F16 : MODE_BF16, X, W_pairs, epi, H, pre, F, B, 2 * Fp, K, (hipStream_t)stream);
+}
+
+extern "C" size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F) {
+    return B > 0 && F > 0 ? (size_t)grad_runs(B, F, true) * 2 * (size_t)F * 4 : 0;
+}
+
+extern "C" int bt_gated_grad(const void* dH, int dtype, const float* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
+                             int64_t F, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "bt_gated_grad";
+    if (!dH || !pre || !G || B <= 0 || F <= 0 || (dtype != BT_F32 && dtype != BT_F16 && dtype != BT_BF16) || (dtype != BT_F32 && !scale)) {
+        set_error("%s: null pointer, empty shape or bad dtype", who);
+        return BT_ERR_INVALID;
+    }
+    if (F >= (1ll << 23) || B >= (1ll << 31) || (dtype != BT_F32 && (((uintptr_t)pre) | ((uintptr_t)G)) % 16 != 0)) {
+        set_error("%s: F below 2^23, B below 2^31, the projections and G 16-byte aligned", who);
+        return BT_ERR_INVALID;
+    }
+    if (dBias && (bias_dtype != BT_F32 && bias_dtype != BT_F16 && bias_dtype != BT_BF16)) {
+        set_error("%s: unsupported bias dtype", who);
+        return BT_ERR_INVALID;
+    }
+    if (dBias && (!workspace || workspace_bytes < bt_gated_grad_workspace_bytes(B, F) || ((uintptr_t)workspace) % 256 != 0)) {
+        set_error("%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, bt_gated_grad_workspace_bytes(B, F), workspace_bytes);
+        return BT_ERR_WORKSPACE;
+    }
+    GatedGradParams p = {};
+    int64_t runs = grad_runs(B, F, dBias != nullptr);
+    p.rows = ceil_div(B, runs);
+    runs = ceil_div(B, p.rows);  // (so that none is empty)
+    p.dH = dH; p.pre = pre; p.scale = scale; p.G = G; p.parts = dBias ? (float*)workspace : nullptr;
+    p.B = B; p.F = (int)F; p.Fp = dtype == BT_F32 ? (int)F : (int)padded(F);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == BT_F32) launch_gated_grad<BT_F32>(p, runs, st);
+    else if (dtype == BT_F16) launch_gated_grad<BT_F16>(p, runs, st);
+    else launch_gated_grad<BT_BF16>(p, runs, st);
+    const int rc = check_launch(who);
+    return rc || !dBias ? rc : launch_column_sum(p.parts, runs, 2 * F, dBias, bias_dtype, st, who);
+}

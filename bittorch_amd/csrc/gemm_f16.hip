@@ -48,7 +48,12 @@ struct GemmFParams {
     void* Y;              // [M, N]
     int64_t Kb;           // packed weight rows
     Epilogue epi;
+    float* pre;           // OUT_GATED: [M, N] the two projections in fp32, column pairs of gate and up in turn, or null
+    int64_t H;            // OUT_GATED: columns of Y, at most N / 2
 };
+// What becomes of a tile's sums: the linear layer's output; the SwiGLU of a layer whose columns are [gate | up], of the projections
+// rounded to the output's type; or the same of the projections as they are, in fp32, with a copy of them for the gradient.
+enum { OUT_LINEAR = 0, OUT_SWIGLU = 1, OUT_GATED = 2 };
 static_assert(offsetof(GemmFParams, Y) == 64, "first argument line as laid out above");
 
 // Stages of activations in LDS; of weights one fewer, since a wave has its own in registers half a stage before it needs them.
@@ -156,16 +161,63 @@ __device__ __forceinline__ void fd_epilogue_swiglu(const GemmFParams& p, const v
     }
 }
 
+// The training form (OUT_GATED): h = rd(silu(g) u) from the fp32 sums, one rounding, and where a backward pass follows g and u beside it.
+// They are kept in fp32: gate and up rounded to 16 bits would put two more roundings of their size into every gradient (with them
+// and the 16-bit operands of the gradient's products dx of bf16 rows is off by 2.0 times the rounding of dx itself, with fp32 by 1.4), for 28
+// bytes an output instead of 20 through memory in forward and backward.  A lane's four values of a row are 16 bytes of `pre`.
+template <int MODE, int MB>
+__device__ __forceinline__ void fd_epilogue_gated(const GemmFParams& p, const v4f (&acc)[MB][4], int64_t m0, int g, int64_t col,
+                                                  int rows_left, const float (&ws)[4], const float (&bs)[4]) {
+    constexpr int YDT = MODE == MODE_F16 ? BT_F16 : BT_BF16;
+    const int64_t row_bytes = p.H * 2;
+    char* row = (char*)p.Y + m0 * row_bytes;
+    const uint32_t lane_off = (uint32_t)(4 * g) * (uint32_t)row_bytes + (uint32_t)col * 2u;
+    float* pre = p.pre + (m0 + 4 * g) * p.N + 2 * col;
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++) {
+        if (16 * mb >= rows_left) return;  // (uniform)
+        uint32_t d[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            float y[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                float a = acc[mb][t][r];
+                if constexpr (MODE == MODE_BF16) a *= 0.5f;  // weights were decoded as +-2.0
+                y[t] = epi_float(a, ws[t], bs[t]);
+            }
+            if (p.pre && 16 * mb + 4 * g + r < rows_left)
+                st4_nt(pre + r * p.N, __builtin_bit_cast(uint32_t, y[0]), __builtin_bit_cast(uint32_t, y[1]),
+                       __builtin_bit_cast(uint32_t, y[2]), __builtin_bit_cast(uint32_t, y[3]));
+            d[r] = two_of<YDT>(y[0] * sigmoid_fast(y[0]) * y[2], y[1] * sigmoid_fast(y[1]) * y[3]);
+        }
+        if (p.H % 4 == 0) {  // (uniform; a pair of lanes has four columns that exist, or none)
+            if (col < p.H) pairs_store16(row, row_bytes, lane_off, rows_left - 16 * mb, g, d);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (16 * mb + 4 * g + r < rows_left)
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+                        if (col + t < p.H) *(uint16_t*)(row + r * row_bytes + lane_off + 2 * t) = (uint16_t)(d[r] >> (16 * t));
+        }
+        row += 16 * row_bytes;
+        pre += 16 * p.N;
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // One tile of 16 NR rows (48: a wave stages 64, the last ones repeated).  TAIL: K is not a multiple of 64 (of 8 it is): the lanes whose k lies past
 // the end load something of their own row or column instead and their activations are zeroed on the way to the MFMAs.
 // KG = 2: two groups of four waves, each on its run of the stages; they add their sums through LDS and store half the rows each
 // (of 48: 32 and 16).
-// SW: the SwiGLU output stage on a copy in gate/up pair order (stored tiles 2 i, 2 i + 1 are 16 columns of the gate and the same of up):
+// SW (OUT_SWIGLU, OUT_GATED): the output stage on a copy in gate/up pair order (stored tiles 2 i, 2 i + 1 are 16 columns of the gate and the same of up):
 // a lane takes two columns of either, so that no sum changes lanes.
-template <int MODE, int SRC, int NR, int KG, bool TAIL, bool RN, bool SW>
+template <int MODE, int SRC, int NR, int KG, bool TAIL, bool RN, int OUT>
 __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_t m0, const int tile_n, uint8_t* lds_all) {
     constexpr int NB = (NR + 1) / 2, BM = 16 * NR, A_BYTES = NB * 4096, NST = fd_stages(NB, KG), W_AT = NST * A_BYTES;
     constexpr int A_LOADS = NB, W_LOADS = SRC == W_ROWS ? 4 : 1, LOADS = A_LOADS + W_LOADS;
+    constexpr bool SW = OUT != OUT_LINEAR;
     const int lane = threadIdx.x & 63;
     const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave_all & 3, group = KG == 1 ? 0 : wave_all >> 2;
     uint8_t* const lds = lds_all + group * fd_group_bytes(NB, KG);
@@ -447,7 +499,8 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
     }
     const bool stores = SW ? scol < half_n : col_ok;
     auto store = [&](const auto& sums, int64_t row0, int left) {
-        if constexpr (SW) fd_epilogue_swiglu<MODE>(p, sums, row0, g, scol, left, ws, bs);
+        if constexpr (OUT == OUT_GATED) fd_epilogue_gated<MODE>(p, sums, row0, g, scol, left, ws, bs);
+        else if constexpr (OUT == OUT_SWIGLU) fd_epilogue_swiglu<MODE>(p, sums, row0, g, scol, left, ws, bs);
         else if (p.epi.residual) fd_epilogue<MODE, true, RN>(p, sums, row0, g, ncol, left, ws, bs);
         else fd_epilogue<MODE, false, RN>(p, sums, row0, g, ncol, left, ws, bs);
     };
@@ -478,7 +531,7 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
 }
 
 // NR: tiles of 16 NR rows.  NF > 0: an XCD's tiles from p.fine_from on are computed in tiles of 16 NF rows.
-template <int MODE, int SRC, int NR, int NF, int KG, bool TAIL, bool RN, bool SW>
+template <int MODE, int SRC, int NR, int NF, int KG, bool TAIL, bool RN, int OUT>
 __global__ __launch_bounds__(256 * KG, KG == 2 || NR == 8 ? 2 : NR == 4 ? 3 : 4) void gemm_f16_kernel(GemmFParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[KG * fd_group_bytes((NR + 1) / 2, KG)];
     // XCD-aware tile order: the 8 XCDs each take a contiguous run of tiles, walked in groups of four row tiles, so that one
@@ -500,11 +553,11 @@ __global__ __launch_bounds__(256 * KG, KG == 2 || NR == 8 ? 2 : NR == 4 ? 3 : 4)
     if constexpr (NF > 0) {
         if (fine) {
             const int64_t mf = m0 + (int64_t)(f % parts) * (16 * NF);
-            if (mf < p.M) gemm_f16_tile<MODE, SRC, NF, 1, TAIL, RN, SW>(p, mf, (int)tn, lds);
+            if (mf < p.M) gemm_f16_tile<MODE, SRC, NF, 1, TAIL, RN, OUT>(p, mf, (int)tn, lds);
             return;
         }
     }
-    gemm_f16_tile<MODE, SRC, NR, KG, TAIL, RN, SW>(p, m0, (int)tn, lds);
+    gemm_f16_tile<MODE, SRC, NR, KG, TAIL, RN, OUT>(p, m0, (int)tn, lds);
 }
 
 // X and Y are read and written in 16- and 8-byte pieces; 32-bit byte offsets span a tile's rows of X, 16 rows of Y and, for
@@ -551,9 +604,9 @@ double gemm_f16_cost(int64_t M, int64_t N, int64_t K) {
     return us;
 }
 
-template <int MODE, int SRC, int NR, bool TAIL, bool RN = false, bool SW = false>
+template <int MODE, int SRC, int NR, bool TAIL, bool RN = false, int OUT = OUT_LINEAR>
 static int launch_gemm_f16_cfg(GemmFParams p, hipStream_t st) {
-    const char* who = SRC == W_TILES ? "bt_ternary_linear_tiled_forward" : "bt_ternary_linear_packed_forward";
+    const char* who = OUT == OUT_GATED ? "bt_ternary_gated_forward" : SRC == W_TILES ? "bt_ternary_linear_tiled_forward" : "bt_ternary_linear_packed_forward";
     p.tiles_n = (int)ceil_div(p.N, F_BN);
     p.tiles_m = (int)ceil_div(p.M, 16 * NR);
     const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
@@ -570,26 +623,29 @@ static int launch_gemm_f16_cfg(GemmFParams p, hipStream_t st) {
             const int rem = p.per_xcd % (int)(2 * gemm_compute_units() / 8);
             p.fine_from = p.per_xcd - rem;
             const dim3 grid((unsigned)(8 * (p.fine_from + parts * rem)));
-            if (parts == 2) hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, 8, 4, 1, TAIL, RN, SW>), grid, block, 0, st, p);
-            else hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, 8, 2, 1, TAIL, RN, SW>), grid, block, 0, st, p);
+            if (parts == 2) hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, 8, 4, 1, TAIL, RN, OUT>), grid, block, 0, st, p);
+            else hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, 8, 2, 1, TAIL, RN, OUT>), grid, block, 0, st, p);
             return check_launch(who);
         }
     }
     if constexpr (NR != 8) {
         if (NR == 3 || (total <= gemm_compute_units() && f16_splits_k(p.wstages))) {
-            hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, NR, 0, 2, TAIL, RN, SW>), dim3((unsigned)(8 * p.per_xcd)), dim3(512), 0, st, p);
+            hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, NR, 0, 2, TAIL, RN, OUT>), dim3((unsigned)(8 * p.per_xcd)), dim3(512), 0, st, p);
             return check_launch(who);
         }
     }
-    if constexpr (NR != 3) hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, NR, 0, 1, TAIL, RN, SW>), dim3((unsigned)(8 * p.per_xcd)), block, 0, st, p);
+    if constexpr (NR != 3) hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, NR, 0, 1, TAIL, RN, OUT>), dim3((unsigned)(8 * p.per_xcd)), block, 0, st, p);
     return check_launch(who);
 }
 template <int MODE, int SRC, int NR>
 static int launch_gemm_f16_src(const GemmFParams& p, int epi_op, hipStream_t st) {
     if constexpr (SRC == W_TILES) {
         if (epi_op == EPI_SWIGLU_PAIRS)
-            return p.K % F_BK != 0 ? launch_gemm_f16_cfg<MODE, SRC, NR, true, false, true>(p, st)
-                                   : launch_gemm_f16_cfg<MODE, SRC, NR, false, false, true>(p, st);
+            return p.K % F_BK != 0 ? launch_gemm_f16_cfg<MODE, SRC, NR, true, false, OUT_SWIGLU>(p, st)
+                                   : launch_gemm_f16_cfg<MODE, SRC, NR, false, false, OUT_SWIGLU>(p, st);
+        if (p.H)
+            return p.K % F_BK != 0 ? launch_gemm_f16_cfg<MODE, SRC, NR, true, false, OUT_GATED>(p, st)
+                                   : launch_gemm_f16_cfg<MODE, SRC, NR, false, false, OUT_GATED>(p, st);
         // (rows of any length come with K of any length: one instance)
         if (p.N % 4 != 0) return launch_gemm_f16_cfg<MODE, SRC, NR, true, true>(p, st);
     }
@@ -617,6 +673,19 @@ int launch_gemm_f16(int mode, const void* X, const uint8_t* W_T, int w_layout, c
     double us;
     const int rows = gemm_f16_plan(M, N, K, &us), src = w_source(layout_tiled(w_layout), false, W_T, N);
     return mode == MODE_F16 ? launch_gemm_f16_rows<MODE_F16>(p, rows, src, epi_op, st) : launch_gemm_f16_rows<MODE_BF16>(p, rows, src, epi_op, st);
+}
+// The training form of the SwiGLU output stage: Y [M, H] = silu(g) u of the layer [gate | up] with N / 2 >= H columns each (N % 32 == 0, a
+// tiled copy in pair order), pre [M, N] or null
+int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, float* pre, int64_t H, int64_t M,
+                          int64_t N, int64_t K, hipStream_t st) {
+    GemmFParams p = {};
+    p.X = (const uint16_t*)X; p.W_T = W_tiled; p.Y = Y; p.epi = epi; p.pre = pre; p.H = H;
+    p.M = M; p.N = N; p.K = K; p.Kb = ceil_div(K, 4);
+    p.wstages = (int)ceil_div(K, F_BK);
+    p.tiles16 = tiles16_arg(N, W_LAYOUT_TILED);
+    double us;
+    const int rows = gemm_f16_plan(M, N, K, &us);
+    return mode == MODE_F16 ? launch_gemm_f16_rows<MODE_F16>(p, rows, W_TILES, 0, st) : launch_gemm_f16_rows<MODE_BF16>(p, rows, W_TILES, 0, st);
 }
 
 }  // namespace bt

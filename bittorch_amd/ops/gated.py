@@ -1,0 +1,138 @@
+"""``ternary_gated_linear``: the gated pair of a feed-forward block on full-precision masters, ``silu(gate(x)) * up(x)``, with its
+gradient.
+
+No counterpart in ``bittorch.ops``; the arithmetic is that of two ``TernaryLinear`` layers (``bittorch/nn/ternary_linear_cuda.py:23-111``)
+and of the SwiGLU between them (``js/src/models/TernaryTransformer.ts:366-423``).  Both masters are ternarised as they are read, one
+product forms both projections with ``silu(g) * u`` in its output stage, and one pass over the kept projections feeds both products
+of the gradient.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+from torch import Tensor
+
+from ..quant.ternary import ternary_quantize_ste
+
+
+def _half(t: Optional[Tensor]) -> Optional[Tensor]:
+    """What autocast does with an argument of a ternary layer: GPU floating-point tensors become fp16."""
+    return None if t is None else t.half()
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, gate: Tensor, up: Tensor, gate_bias: Optional[Tensor], up_bias: Optional[Tensor],
+                threshold_factor: float, per_channel: bool, keep: bool) -> Tensor:
+        ctx.masters = gate.dtype, None if gate_bias is None else gate_bias.dtype, None if up_bias is None else up_bias.dtype
+        ctx.x_dtype = x.dtype
+        if not torch.is_autocast_enabled("cuda"):
+            return _GatedLinear._forward(ctx, x, gate, up, gate_bias, up_bias, threshold_factor, per_channel, keep, False)
+        with torch.autocast("cuda", enabled=False):  # (as TernaryLinear: fp32 masters are rounded as the quantizer reads them)
+            as_half = gate.dtype == torch.float32
+            return _GatedLinear._forward(ctx, _half(x), gate if as_half else _half(gate), up if as_half else _half(up), _half(gate_bias),
+                                         _half(up_bias), threshold_factor, per_channel, keep, as_half)
+
+    @staticmethod
+    def _forward(ctx, x, gate, up, gate_bias, up_bias, threshold_factor, per_channel, keep, as_half) -> Tensor:
+        from .. import _C
+
+        f, k = gate.shape
+        rows = x.dtype == torch.float32
+        w, w_back, scale, bias = _C.gated_weights(gate, up, gate_bias, up_bias, threshold_factor, per_channel, as_half, rows,
+                                                  back=keep and ctx.needs_input_grad[0])
+        x2 = x.reshape(-1, k)
+        if rows:
+            # (the fp32 gradient kernels take four columns and more)
+            x2 = F.pad(x2, (0, 4 - k)) if k < 4 else x2.contiguous()
+            pre = _C.ternary_linear_packed_forward(x2, w, scale[:2 * f], bias, x2.shape[1])
+            h = _C.swiglu(pre[:, :f], pre[:, f:])
+            w_back = w
+        else:
+            if k % 8 or not x2.is_contiguous() or x2.data_ptr() % 16:
+                x2 = F.pad(x2, (0, -k % 8)) if k % 8 else x2.clone(memory_format=torch.contiguous_format)
+            h, pre = _C.ternary_gated_forward(x2, w, scale, bias, f, keep)
+        if keep:
+            ctx.save_for_backward(x2, pre, w_back, scale)
+            ctx.shape = f, k
+        return h.reshape(*x.shape[:-1], f)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh: Tensor):
+        with torch.autocast("cuda", enabled=False):  # (as the forward)
+            return _GatedLinear._backward(ctx, dh)
+
+    @staticmethod
+    def _backward(ctx, dh: Tensor):
+        from .. import _C
+
+        x2, pre, w_back, scale = ctx.saved_tensors
+        (f, k), (w_dtype, gb_dtype, ub_dtype) = ctx.shape, ctx.masters
+        want_x, want_g, want_u, want_gb, want_ub = ctx.needs_input_grad[:5]
+        lead, dh = dh.shape[:-1], dh.reshape(-1, f).contiguous()
+        dx = dg = du = dgb = dub = None
+        want_w, want_b = want_g or want_u, want_gb or want_ub
+        b_dtype = (gb_dtype if gb_dtype == ub_dtype or not want_ub else ub_dtype if not want_gb else torch.float32) if want_b else None
+        if dh.dtype == torch.float32:
+            g, db = _C.gated_grad(dh, pre, None, b_dtype)
+            if want_x:
+                dx = _C.linear_grad_input(g, w_back, scale[:2 * f], x2.shape[1])
+            if want_w:
+                dw, _ = _C.linear_grad_weight(g, x2, scale[:2 * f])
+            fv = f
+        else:
+            g, db = _C.gated_grad(dh, pre, scale, b_dtype)
+            fv = g.shape[1] // 2
+            one = scale[2 * fv:]
+            if want_x:
+                dx = _C.ternary_linear_tiled_forward(g, w_back, one, None, 2 * fv, k)
+            if want_w:
+                dw = _C.linear_grad_weight_16(g, x2, one, dh.dtype if w_dtype == dh.dtype else torch.float32)
+        if want_x:
+            dx = dx[:, :k].contiguous().reshape(*lead, k).to(ctx.x_dtype)
+        if want_w:
+            dg, du = (t.to(w_dtype).contiguous() for t in (dw[:f, :k], dw[fv:fv + f, :k]))
+        if want_b:
+            dgb, dub = db[:f].to(gb_dtype) if want_gb else None, db[f:].to(ub_dtype) if want_ub else None
+        return dx, dg if want_g else None, du if want_u else None, dgb, dub, None, None, None
+
+
+def _check_gated(x: Tensor, gate: Tensor, up: Tensor, gate_bias: Optional[Tensor], up_bias: Optional[Tensor]) -> None:
+    def check(cond: bool, msg: str) -> None:
+        if not cond:
+            raise RuntimeError(msg)
+
+    check(gate.dim() == 2 and gate.shape == up.shape and gate.dtype == up.dtype, "gate and up weights must match, 2D [F, K]")
+    check(gate.numel() > 0, "weight is empty")
+    check(x.dim() >= 1 and x.numel() > 0, "x is empty")
+    check(x.shape[-1] == gate.shape[1], "input K doesn't match weight K")
+    for b in (gate_bias, up_bias):
+        check(b is None or (b.dim() == 1 and b.shape[0] == gate.shape[0]), "bias shape mismatch")
+    check(all(t is None or t.device == x.device for t in (gate, up, gate_bias, up_bias)), "All tensors must be on one device")
+
+
+def ternary_gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate_bias: Optional[Tensor] = None,
+                         up_bias: Optional[Tensor] = None, threshold_factor: float = 0.05, per_channel: bool = True) -> Tensor:
+    """``silu(linear(x, T(gate_weight), gate_bias)) * linear(x, T(up_weight), up_bias)`` with ``T(w) = ternary_quantize(w)`` times its
+    scale: ``x`` ``(*, K)``, masters ``(F, K)``, result ``(*, F)`` in ``x``'s dtype.
+
+    On the GPU ``x`` and the masters are fp32, fp16 or bf16, in any combination; 16-bit results are rounded once, from fp32 projections.
+    Differentiable (once) in all five tensors with the straight-through gradient of ``TernaryLinear``; the gradients of the masters and
+    biases have their dtype.  Under autocast it runs in fp16, as ``TernaryLinear``.  On the CPU: the same in plain torch operations."""
+    _check_gated(x, gate_weight, up_weight, gate_bias, up_bias)
+    if not x.is_cuda:
+        g, u = (F.linear(x, (q * s.reshape(-1, 1)).to(x.dtype), None if b is None else b.to(x.dtype))
+                for (q, s), b in ((ternary_quantize_ste(w, threshold_factor, per_channel), b)
+                                  for w, b in ((gate_weight, gate_bias), (up_weight, up_bias))))
+        return F.silu(g) * u
+    kinds = (torch.float32, torch.float16, torch.bfloat16)
+    if x.dtype not in kinds or gate_weight.dtype not in kinds or any(b is not None and b.dtype not in kinds for b in (gate_bias, up_bias)):
+        raise RuntimeError("x, weights and biases must be float32, float16 or bfloat16")
+    if gate_weight.shape[0] < 2 and x.dtype == torch.float32 and not torch.is_autocast_enabled("cuda"):
+        raise RuntimeError("fp32 rows need at least 2 output features")
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate_weight, up_weight, gate_bias, up_bias))
+    return _GatedLinear.apply(x, gate_weight, up_weight, gate_bias, up_bias, threshold_factor, per_channel, keep)

@@ -1,0 +1,404 @@
+"""``ops.ternary_gated_linear``: ``silu(gate(x)) * up(x)`` on full-precision masters and its gradient, against 64 bits.
+
+The 16-bit gradient has an operand of its own, ``G`` (the gradient of both projections times their scales, rounded to 16 bits): it is
+checked element by element against the formula, and both products against 64-bit products of that very ``G``.
+"""
+import pytest
+import torch
+
+from conftest import announce
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+# rows, K, F: one of each; odd ones; halves that fill no tile, a last stage of the contraction, both sides of 64 and 128 rows, a contraction
+# long enough for two groups of waves
+SHAPES = [(1, 8, 2), (3, 7, 5), (2, 3, 9), (5, 1, 24), (1, 640, 48), (17, 100, 37), (64, 512, 256), (65, 1001, 33), (129, 520, 272), (300, 1100, 546),
+          (40, 2560, 688), (1000, 264, 520)]
+
+
+def _gated(*args, **kwargs):
+    from bittorch_amd import ops
+    return ops.ternary_gated_linear(*args, **kwargs)
+
+
+def _inputs(rows, k, f, dt, wt=None, bias=True, seed=0):
+    g = torch.Generator().manual_seed(seed * 977 + rows * 31 + k * 7 + f)
+    mk = lambda std, *shape: torch.randn(*shape, generator=g) * std
+    wt = wt or dt
+    x, wg, wu, dh = mk(1, rows, k).to(dt), mk(0.05, f, k).to(wt), mk(0.05, f, k).to(wt), mk(0.1, rows, f).to(dt)
+    bg, bu = (mk(0.3, f).to(wt), mk(0.3, f).to(wt)) if bias else (None, None)
+    return [None if t is None else t.cuda() for t in (x, wg, wu, bg, bu, dh)]
+
+
+def _ternary(w, threshold_factor=0.05, per_channel=True):
+    from bittorch_amd.quant import ternary_quantize
+    q, s = ternary_quantize(w.detach().cpu(), threshold_factor, per_channel)
+    return q.double().cuda(), s.double().reshape(-1).expand(w.shape[0]).cuda()
+
+
+class _Reference:
+    """The operator in 64 bits, with what fp32 evaluation may add to each value."""
+
+    def __init__(self, x, wg, wu, bg, bu, dh, **quant):
+        (self.tg, self.ag), (self.tu, self.au) = _ternary(wg, **quant), _ternary(wu, **quant)
+        x, dh, k = x.detach().double(), dh.double(), x.shape[1]
+        self.x, self.dh = x, dh
+        zero = torch.zeros(wg.shape[0], dtype=torch.float64, device=x.device)
+        bg, bu = (zero if b is None else b.detach().double() for b in (bg, bu))
+        g, u = x @ self.tg.t() * self.ag + bg, x @ self.tu.t() * self.au + bu
+        # A product of K terms: in the matrix cores 32 of them at a time, K / 32 sums one after the other (twice that where K is split),
+        # each rounded by at most one step; scale and bias once each.  fp32 rows: three 16-bit terms a value, so three times the sums, and
+        # half a step of the value in the third.
+        chain = U * 2 * (3 * k / 32 + 40)
+        self.tol_g = chain * (x.abs() @ self.tg.abs().t()) * self.ag + 4 * U * (g.abs() + bg.abs())
+        self.tol_u = chain * (x.abs() @ self.tu.abs().t()) * self.au + 4 * U * (u.abs() + bu.abs())
+        sig = 1 / (1 + torch.exp(-g))
+        self.g, self.u, silu = g, u, g * sig
+        self.h = silu * u
+        # silu' lies within -0.1 and 1.1; exp's argument is rounded (|g| U of the result), exp, the sum, the reciprocal, two products
+        self.tol_h = 1.1 * u.abs() * self.tol_g + silu.abs() * self.tol_u + (g.abs() + 16) * U * self.h.abs()
+        slope = sig * (1 + g * (1 - sig))
+        self.dg, self.du = dh * u * slope, dh * silu
+        # |silu''| is at most 1/2; 1 - sig is off by a step of 1, which g multiplies
+        self.tol_dg = dh.abs() * (slope.abs() * self.tol_u + 0.5 * u.abs() * self.tol_g + u.abs() * sig * (3 * g.abs() + 16) * U)
+        self.tol_du = dh.abs() * (1.1 * self.tol_g + silu.abs() * (g.abs() + 16) * U)
+
+
+def _assert_within(got, want, tol, what):
+    half, tiny = torch.finfo(got.dtype).eps / 2, torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    off = (got.double() - want).abs() - (tol + half * (want.abs() + tol) + tiny)
+    assert bool((off <= 0).all()), f"{what}: {float(off.max())} over its bound"
+
+
+def _norm_error(got, want):
+    return float((got.double() - want).norm() / want.norm().clamp(min=1e-300))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,k,f", SHAPES)
+def test_forward_and_gradient(rows, k, f, dt):
+    announce("gated", rows, k, f, dt)
+    x, wg, wu, bg, bu, dh = _inputs(rows, k, f, dt)
+    ref = _Reference(x, wg, wu, bg, bu, dh)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    h = _gated(*leaves)
+    assert h.shape == (rows, f) and h.dtype == dt
+    _assert_within(h.detach(), ref.h, ref.tol_h, "h")
+    with torch.no_grad():
+        assert torch.equal(_gated(*leaves), h)
+    dx, dwg, dwu, dbg, dbu = torch.autograd.grad(h, leaves, dh, retain_graph=True)
+    again = torch.autograd.grad(h, leaves, dh)
+    assert all(torch.equal(a, b) and a.is_contiguous() for a, b in zip(again, (dx, dwg, dwu, dbg, dbu)))
+    assert dx.shape == x.shape and dwg.shape == wg.shape and dbu.shape == bu.shape and {t.dtype for t in again} == {dt}
+    # the sums of the biases: `rows` additions at most, in fp32, before they are rounded
+    for got, v, tol in ((dbg, ref.dg, ref.tol_dg), (dbu, ref.du, ref.tol_du)):
+        _assert_within(got, v.sum(0), tol.sum(0) + U * (rows + 4) * v.abs().sum(0), "bias")
+    # both products: each term's own error, and where rows are 16-bit half a step of G
+    half = 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2
+    chain = lambda n: U * 2 * (3 * n / 32 + 80)
+    parts = [(ref.dg, ref.tol_dg, ref.ag, ref.tg), (ref.du, ref.tol_du, ref.au, ref.tu)]
+    tiny = 0.0 if dt == torch.float32 else torch.finfo(dt).smallest_normal * half
+    want = sum((v * a) @ t for v, _, a, t in parts)
+    tol = sum(((tol * (1 + half) + (half + chain(2 * f)) * v.abs()) * a + tiny) @ t.abs() for v, tol, a, t in parts)
+    _assert_within(dx, want, tol, "dx")
+    for got, (v, tol, a, _) in zip((dwg, dwu), parts):
+        want_w = ((v * a).t() @ ref.x)
+        tol_w = ((tol * (1 + half) + (half + chain(rows)) * v.abs()) * a + tiny).t() @ ref.x.abs()
+        _assert_within(got, want_w, tol_w, "dW")
+        if dt != torch.float32 and rows * k >= 64:
+            # two roundings of at most half a step, independent of each other and of their neighbours': their root of squares
+            # (1.42 halves), the largest they could be in every single place
+            assert _norm_error(got, want_w) <= 1.42 * half
+    if dt != torch.float32 and rows * k >= 64:
+        assert _norm_error(dx, want) <= 1.42 * half and _norm_error(h.detach(), ref.h) <= 1.01 * half
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,k,f", [(33, 264, 48), (300, 1100, 546), (257, 512, 1000)])
+def test_stages_of_the_16_bit_gradient(rows, k, f, dt):
+    announce("gated stages", rows, k, f, dt)
+    from bittorch_amd import _C
+    x, wg, wu, bg, bu, dh = _inputs(rows, k, f, dt, seed=1)
+    ref = _Reference(x, wg, wu, bg, bu, dh)
+    fp = (f + 15) // 16 * 16
+    w, w_back, scale, bias = _C.gated_weights(wg, wu, bg, bu, back=True)
+    xp = torch.nn.functional.pad(x, (0, -k % 8))
+    h, pre = _C.ternary_gated_forward(xp, w, scale, bias, f, True)
+    assert torch.equal(h, _C.ternary_gated_forward(xp, w, scale, bias, f)[0])
+    pairs = pre.reshape(rows, fp // 2, 2, 2)
+    _assert_within(pairs[:, :, 0].reshape(rows, fp)[:, :f], ref.g, ref.tol_g, "g")
+    _assert_within(pairs[:, :, 1].reshape(rows, fp)[:, :f], ref.u, ref.tol_u, "u")
+    g, db = _C.gated_grad(dh, pre, scale, torch.float32)
+    assert g.shape == (rows, 2 * fp) and not g[:, f:fp].any() and not g[:, fp + f:].any()
+    _assert_within(g[:, :f], ref.dg * ref.ag, ref.tol_dg * ref.ag, "G gate")
+    _assert_within(g[:, fp:fp + f], ref.du * ref.au, ref.tol_du * ref.au, "G up")
+    assert torch.equal(g, _C.gated_grad(dh, pre, scale)[0])
+    # the copy for the input's gradient holds the codes' transpose: a product of a unit row reads one feature's weights
+    eye = torch.zeros(2 * f, 2 * fp, dtype=dt, device="cuda")
+    eye[torch.arange(f), torch.arange(f)] = 1
+    eye[torch.arange(f) + f, torch.arange(f) + fp] = 1
+    rows_of = _C.ternary_linear_tiled_forward(eye, w_back, scale[2 * fp:], None, 2 * fp, k)
+    assert torch.equal(rows_of.double(), torch.cat((ref.tg, ref.tu)))
+    dx = _C.ternary_linear_tiled_forward(g, w_back, scale[2 * fp:], None, 2 * fp, k)
+    g64 = g.double()
+    codes = torch.zeros(2 * fp, k, dtype=torch.float64, device="cuda")
+    codes[:f], codes[fp:fp + f] = ref.tg, ref.tu
+    _assert_within(dx, g64 @ codes, U * 2 * (2 * fp / 32 + 80) * (g64.abs() @ codes.abs()), "dx")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,wt", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32), (torch.float32, torch.bfloat16),
+                                   (torch.bfloat16, torch.float16)])
+def test_masters_of_another_dtype(dt, wt):
+    x, wg, wu, bg, bu, dh = _inputs(70, 264, 80, dt, wt, seed=2)
+    ref = _Reference(x, wg, wu, bg, bu, dh)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    h = _gated(*leaves)
+    _assert_within(h.detach(), ref.h, ref.tol_h, "h")
+    grads = torch.autograd.grad(h, leaves, dh)
+    assert [t.dtype for t in grads] == [dt, wt, wt, wt, wt]
+    eps = max(torch.finfo(d).eps for d in (dt, wt))
+    want = [(ref.dg * ref.ag) @ ref.tg + (ref.du * ref.au) @ ref.tu, (ref.dg * ref.ag).t() @ ref.x, (ref.du * ref.au).t() @ ref.x,
+            ref.dg.sum(0), ref.du.sum(0)]
+    for got, w in zip(grads, want):  # up to three roundings to 16 bits: G, the product, the masters' dtype
+        assert _norm_error(got, w) <= 1.74 * eps / 2 + 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_quantizer_settings_and_rows_without_weights(dt):
+    x, wg, wu, _, _, dh = _inputs(20, 128, 40, dt, bias=False, seed=3)
+    wg[3], wu[5] = 0, 0
+    wg[4, 1:] = 0
+    for quant in (dict(threshold_factor=0.7), dict(threshold_factor=0.0), dict(per_channel=False), dict(threshold_factor=0.5, per_channel=False)):
+        ref = _Reference(x, wg, wu, None, None, dh, **quant)
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+        h = _gated(*leaves, **quant)
+        _assert_within(h.detach(), ref.h, ref.tol_h, quant)
+        dx, dwg, dwu = torch.autograd.grad(h, leaves, dh)
+        # (the third: a 16-bit master's scale of 1e-8 is 0 or a rounded 1e-8; those rows are too small to matter in a norm)
+        half = torch.finfo(dt).eps / 2
+        assert _norm_error(dx, (ref.dg * ref.ag) @ ref.tg + (ref.du * ref.au) @ ref.tu) <= 1.42 * half + 2e-6
+        assert _norm_error(dwg, (ref.dg * ref.ag).t() @ ref.x) <= 1.42 * half + 2e-6
+
+
+@pytest.mark.gpu
+def test_parts_of_the_call():
+    """One bias, one leaf, one master twice, and inputs that lie in other ways."""
+    x, wg, wu, bg, bu, dh = _inputs(48, 264, 72, torch.bfloat16, seed=4)
+    full = [t.clone().requires_grad_() for t in (x, wg, wu, bg, bu)]
+    want = torch.autograd.grad(_gated(*full), full, dh)
+    for n in range(5):
+        args = [t.detach() for t in full]
+        args[n].requires_grad_()
+        got, = torch.autograd.grad(_gated(*args), args[n], dh)
+        assert torch.equal(got, want[n]), n
+    for args in ((x, wg, wu, bg, None), (x, wg, wu, None, bu), (x, wg, wu, None, None)):
+        ref = _Reference(*args, dh)
+        _assert_within(_gated(*args), ref.h, ref.tol_h, "one bias")
+    ref = _Reference(x, wg, wg, None, None, dh)
+    w = wg.clone().requires_grad_()
+    twice, = torch.autograd.grad(_gated(x, w, w), w, dh)
+    assert _norm_error(twice, (ref.dg * ref.ag + ref.du * ref.au).t() @ ref.x) <= 2 * torch.finfo(torch.bfloat16).eps / 2
+    # leading dimensions, columns before rows, rows inside a wider matrix, an odd start, strided and expanded gradients and masters
+    h = _gated(*[t.detach() for t in full])
+    wide = torch.randn(48, 264 * 2 + 1, device="cuda").bfloat16()
+    wide[:, 1:265] = x
+    flat = torch.zeros(48 * 264 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(48, 264).copy_(x)
+    for other in (x.reshape(6, 8, 264), x.t().contiguous().t(), wide[:, 1:265], flat):
+        o = other.detach().requires_grad_()
+        out = _gated(o, wg.t().contiguous().t(), wu, bg, bu)
+        assert out.shape == (*o.shape[:-1], 72) and torch.equal(out.reshape(48, 72), h)
+        grad, = torch.autograd.grad(out, o, dh.reshape(out.shape))
+        assert torch.equal(grad.reshape(48, 264), want[0])
+    one = _gated(x[5], wg, wu, bg, bu)
+    assert one.shape == (72,) and torch.equal(one, _gated(x[5:6], wg, wu, bg, bu)[0])
+    out = _gated(*full)
+    a = torch.autograd.grad(out, full, dh.t().contiguous().t(), retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, want))
+    b = torch.autograd.grad(out.sum(), full, retain_graph=True)
+    c = torch.autograd.grad(out, full, torch.ones_like(out), retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(b, c))
+    dx, = torch.autograd.grad(out, full[0], dh.clone().requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_slopes(dt):
+    """The gradient of the input and the biases against differences of the forward (the masters' is a straight-through one)."""
+    x, wg, wu, bg, bu, dh = _inputs(9, 64, 24, torch.float32, seed=5)
+    x, dh = x.to(dt).float(), dh.to(dt).float()
+    args = [t.to(dt).requires_grad_() for t in (x, wg, wu, bg, bu)]
+    grads = torch.autograd.grad(_gated(*args), args, dh.to(dt))
+    args = [t.detach().float() for t in args]  # (differences in fp32, of the same values)
+    for n in (0, 3, 4):
+        step = torch.randn(args[n].shape, generator=torch.Generator().manual_seed(n)).cuda()
+        ends = []
+        for sign in (1, -1):
+            moved = list(args)
+            moved[n] = moved[n] + sign * 1e-2 * step
+            ends.append(float((_gated(*moved).double() * dh).sum()))
+        slope, want = (ends[0] - ends[1]) / 2e-2, float((grads[n].double() * step).sum())
+        # the gradient's roundings (two halves of a step), and the differences': the third derivative in 1e-2, their own sum's steps
+        size = float((grads[n].double().square() * step.double().square()).sum().sqrt())
+        assert abs(slope - want) <= (1e-2 + 8 * torch.finfo(dt).eps) * size + 1e-3, (n, slope, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_saturated_and_unusual_rows_stay_by_themselves(dt):
+    x, wg, wu, bg, bu, dh = _inputs(80, 256, 64, dt, seed=6)
+    x[3], x[5] = 0, x[5] * 500  # (gates beyond +-88 where exp over- and underflows)
+    ref = _Reference(x, wg, wu, bg, bu, dh)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    h = _gated(*leaves)
+    dx, = torch.autograd.grad(h, leaves[0], dh)
+    if dt != torch.float16:
+        assert bool(h.isfinite().all()) and bool(dx.isfinite().all())
+        assert float(ref.g[5].abs().max()) > 89
+        _assert_within(h.detach(), ref.h, ref.tol_h, "saturated")
+    y = x.detach().clone()
+    y[7, 3], y[70, 9] = float("nan"), float("inf")
+    y.requires_grad_()
+    other = [i for i in range(80) if i not in (7, 70)]
+    h2 = _gated(y, *leaves[1:])
+    dx2, = torch.autograd.grad(h2, y, dh)
+    assert torch.equal(h2[other], h[other]) and torch.equal(dx2[other], dx[other])
+    assert bool(h2[7].isnan().all())
+
+
+@pytest.mark.gpu
+def test_autocast_is_the_half_precision_call():
+    x, wg, wu, bg, bu, dh = _inputs(50, 136, 40, torch.float32, seed=7)
+    full = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    with torch.autocast("cuda", dtype=torch.float16):
+        h = _gated(*full)
+    half = [t.detach().half().requires_grad_() for t in full]
+    want = _gated(*half)
+    assert h.dtype == torch.float16 and torch.equal(h, want)
+    grads = torch.autograd.grad(h, full, dh.half())
+    for got, w in zip(grads, torch.autograd.grad(want, half, dh.half())):
+        # the same fp16 sums; biases and masters may keep more of them
+        assert got.dtype == torch.float32 and _norm_error(got, w.double()) <= torch.finfo(torch.float16).eps / 2 + 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_streams_and_captured_graphs(dt):
+    x, wg, wu, bg, bu, dh = _inputs(100, 264, 144, dt, seed=8)
+
+    def step(*args):
+        leaves = [t.detach().requires_grad_() for t in args[:5]]
+        h = _gated(*leaves)
+        return (h.detach(), *torch.autograd.grad(h, leaves, args[5]))
+
+    want = step(x, wg, wu, bg, bu, dh)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(x, wg, wu, bg, bu, dh)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del got
+    graphs = []
+    for sign in (1, -1):
+        static = [t.clone() for t in (x * sign, wg, wu, bg, bu, dh)]
+        expect = [t.clone() for t in step(*static)]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((graph, static, out, expect))
+    for _ in range(3):
+        for graph, static, out, expect in graphs:
+            for t in out:
+                t.fill_(7)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, expect))
+            assert all(torch.equal(a, b) for a, b in zip(step(*static), expect))
+
+
+@pytest.mark.gpu
+def test_agrees_with_two_layers_and_their_product():
+    """The training form beside the layers that it stands for: the same codes and scales, so the same values up to their roundings."""
+    import bittorch_amd as bt
+    x, wg, wu, bg, bu, dh = _inputs(128, 256, 192, torch.float32, seed=9)
+    layers = []
+    for w, b in ((wg, bg), (wu, bu)):
+        layer = bt.nn.TernaryLinear(256, 192).cuda()
+        with torch.no_grad():
+            layer.weight.copy_(w)
+            layer.bias.copy_(b)
+        layers.append(layer)
+    y = x.clone().requires_grad_()
+    h = torch.nn.functional.silu(layers[0](y)) * layers[1](y)
+    h.backward(dh)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    ours = _gated(*leaves)
+    assert _norm_error(ours, h.double()) <= 1e-6
+    for a, b in zip(torch.autograd.grad(ours, leaves, dh), (y.grad, layers[0].weight.grad, layers[1].weight.grad, layers[0].bias.grad, layers[1].bias.grad)):
+        assert _norm_error(a, b.double()) <= 2e-6
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float64])
+def test_cpu_is_the_two_layers(dt):
+    from bittorch_amd import nn
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(5, 3, 20, generator=g, dtype=dt, requires_grad=True)
+    layers = [nn.TernaryLinear(20, 12).to(dt) for _ in range(2)]
+    args = [layers[0].weight, layers[1].weight, layers[0].bias, layers[1].bias]
+    want = torch.nn.functional.silu(layers[0](x)) * layers[1](x)
+    got = _gated(x, *args)
+    assert torch.equal(got, want)
+    dh = torch.randn(got.shape, generator=g, dtype=dt)
+    for a, b in zip(torch.autograd.grad(got, [x, *args], dh), torch.autograd.grad(want, [x, *args], dh)):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    from bittorch_amd import _lib
+    x, w = torch.randn(4, 16), torch.randn(8, 16)
+    for args, text in [((x, w, w[:7]), "must match"), ((x, w, w.half()), "must match"), ((x, w[0], w[0]), "must match"),
+                       ((x[:, :15], w, w), "input K"), ((x[:0], w, w), "x is empty"), ((x, w[:0], w[:0]), "weight is empty"),
+                       ((x, w, w, torch.ones(7)), "bias shape"), ((x, w, w, None, torch.ones(8, 1)), "bias shape")]:
+        with pytest.raises(RuntimeError, match=text):
+            _gated(*args)
+    lib, at = _lib.load(), 1 << 20  # (never read: every call ends before a launch)
+    weights = lambda g=at, n=8, b=None, bdt=0, F=8, K=16, pairs=at, back=None, rows=None, scale=at, bias=None: lib.bt_gated_weights(
+        g, at, at, at, n, b, b, bdt, F, K, pairs, back, rows, scale, bias, None)
+    for kwargs, text in [(dict(g=None), "null"), (dict(scale=None), "null"), (dict(F=0), "empty"), (dict(pairs=None), "null"), (dict(rows=at), "both"),
+                         (dict(pairs=None, back=at, rows=at), "both"), (dict(n=3), "scale size"), (dict(b=at), "bias"),
+                         (dict(b=at, bias=at, bdt=3), "bias"), (dict(pairs=at + 16), "aligned"), (dict(back=at + 16), "aligned"),
+                         (dict(F=1 << 23, n=1), "2^23"), (dict(K=1 << 23), "2^23"), (dict(F=1 << 20, K=1 << 20, n=1), "4 GiB")]:
+        assert weights(**kwargs) == -1, kwargs
+        assert text in _lib.last_error(), (kwargs, _lib.last_error())
+    forward = lambda X=at, dt=2, W=at, h=at, pre=None, B=4, F=8, K=16: lib.bt_ternary_gated_forward(X, dt, W, at, None, h, pre, B, F, K, None)
+    for kwargs in (dict(X=None), dict(dt=0), dict(dt=5), dict(W=None), dict(h=None), dict(B=0), dict(K=12), dict(X=at + 8), dict(W=at + 128), dict(pre=at + 8),
+                   dict(h=at + 4), dict(F=1 << 23), dict(B=1 << 31)):
+        assert forward(**kwargs) == -1, kwargs
+        assert "bt_ternary_gated_forward" in _lib.last_error()
+    grad = lambda dh=at, dt=2, pre=at, scale=at, G=at, db=None, bdt=0, B=4, F=8, ws=None, n=0: lib.bt_gated_grad(
+        dh, dt, pre, scale, G, db, bdt, B, F, ws, n, None)
+    for kwargs in (dict(dh=None), dict(pre=None), dict(G=None), dict(scale=None), dict(dt=3), dict(F=0), dict(B=1 << 31), dict(pre=at + 4), dict(G=at + 4),
+                   dict(db=at, bdt=3)):
+        assert grad(**kwargs) == -1, kwargs
+    need = lib.bt_gated_grad_workspace_bytes(4, 8)
+    assert need > 0 and lib.bt_gated_grad_workspace_bytes(0, 8) == 0
+    assert grad(db=at) == -2 and grad(db=at, ws=at, n=need - 1) == -2 and grad(db=at, ws=at + 8, n=need) == -2
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    x, w = torch.randn(4, 16, device="cuda"), torch.randn(8, 16, device="cuda")
+    with pytest.raises(RuntimeError, match="one device"):
+        _gated(x, w.cpu(), w.cpu())
+    with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+        _gated(x.double(), w, w)
+    with pytest.raises(RuntimeError, match="at least 2 output features"):
+        _gated(x, w[:1], w[:1])
+    assert _gated(x.half(), w[:1], w[:1]).shape == (4, 1)
