@@ -11,12 +11,16 @@
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/autocast_mode.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -36,7 +40,9 @@ namespace {
     X(bt_linear_grad_weight_16_workspace_bytes) X(bt_ternary_linear_tiled_forward) X(bt_ternary_linear_packed_forward)         \
     X(bt_ternary_linear_tensor_core_forward) X(bt_quantize_pack) X(bt_ternary_linear_grad_input) X(bt_linear_grad_weight)      \
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
-    X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout)
+    X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
+    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_weights) X(bt_ternary_gated_forward) X(bt_gated_grad)                \
+    X(bt_gated_grad_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     BT_FUNCTIONS(X)
@@ -100,6 +106,12 @@ struct Unlocked {  // the interpreter, until the end of the block however it is 
 };
 // The library's call without the interpreter lock, as through ctypes.  Its arguments are values: what they are read from (tensors, whose
 // accessors may throw and which other threads may point elsewhere) is asked under the lock.
+void check_status(int rc) {
+    if (rc != 0) {
+        const char* text = lib.bt_last_error();
+        TORCH_CHECK_WITH(Error, false, text && text[0] ? std::string(text) : "libbittorch_hip call failed (" + std::to_string(rc) + ")");
+    }
+}
 template <typename... P>
 void call(int (*f)(P...), std::common_type_t<P>... args) {
     int rc;
@@ -107,10 +119,7 @@ void call(int (*f)(P...), std::common_type_t<P>... args) {
         const Unlocked unlocked;
         rc = f(args...);
     }
-    if (rc != 0) {
-        const char* text = lib.bt_last_error();
-        TORCH_CHECK_WITH(Error, false, text && text[0] ? std::string(text) : "libbittorch_hip call failed (" + std::to_string(rc) + ")");
-    }
+    check_status(rc);
 }
 
 bool as_int(PyObject* o, int64_t* v) {
@@ -508,6 +517,313 @@ PyObject* unpack_dequant(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- calls that are differentiated: the autograd functions of ops/fused.py and ops/gated.py -----------------------------------
+// A training call of a small layer spends more time in those two Python functions than on the GPU (the norm of 777 x 1001 and its gradient:
+// 146 us a step, of kernels that take 15).  Backward passes run on autograd's own threads, which do not hold the interpreter lock.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using MaybeTensor = std::optional<at::Tensor>;
+
+const void* data_of(const MaybeTensor& t) { return t ? t->const_data_ptr() : nullptr; }
+int tag_of(const MaybeTensor& t) { return t ? tag(t->scalar_type()) : 0; }
+MaybeTensor maybe(const at::Tensor* t) { return t ? MaybeTensor(*t) : std::nullopt; }
+
+// A gradient for each argument of a forward, and whether it is wanted: autograd asks by the number of a tensor argument that there was.
+struct Wanted {
+    variable_list grads;
+    std::vector<bool> want;
+    Wanted(AutogradContext* ctx, size_t args, std::initializer_list<bool> there) : grads(args), want(there.size()) {
+        size_t edge = 0, i = 0;
+        for (bool t : there) want[i++] = t && ctx->needs_input_grad(edge++);
+    }
+};
+// What the gradients are where a graph of the backward pass is kept (`graph`): values whose own gradient is an error.
+variable_list once(const char* name, bool graph, variable_list grads, const variable_list& incoming) {
+    bool depends = false;
+    for (const at::Tensor& t : incoming) depends = depends || (t.defined() && t.requires_grad());
+    if (!graph || !depends) return grads;
+    const at::AutoGradMode on(true);
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string("trying to differentiate twice a function that was marked with @once_differentiable (") + name + ")", (int64_t)grads.size());
+    variable_list out(grads.size()), some;
+    std::vector<size_t> at;
+    for (size_t i = 0; i < grads.size(); i++)
+        if (grads[i].defined()) {
+            some.push_back(grads[i].detach().requires_grad_());
+            at.push_back(i);
+        }
+    some = (*error)(std::move(some));
+    for (size_t i = 0; i < at.size(); i++) out[at[i]] = some[i];
+    return out;
+}
+
+struct NormFlags {
+    double eps;
+    bool store, quantize, operand_order, rowsum;
+};
+struct NormOut {
+    at::Tensor s, y, q, s_x, rowsum, rstd;
+};
+NormOut add_norm_run(const at::Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight, const NormFlags& f, bool want_rstd) {
+    const int64_t K = x.size(-1), B = x.numel() / K;
+    const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+    NormOut o;
+    if (residual) o.s = output(x.sizes(), residual->scalar_type(), x);
+    if (f.store) o.y = output(x.sizes(), x.scalar_type(), x);
+    if (f.quantize) {
+        o.q = output(x.sizes(), at::kChar, x);
+        o.s_x = output(lead, at::kFloat, x);
+    }
+    if (f.rowsum) o.rowsum = output(lead, at::kInt, x);
+    if (want_rstd) o.rstd = output({B}, at::kFloat, x);
+    auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    void* st = stream_of(x.get_device());
+    call(lib.bt_add_rmsnorm, x.const_data_ptr(), K, tag(x.scalar_type()), data_of(residual), residual ? K : 0, tag_of(residual), data_of(weight),
+         tag_of(weight), (float)f.eps, B, K, ptr(o.s), ptr(o.y), (float*)ptr(o.rstd), (int8_t*)ptr(o.q), (float*)ptr(o.s_x), (int32_t*)ptr(o.rowsum),
+         f.operand_order ? 1 : 0, st);
+    return o;
+}
+
+struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight, double eps,
+                                 bool store, bool quantize, bool operand_order, bool rowsum) {
+        NormOut o = add_norm_run(x, residual, weight, {eps, store, quantize, operand_order, rowsum}, true);
+        ctx->set_materialize_grads(false);
+        variable_list out, none;
+        for (at::Tensor* t : {&o.s, &o.y, &o.q, &o.s_x, &o.rowsum})
+            if (t->defined()) {
+                out.push_back(*t);
+                if (t != &o.s && t != &o.y) none.push_back(*t);
+            }
+        ctx->mark_non_differentiable(none);
+        ctx->save_for_backward({residual ? o.s : x, o.rstd, weight ? *weight : at::Tensor()});
+        ctx->saved_data["residual"] = residual.has_value();
+        ctx->saved_data["store"] = store;
+        ctx->saved_data["dtype"] = x.scalar_type();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &s = saved[0], &rstd = saved[1], &weight = saved[2];
+        const bool has_residual = ctx->saved_data["residual"].toBool(), stored = ctx->saved_data["store"].toBool();
+        const at::ScalarType x_dtype = ctx->saved_data["dtype"].toScalarType();
+        Wanted w(ctx, 8, {true, has_residual, weight.defined()});
+        const bool want_x = w.want[0], want_r = w.want[1], want_w = w.want[2];
+        const at::Tensor d_sum = has_residual ? incoming[0] : at::Tensor(), d_norm = stored ? incoming[has_residual ? 1 : 0] : at::Tensor();
+        const bool graph = at::GradMode::is_enabled();
+        const at::NoGradGuard no_grad;
+        const c10::DeviceGuard guard(s.device());
+        if (!d_norm.defined()) {  // the norm was not used
+            if (d_sum.defined()) {
+                if (want_x) w.grads[0] = d_sum.to(x_dtype);
+                if (want_r) w.grads[1] = d_sum;
+            }
+            if (want_w) w.grads[2] = at::zeros_like(weight);
+        } else {
+            const int64_t K = s.size(-1), B = s.numel() / K;
+            const at::Tensor dy = d_norm.contiguous(), ds = d_sum.defined() ? d_sum.contiguous() : d_sum;
+            const bool one = x_dtype == s.scalar_type();
+            at::Tensor dx, dr, dw;
+            if (want_r || (one && want_x)) dr = output(s.sizes(), s.scalar_type(), s);
+            if (want_x && !one) dx = output(s.sizes(), x_dtype, s);
+            if (want_w) dw = output({K}, weight.scalar_type(), s);
+            const Scratch ws(want_w ? lib.bt_add_rmsnorm_backward_workspace_bytes(B, K) : 0, s);
+            auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+            check_status(lib.bt_add_rmsnorm_backward(
+                s.const_data_ptr(), tag(s.scalar_type()), (const float*)rstd.const_data_ptr(), weight.defined() ? weight.const_data_ptr() : nullptr,
+                weight.defined() ? tag(weight.scalar_type()) : 0, dy.const_data_ptr(), tag(x_dtype), ds.defined() ? ds.const_data_ptr() : nullptr, B, K,
+                ptr(dx), ptr(dr), ptr(dw), ws.ptr(), ws.size(), stream_of(s.get_device())));
+            if (want_x) w.grads[0] = one ? dr : dx;
+            if (want_r) w.grads[1] = dr;
+            if (want_w) w.grads[2] = dw;
+        }
+        return once("add_rmsnorm", graph, std::move(w.grads), incoming);
+    }
+};
+
+bool differentiated(std::initializer_list<const at::Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor* t : ts)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+PyObject* tuple_of(const variable_list& list, PyObject* first) {
+    PyObject* out = PyTuple_New((Py_ssize_t)list.size() + (first ? 1 : 0));
+    if (!out) return nullptr;
+    Py_ssize_t i = 0;
+    if (first) {
+        Py_INCREF(first);
+        PyTuple_SET_ITEM(out, i++, first);
+    }
+    for (const at::Tensor& t : list) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+    return out;
+}
+
+// add_rmsnorm(x, residual, weight, eps, store, quantize, operand_order, return_rowsum) -> (s, [y], [q, s_x], [rowsum])
+PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    int device;
+    NormFlags f;
+    ORDINARY(n_args == 8);
+    const at::Tensor* x = rows_of(a[0], &device);
+    ORDINARY(x && as_float(a[3], &f.eps) && as_bool(a[4], &f.store) && as_bool(a[5], &f.quantize) && as_bool(a[6], &f.operand_order) &&
+             as_bool(a[7], &f.rowsum));
+    const int64_t K = x->size(-1);
+    ORDINARY((f.store || f.quantize) && (f.quantize || !f.rowsum));
+    const at::Tensor *residual = nullptr, *weight = nullptr;
+    if (a[1] != Py_None) {
+        residual = plain(a[1], device);
+        ORDINARY(residual && residual->sizes() == x->sizes() && (residual->scalar_type() == x->scalar_type() || residual->scalar_type() == at::kFloat));
+    }
+    if (a[2] != Py_None) {
+        weight = plain(a[2], device);
+        ORDINARY(weight && weight->dim() == 1 && weight->size(0) == K && (weight->scalar_type() == x->scalar_type() || weight->scalar_type() == at::kFloat));
+    }
+    if (differentiated({x, residual, weight}))
+        return tuple_of(AddRMSNorm::apply(*x, maybe(residual), maybe(weight), f.eps, f.store, f.quantize, f.operand_order, f.rowsum),
+                        residual ? nullptr : a[0]);
+    NormOut o = add_norm_run(*x, maybe(residual), maybe(weight), f, false);
+    variable_list out;
+    for (at::Tensor* t : {&o.s, &o.y, &o.q, &o.s_x, &o.rowsum})
+        if (t->defined()) out.push_back(std::move(*t));
+    return tuple_of(out, residual ? nullptr : a[0]);
+    END_HANDLE_TH_ERRORS
+}
+
+struct GatedOut {
+    at::Tensor h, pre, w_back, scale;
+};
+// fp32 rows: K >= 4, F >= 2; 16-bit rows: K % 8 == 0 and 16-byte aligned.  All tensors contiguous.
+GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const MaybeTensor& gate_bias, const MaybeTensor& up_bias,
+                   double threshold, bool per_channel, bool keep, bool want_back) {
+    const int64_t F = gate.size(0), K = gate.size(1), Kb = (K + 3) / 4, B = x.numel() / K;
+    const bool rows = x.scalar_type() == at::kFloat;
+    const int64_t Fv = rows ? F : (F + 15) / 16 * 16;
+    const int dt = tag(x.scalar_type()), wdt = tag(gate.scalar_type());
+    void* st = stream_of(x.get_device());
+    // the packed bytes of both layers and their scales, read by the next launch alone
+    const at::Tensor packed = output({2, Kb, F}, at::kByte, x), scales = output({2, per_channel ? F : 1}, at::kFloat, x);
+    uint8_t* const codes[2] = {(uint8_t*)packed.data_ptr(), (uint8_t*)packed.data_ptr() + Kb * F};
+    float* const absmax[2] = {(float*)scales.data_ptr(), (float*)scales.data_ptr() + scales.size(1)};
+    for (int i = 0; i < 2; i++)
+        call(lib.bt_quantize_pack, (i ? up : gate).const_data_ptr(), wdt, F, K, threshold, per_channel ? 1 : 0, codes[i], absmax[i], nullptr, st);
+    GatedOut o;
+    const at::Tensor w = rows ? output({Kb, 2 * F}, at::kByte, x) : output({(int64_t)lib.bt_tiled_weights_bytes(2 * Fv, K)}, at::kByte, x);
+    if (rows) o.w_back = w;
+    else if (want_back) o.w_back = output({(int64_t)lib.bt_tiled_weights_bytes(K, 2 * Fv)}, at::kByte, x);
+    o.scale = output({2 * Fv + 1}, at::kFloat, x);
+    at::Tensor bias;
+    if (gate_bias || up_bias) bias = output({2 * Fv}, at::kFloat, x);
+    float* const scale_at = (float*)o.scale.data_ptr();
+    float* const bias_at = bias.defined() ? (float*)bias.data_ptr() : nullptr;
+    call(lib.bt_gated_weights, codes[0], codes[1], absmax[0], absmax[1], scales.size(1), data_of(gate_bias), data_of(up_bias),
+         gate_bias ? tag_of(gate_bias) : tag_of(up_bias), F, K, rows ? nullptr : (uint8_t*)w.data_ptr(),
+         !rows && want_back ? (uint8_t*)o.w_back.data_ptr() : nullptr, rows ? (uint8_t*)w.data_ptr() : nullptr, scale_at, bias_at, st);
+    o.h = output(with_last(x, F), x.scalar_type(), x);
+    if (rows || keep) o.pre = output({B, 2 * Fv}, at::kFloat, x);
+    if (!rows) {
+        call(lib.bt_ternary_gated_forward, x.const_data_ptr(), dt, (const uint8_t*)w.const_data_ptr(), scale_at, bias_at, o.h.data_ptr(),
+             keep ? (float*)o.pre.data_ptr() : nullptr, B, F, K, st);
+        return o;
+    }
+    const Scratch ws(lib.bt_packed_forward_workspace_bytes(B, 2 * F, K, dt), x);
+    call(lib.bt_ternary_linear_packed_forward, x.const_data_ptr(), dt, (const uint8_t*)w.const_data_ptr(), scale_at, BT_F32, 2 * F, bias_at, BT_F32,
+         o.pre.data_ptr(), B, 2 * F, K, ws.ptr(), ws.size(), st);
+    call(lib.bt_swiglu, o.pre.const_data_ptr(), 2 * F, (const float*)o.pre.const_data_ptr() + F, 2 * F, BT_F32, B, F, o.h.data_ptr(), nullptr, nullptr, 0, st);
+    return o;
+}
+
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const MaybeTensor& gate_bias,
+                              const MaybeTensor& up_bias, double threshold, bool per_channel) {
+        GatedOut o = gated_run(x, gate, up, gate_bias, up_bias, threshold, per_channel, true, x.requires_grad());
+        ctx->save_for_backward({x, o.pre, o.w_back, o.scale});
+        ctx->saved_data["shape"] = std::vector<int64_t>{gate.size(0), gate.size(1)};
+        ctx->saved_data["dtype"] = gate.scalar_type();
+        ctx->saved_data["biases"] = (int64_t)((gate_bias ? 1 : 0) | (up_bias ? 2 : 0));
+        ctx->saved_data["bias_dtype"] = gate_bias ? gate_bias->scalar_type() : up_bias ? up_bias->scalar_type() : at::kFloat;
+        return o.h;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &pre = saved[1], &w_back = saved[2], &scale = saved[3];
+        const int64_t biases = ctx->saved_data["biases"].toInt();
+        Wanted w(ctx, 7, {true, true, true, (biases & 1) != 0, (biases & 2) != 0});
+        if (!incoming[0].defined()) return w.grads;
+        const auto shape = ctx->saved_data["shape"].toIntVector();
+        const at::ScalarType w_dtype = ctx->saved_data["dtype"].toScalarType(), b_dtype = ctx->saved_data["bias_dtype"].toScalarType();
+        const bool graph = at::GradMode::is_enabled();
+        const at::NoGradGuard no_grad;
+        const c10::DeviceGuard guard(x.device());
+        const int64_t F = shape[0], K = shape[1], B = x.numel() / K;
+        const bool rows = x.scalar_type() == at::kFloat;
+        const int64_t Fv = rows ? F : (F + 15) / 16 * 16;
+        const int dt = tag(x.scalar_type());
+        const bool want_w = w.want[1] || w.want[2], want_b = w.want[3] || w.want[4];
+        void* st = stream_of(x.get_device());
+        const at::Tensor dh = incoming[0].contiguous(), g = output({B, 2 * Fv}, x.scalar_type(), x);
+        const float *scale_at = (const float*)scale.const_data_ptr(), *one = scale_at + 2 * Fv;
+        at::Tensor db;
+        if (want_b) db = output({2 * F}, b_dtype, x);
+        {
+            const Scratch ws(want_b ? lib.bt_gated_grad_workspace_bytes(B, F) : 0, x);
+            check_status(lib.bt_gated_grad(dh.const_data_ptr(), dt, (const float*)pre.const_data_ptr(), scale_at, g.data_ptr(), want_b ? db.data_ptr() : nullptr,
+                                           want_b ? tag(b_dtype) : 0, B, F, ws.ptr(), ws.size(), st));
+        }
+        if (w.want[0]) {
+            w.grads[0] = output(x.sizes(), x.scalar_type(), x);
+            if (rows) {
+                check_status(lib.bt_ternary_linear_grad_input((const float*)g.const_data_ptr(), (const uint8_t*)w_back.const_data_ptr(), scale_at, 2 * F,
+                                                              (float*)w.grads[0].data_ptr(), B, 2 * F, K, st));
+            } else {
+                const Scratch ws(lib.bt_tiled_forward_workspace_bytes(B, K, 2 * Fv, dt), x);
+                check_status(lib.bt_ternary_linear_tiled_forward(g.const_data_ptr(), 2 * Fv, dt, 0, nullptr, 0, 0.0f, (const uint8_t*)w_back.const_data_ptr(),
+                                                                 one, BT_F32, 1, nullptr, 0, nullptr, 0, w.grads[0].data_ptr(), B, K, 2 * Fv, ws.ptr(), ws.size(), st));
+            }
+        }
+        if (want_w) {
+            const at::ScalarType dtype = w_dtype == x.scalar_type() ? w_dtype : at::kFloat;
+            at::Tensor dw = output({2 * Fv, K}, dtype, x);
+            if (rows) {
+                const Scratch ws(lib.bt_linear_grad_weight_workspace_bytes(B, 2 * F, K), x);
+                check_status(lib.bt_linear_grad_weight((const float*)g.const_data_ptr(), (const float*)x.const_data_ptr(), scale_at, 2 * F, (float*)dw.data_ptr(),
+                                                       nullptr, B, 2 * F, K, ws.ptr(), ws.size(), st));
+            } else {
+                const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fv, K), x);
+                check_status(lib.bt_linear_grad_weight_16(g.const_data_ptr(), x.const_data_ptr(), dt, one, BT_F32, 1, dw.data_ptr(), tag(dtype), B, 2 * Fv, K,
+                                                          ws.ptr(), ws.size(), st));
+            }
+            for (int i = 0; i < 2; i++)
+                if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * Fv, F).to(w_dtype);
+        }
+        for (int i = 0; i < 2; i++)
+            if (w.want[3 + i]) w.grads[3 + i] = db.narrow(0, i * F, F);
+        return once("ternary_gated_linear", graph, std::move(w.grads), incoming);
+    }
+};
+
+// gated_linear(x, gate, up, gate_bias, up_bias, threshold_factor, per_channel) -> h, where no autocast asks for another dtype
+PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    int device;
+    double threshold;
+    bool per_channel;
+    ORDINARY(n_args == 7);
+    const at::Tensor* x = rows_of(a[0], &device);
+    ORDINARY(x && as_float(a[5], &threshold) && as_bool(a[6], &per_channel) && !at::autocast::is_autocast_enabled(at::kCUDA));
+    const at::Tensor *gate = plain(a[1], device), *up = plain(a[2], device), *gate_bias = nullptr, *up_bias = nullptr;
+    ORDINARY(gate && up && gate->dim() == 2 && gate->sizes() == up->sizes() && gate->scalar_type() == up->scalar_type() && tag(gate->scalar_type()) >= 0);
+    const int64_t F = gate->size(0), K = gate->size(1);
+    ORDINARY(x->size(-1) == K && (x->scalar_type() == at::kFloat ? K >= 4 && F >= 2 : K % 8 == 0 && aligned(*x, 16)));
+    if (a[3] != Py_None) ORDINARY((gate_bias = vec(a[3], F, false, device)));
+    if (a[4] != Py_None) ORDINARY((up_bias = vec(a[4], F, false, device)) && (!gate_bias || gate_bias->scalar_type() == up_bias->scalar_type()));
+    if (differentiated({x, gate, up, gate_bias, up_bias}))
+        return THPVariable_Wrap(GatedLinear::apply(*x, *gate, *up, maybe(gate_bias), maybe(up_bias), threshold, per_channel));
+    return THPVariable_Wrap(gated_run(*x, *gate, *up, maybe(gate_bias), maybe(up_bias), threshold, per_channel, false, false).h);
+    END_HANDLE_TH_ERRORS
+}
+
 // generic_kernel_asked(): whether BITTORCH_KERNEL=generic, read now
 PyObject* generic_kernel_asked(PyObject*, PyObject* const*, Py_ssize_t) {
     const char* env = std::getenv("BITTORCH_KERNEL");
@@ -559,7 +875,7 @@ PyObject* names(PyObject*, PyObject* const*, Py_ssize_t) {
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(names), METHOD(stamp), METHOD(tiled_forward), METHOD(packed_forward), METHOD(tensor_core_forward),
                          METHOD(quantize_pack), METHOD(grad_input), METHOD(grad_weight),
-                         METHOD(grad_weight_16), METHOD(unpack_dequant), METHOD(rmsnorm_int8), METHOD(swiglu_int8), METHOD(gemm_i8_tiled), METHOD(swiglu_i8_tiled), METHOD(act_quant_int8),
+                         METHOD(grad_weight_16), METHOD(unpack_dequant), METHOD(rmsnorm_int8), METHOD(swiglu_int8), METHOD(gemm_i8_tiled), METHOD(swiglu_i8_tiled), METHOD(act_quant_int8), METHOD(add_rmsnorm), METHOD(gated_linear),
                          METHOD(generic_kernel_asked), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Native host side of small calls (csrc/calls.cpp)", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

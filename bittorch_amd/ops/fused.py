@@ -79,6 +79,9 @@ def add_rmsnorm(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor] 
     and ``weight`` through ``s`` and ``y`` (once: no graph of the backward pass is kept); ``q`` carries no gradient."""
     from .. import _C
 
+    out = _C._N.add_rmsnorm(x, residual, weight, eps, store, quantize, operand_order, return_rowsum)
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
         out = _AddRMSNorm.apply(x, residual, weight, eps, store, quantize, operand_order, return_rowsum)
         return out if residual is not None else (x, *out)

@@ -123,6 +123,12 @@ def ternary_gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate
     On the GPU ``x`` and the masters are fp32, fp16 or bf16, in any combination; 16-bit results are rounded once, from fp32 projections.
     Differentiable (once) in all five tensors with the straight-through gradient of ``TernaryLinear``; the gradients of the masters and
     biases have their dtype.  Under autocast it runs in fp16, as ``TernaryLinear``.  On the CPU: the same in plain torch operations."""
+    if x.is_cuda:
+        from .. import _C
+
+        h = _C._N.gated_linear(x, gate_weight, up_weight, gate_bias, up_bias, threshold_factor, per_channel)
+        if h is not None:
+            return h
     _check_gated(x, gate_weight, up_weight, gate_bias, up_bias)
     if not x.is_cuda:
         g, u = (F.linear(x, (q * s.reshape(-1, 1)).to(x.dtype), None if b is None else b.to(x.dtype))

@@ -283,6 +283,43 @@ def test_streams_and_captured_graphs():
             assert all(torch.equal(a, b) for a, b in zip(step(*static), expect))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,rt", TYPES)
+def test_native_and_python_calls_agree(dt, rt, monkeypatch):
+    """csrc/calls.cpp and ops/fused.py, bit for bit, and each refuses a second derivative."""
+    from bittorch_amd import _C, _lib
+    ops = _ops()
+    x, res, w, ds, dy = [t.reshape(t.shape[0] // 3, 3, -1) if t.dim() == 2 else t for t in _inputs(21, 264, dt, rt, seed=9)]
+    native, got = _C._N, []
+    for calls in (native, _lib._PythonCalls()):
+        monkeypatch.setattr(_C, "_N", calls)
+        outs = []
+        for residual in (res, None):
+            for weight in (w, w.float(), None):
+                for flags in (dict(), dict(quantize=True, return_rowsum=True), dict(store=False, quantize=True)):
+                    outs += ops.add_rmsnorm(x, residual, weight, EPS, **flags)
+                    leaves = [t.clone().requires_grad_() for t in (x, residual, weight) if t is not None]
+                    it = iter(leaves)
+                    args = [None if t is None else next(it) for t in (x, residual, weight)]
+                    out = ops.add_rmsnorm(*args, EPS, **flags)
+                    outs += [t.detach() for t in out]
+                    assert [t.requires_grad for t in out] == [True] * (1 + flags.get("store", True)) + [False] * (len(out) - 1 - flags.get("store", True))
+                    for used, incoming in (((0, 1), (ds, dy)), ((0,), (ds,)), ((1,), (dy,))):
+                        if max(used) == 1 and not flags.get("store", True):
+                            continue
+                        incoming = [g if i else g.to(out[0].dtype) for i, g in zip(used, incoming)]
+                        grads = torch.autograd.grad([out[i] for i in used], leaves, incoming, retain_graph=True, allow_unused=True)
+                        outs += [t for t in grads if t is not None]
+        got.append(outs)
+        leaf = x.clone().requires_grad_()
+        dx, = torch.autograd.grad(ops.add_rmsnorm(leaf, res, w, EPS)[1], leaf, dy.clone().requires_grad_(), create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.sum().backward()
+    assert len(got[0]) == len(got[1]) > 50
+    for a, b in zip(*got):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+
+
 def test_refusals():
     from bittorch_amd import _C, _lib, ops
     x = torch.randn(4, 16)

@@ -71,6 +71,7 @@ def _assert_within(got, want, tol, what):
 
 
 def _norm_error(got, want):
+    got = got.detach()
     return float((got.double() - want).norm() / want.norm().clamp(min=1e-300))
 
 
@@ -321,6 +322,39 @@ def test_streams_and_captured_graphs(dt):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, expect))
             assert all(torch.equal(a, b) for a, b in zip(step(*static), expect))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,wt", [(d, d) for d in DTYPES] + [(torch.bfloat16, torch.float32), (torch.float32, torch.float16), (torch.float16, torch.bfloat16)])
+def test_native_and_python_calls_agree(dt, wt, monkeypatch):
+    """csrc/calls.cpp and ops/gated.py, bit for bit, for every set of wanted gradients."""
+    from bittorch_amd import _C, _lib
+    x, wg, wu, bg, bu, dh = _inputs(36, 72, 44, dt, wt, seed=10)
+    x, dh = x.reshape(4, 9, 72), dh.reshape(4, 9, 44)
+    native, got = _C._N, []
+    for calls in (native, _lib._PythonCalls()):
+        monkeypatch.setattr(_C, "_N", calls)
+        outs = []
+        for biases in ((bg, bu), (bg, None), (None, bu), (None, None)):
+            for quant in (dict(), dict(threshold_factor=0.4, per_channel=False)):
+                args = [t if t is None else t.clone().requires_grad_() for t in (x, wg, wu, *biases)]
+                leaves = [t for t in args if t is not None]
+                h = _gated(*args, **quant)
+                outs += [h.detach(), *torch.autograd.grad(h, leaves, dh, retain_graph=True)]
+                outs += [torch.autograd.grad(h, leaf, dh, retain_graph=True)[0] for leaf in leaves]
+                for n in range(len(leaves)):
+                    one = [t if t is None else t.detach() for t in args]
+                    at = [i for i, t in enumerate(args) if t is not None][n]
+                    one[at].requires_grad_()
+                    outs += torch.autograd.grad(_gated(*one, **quant), one[at], dh)
+        got.append(outs)
+        leaf = x.clone().requires_grad_()
+        dx, = torch.autograd.grad(_gated(leaf, wg, wu), leaf, dh.clone().requires_grad_(), create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.sum().backward()
+    assert len(got[0]) == len(got[1]) > 50
+    for a, b in zip(*got):
+        assert a.shape == b.shape and a.dtype == b.dtype and a.is_contiguous() and torch.equal(a, b)
 
 
 @pytest.mark.gpu
