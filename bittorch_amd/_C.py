@@ -856,7 +856,7 @@ def add_rmsnorm_backward(s: Tensor, rstd: Tensor, weight: Optional[Tensor], d_su
 def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, up_bias: Optional[Tensor] = None,
                   threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, rows: bool = False, back: bool = False):
     """The operands of the gated pair, of two masters ``[F, K]`` quantized as :func:`ternary_quantize_pack` does: ``(W_pairs, W_back,
-    scale, bias)`` as ``bt_gated_weights`` makes them; ``rows``: ``W_rows [ceil(K/4), 2 F]`` in the first place; ``back``: with the copy
+    scale, bias)`` as ``bt_gated_quantize`` makes them; ``rows``: ``W_rows [ceil(K/4), 2 F]`` in the first place; ``back``: with the copy
     for the input's gradient (otherwise None)."""
     _check(gate.dim() == 2 and gate.shape == up.shape and gate.dtype == up.dtype, "gate and up weights must match, 2D [F, K]")
     _check(gate.numel() > 0, "weight is empty")
@@ -874,29 +874,25 @@ def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, 
         bdt = bdt if bdt in _DT and all(b is None or b.dtype == bdt for b in biases) else torch.float32
         biases = [None if b is None else b.to(bdt).contiguous() for b in biases]
     Fv = F if rows else (F + 15) // 16 * 16
-    packed = torch.empty((2, Kb, F), dtype=torch.uint8, device=dev)
-    scales = torch.empty((2, F if per_channel else 1), dtype=torch.float32, device=dev)
     w = torch.empty((Kb, 2 * F) if rows else (_L.bt_tiled_weights_bytes(2 * Fv, K),), dtype=torch.uint8, device=dev)
     w_back = torch.empty((_L.bt_tiled_weights_bytes(K, 2 * Fv),), dtype=torch.uint8, device=dev) if back and not rows else None
     scale = torch.empty((2 * Fv + 1,), dtype=torch.float32, device=dev)
     has_bias = any(b is not None for b in biases)
     bias = torch.empty((2 * Fv,), dtype=torch.float32, device=dev) if has_bias else None
     with _on(gate):
-        st = _stream(gate)
-        for i, m in enumerate(masters):
-            _status(_L.bt_quantize_pack(m.data_ptr(), wdt, F, K, float(threshold_factor), int(bool(per_channel)), packed[i].data_ptr(),
-                                        scales[i].data_ptr(), None, st))
-        _status(_L.bt_gated_weights(packed[0].data_ptr(), packed[1].data_ptr(), scales[0].data_ptr(), scales[1].data_ptr(),
-                                    scales.shape[1], _ptr(biases[0]), _ptr(biases[1]), _DT[bdt] if has_bias else 0, F, K,
-                                    None if rows else w.data_ptr(), _ptr(w_back), w.data_ptr() if rows else None, scale.data_ptr(),
-                                    _ptr(bias), st))
+        ws = _workspace(_L.bt_gated_quantize_workspace_bytes(F, K, int(bool(per_channel))), dev)
+        _status(_L.bt_gated_quantize(masters[0].data_ptr(), masters[1].data_ptr(), wdt, F, K, float(threshold_factor), int(bool(per_channel)),
+                                     _ptr(biases[0]), _ptr(biases[1]), _DT[bdt] if has_bias else 0, None if rows else w.data_ptr(), _ptr(w_back),
+                                     w.data_ptr() if rows else None, scale.data_ptr(), _ptr(bias), _ptr(ws), 0 if ws is None else ws.numel(),
+                                     _stream(gate)))
     return w, w_back, scale, bias
 
 
 def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optional[Tensor], out_features: int,
-                          want_pre: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
-    """``silu(gate) * up`` ``[B, F]`` of 16-bit rows ``[B, K]`` (K % 8 == 0, zeros behind a shorter weight row) on the operands of
-    :func:`gated_weights`, and with ``want_pre`` the two projections ``[B, 2 Fp]`` fp32 as :func:`gated_grad` reads them."""
+                          want_pre: bool = False) -> Tuple[Tensor, Optional[Tensor], Tensor]:
+    """``silu(gate) * up`` ``[B, F]`` of 16-bit rows ``[B, K]`` on the operands of :func:`gated_weights`; with ``want_pre`` the two
+    projections ``[B, 2 Fp]`` fp32 as :func:`gated_grad` reads them; and the rows as the kernels read them (a padded copy of ``X`` where
+    K is no multiple of 8 or it is not 16-byte aligned)."""
     _check(X.dim() == 2 and X.numel() > 0 and X.dtype in (torch.float16, torch.bfloat16), "X must be 2D fp16 or bf16")
     B, K = X.shape
     F, Fp = out_features, (out_features + 15) // 16 * 16
@@ -906,12 +902,13 @@ def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optio
            "scale and bias must be fp32 with an entry for each padded feature")
     _check(_all_cuda(X, W_pairs, scale, bias), "All tensors must be CUDA")
     X, scale, bias = X.contiguous(), scale.contiguous(), None if bias is None else bias.contiguous()
+    rows = X if K % 8 == 0 and X.data_ptr() % 16 == 0 else torch.empty((B, (K + 7) // 8 * 8), dtype=X.dtype, device=X.device)
     h = torch.empty((B, F), dtype=X.dtype, device=X.device)
     pre = torch.empty((B, 2 * Fp), dtype=torch.float32, device=X.device) if want_pre else None
     with _on(X):
-        _status(_L.bt_ternary_gated_forward(X.data_ptr(), _DT[X.dtype], W_pairs.data_ptr(), scale.data_ptr(), _ptr(bias), h.data_ptr(),
-                                            _ptr(pre), B, F, K, _stream(X)))
-    return h, pre
+        _status(_L.bt_ternary_gated_forward(X.data_ptr(), _DT[X.dtype], None if rows is X else rows.data_ptr(), W_pairs.data_ptr(),
+                                            scale.data_ptr(), _ptr(bias), h.data_ptr(), _ptr(pre), B, F, K, _stream(X)))
+    return h, pre, rows
 
 
 def gated_grad(dH: Tensor, pre: Tensor, scale: Optional[Tensor], bias_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Optional[Tensor]]:

@@ -382,30 +382,33 @@ __global__ __launch_bounds__(256) void add_rmsnorm_gradw_any_kernel(AddNormGradP
     p.parts[(int64_t)blockIdx.y * p.K + k] = sum;
 }
 
-// Sums over the rows of `parts`: a workgroup takes 64 columns, its four waves every fourth row each.
-__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ parts, int64_t n, int64_t K, void* out, int dtype) {
-    __shared__ float sums[4][64];
+// Sums over the rows of `parts`: a workgroup takes 64 columns, its sixteen waves every sixteenth row each (a row of them at a time in
+// flight: with four waves 256 rows of 2560 took 6.5 us, most of it waiting).
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ parts, int64_t n, int64_t K, void* out, int dtype) {
+    __shared__ float sums[16][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t k = (int64_t)blockIdx.x * 64 + lane;
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (four loads in flight)
     if (k < K) {
         int64_t i = wave;
-        for (; i + 12 < n; i += 16)
+        for (; i + 48 < n; i += 64)
 #pragma unroll
-            for (int u = 0; u < 4; u++) a[u] += parts[(i + 4 * u) * K + k];
-        for (; i < n; i += 4) a[0] += parts[i * K + k];
+            for (int u = 0; u < 4; u++) a[u] += parts[(i + 16 * u) * K + k];
+        for (; i < n; i += 16) a[0] += parts[i * K + k];
     }
     sums[wave][lane] = (a[0] + a[1]) + (a[2] + a[3]);
     __syncthreads();
     if (wave == 0 && k < K) {
-        const float v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 16; q += 4) v += (sums[q][lane] + sums[q + 1][lane]) + (sums[q + 2][lane] + sums[q + 3][lane]);
         if (dtype == BT_F32) store_elem<BT_F32>(out, k, v);
         else if (dtype == BT_F16) store_elem<BT_F16>(out, k, v);
         else store_elem<BT_BF16>(out, k, v);
     }
 }
 int launch_column_sum(const float* parts, int64_t n, int64_t K, void* out, int out_dtype, hipStream_t st, const char* who) {
-    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)ceil_div(K, 64)), dim3(256), 0, st, parts, n, K, out, out_dtype);
+    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)ceil_div(K, 64)), dim3(1024), 0, st, parts, n, K, out, out_dtype);
     return check_launch(who);
 }
 

@@ -41,7 +41,7 @@ namespace {
     X(bt_ternary_linear_tensor_core_forward) X(bt_quantize_pack) X(bt_ternary_linear_grad_input) X(bt_linear_grad_weight)      \
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
     X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
-    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_weights) X(bt_ternary_gated_forward) X(bt_gated_grad)                \
+    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_ternary_gated_forward) X(bt_gated_grad)                \
     X(bt_gated_grad_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -692,38 +692,42 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 struct GatedOut {
-    at::Tensor h, pre, w_back, scale;
+    at::Tensor h, rows, pre, w_back, scale;  // rows: x, or the copy of it that the kernels read
 };
-// fp32 rows: K >= 4, F >= 2; 16-bit rows: K % 8 == 0 and 16-byte aligned.  All tensors contiguous.
+// fp32 rows: K >= 4, F >= 2.  All tensors contiguous.
 GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const MaybeTensor& gate_bias, const MaybeTensor& up_bias,
                    double threshold, bool per_channel, bool keep, bool want_back) {
     const int64_t F = gate.size(0), K = gate.size(1), Kb = (K + 3) / 4, B = x.numel() / K;
-    const bool rows = x.scalar_type() == at::kFloat;
-    const int64_t Fv = rows ? F : (F + 15) / 16 * 16;
-    const int dt = tag(x.scalar_type()), wdt = tag(gate.scalar_type());
+    const bool fp32 = x.scalar_type() == at::kFloat;
+    const int64_t Fv = fp32 ? F : (F + 15) / 16 * 16;
+    const int dt = tag(x.scalar_type());
     void* st = stream_of(x.get_device());
-    // the packed bytes of both layers and their scales, read by the next launch alone
-    const at::Tensor packed = output({2, Kb, F}, at::kByte, x), scales = output({2, per_channel ? F : 1}, at::kFloat, x);
-    uint8_t* const codes[2] = {(uint8_t*)packed.data_ptr(), (uint8_t*)packed.data_ptr() + Kb * F};
-    float* const absmax[2] = {(float*)scales.data_ptr(), (float*)scales.data_ptr() + scales.size(1)};
-    for (int i = 0; i < 2; i++)
-        call(lib.bt_quantize_pack, (i ? up : gate).const_data_ptr(), wdt, F, K, threshold, per_channel ? 1 : 0, codes[i], absmax[i], nullptr, st);
     GatedOut o;
-    const at::Tensor w = rows ? output({Kb, 2 * F}, at::kByte, x) : output({(int64_t)lib.bt_tiled_weights_bytes(2 * Fv, K)}, at::kByte, x);
-    if (rows) o.w_back = w;
+    o.rows = x;
+    const at::Tensor w = fp32 ? output({Kb, 2 * F}, at::kByte, x) : output({(int64_t)lib.bt_tiled_weights_bytes(2 * Fv, K)}, at::kByte, x);
+    if (fp32) o.w_back = w;
     else if (want_back) o.w_back = output({(int64_t)lib.bt_tiled_weights_bytes(K, 2 * Fv)}, at::kByte, x);
     o.scale = output({2 * Fv + 1}, at::kFloat, x);
     at::Tensor bias;
     if (gate_bias || up_bias) bias = output({2 * Fv}, at::kFloat, x);
     float* const scale_at = (float*)o.scale.data_ptr();
     float* const bias_at = bias.defined() ? (float*)bias.data_ptr() : nullptr;
-    call(lib.bt_gated_weights, codes[0], codes[1], absmax[0], absmax[1], scales.size(1), data_of(gate_bias), data_of(up_bias),
-         gate_bias ? tag_of(gate_bias) : tag_of(up_bias), F, K, rows ? nullptr : (uint8_t*)w.data_ptr(),
-         !rows && want_back ? (uint8_t*)o.w_back.data_ptr() : nullptr, rows ? (uint8_t*)w.data_ptr() : nullptr, scale_at, bias_at, st);
+    {
+        const Scratch ws(lib.bt_gated_quantize_workspace_bytes(F, K, per_channel ? 1 : 0), x);
+        call(lib.bt_gated_quantize, gate.const_data_ptr(), up.const_data_ptr(), tag(gate.scalar_type()), F, K, threshold, per_channel ? 1 : 0,
+             data_of(gate_bias), data_of(up_bias), gate_bias ? tag_of(gate_bias) : tag_of(up_bias), fp32 ? nullptr : (uint8_t*)w.data_ptr(),
+             !fp32 && want_back ? (uint8_t*)o.w_back.data_ptr() : nullptr, fp32 ? (uint8_t*)w.data_ptr() : nullptr, scale_at, bias_at, ws.ptr(),
+             ws.size(), st);
+    }
     o.h = output(with_last(x, F), x.scalar_type(), x);
-    if (rows || keep) o.pre = output({B, 2 * Fv}, at::kFloat, x);
-    if (!rows) {
-        call(lib.bt_ternary_gated_forward, x.const_data_ptr(), dt, (const uint8_t*)w.const_data_ptr(), scale_at, bias_at, o.h.data_ptr(),
+    if (fp32 || keep) o.pre = output({B, 2 * Fv}, at::kFloat, x);
+    if (!fp32) {
+        void* padded = nullptr;
+        if (K % 8 != 0 || !aligned(x, 16)) {
+            o.rows = output({B, (K + 7) / 8 * 8}, x.scalar_type(), x);
+            padded = o.rows.data_ptr();
+        }
+        call(lib.bt_ternary_gated_forward, x.const_data_ptr(), dt, padded, (const uint8_t*)w.const_data_ptr(), scale_at, bias_at, o.h.data_ptr(),
              keep ? (float*)o.pre.data_ptr() : nullptr, B, F, K, st);
         return o;
     }
@@ -738,7 +742,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const MaybeTensor& gate_bias,
                               const MaybeTensor& up_bias, double threshold, bool per_channel) {
         GatedOut o = gated_run(x, gate, up, gate_bias, up_bias, threshold, per_channel, true, x.requires_grad());
-        ctx->save_for_backward({x, o.pre, o.w_back, o.scale});
+        ctx->save_for_backward({o.rows, o.pre, o.w_back, o.scale});
         ctx->saved_data["shape"] = std::vector<int64_t>{gate.size(0), gate.size(1)};
         ctx->saved_data["dtype"] = gate.scalar_type();
         ctx->saved_data["biases"] = (int64_t)((gate_bias ? 1 : 0) | (up_bias ? 2 : 0));
@@ -756,7 +760,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         const bool graph = at::GradMode::is_enabled();
         const at::NoGradGuard no_grad;
         const c10::DeviceGuard guard(x.device());
-        const int64_t F = shape[0], K = shape[1], B = x.numel() / K;
+        const int64_t F = shape[0], K = shape[1], Kr = x.size(-1), B = x.numel() / Kr;  // (a padded copy has longer rows)
         const bool rows = x.scalar_type() == at::kFloat;
         const int64_t Fv = rows ? F : (F + 15) / 16 * 16;
         const int dt = tag(x.scalar_type());
@@ -772,7 +776,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
                                            want_b ? tag(b_dtype) : 0, B, F, ws.ptr(), ws.size(), st));
         }
         if (w.want[0]) {
-            w.grads[0] = output(x.sizes(), x.scalar_type(), x);
+            w.grads[0] = output(with_last(incoming[0], K), x.scalar_type(), x);
             if (rows) {
                 check_status(lib.bt_ternary_linear_grad_input((const float*)g.const_data_ptr(), (const uint8_t*)w_back.const_data_ptr(), scale_at, 2 * F,
                                                               (float*)w.grads[0].data_ptr(), B, 2 * F, K, st));
@@ -784,18 +788,18 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         }
         if (want_w) {
             const at::ScalarType dtype = w_dtype == x.scalar_type() ? w_dtype : at::kFloat;
-            at::Tensor dw = output({2 * Fv, K}, dtype, x);
+            at::Tensor dw = output({2 * Fv, Kr}, dtype, x);
             if (rows) {
                 const Scratch ws(lib.bt_linear_grad_weight_workspace_bytes(B, 2 * F, K), x);
                 check_status(lib.bt_linear_grad_weight((const float*)g.const_data_ptr(), (const float*)x.const_data_ptr(), scale_at, 2 * F, (float*)dw.data_ptr(),
                                                        nullptr, B, 2 * F, K, ws.ptr(), ws.size(), st));
             } else {
-                const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fv, K), x);
-                check_status(lib.bt_linear_grad_weight_16(g.const_data_ptr(), x.const_data_ptr(), dt, one, BT_F32, 1, dw.data_ptr(), tag(dtype), B, 2 * Fv, K,
+                const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fv, Kr), x);
+                check_status(lib.bt_linear_grad_weight_16(g.const_data_ptr(), x.const_data_ptr(), dt, one, BT_F32, 1, dw.data_ptr(), tag(dtype), B, 2 * Fv, Kr,
                                                           ws.ptr(), ws.size(), st));
             }
             for (int i = 0; i < 2; i++)
-                if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * Fv, F).to(w_dtype);
+                if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * Fv, F).narrow(1, 0, K).to(w_dtype).contiguous();
         }
         for (int i = 0; i < 2; i++)
             if (w.want[3 + i]) w.grads[3 + i] = db.narrow(0, i * F, F);
@@ -815,7 +819,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *gate = plain(a[1], device), *up = plain(a[2], device), *gate_bias = nullptr, *up_bias = nullptr;
     ORDINARY(gate && up && gate->dim() == 2 && gate->sizes() == up->sizes() && gate->scalar_type() == up->scalar_type() && tag(gate->scalar_type()) >= 0);
     const int64_t F = gate->size(0), K = gate->size(1);
-    ORDINARY(x->size(-1) == K && (x->scalar_type() == at::kFloat ? K >= 4 && F >= 2 : K % 8 == 0 && aligned(*x, 16)));
+    ORDINARY(x->size(-1) == K && (x->scalar_type() != at::kFloat || (K >= 4 && F >= 2)));
     if (a[3] != Py_None) ORDINARY((gate_bias = vec(a[3], F, false, device)));
     if (a[4] != Py_None) ORDINARY((up_bias = vec(a[4], F, false, device)) && (!gate_bias || gate_bias->scalar_type() == up_bias->scalar_type()));
     if (differentiated({x, gate, up, gate_bias, up_bias}))

@@ -23,9 +23,13 @@ namespace bt {
 
 int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, float* pre, int64_t H, int64_t M,
                           int64_t N, int64_t K, hipStream_t st);
+int launch_pad_rows(const void* X, int64_t B, int64_t K, void* P, hipStream_t st);
+float quantize_clamp_min(int w_dtype);
 bool gemm_f16_supported(int64_t N, int64_t K, const void* X, const void* W_T, const void* Y, bool tiled);
 
-// ---- the two layers' packed weights as one operand ----------------------------------------------------------------------
+static int64_t padded(int64_t F) { return ceil_div(F, 16) * 16; }
+
+// ---- the two masters as one operand ---------------------------------------------------------------------------------------
 
 struct GatedWeightsParams {
     const uint8_t* W[2];      // gate, up: packed [ceil(K / 4), F]
@@ -38,7 +42,7 @@ struct GatedWeightsParams {
     uint8_t* rows;            // or both as they lie, side by side: [Kb, 2 F]
     float* scale;             // [2 Fv + 1], the last one 1 (the scale of products that have none)
     float* bias;              // [2 Fv] or null
-    uint32_t n_pairs, n_back, n_rows;  // workgroups of each part, in this order; one more for the vectors
+    uint32_t n_pairs, n_back, n_rows;  // workgroups of each part, in this order; behind them those of the vectors
     uint32_t steps, back_steps;        // 64-wide steps of the two tiled copies
 };
 
@@ -52,7 +56,13 @@ __device__ __forceinline__ u32x4 codes16(const uint8_t* row, int64_t n, int64_t 
     return d;
 }
 
-// Bound by the packed bytes, read once for each copy and written once; all parts in one launch.
+// the codes at bits 0, 8, 16, 24 as one byte
+__device__ __forceinline__ uint32_t byte_of_codes(uint32_t t) {
+    const uint32_t x = t & 0x03030303u;
+    return (x | x >> 6 | x >> 12 | x >> 18) & 0xffu;
+}
+
+// From packed bytes.  Bound by them, read once for each copy and written once; all parts in one launch.
 __global__ __launch_bounds__(256) void gated_weights_kernel(GatedWeightsParams p) {
     constexpr int PITCH = 256 + 16;
     __shared__ __attribute__((aligned(16))) uint8_t block[16 * PITCH];
@@ -101,10 +111,7 @@ __global__ __launch_bounds__(256) void gated_weights_kernel(GatedWeightsParams p
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const uint32_t x = (d[r] >> (2 * c)) & 0x03030303u;
-                out[c] |= ((x | x >> 6 | x >> 12 | x >> 18) & 0xffu) << (8 * r);
-            }
+            for (int c = 0; c < 4; c++) out[c] |= byte_of_codes(d[r] >> (2 * c)) << (8 * r);
         ((uint4*)p.back)[(t * S + s) * 16 + 4 * g + q] = make_uint4(out[0], out[1], out[2], out[3]);
         return;
     }
@@ -122,14 +129,167 @@ __global__ __launch_bounds__(256) void gated_weights_kernel(GatedWeightsParams p
             for (int e = 0; n + e < p.F; e++) dst[n + e] = src[n + e];
         return;
     }
-    for (int64_t n = tid; n < 2 * p.Fv; n += 256) {
+    const int64_t n = (int64_t)(wg - p.n_rows) * 256 + tid;
+    if (n < 2 * p.Fv) {
         const int half = n >= p.Fv;
         const int64_t f = n - (half ? p.Fv : 0);
         p.scale[n] = f < p.F ? p.a[half][p.one_scale ? 0 : f] : 0.0f;
         if (p.bias) p.bias[n] = f < p.F && p.b[half] ? load_elem_rt(p.b[half], p.bias_dtype, f) : 0.0f;
+    } else if (n == 2 * p.Fv) {
+        p.scale[n] = 1.0f;
     }
-    if (tid == 0) p.scale[2 * p.Fv] = 1.0f;
 }
+
+struct GatedQuantizeParams {
+    const void* W[2];         // masters gate, up [F, K]
+    const void* b[2];
+    int bias_dtype;
+    float tf, clamp_min;
+    int F, K, Fv;             // as above
+    int tiles, per_xcd;       // of 16 features, both halves
+    uint8_t *pairs, *back, *rows;
+    float *scale, *bias;
+    uint32_t steps, back_steps;
+};
+
+// Masters of a DT (BT_F32_AS_F16: fp32, rounded to fp16 as they are read)
+constexpr int master_storage(int dt) { return dt == BT_F32_AS_F16 ? BT_F32 : dt; }
+
+// The same from the masters in one pass: a workgroup takes the 16 features of a tile of the copies.  A wave keeps a feature's row in
+// registers (ITERS pieces of eight values a lane, K <= 512 ITERS), reduces its absolute maximum, and puts the codes of four k to a byte into
+// LDS, from where they leave in each layout: the pairs' tile is one run of memory, its dwords are LDS's; a thread turns the codes of 16 k
+// into 64 bytes of the transpose.  The quantizer's arithmetic is that of quantize_pack.hip, on the same values.  Bound by the masters,
+// read once: 2 x 6912 x 2560 bf16 (71 MB) takes 18 us, two passes of the quantizer and the copy of their bytes 34.
+template <int DT, int ITERS, bool RAG>
+__global__ __launch_bounds__(512) void gated_quantize_kernel(GatedQuantizeParams p) {
+    constexpr int ST = master_storage(DT), PITCH = ITERS * 128 + 4, RPW = 2;
+    constexpr bool BOTH = ITERS * (ST == BT_F32 ? 2 : 1) <= 10;  // both rows of a wave in registers at once
+    __shared__ __attribute__((aligned(16))) uint8_t codes[16 * PITCH];
+    const int lin = (int)(blockIdx.x & 7) * p.per_xcd + (int)(blockIdx.x >> 3);
+    if (lin >= p.tiles) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per_half = p.tiles / 2, half = lin >= per_half, tile = lin - half * per_half, f0 = 16 * tile;
+    const int K = p.K;
+    const void* const W = p.W[half];
+    Raw8<ST> in[BOTH ? RPW : 1][ITERS];
+    auto load = [&](int r, Raw8<ST> (&to)[ITERS]) {
+        const int f = f0 + RPW * wave + r;
+        const int64_t row = (int64_t)(f < p.F ? f : p.F - 1) * K;  // (a feature past the last one: that row again, its codes are not kept)
+#pragma unroll
+        for (int i = 0; i < ITERS; i++) to[i] = load_raw8<ST>(W, row + piece_at((i * 64 + lane) * 8, K));
+    };
+    if constexpr (BOTH) {
+#pragma unroll
+        for (int r = 0; r < RPW; r++) load(r, in[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < RPW; r++) {
+        const int f = f0 + RPW * wave + r;
+        const bool there = f < p.F;  // (uniform)
+        if constexpr (!BOTH) load(r, in[0]);
+        Raw8<ST> (&row)[ITERS] = in[BOTH ? r : 0];
+        auto values = [&](int i, float (&v)[8]) {
+            widen_piece<ST, RAG>(row[i], (i * 64 + lane) * 8, K, v);
+            if constexpr (DT == BT_F32_AS_F16) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = round_to_dtype(v[e], BT_F16);
+            }
+        };
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ITERS; i++) {
+            float v[8];
+            values(i, v);
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(v[e]));
+        }
+        const float s = fmaxf(wave_max(amax), p.clamp_min);
+        const float thr = round_to_dtype(__fmul_rn(p.tf, s), DT == BT_F32_AS_F16 ? BT_F16 : DT);
+        // (widened again, not kept in fp32 from above: half the registers)
+#pragma unroll
+        for (int i = 0; i < ITERS; i++)
+#pragma unroll
+            for (int q = 0; q < (ST == BT_F32 ? 2 : 1); q++) asm volatile("" : "+v"(row[i].d[q]));
+#pragma unroll
+        for (int i = 0; i < ITERS; i++) {
+            float v[8];
+            values(i, v);
+            uint32_t c = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) c |= (fabsf(v[e]) > thr ? (v[e] < 0.0f ? 2u : 1u) : 0u) << (2 * e);
+            const int k = (i * 64 + lane) * 8;  // (zeros behind the row's end)
+            c = !there || k >= K ? 0u : RAG && k + 8 > K ? c & ((1u << (2 * (K - k))) - 1u) : c;
+            *(uint16_t*)(codes + (RPW * wave + r) * PITCH + (i * 64 + lane) * 2) = (uint16_t)c;
+        }
+        if (lane == 0 && f < p.Fv) {
+            const int at = half * p.Fv + f;
+            p.scale[at] = there ? s : 0.0f;
+            if (p.bias) p.bias[at] = there && p.b[half] ? load_elem_rt(p.b[half], p.bias_dtype, f) : 0.0f;
+            if (at == 0) p.scale[2 * p.Fv] = 1.0f;
+        }
+    }
+    __syncthreads();
+    if (p.pairs) {
+        uint32_t* const out = (uint32_t*)p.pairs + (int64_t)(2 * tile + half) * p.steps * 64;
+        for (uint32_t i = tid; i < p.steps * 64; i += 512)
+            out[i] = *(const uint32_t*)(codes + (i & 15) * PITCH + 16 * (i >> 6) + 4 * ((i >> 4) & 3));
+    }
+    if (!p.back && !p.rows) return;
+    const uint32_t n0 = (uint32_t)(half * p.Fv + f0);
+    for (int kt = tid; 16 * kt < K; kt += 512) {
+        uint32_t t[4][4];  // [features 4 r .. + 3][byte 4 kt + q]
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            uint32_t d[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[i] = *(const uint32_t*)(codes + (4 * r + i) * PITCH + 4 * kt);
+            transpose4x4_bytes(d[0], d[1], d[2], d[3], t[r]);
+        }
+        if (p.back) {
+            uint4* const out = (uint4*)p.back + ((int64_t)kt * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                uint32_t o[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[c] |= byte_of_codes(t[r][q] >> (2 * c)) << (8 * r);
+                out[q] = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            // (the copy's last step holds features past both halves: zeros, from the workgroup of the last tile)
+            if (lin == p.tiles - 1)
+                for (uint32_t g = (n0 >> 4) + 1; g < 4 * p.back_steps; g++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        ((uint4*)p.back)[((int64_t)kt * p.back_steps + (g >> 2)) * 16 + 4 * (g & 3) + q] = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (16 * kt + 4 * q >= K) break;
+                uint8_t* dst = p.rows + (int64_t)(4 * kt + q) * 2 * p.F + half * p.F + f0;
+                const u32x4 v = {t[0][q], t[1][q], t[2][q], t[3][q]};
+                if (f0 + 16 <= p.F) *(u32x4_a1*)dst = v;
+                else
+                    for (int e = 0; f0 + e < p.F; e++) dst[e] = (uint8_t)(v[e >> 2] >> (8 * (e & 3)));
+            }
+        }
+    }
+}
+
+template <int DT>
+static void launch_gated_quantize(const GatedQuantizeParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)(8 * p.per_xcd)), block(512);
+#define BT_GQ(IT)                                                                                          \
+    if (p.K <= 512 * IT) {                                                                                 \
+        if (p.K % 8 == 0) hipLaunchKernelGGL((gated_quantize_kernel<DT, IT, false>), grid, block, 0, st, p); \
+        else hipLaunchKernelGGL((gated_quantize_kernel<DT, IT, true>), grid, block, 0, st, p);              \
+        return;                                                                                            \
+    }
+    BT_GQ(2) BT_GQ(5) BT_GQ(8) BT_GQ(16)
+#undef BT_GQ
+}
+// Rows that a wave holds, with a scale each; the others are quantized by bt_quantize_pack and their bytes put in place
+static bool gated_quantizes(int64_t K, bool per_channel) { return per_channel && K >= 8 && K <= 8192; }
 
 // ---- gradient of silu(g) u ------------------------------------------------------------------------------------------------
 
@@ -227,7 +387,6 @@ __global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p
     p.parts[(int64_t)blockIdx.y * 2 * F + F + k] = bu;
 }
 
-static int64_t padded(int64_t F) { return ceil_div(F, 16) * 16; }
 // Runs of rows of the gradient kernel: enough workgroups for the chip; 64 at most where each leaves sums behind
 static int64_t grad_runs(int64_t B, int64_t F, bool sums) {
     const int64_t across = ceil_div(F, 2048), want = std::max<int64_t>(1, 8 * gemm_compute_units() / across);
@@ -249,16 +408,25 @@ static void launch_gated_grad(const GatedGradParams& p, int64_t runs, hipStream_
 
 using namespace bt;
 
-extern "C" int bt_gated_weights(const uint8_t* gate_T, const uint8_t* up_T, const float* gate_scale, const float* up_scale, int64_t scale_len,
-                                const void* gate_bias, const void* up_bias, int bias_dtype, int64_t F, int64_t K, uint8_t* W_pairs,
-                                uint8_t* W_back, uint8_t* W_rows, float* scale, float* bias, void* stream) {
-    const char* who = "bt_gated_weights";
-    if (!gate_T || !up_T || !gate_scale || !up_scale || !scale || F <= 0 || K <= 0 || (!W_pairs && !W_rows) || (W_rows && (W_pairs || W_back))) {
+extern "C" size_t bt_gated_quantize_workspace_bytes(int64_t F, int64_t K, int per_channel) {
+    if (F <= 0 || K <= 0 || gated_quantizes(K, per_channel != 0)) return 0;
+    return (size_t)(2 * ceil_div(ceil_div(K, 4) * F, 256) * 256 + 2 * (per_channel ? F : 1) * 4);  // [gate's bytes][up's][scales]
+}
+
+extern "C" int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, int64_t K, double threshold_factor, int per_channel,
+                                 const void* gate_bias, const void* up_bias, int bias_dtype, uint8_t* W_pairs, uint8_t* W_back, uint8_t* W_rows,
+                                 float* scale, float* bias, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "bt_gated_quantize";
+    if (!gate || !up || !scale || F <= 0 || K <= 0 || (!W_pairs && !W_rows) || (W_rows && (W_pairs || W_back))) {
         set_error("%s: null pointer or empty shape, or both the tiled copies and the rows asked for", who);
         return BT_ERR_INVALID;
     }
-    if ((scale_len != F && scale_len != 1) || ((gate_bias || up_bias) && (!bias || (bias_dtype != BT_F32 && bias_dtype != BT_F16 && bias_dtype != BT_BF16)))) {
-        set_error("%s: scale size doesn't match F, or a bias without room for it or of an unsupported dtype", who);
+    if (w_dtype != BT_F32 && w_dtype != BT_F16 && w_dtype != BT_BF16 && w_dtype != BT_F32_AS_F16) {
+        set_error("%s: unsupported weight dtype %d", who, w_dtype);
+        return BT_ERR_INVALID;
+    }
+    if ((gate_bias || up_bias) && (!bias || (bias_dtype != BT_F32 && bias_dtype != BT_F16 && bias_dtype != BT_BF16))) {
+        set_error("%s: a bias without room for it or of an unsupported dtype", who);
         return BT_ERR_INVALID;
     }
     const int64_t Fp = padded(F);
@@ -267,20 +435,46 @@ extern "C" int bt_gated_weights(const uint8_t* gate_T, const uint8_t* up_T, cons
         set_error("%s: F and K below 2^23, copies 256-byte aligned and below 4 GiB (F=%lld, K=%lld)", who, (long long)F, (long long)K);
         return BT_ERR_INVALID;
     }
+    const size_t need = bt_gated_quantize_workspace_bytes(F, K, per_channel);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace) % 256 != 0)) {
+        set_error("%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, need, workspace_bytes);
+        return BT_ERR_WORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t Fv = W_rows ? F : Fp, Kb = ceil_div(K, 4);
+    const uint32_t steps = (uint32_t)ceil_div(Kb, 16), back_steps = (uint32_t)ceil_div(2 * Fp, 64);
+    if (!need) {
+        GatedQuantizeParams p = {};
+        p.W[0] = gate; p.W[1] = up; p.b[0] = gate_bias; p.b[1] = up_bias; p.bias_dtype = bias_dtype;
+        p.tf = (float)threshold_factor; p.clamp_min = quantize_clamp_min(w_dtype);
+        p.F = (int)F; p.K = (int)K; p.Fv = (int)Fv; p.tiles = (int)(2 * ceil_div(F, 16)); p.per_xcd = (int)ceil_div(p.tiles, 8);
+        p.pairs = W_pairs; p.back = W_back; p.rows = W_rows; p.scale = scale; p.bias = bias; p.steps = steps; p.back_steps = back_steps;
+        if (w_dtype == BT_F32) launch_gated_quantize<BT_F32>(p, st);
+        else if (w_dtype == BT_F16) launch_gated_quantize<BT_F16>(p, st);
+        else if (w_dtype == BT_BF16) launch_gated_quantize<BT_BF16>(p, st);
+        else launch_gated_quantize<BT_F32_AS_F16>(p, st);
+        return check_launch(who);
+    }
+    uint8_t* codes[2] = {(uint8_t*)workspace, (uint8_t*)workspace + ceil_div(Kb * F, 256) * 256};
+    float* absmax[2];
+    absmax[0] = (float*)((uint8_t*)workspace + 2 * ceil_div(Kb * F, 256) * 256);
+    absmax[1] = absmax[0] + (per_channel ? F : 1);
+    for (int i = 0; i < 2; i++)
+        if (int rc = bt_quantize_pack(i ? up : gate, w_dtype, F, K, threshold_factor, per_channel, codes[i], absmax[i], nullptr, stream)) return rc;
     GatedWeightsParams p = {};
-    p.W[0] = gate_T; p.W[1] = up_T; p.a[0] = gate_scale; p.a[1] = up_scale; p.b[0] = gate_bias; p.b[1] = up_bias;
-    p.bias_dtype = bias_dtype; p.one_scale = scale_len == 1 && F != 1;
-    p.F = F; p.Fv = W_rows ? F : Fp; p.K = K; p.Kb = ceil_div(K, 4);
+    p.W[0] = codes[0]; p.W[1] = codes[1]; p.a[0] = absmax[0]; p.a[1] = absmax[1]; p.b[0] = gate_bias; p.b[1] = up_bias;
+    p.bias_dtype = bias_dtype; p.one_scale = !per_channel;
+    p.F = F; p.Fv = Fv; p.K = K; p.Kb = Kb;
     p.pairs = W_pairs; p.back = W_back; p.rows = W_rows; p.scale = scale; p.bias = bias;
-    p.steps = (uint32_t)ceil_div(p.Kb, 16); p.back_steps = (uint32_t)ceil_div(2 * Fp, 64);
-    p.n_pairs = W_pairs ? (uint32_t)(2 * ceil_div(p.Kb, 16) * ceil_div(Fp, 256)) : 0;
-    p.n_back = W_back ? (uint32_t)(ceil_div(K, 16) * ceil_div(ceil_div(2 * Fp, 64), 16)) : 0;
-    p.n_rows = W_rows ? (uint32_t)ceil_div(p.Kb * 2 * ceil_div(F, 16), 256) : 0;
-    hipLaunchKernelGGL(gated_weights_kernel, dim3(p.n_pairs + p.n_back + p.n_rows + 1), dim3(256), 0, (hipStream_t)stream, p);
+    p.steps = steps; p.back_steps = back_steps;
+    p.n_pairs = W_pairs ? (uint32_t)(2 * steps * ceil_div(Fp, 256)) : 0;
+    p.n_back = W_back ? (uint32_t)(ceil_div(K, 16) * ceil_div(back_steps, 16)) : 0;
+    p.n_rows = W_rows ? (uint32_t)ceil_div(Kb * 2 * ceil_div(F, 16), 256) : 0;
+    hipLaunchKernelGGL(gated_weights_kernel, dim3(p.n_pairs + p.n_back + p.n_rows + (unsigned)(2 * Fv / 256 + 1)), dim3(256), 0, st, p);
     return check_launch(who);
 }
 
-extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
+extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
                                         float* pre, int64_t B, int64_t F, int64_t K, void* stream) {
     const char* who = "bt_ternary_gated_forward";
     if (!X || !W_pairs || !scale || !H || B <= 0 || F <= 0 || K <= 0 || (x_dtype != BT_F16 && x_dtype != BT_BF16)) {
@@ -288,16 +482,20 @@ extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, const uint8_
         return BT_ERR_INVALID;
     }
     const int64_t Fp = padded(F);
-    if (K % 8 != 0 || F >= (1ll << 23) || B >= (1ll << 31) || ((uintptr_t)W_pairs) % 256 != 0 || bt_tiled_weights_bytes(2 * Fp, K) >= (1ull << 32) ||
-        ((uintptr_t)pre) % 16 != 0 || !gemm_f16_supported(2 * Fp, K, X, W_pairs, H, true)) {
-        set_error("%s: K must be a multiple of 8, F and K below 2^23, buffers 16-byte and the weights 256-byte aligned (F=%lld, K=%lld)", who,
-                  (long long)F, (long long)K);
+    const void* rows = X_padded ? X_padded : X;
+    const int64_t Kr = X_padded ? ceil_div(K, 8) * 8 : K;  // values of a row of them
+    if (F >= (1ll << 23) || K >= (1ll << 23) || B >= (1ll << 31) || ((uintptr_t)W_pairs) % 256 != 0 || bt_tiled_weights_bytes(2 * Fp, K) >= (1ull << 32) ||
+        ((uintptr_t)X) % 2 != 0 || ((uintptr_t)pre) % 16 != 0 || !gemm_f16_supported(2 * Fp, Kr, rows, W_pairs, H, true)) {
+        set_error("%s: rows whose length is no multiple of 8 or that are not 16-byte aligned need X_padded; F and K below 2^23, buffers 16-byte "
+                  "and the weights 256-byte aligned (F=%lld, K=%lld)", who, (long long)F, (long long)K);
         return BT_ERR_INVALID;
     }
+    if (X_padded)
+        if (int rc = launch_pad_rows(X, B, K, X_padded, (hipStream_t)stream)) return rc;
     Epilogue epi = {};
     epi.scale = scale; epi.scale_dtype = BT_F32;
     epi.bias = bias; epi.bias_dtype = BT_F32;
-    return launch_gemm_f16_gated(x_dtype == BT_F16 ? MODE_F16 : MODE_BF16, X, W_pairs, epi, H, pre, F, B, 2 * Fp, K, (hipStream_t)stream);
+    return launch_gemm_f16_gated(x_dtype == BT_F16 ? MODE_F16 : MODE_BF16, rows, W_pairs, epi, H, pre, F, B, 2 * Fp, Kr, (hipStream_t)stream);
 }
 
 extern "C" size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F) {

@@ -516,6 +516,15 @@ static int launch_quantize(const void* W, int64_t N, int64_t K, float tf, float 
     return check_launch("bt_quantize_pack");
 }
 
+// 1e-8 rounded to the weight dtype (fp16: 0, bf16: nearest bf16)
+float quantize_clamp_min(int w_dtype) {
+    if (w_dtype == BT_F16 || w_dtype == BT_F32_AS_F16) return 0.0f;
+    if (w_dtype != BT_BF16) return 1e-8f;
+    uint32_t u = __builtin_bit_cast(uint32_t, 1e-8f);
+    u += 0x7fffu + ((u >> 16) & 1u);
+    return __builtin_bit_cast(float, u & 0xffff0000u);
+}
+
 template <int DT>
 static void launch_absmax(const void* W, int64_t total, float* scale, hipStream_t st) {
     const int vec_ok = (((uintptr_t)W) % 16 == 0) ? 1 : 0;
@@ -538,15 +547,7 @@ extern "C" int bt_quantize_pack(const void* W, int w_dtype, int64_t N, int64_t K
     }
     hipStream_t st = (hipStream_t)stream;
     const float tf = (float)threshold_factor;
-    // 1e-8 rounded to the weight dtype (fp16: 0, bf16: nearest bf16)
-    float clamp_min = 1e-8f;
-    if (w_dtype == BT_F16 || w_dtype == BT_F32_AS_F16) clamp_min = 0.0f;
-    if (w_dtype == BT_BF16) {
-        uint32_t u = __builtin_bit_cast(uint32_t, clamp_min);
-        u += 0x7fffu + ((u >> 16) & 1u);
-        u &= 0xffff0000u;
-        clamp_min = __builtin_bit_cast(float, u);
-    }
+    const float clamp_min = quantize_clamp_min(w_dtype);
     if (!per_channel) {
         // tensor scale: zero, absmax over everything; the quantizing kernel floors it, for itself and in place
         hipLaunchKernelGGL(set_scalar_kernel, dim3(1), dim3(1), 0, st, scale, 0.0f);

@@ -52,9 +52,7 @@ class _GatedLinear(torch.autograd.Function):
             h = _C.swiglu(pre[:, :f], pre[:, f:])
             w_back = w
         else:
-            if k % 8 or not x2.is_contiguous() or x2.data_ptr() % 16:
-                x2 = F.pad(x2, (0, -k % 8)) if k % 8 else x2.clone(memory_format=torch.contiguous_format)
-            h, pre = _C.ternary_gated_forward(x2, w, scale, bias, f, keep)
+            h, pre, x2 = _C.ternary_gated_forward(x2, w, scale, bias, f, keep)
         if keep:
             ctx.save_for_backward(x2, pre, w_back, scale)
             ctx.shape = f, k

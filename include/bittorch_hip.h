@@ -248,23 +248,26 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  * The gated pair of a feed-forward block in training, H = silu(g) * u of g = X gate^T + b, u = X up^T + b with two ternary layers of F
  * outputs each (no counterpart in the reference's Python/CUDA code; SwiGLU MLP of its JS runtime, TernaryTransformer.ts:366-423).
  * Fp = F rounded up to a multiple of 16.
- *   bt_gated_weights: what the calls below read, of the two layers' packed bytes [ceil(K/4), F] (bt_quantize_pack), fp32 scales (F
- *     entries or one each) and biases (bias_dtype, or NULL):
+ *   bt_gated_quantize: what the calls below read, of the two masters [F, K] (w_dtype and quantization as in bt_quantize_pack) and biases
+ *     (bias_dtype, or NULL each):
  *       W_pairs  bt_tiled_weights_bytes(2 Fp, K) bytes: the decode-tiled copy of [gate | up] in BT_TILES_GATE_UP_PAIRS order;
  *       W_back   (optional) bt_tiled_weights_bytes(K, 2 Fp) bytes: the decode-tiled copy of their transpose, a layer with K outputs
  *                and 2 Fp inputs, for bt_ternary_linear_tiled_forward on the gradient G;
- *       W_rows   instead of the two: [ceil(K/4), 2 F], both side by side;
+ *       W_rows   instead of the two: the packed bytes [ceil(K/4), 2 F], gate and up side by side;
  *       scale    [2 Fp + 1] (2 F + 1 with W_rows): both layers' scales, zeros behind each, and a 1; bias [2 Fp] (2 F) or NULL.
- *   bt_ternary_gated_forward: fp16 / bf16 rows X [B,K], K % 8 == 0 (zeros behind a shorter row); H [B,F] in x_dtype, rounded once;
+ *     workspace: at least bt_gated_quantize_workspace_bytes(F,K,per_channel) bytes.
+ *   bt_ternary_gated_forward: fp16 / bf16 rows X [B,K]; where K % 8 != 0 or X is not 16-byte aligned, X_padded [B, K rounded up to 8] takes
+ *     a copy of them (zeros behind each), otherwise it is NULL; H [B,F] in x_dtype, rounded once;
  *     pre (optional) [B, 2 Fp] fp32: g and u, columns 2 i and 2 i + 1 of either at 4 i .. 4 i + 3.
  *   bt_gated_grad: G = d(H . dH)/d[g | u].  16-bit dtype: pre as above, G [B, 2 Fp] in dtype, each half times its scale; BT_F32: pre is
  *     [g | u] [B, 2 F] and G [B, 2 F] without scales (scale unused).  dBias (optional) [2 F] in bias_dtype: the sums over the rows without
  *     scales; with it a workspace of bt_gated_grad_workspace_bytes(B,F).
  */
-int bt_gated_weights(const uint8_t* gate_T, const uint8_t* up_T, const float* gate_scale, const float* up_scale, int64_t scale_len,
-                     const void* gate_bias, const void* up_bias, int bias_dtype, int64_t F, int64_t K, uint8_t* W_pairs, uint8_t* W_back,
-                     uint8_t* W_rows, float* scale, float* bias, void* stream);
-int bt_ternary_gated_forward(const void* X, int x_dtype, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
+size_t bt_gated_quantize_workspace_bytes(int64_t F, int64_t K, int per_channel);
+int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, int64_t K, double threshold_factor, int per_channel,
+                      const void* gate_bias, const void* up_bias, int bias_dtype, uint8_t* W_pairs, uint8_t* W_back, uint8_t* W_rows,
+                      float* scale, float* bias, void* workspace, size_t workspace_bytes, void* stream);
+int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
                              float* pre, int64_t B, int64_t F, int64_t K, void* stream);
 size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F);
 int bt_gated_grad(const void* dH, int dtype, const float* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,

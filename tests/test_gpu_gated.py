@@ -12,8 +12,10 @@ U = 2.0 ** -24
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 # rows, K, F: one of each; odd ones; halves that fill no tile, a last stage of the contraction, both sides of 64 and 128 rows, a contraction
 # long enough for two groups of waves
+# a feature too long for the registers of a wave
 SHAPES = [(1, 8, 2), (3, 7, 5), (2, 3, 9), (5, 1, 24), (1, 640, 48), (17, 100, 37), (64, 512, 256), (65, 1001, 33), (129, 520, 272), (300, 1100, 546),
-          (40, 2560, 688), (1000, 264, 520)]
+          (40, 2560, 688), (1000, 264, 520), (35, 4096, 64), (33, 5003, 40),
+          (20, 8192, 48), (17, 8200, 33)]
 
 
 def _gated(*args, **kwargs):
@@ -125,9 +127,9 @@ def test_stages_of_the_16_bit_gradient(rows, k, f, dt):
     ref = _Reference(x, wg, wu, bg, bu, dh)
     fp = (f + 15) // 16 * 16
     w, w_back, scale, bias = _C.gated_weights(wg, wu, bg, bu, back=True)
-    xp = torch.nn.functional.pad(x, (0, -k % 8))
-    h, pre = _C.ternary_gated_forward(xp, w, scale, bias, f, True)
-    assert torch.equal(h, _C.ternary_gated_forward(xp, w, scale, bias, f)[0])
+    h, pre, read = _C.ternary_gated_forward(x, w, scale, bias, f, True)
+    assert torch.equal(h, _C.ternary_gated_forward(x, w, scale, bias, f)[0])
+    assert torch.equal(read, torch.nn.functional.pad(x, (0, -k % 8)))
     pairs = pre.reshape(rows, fp // 2, 2, 2)
     _assert_within(pairs[:, :, 0].reshape(rows, fp)[:, :f], ref.g, ref.tol_g, "g")
     _assert_within(pairs[:, :, 1].reshape(rows, fp)[:, :f], ref.u, ref.tol_u, "u")
@@ -403,15 +405,20 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=text):
             _gated(*args)
     lib, at = _lib.load(), 1 << 20  # (never read: every call ends before a launch)
-    weights = lambda g=at, n=8, b=None, bdt=0, F=8, K=16, pairs=at, back=None, rows=None, scale=at, bias=None: lib.bt_gated_weights(
-        g, at, at, at, n, b, b, bdt, F, K, pairs, back, rows, scale, bias, None)
+    weights = lambda g=at, dt=2, pc=1, b=None, bdt=0, F=8, K=16, pairs=at, back=None, rows=None, scale=at, bias=None, ws=None, n=0: lib.bt_gated_quantize(
+        g, at, dt, F, K, 0.05, pc, b, b, bdt, pairs, back, rows, scale, bias, ws, n, None)
     for kwargs, text in [(dict(g=None), "null"), (dict(scale=None), "null"), (dict(F=0), "empty"), (dict(pairs=None), "null"), (dict(rows=at), "both"),
-                         (dict(pairs=None, back=at, rows=at), "both"), (dict(n=3), "scale size"), (dict(b=at), "bias"),
+                         (dict(pairs=None, back=at, rows=at), "both"), (dict(dt=3), "dtype"), (dict(b=at), "bias"),
                          (dict(b=at, bias=at, bdt=3), "bias"), (dict(pairs=at + 16), "aligned"), (dict(back=at + 16), "aligned"),
-                         (dict(F=1 << 23, n=1), "2^23"), (dict(K=1 << 23), "2^23"), (dict(F=1 << 20, K=1 << 20, n=1), "4 GiB")]:
+                         (dict(F=1 << 23), "2^23"), (dict(K=1 << 23), "2^23"), (dict(F=1 << 20, K=1 << 20), "4 GiB")]:
         assert weights(**kwargs) == -1, kwargs
         assert text in _lib.last_error(), (kwargs, _lib.last_error())
-    forward = lambda X=at, dt=2, W=at, h=at, pre=None, B=4, F=8, K=16: lib.bt_ternary_gated_forward(X, dt, W, at, None, h, pre, B, F, K, None)
+    # a workspace where the rows are longer than a wave holds, or share one scale
+    assert lib.bt_gated_quantize_workspace_bytes(8, 16, 1) == 0 and lib.bt_gated_quantize_workspace_bytes(0, 16, 0) == 0
+    for kwargs in (dict(pc=0), dict(K=8200), dict(K=4)):
+        need = lib.bt_gated_quantize_workspace_bytes(8, kwargs.get("K", 16), kwargs.get("pc", 1))
+        assert need > 0 and weights(**kwargs) == -2 and weights(ws=at, n=need - 1, **kwargs) == -2 and weights(ws=at + 64, n=need, **kwargs) == -2
+    forward = lambda X=at, dt=2, W=at, h=at, pre=None, B=4, F=8, K=16: lib.bt_ternary_gated_forward(X, dt, None, W, at, None, h, pre, B, F, K, None)
     for kwargs in (dict(X=None), dict(dt=0), dict(dt=5), dict(W=None), dict(h=None), dict(B=0), dict(K=12), dict(X=at + 8), dict(W=at + 128), dict(pre=at + 8),
                    dict(h=at + 4), dict(F=1 << 23), dict(B=1 << 31)):
         assert forward(**kwargs) == -1, kwargs
