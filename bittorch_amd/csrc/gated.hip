@@ -58,8 +58,8 @@ __device__ __forceinline__ u32x4 codes16(const uint8_t* row, int64_t n, int64_t 
 
 // the codes at bits 0, 8, 16, 24 as one byte
 __device__ __forceinline__ uint32_t byte_of_codes(uint32_t t) {
-    const uint32_t x = t & 0x03030303u;
-    return (x | x >> 6 | x >> 12 | x >> 18) & 0xffu;
+    const uint32_t x = t & 0x03030303u, y = x | x >> 6;
+    return (y | y >> 12) & 0xffu;
 }
 
 // From packed bytes.  Bound by them, read once for each copy and written once; all parts in one launch.
@@ -157,8 +157,8 @@ constexpr int master_storage(int dt) { return dt == BT_F32_AS_F16 ? BT_F32 : dt;
 
 // The same from the masters in one pass: a workgroup takes the 16 features of a tile of the copies.  A wave keeps a feature's row in
 // registers (ITERS pieces of eight values a lane, K <= 512 ITERS), reduces its absolute maximum, and puts the codes of four k to a byte into
-// LDS, from where they leave in each layout: the pairs' tile is one run of memory, its dwords are LDS's; a thread turns the codes of 16 k
-// into 64 bytes of the transpose.  The quantizer's arithmetic is that of quantize_pack.hip, on the same values.  Bound by the masters,
+// LDS, from where they leave in each layout: the pairs' tile is one run of memory, its dwords are LDS's; a thread turns the codes of four
+// k into 16 bytes of the transpose.  The quantizer's arithmetic is that of quantize_pack.hip, on the same values.  Bound by the masters,
 // read once: 2 x 6912 x 2560 bf16 (71 MB) takes 18 us, two passes of the quantizer and the copy of their bytes 34.
 template <int DT, int ITERS, bool RAG>
 __global__ __launch_bounds__(512) void gated_quantize_kernel(GatedQuantizeParams p) {
@@ -236,43 +236,44 @@ __global__ __launch_bounds__(512) void gated_quantize_kernel(GatedQuantizeParams
     }
     if (!p.back && !p.rows) return;
     const uint32_t n0 = (uint32_t)(half * p.Fv + f0);
-    for (int kt = tid; 16 * kt < K; kt += 512) {
-        uint32_t t[4][4];  // [features 4 r .. + 3][byte 4 kt + q]
+    for (int kb = tid; 4 * kb < K; kb += 512) {  // (the four threads of 16 k read the same dwords)
+        uint32_t t[4];  // the bytes kb of features 4 r .. + 3
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             uint32_t d[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) d[i] = *(const uint32_t*)(codes + (4 * r + i) * PITCH + 4 * kt);
-            transpose4x4_bytes(d[0], d[1], d[2], d[3], t[r]);
+            for (int i = 0; i < 4; i++) d[i] = *(const uint32_t*)(codes + (4 * r + i) * PITCH + (kb & ~3)) >> (8 * (kb & 3)) & 0xffu;
+            t[r] = d[0] | d[1] << 8 | d[2] << 16 | d[3] << 24;
         }
         if (p.back) {
-            uint4* const out = (uint4*)p.back + ((int64_t)kt * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3);
+            uint4* const out = (uint4*)p.back + ((int64_t)(kb >> 2) * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3) + (kb & 3);
+            uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                uint32_t o[4] = {0u, 0u, 0u, 0u};
+            for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) o[c] |= byte_of_codes(t[r][q] >> (2 * c)) << (8 * r);
-                out[q] = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-            // (the copy's last step holds features past both halves: zeros, from the workgroup of the last tile)
-            if (lin == p.tiles - 1)
-                for (uint32_t g = (n0 >> 4) + 1; g < 4 * p.back_steps; g++)
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        ((uint4*)p.back)[((int64_t)kt * p.back_steps + (g >> 2)) * 16 + 4 * (g & 3) + q] = make_uint4(0u, 0u, 0u, 0u);
+                for (int c = 0; c < 4; c++) o[c] |= byte_of_codes(t[r] >> (2 * c)) << (8 * r);
+            *out = make_uint4(o[0], o[1], o[2], o[3]);
         } else {
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (16 * kt + 4 * q >= K) break;
-                uint8_t* dst = p.rows + (int64_t)(4 * kt + q) * 2 * p.F + half * p.F + f0;
-                const u32x4 v = {t[0][q], t[1][q], t[2][q], t[3][q]};
-                if (f0 + 16 <= p.F) *(u32x4_a1*)dst = v;
-                else
-                    for (int e = 0; f0 + e < p.F; e++) dst[e] = (uint8_t)(v[e >> 2] >> (8 * (e & 3)));
-            }
+            uint8_t* dst = p.rows + (int64_t)kb * 2 * p.F + half * p.F + f0;
+            const u32x4 v = {t[0], t[1], t[2], t[3]};
+            if (f0 + 16 <= p.F) *(u32x4_a1*)dst = v;
+            else
+                for (int e = 0; f0 + e < p.F; e++) dst[e] = (uint8_t)(v[e >> 2] >> (8 * (e & 3)));
         }
+    }
+    // the features of the transpose's last step past both halves, from the workgroup of the last tile
+    if (p.back && lin == p.tiles - 1) {
+        const int kbs = (K + 15) / 16 * 4;
+        const uint32_t first = (n0 >> 4) + 1, groups = 4 * p.back_steps - first;
+        for (uint32_t i = tid; i < kbs * groups; i += 512) {
+            const uint32_t kb = i % kbs, g = first + i / kbs;
+            ((uint4*)p.back)[((int64_t)(kb >> 2) * p.back_steps + (g >> 2)) * 16 + 4 * (g & 3) + (kb & 3)] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    if (p.back) {  // bytes of the last column tile behind K
+        const int kbs = (K + 15) / 16 * 4, kb = (K + 3) / 4 + tid;
+        if (kb < kbs)
+            ((uint4*)p.back)[((int64_t)(kb >> 2) * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3) + (kb & 3)] = make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
