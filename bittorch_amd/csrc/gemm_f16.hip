@@ -576,6 +576,25 @@ bool gemm_f16_supported(int64_t N, int64_t K, const void* X, const void* W_T, co
 // the other tiles' waves for company (1000 x 13824 x 2560 66.9 / 81.2).
 static bool f16_splits_k(int64_t stages) { return stages >= 24; }
 
+// The last, partly filled round of 128-row tiles: an XCD's tiles from `from` on are cut into `parts` finer ones.  Up to half of the
+// slots (two to a compute unit): gemm_dma_parts.  More than one tile a compute unit and up to one and a half: one whole tile each, the
+// others in quarters or halves beside it, so that every compute unit has the same.  us, tiled bf16, tiles of 64 rows throughout / this:
+// 4096 x 2560 x 13824 232 / 204, 4096 x 2560 x 6912 116 / 99, 3000 x 4096 x 11008 194 / 174, 2600 x 4096 x 4096 71 / 64, 1200 x 8192 x
+// 8192 134 / 113; cut so from more on, it is the slower one (1000 x 13824 x 2560, 22 of 32 quartered, 54 / 62).
+struct F16Tail {
+    int parts;
+    int64_t from;   // of an XCD's tiles
+    double rounds;  // price in tiles a compute unit
+};
+static F16Tail f16_tail(int64_t tiles) {
+    const int64_t per_xcd = ceil_div(tiles, 8), cus = gemm_compute_units() / 8, rem = per_xcd % (2 * cus), more = rem - cus;
+    const int parts = gemm_dma_parts(tiles);
+    const double rounds = 2.0 * (double)(per_xcd / (2 * cus));
+    if (parts > 1) return {parts, per_xcd - rem, rounds + (parts == 2 ? 1.2 : 0.6)};
+    if (more > 0 && 2 * more <= cus && !gemm_whole_tiles()) return {4 * more <= cus ? 4 : 2, per_xcd - more, rounds + (4 * more <= cus ? 1.3 : 1.6)};
+    return {1, per_xcd, (double)ceil_div(tiles, gemm_compute_units())};
+}
+
 // Rows of the tiles in units of 16, and what the launch takes in microseconds.  Up to one tile of 32, then of 48 (where two groups of
 // waves share it), then of 64 rows for each compute unit the launch is one tile deep; beyond that a compute unit's run of tiles is priced.  Measured (tiles of 128 / 64 /
 // 32 rows, us, row-major weights): M = 512, 1024, 1536, 2048, 3072, 4096 with N = K = 4096 30 / 30 / 25, 33 / 31 / 40,
@@ -594,9 +613,8 @@ static int gemm_f16_plan(int64_t M, int64_t N, int64_t K, double* us) {
     const int parts = gemm_dma_parts(t4);
     const double n4 = parts == 1 ? (double)ceil_div(t4, C) : (double)(2 * (t4 / (2 * C))) + (parts == 2 ? 1.2 : 0.6);
     const double p4 = n4 * (2.0 + 0.0113 * (double)K), p2 = (double)ceil_div(t2, C) * (1.3 + 0.0062 * (double)K);
-    const bool half = p2 < p4 && !whole;
-    *us = 4.0 + (half ? p2 : p4);
-    return half ? 4 : 8;
+    *us = 4.0 + (p2 < p4 && !whole ? p2 : p4);  // (what the other kernels' prices were fitted against)
+    return p2 < f16_tail(t4).rounds * (2.0 + 0.0113 * (double)K) && !whole ? 4 : 8;
 }
 double gemm_f16_cost(int64_t M, int64_t N, int64_t K) {
     double us;
@@ -618,12 +636,11 @@ static int launch_gemm_f16_cfg(GemmFParams p, hipStream_t st) {
     p.fine_from = p.per_xcd;
     const dim3 block(256);
     if constexpr (NR == 8) {
-        const int parts = gemm_dma_parts(total);
-        if (parts > 1) {
-            const int rem = p.per_xcd % (int)(2 * gemm_compute_units() / 8);
-            p.fine_from = p.per_xcd - rem;
-            const dim3 grid((unsigned)(8 * (p.fine_from + parts * rem)));
-            if (parts == 2) hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, 8, 4, 1, TAIL, RN, OUT>), grid, block, 0, st, p);
+        const F16Tail tail = f16_tail(total);
+        if (tail.parts > 1) {
+            p.fine_from = (int)tail.from;
+            const dim3 grid((unsigned)(8 * (p.fine_from + tail.parts * (p.per_xcd - p.fine_from))));
+            if (tail.parts == 2) hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, 8, 4, 1, TAIL, RN, OUT>), grid, block, 0, st, p);
             else hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, 8, 2, 1, TAIL, RN, OUT>), grid, block, 0, st, p);
             return check_launch(who);
         }
