@@ -853,26 +853,52 @@ def add_rmsnorm_backward(s: Tensor, rstd: Tensor, weight: Optional[Tensor], d_su
     return (dr if one and want_x else dx), (dr if want_residual else None), dw
 
 
+def _gated_operands(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor], up_bias: Optional[Tensor], as_half: bool):
+    """The checked masters and biases as the kernels read them: ``(masters, their tag, biases, their tag)``."""
+    _check(gate.dim() == 2 and gate.shape == up.shape and gate.dtype == up.dtype, "gate and up weights must match, 2D [F, K]")
+    _check(gate.numel() > 0, "weight is empty")
+    _check(not as_half or gate.dtype == torch.float32, "as_half takes fp32 weights")
+    biases = [None if b is None else b.detach() for b in (gate_bias, up_bias)]
+    given = [b for b in biases if b is not None]
+    for b in given:
+        _check(b.dim() == 1 and b.shape[0] == gate.shape[0], "bias shape mismatch")
+    _check(_all_cuda(gate, up, *biases), "All tensors must be CUDA")
+    b_dtype = given[0].dtype if given and given[0].dtype in _DT and all(b.dtype == given[0].dtype for b in given) else torch.float32
+    return ([t.detach().contiguous() for t in (gate, up)], _F32_AS_F16 if as_half else _dt(gate, "weight"),
+            [None if b is None else b.to(b_dtype).contiguous() for b in biases], _DT[b_dtype])
+
+
+def gated_masters_forward(X: Tensor, gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, up_bias: Optional[Tensor] = None,
+                          threshold_factor: float = 0.05, as_half: bool = False) -> Tensor:
+    """``silu(gate) * up`` ``[1, F]`` of one row ``[1, K]`` (:func:`gated_masters_serves`) straight from the masters ``[F, K]``, each
+    quantized per feature as it is read."""
+    _check(X.dim() == 2 and X.shape[0] == 1 and X.numel() > 0 and X.dtype in _DT, "X must be one row, float32, float16 or bfloat16")
+    masters, wdt, biases, bdt = _gated_operands(gate, up, gate_bias, up_bias, as_half)
+    F, K = gate.shape
+    _check(K == X.shape[1], "input K doesn't match weight K")
+    _check(X.device == gate.device, "All tensors must be CUDA")
+    X = X.contiguous()
+    h = torch.empty((1, F), dtype=X.dtype, device=X.device)
+    with _on(X):
+        _status(_L.bt_gated_masters_forward(X.data_ptr(), _DT[X.dtype], masters[0].data_ptr(), masters[1].data_ptr(), wdt, float(threshold_factor),
+                                            _ptr(biases[0]), _ptr(biases[1]), bdt, h.data_ptr(), F, K, _stream(X)))
+    return h
+
+
+def gated_masters_serves(rows: int, masters: Tensor, per_channel: bool = True, as_half: bool = False) -> bool:
+    """Whether :func:`gated_masters_forward` takes a call of so many rows on such masters."""
+    wdt = _F32_AS_F16 if as_half else _dt(masters, "weight")
+    return bool(_L.bt_gated_masters_serves(rows, masters.shape[1], wdt, int(bool(per_channel))))
+
+
 def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, up_bias: Optional[Tensor] = None,
                   threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, rows: bool = False, back: bool = False):
     """The operands of the gated pair, of two masters ``[F, K]`` quantized as :func:`ternary_quantize_pack` does: ``(W_pairs, W_back,
     scale, bias)`` as ``bt_gated_quantize`` makes them; ``rows``: ``W_rows [ceil(K/4), 2 F]`` in the first place; ``back``: with the copy
     for the input's gradient (otherwise None)."""
-    _check(gate.dim() == 2 and gate.shape == up.shape and gate.dtype == up.dtype, "gate and up weights must match, 2D [F, K]")
-    _check(gate.numel() > 0, "weight is empty")
-    _check(not as_half or gate.dtype == torch.float32, "as_half takes fp32 weights")
-    F, K = gate.shape
-    for b in (gate_bias, up_bias):
-        _check(b is None or (b.dim() == 1 and b.shape[0] == F), "bias shape mismatch")
-    _check(_all_cuda(gate, up, gate_bias, up_bias), "All tensors must be CUDA")
-    dev, Kb = gate.device, (K + 3) // 4
-    wdt = _F32_AS_F16 if as_half else _dt(gate, "weight")
-    masters = [t.detach().contiguous() for t in (gate, up)]
-    biases = [None if b is None else b.detach() for b in (gate_bias, up_bias)]
-    if any(b is not None for b in biases):
-        bdt = next(b.dtype for b in biases if b is not None)
-        bdt = bdt if bdt in _DT and all(b is None or b.dtype == bdt for b in biases) else torch.float32
-        biases = [None if b is None else b.to(bdt).contiguous() for b in biases]
+    masters, wdt, biases, bdt = _gated_operands(gate, up, gate_bias, up_bias, as_half)
+    (F, K), dev = gate.shape, gate.device
+    Kb = (K + 3) // 4
     Fv = F if rows else (F + 15) // 16 * 16
     w = torch.empty((Kb, 2 * F) if rows else (_L.bt_tiled_weights_bytes(2 * Fv, K),), dtype=torch.uint8, device=dev)
     w_back = torch.empty((_L.bt_tiled_weights_bytes(K, 2 * Fv),), dtype=torch.uint8, device=dev) if back and not rows else None
@@ -882,7 +908,7 @@ def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, 
     with _on(gate):
         ws = _workspace(_L.bt_gated_quantize_workspace_bytes(F, K, int(bool(per_channel))), dev)
         _status(_L.bt_gated_quantize(masters[0].data_ptr(), masters[1].data_ptr(), wdt, F, K, float(threshold_factor), int(bool(per_channel)),
-                                     _ptr(biases[0]), _ptr(biases[1]), _DT[bdt] if has_bias else 0, None if rows else w.data_ptr(), _ptr(w_back),
+                                     _ptr(biases[0]), _ptr(biases[1]), bdt, None if rows else w.data_ptr(), _ptr(w_back),
                                      w.data_ptr() if rows else None, scale.data_ptr(), _ptr(bias), _ptr(ws), 0 if ws is None else ws.numel(),
                                      _stream(gate)))
     return w, w_back, scale, bias

@@ -229,6 +229,18 @@ static void launch_add_rmsnorm_dt(const AddNormParams& p, int64_t B, hipStream_t
         hipLaunchKernelGGL((add_rmsnorm_any_kernel<DT, RT>), dim3((unsigned)B), dim3(256), 0, st, p);
         return;
     }
+    // A wave to a row where there are rows for all of them and it holds the row in few registers; a workgroup's barriers and idle lanes
+    // cost the short rows most.  us, a workgroup / a wave to a row, bf16: 65536 x 256 89.4 / 32.7, 16384 x 768 27.4 / 17.3 (with int8 36.5 /
+    // 19.3), 8192 x 1024 15.5 / 12.0, 4096 x 2560 19.2 / 17.0 (20.7 / 17.7); an fp32 stream 8192 x 1536 29.1 / 30.4, 4096 x 2560 25.4 / 25.8.
+    if (B >= 1024 && p.K <= (RT == BT_F32 ? 1024 : 2560)) {
+        if (p.K <= 512) launch_add_rmsnorm_cfg<DT, RT, 1, 1>(p, B, st);
+        else if (p.K <= 1024) launch_add_rmsnorm_cfg<DT, RT, 2, 1>(p, B, st);
+        else if constexpr (RT != BT_F32) {
+            if (p.K <= 1536) launch_add_rmsnorm_cfg<DT, RT, 3, 1>(p, B, st);
+            else launch_add_rmsnorm_cfg<DT, RT, 5, 1>(p, B, st);
+        }
+        return;
+    }
     if (p.K <= 2048) launch_add_rmsnorm_cfg<DT, RT, 1, 4>(p, B, st);
     else if (p.K <= 4096) launch_add_rmsnorm_cfg<DT, RT, 2, 4>(p, B, st);
     else if (p.K <= 8192) launch_add_rmsnorm_cfg<DT, RT, 4, 4>(p, B, st);
@@ -275,20 +287,40 @@ __global__ __launch_bounds__(512) void add_rmsnorm_grad_kernel(AddNormGradParams
     const float inv_k = 1.0f / (float)K;
     const bool has_g = p.dS != nullptr;
     const void* const dS = has_g ? p.dS : p.S;  // (without it the loads read the sum once more and their values are not used)
+    struct Row {
+        Raw8<RT> s[ITERS], g[ITERS];
+        Raw8<DT> dy[ITERS];
+        float r;
+    };
+    auto load = [&](int64_t row, Row& to) {
+        row = row < p.B ? row : p.B - 1;
+        to.r = p.rstd[row];
+#pragma unroll
+        for (int i = 0; i < ITERS; i++) to.s[i] = load_raw8<RT>(p.S, row * K + piece_at(at(i), K));
+#pragma unroll
+        for (int i = 0; i < ITERS; i++) to.dy[i] = load_raw8<DT>(p.dY, row * K + piece_at(at(i), K));
+#pragma unroll
+        for (int i = 0; i < ITERS; i++) to.g[i] = load_raw8<RT>(dS, row * K + piece_at(at(i), K));
+    };
+    constexpr bool AHEAD = ITERS < 4 || RT != BT_F32;  // (registers for a second row)
     int turn = 0;
-    for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < p.B; row0 += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
+    Row next;
+    if constexpr (AHEAD) load((int64_t)blockIdx.x * GROUPS + group, next);
+    for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < p.B; row0 += step, turn ^= 1) {
         // (every group passes the barriers; one past the last row computes that row again and stores nothing)
         const bool ok = row0 + group < p.B;
         const int64_t row = ok ? row0 + group : p.B - 1;
-        Raw8<RT> s_in[ITERS], g_in[ITERS];
-        Raw8<DT> dy_in[ITERS];
-        const float r = p.rstd[row];
-#pragma unroll
-        for (int i = 0; i < ITERS; i++) s_in[i] = load_raw8<RT>(p.S, row * K + piece_at(at(i), K));
-#pragma unroll
-        for (int i = 0; i < ITERS; i++) dy_in[i] = load_raw8<DT>(p.dY, row * K + piece_at(at(i), K));
-#pragma unroll
-        for (int i = 0; i < ITERS; i++) g_in[i] = load_raw8<RT>(dS, row * K + piece_at(at(i), K));
+        Row now;
+        if constexpr (AHEAD) {
+            now = next;
+            load(row0 + step + group, next);  // in flight while this row is worked on (4096 x 2560 bf16: 21.9 -> 19.9 us)
+        } else {
+            load(row, now);
+        }
+        const Raw8<RT> (&s_in)[ITERS] = now.s, (&g_in)[ITERS] = now.g;
+        const Raw8<DT> (&dy_in)[ITERS] = now.dy;
+        const float r = now.r;
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < ITERS; i++) {

@@ -42,7 +42,7 @@ namespace {
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
     X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
     X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_ternary_gated_forward) X(bt_gated_grad)                \
-    X(bt_gated_grad_workspace_bytes)
+    X(bt_gated_grad_workspace_bytes) X(bt_gated_masters_serves) X(bt_gated_masters_forward)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     BT_FUNCTIONS(X)
@@ -704,6 +704,12 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
     void* st = stream_of(x.get_device());
     GatedOut o;
     o.rows = x;
+    if (!keep && lib.bt_gated_masters_serves(B, K, tag(gate.scalar_type()), per_channel ? 1 : 0)) {
+        o.h = output(with_last(x, F), x.scalar_type(), x);
+        call(lib.bt_gated_masters_forward, x.const_data_ptr(), dt, gate.const_data_ptr(), up.const_data_ptr(), tag(gate.scalar_type()), threshold,
+             data_of(gate_bias), data_of(up_bias), gate_bias ? tag_of(gate_bias) : tag_of(up_bias), o.h.data_ptr(), F, K, st);
+        return o;
+    }
     const at::Tensor w = fp32 ? output({Kb, 2 * F}, at::kByte, x) : output({(int64_t)lib.bt_tiled_weights_bytes(2 * Fv, K)}, at::kByte, x);
     if (fp32) o.w_back = w;
     else if (want_back) o.w_back = output({(int64_t)lib.bt_tiled_weights_bytes(K, 2 * Fv)}, at::kByte, x);

@@ -292,6 +292,120 @@ static void launch_gated_quantize(const GatedQuantizeParams& p, hipStream_t st) 
 // Rows that a wave holds, with a scale each; the others are quantized by bt_quantize_pack and their bytes put in place
 static bool gated_quantizes(int64_t K, bool per_channel) { return per_channel && K >= 8 && K <= 8192; }
 
+// ---- one row on the masters, without a copy of them -------------------------------------------------------------------------
+
+struct GatedMastersParams {
+    const void* W[2];         // masters gate, up [F, K]
+    const void* b[2];
+    const void* X;            // [K]
+    void* H;                  // [F]
+    int bias_dtype, x_dtype;
+    float tf, clamp_min;
+    int F, K;
+};
+
+template <int XT, bool RAG, int ITERS>
+__device__ __forceinline__ void load_row(const void* X, int lane, int K, float (&x)[ITERS][8]) {
+    Raw8<XT> in[ITERS];
+#pragma unroll
+    for (int i = 0; i < ITERS; i++) in[i] = load_raw8<XT>(X, piece_at((i * 64 + lane) * 8, K));
+#pragma unroll
+    for (int i = 0; i < ITERS; i++) widen_piece<XT, RAG>(in[i], (i * 64 + lane) * 8, K, x[i]);
+}
+
+// Forward alone: the masters are read once, ternarised in registers and multiplied there.  A wave takes one feature at a time, the gate's
+// row and up's (as gated_quantize_kernel holds them), the next one's on their way; a lane's columns are the same for every feature, so
+// the activations stay in its registers.  A product is the activation or its negative or nothing, a sum 8 ITERS terms in a lane and a tree
+// over the lanes, in fp32.  Bound by the masters' bytes, and by whole features for the waves of the chip: 2 x 6912 x 2560 bf16 (71 MB), 3.4
+// features a wave, 18.7 us, 34 through the copies and the tiled product; 2 x 11008 x 4096 bf16 43 and 63, fp32 masters of 2 x 6912 x 2560
+// 31 and 45.  (More rows share the masters' pass there: 34 us up to 32 of them.)
+template <int DT, int ITERS, bool RAG>
+__global__ __launch_bounds__(512) void gated_masters_kernel(GatedMastersParams p) {
+    constexpr int ST = master_storage(DT);
+    constexpr bool AHEAD = ITERS * (ST == BT_F32 ? 2 : 1) <= 10;  // (registers for a second pair of rows)
+    const int lane = threadIdx.x & 63, first = (int)blockIdx.x * 8 + (int)(threadIdx.x >> 6), step = (int)gridDim.x * 8;
+    const int K = p.K, F = p.F;
+    struct Rows {
+        Raw8<ST> d[2][ITERS];
+    };
+    auto load = [&](int f, Rows& to) {
+        const int64_t row = (int64_t)(f < F ? f : F - 1) * K;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < ITERS; i++) to.d[h][i] = load_raw8<ST>(p.W[h], row + piece_at((i * 64 + lane) * 8, K));
+    };
+    Rows in, next;
+    load(first, AHEAD ? next : in);
+    float x[ITERS][8];
+    if (p.x_dtype == BT_F32) load_row<BT_F32, RAG>(p.X, lane, K, x);
+    else if (p.x_dtype == BT_F16) load_row<BT_F16, RAG>(p.X, lane, K, x);
+    else load_row<BT_BF16, RAG>(p.X, lane, K, x);
+    for (int f = first; f < F; f += step) {
+        if constexpr (AHEAD) {
+            in = next;
+            load(f + step, next);
+        }
+        auto values = [&](int h, int i, float (&v)[8]) {
+            widen_piece<ST, RAG>(in.d[h][i], (i * 64 + lane) * 8, K, v);
+            if constexpr (DT == BT_F32_AS_F16) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = round_to_dtype(v[e], BT_F16);
+            }
+        };
+        float y[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float amax = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ITERS; i++) {
+                float v[8];
+                values(h, i, v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(v[e]));
+            }
+            const float s = fmaxf(wave_max(amax), p.clamp_min);
+            const float thr = round_to_dtype(__fmul_rn(p.tf, s), DT == BT_F32_AS_F16 ? BT_F16 : DT);
+            // (widened again, not kept in fp32 from above: half the registers)
+#pragma unroll
+            for (int i = 0; i < ITERS; i++)
+#pragma unroll
+                for (int q = 0; q < (ST == BT_F32 ? 2 : 1); q++) asm volatile("" : "+v"(in.d[h][i].d[q]));
+#pragma unroll
+            for (int i = 0; i < ITERS; i++) {
+                float v[8];
+                values(h, i, v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum = __builtin_fmaf(x[i][e], fabsf(v[e]) > thr ? copysignf(1.0f, v[e]) : 0.0f, sum);
+            }
+            y[h] = epi_float(wave_sum_f32(sum), s, p.b[h] ? load_elem_rt(p.b[h], p.bias_dtype, f) : 0.0f);
+        }
+        if constexpr (!AHEAD) load(f + step, in);
+        if (lane == 0) {
+            if (p.x_dtype == BT_F32) store_elem<BT_F32>(p.H, f, __fdiv_rn(y[0], __fadd_rn(1.0f, exp_fixed(-y[0]))) * y[1]);
+            else if (p.x_dtype == BT_F16) store_elem<BT_F16>(p.H, f, y[0] * sigmoid_fast(y[0]) * y[1]);
+            else store_elem<BT_BF16>(p.H, f, y[0] * sigmoid_fast(y[0]) * y[1]);
+        }
+    }
+}
+
+template <int DT, int ITERS>
+static void launch_gated_masters_cfg(const GatedMastersParams& p, hipStream_t st, dim3 grid) {
+    if (p.K % 8 == 0) hipLaunchKernelGGL((gated_masters_kernel<DT, ITERS, false>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((gated_masters_kernel<DT, ITERS, true>), grid, dim3(512), 0, st, p);
+}
+template <int DT>
+static void launch_gated_masters(const GatedMastersParams& p, hipStream_t st) {
+    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(p.F, 8), gemm_compute_units()));
+    if (p.K <= 1024) launch_gated_masters_cfg<DT, 2>(p, st, grid);
+    else if (p.K <= 2560) launch_gated_masters_cfg<DT, 5>(p, st, grid);
+    else if constexpr (master_storage(DT) != BT_F32) hipLaunchKernelGGL((gated_masters_kernel<DT, 8, false>), grid, dim3(512), 0, st, p);
+}
+// Rows of masters that a wave holds twice beside the activations, with a scale each
+static bool masters_serve(int64_t B, int64_t K, int w_dtype, bool per_channel) {
+    return per_channel && B == 1 && K >= 8 && (K <= 2560 || (K <= 4096 && K % 8 == 0 && (w_dtype == BT_F16 || w_dtype == BT_BF16)));
+}
+
 // ---- gradient of silu(g) u ------------------------------------------------------------------------------------------------
 
 struct GatedGradParams {
@@ -497,6 +611,36 @@ extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padd
     epi.scale = scale; epi.scale_dtype = BT_F32;
     epi.bias = bias; epi.bias_dtype = BT_F32;
     return launch_gemm_f16_gated(x_dtype == BT_F16 ? MODE_F16 : MODE_BF16, rows, W_pairs, epi, H, pre, F, B, 2 * Fp, Kr, (hipStream_t)stream);
+}
+
+extern "C" int bt_gated_masters_serves(int64_t B, int64_t K, int w_dtype, int per_channel) { return masters_serve(B, K, w_dtype, per_channel != 0); }
+
+extern "C" int bt_gated_masters_forward(const void* X, int x_dtype, const void* gate, const void* up, int w_dtype, double threshold_factor,
+                                        const void* gate_bias, const void* up_bias, int bias_dtype, void* H, int64_t F, int64_t K, void* stream) {
+    const char* who = "bt_gated_masters_forward";
+    if (!X || !gate || !up || !H || F <= 0 || K <= 0 || (x_dtype != BT_F32 && x_dtype != BT_F16 && x_dtype != BT_BF16)) {
+        set_error("%s: null pointer, empty shape or bad dtype", who);
+        return BT_ERR_INVALID;
+    }
+    if ((w_dtype != BT_F32 && w_dtype != BT_F16 && w_dtype != BT_BF16 && w_dtype != BT_F32_AS_F16) ||
+        ((gate_bias || up_bias) && bias_dtype != BT_F32 && bias_dtype != BT_F16 && bias_dtype != BT_BF16)) {
+        set_error("%s: unsupported weight or bias dtype", who);
+        return BT_ERR_INVALID;
+    }
+    if (!masters_serve(1, K, w_dtype, true) || F >= (1ll << 23)) {
+        set_error("%s: a row that bt_gated_masters_serves takes, F below 2^23 (F=%lld, K=%lld)", who, (long long)F, (long long)K);
+        return BT_ERR_INVALID;
+    }
+    GatedMastersParams p = {};
+    p.W[0] = gate; p.W[1] = up; p.b[0] = gate_bias; p.b[1] = up_bias; p.bias_dtype = bias_dtype; p.X = X; p.x_dtype = x_dtype; p.H = H;
+    p.tf = (float)threshold_factor; p.clamp_min = quantize_clamp_min(w_dtype);
+    p.F = (int)F; p.K = (int)K;
+    hipStream_t st = (hipStream_t)stream;
+    if (w_dtype == BT_F32) launch_gated_masters<BT_F32>(p, st);
+    else if (w_dtype == BT_F16) launch_gated_masters<BT_F16>(p, st);
+    else if (w_dtype == BT_BF16) launch_gated_masters<BT_BF16>(p, st);
+    else launch_gated_masters<BT_F32_AS_F16>(p, st);
+    return check_launch(who);
 }
 
 extern "C" size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F) {

@@ -42,9 +42,12 @@ class _GatedLinear(torch.autograd.Function):
 
         f, k = gate.shape
         rows = x.dtype == torch.float32
+        x2 = x.reshape(-1, k)
+        if not keep and _C.gated_masters_serves(x2.shape[0], gate, per_channel, as_half):
+            h = _C.gated_masters_forward(x2, gate, up, gate_bias, up_bias, threshold_factor, as_half)
+            return h.reshape(*x.shape[:-1], f)
         w, w_back, scale, bias = _C.gated_weights(gate, up, gate_bias, up_bias, threshold_factor, per_channel, as_half, rows,
                                                   back=keep and ctx.needs_input_grad[0])
-        x2 = x.reshape(-1, k)
         if rows:
             # (the fp32 gradient kernels take four columns and more)
             x2 = F.pad(x2, (0, 4 - k)) if k < 4 else x2.contiguous()

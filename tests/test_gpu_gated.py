@@ -89,7 +89,11 @@ def test_forward_and_gradient(rows, k, f, dt):
     assert h.shape == (rows, f) and h.dtype == dt
     _assert_within(h.detach(), ref.h, ref.tol_h, "h")
     with torch.no_grad():
-        assert torch.equal(_gated(*leaves), h)
+        alone = _gated(*leaves)
+        if rows > 1:
+            assert torch.equal(alone, h)
+        else:  # straight from the masters: other sums, the same bound
+            _assert_within(alone, ref.h, ref.tol_h, "h without a gradient")
     dx, dwg, dwu, dbg, dbu = torch.autograd.grad(h, leaves, dh, retain_graph=True)
     again = torch.autograd.grad(h, leaves, dh)
     assert all(torch.equal(a, b) and a.is_contiguous() for a, b in zip(again, (dx, dwg, dwu, dbg, dbu)))
@@ -115,6 +119,28 @@ def test_forward_and_gradient(rows, k, f, dt):
             assert _norm_error(got, want_w) <= 1.42 * half
     if dt != torch.float32 and rows * k >= 64:
         assert _norm_error(dx, want) <= 1.42 * half and _norm_error(h.detach(), ref.h) <= 1.01 * half
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,wt", [(d, d) for d in DTYPES] + [(torch.bfloat16, torch.float32), (torch.float32, torch.float16)])
+@pytest.mark.parametrize("rows,k,f", [(1, 8, 1), (1, 15, 3), (1, 1024, 9), (1, 1025, 40), (1, 2560, 16), (1, 2559, 70), (1, 2561, 33), (1, 4096, 33),
+                                      (1, 4097, 16), (2, 64, 16), (1, 7, 16), (1, 1000, 20000)])
+def test_one_row_without_a_gradient(rows, k, f, dt, wt):
+    """The row that is multiplied as the masters are read, and the calls next to it that are not."""
+    announce("gated masters", rows, k, f, dt, wt)
+    from bittorch_amd import _C
+    for bias in (True, False):
+        x, wg, wu, bg, bu, dh = _inputs(rows, k, f, dt, wt, bias, seed=11)
+        assert _C.gated_masters_serves(rows, wg) == (rows == 1 and k >= 8 and (k <= 2560 or (k <= 4096 and k % 8 == 0 and wt != torch.float32)))
+        assert not _C.gated_masters_serves(rows, wg, False)
+        if f == 1 and dt == torch.float32:
+            continue
+        wg[0] = 0
+        ref = _Reference(x, wg, wu, bg, bu, dh)
+        h = _gated(x, wg, wu, bg, bu)
+        # (a lane adds up to 8 (K / 512 + 1) products one after the other here, then over the lanes: within the bound's 6 K / 32 + 80)
+        _assert_within(h, ref.h, ref.tol_h, "h")
+        assert torch.equal(h, _gated(x, wg, wu, bg, bu))
 
 
 @pytest.mark.gpu
@@ -218,6 +244,8 @@ def test_parts_of_the_call():
         assert torch.equal(grad.reshape(48, 264), want[0])
     one = _gated(x[5], wg, wu, bg, bu)
     assert one.shape == (72,) and torch.equal(one, _gated(x[5:6], wg, wu, bg, bu)[0])
+    odd = torch.zeros(2 * 72 * 264 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(2, 72, 264).copy_(torch.stack((wg, wu)))
+    assert torch.equal(_gated(x[5], odd[0], odd[1], bg, bu), one) and torch.equal(_gated(x, odd[0], odd[1], bg, bu), h)
     out = _gated(*full)
     a = torch.autograd.grad(out, full, dh.t().contiguous().t(), retain_graph=True)
     assert all(torch.equal(p, q) for p, q in zip(a, want))
@@ -423,6 +451,12 @@ def test_refusals():
                    dict(h=at + 4), dict(F=1 << 23), dict(B=1 << 31)):
         assert forward(**kwargs) == -1, kwargs
         assert "bt_ternary_gated_forward" in _lib.last_error()
+    few = lambda X=at, xd=2, g=at, wd=2, b=None, bdt=0, h=at, F=8, K=16: lib.bt_gated_masters_forward(X, xd, g, at, wd, 0.05, b, b, bdt, h, F, K, None)
+    for kwargs in (dict(X=None), dict(xd=3), dict(g=None), dict(wd=3), dict(b=at, bdt=3), dict(h=None), dict(K=4), dict(K=4097), dict(wd=0, K=2568), dict(K=2561), dict(F=0),
+                   dict(F=1 << 23)):
+        assert few(**kwargs) == -1, kwargs
+        assert "bt_gated_masters_forward" in _lib.last_error()
+    assert lib.bt_gated_masters_serves(1, 16, 2, 1) == 1 and lib.bt_gated_masters_serves(0, 16, 2, 1) == 0
     grad = lambda dh=at, dt=2, pre=at, scale=at, G=at, db=None, bdt=0, B=4, F=8, ws=None, n=0: lib.bt_gated_grad(
         dh, dt, pre, scale, G, db, bdt, B, F, ws, n, None)
     for kwargs in (dict(dh=None), dict(pre=None), dict(G=None), dict(scale=None), dict(dt=3), dict(F=0), dict(B=1 << 31), dict(pre=at + 4), dict(G=at + 4),
