@@ -56,6 +56,44 @@ class PackedWeightCache:
         self.key, self.value = None, None
 
 
+def _state(weight: Tensor) -> tuple:
+    return weight._version, weight.data_ptr(), weight.dtype, weight.device
+
+
+class GatedWeightCache:
+    """The packed weights of a gated pair (``_C.gated_weights``: both layers in one tiled copy, tiles of gate and up in turn), kept by the
+    same rules."""
+
+    __slots__ = ("key", "value")
+
+    def __init__(self) -> None:
+        self.key = None
+        self.value = None
+
+    def get(self, gate, up):
+        from .. import _C
+
+        given = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
+        key = (*(_state(t) for t in given), gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel))
+        if key != self.key:
+            with torch.no_grad():
+                w, _, scale, bias = _C.gated_weights(gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)
+            self.key, self.value = key, (w, scale[:-1], bias)
+        return self.value
+
+    def forward(self, x: Tensor, gate, up) -> Tensor:
+        """``silu(gate(x)) * up(x)`` as ``TernarySwiGLU`` computes it."""
+        from .. import _C
+
+        w, scale, bias = self.get(gate, up)
+        f = gate.out_features
+        h = _C.ternary_linear_tiled_forward(x.contiguous(), w, scale, bias, gate.in_features, scale.numel(), swiglu_pairs=True)
+        return h if h.shape[-1] == f else h[..., :f].contiguous()
+
+    def clear(self) -> None:
+        self.key, self.value = None, None
+
+
 def cache_usable(x: Tensor, weight: Tensor) -> bool:
     """The cache holds the quantization of the stored weights in their own dtype.  A training forward
     re-quantizes (see above).  Under autocast the autograd function quantizes an fp16 copy instead

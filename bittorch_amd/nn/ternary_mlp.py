@@ -1,4 +1,6 @@
-"""``TernarySwiGLU``: the block MLP ``down(silu(gate(h)) * up(h))`` over packed ternary weights
+"""``TernaryGatedMLP`` and ``TernarySwiGLU``: the block MLP in training, on full-precision masters, and over packed weights.
+
+``TernarySwiGLU``: the block MLP ``down(silu(gate(h)) * up(h))`` over packed ternary weights
 with the glue fused (no counterpart in ``bittorch.nn``; structure of the reference's JS runtime,
 ``js/src/models/TernaryTransformer.ts:366-423``, and of its pre-norm block, ``:489-521``).
 
@@ -12,10 +14,67 @@ from __future__ import annotations
 
 from typing import Optional
 
+import torch
 import torch.nn as nn
+import torch.nn.functional as F
 from torch import Tensor
 
+from ._packed_cache import GatedWeightCache, cache_usable
+from .ternary_linear import BackendType, TernaryLinear
 from .ternary_linear_infer import TernaryLinearInference
+
+
+class TernaryGatedMLP(nn.Module):
+    """``down(silu(gate(h)) * up(h))`` of three ``TernaryLinear`` layers (``gate``, ``up``, ``down``: the keys of the state dict), for
+    training: on the GPU the gated pair is one operator (``ops.ternary_gated_linear``: both masters ternarised in one pass, one product
+    forward, two backward) and the residual connection and norm in front of it another (``ops.add_rmsnorm``).
+
+    Without a gradient (evaluation) the packed weights are kept until the masters change, as in ``TernaryLinear``, and the values are
+    those of the converted module.  ``to_inference()`` gives that module, a ``TernarySwiGLU``."""
+
+    def __init__(self, d_model: int, ffn: int, bias: bool = False, threshold_factor: float = 0.05, per_channel: bool = True,
+                 backend: BackendType = "auto") -> None:
+        super().__init__()
+        make = lambda i, o: TernaryLinear(i, o, bias=bias, threshold_factor=threshold_factor, per_channel=per_channel, backend=backend)
+        self.gate, self.up, self.down = make(d_model, ffn), make(d_model, ffn), make(ffn, d_model)
+        self._packed = GatedWeightCache()
+
+    def hidden(self, h: Tensor) -> Tensor:
+        """``silu(gate(h)) * up(h)``."""
+        gate, up = self.gate, self.up
+        alike = (type(gate) is TernaryLinear and type(up) is TernaryLinear and gate.quantize and up.quantize
+                 and gate.threshold_factor == up.threshold_factor and gate.per_channel == up.per_channel and h.dtype != torch.float64)
+        if not alike or not gate._should_use_cuda_kernel(h):
+            return F.silu(gate(h)) * up(h)
+        if cache_usable(h, gate.weight) and cache_usable(h, up.weight) and not (torch.is_grad_enabled() and h.requires_grad):
+            return self._packed.forward(h, gate, up)
+        from ..ops.gated import ternary_gated_linear
+        return ternary_gated_linear(h, gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)
+
+    def forward(self, x: Tensor, norm_weight: Optional[Tensor] = None, eps: Optional[float] = None, residual: Optional[Tensor] = None) -> Tensor:
+        """``down(silu(gate(h)) * up(h)) [+ residual]`` with ``h = rmsnorm(x, norm_weight, eps)`` when ``eps`` is given and ``h = x``
+        otherwise (the signature of ``TernarySwiGLU``)."""
+        if eps is not None:
+            if x.is_cuda:
+                from ..ops.fused import add_rmsnorm
+                x = add_rmsnorm(x, None, norm_weight, eps)[1]
+            else:
+                x = F.rms_norm(x, (x.shape[-1],), norm_weight, eps)
+        y = self.down(self.hidden(x))
+        return y if residual is None else y + residual
+
+    def invalidate_packed_cache(self) -> None:
+        """Forget the kept packed weights (needed only after an evaluation-time write through ``weight.data``)."""
+        self._packed.clear()
+        for layer in (self.gate, self.up, self.down):
+            if isinstance(layer, TernaryLinear):
+                layer.invalidate_packed_cache()
+
+    def to_inference(self, compute: str = "float", fuse_gate_up: bool = False) -> "TernarySwiGLU":
+        """The same MLP over packed weights (a copy: the masters stay as they are)."""
+        from ..utils.convert import ternary_linear_to_infer
+        return TernarySwiGLU(*(ternary_linear_to_infer(m) if isinstance(m, TernaryLinear) else m for m in (self.gate, self.up, self.down)),
+                             compute=compute, fuse_gate_up=fuse_gate_up)
 
 
 class TernarySwiGLU(nn.Module):
@@ -93,7 +152,6 @@ class TernarySwiGLU(nn.Module):
         from ..ops import fused
 
         if not x.is_cuda:
-            import torch.nn.functional as F
             h = x if eps is None else F.rms_norm(x, (x.shape[-1],), norm_weight, eps)
             g, u = self._gate_up(h)
             return self.down(F.silu(g) * u, residual)

@@ -92,6 +92,21 @@ class BlockStack:
                 x = blk(x)
             return self.final(x)
 
+    def forward_train(self):
+        """The training modules with the glue between their layers fused, differentiable: the residual connections with the norms behind
+        them (``ops.add_rmsnorm``), gate and up with the SwiGLU between them (``ops.ternary_gated_linear``)."""
+        F, ops = self.F, self.bt.ops
+        eps_of = lambda norm: norm.eps or self.torch.finfo(self.act_dtype).eps
+        x, branch = self.emb(self.tokens), None
+        for blk in self.blocks:
+            x, h = ops.add_rmsnorm(x, None, blk.n1.weight, eps_of(blk.n1)) if branch is None else ops.add_rmsnorm(branch, x, blk.n1.weight, eps_of(blk.n1))
+            b, t, _ = h.shape
+            q, k, v = (m(h).view(b, t, self.heads, -1).transpose(1, 2) for m in (blk.q, blk.k, blk.v))
+            a = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=self.attn_scale).transpose(1, 2).reshape(b, t, -1)
+            x, h = ops.add_rmsnorm(blk.o(a), x, blk.n2.weight, eps_of(blk.n2))
+            branch = blk.down(ops.ternary_gated_linear(h, blk.gate.weight, blk.up.weight))
+        return ops.add_rmsnorm(branch, x, self.final.weight, eps_of(self.final))[1]
+
     def drop_packed_caches(self):
         for m in self.blocks.modules():
             if isinstance(m, self.bt.nn.TernaryLinear):

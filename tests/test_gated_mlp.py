@@ -1,0 +1,176 @@
+"""``nn.TernaryGatedMLP`` and the operators of a pre-norm block's feed-forward half together, as a training program uses them."""
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import bittorch_amd as bt
+from conftest import announce
+
+EPS = 1e-5
+
+
+def _mlp(d, ffn, seed=0, **kwargs):
+    torch.manual_seed(seed)
+    return bt.nn.TernaryGatedMLP(d, ffn, **kwargs)
+
+
+def _norm_error(got, want):
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    return float((got - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_on_the_cpu_it_is_the_three_layers(bias):
+    mlp = _mlp(24, 40, bias=bias)
+    assert sorted(mlp.state_dict()) == sorted(f"{m}.{p}" for m in ("gate", "up", "down") for p in (("weight", "bias") if bias else ("weight",)))
+    x, res = torch.randn(2, 5, 24), torch.randn(2, 5, 24)
+    want = mlp.down(F.silu(mlp.gate(x)) * mlp.up(x))
+    assert torch.equal(mlp(x), want) and torch.equal(mlp(x, residual=res), want + res)
+    w = 1 + 0.1 * torch.randn(24)
+    h = F.rms_norm(x, (24,), w, EPS)
+    assert torch.equal(mlp(x, w, EPS, res), mlp.down(F.silu(mlp.gate(h)) * mlp.up(h)) + res)
+    other = copy.deepcopy(mlp)
+    other.load_state_dict(mlp.state_dict())
+    assert torch.equal(other(x), want)
+    with torch.no_grad():
+        assert torch.allclose(mlp.to_inference()(x), want, rtol=1e-5, atol=1e-6)
+        assert torch.allclose(bt.utils.convert_linear_layers(torch.nn.Sequential(mlp))[0](x), want, rtol=1e-5, atol=1e-6)
+    mlp.gate.quantize = False
+    assert torch.equal(mlp(x), mlp.down(F.silu(F.linear(x, mlp.gate.weight, mlp.gate.bias)) * mlp.up(x)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,ffn,bias", [(96, 160, False), (100, 70, True)])
+def test_training_step_and_evaluation(d, ffn, bias, dt):
+    announce("gated mlp", d, ffn, bias, dt)
+    mlp = _mlp(d, ffn, seed=1, bias=bias).cuda()
+    ref = copy.deepcopy(mlp).double().cpu()
+    g = torch.Generator().manual_seed(2)
+    x, dy = torch.randn(3, 21, d, generator=g).to(dt), torch.randn(3, 21, d, generator=g).to(dt)
+    xc, xr = x.cuda().requires_grad_(), x.double().requires_grad_()
+    y = mlp(xc)
+    y.backward(dy.cuda())
+    want = ref(xr)
+    want.backward(dy.double())
+    # half a step each: h, the down projection's output and, backward, its gradient, G and the products; TernaryLinear rounds its scale too
+    half = torch.finfo(dt).eps / 2
+    tol = 3 * half + 1e-5
+    assert y.dtype == dt and _norm_error(y, want) <= tol
+    assert _norm_error(xc.grad, xr.grad) <= tol
+    for (name, p), q in zip(mlp.named_parameters(), ref.parameters()):
+        assert p.grad.dtype == p.dtype and _norm_error(p.grad, q.grad) <= tol, name
+    with torch.no_grad():
+        kept = mlp(xc)
+        assert _norm_error(kept, want) <= tol + 2 * half  # (the projections rounded, and silu, as the converted module rounds them)
+        assert mlp._packed.key is not None
+        fused = mlp.to_inference(fuse_gate_up=True)
+        assert torch.equal(mlp.hidden(xc), fused.gate_up.forward_swiglu(xc) if ffn % 16 == 0 else bt.ops.swiglu(fused.gate_up(xc)[..., :ffn], fused.gate_up(xc)[..., ffn:]))
+        for p in mlp.parameters():
+            p.mul_(-1.5)
+        assert torch.equal(mlp.hidden(xc), copy.deepcopy(mlp).hidden(xc)) and not torch.equal(mlp(xc), kept)
+        mlp.gate.weight.data.zero_()  # (unseen by the version counter)
+        mlp.invalidate_packed_cache()
+        if not bias:
+            assert not mlp.hidden(xc).any()
+        one = mlp.hidden(xc[0, 0])
+        assert one.shape == (ffn,)
+    frozen = _mlp(d, ffn, seed=1, bias=bias).cuda().requires_grad_(False)
+    z = x.cuda().requires_grad_()
+    frozen(z).backward(dy.cuda())
+    assert _norm_error(z.grad, xr.grad) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,stream", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                       (torch.float16, torch.float32)])
+@pytest.mark.parametrize("rows,d,ffn", [(1, 64, 48), (130, 264, 176), (77, 129, 90)])
+def test_feed_forward_half_of_a_block(rows, d, ffn, dt, stream):
+    """A branch is added to the stream and normed, the gated pair and the down projection follow, and their sum is normed again: forward and
+    every gradient against the same in 64 bits."""
+    announce("block half", rows, d, ffn, dt, stream)
+    g = torch.Generator().manual_seed(rows + d)
+    mk = lambda std, *shape: torch.randn(*shape, generator=g) * std
+    branch, x, ds, dy = mk(1, rows, d).to(dt), mk(2, rows, d).to(stream), mk(1, rows, d).to(stream), mk(1, rows, d).to(dt)
+    n1, n2 = (1 + mk(0.1, d)).to(dt), (1 + mk(0.1, d)).to(dt)
+    mlp = _mlp(d, ffn, seed=3).to(dt)
+    ref = copy.deepcopy(mlp).double()
+    # (a 16-bit master's threshold is rounded to 16 bits: the codes are taken from the masters as they are trained)
+    for layer, trained in ((ref.gate, mlp.gate), (ref.up, mlp.up), (ref.down, mlp.down)):
+        q, s = trained.get_quantized_weight()
+        with torch.no_grad():
+            layer.weight.copy_(q.double() * s.double().reshape(-1, 1))
+    mlp = mlp.cuda()
+    leaves = [t.cuda().requires_grad_() for t in (branch, x, n1, n2)]
+    s1, h = bt.ops.add_rmsnorm(leaves[0], leaves[1], leaves[2], EPS)
+    out = bt.ops.add_rmsnorm(mlp(h), s1, leaves[3], EPS)
+    got = torch.autograd.grad(out, [*leaves, *mlp.parameters()], (ds.cuda(), dy.cuda()))
+
+    refs = [t.double().requires_grad_() for t in (branch, x, n1, n2)]
+    t1 = refs[0] + refs[1]
+    t1 = t1 + (t1.detach().to(stream).double() - t1.detach())  # (the stream as it is stored)
+    hr = F.rms_norm(t1, (d,), refs[2], EPS)
+    t2 = t1 + ref(hr)
+    nr = F.rms_norm(t2, (d,), refs[3], EPS)
+    want = torch.autograd.grad((t2, nr), [*refs, *ref.parameters()], (ds.double(), dy.double()))
+    # forward: at most five roundings to 16 bits one after the other (the sum, the norm, h, the down projection and its scale), backward
+    # five more; independent of each other, so their root of squares and not their sum: sqrt(10) halves of a step
+    tol = 3.2 * torch.finfo(dt).eps / 2 + 1e-5
+    for a, b in zip(out, (t2, nr)):
+        assert _norm_error(a, b) <= tol
+    for a, b in zip(got, want):
+        assert _norm_error(a, b) <= tol
+
+
+@pytest.mark.gpu
+def test_block_stack_training_forward_and_gradient():
+    """Two blocks, fused glue and unfused modules: the same loss and gradients up to fp32's sums."""
+    from bittorch_amd.utils.block_stack import BlockStack
+    std = dict(q=0.02, k=0.02, v=0.02, o=0.01, gate=0.01, up=0.01, down=0.005)
+    stack = BlockStack("cuda", layers=2, d_model=128, heads=4, ffn=208, batch=2, seq=24, vocab=64, act_dtype=torch.float32, master_std=std)
+    params = [*stack.emb.parameters(), *stack.blocks.parameters(), *stack.final.parameters()]
+    dy = torch.randn(2, 24, 128, generator=torch.Generator().manual_seed(1)).cuda()
+    fused = stack.forward_train()
+    got = torch.autograd.grad(fused, params, dy)
+    x = stack.emb(stack.tokens)
+    for blk in stack.blocks:
+        x = blk(x)
+    plain = stack.final(x)
+    want = torch.autograd.grad(plain, params, dy)
+    # fp32 sums of up to 208 terms in another order, through two blocks
+    assert _norm_error(fused, plain) <= 1e-5
+    for a, b in zip(got, want):
+        assert _norm_error(a, b) <= 2e-5
+
+
+@pytest.mark.gpu
+def test_training_step_captured_and_replayed():
+    """A step on fresh leaves in a graph, replayed between eager steps of the same module."""
+    mlp = _mlp(136, 80, seed=4).to(torch.bfloat16).cuda()
+    x, dy = torch.randn(40, 136, device="cuda").bfloat16(), torch.randn(40, 136, device="cuda").bfloat16()
+    n = torch.ones(136, device="cuda", dtype=torch.bfloat16)
+
+    def step(x, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, n, mlp.gate.weight, mlp.up.weight)]
+        s, h = bt.ops.add_rmsnorm(leaves[0], x, leaves[1], EPS)
+        out = bt.ops.ternary_gated_linear(h, *leaves[2:])
+        return (out.detach(), *torch.autograd.grad((s, out), leaves, (dy, out.detach())))
+
+    static = [x.clone(), dy.clone()]
+    expect = [t.clone() for t in step(*static)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for k in range(3):
+        new = x * (k + 1)
+        static[0].copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step(new, dy)))
+    static[0].copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, expect))
