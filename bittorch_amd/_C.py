@@ -917,7 +917,7 @@ def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, 
 def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optional[Tensor], out_features: int,
                           want_pre: bool = False) -> Tuple[Tensor, Optional[Tensor], Tensor]:
     """``silu(gate) * up`` ``[B, F]`` of 16-bit rows ``[B, K]`` on the operands of :func:`gated_weights`; with ``want_pre`` the two
-    projections ``[B, 2 Fp]`` fp32 as :func:`gated_grad` reads them; and the rows as the kernels read them (a padded copy of ``X`` where
+    projections (int32 ``[B, 3 Fp / 2]``, 24 bits each) as :func:`gated_grad` reads them; and the rows as the kernels read them (a padded copy of ``X`` where
     K is no multiple of 8 or it is not 16-byte aligned)."""
     _check(X.dim() == 2 and X.numel() > 0 and X.dtype in (torch.float16, torch.bfloat16), "X must be 2D fp16 or bf16")
     B, K = X.shape
@@ -930,7 +930,7 @@ def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optio
     X, scale, bias = X.contiguous(), scale.contiguous(), None if bias is None else bias.contiguous()
     rows = X if K % 8 == 0 and X.data_ptr() % 16 == 0 else torch.empty((B, (K + 7) // 8 * 8), dtype=X.dtype, device=X.device)
     h = torch.empty((B, F), dtype=X.dtype, device=X.device)
-    pre = torch.empty((B, 2 * Fp), dtype=torch.float32, device=X.device) if want_pre else None
+    pre = torch.empty((B, Fp // 2 * 3), dtype=torch.int32, device=X.device) if want_pre else None
     with _on(X):
         _status(_L.bt_ternary_gated_forward(X.data_ptr(), _DT[X.dtype], None if rows is X else rows.data_ptr(), W_pairs.data_ptr(),
                                             scale.data_ptr(), _ptr(bias), h.data_ptr(), _ptr(pre), B, F, K, _stream(X)))
@@ -939,11 +939,12 @@ def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optio
 
 def gated_grad(dH: Tensor, pre: Tensor, scale: Optional[Tensor], bias_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Optional[Tensor]]:
     """Gradient of ``silu(gate) * up`` in both projections, ``[B, 2 Fp]`` in 16 bits times their scales, or ``[B, 2 F]`` fp32 without
-    (``pre`` then is ``[gate | up]``); with ``bias_dtype`` also its sums over the rows ``[2 F]``, without scales."""
+    (``pre`` then is ``[gate | up]`` in fp32); with ``bias_dtype`` also its sums over the rows ``[2 F]``, without scales."""
     _check(dH.dim() == 2 and dH.numel() > 0 and dH.dtype in _DT, "dH must be 2D float32, float16 or bfloat16")
     B, F = dH.shape
     Fv = F if dH.dtype == torch.float32 else (F + 15) // 16 * 16
-    _check(pre.dtype == torch.float32 and pre.shape == (B, 2 * Fv) and pre.is_contiguous(), "the projections must be fp32 [B, 2 F]")
+    kept = (torch.float32, (B, 2 * F)) if dH.dtype == torch.float32 else (torch.int32, (B, Fv // 2 * 3))
+    _check((pre.dtype, pre.shape) == kept and pre.is_contiguous(), "the projections must be those that the forward kept")
     _check(dH.dtype == torch.float32 or (scale is not None and scale.dtype == torch.float32 and scale.numel() >= 2 * Fv and scale.is_contiguous()),
            "scale must be fp32 with an entry for each padded feature")
     _check(_all_cuda(dH, pre, scale), "All tensors must be CUDA")

@@ -726,7 +726,8 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
              ws.size(), st);
     }
     o.h = output(with_last(x, F), x.scalar_type(), x);
-    if (fp32 || keep) o.pre = output({B, 2 * Fv}, at::kFloat, x);
+    if (fp32) o.pre = output({B, 2 * F}, at::kFloat, x);
+    else if (keep) o.pre = output({B, Fv / 2 * 3}, at::kInt, x);
     if (!fp32) {
         void* padded = nullptr;
         if (K % 8 != 0 || !aligned(x, 16)) {
@@ -734,7 +735,7 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
             padded = o.rows.data_ptr();
         }
         call(lib.bt_ternary_gated_forward, x.const_data_ptr(), dt, padded, (const uint8_t*)w.const_data_ptr(), scale_at, bias_at, o.h.data_ptr(),
-             keep ? (float*)o.pre.data_ptr() : nullptr, B, F, K, st);
+             keep ? o.pre.data_ptr() : nullptr, B, F, K, st);
         return o;
     }
     const Scratch ws(lib.bt_packed_forward_workspace_bytes(B, 2 * F, K, dt), x);
@@ -778,7 +779,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         if (want_b) db = output({2 * F}, b_dtype, x);
         {
             const Scratch ws(want_b ? lib.bt_gated_grad_workspace_bytes(B, F) : 0, x);
-            check_status(lib.bt_gated_grad(dh.const_data_ptr(), dt, (const float*)pre.const_data_ptr(), scale_at, g.data_ptr(), want_b ? db.data_ptr() : nullptr,
+            check_status(lib.bt_gated_grad(dh.const_data_ptr(), dt, pre.const_data_ptr(), scale_at, g.data_ptr(), want_b ? db.data_ptr() : nullptr,
                                            want_b ? tag(b_dtype) : 0, B, F, ws.ptr(), ws.size(), st));
         }
         if (w.want[0]) {

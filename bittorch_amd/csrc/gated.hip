@@ -21,7 +21,7 @@
 
 namespace bt {
 
-int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, float* pre, int64_t H, int64_t M,
+int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, uint32_t* pre, int64_t H, int64_t M,
                           int64_t N, int64_t K, hipStream_t st);
 int launch_pad_rows(const void* X, int64_t B, int64_t K, void* P, hipStream_t st);
 float quantize_clamp_min(int w_dtype);
@@ -286,7 +286,7 @@ static void launch_gated_quantize(const GatedQuantizeParams& p, hipStream_t st) 
         else hipLaunchKernelGGL((gated_quantize_kernel<DT, IT, true>), grid, block, 0, st, p);              \
         return;                                                                                            \
     }
-    BT_GQ(2) BT_GQ(5) BT_GQ(8) BT_GQ(16)
+    BT_GQ(1) BT_GQ(2) BT_GQ(3) BT_GQ(5) BT_GQ(8) BT_GQ(16)
 #undef BT_GQ
 }
 // Rows that a wave holds, with a scale each; the others are quantized by bt_quantize_pack and their bytes put in place
@@ -410,7 +410,7 @@ static bool masters_serve(int64_t B, int64_t K, int w_dtype, bool per_channel) {
 
 struct GatedGradParams {
     const void* dH;       // [B, F]
-    const float* pre;     // 16-bit rows: [B, 2 Fp], column pairs of gate and up in turn; fp32 rows: [B, 2 F], gate | up
+    const void* pre;      // 16-bit rows: [B, 3 Fp / 2] dwords, column pairs of gate and up in turn in 24 bits; fp32 rows: [B, 2 F], gate | up
     const float* scale;   // 16-bit rows: [2 Fp]
     void* G;              // [B, 2 Fp] / [B, 2 F]
     float* parts;         // [gridDim.y, 2 Fp] sums of dg | du, or null
@@ -449,10 +449,13 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
             widen_piece<DT, RAG>(g_in, k, F, g);
             widen_piece<DT, RAG>(u_in, k, F, u);
         } else {
-            const v4f* at = (const v4f*)(p.pre + row * 2 * Fp + 2 * k);
+            const u32x4* at = (const u32x4*)((const uint32_t*)p.pre + (row * Fp + k) / 2 * 3);
+            const u32x4 a = at[0], b = at[1], c = at[2];
+            const uint32_t d[12] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3], c[0], c[1], c[2], c[3]};
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const v4f v = at[q];
+                float v[4];
+                unpack24(d[3 * q], d[3 * q + 1], d[3 * q + 2], v);
                 g[2 * q] = v[0]; g[2 * q + 1] = v[1];
                 u[2 * q] = v[2]; u[2 * q + 1] = v[3];
             }
@@ -487,11 +490,20 @@ __global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p
     const int k = threadIdx.x, F = p.F, Fp = p.Fp;
     if (k >= Fp) return;
     const int64_t first = (int64_t)blockIdx.y * p.rows, last = std::min(first + p.rows, p.B);
-    const int at_g = DT == BT_F32 ? k : 4 * (k >> 1) + (k & 1), at_u = DT == BT_F32 ? F + k : at_g + 2;
     float bg = 0.0f, bu = 0.0f;
     for (int64_t row = first; row < last; row++) {
         float dg = 0.0f, du = 0.0f;
-        if (k < F) gated_grad_value<DT>(load_elem<DT>(p.dH, row * F + k), p.pre[row * 2 * Fp + at_g], p.pre[row * 2 * Fp + at_u], dg, du);
+        if (k < F) {
+            float v[4];
+            if constexpr (DT == BT_F32) {
+                v[k & 1] = ((const float*)p.pre)[row * 2 * F + k];
+                v[2 + (k & 1)] = ((const float*)p.pre)[row * 2 * F + F + k];
+            } else {
+                const uint32_t* at = (const uint32_t*)p.pre + row * (Fp / 2 * 3) + 3 * (k >> 1);
+                unpack24(at[0], at[1], at[2], v);
+            }
+            gated_grad_value<DT>(load_elem<DT>(p.dH, row * F + k), v[k & 1], v[2 + (k & 1)], dg, du);
+        }
         bg += dg;
         bu += du;
         store_elem<DT>(p.G, row * 2 * Fp + k, DT != BT_F32 ? dg * p.scale[k] : dg);
@@ -502,10 +514,9 @@ __global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p
     p.parts[(int64_t)blockIdx.y * 2 * F + F + k] = bu;
 }
 
-// Runs of rows of the gradient kernel: enough workgroups for the chip; 64 at most where each leaves sums behind
+// Runs of rows of the gradient kernel: eight workgroups a compute unit; two where each leaves sums behind
 static int64_t grad_runs(int64_t B, int64_t F, bool sums) {
-    const int64_t across = ceil_div(F, 2048), want = std::max<int64_t>(1, 8 * gemm_compute_units() / across);
-    return std::min<int64_t>(B, sums ? std::min<int64_t>(want, 64) : want);
+    return std::min<int64_t>(B, std::max<int64_t>(1, (sums ? 2 : 8) * gemm_compute_units() / ceil_div(F, 2048)));
 }
 
 template <int DT>
@@ -590,7 +601,7 @@ extern "C" int bt_gated_quantize(const void* gate, const void* up, int w_dtype, 
 }
 
 extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
-                                        float* pre, int64_t B, int64_t F, int64_t K, void* stream) {
+                                        void* pre, int64_t B, int64_t F, int64_t K, void* stream) {
     const char* who = "bt_ternary_gated_forward";
     if (!X || !W_pairs || !scale || !H || B <= 0 || F <= 0 || K <= 0 || (x_dtype != BT_F16 && x_dtype != BT_BF16)) {
         set_error("%s: null pointer, empty shape or bad dtype (fp16 and bf16 rows)", who);
@@ -610,7 +621,7 @@ extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padd
     Epilogue epi = {};
     epi.scale = scale; epi.scale_dtype = BT_F32;
     epi.bias = bias; epi.bias_dtype = BT_F32;
-    return launch_gemm_f16_gated(x_dtype == BT_F16 ? MODE_F16 : MODE_BF16, rows, W_pairs, epi, H, pre, F, B, 2 * Fp, Kr, (hipStream_t)stream);
+    return launch_gemm_f16_gated(x_dtype == BT_F16 ? MODE_F16 : MODE_BF16, rows, W_pairs, epi, H, (uint32_t*)pre, F, B, 2 * Fp, Kr, (hipStream_t)stream);
 }
 
 extern "C" int bt_gated_masters_serves(int64_t B, int64_t K, int w_dtype, int per_channel) { return masters_serve(B, K, w_dtype, per_channel != 0); }
@@ -647,7 +658,7 @@ extern "C" size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F) {
     return B > 0 && F > 0 ? (size_t)grad_runs(B, F, true) * 2 * (size_t)F * 4 : 0;
 }
 
-extern "C" int bt_gated_grad(const void* dH, int dtype, const float* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
+extern "C" int bt_gated_grad(const void* dH, int dtype, const void* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
                              int64_t F, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "bt_gated_grad";
     if (!dH || !pre || !G || B <= 0 || F <= 0 || (dtype != BT_F32 && dtype != BT_F16 && dtype != BT_BF16) || (dtype != BT_F32 && !scale)) {

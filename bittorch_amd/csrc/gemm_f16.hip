@@ -48,7 +48,7 @@ struct GemmFParams {
     void* Y;              // [M, N]
     int64_t Kb;           // packed weight rows
     Epilogue epi;
-    float* pre;           // OUT_GATED: [M, N] the two projections in fp32, column pairs of gate and up in turn, or null
+    uint32_t* pre;        // OUT_GATED: [M, 3 N / 4] the two projections in 24 bits each, column pairs of gate and up in turn, or null
     int64_t H;            // OUT_GATED: columns of Y, at most N / 2
 };
 // What becomes of a tile's sums: the linear layer's output; the SwiGLU of a layer whose columns are [gate | up], of the projections
@@ -162,9 +162,9 @@ __device__ __forceinline__ void fd_epilogue_swiglu(const GemmFParams& p, const v
 }
 
 // The training form (OUT_GATED): h = rd(silu(g) u) from the fp32 sums, one rounding, and where a backward pass follows g and u beside it.
-// They are kept in fp32: gate and up rounded to 16 bits would put two more roundings of their size into every gradient (with them
-// and the 16-bit operands of the gradient's products dx of bf16 rows is off by 2.0 times the rounding of dx itself, with fp32 by 1.4), for 28
-// bytes an output instead of 20 through memory in forward and backward.  A lane's four values of a row are 16 bytes of `pre`.
+// They are kept in 24 bits: rounded to 16 they would put two more roundings of their size into every gradient (with them and the 16-bit
+// operand of the gradient's products dx of bf16 rows is off by 2.0 times the rounding of dx itself; with 24 or 32 bits by 1.4), and 24 are
+// three quarters of fp32's way through memory, forward and backward.  A lane's four values of a row are 12 bytes of `pre`.
 template <int MODE, int MB>
 __device__ __forceinline__ void fd_epilogue_gated(const GemmFParams& p, const v4f (&acc)[MB][4], int64_t m0, int g, int64_t col,
                                                   int rows_left, const float (&ws)[4], const float (&bs)[4]) {
@@ -172,7 +172,8 @@ __device__ __forceinline__ void fd_epilogue_gated(const GemmFParams& p, const v4
     const int64_t row_bytes = p.H * 2;
     char* row = (char*)p.Y + m0 * row_bytes;
     const uint32_t lane_off = (uint32_t)(4 * g) * (uint32_t)row_bytes + (uint32_t)col * 2u;
-    float* pre = p.pre + (m0 + 4 * g) * p.N + 2 * col;
+    const int64_t pre_row = p.N / 4 * 3;  // dwords
+    uint32_t* pre = p.pre + (m0 + 4 * g) * pre_row + 3 * (col >> 1);
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) {
         if (16 * mb >= rows_left) return;  // (uniform)
@@ -186,9 +187,12 @@ __device__ __forceinline__ void fd_epilogue_gated(const GemmFParams& p, const v4
                 if constexpr (MODE == MODE_BF16) a *= 0.5f;  // weights were decoded as +-2.0
                 y[t] = epi_float(a, ws[t], bs[t]);
             }
-            if (p.pre && 16 * mb + 4 * g + r < rows_left)
-                st4_nt(pre + r * p.N, __builtin_bit_cast(uint32_t, y[0]), __builtin_bit_cast(uint32_t, y[1]),
-                       __builtin_bit_cast(uint32_t, y[2]), __builtin_bit_cast(uint32_t, y[3]));
+            if (p.pre && 16 * mb + 4 * g + r < rows_left) {
+                uint32_t q[3];
+                pack24(y, q);
+#pragma unroll
+                for (int e = 0; e < 3; e++) __builtin_nontemporal_store(q[e], pre + r * pre_row + e);
+            }
             d[r] = two_of<YDT>(y[0] * sigmoid_fast(y[0]) * y[2], y[1] * sigmoid_fast(y[1]) * y[3]);
         }
         if (p.H % 4 == 0) {  // (uniform; a pair of lanes has four columns that exist, or none)
@@ -202,7 +206,7 @@ __device__ __forceinline__ void fd_epilogue_gated(const GemmFParams& p, const v4
                         if (col + t < p.H) *(uint16_t*)(row + r * row_bytes + lane_off + 2 * t) = (uint16_t)(d[r] >> (16 * t));
         }
         row += 16 * row_bytes;
-        pre += 16 * p.N;
+        pre += 16 * pre_row;
         __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -692,8 +696,8 @@ int launch_gemm_f16(int mode, const void* X, const uint8_t* W_T, int w_layout, c
     return mode == MODE_F16 ? launch_gemm_f16_rows<MODE_F16>(p, rows, src, epi_op, st) : launch_gemm_f16_rows<MODE_BF16>(p, rows, src, epi_op, st);
 }
 // The training form of the SwiGLU output stage: Y [M, H] = silu(g) u of the layer [gate | up] with N / 2 >= H columns each (N % 32 == 0, a
-// tiled copy in pair order), pre [M, N] or null
-int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, float* pre, int64_t H, int64_t M,
+// tiled copy in pair order), pre [M, 3 N / 4] or null
+int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, uint32_t* pre, int64_t H, int64_t M,
                           int64_t N, int64_t K, hipStream_t st) {
     GemmFParams p = {};
     p.X = (const uint16_t*)X; p.W_T = W_tiled; p.Y = Y; p.epi = epi; p.pre = pre; p.H = H;

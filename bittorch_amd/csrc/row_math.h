@@ -99,6 +99,25 @@ __device__ __forceinline__ void swiglu_store16(char* row, int64_t row_bytes, uin
     for (int r = 0; r < 4; r++) d[r] = two_of<DT>(gate[2 * r], gate[2 * r + 1]);
     pairs_store16(row, row_bytes, lane_off, left, g, d);
 }
+// Four fp32 values rounded to 24 bits each (sign, exponent, 15 bits of fraction) in three dwords, and back.  Rounding adds half of the last
+// kept bit; a NaN is cut off instead, so that it stays one.
+__device__ __forceinline__ void pack24(const float (&v)[4], uint32_t (&d)[3]) {
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v[i]);
+        t[i] = (v[i] == v[i] ? u + 0x80u : u) >> 8;
+    }
+    d[0] = t[0] | t[1] << 24;
+    d[1] = t[1] >> 8 | t[2] << 16;
+    d[2] = t[2] >> 16 | t[3] << 8;
+}
+__device__ __forceinline__ void unpack24(uint32_t d0, uint32_t d1, uint32_t d2, float (&v)[4]) {
+    v[0] = __builtin_bit_cast(float, d0 << 8);
+    v[1] = __builtin_bit_cast(float, (d0 >> 16 & 0xff00u) | d1 << 16);
+    v[2] = __builtin_bit_cast(float, (d1 >> 8 & 0xffff00u) | d2 << 24);
+    v[3] = __builtin_bit_cast(float, d2 & 0xffffff00u);
+}
 // 1 / (1 + exp(-g)) to a few units in the last place of fp32, where the result is rounded to 16 bits afterwards
 __device__ __forceinline__ float sigmoid_fast(float g) {
     return __builtin_amdgcn_rcpf(__fadd_rn(1.0f, __builtin_amdgcn_exp2f(__fmul_rn(g, -1.44269504088896341f))));

@@ -258,11 +258,12 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *     workspace: at least bt_gated_quantize_workspace_bytes(F,K,per_channel) bytes.
  *   bt_ternary_gated_forward: fp16 / bf16 rows X [B,K]; where K % 8 != 0 or X is not 16-byte aligned, X_padded [B, K rounded up to 8] takes
  *     a copy of them (zeros behind each), otherwise it is NULL; H [B,F] in x_dtype, rounded once;
- *     pre (optional) [B, 2 Fp] fp32: g and u, columns 2 i and 2 i + 1 of either at 4 i .. 4 i + 3.
+ *     pre (optional) [B, 3 Fp / 2] dwords: g and u in 24 bits each (fp32 rounded to 16 bits of significand), dwords 3 i .. 3 i + 2 those
+ *     of g's columns 2 i and 2 i + 1 and u's, low bits first.
  *   bt_gated_masters_forward: H [F] of one row X [K] (any x_dtype) straight from the masters, quantized as they are read, with a scale for
  *     each feature; bt_gated_masters_serves says whether a call of B rows is one of those.
  *   bt_gated_grad: G = d(H . dH)/d[g | u].  16-bit dtype: pre as above, G [B, 2 Fp] in dtype, each half times its scale; BT_F32: pre is
- *     [g | u] [B, 2 F] and G [B, 2 F] without scales (scale unused).  dBias (optional) [2 F] in bias_dtype: the sums over the rows without
+ *     [g | u] [B, 2 F] fp32 and G [B, 2 F] without scales (scale unused).  dBias (optional) [2 F] in bias_dtype: the sums over the rows without
  *     scales; with it a workspace of bt_gated_grad_workspace_bytes(B,F).
  */
 size_t bt_gated_quantize_workspace_bytes(int64_t F, int64_t K, int per_channel);
@@ -270,12 +271,12 @@ int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, 
                       const void* gate_bias, const void* up_bias, int bias_dtype, uint8_t* W_pairs, uint8_t* W_back, uint8_t* W_rows,
                       float* scale, float* bias, void* workspace, size_t workspace_bytes, void* stream);
 int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
-                             float* pre, int64_t B, int64_t F, int64_t K, void* stream);
+                             void* pre, int64_t B, int64_t F, int64_t K, void* stream);
 int bt_gated_masters_serves(int64_t B, int64_t K, int w_dtype, int per_channel);
 int bt_gated_masters_forward(const void* X, int x_dtype, const void* gate, const void* up, int w_dtype, double threshold_factor,
                              const void* gate_bias, const void* up_bias, int bias_dtype, void* H, int64_t F, int64_t K, void* stream);
 size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F);
-int bt_gated_grad(const void* dH, int dtype, const float* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
+int bt_gated_grad(const void* dH, int dtype, const void* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
                   int64_t F, void* workspace, size_t workspace_bytes, void* stream);
 
 /*

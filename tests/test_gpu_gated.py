@@ -43,7 +43,7 @@ class _Reference:
 
     def __init__(self, x, wg, wu, bg, bu, dh, **quant):
         (self.tg, self.ag), (self.tu, self.au) = _ternary(wg, **quant), _ternary(wu, **quant)
-        x, dh, k = x.detach().double(), dh.double(), x.shape[1]
+        dt, x, dh, k = x.dtype, x.detach().double(), dh.double(), x.shape[1]
         self.x, self.dh = x, dh
         zero = torch.zeros(wg.shape[0], dtype=torch.float64, device=x.device)
         bg, bu = (zero if b is None else b.detach().double() for b in (bg, bu))
@@ -56,10 +56,16 @@ class _Reference:
         self.tol_u = chain * (x.abs() @ self.tu.abs().t()) * self.au + 4 * U * (u.abs() + bu.abs())
         sig = 1 / (1 + torch.exp(-g))
         self.g, self.u, silu = g, u, g * sig
-        self.h = silu * u
+        self.h, self.sig = silu * u, sig
         # silu' lies within -0.1 and 1.1; exp's argument is rounded (|g| U of the result), exp, the sum, the reciprocal, two products
         self.tol_h = 1.1 * u.abs() * self.tol_g + silu.abs() * self.tol_u + (g.abs() + 16) * U * self.h.abs()
-        slope = sig * (1 + g * (1 - sig))
+        if dt != torch.float32:  # (the gradient reads g and u in 24 bits: half a step is 2^-16 of a value)
+            self.tol_g, self.tol_u = self.tol_g + 2.0 ** -16 * g.abs(), self.tol_u + 2.0 ** -16 * u.abs()
+        self.follow()
+
+    def follow(self):
+        dh, g, u, sig = self.dh, self.g, self.u, self.sig
+        silu, slope = g * sig, sig * (1 + g * (1 - sig))
         self.dg, self.du = dh * u * slope, dh * silu
         # |silu''| is at most 1/2; 1 - sig is off by a step of 1, which g multiplies
         self.tol_dg = dh.abs() * (slope.abs() * self.tol_u + 0.5 * u.abs() * self.tol_g + u.abs() * sig * (3 * g.abs() + 16) * U)
@@ -156,9 +162,11 @@ def test_stages_of_the_16_bit_gradient(rows, k, f, dt):
     h, pre, read = _C.ternary_gated_forward(x, w, scale, bias, f, True)
     assert torch.equal(h, _C.ternary_gated_forward(x, w, scale, bias, f)[0])
     assert torch.equal(read, torch.nn.functional.pad(x, (0, -k % 8)))
-    pairs = pre.reshape(rows, fp // 2, 2, 2)
-    _assert_within(pairs[:, :, 0].reshape(rows, fp)[:, :f], ref.g, ref.tol_g, "g")
-    _assert_within(pairs[:, :, 1].reshape(rows, fp)[:, :f], ref.u, ref.tol_u, "u")
+    # 24 bits a value: g, g, u, u of two columns in three dwords
+    b = pre.view(torch.uint8).reshape(rows, fp // 2, 4, 3).to(torch.int32)
+    pairs = (b[..., 0] << 8 | b[..., 1] << 16 | b[..., 2] << 24).view(torch.float32).reshape(rows, fp // 2, 2, 2)
+    for n, (v, tol, what) in enumerate(((ref.g, ref.tol_g, "g"), (ref.u, ref.tol_u, "u"))):
+        _assert_within(pairs[:, :, n].reshape(rows, fp)[:, :f], v, tol, what)
     g, db = _C.gated_grad(dh, pre, scale, torch.float32)
     assert g.shape == (rows, 2 * fp) and not g[:, f:fp].any() and not g[:, fp + f:].any()
     _assert_within(g[:, :f], ref.dg * ref.ag, ref.tol_dg * ref.ag, "G gate")
