@@ -892,25 +892,21 @@ def gated_masters_serves(rows: int, masters: Tensor, per_channel: bool = True, a
 
 
 def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, up_bias: Optional[Tensor] = None,
-                  threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, rows: bool = False, back: bool = False):
+                  threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, back: bool = False):
     """The operands of the gated pair, of two masters ``[F, K]`` quantized as :func:`ternary_quantize_pack` does: ``(W_pairs, W_back,
-    scale, bias)`` as ``bt_gated_quantize`` makes them; ``rows``: ``W_rows [ceil(K/4), 2 F]`` in the first place; ``back``: with the copy
-    for the input's gradient (otherwise None)."""
+    scale, bias)`` as ``bt_gated_quantize`` makes them; ``back``: with the copy for the input's gradient (otherwise None)."""
     masters, wdt, biases, bdt = _gated_operands(gate, up, gate_bias, up_bias, as_half)
     (F, K), dev = gate.shape, gate.device
-    Kb = (K + 3) // 4
-    Fv = F if rows else (F + 15) // 16 * 16
-    w = torch.empty((Kb, 2 * F) if rows else (_L.bt_tiled_weights_bytes(2 * Fv, K),), dtype=torch.uint8, device=dev)
-    w_back = torch.empty((_L.bt_tiled_weights_bytes(K, 2 * Fv),), dtype=torch.uint8, device=dev) if back and not rows else None
-    scale = torch.empty((2 * Fv + 1,), dtype=torch.float32, device=dev)
-    has_bias = any(b is not None for b in biases)
-    bias = torch.empty((2 * Fv,), dtype=torch.float32, device=dev) if has_bias else None
+    Fp = (F + 15) // 16 * 16
+    w = torch.empty((_L.bt_tiled_weights_bytes(2 * Fp, K),), dtype=torch.uint8, device=dev)
+    w_back = torch.empty((_L.bt_tiled_weights_bytes(K, 2 * Fp),), dtype=torch.uint8, device=dev) if back else None
+    scale = torch.empty((2 * Fp + 1,), dtype=torch.float32, device=dev)
+    bias = torch.empty((2 * Fp,), dtype=torch.float32, device=dev) if any(b is not None for b in biases) else None
     with _on(gate):
         ws = _workspace(_L.bt_gated_quantize_workspace_bytes(F, K, int(bool(per_channel))), dev)
         _status(_L.bt_gated_quantize(masters[0].data_ptr(), masters[1].data_ptr(), wdt, F, K, float(threshold_factor), int(bool(per_channel)),
-                                     _ptr(biases[0]), _ptr(biases[1]), bdt, None if rows else w.data_ptr(), _ptr(w_back),
-                                     w.data_ptr() if rows else None, scale.data_ptr(), _ptr(bias), _ptr(ws), 0 if ws is None else ws.numel(),
-                                     _stream(gate)))
+                                     _ptr(biases[0]), _ptr(biases[1]), bdt, w.data_ptr(), _ptr(w_back), scale.data_ptr(), _ptr(bias), _ptr(ws),
+                                     0 if ws is None else ws.numel(), _stream(gate)))
     return w, w_back, scale, bias
 
 
@@ -937,23 +933,22 @@ def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optio
     return h, pre, rows
 
 
-def gated_grad(dH: Tensor, pre: Tensor, scale: Optional[Tensor], bias_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Optional[Tensor]]:
-    """Gradient of ``silu(gate) * up`` in both projections, ``[B, 2 Fp]`` in 16 bits times their scales, or ``[B, 2 F]`` fp32 without
-    (``pre`` then is ``[gate | up]`` in fp32); with ``bias_dtype`` also its sums over the rows ``[2 F]``, without scales."""
+def gated_grad(dH: Tensor, pre: Tensor, scale: Tensor, bias_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Optional[Tensor]]:
+    """Gradient of ``silu(gate) * up`` in both projections times their scales, ``[B, 2 Fp]`` (``pre`` as :func:`ternary_gated_forward` kept
+    it, or for fp32 rows ``[gate | up]`` ``[B, 2 Fp]``); with ``bias_dtype`` also its sums over the rows ``[2 F]``, without scales."""
     _check(dH.dim() == 2 and dH.numel() > 0 and dH.dtype in _DT, "dH must be 2D float32, float16 or bfloat16")
     B, F = dH.shape
-    Fv = F if dH.dtype == torch.float32 else (F + 15) // 16 * 16
-    kept = (torch.float32, (B, 2 * F)) if dH.dtype == torch.float32 else (torch.int32, (B, Fv // 2 * 3))
+    Fp = (F + 15) // 16 * 16
+    kept = (torch.float32, (B, 2 * Fp)) if dH.dtype == torch.float32 else (torch.int32, (B, Fp // 2 * 3))
     _check((pre.dtype, pre.shape) == kept and pre.is_contiguous(), "the projections must be those that the forward kept")
-    _check(dH.dtype == torch.float32 or (scale is not None and scale.dtype == torch.float32 and scale.numel() >= 2 * Fv and scale.is_contiguous()),
-           "scale must be fp32 with an entry for each padded feature")
+    _check(scale.dtype == torch.float32 and scale.numel() >= 2 * Fp and scale.is_contiguous(), "scale must be fp32 with an entry for each padded feature")
     _check(_all_cuda(dH, pre, scale), "All tensors must be CUDA")
     dH = dH.contiguous()
-    G = torch.empty((B, 2 * Fv), dtype=dH.dtype, device=dH.device)
+    G = torch.empty((B, 2 * Fp), dtype=dH.dtype, device=dH.device)
     db = None if bias_dtype is None else torch.empty((2 * F,), dtype=bias_dtype, device=dH.device)
     with _on(dH):
         ws = None if db is None else _workspace(_L.bt_gated_grad_workspace_bytes(B, F), dH.device)
-        _status(_L.bt_gated_grad(dH.data_ptr(), _DT[dH.dtype], pre.data_ptr(), _ptr(scale), G.data_ptr(), _ptr(db),
+        _status(_L.bt_gated_grad(dH.data_ptr(), _DT[dH.dtype], pre.data_ptr(), scale.data_ptr(), G.data_ptr(), _ptr(db),
                                  0 if db is None else _DT[bias_dtype], B, F, _ptr(ws), 0 if ws is None else ws.numel(), _stream(dH)))
     return G, db
 

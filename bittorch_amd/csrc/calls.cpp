@@ -694,12 +694,11 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 struct GatedOut {
     at::Tensor h, rows, pre, w_back, scale;  // rows: x, or the copy of it that the kernels read
 };
-// fp32 rows: K >= 4, F >= 2.  All tensors contiguous.
+// fp32 rows: K >= 4.  All tensors contiguous.
 GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const MaybeTensor& gate_bias, const MaybeTensor& up_bias,
                    double threshold, bool per_channel, bool keep, bool want_back) {
-    const int64_t F = gate.size(0), K = gate.size(1), Kb = (K + 3) / 4, B = x.numel() / K;
+    const int64_t F = gate.size(0), K = gate.size(1), Fp = (F + 15) / 16 * 16, B = x.numel() / K;
     const bool fp32 = x.scalar_type() == at::kFloat;
-    const int64_t Fv = fp32 ? F : (F + 15) / 16 * 16;
     const int dt = tag(x.scalar_type());
     void* st = stream_of(x.get_device());
     GatedOut o;
@@ -710,24 +709,22 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
              data_of(gate_bias), data_of(up_bias), gate_bias ? tag_of(gate_bias) : tag_of(up_bias), o.h.data_ptr(), F, K, st);
         return o;
     }
-    const at::Tensor w = fp32 ? output({Kb, 2 * F}, at::kByte, x) : output({(int64_t)lib.bt_tiled_weights_bytes(2 * Fv, K)}, at::kByte, x);
-    if (fp32) o.w_back = w;
-    else if (want_back) o.w_back = output({(int64_t)lib.bt_tiled_weights_bytes(K, 2 * Fv)}, at::kByte, x);
-    o.scale = output({2 * Fv + 1}, at::kFloat, x);
+    const at::Tensor w = output({(int64_t)lib.bt_tiled_weights_bytes(2 * Fp, K)}, at::kByte, x);
+    if (want_back) o.w_back = output({(int64_t)lib.bt_tiled_weights_bytes(K, 2 * Fp)}, at::kByte, x);
+    o.scale = output({2 * Fp + 1}, at::kFloat, x);
     at::Tensor bias;
-    if (gate_bias || up_bias) bias = output({2 * Fv}, at::kFloat, x);
+    if (gate_bias || up_bias) bias = output({2 * Fp}, at::kFloat, x);
     float* const scale_at = (float*)o.scale.data_ptr();
     float* const bias_at = bias.defined() ? (float*)bias.data_ptr() : nullptr;
     {
         const Scratch ws(lib.bt_gated_quantize_workspace_bytes(F, K, per_channel ? 1 : 0), x);
         call(lib.bt_gated_quantize, gate.const_data_ptr(), up.const_data_ptr(), tag(gate.scalar_type()), F, K, threshold, per_channel ? 1 : 0,
-             data_of(gate_bias), data_of(up_bias), gate_bias ? tag_of(gate_bias) : tag_of(up_bias), fp32 ? nullptr : (uint8_t*)w.data_ptr(),
-             !fp32 && want_back ? (uint8_t*)o.w_back.data_ptr() : nullptr, fp32 ? (uint8_t*)w.data_ptr() : nullptr, scale_at, bias_at, ws.ptr(),
-             ws.size(), st);
+             data_of(gate_bias), data_of(up_bias), gate_bias ? tag_of(gate_bias) : tag_of(up_bias), (uint8_t*)w.data_ptr(),
+             want_back ? (uint8_t*)o.w_back.data_ptr() : nullptr, scale_at, bias_at, ws.ptr(), ws.size(), st);
     }
     o.h = output(with_last(x, F), x.scalar_type(), x);
-    if (fp32) o.pre = output({B, 2 * F}, at::kFloat, x);
-    else if (keep) o.pre = output({B, Fv / 2 * 3}, at::kInt, x);
+    if (fp32) o.pre = output({B, 2 * Fp}, at::kFloat, x);
+    else if (keep) o.pre = output({B, Fp / 2 * 3}, at::kInt, x);
     if (!fp32) {
         void* padded = nullptr;
         if (K % 8 != 0 || !aligned(x, 16)) {
@@ -738,10 +735,10 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
              keep ? o.pre.data_ptr() : nullptr, B, F, K, st);
         return o;
     }
-    const Scratch ws(lib.bt_packed_forward_workspace_bytes(B, 2 * F, K, dt), x);
-    call(lib.bt_ternary_linear_packed_forward, x.const_data_ptr(), dt, (const uint8_t*)w.const_data_ptr(), scale_at, BT_F32, 2 * F, bias_at, BT_F32,
-         o.pre.data_ptr(), B, 2 * F, K, ws.ptr(), ws.size(), st);
-    call(lib.bt_swiglu, o.pre.const_data_ptr(), 2 * F, (const float*)o.pre.const_data_ptr() + F, 2 * F, BT_F32, B, F, o.h.data_ptr(), nullptr, nullptr, 0, st);
+    const Scratch ws(lib.bt_tiled_forward_workspace_bytes(B, 2 * Fp, K, dt), x);
+    call(lib.bt_ternary_linear_tiled_forward, x.const_data_ptr(), K, dt, 0, nullptr, 0, 0.0f, (const uint8_t*)w.const_data_ptr(), scale_at, BT_F32, 2 * Fp,
+         bias_at, BT_F32, nullptr, BT_EPI_NATURAL_FROM_PAIRS, o.pre.data_ptr(), B, 2 * Fp, K, ws.ptr(), ws.size(), st);
+    call(lib.bt_swiglu, o.pre.const_data_ptr(), 2 * Fp, (const float*)o.pre.const_data_ptr() + Fp, 2 * Fp, BT_F32, B, F, o.h.data_ptr(), nullptr, nullptr, 0, st);
     return o;
 }
 
@@ -768,13 +765,13 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         const at::NoGradGuard no_grad;
         const c10::DeviceGuard guard(x.device());
         const int64_t F = shape[0], K = shape[1], Kr = x.size(-1), B = x.numel() / Kr;  // (a padded copy has longer rows)
-        const bool rows = x.scalar_type() == at::kFloat;
-        const int64_t Fv = rows ? F : (F + 15) / 16 * 16;
+        const bool fp32 = x.scalar_type() == at::kFloat;
+        const int64_t Fp = (F + 15) / 16 * 16;
         const int dt = tag(x.scalar_type());
         const bool want_w = w.want[1] || w.want[2], want_b = w.want[3] || w.want[4];
         void* st = stream_of(x.get_device());
-        const at::Tensor dh = incoming[0].contiguous(), g = output({B, 2 * Fv}, x.scalar_type(), x);
-        const float *scale_at = (const float*)scale.const_data_ptr(), *one = scale_at + 2 * Fv;
+        const at::Tensor dh = incoming[0].contiguous(), g = output({B, 2 * Fp}, x.scalar_type(), x);
+        const float *scale_at = (const float*)scale.const_data_ptr(), *one = scale_at + 2 * Fp;
         at::Tensor db;
         if (want_b) db = output({2 * F}, b_dtype, x);
         {
@@ -784,29 +781,24 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         }
         if (w.want[0]) {
             w.grads[0] = output(with_last(incoming[0], K), x.scalar_type(), x);
-            if (rows) {
-                check_status(lib.bt_ternary_linear_grad_input((const float*)g.const_data_ptr(), (const uint8_t*)w_back.const_data_ptr(), scale_at, 2 * F,
-                                                              (float*)w.grads[0].data_ptr(), B, 2 * F, K, st));
-            } else {
-                const Scratch ws(lib.bt_tiled_forward_workspace_bytes(B, K, 2 * Fv, dt), x);
-                check_status(lib.bt_ternary_linear_tiled_forward(g.const_data_ptr(), 2 * Fv, dt, 0, nullptr, 0, 0.0f, (const uint8_t*)w_back.const_data_ptr(),
-                                                                 one, BT_F32, 1, nullptr, 0, nullptr, 0, w.grads[0].data_ptr(), B, K, 2 * Fv, ws.ptr(), ws.size(), st));
-            }
+            const Scratch ws(lib.bt_tiled_forward_workspace_bytes(B, K, 2 * Fp, dt), x);
+            check_status(lib.bt_ternary_linear_tiled_forward(g.const_data_ptr(), 2 * Fp, dt, 0, nullptr, 0, 0.0f, (const uint8_t*)w_back.const_data_ptr(), one,
+                                                             BT_F32, 1, nullptr, 0, nullptr, 0, w.grads[0].data_ptr(), B, K, 2 * Fp, ws.ptr(), ws.size(), st));
         }
         if (want_w) {
             const at::ScalarType dtype = w_dtype == x.scalar_type() ? w_dtype : at::kFloat;
-            at::Tensor dw = output({2 * Fv, Kr}, dtype, x);
-            if (rows) {
-                const Scratch ws(lib.bt_linear_grad_weight_workspace_bytes(B, 2 * F, K), x);
-                check_status(lib.bt_linear_grad_weight((const float*)g.const_data_ptr(), (const float*)x.const_data_ptr(), scale_at, 2 * F, (float*)dw.data_ptr(),
-                                                       nullptr, B, 2 * F, K, ws.ptr(), ws.size(), st));
+            at::Tensor dw = output({2 * Fp, Kr}, dtype, x);
+            if (fp32) {
+                const Scratch ws(lib.bt_linear_grad_weight_workspace_bytes(B, 2 * Fp, Kr), x);
+                check_status(lib.bt_linear_grad_weight((const float*)g.const_data_ptr(), (const float*)x.const_data_ptr(), one, 1, (float*)dw.data_ptr(),
+                                                       nullptr, B, 2 * Fp, Kr, ws.ptr(), ws.size(), st));
             } else {
-                const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fv, Kr), x);
-                check_status(lib.bt_linear_grad_weight_16(g.const_data_ptr(), x.const_data_ptr(), dt, one, BT_F32, 1, dw.data_ptr(), tag(dtype), B, 2 * Fv, Kr,
+                const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fp, Kr), x);
+                check_status(lib.bt_linear_grad_weight_16(g.const_data_ptr(), x.const_data_ptr(), dt, one, BT_F32, 1, dw.data_ptr(), tag(dtype), B, 2 * Fp, Kr,
                                                           ws.ptr(), ws.size(), st));
             }
             for (int i = 0; i < 2; i++)
-                if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * Fv, F).narrow(1, 0, K).to(w_dtype).contiguous();
+                if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * Fp, F).narrow(1, 0, K).to(w_dtype).contiguous();
         }
         for (int i = 0; i < 2; i++)
             if (w.want[3 + i]) w.grads[3 + i] = db.narrow(0, i * F, F);
@@ -826,7 +818,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *gate = plain(a[1], device), *up = plain(a[2], device), *gate_bias = nullptr, *up_bias = nullptr;
     ORDINARY(gate && up && gate->dim() == 2 && gate->sizes() == up->sizes() && gate->scalar_type() == up->scalar_type() && tag(gate->scalar_type()) >= 0);
     const int64_t F = gate->size(0), K = gate->size(1);
-    ORDINARY(x->size(-1) == K && (x->scalar_type() != at::kFloat || (K >= 4 && F >= 2)));
+    ORDINARY(x->size(-1) == K && (x->scalar_type() != at::kFloat || K >= 4));
     if (a[3] != Py_None) ORDINARY((gate_bias = vec(a[3], F, false, device)));
     if (a[4] != Py_None) ORDINARY((up_bias = vec(a[4], F, false, device)) && (!gate_bias || gate_bias->scalar_type() == up_bias->scalar_type()));
     if (differentiated({x, gate, up, gate_bias, up_bias}))

@@ -14,7 +14,8 @@
 // of the matrix cores; it serves both products behind it: dx = G [T_g; T_u] on a second tiled copy of the codes, in which the contraction
 // runs over the output features, by the forward's kernel, and dW = G^T x by the weight gradient's (grad_w16.hip).  a times dg, not
 // dg, is what is rounded, so that neither product has a scale of its own.
-// fp32 rows: the same steps on the fp32 kernels, G without the scales, which those kernels apply.
+// fp32 rows: the same steps on the fp32 kernels and the same copies, the projections stored in fp32 and h by the SwiGLU row kernel.  (On the
+// packed bytes as rows the fp32 products take longer: 4096 x 4096 x 768 forward 74 us, 68 on the copy, its transpose 89 and 77.)
 //
 // Features are padded to Fp = F rounded up to 16 where the matrix cores read them: zero codes, scales and biases, zero columns of G.
 #include "row_vec.h"
@@ -36,13 +37,12 @@ struct GatedWeightsParams {
     const float* a[2];        // their scales: F entries or one
     const void* b[2];         // biases or null
     int bias_dtype, one_scale;
-    int64_t F, Fv, K, Kb;     // Fv: features of a half in the outputs (F, or F padded)
-    uint8_t* pairs;           // forward: tiled copy in pair order of [gate | up], 2 Fv columns
-    uint8_t* back;            // backward: tiled copy of the transpose: K columns, contraction over 2 Fv
-    uint8_t* rows;            // or both as they lie, side by side: [Kb, 2 F]
-    float* scale;             // [2 Fv + 1], the last one 1 (the scale of products that have none)
-    float* bias;              // [2 Fv] or null
-    uint32_t n_pairs, n_back, n_rows;  // workgroups of each part, in this order; behind them those of the vectors
+    int64_t F, Fp, K, Kb;
+    uint8_t* pairs;           // forward: tiled copy in pair order of [gate | up], 2 Fp columns
+    uint8_t* back;            // backward: tiled copy of the transpose: K columns, contraction over 2 Fp
+    float* scale;             // [2 Fp + 1], the last one 1 (the scale of products that have none)
+    float* bias;              // [2 Fp] or null
+    uint32_t n_pairs, n_back;          // workgroups of each part, in this order; behind them those of the vectors
     uint32_t steps, back_steps;        // 64-wide steps of the two tiled copies
 };
 
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256) void gated_weights_kernel(GatedWeightsParams p
         __syncthreads();
         const int tile = tid >> 4, g = (tid >> 2) & 3, j = 4 * (tid & 3);
         const int64_t t = (n0 >> 4) + tile;
-        if (16 * t >= p.Fv) return;
+        if (16 * t >= p.Fp) return;
         uint32_t row[4], out[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) row[r] = *(const uint32_t*)(block + (4 * g + r) * PITCH + 16 * tile + j);
@@ -103,9 +103,9 @@ __global__ __launch_bounds__(256) void gated_weights_kernel(GatedWeightsParams p
         if (s >= S) return;
         const int64_t kb = 4 * t + q, n = 64 * s + 16 * g;
         u32x4 d = {0u, 0u, 0u, 0u};
-        if (kb < p.Kb && n < 2 * p.Fv) {
-            const int half = n >= p.Fv;
-            d = codes16(p.W[half] + kb * p.F, n - (half ? p.Fv : 0), p.F);
+        if (kb < p.Kb && n < 2 * p.Fp) {
+            const int half = n >= p.Fp;
+            d = codes16(p.W[half] + kb * p.F, n - (half ? p.Fp : 0), p.F);
         }
         uint32_t out[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -115,27 +115,13 @@ __global__ __launch_bounds__(256) void gated_weights_kernel(GatedWeightsParams p
         ((uint4*)p.back)[(t * S + s) * 16 + 4 * g + q] = make_uint4(out[0], out[1], out[2], out[3]);
         return;
     }
-    wg -= p.n_back;
-    if (wg < p.n_rows) {
-        const int64_t i = ((int64_t)wg * 256 + tid) * 16, per_row = (p.F + 15) / 16 * 16;  // (one row of one half: per_row / 16 threads)
-        const int64_t kb = i / (2 * per_row), n2 = i - kb * 2 * per_row;
-        if (kb >= p.Kb) return;
-        const int half = n2 >= per_row;
-        const int64_t n = n2 - (half ? per_row : 0);
-        const uint8_t* src = p.W[half] + kb * p.F;
-        uint8_t* dst = p.rows + kb * 2 * p.F + (half ? p.F : 0);
-        if (n + 16 <= p.F) *(u32x4_a1*)(dst + n) = *(const u32x4_a1*)(src + n);
-        else
-            for (int e = 0; n + e < p.F; e++) dst[n + e] = src[n + e];
-        return;
-    }
-    const int64_t n = (int64_t)(wg - p.n_rows) * 256 + tid;
-    if (n < 2 * p.Fv) {
-        const int half = n >= p.Fv;
-        const int64_t f = n - (half ? p.Fv : 0);
+    const int64_t n = (int64_t)(wg - p.n_back) * 256 + tid;
+    if (n < 2 * p.Fp) {
+        const int half = n >= p.Fp;
+        const int64_t f = n - (half ? p.Fp : 0);
         p.scale[n] = f < p.F ? p.a[half][p.one_scale ? 0 : f] : 0.0f;
         if (p.bias) p.bias[n] = f < p.F && p.b[half] ? load_elem_rt(p.b[half], p.bias_dtype, f) : 0.0f;
-    } else if (n == 2 * p.Fv) {
+    } else if (n == 2 * p.Fp) {
         p.scale[n] = 1.0f;
     }
 }
@@ -145,9 +131,9 @@ struct GatedQuantizeParams {
     const void* b[2];
     int bias_dtype;
     float tf, clamp_min;
-    int F, K, Fv;             // as above
+    int F, K, Fp;             // as above
     int tiles, per_xcd;       // of 16 features, both halves
-    uint8_t *pairs, *back, *rows;
+    uint8_t *pairs, *back;
     float *scale, *bias;
     uint32_t steps, back_steps;
 };
@@ -221,21 +207,18 @@ __global__ __launch_bounds__(512) void gated_quantize_kernel(GatedQuantizeParams
             c = !there || k >= K ? 0u : RAG && k + 8 > K ? c & ((1u << (2 * (K - k))) - 1u) : c;
             *(uint16_t*)(codes + (RPW * wave + r) * PITCH + (i * 64 + lane) * 2) = (uint16_t)c;
         }
-        if (lane == 0 && f < p.Fv) {
-            const int at = half * p.Fv + f;
+        if (lane == 0 && f < p.Fp) {
+            const int at = half * p.Fp + f;
             p.scale[at] = there ? s : 0.0f;
             if (p.bias) p.bias[at] = there && p.b[half] ? load_elem_rt(p.b[half], p.bias_dtype, f) : 0.0f;
-            if (at == 0) p.scale[2 * p.Fv] = 1.0f;
+            if (at == 0) p.scale[2 * p.Fp] = 1.0f;
         }
     }
     __syncthreads();
-    if (p.pairs) {
-        uint32_t* const out = (uint32_t*)p.pairs + (int64_t)(2 * tile + half) * p.steps * 64;
-        for (uint32_t i = tid; i < p.steps * 64; i += 512)
-            out[i] = *(const uint32_t*)(codes + (i & 15) * PITCH + 16 * (i >> 6) + 4 * ((i >> 4) & 3));
-    }
-    if (!p.back && !p.rows) return;
-    const uint32_t n0 = (uint32_t)(half * p.Fv + f0);
+    uint32_t* const pairs = (uint32_t*)p.pairs + (int64_t)(2 * tile + half) * p.steps * 64;
+    for (uint32_t i = tid; i < p.steps * 64; i += 512) pairs[i] = *(const uint32_t*)(codes + (i & 15) * PITCH + 16 * (i >> 6) + 4 * ((i >> 4) & 3));
+    if (!p.back) return;
+    const uint32_t n0 = (uint32_t)(half * p.Fp + f0);
     for (int kb = tid; 4 * kb < K; kb += 512) {  // (the four threads of 16 k read the same dwords)
         uint32_t t[4];  // the bytes kb of features 4 r .. + 3
 #pragma unroll
@@ -245,35 +228,27 @@ __global__ __launch_bounds__(512) void gated_quantize_kernel(GatedQuantizeParams
             for (int i = 0; i < 4; i++) d[i] = *(const uint32_t*)(codes + (4 * r + i) * PITCH + (kb & ~3)) >> (8 * (kb & 3)) & 0xffu;
             t[r] = d[0] | d[1] << 8 | d[2] << 16 | d[3] << 24;
         }
-        if (p.back) {
-            uint4* const out = (uint4*)p.back + ((int64_t)(kb >> 2) * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3) + (kb & 3);
-            uint32_t o[4] = {0u, 0u, 0u, 0u};
+        uint4* const out = (uint4*)p.back + ((int64_t)(kb >> 2) * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3) + (kb & 3);
+        uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int r = 0; r < 4; r++)
+        for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) o[c] |= byte_of_codes(t[r] >> (2 * c)) << (8 * r);
-            *out = make_uint4(o[0], o[1], o[2], o[3]);
-        } else {
-            uint8_t* dst = p.rows + (int64_t)kb * 2 * p.F + half * p.F + f0;
-            const u32x4 v = {t[0], t[1], t[2], t[3]};
-            if (f0 + 16 <= p.F) *(u32x4_a1*)dst = v;
-            else
-                for (int e = 0; f0 + e < p.F; e++) dst[e] = (uint8_t)(v[e >> 2] >> (8 * (e & 3)));
-        }
+            for (int c = 0; c < 4; c++) o[c] |= byte_of_codes(t[r] >> (2 * c)) << (8 * r);
+        *out = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    // the features of the transpose's last step past both halves, from the workgroup of the last tile
-    if (p.back && lin == p.tiles - 1) {
-        const int kbs = (K + 15) / 16 * 4;
+    // the bytes of the last column tile behind K
+    const uint32_t kbs = (uint32_t)(K + 15) / 16 * 4, kb_end = (uint32_t)(K + 3) / 4;
+    if (kb_end + tid < kbs) {
+        const uint32_t kb = kb_end + tid;
+        ((uint4*)p.back)[((int64_t)(kb >> 2) * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3) + (kb & 3)] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    // the features of the last step past both halves, from the workgroup of the last tile
+    if (lin == p.tiles - 1) {
         const uint32_t first = (n0 >> 4) + 1, groups = 4 * p.back_steps - first;
         for (uint32_t i = tid; i < kbs * groups; i += 512) {
             const uint32_t kb = i % kbs, g = first + i / kbs;
             ((uint4*)p.back)[((int64_t)(kb >> 2) * p.back_steps + (g >> 2)) * 16 + 4 * (g & 3) + (kb & 3)] = make_uint4(0u, 0u, 0u, 0u);
         }
-    }
-    if (p.back) {  // bytes of the last column tile behind K
-        const int kbs = (K + 15) / 16 * 4, kb = (K + 3) / 4 + tid;
-        if (kb < kbs)
-            ((uint4*)p.back)[((int64_t)(kb >> 2) * p.back_steps + (n0 >> 6)) * 16 + 4 * ((n0 >> 4) & 3) + (kb & 3)] = make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
@@ -410,10 +385,10 @@ static bool masters_serve(int64_t B, int64_t K, int w_dtype, bool per_channel) {
 
 struct GatedGradParams {
     const void* dH;       // [B, F]
-    const void* pre;      // 16-bit rows: [B, 3 Fp / 2] dwords, column pairs of gate and up in turn in 24 bits; fp32 rows: [B, 2 F], gate | up
-    const float* scale;   // 16-bit rows: [2 Fp]
-    void* G;              // [B, 2 Fp] / [B, 2 F]
-    float* parts;         // [gridDim.y, 2 Fp] sums of dg | du, or null
+    const void* pre;      // 16-bit rows: [B, 3 Fp / 2] dwords, column pairs of gate and up in turn in 24 bits; fp32 rows: [B, 2 Fp], gate | up
+    const float* scale;   // [2 Fp]
+    void* G;              // [B, 2 Fp]
+    float* parts;         // [gridDim.y, 2 F] sums of dg | du, or null
     int64_t B, rows;      // rows: of a workgroup
     int F, Fp;
 };
@@ -436,8 +411,8 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
     float ag[8], au[8], bg[8], bu[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        ag[e] = DT != BT_F32 ? p.scale[k + e] : 1.0f;
-        au[e] = DT != BT_F32 ? p.scale[Fp + k + e] : 1.0f;
+        ag[e] = p.scale[k + e];
+        au[e] = p.scale[Fp + k + e];
         bg[e] = bu[e] = 0.0f;
     }
 #pragma unroll 2
@@ -445,9 +420,8 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
         float dh[8], g[8], u[8];
         const Raw8<DT> dh_in = load_raw8<DT>(p.dH, row * F + piece_at(k, F));
         if constexpr (DT == BT_F32) {
-            const Raw8<DT> g_in = load_raw8<DT>(p.pre, row * 2 * F + piece_at(k, F)), u_in = load_raw8<DT>(p.pre, row * 2 * F + F + piece_at(k, F));
-            widen_piece<DT, RAG>(g_in, k, F, g);
-            widen_piece<DT, RAG>(u_in, k, F, u);
+            widen8<DT>(load_raw8<DT>(p.pre, row * 2 * Fp + k), g);
+            widen8<DT>(load_raw8<DT>(p.pre, row * 2 * Fp + Fp + k), u);
         } else {
             const u32x4* at = (const u32x4*)((const uint32_t*)p.pre + (row * Fp + k) / 2 * 3);
             const u32x4 a = at[0], b = at[1], c = at[2];
@@ -467,16 +441,11 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
             gated_grad_value<DT>(dh[e], g[e], u[e], dg, du);
             bg[e] += dg;
             bu[e] += du;
-            g[e] = DT != BT_F32 ? dg * ag[e] : dg;
-            u[e] = DT != BT_F32 ? du * au[e] : du;
+            g[e] = dg * ag[e];
+            u[e] = du * au[e];
         }
-        if constexpr (DT == BT_F32) {
-            store_piece<DT, RAG>(p.G, row * 2 * F, k, F, g);
-            store_piece<DT, RAG>(p.G, row * 2 * F + F, k, F, u);
-        } else {
-            store8u<DT>(p.G, row * 2 * Fp + k, g);
-            store8u<DT>(p.G, row * 2 * Fp + Fp + k, u);
-        }
+        store8u<DT>(p.G, row * 2 * Fp + k, g);
+        store8u<DT>(p.G, row * 2 * Fp + Fp + k, u);
     }
     if (!p.parts) return;
     float* out = p.parts + (int64_t)blockIdx.y * 2 * F;
@@ -496,8 +465,8 @@ __global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p
         if (k < F) {
             float v[4];
             if constexpr (DT == BT_F32) {
-                v[k & 1] = ((const float*)p.pre)[row * 2 * F + k];
-                v[2 + (k & 1)] = ((const float*)p.pre)[row * 2 * F + F + k];
+                v[k & 1] = ((const float*)p.pre)[row * 2 * Fp + k];
+                v[2 + (k & 1)] = ((const float*)p.pre)[row * 2 * Fp + Fp + k];
             } else {
                 const uint32_t* at = (const uint32_t*)p.pre + row * (Fp / 2 * 3) + 3 * (k >> 1);
                 unpack24(at[0], at[1], at[2], v);
@@ -506,8 +475,8 @@ __global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p
         }
         bg += dg;
         bu += du;
-        store_elem<DT>(p.G, row * 2 * Fp + k, DT != BT_F32 ? dg * p.scale[k] : dg);
-        store_elem<DT>(p.G, row * 2 * Fp + Fp + k, DT != BT_F32 ? du * p.scale[Fp + k] : du);
+        store_elem<DT>(p.G, row * 2 * Fp + k, dg * p.scale[k]);
+        store_elem<DT>(p.G, row * 2 * Fp + Fp + k, du * p.scale[Fp + k]);
     }
     if (!p.parts || k >= F) return;
     p.parts[(int64_t)blockIdx.y * 2 * F + k] = bg;
@@ -540,11 +509,11 @@ extern "C" size_t bt_gated_quantize_workspace_bytes(int64_t F, int64_t K, int pe
 }
 
 extern "C" int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, int64_t K, double threshold_factor, int per_channel,
-                                 const void* gate_bias, const void* up_bias, int bias_dtype, uint8_t* W_pairs, uint8_t* W_back, uint8_t* W_rows,
+                                 const void* gate_bias, const void* up_bias, int bias_dtype, uint8_t* W_pairs, uint8_t* W_back,
                                  float* scale, float* bias, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "bt_gated_quantize";
-    if (!gate || !up || !scale || F <= 0 || K <= 0 || (!W_pairs && !W_rows) || (W_rows && (W_pairs || W_back))) {
-        set_error("%s: null pointer or empty shape, or both the tiled copies and the rows asked for", who);
+    if (!gate || !up || !scale || !W_pairs || F <= 0 || K <= 0) {
+        set_error("%s: null pointer or empty shape", who);
         return BT_ERR_INVALID;
     }
     if (w_dtype != BT_F32 && w_dtype != BT_F16 && w_dtype != BT_BF16 && w_dtype != BT_F32_AS_F16) {
@@ -567,14 +536,14 @@ extern "C" int bt_gated_quantize(const void* gate, const void* up, int w_dtype, 
         return BT_ERR_WORKSPACE;
     }
     hipStream_t st = (hipStream_t)stream;
-    const int64_t Fv = W_rows ? F : Fp, Kb = ceil_div(K, 4);
+    const int64_t Kb = ceil_div(K, 4);
     const uint32_t steps = (uint32_t)ceil_div(Kb, 16), back_steps = (uint32_t)ceil_div(2 * Fp, 64);
     if (!need) {
         GatedQuantizeParams p = {};
         p.W[0] = gate; p.W[1] = up; p.b[0] = gate_bias; p.b[1] = up_bias; p.bias_dtype = bias_dtype;
         p.tf = (float)threshold_factor; p.clamp_min = quantize_clamp_min(w_dtype);
-        p.F = (int)F; p.K = (int)K; p.Fv = (int)Fv; p.tiles = (int)(2 * ceil_div(F, 16)); p.per_xcd = (int)ceil_div(p.tiles, 8);
-        p.pairs = W_pairs; p.back = W_back; p.rows = W_rows; p.scale = scale; p.bias = bias; p.steps = steps; p.back_steps = back_steps;
+        p.F = (int)F; p.K = (int)K; p.Fp = (int)Fp; p.tiles = (int)(2 * ceil_div(F, 16)); p.per_xcd = (int)ceil_div(p.tiles, 8);
+        p.pairs = W_pairs; p.back = W_back; p.scale = scale; p.bias = bias; p.steps = steps; p.back_steps = back_steps;
         if (w_dtype == BT_F32) launch_gated_quantize<BT_F32>(p, st);
         else if (w_dtype == BT_F16) launch_gated_quantize<BT_F16>(p, st);
         else if (w_dtype == BT_BF16) launch_gated_quantize<BT_BF16>(p, st);
@@ -590,13 +559,12 @@ extern "C" int bt_gated_quantize(const void* gate, const void* up, int w_dtype, 
     GatedWeightsParams p = {};
     p.W[0] = codes[0]; p.W[1] = codes[1]; p.a[0] = absmax[0]; p.a[1] = absmax[1]; p.b[0] = gate_bias; p.b[1] = up_bias;
     p.bias_dtype = bias_dtype; p.one_scale = !per_channel;
-    p.F = F; p.Fv = Fv; p.K = K; p.Kb = Kb;
-    p.pairs = W_pairs; p.back = W_back; p.rows = W_rows; p.scale = scale; p.bias = bias;
+    p.F = F; p.Fp = Fp; p.K = K; p.Kb = Kb;
+    p.pairs = W_pairs; p.back = W_back; p.scale = scale; p.bias = bias;
     p.steps = steps; p.back_steps = back_steps;
-    p.n_pairs = W_pairs ? (uint32_t)(2 * steps * ceil_div(Fp, 256)) : 0;
+    p.n_pairs = (uint32_t)(2 * steps * ceil_div(Fp, 256));
     p.n_back = W_back ? (uint32_t)(ceil_div(K, 16) * ceil_div(back_steps, 16)) : 0;
-    p.n_rows = W_rows ? (uint32_t)ceil_div(Kb * 2 * ceil_div(F, 16), 256) : 0;
-    hipLaunchKernelGGL(gated_weights_kernel, dim3(p.n_pairs + p.n_back + p.n_rows + (unsigned)(2 * Fv / 256 + 1)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(gated_weights_kernel, dim3(p.n_pairs + p.n_back + (unsigned)(2 * Fp / 256 + 1)), dim3(256), 0, st, p);
     return check_launch(who);
 }
 
@@ -661,11 +629,11 @@ extern "C" size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F) {
 extern "C" int bt_gated_grad(const void* dH, int dtype, const void* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
                              int64_t F, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "bt_gated_grad";
-    if (!dH || !pre || !G || B <= 0 || F <= 0 || (dtype != BT_F32 && dtype != BT_F16 && dtype != BT_BF16) || (dtype != BT_F32 && !scale)) {
+    if (!dH || !pre || !G || B <= 0 || F <= 0 || (dtype != BT_F32 && dtype != BT_F16 && dtype != BT_BF16) || !scale) {
         set_error("%s: null pointer, empty shape or bad dtype", who);
         return BT_ERR_INVALID;
     }
-    if (F >= (1ll << 23) || B >= (1ll << 31) || (dtype != BT_F32 && (((uintptr_t)pre) | ((uintptr_t)G)) % 16 != 0)) {
+    if (F >= (1ll << 23) || B >= (1ll << 31) || (((uintptr_t)pre) | ((uintptr_t)G)) % 16 != 0) {
         set_error("%s: F below 2^23, B below 2^31, the projections and G 16-byte aligned", who);
         return BT_ERR_INVALID;
     }
@@ -682,7 +650,7 @@ extern "C" int bt_gated_grad(const void* dH, int dtype, const void* pre, const f
     p.rows = ceil_div(B, runs);
     runs = ceil_div(B, p.rows);  // (so that none is empty)
     p.dH = dH; p.pre = pre; p.scale = scale; p.G = G; p.parts = dBias ? (float*)workspace : nullptr;
-    p.B = B; p.F = (int)F; p.Fp = dtype == BT_F32 ? (int)F : (int)padded(F);
+    p.B = B; p.F = (int)F; p.Fp = (int)padded(F);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == BT_F32) launch_gated_grad<BT_F32>(p, runs, st);
     else if (dtype == BT_F16) launch_gated_grad<BT_F16>(p, runs, st);

@@ -41,19 +41,18 @@ class _GatedLinear(torch.autograd.Function):
         from .. import _C
 
         f, k = gate.shape
-        rows = x.dtype == torch.float32
         x2 = x.reshape(-1, k)
         if not keep and _C.gated_masters_serves(x2.shape[0], gate, per_channel, as_half):
             h = _C.gated_masters_forward(x2, gate, up, gate_bias, up_bias, threshold_factor, as_half)
             return h.reshape(*x.shape[:-1], f)
-        w, w_back, scale, bias = _C.gated_weights(gate, up, gate_bias, up_bias, threshold_factor, per_channel, as_half, rows,
+        w, w_back, scale, bias = _C.gated_weights(gate, up, gate_bias, up_bias, threshold_factor, per_channel, as_half,
                                                   back=keep and ctx.needs_input_grad[0])
-        if rows:
-            # (the fp32 gradient kernels take four columns and more)
+        if x.dtype == torch.float32:
+            # (the fp32 kernel of the masters' gradient takes four columns and more)
             x2 = F.pad(x2, (0, 4 - k)) if k < 4 else x2.contiguous()
-            pre = _C.ternary_linear_packed_forward(x2, w, scale[:2 * f], bias, x2.shape[1])
-            h = _C.swiglu(pre[:, :f], pre[:, f:])
-            w_back = w
+            fp = scale.numel() // 2
+            pre = _C.ternary_linear_tiled_forward(x2, w, scale[:2 * fp], bias, x2.shape[1], 2 * fp, natural_from_pairs=True)
+            h = _C.swiglu(pre[:, :f], pre[:, fp:fp + f])
         else:
             h, pre, x2 = _C.ternary_gated_forward(x2, w, scale, bias, f, keep)
         if keep:
@@ -78,25 +77,17 @@ class _GatedLinear(torch.autograd.Function):
         dx = dg = du = dgb = dub = None
         want_w, want_b = want_g or want_u, want_gb or want_ub
         b_dtype = (gb_dtype if gb_dtype == ub_dtype or not want_ub else ub_dtype if not want_gb else torch.float32) if want_b else None
-        if dh.dtype == torch.float32:
-            g, db = _C.gated_grad(dh, pre, None, b_dtype)
-            if want_x:
-                dx = _C.linear_grad_input(g, w_back, scale[:2 * f], x2.shape[1])
-            if want_w:
-                dw, _ = _C.linear_grad_weight(g, x2, scale[:2 * f])
-            fv = f
-        else:
-            g, db = _C.gated_grad(dh, pre, scale, b_dtype)
-            fv = g.shape[1] // 2
-            one = scale[2 * fv:]
-            if want_x:
-                dx = _C.ternary_linear_tiled_forward(g, w_back, one, None, 2 * fv, k)
-            if want_w:
-                dw = _C.linear_grad_weight_16(g, x2, one, dh.dtype if w_dtype == dh.dtype else torch.float32)
+        g, db = _C.gated_grad(dh, pre, scale, b_dtype)
+        fp = g.shape[1] // 2
+        one = scale[2 * fp:]
         if want_x:
-            dx = dx[:, :k].contiguous().reshape(*lead, k).to(ctx.x_dtype)
+            dx = _C.ternary_linear_tiled_forward(g, w_back, one, None, 2 * fp, k).reshape(*lead, k).to(ctx.x_dtype)
+        if want_w and dh.dtype == torch.float32:
+            dw, _ = _C.linear_grad_weight(g, x2, one)
+        elif want_w:
+            dw = _C.linear_grad_weight_16(g, x2, one, dh.dtype if w_dtype == dh.dtype else torch.float32)
         if want_w:
-            dg, du = (t.to(w_dtype).contiguous() for t in (dw[:f, :k], dw[fv:fv + f, :k]))
+            dg, du = (t.to(w_dtype).contiguous() for t in (dw[:f, :k], dw[fp:fp + f, :k]))
         if want_b:
             dgb, dub = db[:f].to(gb_dtype) if want_gb else None, db[f:].to(ub_dtype) if want_ub else None
         return dx, dg if want_g else None, du if want_u else None, dgb, dub, None, None, None
@@ -139,7 +130,5 @@ def ternary_gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate
     kinds = (torch.float32, torch.float16, torch.bfloat16)
     if x.dtype not in kinds or gate_weight.dtype not in kinds or any(b is not None and b.dtype not in kinds for b in (gate_bias, up_bias)):
         raise RuntimeError("x, weights and biases must be float32, float16 or bfloat16")
-    if gate_weight.shape[0] < 2 and x.dtype == torch.float32 and not torch.is_autocast_enabled("cuda"):
-        raise RuntimeError("fp32 rows need at least 2 output features")
     keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate_weight, up_weight, gate_bias, up_bias))
     return _GatedLinear.apply(x, gate_weight, up_weight, gate_bias, up_bias, threshold_factor, per_channel, keep)
