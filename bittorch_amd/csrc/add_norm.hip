@@ -446,7 +446,7 @@ int launch_column_sum(const float* parts, int64_t n, int64_t K, void* out, int o
 
 // Waves to a row: a lane holds at most three pieces (four of the longest rows), with more of them the registers of a row's operands
 // and sums run over.
-static bool grad_any(int64_t K) { return K < 8 || K > 16384; }
+static bool grad_any(int64_t K) { return K < 8 || K > 16384 || option(OPT_ROWOP_GENERIC); }
 static int grad_waves(int64_t K) { return K <= 3 * 512 ? 1 : K <= 6 * 512 ? 2 : K <= 12 * 512 ? 4 : 8; }
 // Rows of `parts`: workgroups of the gradient kernel, one for each compute unit at most (their sums are K floats each)
 static int64_t grad_parts(int64_t B, int64_t K) {

@@ -107,6 +107,14 @@ def _check_gated(x: Tensor, gate: Tensor, up: Tensor, gate_bias: Optional[Tensor
     check(all(t is None or t.device == x.device for t in (gate, up, gate_bias, up_bias)), "All tensors must be on one device")
 
 
+def _one_by_one(x, gate, up, gate_bias, up_bias, threshold_factor, per_channel) -> Tensor:
+    from ..nn.ternary_linear_cuda import TernaryLinearCUDAFunction
+
+    _check_gated(x, gate, up, gate_bias, up_bias)
+    g, u = (TernaryLinearCUDAFunction.apply(x, w, b, threshold_factor, per_channel, None) for w, b in ((gate, gate_bias), (up, up_bias)))
+    return F.silu(g) * u
+
+
 def ternary_gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate_bias: Optional[Tensor] = None,
                          up_bias: Optional[Tensor] = None, threshold_factor: float = 0.05, per_channel: bool = True) -> Tensor:
     """``silu(linear(x, T(gate_weight), gate_bias)) * linear(x, T(up_weight), up_bias)`` with ``T(w) = ternary_quantize(w)`` times its
@@ -118,6 +126,8 @@ def ternary_gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate
     if x.is_cuda:
         from .. import _C
 
+        if _C._N.generic_kernel_asked():  # (BITTORCH_KERNEL=generic: the layers one by one, which know that switch)
+            return _one_by_one(x, gate_weight, up_weight, gate_bias, up_bias, threshold_factor, per_channel)
         h = _C._N.gated_linear(x, gate_weight, up_weight, gate_bias, up_bias, threshold_factor, per_channel)
         if h is not None:
             return h

@@ -106,6 +106,26 @@ def test_gradient_is_the_formula(rows, k, dt, rt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,rt", TYPES)
+def test_shape_generic_kernels(dt, rt):
+    """Option ROWOP_GENERIC: the element-wise kernels at a size that the others serve; the same forward bits."""
+    from _util import set_option
+    ops = _ops()
+    x, res, w, ds, dy = _inputs(70, 520, dt, rt, seed=4)
+    want = ops.add_rmsnorm(x, res, w, EPS, quantize=True, return_rowsum=True)
+    set_option("ROWOP_GENERIC", "1")
+    for a, b in zip(ops.add_rmsnorm(x, res, w, EPS, quantize=True, return_rowsum=True), want):
+        assert torch.equal(a, b)
+    leaves = [t.requires_grad_() for t in (x, res, w)]
+    s, y = ops.add_rmsnorm(*leaves, EPS)
+    (d, d_tol), (dw, dw_tol) = _reference_grads(s.detach(), w.detach(), ds, dy)
+    dx, dr, dwt = torch.autograd.grad((s, y), leaves, (ds, dy))
+    _assert_within(dx, d, d_tol, "dx")
+    _assert_within(dr, d, d_tol, "dresidual")
+    _assert_within(dwt, dw, dw_tol, "dweight")
+
+
+@pytest.mark.gpu
 def test_gradient_of_parts_of_the_call():
     """One output used, one input wanted, no weight, an fp32 weight, no residual."""
     ops = _ops()

@@ -394,6 +394,23 @@ def test_native_and_python_calls_agree(dt, wt, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_generic_kernels_when_asked_for(dt, monkeypatch):
+    """BITTORCH_KERNEL=generic: the shape-generic kernels of the layers, one by one, and the same values."""
+    x, wg, wu, bg, bu, dh = _inputs(20, 72, 40, dt, seed=12)
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    want = _gated(*leaves)
+    grads = torch.autograd.grad(want, leaves, dh)
+    monkeypatch.setenv("BITTORCH_KERNEL", "generic")
+    got = _gated(*leaves)
+    # the projections, silu and their product rounded one by one; the scales and the gradients of the projections too
+    tol = 4 * torch.finfo(dt).eps / 2 + 1e-6
+    assert _norm_error(got, want.double()) <= tol
+    for a, b in zip(torch.autograd.grad(got, leaves, dh), grads):
+        assert _norm_error(a, b.double()) <= tol
+
+
+@pytest.mark.gpu
 def test_agrees_with_two_layers_and_their_product():
     """The training form beside the layers that it stands for: the same codes and scales, so the same values up to their roundings."""
     import bittorch_amd as bt
