@@ -156,6 +156,18 @@ def test_gradient_of_parts_of_the_call():
     _assert_within(torch.autograd.grad((s, y), x1, (ds, dy))[0], d, tol, "with int8 rows")
     s, q, s_x = ops.add_rmsnorm(x1, res, w, EPS, store=False, quantize=True)
     assert torch.equal(torch.autograd.grad(s, x1, ds)[0], ds)
+    # one tensor as both: its gradient is the sum of the two, which are one tensor
+    both = x.clone().requires_grad_()
+    s, y = ops.add_rmsnorm(both, both, w, EPS)
+    twice, = torch.autograd.grad((s, y), both, (ds, dy))
+    x2, r2 = x.clone().requires_grad_(), x.clone().requires_grad_()
+    once = torch.autograd.grad(ops.add_rmsnorm(x2, r2, w, EPS), (x2, r2), (ds, dy))
+    assert torch.equal(once[0], once[1]) and torch.equal(twice, once[0] + once[1])
+    row = res[:1].clone().requires_grad_()  # (a broadcast stream)
+    s, y = ops.add_rmsnorm(x, row.expand_as(x), w, EPS)
+    got, = torch.autograd.grad((s, y), row, (ds, dy))
+    full = row.detach().expand_as(x).contiguous().requires_grad_()
+    assert torch.equal(got, torch.autograd.grad(ops.add_rmsnorm(x, full, w, EPS), full, (ds, dy))[0].sum(0, keepdim=True))
     # a second derivative is refused
     s, y = ops.add_rmsnorm(x1, res, w, EPS)
     dx, = torch.autograd.grad(y, x1, dy, create_graph=True)

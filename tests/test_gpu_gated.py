@@ -220,6 +220,30 @@ def test_quantizer_settings_and_rows_without_weights(dt):
 
 
 @pytest.mark.gpu
+def test_projections_beyond_two_to_the_31_dwords():
+    """70000 rows of 22000 features: the kept projections pass 2^31 dwords and 2^33 bytes, G 2^31 elements."""
+    announce("gated", 70000, 64, 22000)
+    from bittorch_amd import _C
+    rows, k, f = 70000, 64, 22000
+    g = torch.Generator().manual_seed(13)
+    wg, wu = ((torch.randn(f, k, generator=g) * 0.05).bfloat16().cuda() for _ in range(2))
+    pick = [0, 1, 34999, 65535, 65536, rows - 2, rows - 1]
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[pick] = torch.randn(7, k, generator=g).bfloat16().cuda()
+    w, w_back, scale, _ = _C.gated_weights(wg, wu, back=True)
+    h, pre, _ = _C.ternary_gated_forward(x, w, scale, None, f, True)
+    few_h, few_pre, _ = _C.ternary_gated_forward(x[pick], w, scale, None, f, True)  # (one stage of k: the same sums in tiles of any size)
+    assert torch.equal(h[pick], few_h) and torch.equal(pre[pick], few_pre) and not h[2:34999].any()
+    dh = torch.zeros_like(h)
+    dh[pick] = torch.randn(7, f, generator=g).bfloat16().cuda()
+    grad, db = _C.gated_grad(dh, pre, scale, torch.float32)
+    few, few_db = _C.gated_grad(dh[pick], few_pre, scale, torch.float32)
+    assert torch.equal(grad[pick], few) and not grad[2:34999].any()
+    # (seven terms other than zero, added in another order)
+    assert bool(((db - few_db).abs() <= 8 * U * 7 * few_db.abs().clamp(min=dh.abs().max().float())).all())
+
+
+@pytest.mark.gpu
 def test_parts_of_the_call():
     """One bias, one leaf, one master twice, and inputs that lie in other ways."""
     x, wg, wu, bg, bu, dh = _inputs(48, 264, 72, torch.bfloat16, seed=4)
