@@ -302,7 +302,7 @@ __global__ __launch_bounds__(512) void add_rmsnorm_grad_kernel(AddNormGradParams
 #pragma unroll
         for (int i = 0; i < ITERS; i++) to.g[i] = load_raw8<RT>(dS, row * K + piece_at(at(i), K));
     };
-    constexpr bool AHEAD = ITERS < 4 || RT != BT_F32;  // (registers for a second row)
+    constexpr bool AHEAD = ITERS + (RAG ? 1 : 0) < (RT == BT_F32 ? 4 : 5);  // (registers for a second row)
     int turn = 0;
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     Row next;

@@ -261,11 +261,12 @@ static void launch_gated_quantize(const GatedQuantizeParams& p, hipStream_t st) 
         else hipLaunchKernelGGL((gated_quantize_kernel<DT, IT, true>), grid, block, 0, st, p);              \
         return;                                                                                            \
     }
-    BT_GQ(1) BT_GQ(2) BT_GQ(3) BT_GQ(5) BT_GQ(8) BT_GQ(16)
+    BT_GQ(1) BT_GQ(2) BT_GQ(3) BT_GQ(5) BT_GQ(8)
 #undef BT_GQ
+    hipLaunchKernelGGL((gated_quantize_kernel<DT, 16, false>), grid, block, 0, st, p);
 }
 // Rows that a wave holds, with a scale each; the others are quantized by bt_quantize_pack and their bytes put in place
-static bool gated_quantizes(int64_t K, bool per_channel) { return per_channel && K >= 8 && K <= 8192; }
+static bool gated_quantizes(int64_t K, bool per_channel) { return per_channel && K >= 8 && K <= (K % 8 == 0 ? 8192 : 4096); }
 
 // ---- one row on the masters, without a copy of them -------------------------------------------------------------------------
 

@@ -14,7 +14,7 @@ DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 # long enough for two groups of waves
 # a feature too long for the registers of a wave
 SHAPES = [(1, 8, 2), (3, 1, 1), (3, 7, 5), (2, 3, 9), (5, 1, 24), (1, 640, 48), (17, 100, 37), (64, 512, 256), (65, 1001, 33), (129, 520, 272), (300, 1100, 546),
-          (40, 2560, 688), (1000, 264, 520), (35, 4096, 64), (33, 5003, 40),
+          (40, 2560, 688), (1000, 264, 520), (35, 4096, 64), (33, 4093, 40), (9, 5003, 20),
           (20, 8192, 48), (17, 8200, 33)]
 
 
