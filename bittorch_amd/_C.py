@@ -892,9 +892,10 @@ def gated_masters_serves(rows: int, masters: Tensor, per_channel: bool = True, a
 
 
 def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, up_bias: Optional[Tensor] = None,
-                  threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, back: bool = False):
+                  threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, back: bool = False, ranged: bool = False):
     """The operands of the gated pair, of two masters ``[F, K]`` quantized as :func:`ternary_quantize_pack` does: ``(W_pairs, W_back,
-    scale, bias)`` as ``bt_gated_quantize`` makes them; ``back``: with the copy for the input's gradient (otherwise None)."""
+    scale, bias)`` as ``bt_gated_quantize`` makes them; ``back``: with the copy for the input's gradient (otherwise None); ``ranged``: with
+    ``bt_gated_range``, for the gradient of fp16 rows."""
     masters, wdt, biases, bdt = _gated_operands(gate, up, gate_bias, up_bias, as_half)
     (F, K), dev = gate.shape, gate.device
     Fp = (F + 15) // 16 * 16
@@ -907,6 +908,8 @@ def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, 
         _status(_L.bt_gated_quantize(masters[0].data_ptr(), masters[1].data_ptr(), wdt, F, K, float(threshold_factor), int(bool(per_channel)),
                                      _ptr(biases[0]), _ptr(biases[1]), bdt, w.data_ptr(), _ptr(w_back), scale.data_ptr(), _ptr(bias), _ptr(ws),
                                      0 if ws is None else ws.numel(), _stream(gate)))
+        if ranged:
+            _status(_L.bt_gated_range(scale.data_ptr(), F, _stream(gate)))
     return w, w_back, scale, bias
 
 
@@ -934,14 +937,14 @@ def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optio
 
 
 def gated_grad(dH: Tensor, pre: Tensor, scale: Tensor, bias_dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Optional[Tensor]]:
-    """Gradient of ``silu(gate) * up`` in both projections times their scales, ``[B, 2 Fp]`` (``pre`` as :func:`ternary_gated_forward` kept
+    """Gradient of ``silu(gate) * up`` in both projections times their scales over ``scale``'s last entry, ``[B, 2 Fp]`` (``pre`` as :func:`ternary_gated_forward` kept
     it, or for fp32 rows ``[gate | up]`` ``[B, 2 Fp]``); with ``bias_dtype`` also its sums over the rows ``[2 F]``, without scales."""
     _check(dH.dim() == 2 and dH.numel() > 0 and dH.dtype in _DT, "dH must be 2D float32, float16 or bfloat16")
     B, F = dH.shape
     Fp = (F + 15) // 16 * 16
     kept = (torch.float32, (B, 2 * Fp)) if dH.dtype == torch.float32 else (torch.int32, (B, Fp // 2 * 3))
     _check((pre.dtype, pre.shape) == kept and pre.is_contiguous(), "the projections must be those that the forward kept")
-    _check(scale.dtype == torch.float32 and scale.numel() >= 2 * Fp and scale.is_contiguous(), "scale must be fp32 with an entry for each padded feature")
+    _check(scale.dtype == torch.float32 and scale.numel() == 2 * Fp + 1 and scale.is_contiguous(), "scale must be that of gated_weights")
     _check(_all_cuda(dH, pre, scale), "All tensors must be CUDA")
     dH = dH.contiguous()
     G = torch.empty((B, 2 * Fp), dtype=dH.dtype, device=dH.device)

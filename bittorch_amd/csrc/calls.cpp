@@ -41,8 +41,8 @@ namespace {
     X(bt_ternary_linear_tensor_core_forward) X(bt_quantize_pack) X(bt_ternary_linear_grad_input) X(bt_linear_grad_weight)      \
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
     X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
-    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_ternary_gated_forward) X(bt_gated_grad)                \
-    X(bt_gated_grad_workspace_bytes) X(bt_gated_masters_serves) X(bt_gated_masters_forward)
+    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_range)                    \
+    X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_workspace_bytes) X(bt_gated_masters_serves) X(bt_gated_masters_forward)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     BT_FUNCTIONS(X)
@@ -722,6 +722,7 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
              data_of(gate_bias), data_of(up_bias), gate_bias ? tag_of(gate_bias) : tag_of(up_bias), (uint8_t*)w.data_ptr(),
              want_back ? (uint8_t*)o.w_back.data_ptr() : nullptr, scale_at, bias_at, ws.ptr(), ws.size(), st);
     }
+    if (keep && x.scalar_type() == at::kHalf) call(lib.bt_gated_range, scale_at, F, st);
     o.h = output(with_last(x, F), x.scalar_type(), x);
     if (fp32) o.pre = output({B, 2 * Fp}, at::kFloat, x);
     else if (keep) o.pre = output({B, Fp / 2 * 3}, at::kInt, x);

@@ -13,7 +13,9 @@
 // order.  One pass (gated_grad_kernel) makes G = [a_g dg | a_u du] of dh and the kept projections, rounded once to 16 bits as an operand
 // of the matrix cores; it serves both products behind it: dx = G [T_g; T_u] on a second tiled copy of the codes, in which the contraction
 // runs over the output features, by the forward's kernel, and dW = G^T x by the weight gradient's (grad_w16.hip).  a times dg, not
-// dg, is what is rounded, so that neither product has a scale of its own.
+// dg, is what is rounded, so that neither product has a scale for each feature.  For fp16 both are divided by a power of two above every a
+// (gated_range_kernel), which the products multiply their sums by: fp16 has no range for a (0.01 where dg is 1e-4 would leave 4 bits of it),
+// and so G keeps what fp16 keeps of dg.
 // fp32 rows: the same steps on the fp32 kernels and the same copies, the projections stored in fp32 and h by the SwiGLU row kernel.  (On the
 // packed bytes as rows the fp32 products take longer: 4096 x 4096 x 768 forward 74 us, 68 on the copy, its transpose 89 and 77.)
 //
@@ -40,7 +42,7 @@ struct GatedWeightsParams {
     int64_t F, Fp, K, Kb;
     uint8_t* pairs;           // forward: tiled copy in pair order of [gate | up], 2 Fp columns
     uint8_t* back;            // backward: tiled copy of the transpose: K columns, contraction over 2 Fp
-    float* scale;             // [2 Fp + 1], the last one 1 (the scale of products that have none)
+    float* scale;             // [2 Fp + 1], the last one what products of G multiply by: 1, or gated_range_kernel's
     float* bias;              // [2 Fp] or null
     uint32_t n_pairs, n_back;          // workgroups of each part, in this order; behind them those of the vectors
     uint32_t steps, back_steps;        // 64-wide steps of the two tiled copies
@@ -145,7 +147,7 @@ constexpr int master_storage(int dt) { return dt == BT_F32_AS_F16 ? BT_F32 : dt;
 // registers (ITERS pieces of eight values a lane, K <= 512 ITERS), reduces its absolute maximum, and puts the codes of four k to a byte into
 // LDS, from where they leave in each layout: the pairs' tile is one run of memory, its dwords are LDS's; a thread turns the codes of four
 // k into 16 bytes of the transpose.  The quantizer's arithmetic is that of quantize_pack.hip, on the same values.  Bound by the masters,
-// read once: 2 x 6912 x 2560 bf16 (71 MB) takes 18 us, two passes of the quantizer and the copy of their bytes 34.
+// read once: 2 x 6912 x 2560 bf16 (71 MB) takes 20 us, two passes of the quantizer and the copy of their bytes 34.
 template <int DT, int ITERS, bool RAG>
 __global__ __launch_bounds__(512) void gated_quantize_kernel(GatedQuantizeParams p) {
     constexpr int ST = master_storage(DT), PITCH = ITERS * 128 + 4, RPW = 2;
@@ -268,6 +270,21 @@ static void launch_gated_quantize(const GatedQuantizeParams& p, hipStream_t st) 
 // Rows that a wave holds, with a scale each; the others are quantized by bt_quantize_pack and their bytes put in place
 static bool gated_quantizes(int64_t K, bool per_channel) { return per_channel && K >= 8 && K <= (K % 8 == 0 ? 8192 : 4096); }
 
+// scale[n] = the power of two 2^e with scale[i] in [0, 2^e] for all i < n.  One workgroup, its time is its launch.
+__global__ __launch_bounds__(1024) void gated_range_kernel(float* scale, int n) {
+    __shared__ float part[16];
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, scale[i]);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 0; i < 16; i++) m = fmaxf(m, part[i]);
+    // the exponent above m's, kept where 2^e and 2^-e are ordinary numbers (an infinite m: the largest, of a gradient that is none)
+    const int e = (int)(__builtin_bit_cast(uint32_t, m) >> 23) - 126;
+    scale[n] = __builtin_bit_cast(float, (uint32_t)(127 + (e < -125 ? -125 : e > 125 ? 125 : e)) << 23);
+}
+
 // ---- one row on the masters, without a copy of them -------------------------------------------------------------------------
 
 struct GatedMastersParams {
@@ -387,7 +404,7 @@ static bool masters_serve(int64_t B, int64_t K, int w_dtype, bool per_channel) {
 struct GatedGradParams {
     const void* dH;       // [B, F]
     const void* pre;      // 16-bit rows: [B, 3 Fp / 2] dwords, column pairs of gate and up in turn in 24 bits; fp32 rows: [B, 2 Fp], gate | up
-    const float* scale;   // [2 Fp]
+    const float* scale;   // [2 Fp + 1], the last one a power of two
     void* G;              // [B, 2 Fp]
     float* parts;         // [gridDim.y, 2 F] sums of dg | du, or null
     int64_t B, rows;      // rows: of a workgroup
@@ -410,10 +427,11 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
     if (k >= Fp) return;
     const int64_t first = (int64_t)blockIdx.y * p.rows, last = std::min(first + p.rows, p.B);
     float ag[8], au[8], bg[8], bu[8];
+    const float unit = __fdiv_rn(1.0f, p.scale[2 * Fp]);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        ag[e] = p.scale[k + e];
-        au[e] = p.scale[Fp + k + e];
+        ag[e] = p.scale[k + e] * unit;
+        au[e] = p.scale[Fp + k + e] * unit;
         bg[e] = bu[e] = 0.0f;
     }
 #pragma unroll 2
@@ -461,6 +479,7 @@ __global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p
     if (k >= Fp) return;
     const int64_t first = (int64_t)blockIdx.y * p.rows, last = std::min(first + p.rows, p.B);
     float bg = 0.0f, bu = 0.0f;
+    const float unit = __fdiv_rn(1.0f, p.scale[2 * Fp]);
     for (int64_t row = first; row < last; row++) {
         float dg = 0.0f, du = 0.0f;
         if (k < F) {
@@ -476,8 +495,8 @@ __global__ __launch_bounds__(64) void gated_grad_narrow_kernel(GatedGradParams p
         }
         bg += dg;
         bu += du;
-        store_elem<DT>(p.G, row * 2 * Fp + k, dg * p.scale[k]);
-        store_elem<DT>(p.G, row * 2 * Fp + Fp + k, du * p.scale[Fp + k]);
+        store_elem<DT>(p.G, row * 2 * Fp + k, dg * (p.scale[k] * unit));
+        store_elem<DT>(p.G, row * 2 * Fp + Fp + k, du * (p.scale[Fp + k] * unit));
     }
     if (!p.parts || k >= F) return;
     p.parts[(int64_t)blockIdx.y * 2 * F + k] = bg;
@@ -566,6 +585,16 @@ extern "C" int bt_gated_quantize(const void* gate, const void* up, int w_dtype, 
     p.n_pairs = (uint32_t)(2 * steps * ceil_div(Fp, 256));
     p.n_back = W_back ? (uint32_t)(ceil_div(K, 16) * ceil_div(back_steps, 16)) : 0;
     hipLaunchKernelGGL(gated_weights_kernel, dim3(p.n_pairs + p.n_back + (unsigned)(2 * Fp / 256 + 1)), dim3(256), 0, st, p);
+    return check_launch(who);
+}
+
+extern "C" int bt_gated_range(float* scale, int64_t F, void* stream) {
+    const char* who = "bt_gated_range";
+    if (!scale || F <= 0 || F >= (1ll << 23)) {
+        set_error("%s: null pointer, or F not between 1 and 2^23", who);
+        return BT_ERR_INVALID;
+    }
+    hipLaunchKernelGGL(gated_range_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, scale, (int)(2 * padded(F)));
     return check_launch(who);
 }
 

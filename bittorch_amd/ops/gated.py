@@ -46,7 +46,7 @@ class _GatedLinear(torch.autograd.Function):
             h = _C.gated_masters_forward(x2, gate, up, gate_bias, up_bias, threshold_factor, as_half)
             return h.reshape(*x.shape[:-1], f)
         w, w_back, scale, bias = _C.gated_weights(gate, up, gate_bias, up_bias, threshold_factor, per_channel, as_half,
-                                                  back=keep and ctx.needs_input_grad[0])
+                                                  back=keep and ctx.needs_input_grad[0], ranged=keep and x.dtype == torch.float16)
         if x.dtype == torch.float32:
             # (the fp32 kernel of the masters' gradient takes four columns and more)
             x2 = F.pad(x2, (0, 4 - k)) if k < 4 else x2.contiguous()

@@ -254,6 +254,7 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *       W_back   (optional) bt_tiled_weights_bytes(K, 2 Fp) bytes: the decode-tiled copy of their transpose, a layer with K outputs
  *                and 2 Fp inputs, for bt_ternary_linear_tiled_forward on the gradient G;
  *       scale    [2 Fp + 1]: both layers' scales, zeros behind each, and a 1; bias [2 Fp] or NULL.
+ *     bt_gated_range puts a power of two that no scale exceeds in the place of that 1.
  *     fp32 rows read W_pairs through bt_ternary_linear_tiled_forward (BT_EPI_NATURAL_FROM_PAIRS) and bt_swiglu.
  *     workspace: at least bt_gated_quantize_workspace_bytes(F,K,per_channel) bytes.
  *   bt_ternary_gated_forward: fp16 / bf16 rows X [B,K]; where K % 8 != 0 or X is not 16-byte aligned, X_padded [B, K rounded up to 8] takes
@@ -262,7 +263,8 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *     of g's columns 2 i and 2 i + 1 and u's, low bits first.
  *   bt_gated_masters_forward: H [F] of one row X [K] (any x_dtype) straight from the masters, quantized as they are read, with a scale for
  *     each feature; bt_gated_masters_serves says whether a call of B rows is one of those.
- *   bt_gated_grad: G [B, 2 Fp] in dtype = d(H . dH)/d[g | u], each half times its scale.  16-bit dtype: pre as above; BT_F32: [g | u]
+ *   bt_gated_grad: G [B, 2 Fp] in dtype = d(H . dH)/d[g | u], each half times its scale over scale[2 Fp], which both products of G
+ *     multiply by (fp16: with bt_gated_range, so that G has fp16's range for the gradient alone).  16-bit dtype: pre as above; BT_F32: [g | u]
  *     [B, 2 Fp] fp32.  dBias (optional) [2 F] in bias_dtype: the sums over the rows without scales; with it a workspace of
  *     bt_gated_grad_workspace_bytes(B,F).
  */
@@ -270,6 +272,7 @@ size_t bt_gated_quantize_workspace_bytes(int64_t F, int64_t K, int per_channel);
 int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, int64_t K, double threshold_factor, int per_channel,
                       const void* gate_bias, const void* up_bias, int bias_dtype, uint8_t* W_pairs, uint8_t* W_back,
                       float* scale, float* bias, void* workspace, size_t workspace_bytes, void* stream);
+int bt_gated_range(float* scale, int64_t F, void* stream);
 int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
                              void* pre, int64_t B, int64_t F, int64_t K, void* stream);
 int bt_gated_masters_serves(int64_t B, int64_t K, int w_dtype, int per_channel);

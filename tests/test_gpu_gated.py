@@ -3,6 +3,8 @@
 The 16-bit gradient has an operand of its own, ``G`` (the gradient of both projections times their scales, rounded to 16 bits): it is
 checked element by element against the formula, and both products against 64-bit products of that very ``G``.
 """
+import math
+
 import pytest
 import torch
 
@@ -521,3 +523,51 @@ def test_refusals_on_the_gpu():
     with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
         _gated(x.double(), w, w)
     assert _gated(x, w[:1], w[:1]).shape == _gated(x.half(), w[:1], w[:1]).shape == (4, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("autocast", [False, True])
+@pytest.mark.parametrize("per_channel", [True, False])
+@pytest.mark.parametrize("rows,k,f", [(3, 96, 5), (70, 512, 340), (65, 333, 200)])
+def test_small_gradients_of_fp16_rows(rows, k, f, per_channel, autocast):
+    """Incoming gradients near fp16's smallest numbers, scales of 1/100: G has to keep what fp16 keeps of them without the scale."""
+    announce("gated small", rows, k, f, per_channel, autocast)
+    g = torch.Generator().manual_seed(rows + f)
+    x, dh = torch.randn(rows, k, generator=g).half().cuda(), (torch.randn(rows, f, generator=g) * 2.0 ** -12).half().cuda()
+    wg, wu = ((torch.randn(f, k, generator=g) * 0.003).half().cuda() for _ in range(2))
+    ref = _Reference(x, wg, wu, None, None, dh, per_channel=per_channel)
+    leaves = [(t.float() if autocast else t).requires_grad_() for t in (x, wg, wu)]
+    with torch.autocast("cuda", enabled=autocast):
+        h = _gated(*leaves, per_channel=per_channel)
+    assert h.dtype == torch.float16
+    dx, dwg, dwu = torch.autograd.grad(h, leaves, dh)
+    # half a step of G: 2^-11 of it, and 2^-25 among the subnormal numbers, in units of at most twice the largest scale
+    half, chain = 2.0 ** -11, lambda n: U * 2 * (3 * n / 32 + 80)
+    least = 2.0 ** -25 * 2 * float(max(ref.ag.max(), ref.au.max()))
+    parts = [(ref.dg, ref.tol_dg, ref.ag, ref.tg), (ref.du, ref.tol_du, ref.au, ref.tu)]
+    off = lambda n: [(tol * (1 + half) + (half + chain(n)) * v.abs()) * a + least for v, tol, a, _ in parts]
+    want = sum((v * a) @ t for v, _, a, t in parts)
+    tol = sum(o @ t.abs() for o, (_, _, _, t) in zip(off(2 * f), parts))
+    # (under autocast dx is rounded to fp16 all the same, and widened)
+    bound = tol + half * (want.abs() + tol) + 2.0 ** -25
+    assert bool(((dx.double() - want).abs() <= bound).all())
+    for got, o, (v, _, a, _) in zip((dwg, dwu), off(rows), parts):
+        want_w, tol_w = (v * a).t() @ ref.x, o.t() @ ref.x.abs()
+        bound = tol_w + half * (want_w.abs() + tol_w) + 2.0 ** -25
+        assert bool(((got.double() - want_w).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f,largest", [(1, 0.7), (16, 1.0), (5000, 0.011), (40, 3e-9), (40, 1e-30), (40, 3e38)])
+def test_range_of_the_scales(f, largest):
+    from bittorch_amd import _C
+    fp = (f + 15) // 16 * 16
+    scale = torch.rand(2 * fp + 1, generator=torch.Generator().manual_seed(f)).mul_(largest * 0.9).cuda()
+    scale[fp // 2] = largest
+    scale[2 * fp] = -1
+    before = scale.clone()
+    _C._status(_C._L.bt_gated_range(scale.data_ptr(), f, _C._stream(scale)))
+    assert torch.equal(scale[:2 * fp], before[:2 * fp])
+    top = float(scale[2 * fp])
+    mantissa, exponent = math.frexp(top)
+    assert mantissa == 0.5 and exponent - 1 == min(125, max(-125, math.frexp(float(before[fp // 2]))[1]))
