@@ -41,8 +41,9 @@ namespace {
     X(bt_ternary_linear_tensor_core_forward) X(bt_quantize_pack) X(bt_ternary_linear_grad_input) X(bt_linear_grad_weight)      \
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
     X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
-    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_range)                    \
-    X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_workspace_bytes) X(bt_gated_masters_serves) X(bt_gated_masters_forward)
+    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_range)                     \
+    X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_weight) X(bt_gated_grad_workspace_bytes)                      \
+    X(bt_gated_masters_serves) X(bt_gated_masters_forward)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     BT_FUNCTIONS(X)
@@ -788,18 +789,19 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         }
         if (want_w) {
             const at::ScalarType dtype = w_dtype == x.scalar_type() ? w_dtype : at::kFloat;
-            at::Tensor dw = output({2 * Fp, Kr}, dtype, x);
+            const int64_t rows = fp32 ? Fp : F;  // of a half
+            at::Tensor dw = output({2 * rows, K}, dtype, x);
             if (fp32) {
-                const Scratch ws(lib.bt_linear_grad_weight_workspace_bytes(B, 2 * Fp, Kr), x);
+                const Scratch ws(lib.bt_linear_grad_weight_workspace_bytes(B, 2 * Fp, K), x);
                 check_status(lib.bt_linear_grad_weight((const float*)g.const_data_ptr(), (const float*)x.const_data_ptr(), one, 1, (float*)dw.data_ptr(),
-                                                       nullptr, B, 2 * Fp, Kr, ws.ptr(), ws.size(), st));
+                                                       nullptr, B, 2 * Fp, K, ws.ptr(), ws.size(), st));
             } else {
                 const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fp, Kr), x);
-                check_status(lib.bt_linear_grad_weight_16(g.const_data_ptr(), x.const_data_ptr(), dt, one, BT_F32, 1, dw.data_ptr(), tag(dtype), B, 2 * Fp, Kr,
-                                                          ws.ptr(), ws.size(), st));
+                check_status(lib.bt_gated_grad_weight(g.const_data_ptr(), x.const_data_ptr(), dt, one, dw.data_ptr(), tag(dtype), B, F, K, ws.ptr(),
+                                                      ws.size(), st));
             }
             for (int i = 0; i < 2; i++)
-                if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * Fp, F).narrow(1, 0, K).to(w_dtype).contiguous();
+                if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * rows, F).to(w_dtype);
         }
         for (int i = 0; i < 2; i++)
             if (w.want[3 + i]) w.grads[3 + i] = db.narrow(0, i * F, F);

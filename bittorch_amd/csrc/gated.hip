@@ -270,7 +270,7 @@ static void launch_gated_quantize(const GatedQuantizeParams& p, hipStream_t st) 
 // Rows that a wave holds, with a scale each; the others are quantized by bt_quantize_pack and their bytes put in place
 static bool gated_quantizes(int64_t K, bool per_channel) { return per_channel && K >= 8 && K <= (K % 8 == 0 ? 8192 : 4096); }
 
-// scale[n] = the power of two 2^e with scale[i] in [0, 2^e] for all i < n.  One workgroup, its time is its launch.
+// scale[n] = the least power of two 2^e with scale[i] < 2^e for all i < n, within 2^-24 .. 2^15.  One workgroup, its time is its launch.
 __global__ __launch_bounds__(1024) void gated_range_kernel(float* scale, int n) {
     __shared__ float part[16];
     float m = 0.0f;
@@ -280,9 +280,9 @@ __global__ __launch_bounds__(1024) void gated_range_kernel(float* scale, int n) 
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int i = 0; i < 16; i++) m = fmaxf(m, part[i]);
-    // the exponent above m's, kept where 2^e and 2^-e are ordinary numbers (an infinite m: the largest, of a gradient that is none)
+    // the exponent above m's, among those of fp16 (the weight gradient's kernel takes its scale in the rows' type)
     const int e = (int)(__builtin_bit_cast(uint32_t, m) >> 23) - 126;
-    scale[n] = __builtin_bit_cast(float, (uint32_t)(127 + (e < -125 ? -125 : e > 125 ? 125 : e)) << 23);
+    scale[n] = __builtin_bit_cast(float, (uint32_t)(127 + (e < -24 ? -24 : e > 15 ? 15 : e)) << 23);
 }
 
 // ---- one row on the masters, without a copy of them -------------------------------------------------------------------------

@@ -33,7 +33,9 @@ struct GradW16Params {
     float* part;          // into [part][tile][accumulator][thread]
     int scale_bcast, scale_dtype;
     const void* scale;    // [N] or one entry
-    void* out;            // [N, K]
+    void* out;            // [N, K]; PADDED: [2 features, cols]
+    int64_t cols;         // PADDED: the output has so many of the K columns,
+    int features;         // and of either half of the N rows so many, one half's behind the other's
 };
 
 // first row and column of a tile of 32 T x 32 T outputs
@@ -47,17 +49,37 @@ __device__ __forceinline__ void grad_w16_tile(uint32_t lin, uint32_t tiles_n, ui
     k0 = (int64_t)tk * (32 * T);
 }
 
-// One row's sums of `count` consecutive columns: each is rounded as the 16-bit product of two matrices would be, scaled and
-// rounded again, what the unfused operations give.
-template <int DT, bool OUT32, int COUNT>
-__device__ __forceinline__ void grad_w16_store(void* out, int64_t at, const float (&sum)[COUNT], float scale) {
+// Output row n's sums of COUNT consecutive columns from k on: each is rounded as the 16-bit product of two matrices would be, scaled and
+// rounded again, what the unfused operations give.  PADDED: N and K are rounded up and the output is not, so that its rows start
+// anywhere and end inside a run.  (An instance of its own: the others' last stage would take 2.5 us longer with it, 300 x 768 x 768 9.6 / 12.2.)
+template <int DT, bool OUT32, bool PADDED, int COUNT>
+__device__ __forceinline__ void grad_w16_store(const GradW16Params& p, int64_t n, int64_t k, const float (&sum)[COUNT], float scale) {
+    typedef u32x4 __attribute__((aligned(2))) vec4_a2;
+    typedef u32x2 __attribute__((aligned(2))) vec2_a2;
+    void* const out = p.out;
+    int64_t at = n * p.K + k;
+    if constexpr (PADDED) {
+        const int half = (int)(p.N >> 1), h = (int)n >= half, f = (int)n - (h ? half : 0);
+        if (f >= p.features) return;
+        at = (int64_t)((h ? p.features : 0) + f) * p.cols + k;
+    }
     const float s16 = round_to_dtype(scale, DT);
     float v[COUNT];
 #pragma unroll
     for (int b = 0; b < COUNT; b++) v[b] = round_to_dtype(__fmul_rn(round_to_dtype(sum[b], DT), s16), DT);
+    if (PADDED && k + COUNT > p.cols) {
+#pragma unroll
+        for (int b = 0; b < COUNT - 1; b++)
+            if (k + b < p.cols) store_elem<OUT32 ? BT_F32 : DT>(out, at + b, v[b]);
+        return;
+    }
     if constexpr (OUT32) {
 #pragma unroll
-        for (int b = 0; b < COUNT; b += 4) *(v4f*)((float*)out + at + b) = v4f{v[b], v[b + 1], v[b + 2], v[b + 3]};
+        for (int b = 0; b < COUNT; b += 4) {
+            const v4f q = {v[b], v[b + 1], v[b + 2], v[b + 3]};
+            if constexpr (PADDED) *(vec4_a2*)((float*)out + at + b) = __builtin_bit_cast(u32x4, q);
+            else *(v4f*)((float*)out + at + b) = q;
+        }
     } else {
         uint32_t d[COUNT / 2];
 #pragma unroll
@@ -66,12 +88,15 @@ __device__ __forceinline__ void grad_w16_store(void* out, int64_t at, const floa
             const uint16_t h16 = DT == BT_F16 ? f32_to_f16_bits(v[2 * b + 1]) : f32_to_bf16_bits(v[2 * b + 1]);
             d[b] = (uint32_t)l16 | (uint32_t)h16 << 16;
         }
-        if constexpr (COUNT == 8) *(u32x4*)((uint16_t*)out + at) = u32x4{d[0], d[1], d[2], d[3]};
-        else *(u32x2*)((uint16_t*)out + at) = u32x2{d[0], d[1]};
+        uint16_t* const to = (uint16_t*)out + at;
+        if constexpr (COUNT == 8 && PADDED) *(vec4_a2*)to = u32x4{d[0], d[1], d[2], d[3]};
+        else if constexpr (COUNT == 8) *(u32x4*)to = u32x4{d[0], d[1], d[2], d[3]};
+        else if constexpr (PADDED) *(vec2_a2*)to = u32x2{d[0], d[1]};
+        else *(u32x2*)to = u32x2{d[0], d[1]};
     }
 }
 
-template <int MODE, bool OUT32, int T>
+template <int MODE, bool OUT32, int T, bool PADDED>
 __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
     constexpr int DT = MODE == MODE_F16 ? BT_F16 : BT_BF16;
     constexpr int SROWS = T == 8 ? 32 : 64;  // rows of a stage
@@ -276,7 +301,7 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         const int64_t n = n0 + (T == 8 ? 128 : 4) * hi + 8 * (4 * g + c);
-        if (n >= p.N || k >= p.K) continue;
+        if (n >= p.N || k >= (PADDED ? p.cols : p.K)) continue;
         float sc[T];
 #pragma unroll
         for (int a = 0; a < T; a++) sc[a] = load_elem_rt(p.scale, p.scale_dtype, p.scale_bcast ? 0 : n + a);
@@ -285,7 +310,7 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
             float v[T];
 #pragma unroll
             for (int b = 0; b < T; b++) v[b] = acc[a][b][c];
-            grad_w16_store<DT, OUT32>(p.out, (n + a) * p.K + k, v, sc[a]);
+            grad_w16_store<DT, OUT32, PADDED>(p, n + a, k, v, sc[a]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -293,7 +318,7 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
 
 // The tiles summed in parts: a thread adds the parts of four of an accumulator row's column blocks, in order, and finishes
 // their 4 x 4 outputs.  Bound by reading the parts.
-template <int MODE, bool OUT32, int T>
+template <int MODE, bool OUT32, int T, bool PADDED>
 __global__ __launch_bounds__(256) void grad_w16_reduce_kernel(GradW16Params p) {
     constexpr int DT = MODE == MODE_F16 ? BT_F16 : BT_BF16;
     constexpr uint32_t H = T / 4;
@@ -313,13 +338,13 @@ __global__ __launch_bounds__(256) void grad_w16_reduce_kernel(GradW16Params p) {
         for (int b = 0; b < 4; b++) sum[b] += src[256 * b];
     }
     const int64_t k = k0 + (T == 8 ? 128 : 4) * lo + 8 * i + 4 * h;
-    if (k >= p.K) return;
+    if (k >= (PADDED ? p.cols : p.K)) return;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         const int64_t n = n0 + (T == 8 ? 128 : 4) * hi + 8 * (4 * g + c) + a;
         if (n >= p.N) continue;
         const float v[4] = {sum[0][c], sum[1][c], sum[2][c], sum[3][c]};
-        grad_w16_store<DT, OUT32>(p.out, n * p.K + k, v, load_elem_rt(p.scale, p.scale_dtype, p.scale_bcast ? 0 : n));
+        grad_w16_store<DT, OUT32, PADDED>(p, n, k, v, load_elem_rt(p.scale, p.scale_dtype, p.scale_bcast ? 0 : n));
     }
 }
 
@@ -375,20 +400,26 @@ static GradW16Plan grad_w16_plan(int64_t M, int64_t N, int64_t K) {
     return best;
 }
 
-template <int MODE, bool OUT32, int T>
+template <int MODE, bool OUT32, int T, bool PADDED>
 static void launch_grad_w16_tiles(const GradW16Params& p, int64_t tail, hipStream_t st) {
-    hipLaunchKernelGGL((grad_w16_kernel<MODE, OUT32, T>), dim3((unsigned)(8 * (p.whole + p.per_xcd_tail))), dim3(256), 0, st, p);
-    if (tail) hipLaunchKernelGGL((grad_w16_reduce_kernel<MODE, OUT32, T>), dim3((unsigned)(T * T / 4 * tail)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((grad_w16_kernel<MODE, OUT32, T, PADDED>), dim3((unsigned)(8 * (p.whole + p.per_xcd_tail))), dim3(256), 0, st, p);
+    if (tail) hipLaunchKernelGGL((grad_w16_reduce_kernel<MODE, OUT32, T, PADDED>), dim3((unsigned)(T * T / 4 * tail)), dim3(256), 0, st, p);
 }
 template <int MODE, bool OUT32>
-static void launch_grad_w16(const GradW16Params& p, const GradW16Plan& plan, hipStream_t st) {
-    if (plan.T == 8) launch_grad_w16_tiles<MODE, OUT32, 8>(p, plan.tail, st);
-    else launch_grad_w16_tiles<MODE, OUT32, 4>(p, plan.tail, st);
+static void launch_grad_w16(const GradW16Params& p, const GradW16Plan& plan, bool padded, hipStream_t st) {
+    if (padded && plan.T == 8) launch_grad_w16_tiles<MODE, OUT32, 8, true>(p, plan.tail, st);
+    else if (padded) launch_grad_w16_tiles<MODE, OUT32, 4, true>(p, plan.tail, st);
+    else if (plan.T == 8) launch_grad_w16_tiles<MODE, OUT32, 8, false>(p, plan.tail, st);
+    else launch_grad_w16_tiles<MODE, OUT32, 4, false>(p, plan.tail, st);
 }
 
 }  // namespace bt
 
 using namespace bt;
+
+static int grad_w16(const char* who, const void* dY, const void* X, int dtype, const void* scale, int scale_dtype, int64_t scale_len, void* dW,
+                    int out_dtype, int64_t M, int64_t N, int64_t K, int64_t cols, int64_t features, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 extern "C" size_t bt_linear_grad_weight_16_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
@@ -399,7 +430,25 @@ extern "C" size_t bt_linear_grad_weight_16_workspace_bytes(int64_t M, int64_t N,
 extern "C" int bt_linear_grad_weight_16(const void* dY, const void* X, int dtype, const void* scale, int scale_dtype,
                                         int64_t scale_len, void* dW, int out_dtype, int64_t M, int64_t N, int64_t K,
                                         void* workspace, size_t workspace_bytes, void* stream) {
-    const char* who = "bt_linear_grad_weight_16";
+    return grad_w16("bt_linear_grad_weight_16", dY, X, dtype, scale, scale_dtype, scale_len, dW, out_dtype, M, N, K, K, N / 2, workspace,
+                    workspace_bytes, stream);
+}
+
+extern "C" int bt_gated_grad_weight(const void* G, const void* X, int dtype, const float* factor, void* dW, int out_dtype, int64_t B, int64_t F,
+                                    int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "bt_gated_grad_weight";
+    if (F <= 0 || K <= 0 || F >= (1ll << 23) || K >= (1ll << 23)) {
+        set_error("%s: F and K between 1 and 2^23 (F=%lld, K=%lld)", who, (long long)F, (long long)K);
+        return BT_ERR_INVALID;
+    }
+    const int64_t Fp = ceil_div(F, 16) * 16;
+    return grad_w16(who, G, X, dtype, factor, BT_F32, 1, dW, out_dtype, B, 2 * Fp, ceil_div(K, 8) * 8, K, F, workspace, workspace_bytes, stream);
+}
+
+static int grad_w16(const char* who, const void* dY, const void* X, int dtype, const void* scale, int scale_dtype, int64_t scale_len, void* dW,
+                    int out_dtype, int64_t M, int64_t N, int64_t K, int64_t cols, int64_t features, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    const bool padded = cols != K || 2 * features != N;
     if (!dY || !X || !scale || !dW || M <= 0 || N <= 0 || K <= 0) {
         set_error("%s: null pointer or empty shape", who);
         return BT_ERR_INVALID;
@@ -413,7 +462,8 @@ extern "C" int bt_linear_grad_weight_16(const void* dY, const void* X, int dtype
         return BT_ERR_INVALID;
     }
     // (32-bit byte offsets span a stage's 32 rows and the columns of a last tile)
-    if (N % 8 || K % 8 || N >= (1ll << 24) || K >= (1ll << 24) || (((uintptr_t)dY) | ((uintptr_t)X) | ((uintptr_t)dW)) % 16 ||
+    if (N % 8 || K % 8 || N >= (1ll << 24) || K >= (1ll << 24) || (((uintptr_t)dY) | ((uintptr_t)X)) % 16 ||
+        ((uintptr_t)dW) % (padded ? dtype_size(out_dtype) : 16) ||
         ((uintptr_t)scale) % dtype_size(scale_dtype) || ceil_div(N, 128) * ceil_div(K, 128) >= (1ll << 28) || M >= (1ll << 40) / std::max(N, K)) {
         set_error("%s: N and K must be multiples of 8 below 2^24, buffers 16-byte aligned", who);
         return BT_ERR_INVALID;
@@ -425,7 +475,7 @@ extern "C" int bt_linear_grad_weight_16(const void* dY, const void* X, int dtype
     }
     const GradW16Plan plan = grad_w16_plan(M, N, K);
     GradW16Params p = {};
-    p.G = (const uint16_t*)dY; p.X = (const uint16_t*)X; p.M = M; p.N = N; p.K = K; p.out = dW;
+    p.G = (const uint16_t*)dY; p.X = (const uint16_t*)X; p.M = M; p.N = N; p.K = K; p.out = dW; p.cols = cols; p.features = (int)features;
     p.scale = scale; p.scale_dtype = scale_dtype; p.scale_bcast = scale_len == 1 ? 1 : 0;
     p.tiles_n = (int)ceil_div(N, 32 * plan.T); p.tiles_k = (int)ceil_div(K, 32 * plan.T);
     p.whole = (int)ceil_div(plan.tiles - plan.tail, 8);
@@ -435,11 +485,11 @@ extern "C" int bt_linear_grad_weight_16(const void* dY, const void* X, int dtype
     p.per_xcd_tail = (int)(plan.long_first ? 2 * ceil_div(plan.tail, 8) : ceil_div(plan.tail * plan.splits, 8));
     hipStream_t st = (hipStream_t)stream;
     if (dtype == BT_F16) {
-        if (out_dtype == BT_F32) launch_grad_w16<MODE_F16, true>(p, plan, st);
-        else launch_grad_w16<MODE_F16, false>(p, plan, st);
+        if (out_dtype == BT_F32) launch_grad_w16<MODE_F16, true>(p, plan, padded, st);
+        else launch_grad_w16<MODE_F16, false>(p, plan, padded, st);
     } else {
-        if (out_dtype == BT_F32) launch_grad_w16<MODE_BF16, true>(p, plan, st);
-        else launch_grad_w16<MODE_BF16, false>(p, plan, st);
+        if (out_dtype == BT_F32) launch_grad_w16<MODE_BF16, true>(p, plan, padded, st);
+        else launch_grad_w16<MODE_BF16, false>(p, plan, padded, st);
     }
     return check_launch(who);
 }

@@ -84,10 +84,10 @@ class _GatedLinear(torch.autograd.Function):
             dx = _C.ternary_linear_tiled_forward(g, w_back, one, None, 2 * fp, k).reshape(*lead, k).to(ctx.x_dtype)
         if want_w and dh.dtype == torch.float32:
             dw, _ = _C.linear_grad_weight(g, x2, one)
-        elif want_w:
-            dw = _C.linear_grad_weight_16(g, x2, one, dh.dtype if w_dtype == dh.dtype else torch.float32)
-        if want_w:
             dg, du = (t.to(w_dtype).contiguous() for t in (dw[:f, :k], dw[fp:fp + f, :k]))
+        elif want_w:
+            dw = _C.gated_grad_weight(g, x2, scale, f, k, dh.dtype if w_dtype == dh.dtype else torch.float32)
+            dg, du = dw[:f].to(w_dtype), dw[f:].to(w_dtype)
         if want_b:
             dgb, dub = db[:f].to(gb_dtype) if want_gb else None, db[f:].to(ub_dtype) if want_ub else None
         return dx, dg if want_g else None, du if want_u else None, dgb, dub, None, None, None

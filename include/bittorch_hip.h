@@ -254,7 +254,7 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *       W_back   (optional) bt_tiled_weights_bytes(K, 2 Fp) bytes: the decode-tiled copy of their transpose, a layer with K outputs
  *                and 2 Fp inputs, for bt_ternary_linear_tiled_forward on the gradient G;
  *       scale    [2 Fp + 1]: both layers' scales, zeros behind each, and a 1; bias [2 Fp] or NULL.
- *     bt_gated_range puts a power of two that no scale exceeds in the place of that 1.
+ *     bt_gated_range puts a power of two that no scale exceeds (within 2^-24 .. 2^15) in the place of that 1.
  *     fp32 rows read W_pairs through bt_ternary_linear_tiled_forward (BT_EPI_NATURAL_FROM_PAIRS) and bt_swiglu.
  *     workspace: at least bt_gated_quantize_workspace_bytes(F,K,per_channel) bytes.
  *   bt_ternary_gated_forward: fp16 / bf16 rows X [B,K]; where K % 8 != 0 or X is not 16-byte aligned, X_padded [B, K rounded up to 8] takes
@@ -267,6 +267,9 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *     multiply by (fp16: with bt_gated_range, so that G has fp16's range for the gradient alone).  16-bit dtype: pre as above; BT_F32: [g | u]
  *     [B, 2 Fp] fp32.  dBias (optional) [2 F] in bias_dtype: the sums over the rows without scales; with it a workspace of
  *     bt_gated_grad_workspace_bytes(B,F).
+ *   bt_gated_grad_weight: dW [2 F, K] (out_dtype: dtype or BT_F32), the masters' gradients one behind the other, = G^T X times the scalar
+ *     factor (scale + 2 Fp): fp16 / bf16 G and rows X [B, K rounded up to 8] (values behind K are read, not used); sums and workspace
+ *     as in bt_linear_grad_weight_16(B, 2 Fp, K rounded up to 8).
  */
 size_t bt_gated_quantize_workspace_bytes(int64_t F, int64_t K, int per_channel);
 int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, int64_t K, double threshold_factor, int per_channel,
@@ -278,6 +281,8 @@ int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const u
 int bt_gated_masters_serves(int64_t B, int64_t K, int w_dtype, int per_channel);
 int bt_gated_masters_forward(const void* X, int x_dtype, const void* gate, const void* up, int w_dtype, double threshold_factor,
                              const void* gate_bias, const void* up_bias, int bias_dtype, void* H, int64_t F, int64_t K, void* stream);
+int bt_gated_grad_weight(const void* G, const void* X, int dtype, const float* factor, void* dW, int out_dtype, int64_t B, int64_t F,
+                         int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F);
 int bt_gated_grad(const void* dH, int dtype, const void* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
                   int64_t F, void* workspace, size_t workspace_bytes, void* stream);

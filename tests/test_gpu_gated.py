@@ -570,4 +570,45 @@ def test_range_of_the_scales(f, largest):
     assert torch.equal(scale[:2 * fp], before[:2 * fp])
     top = float(scale[2 * fp])
     mantissa, exponent = math.frexp(top)
-    assert mantissa == 0.5 and exponent - 1 == min(125, max(-125, math.frexp(float(before[fp // 2]))[1]))
+    assert mantissa == 0.5 and exponent - 1 == min(15, max(-24, math.frexp(float(before[fp // 2]))[1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,k,f", [(1, 1, 1), (40, 13, 20), (300, 100, 33), (500, 1100, 2730), (5000, 1001, 2730), (2048, 2047, 1030), (2048, 2048, 1030),
+                                      (4096, 1026, 4100)])
+def test_weight_gradient_in_rows_of_its_own_length(rows, k, f, dt):
+    """The masters' gradients without the padding of both dimensions: the bits of the padded product, in tiles of both sizes, whole and in parts."""
+    announce("gated grad weight", rows, k, f, dt)
+    from bittorch_amd import _C
+    g = torch.Generator().manual_seed(rows + k)
+    fp, kr = (f + 15) // 16 * 16, (k + 7) // 8 * 8
+    G = torch.randn(rows, 2 * fp, generator=g).to(dt).cuda()
+    x = torch.randn(rows, kr, generator=g).to(dt).cuda()  # (what lies behind k is not used)
+    scale = torch.ones(2 * fp + 1, device="cuda")
+    scale[2 * fp] = 0.25
+    for out in (dt, torch.float32):
+        full = _C.linear_grad_weight_16(G, x, scale[2 * fp:], out)
+        got = _C.gated_grad_weight(G, x, scale, f, k, out)
+        assert torch.equal(got[:f], full[:f, :k]) and torch.equal(got[f:], full[fp:fp + f, :k])
+    guard = torch.full((2 * f * k + 64,), 7.0, dtype=dt, device="cuda")  # nothing in front of the first row or behind the last one
+    ws = _C._workspace(_C._L.bt_linear_grad_weight_16_workspace_bytes(rows, 2 * fp, kr), guard.device)
+    _C._status(_C._L.bt_gated_grad_weight(G.data_ptr(), x.data_ptr(), _C._DT[dt], scale[2 * fp:].data_ptr(), guard[32:].data_ptr(), _C._DT[dt], rows, f, k,
+                                          _C._ptr(ws), 0 if ws is None else ws.numel(), _C._stream(G)))
+    assert bool((guard[:32] == 7).all()) and bool((guard[32 + 2 * f * k:] == 7).all())
+    assert torch.equal(guard[32:32 + 2 * f * k].view(2 * f, k), _C.gated_grad_weight(G, x, scale, f, k, dt))
+
+
+def test_weight_gradient_and_range_refusals():
+    from bittorch_amd import _C, _lib
+    lib, at = _lib.load(), 4096
+    grad = lambda G=at, X=at, dt=2, s=at, out=at, odt=2, B=4, F=8, K=16, ws=None, n=0: lib.bt_gated_grad_weight(G, X, dt, s, out, odt, B, F, K, ws, n, None)
+    for bad in (dict(G=None), dict(X=None), dict(s=None), dict(out=None), dict(B=0), dict(F=0), dict(K=0), dict(F=1 << 23), dict(K=1 << 23), dict(dt=0),
+                dict(odt=1), dict(G=4100), dict(X=4100), dict(out=4100, F=16), dict(out=4097, K=15)):
+        assert grad(**bad) == -1, bad
+    need = lib.bt_linear_grad_weight_16_workspace_bytes(4096, 32, 16)
+    assert need > 0 and grad(B=4096, F=16) == grad(B=4096, F=16, ws=4096, n=need - 1) == grad(B=4096, F=16, ws=4100, n=need) == -2
+    for args in ((None, 8), (at, 0), (at, 1 << 23)):
+        assert lib.bt_gated_range(*args, None) == -1
+    with pytest.raises(RuntimeError, match="16-bit"):
+        _C.gated_grad_weight(torch.zeros(4, 32), torch.zeros(4, 16), torch.zeros(33), 16, 16, torch.float32)
