@@ -3,21 +3,24 @@
 // dtype in the epilogue.
 //
 // The contraction runs over the rows of both operands, so an MFMA fragment, 8 consecutive m of one column, is a column of a
-// row-major matrix.  Lane (i, g) of a wave loads columns 8 i .. +7 of rows 8 g .. +7, eight 16-byte loads; 32 byte permutes
-// turn them into the fragments of eight 16-column blocks, block t holding the columns 8 i + t, and go to LDS in fragment
-// order: no address of a wave's LDS access meets another's bank, and a lane's outputs are eight consecutive k of a row.
+// row-major matrix.  A stage's rows go to LDS as they are loaded, 16 bytes at a time, and transposing LDS reads make the fragments.
+// X's is the first operand of a product, so that a lane's four sums are consecutive k of a row; two pieces of them, exchanged
+// between lanes, are eight.
 //
 // A 256-thread workgroup owns 256 x 256 outputs, a wave 128 x 128 of them (256 accumulators a lane, one wave a SIMD): a stage
 // of 32 m is 64 MFMAs a wave (1024 cycles) for 64 KiB read from and 32 KiB written to LDS per workgroup, and an XCD's 32
-// workgroups read 12 strips of 256 columns.  The matrix cores are busy for 62 % of the time (69 % in
-// one long round), and the rest goes to the issue of a lone wave's other instructions.  4096 x 11008 x 4096 (rows, dY's columns,
-// X's), fp16 to fp32, 345 us = 1.07 PFLOP/s, the last of three rounds of tiles two thirds full; the vendor's product (393 us in a
-// profile) and the pass that scaled and widened its result 449.  The same stages make tiles of 128 x 128 for outputs that would
-// leave compute units idle: a stage is 64 m, half of them for each wave of an operand, and a wave 64 x 64 outputs (768 x 768 of 300
-// rows 10.2 us, 17.5 in tiles of 256).
+// workgroups read 12 strips of 256 columns.  The matrix cores are busy for 65 % of a workgroup's time; LDS is for 33, without
+// conflicts, and a third is the start and end of each tile, which nothing runs beside.  4096 x 11008 x 4096 (rows, dY's columns,
+// X's), fp16 to fp32, 316 us = 1.17 PFLOP/s, the last of three rounds of tiles two thirds full; the vendor's product (393 us in a
+// profile) and the pass that scaled and widened its result 449.  (Fragments permuted in registers on their way to LDS: 326 us; 4096 x
+// 13824 x 2560 bf16 246 and 238, 4096 x 2560 x 2560 70.5 and 64.5.)  The same stages make tiles of 128 x 128 for outputs that would
+// leave compute units idle: a stage is 64 m, half of them for each half of its MFMAs, and a wave 64 x 64 outputs (768 x 768 of 300
+// rows 9.6 us, 17.5 in tiles of 256); two of those workgroups share a compute unit (500 x 5472 x 1104 15.7 us, 18.5 one by one).
 #include "bt_common.h"
 
 namespace bt {
+
+typedef short v4i16 __attribute__((ext_vector_type(4)));
 
 struct GradW16Params {
     const uint16_t* G;    // [M, N]
@@ -49,13 +52,24 @@ __device__ __forceinline__ void grad_w16_tile(uint32_t lin, uint32_t tiles_n, ui
     k0 = (int64_t)tk * (32 * T);
 }
 
-// Output row n's sums of COUNT consecutive columns from k on: each is rounded as the 16-bit product of two matrices would be, scaled and
-// rounded again, what the unfused operations give.  PADDED: N and K are rounded up and the output is not, so that its rows start
-// anywhere and end inside a run.  (An instance of its own: the others' last stage would take 2.5 us longer with it, 300 x 768 x 768 9.6 / 12.2.)
-template <int DT, bool OUT32, bool PADDED, int COUNT>
-__device__ __forceinline__ void grad_w16_store(const GradW16Params& p, int64_t n, int64_t k, const float (&sum)[COUNT], float scale) {
+// A lane's sums of two neighbouring pieces, columns 4 g .. +3 of either, as eight consecutive columns: lanes of even g take the first
+// piece, their own and the next g's, those of odd g the second.  They start at column 16 (g % 2) + 8 (g / 2).
+__device__ __forceinline__ void grad_w16_pair(const v4f& first, const v4f& second, float (&sum)[8]) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const float x = first[c], y = second[c];
+        const auto q = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+        const uint32_t q0 = q[0], q1 = q[1];
+        sum[c] = __builtin_bit_cast(float, q0);
+        sum[4 + c] = __builtin_bit_cast(float, q1);
+    }
+}
+// Output row n's sums of eight columns from k on: each is rounded as the 16-bit product of two matrices would be, scaled and rounded
+// again, what the unfused operations give.  PADDED: N and K are rounded up and the output is not, so that its rows start anywhere and
+// end inside a run.  (An instance of its own: the others' last stage would take 2.5 us longer with it, 300 x 768 x 768 9.6 / 12.2.)
+template <int DT, bool OUT32, bool PADDED>
+__device__ __forceinline__ void grad_w16_store(const GradW16Params& p, int64_t n, int64_t k, const float (&sum)[8], float scale) {
     typedef u32x4 __attribute__((aligned(2))) vec4_a2;
-    typedef u32x2 __attribute__((aligned(2))) vec2_a2;
     void* const out = p.out;
     int64_t at = n * p.K + k;
     if constexpr (PADDED) {
@@ -64,43 +78,47 @@ __device__ __forceinline__ void grad_w16_store(const GradW16Params& p, int64_t n
         at = (int64_t)((h ? p.features : 0) + f) * p.cols + k;
     }
     const float s16 = round_to_dtype(scale, DT);
-    float v[COUNT];
+    float v[8];
 #pragma unroll
-    for (int b = 0; b < COUNT; b++) v[b] = round_to_dtype(__fmul_rn(round_to_dtype(sum[b], DT), s16), DT);
-    if (PADDED && k + COUNT > p.cols) {
+    for (int b = 0; b < 8; b++) v[b] = round_to_dtype(__fmul_rn(round_to_dtype(sum[b], DT), s16), DT);
+    if (PADDED && k + 8 > p.cols) {
 #pragma unroll
-        for (int b = 0; b < COUNT - 1; b++)
+        for (int b = 0; b < 7; b++)
             if (k + b < p.cols) store_elem<OUT32 ? BT_F32 : DT>(out, at + b, v[b]);
         return;
     }
-    if constexpr (OUT32) {
+    uint32_t d[OUT32 ? 8 : 4];
 #pragma unroll
-        for (int b = 0; b < COUNT; b += 4) {
-            const v4f q = {v[b], v[b + 1], v[b + 2], v[b + 3]};
-            if constexpr (PADDED) *(vec4_a2*)((float*)out + at + b) = __builtin_bit_cast(u32x4, q);
-            else *(v4f*)((float*)out + at + b) = q;
-        }
-    } else {
-        uint32_t d[COUNT / 2];
-#pragma unroll
-        for (int b = 0; b < COUNT / 2; b++) {
+    for (int b = 0; b < (OUT32 ? 8 : 4); b++) {
+        if constexpr (OUT32) {
+            d[b] = __builtin_bit_cast(uint32_t, v[b]);
+        } else {
             const uint16_t l16 = DT == BT_F16 ? f32_to_f16_bits(v[2 * b]) : f32_to_bf16_bits(v[2 * b]);
             const uint16_t h16 = DT == BT_F16 ? f32_to_f16_bits(v[2 * b + 1]) : f32_to_bf16_bits(v[2 * b + 1]);
             d[b] = (uint32_t)l16 | (uint32_t)h16 << 16;
         }
-        uint16_t* const to = (uint16_t*)out + at;
-        if constexpr (COUNT == 8 && PADDED) *(vec4_a2*)to = u32x4{d[0], d[1], d[2], d[3]};
-        else if constexpr (COUNT == 8) *(u32x4*)to = u32x4{d[0], d[1], d[2], d[3]};
-        else if constexpr (PADDED) *(vec2_a2*)to = u32x2{d[0], d[1]};
-        else *(u32x2*)to = u32x2{d[0], d[1]};
     }
+#pragma unroll
+    for (int b = 0; b < (OUT32 ? 8 : 4); b += 4) {
+        const u32x4 q = {d[b], d[b + 1], d[b + 2], d[b + 3]};
+        uint8_t* const to = (uint8_t*)out + at * (OUT32 ? 4 : 2) + 4 * b;
+        if constexpr (PADDED) *(vec4_a2*)to = q;
+        else *(u32x4*)to = q;
+    }
+}
+
+// The scales of rows n, n + 16, ..., in front of the first store: a load behind stores waits for them.
+template <int ST, int T>
+__device__ __forceinline__ void grad_w16_scales(const GradW16Params& p, int64_t n, float (&scale)[T]) {
+#pragma unroll
+    for (int a = 0; a < T; a++) scale[a] = load_elem<ST>(p.scale, p.scale_bcast ? 0 : min(n + 16 * a, p.N - 1));
 }
 
 template <int MODE, bool OUT32, int T, bool PADDED>
 __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
     constexpr int DT = MODE == MODE_F16 ? BT_F16 : BT_BF16;
     constexpr int SROWS = T == 8 ? 32 : 64;  // rows of a stage
-    constexpr uint32_t BUF = 32768;  // a stage in LDS: [G, X][half][block t][lane] x 16 bytes
+    constexpr uint32_t BUF = 32768;  // a stage in LDS: [G, X][row][32 T columns]
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
     // each XCD takes a contiguous run of tiles, walked in groups of four row tiles, so that its L2 holds what it shares
     const uint32_t tiles_n = (uint32_t)p.tiles_n, tiles_k = (uint32_t)p.tiles_k, idx = blockIdx.x >> 3;
@@ -150,29 +168,43 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
             __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, bytes, 0x00027000), voff[e], 0, 0));
     };
     auto advance = [&]() { src += step_bytes; left -= step_bytes; };
-    uint8_t* const w_at = lds + 16384 * hi + 8192 * lo + 16 * lane;
-    u32x4 frag;
-    auto permute = [&](int set, int t, int q) {  // dword q of block t
-        frag[q] = perm(r[set][2 * q + 1][t >> 1], r[set][2 * q][t >> 1], (t & 1) ? 0x07060302u : 0x05040100u);
-    };
-    auto write = [&](int buf, int t) { *(u32x4*)(w_at + buf * BUF + 1024 * t) = frag; };
+    // LDS: the rows as they are, pieces of 16 columns at their number ^ (row % 4 + 4 (row / 8 % 2)): eight rows of a piece, what 32
+    // lanes read at a time, lie in all banks.
+    constexpr uint32_t PITCH = 64 * T;
+    uint32_t w_at[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        w_at[e] = 16384 * hi + (8 * g + e + (T == 8 ? 0 : 32 * lo)) * PITCH + 32 * (((T == 8 ? 8 * lo : 0) + (i >> 1)) ^ (e + 4 * (g & 1))) + 16 * (i & 1);
+    auto write = [&](int set, int buf, int e) { *(u32x4*)(lds + w_at[e & 3] + buf * BUF + (e >> 2) * 4 * PITCH) = r[set][e]; };
 
     v4f acc[T][T];
 #pragma unroll
     for (int a = 0; a < T; a++)
 #pragma unroll
         for (int b = 0; b < T; b++) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
+    // Fragment t is piece t of the wave's 16 T columns (T == 4: t % 4, of the stage's half t / 4): a transposing read turns four columns
+    // of four rows, each in a lane, into four rows of a column, for each group of 16 lanes.  Lane (i, g) ends with rows 8 g .. +7 of column i.
     u32x4 fa[8], fb[8];
-    // T == 8: fragment t is block t of the wave's 128 columns; else block t % 4 of its four, of the stage's half t / 4
-    const uint8_t* const a_at = lds + (T == 8 ? 8192 : 4096) * hi + 16 * lane;
-    const uint8_t* const b_at = lds + 16384 + (T == 8 ? 8192 : 4096) * lo + 16 * lane;
-    auto at = [](int buf, int t) { return buf * BUF + (T == 8 ? 1024 * t : 8192 * (t >> 2) + 1024 * (t & 3)); };
-    auto read_a = [&](int buf, int t) { fa[t] = *(const u32x4*)(a_at + at(buf, t)); };
-    auto read_b = [&](int buf, int t) { fb[t] = *(const u32x4*)(b_at + at(buf, t)); };
-    auto mfma = [&](int a, int b) {
+    uint32_t a_at[T], b_at[T];
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        const uint32_t row = 8 * g + (i >> 2), bank = (i >> 2) + 4 * (g & 1);
+        a_at[t] = row * PITCH + 32 * ((T * hi + t) ^ bank) + 8 * (i & 3);
+        b_at[t] = 16384 + row * PITCH + 32 * ((T * lo + t) ^ bank) + 8 * (i & 3);
+    }
+    auto read = [&](uint32_t at, int buf, int t) {
+        u32x2 d[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            d[h] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(lds + at + buf * BUF + (T == 8 ? 0 : 8192 * (t >> 2)) + h * 4 * PITCH)));
+        return u32x4{d[0][0], d[0][1], d[1][0], d[1][1]};
+    };
+    auto read_a = [&](int buf, int t) { fa[t] = read(a_at[t % T], buf, t); };
+    auto read_b = [&](int buf, int t) { fb[t] = read(b_at[t % T], buf, t); };
+    auto mfma = [&](int a, int b) {  // (X first: a lane's four sums are consecutive k of a row)
         v4f& c = acc[a % T][b % T];
-        if constexpr (MODE == MODE_F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(fa[a]), "v"(fb[b]));
-        else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(fa[a]), "v"(fb[b]));
+        if constexpr (MODE == MODE_F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(fb[b]), "v"(fa[a]));
+        else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(fb[b]), "v"(fa[a]));
     };
 
 #pragma unroll
@@ -181,38 +213,35 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
         for (int e = 0; e < 8; e++) load(s, e);
         advance();
     }
-    auto put = [&](int set, int buf, int t) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) permute(set, t, q);
-        write(buf, t);
-    };
-#pragma unroll
-    for (int t = 0; t < 8; t++) put(0, 0, t);
+    for (int e = 0; e < 8; e++) write(0, 0, e);
 #pragma unroll
     for (int e = 0; e < 4; e++) load(0, e);
 #pragma unroll
-    for (int t = 0; t < 4; t++) put(1, 1, t);
+    for (int e = 0; e < 4; e++) write(1, 1, e);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int t = 0; t < 4; t++) { read_a(0, t); read_b(0, t); }
 
     // Stage s (set and buffer constants of its place in the loop).  Four runs of 16 MFMAs go round the quarters of the wave's
     // tile, the next stage the other way round, so that one set of fragments serves: each quarter of them is read behind the
-    // last run that used it, one run ahead of its own first.  A stage's blocks 0 to 3 are written behind the barrier of the
-    // stage before the last, blocks 4 to 7 in front of the last one's; its loads are issued three stages before that.
+    // last run that used it, one run ahead of its own first.  Rows e = 0 to 3 of each eight of a stage are written behind the barrier of
+    // the stage before the last, rows 4 to 7 in front of the last one's; its loads are issued three stages before that.  The reads
+    // and writes are spread over the runs, and a run takes the newest fragments last: four waves keep LDS busy most of the time.
     auto stage = [&](auto SC) {
         constexpr int S = decltype(SC)::value, B = S & 1, F = B ? 4 : 0, O = 4 - F;  // first and other half of X's blocks
         constexpr int S1 = (S + 1) & 3, S2 = (S + 2) & 3;
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (T == 4) {  // two runs of 16, a half of the rows each; the same order of writes and loads
+        if constexpr (T == 4) {
+            // Two runs of 16, a half of the rows each; the same order of writes and loads.  A run begins with the fragments read first.
+            constexpr int A[16] = {0, 0, 1, 1, 0, 2, 1, 2, 2, 0, 3, 1, 3, 2, 3, 3}, BB[16] = {0, 1, 0, 1, 2, 0, 2, 1, 2, 3, 0, 3, 1, 3, 2, 3};
 #pragma unroll
             for (int c = 0; c < 16; c++) {
-                mfma(c >> 2, c & 3);
-                if (c % 4 == 1) read_b(B, 4 + c / 4);
-                if (c % 4 == 3) read_a(B, 4 + c / 4);
+                mfma(A[c], BB[c]);
+                if (c < 12 && c % 3 == 0) read_a(B, 4 + c / 3);
+                if (c < 12 && c % 3 == 1) read_b(B, 4 + c / 3);
+                if (c < 12 && c % 3 == 2) write(S1, 1 - B, 4 + c / 3);
                 if (c % 4 == 2) load(S, 4 + c / 4);
-                permute(S1, 4 + (c >> 2), c & 3);
-                if (c % 4 == 3) write(1 - B, 4 + (c >> 2));
                 __builtin_amdgcn_sched_barrier(0);
             }
             advance();
@@ -220,59 +249,50 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = 0; c < 16; c++) {
-                mfma(4 + (c >> 2), 4 + (c & 3));
-                if (c % 4 == 1) read_b(1 - B, c / 4);
-                if (c % 4 == 3) read_a(1 - B, c / 4);
+                mfma(4 + A[c], 4 + BB[c]);
+                if (c < 12 && c % 3 == 0) read_a(1 - B, c / 3);
+                if (c < 12 && c % 3 == 1) read_b(1 - B, c / 3);
+                if (c < 12 && c % 3 == 2) write(S2, B, c / 3);
                 if (c % 4 == 2) load(S1, c / 4);
-                permute(S2, c >> 2, c & 3);
-                if (c % 4 == 3) write(B, c >> 2);
                 __builtin_amdgcn_sched_barrier(0);
             }
             return;
         }
 #pragma unroll
         for (int c = 0; c < 16; c++) {
-            mfma(c >> 2, F + (c & 3));
-            if (c < 8 && c % 2 == 0) read_b(B, O + c / 2);
-            if (c == 5 || c == 13) load(S, 4 + c / 8);
-            permute(S1, 4 + (c >> 3), (c >> 1) & 3);  // (the second of a pair repeats the first: no instruction)
-            if ((c & 7) == 7) write(1 - B, 4 + (c >> 3));
+            mfma(c & 3, F + (c >> 2));
+            if (c % 4 == 1) read_b(B, O + c / 4);
+            if (c == 3 || c == 11) write(S1, 1 - B, 4 + c / 8);
+            if (c == 6 || c == 14) load(S, 4 + c / 8);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int c = 0; c < 16; c++) {
-            mfma(c >> 2, O + (c & 3));
-            if (c < 8 && c % 2 == 0) read_a(B, 4 + c / 2);
-            if (c == 5 || c == 11) load(S, 6 + c / 8);
-            if (c == 12) advance();
-            if (c < 8) {
-                permute(S1, 6 + (c >> 2), c & 3);
-                if ((c & 3) == 3) write(1 - B, 6 + (c >> 2));
-            }
+            mfma(c & 3, O + (c >> 2));
+            if (c % 4 == 1) read_a(B, 4 + c / 4);
+            if (c == 3 || c == 11) write(S1, 1 - B, 6 + c / 8);
+            if (c == 6 || c == 14) load(S, 6 + c / 8);
             __builtin_amdgcn_sched_barrier(0);
         }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
+        advance();
 #pragma unroll
         for (int c = 0; c < 16; c++) {
             mfma(4 + (c >> 2), O + (c & 3));
-            if (c < 8 && c % 2 == 0) read_a(1 - B, c / 2);
-            if (c == 5 || c == 13) load(S1, c / 8);
-            if (c >= 8) {
-                permute(S2, (c - 8) >> 2, c & 3);
-                if ((c & 3) == 3) write(B, (c - 8) >> 2);
+            if (c == 7) {
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (c >= 8 && c % 2 == 0) read_a(1 - B, c / 2 - 4);
+            if (c == 11) write(S2, B, 0);
+            if (c == 9 || c == 13) load(S1, c / 8 - 1 + (c == 13));
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int c = 0; c < 16; c++) {
             mfma(4 + (c >> 2), F + (c & 3));
-            if (c < 8 && c % 2 == 0) read_b(1 - B, O + c / 2);
-            if (c == 5 || c == 13) load(S1, 2 + c / 8);
-            if (c < 8) {
-                permute(S2, 2 + (c >> 2), c & 3);
-                if ((c & 3) == 3) write(B, 2 + (c >> 2));
-            }
+            if (c % 4 == 1) read_b(1 - B, O + c / 4);
+            if (c == 3 || c == 7 || c == 11) write(S2, B, 1 + c / 4);
+            if (c == 6 || c == 14) load(S1, 2 + c / 8);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -295,22 +315,22 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
             for (int b = 0; b < T; b++) o[256 * (T * a + b)] = acc[a][b];
         return;
     }
-    // lane (i, g): T == 8: rows 8 (4 g + c) + a of the wave's 128, columns 8 i .. +7; T == 4: rows 8 (4 g + c) + 4 hi + a of the
-    // tile's 128, columns 8 i + 4 lo .. +3
-    const int64_t k = k0 + (T == 8 ? 128 : 4) * lo + 8 * i;
+    // lane (i, g): row i of the wave's row piece a
+    int at_end = lane;  // (so that nothing of what follows is kept through the loop: with at most 256 registers two small tiles share a SIMD)
+    asm volatile("" : "+v"(at_end));
+    const int64_t first_n = n0 + 16 * T * hi + (at_end & 15), k = k0 + 16 * T * lo + 16 * (at_end >> 4 & 1) + 8 * (at_end >> 5);
+    float scale[T];
+    if (p.scale_dtype == BT_F32) grad_w16_scales<BT_F32, T>(p, first_n, scale);  // (uniform)
+    else if (p.scale_dtype == BT_F16) grad_w16_scales<BT_F16, T>(p, first_n, scale);
+    else grad_w16_scales<BT_BF16, T>(p, first_n, scale);
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const int64_t n = n0 + (T == 8 ? 128 : 4) * hi + 8 * (4 * g + c);
-        if (n >= p.N || k >= (PADDED ? p.cols : p.K)) continue;
-        float sc[T];
+    for (int a = 0; a < T; a++) {
+        const int64_t n = first_n + 16 * a;
 #pragma unroll
-        for (int a = 0; a < T; a++) sc[a] = load_elem_rt(p.scale, p.scale_dtype, p.scale_bcast ? 0 : n + a);
-#pragma unroll
-        for (int a = 0; a < T; a++) {
-            float v[T];
-#pragma unroll
-            for (int b = 0; b < T; b++) v[b] = acc[a][b][c];
-            grad_w16_store<DT, OUT32, PADDED>(p, n + a, k, v, sc[a]);
+        for (int b = 0; b < T; b += 2) {
+            float v[8];
+            grad_w16_pair(acc[a][b], acc[a][b + 1], v);
+            if (n < p.N && k + 16 * b < (PADDED ? p.cols : p.K)) grad_w16_store<DT, OUT32, PADDED>(p, n, k + 16 * b, v, scale[a]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -337,14 +357,13 @@ __global__ __launch_bounds__(256) void grad_w16_reduce_kernel(GradW16Params p) {
 #pragma unroll
         for (int b = 0; b < 4; b++) sum[b] += src[256 * b];
     }
-    const int64_t k = k0 + (T == 8 ? 128 : 4) * lo + 8 * i + 4 * h;
-    if (k >= (PADDED ? p.cols : p.K)) return;
+    const int64_t n = n0 + 16 * T * hi + 16 * a + i, k = k0 + 16 * T * lo + 64 * h + 16 * (g & 1) + 8 * (g >> 1);
+    const float scale = n < p.N ? load_elem_rt(p.scale, p.scale_dtype, p.scale_bcast ? 0 : n) : 0.0f;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const int64_t n = n0 + (T == 8 ? 128 : 4) * hi + 8 * (4 * g + c) + a;
-        if (n >= p.N) continue;
-        const float v[4] = {sum[0][c], sum[1][c], sum[2][c], sum[3][c]};
-        grad_w16_store<DT, OUT32, PADDED>(p, n, k, v, load_elem_rt(p.scale, p.scale_dtype, p.scale_bcast ? 0 : n));
+    for (int b = 0; b < 4; b += 2) {
+        float v[8];
+        grad_w16_pair(sum[b], sum[b + 1], v);
+        if (n < p.N && k + 16 * b < (PADDED ? p.cols : p.K)) grad_w16_store<DT, OUT32, PADDED>(p, n, k + 16 * b, v, scale);
     }
 }
 
