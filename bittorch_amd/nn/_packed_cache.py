@@ -62,24 +62,39 @@ def _state(weight: Tensor) -> tuple:
 
 class GatedWeightCache:
     """The packed weights of a gated pair (``_C.gated_weights``: both layers in one tiled copy, tiles of gate and up in turn), kept by the
-    same rules."""
+    same rules.  Another stream than the one that packed them waits for it; what a graph being captured packs is the graph's own and not kept."""
 
-    __slots__ = ("key", "value")
+    __slots__ = ("key", "value", "stream", "packed")
 
     def __init__(self) -> None:
-        self.key = None
-        self.value = None
+        self.clear()
+
+    def __reduce__(self):  # (a copy packs for itself)
+        return GatedWeightCache, ()
 
     def get(self, gate, up):
         from .. import _C
 
         given = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
         key = (*(_state(t) for t in given), gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel))
-        if key != self.key:
-            with torch.no_grad():
-                w, _, scale, bias = _C.gated_weights(gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)
-            self.key, self.value = key, (w, scale[:-1], bias)
-        return self.value
+        stream = _C._stream(gate.weight)
+        if key == self.key:
+            if stream != self.stream and not torch.cuda.is_current_stream_capturing():  # (a capture starts behind a synchronization)
+                here = torch.cuda.current_stream(gate.weight.device)
+                here.wait_event(self.packed)
+                for t in self.value:
+                    if t is not None:
+                        t.record_stream(here)
+            return self.value
+        with torch.no_grad():
+            w, _, scale, bias = _C.gated_weights(gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)
+        value = w, scale[:-1], bias
+        if not torch.cuda.is_current_stream_capturing():
+            with torch.cuda.device(gate.weight.device):
+                packed = torch.cuda.Event()
+                packed.record()
+            self.key, self.value, self.stream, self.packed = key, value, stream, packed
+        return value
 
     def forward(self, x: Tensor, gate, up) -> Tensor:
         """``silu(gate(x)) * up(x)`` as ``TernarySwiGLU`` computes it."""
@@ -91,7 +106,7 @@ class GatedWeightCache:
         return h if h.shape[-1] == f else h[..., :f].contiguous()
 
     def clear(self) -> None:
-        self.key, self.value = None, None
+        self.key, self.value, self.stream, self.packed = None, None, None, None
 
 
 def cache_usable(x: Tensor, weight: Tensor) -> bool:

@@ -96,7 +96,7 @@ class BlockStack:
         """The training modules with the glue between their layers fused, differentiable: the residual connections with the norms behind
         them (``ops.add_rmsnorm``), gate and up with the SwiGLU between them (``ops.ternary_gated_linear``)."""
         F, ops = self.F, self.bt.ops
-        eps_of = lambda norm: norm.eps or self.torch.finfo(self.act_dtype).eps
+        eps_of = lambda norm: self.torch.finfo(self.act_dtype).eps if norm.eps is None else norm.eps
         x, branch = self.emb(self.tokens), None
         for blk in self.blocks:
             x, h = ops.add_rmsnorm(x, None, blk.n1.weight, eps_of(blk.n1)) if branch is None else ops.add_rmsnorm(branch, x, blk.n1.weight, eps_of(blk.n1))

@@ -174,3 +174,54 @@ def test_training_step_captured_and_replayed():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, expect))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("learns", ["gate.bias", "up.bias", "down.weight", "x"])
+def test_frozen_weights_with_something_else_that_learns(learns):
+    announce("gated mlp, frozen but for", learns)
+    mlp = _mlp(64, 48, seed=5, bias=True).cuda()
+    x = torch.randn(9, 64, generator=torch.Generator().manual_seed(6)).cuda()
+    want = {n: torch.autograd.grad(mlp(x.requires_grad_()).square().sum(), t)[0] for n, t in (*mlp.named_parameters(), ("x", x)) if n == learns}[learns]
+    x = x.detach().requires_grad_(learns == "x")
+    for n, p in mlp.named_parameters():
+        p.requires_grad_(n == learns)
+    leaf = x if learns == "x" else dict(mlp.named_parameters())[learns]
+    got, = torch.autograd.grad(mlp(x).square().sum(), leaf)
+    # (down.weight: the pair's hidden values come from the kept copy, as those of the converted module, rounded to fp32 at other places)
+    assert _norm_error(got, want) <= 1e-5
+
+
+@pytest.mark.gpu
+def test_kept_weights_on_other_streams_and_in_graphs():
+    announce("gated mlp, kept weights")
+    mlp = _mlp(512, 768, seed=7).cuda().bfloat16()
+    x = torch.randn(33, 512, generator=torch.Generator().manual_seed(8)).cuda().bfloat16()
+    busy = torch.randn(4096, 4096, device="cuda")
+    with torch.no_grad():
+        want = mlp(x).clone()
+        mlp.gate.weight.mul_(1.0)  # (the same values, packed anew)
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                busy = busy @ busy * 1e-3
+            first = mlp(x)  # packs behind all of that
+        second = mlp(x)  # this stream has not waited for it
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want)
+        copied = copy.deepcopy(mlp)
+        assert copied._packed.key is None and torch.equal(copied(x), want)
+        mlp.invalidate_packed_cache()
+        for layer in (mlp.gate, mlp.up, mlp.down):
+            layer(torch.zeros(1, layer.in_features, dtype=x.dtype, device="cuda"))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mlp(x)
+        assert mlp._packed.key is None  # (what the capture packed is written by each replay only)
+        assert torch.equal(mlp(x), want)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(mlp(x), want)
