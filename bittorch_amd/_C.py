@@ -956,22 +956,38 @@ def gated_grad(dH: Tensor, pre: Tensor, scale: Tensor, bias_dtype: Optional[torc
     return G, db
 
 
-def gated_grad_weight(G: Tensor, X: Tensor, scale: Tensor, out_features: int, in_features: int, out_dtype: torch.dtype) -> Tensor:
-    """``[2 F, K]``: the gradients of both 16-bit masters, ``G^T X`` times ``scale``'s last entry, of :func:`gated_grad`'s ``G`` and the rows
-    that :func:`ternary_gated_forward` read."""
-    F, K = out_features, in_features
+def _gated_grad_operands(G: Tensor, X: Tensor, scale: Tensor, F: int, K: int, out_dtype: torch.dtype):
     Fp, Kr = (F + 15) // 16 * 16, (K + 7) // 8 * 8
     _check(G.dim() == 2 and G.dtype in (torch.float16, torch.bfloat16) and X.dtype == G.dtype and G.shape[1] == 2 * Fp
            and X.shape == (G.shape[0], Kr), "G and X must be 16-bit, [B, 2 F] and [B, K] as the other calls pad them")
     _check(out_dtype in (G.dtype, torch.float32), "out_dtype must be G's or float32")
-    _check(scale.dtype == torch.float32 and scale.numel() == 2 * Fp + 1 and scale.is_contiguous(), "scale must be that of gated_weights")
     _check(_all_cuda(G, X, scale), "All tensors must be CUDA")
-    G, X = G.contiguous(), X.contiguous()
-    out = torch.empty((2 * F, K), dtype=out_dtype, device=G.device)
+    return G.contiguous(), X.contiguous(), torch.empty((2 * F, K), dtype=out_dtype, device=G.device), 2 * Fp, Kr
+
+
+def gated_grad_weight(G: Tensor, X: Tensor, scale: Tensor, out_features: int, in_features: int, out_dtype: torch.dtype) -> Tensor:
+    """``[2 F, K]``: the gradients of both 16-bit masters, ``G^T X`` times ``scale``'s last entry, of :func:`gated_grad`'s ``G`` and the rows
+    that :func:`ternary_gated_forward` read; each sum is rounded to 16 bits before the factor and after it."""
+    F, K = out_features, in_features
+    G, X, out, n, Kr = _gated_grad_operands(G, X, scale, F, K, out_dtype)
+    _check(scale.dtype == torch.float32 and scale.numel() == n + 1 and scale.is_contiguous(), "scale must be that of gated_weights")
     with _on(G):
-        ws = _workspace(_L.bt_linear_grad_weight_16_workspace_bytes(G.shape[0], 2 * Fp, Kr), G.device)
-        _status(_L.bt_gated_grad_weight(G.data_ptr(), X.data_ptr(), _DT[G.dtype], scale[2 * Fp:].data_ptr(), out.data_ptr(), _DT[out_dtype],
+        ws = _workspace(_L.bt_linear_grad_weight_16_workspace_bytes(G.shape[0], n, Kr), G.device)
+        _status(_L.bt_gated_grad_weight(G.data_ptr(), X.data_ptr(), _DT[G.dtype], scale[n:].data_ptr(), out.data_ptr(), _DT[out_dtype],
                                         G.shape[0], F, K, _ptr(ws), 0 if ws is None else ws.numel(), _stream(G)))
+    return out
+
+
+def gated_grad_masters(G: Tensor, X: Tensor, scale: Tensor, out_features: int, in_features: int, out_dtype: torch.dtype) -> Tensor:
+    """As :func:`gated_grad_weight`, with a scale for each padded feature (``[2 Fp]``) or one (``[1]``), and the scaled fp32 sums rounded once."""
+    F, K = out_features, in_features
+    G, X, out, n, Kr = _gated_grad_operands(G, X, scale, F, K, out_dtype)
+    _check(scale.dtype == torch.float32 and scale.dim() == 1 and scale.numel() in (1, n) and scale.is_contiguous(),
+           "scale must be fp32 with an entry for each padded feature, or one")
+    with _on(G):
+        ws = _workspace(_L.bt_linear_grad_weight_16_workspace_bytes(G.shape[0], n, Kr), G.device)
+        _status(_L.bt_gated_grad_masters(G.data_ptr(), X.data_ptr(), _DT[G.dtype], scale.data_ptr(), scale.numel(), out.data_ptr(), _DT[out_dtype],
+                                         G.shape[0], F, K, _ptr(ws), 0 if ws is None else ws.numel(), _stream(G)))
     return out
 
 

@@ -86,6 +86,7 @@ SIGNATURES = {
     "bt_gated_masters_forward": (_int, [_vp, _int, _vp, _vp, _int, ctypes.c_double, _vp, _vp, _int, _vp, _i64, _i64, _vp]),
     "bt_gated_grad_workspace_bytes": (_sz, [_i64, _i64]),
     "bt_gated_grad_weight": (_int, [_vp, _vp, _int, _vp, _vp, _int, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "bt_gated_grad_masters": (_int, [_vp, _vp, _int, _vp, _i64, _vp, _int, _i64, _i64, _i64, _vp, _sz, _vp]),
     "bt_gated_grad": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _int, _i64, _i64, _vp, _sz, _vp]),
     "bt_act_quant_i8_rowsum": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _int, _vp]),
     "bt_swiglu_rowsum": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _vp, _vp, _vp, _int, _vp]),

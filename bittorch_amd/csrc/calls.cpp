@@ -42,7 +42,7 @@ namespace {
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
     X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
     X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_range)                     \
-    X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_weight) X(bt_gated_grad_workspace_bytes)                      \
+    X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_masters) X(bt_gated_grad_workspace_bytes)                     \
     X(bt_gated_masters_serves) X(bt_gated_masters_forward)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -797,8 +797,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
                                                        nullptr, B, 2 * Fp, K, ws.ptr(), ws.size(), st));
             } else {
                 const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fp, Kr), x);
-                check_status(lib.bt_gated_grad_weight(g.const_data_ptr(), x.const_data_ptr(), dt, one, dw.data_ptr(), tag(dtype), B, F, K, ws.ptr(),
-                                                      ws.size(), st));
+                check_status(lib.bt_gated_grad_masters(g.const_data_ptr(), x.const_data_ptr(), dt, one, 1, dw.data_ptr(), tag(dtype), B, F, K, ws.ptr(),
+                                                       ws.size(), st));
             }
             for (int i = 0; i < 2; i++)
                 if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * rows, F).to(w_dtype);

@@ -65,9 +65,10 @@ __device__ __forceinline__ void grad_w16_pair(const v4f& first, const v4f& secon
     }
 }
 // Output row n's sums of eight columns from k on: each is rounded as the 16-bit product of two matrices would be, scaled and rounded
-// again, what the unfused operations give.  PADDED: N and K are rounded up and the output is not, so that its rows start anywhere and
+// again, what the unfused operations give; or (ONCE) scaled in fp32 and rounded as it is stored: a sum may lie outside fp16 where its
+// product with the scale does not, and an fp32 output keeps what the sum has.  PADDED: N and K are rounded up and the output is not, so that its rows start anywhere and
 // end inside a run.  (An instance of its own: the others' last stage would take 2.5 us longer with it, 300 x 768 x 768 9.6 / 12.2.)
-template <int DT, bool OUT32, bool PADDED>
+template <int DT, bool OUT32, bool PADDED, bool ONCE>
 __device__ __forceinline__ void grad_w16_store(const GradW16Params& p, int64_t n, int64_t k, const float (&sum)[8], float scale) {
     typedef u32x4 __attribute__((aligned(2))) vec4_a2;
     void* const out = p.out;
@@ -77,10 +78,15 @@ __device__ __forceinline__ void grad_w16_store(const GradW16Params& p, int64_t n
         if (f >= p.features) return;
         at = (int64_t)((h ? p.features : 0) + f) * p.cols + k;
     }
-    const float s16 = round_to_dtype(scale, DT);
     float v[8];
+    if constexpr (ONCE) {
 #pragma unroll
-    for (int b = 0; b < 8; b++) v[b] = round_to_dtype(__fmul_rn(round_to_dtype(sum[b], DT), s16), DT);
+        for (int b = 0; b < 8; b++) v[b] = OUT32 ? __fmul_rn(sum[b], scale) : round_to_dtype(__fmul_rn(sum[b], scale), DT);
+    } else {
+        const float s16 = round_to_dtype(scale, DT);
+#pragma unroll
+        for (int b = 0; b < 8; b++) v[b] = round_to_dtype(__fmul_rn(round_to_dtype(sum[b], DT), s16), DT);
+    }
     if (PADDED && k + 8 > p.cols) {
 #pragma unroll
         for (int b = 0; b < 7; b++)
@@ -114,7 +120,7 @@ __device__ __forceinline__ void grad_w16_scales(const GradW16Params& p, int64_t 
     for (int a = 0; a < T; a++) scale[a] = load_elem<ST>(p.scale, p.scale_bcast ? 0 : min(n + 16 * a, p.N - 1));
 }
 
-template <int MODE, bool OUT32, int T, bool PADDED>
+template <int MODE, bool OUT32, int T, bool PADDED, bool ONCE>
 __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
     constexpr int DT = MODE == MODE_F16 ? BT_F16 : BT_BF16;
     constexpr int SROWS = T == 8 ? 32 : 64;  // rows of a stage
@@ -330,7 +336,7 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
         for (int b = 0; b < T; b += 2) {
             float v[8];
             grad_w16_pair(acc[a][b], acc[a][b + 1], v);
-            if (n < p.N && k + 16 * b < (PADDED ? p.cols : p.K)) grad_w16_store<DT, OUT32, PADDED>(p, n, k + 16 * b, v, scale[a]);
+            if (n < p.N && k + 16 * b < (PADDED ? p.cols : p.K)) grad_w16_store<DT, OUT32, PADDED, ONCE>(p, n, k + 16 * b, v, scale[a]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -338,7 +344,7 @@ __global__ __launch_bounds__(256, 1) void grad_w16_kernel(GradW16Params p) {
 
 // The tiles summed in parts: a thread adds the parts of four of an accumulator row's column blocks, in order, and finishes
 // their 4 x 4 outputs.  Bound by reading the parts.
-template <int MODE, bool OUT32, int T, bool PADDED>
+template <int MODE, bool OUT32, int T, bool PADDED, bool ONCE>
 __global__ __launch_bounds__(256) void grad_w16_reduce_kernel(GradW16Params p) {
     constexpr int DT = MODE == MODE_F16 ? BT_F16 : BT_BF16;
     constexpr uint32_t H = T / 4;
@@ -363,7 +369,7 @@ __global__ __launch_bounds__(256) void grad_w16_reduce_kernel(GradW16Params p) {
     for (int b = 0; b < 4; b += 2) {
         float v[8];
         grad_w16_pair(sum[b], sum[b + 1], v);
-        if (n < p.N && k + 16 * b < (PADDED ? p.cols : p.K)) grad_w16_store<DT, OUT32, PADDED>(p, n, k + 16 * b, v, scale);
+        if (n < p.N && k + 16 * b < (PADDED ? p.cols : p.K)) grad_w16_store<DT, OUT32, PADDED, ONCE>(p, n, k + 16 * b, v, scale);
     }
 }
 
@@ -419,17 +425,22 @@ static GradW16Plan grad_w16_plan(int64_t M, int64_t N, int64_t K) {
     return best;
 }
 
-template <int MODE, bool OUT32, int T, bool PADDED>
+template <int MODE, bool OUT32, int T, bool PADDED, bool ONCE>
 static void launch_grad_w16_tiles(const GradW16Params& p, int64_t tail, hipStream_t st) {
-    hipLaunchKernelGGL((grad_w16_kernel<MODE, OUT32, T, PADDED>), dim3((unsigned)(8 * (p.whole + p.per_xcd_tail))), dim3(256), 0, st, p);
-    if (tail) hipLaunchKernelGGL((grad_w16_reduce_kernel<MODE, OUT32, T, PADDED>), dim3((unsigned)(T * T / 4 * tail)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((grad_w16_kernel<MODE, OUT32, T, PADDED, ONCE>), dim3((unsigned)(8 * (p.whole + p.per_xcd_tail))), dim3(256), 0, st, p);
+    if (tail) hipLaunchKernelGGL((grad_w16_reduce_kernel<MODE, OUT32, T, PADDED, ONCE>), dim3((unsigned)(T * T / 4 * tail)), dim3(256), 0, st, p);
+}
+template <int MODE, bool OUT32, bool PADDED, bool ONCE>
+static void launch_grad_w16_kind(const GradW16Params& p, const GradW16Plan& plan, hipStream_t st) {
+    if (plan.T == 8) launch_grad_w16_tiles<MODE, OUT32, 8, PADDED, ONCE>(p, plan.tail, st);
+    else launch_grad_w16_tiles<MODE, OUT32, 4, PADDED, ONCE>(p, plan.tail, st);
 }
 template <int MODE, bool OUT32>
-static void launch_grad_w16(const GradW16Params& p, const GradW16Plan& plan, bool padded, hipStream_t st) {
-    if (padded && plan.T == 8) launch_grad_w16_tiles<MODE, OUT32, 8, true>(p, plan.tail, st);
-    else if (padded) launch_grad_w16_tiles<MODE, OUT32, 4, true>(p, plan.tail, st);
-    else if (plan.T == 8) launch_grad_w16_tiles<MODE, OUT32, 8, false>(p, plan.tail, st);
-    else launch_grad_w16_tiles<MODE, OUT32, 4, false>(p, plan.tail, st);
+static void launch_grad_w16(const GradW16Params& p, const GradW16Plan& plan, bool padded, bool once, hipStream_t st) {
+    if (padded && once) launch_grad_w16_kind<MODE, OUT32, true, true>(p, plan, st);
+    else if (padded) launch_grad_w16_kind<MODE, OUT32, true, false>(p, plan, st);
+    else if (once) launch_grad_w16_kind<MODE, OUT32, false, true>(p, plan, st);
+    else launch_grad_w16_kind<MODE, OUT32, false, false>(p, plan, st);
 }
 
 }  // namespace bt
@@ -437,7 +448,7 @@ static void launch_grad_w16(const GradW16Params& p, const GradW16Plan& plan, boo
 using namespace bt;
 
 static int grad_w16(const char* who, const void* dY, const void* X, int dtype, const void* scale, int scale_dtype, int64_t scale_len, void* dW,
-                    int out_dtype, int64_t M, int64_t N, int64_t K, int64_t cols, int64_t features, void* workspace,
+                    int out_dtype, int64_t M, int64_t N, int64_t K, int64_t cols, int64_t features, bool once, void* workspace,
                     size_t workspace_bytes, void* stream);
 
 extern "C" size_t bt_linear_grad_weight_16_workspace_bytes(int64_t M, int64_t N, int64_t K) {
@@ -449,23 +460,33 @@ extern "C" size_t bt_linear_grad_weight_16_workspace_bytes(int64_t M, int64_t N,
 extern "C" int bt_linear_grad_weight_16(const void* dY, const void* X, int dtype, const void* scale, int scale_dtype,
                                         int64_t scale_len, void* dW, int out_dtype, int64_t M, int64_t N, int64_t K,
                                         void* workspace, size_t workspace_bytes, void* stream) {
-    return grad_w16("bt_linear_grad_weight_16", dY, X, dtype, scale, scale_dtype, scale_len, dW, out_dtype, M, N, K, K, N / 2, workspace,
+    return grad_w16("bt_linear_grad_weight_16", dY, X, dtype, scale, scale_dtype, scale_len, dW, out_dtype, M, N, K, K, N / 2, false, workspace,
                     workspace_bytes, stream);
 }
 
-extern "C" int bt_gated_grad_weight(const void* G, const void* X, int dtype, const float* factor, void* dW, int out_dtype, int64_t B, int64_t F,
-                                    int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
-    const char* who = "bt_gated_grad_weight";
+// What both forms of the gated pair's masters' gradients share: the padded sizes
+static int gated_grad_w16(const char* who, const void* G, const void* X, int dtype, const float* scale, int64_t scale_len, void* dW, int out_dtype,
+                          int64_t B, int64_t F, int64_t K, bool once, void* workspace, size_t workspace_bytes, void* stream) {
     if (F <= 0 || K <= 0 || F >= (1ll << 23) || K >= (1ll << 23)) {
         set_error("%s: F and K between 1 and 2^23 (F=%lld, K=%lld)", who, (long long)F, (long long)K);
         return BT_ERR_INVALID;
     }
-    const int64_t Fp = ceil_div(F, 16) * 16;
-    return grad_w16(who, G, X, dtype, factor, BT_F32, 1, dW, out_dtype, B, 2 * Fp, ceil_div(K, 8) * 8, K, F, workspace, workspace_bytes, stream);
+    const int64_t N = 2 * ceil_div(F, 16) * 16;
+    return grad_w16(who, G, X, dtype, scale, BT_F32, scale_len, dW, out_dtype, B, N, ceil_div(K, 8) * 8, K, F, once, workspace, workspace_bytes, stream);
+}
+
+extern "C" int bt_gated_grad_weight(const void* G, const void* X, int dtype, const float* factor, void* dW, int out_dtype, int64_t B, int64_t F,
+                                    int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+    return gated_grad_w16("bt_gated_grad_weight", G, X, dtype, factor, 1, dW, out_dtype, B, F, K, false, workspace, workspace_bytes, stream);
+}
+
+extern "C" int bt_gated_grad_masters(const void* G, const void* X, int dtype, const float* scale, int64_t scale_len, void* dW, int out_dtype, int64_t B,
+                                     int64_t F, int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+    return gated_grad_w16("bt_gated_grad_masters", G, X, dtype, scale, scale_len, dW, out_dtype, B, F, K, true, workspace, workspace_bytes, stream);
 }
 
 static int grad_w16(const char* who, const void* dY, const void* X, int dtype, const void* scale, int scale_dtype, int64_t scale_len, void* dW,
-                    int out_dtype, int64_t M, int64_t N, int64_t K, int64_t cols, int64_t features, void* workspace,
+                    int out_dtype, int64_t M, int64_t N, int64_t K, int64_t cols, int64_t features, bool once, void* workspace,
                     size_t workspace_bytes, void* stream) {
     const bool padded = cols != K || 2 * features != N;
     if (!dY || !X || !scale || !dW || M <= 0 || N <= 0 || K <= 0) {
@@ -504,11 +525,11 @@ static int grad_w16(const char* who, const void* dY, const void* X, int dtype, c
     p.per_xcd_tail = (int)(plan.long_first ? 2 * ceil_div(plan.tail, 8) : ceil_div(plan.tail * plan.splits, 8));
     hipStream_t st = (hipStream_t)stream;
     if (dtype == BT_F16) {
-        if (out_dtype == BT_F32) launch_grad_w16<MODE_F16, true>(p, plan, padded, st);
-        else launch_grad_w16<MODE_F16, false>(p, plan, padded, st);
+        if (out_dtype == BT_F32) launch_grad_w16<MODE_F16, true>(p, plan, padded, once, st);
+        else launch_grad_w16<MODE_F16, false>(p, plan, padded, once, st);
     } else {
-        if (out_dtype == BT_F32) launch_grad_w16<MODE_BF16, true>(p, plan, padded, st);
-        else launch_grad_w16<MODE_BF16, false>(p, plan, padded, st);
+        if (out_dtype == BT_F32) launch_grad_w16<MODE_BF16, true>(p, plan, padded, once, st);
+        else launch_grad_w16<MODE_BF16, false>(p, plan, padded, once, st);
     }
     return check_launch(who);
 }

@@ -86,7 +86,7 @@ class _GatedLinear(torch.autograd.Function):
             dw, _ = _C.linear_grad_weight(g, x2, one)
             dg, du = (t.to(w_dtype).contiguous() for t in (dw[:f, :k], dw[fp:fp + f, :k]))
         elif want_w:
-            dw = _C.gated_grad_weight(g, x2, scale, f, k, dh.dtype if w_dtype == dh.dtype else torch.float32)
+            dw = _C.gated_grad_masters(g, x2, one, f, k, dh.dtype if w_dtype == dh.dtype else torch.float32)
             dg, du = dw[:f].to(w_dtype), dw[f:].to(w_dtype)
         if want_b:
             dgb, dub = db[:f].to(gb_dtype) if want_gb else None, db[f:].to(ub_dtype) if want_ub else None

@@ -269,7 +269,9 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *     bt_gated_grad_workspace_bytes(B,F).
  *   bt_gated_grad_weight: dW [2 F, K] (out_dtype: dtype or BT_F32), the masters' gradients one behind the other, = G^T X times the scalar
  *     factor (scale + 2 Fp): fp16 / bf16 G and rows X [B, K rounded up to 8] (values behind K are read, not used); sums and workspace
- *     as in bt_linear_grad_weight_16(B, 2 Fp, K rounded up to 8).
+ *     as in bt_linear_grad_weight_16(B, 2 Fp, K rounded up to 8).  Each sum is rounded to dtype before the factor and after it.
+ *   bt_gated_grad_masters: the same with a scale for each row of G^T X (scale_len 2 Fp) or one (scale_len 1), the scaled sums rounded once, as
+ *     they are stored.
  */
 size_t bt_gated_quantize_workspace_bytes(int64_t F, int64_t K, int per_channel);
 int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, int64_t K, double threshold_factor, int per_channel,
@@ -283,6 +285,8 @@ int bt_gated_masters_forward(const void* X, int x_dtype, const void* gate, const
                              const void* gate_bias, const void* up_bias, int bias_dtype, void* H, int64_t F, int64_t K, void* stream);
 int bt_gated_grad_weight(const void* G, const void* X, int dtype, const float* factor, void* dW, int out_dtype, int64_t B, int64_t F,
                          int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+int bt_gated_grad_masters(const void* G, const void* X, int dtype, const float* scale, int64_t scale_len, void* dW, int out_dtype, int64_t B,
+                          int64_t F, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 size_t bt_gated_grad_workspace_bytes(int64_t B, int64_t F);
 int bt_gated_grad(const void* dH, int dtype, const void* pre, const float* scale, void* G, void* dBias, int bias_dtype, int64_t B,
                   int64_t F, void* workspace, size_t workspace_bytes, void* stream);

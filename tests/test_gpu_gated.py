@@ -612,3 +612,77 @@ def test_weight_gradient_and_range_refusals():
         assert lib.bt_gated_range(*args, None) == -1
     with pytest.raises(RuntimeError, match="16-bit"):
         _C.gated_grad_weight(torch.zeros(4, 32), torch.zeros(4, 16), torch.zeros(33), 16, 16, torch.float32)
+
+
+def _assert_fp16_gradients(leaves, h, dh, ref, rows, f):
+    """Every gradient within what fp16's G may add to it: half a step of each entry, 2^-11 of it and 2^-25 among the subnormal numbers, where
+    G is the gradient times at least a half, so that a feature's own scale, not the largest one, says what that is."""
+    dx, dwg, dwu, *_ = torch.autograd.grad(h, leaves, dh)
+    half, chain = 2.0 ** -11, lambda n: U * 2 * (3 * n / 32 + 80)
+    parts = [(ref.dg, ref.tol_dg, ref.ag, ref.tg), (ref.du, ref.tol_du, ref.au, ref.tu)]
+    off = lambda n: [((tol * (1 + half) + (half + chain(n)) * v.abs()) + 2.0 ** -24) * a for v, tol, a, _ in parts]
+    want = sum((v * a) @ t for v, _, a, t in parts)
+    tol = sum(o @ t.abs() for o, (_, _, _, t) in zip(off(2 * f), parts))
+    # (under autocast dx is rounded to fp16 all the same, and widened)
+    over = (dx.double() - want).abs() / (tol + half * (want.abs() + tol) + 2.0 ** -25)
+    assert bool((over <= 1).all()), f"dx: {float(over.max())} of its bound"
+    for got, o, (v, _, a, _), what in zip((dwg, dwu), off(rows), parts, ("gate", "up")):
+        want_w, tol_w = (v * a).t() @ ref.x, o.t() @ ref.x.abs()
+        last = (half, 2.0 ** -25) if got.dtype == torch.float16 else (2.0 ** -8, 0.0) if got.dtype == torch.bfloat16 else (U, 0.0)
+        over = (got.double() - want_w).abs() / (tol_w + last[0] * (want_w.abs() + tol_w) + last[1])
+        assert bool((over <= 1).all()), f"{what}: {float(over.max())} of its bound"
+    return dx, dwg, dwu
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("autocast", [False, True])
+@pytest.mark.parametrize("rows,k,f", [(512, 264, 48), (600, 129, 40), (2048, 1024, 520)])
+def test_large_gradients_of_small_masters(rows, k, f, autocast):
+    """Sums over the rows beyond fp16 whose product with the masters' scales is far inside it."""
+    announce("gated large", rows, k, f, autocast)
+    g = torch.Generator().manual_seed(rows + f)
+    x, dh = torch.randn(rows, k, generator=g).abs().half().cuda(), ((torch.rand(rows, f, generator=g) + 0.5) * 60 * 512 / rows).half().cuda()
+    wg, wu = ((torch.randn(f, k, generator=g) * 0.003).half().cuda() for _ in range(2))
+    bg, bu = (torch.full((f,), 4.0).half().cuda() for _ in range(2))
+    ref = _Reference(x, wg, wu, bg, bu, dh)
+    assert float((ref.dg.t() @ ref.x).max()) > 65504 and float(((ref.dg * ref.ag).t() @ ref.x).max()) < 4000
+    leaves = [(t.float() if autocast else t).requires_grad_() for t in (x, wg, wu, bg, bu)]
+    with torch.autocast("cuda", enabled=autocast):
+        h = _gated(*leaves)
+    _assert_fp16_gradients(leaves, h, dh, ref, rows, f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,wt", [(torch.float16, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("rows,k,f", [(40, 264, 48), (300, 1001, 37), (2048, 1024, 520)])
+def test_masters_of_more_bits_get_gradients_rounded_once(rows, k, f, dt, wt):
+    """The sums of 16-bit rows in fp32 for fp32 masters: of the product with G as it is, only fp32's own roundings remain."""
+    announce("gated grad masters", rows, k, f, dt, wt)
+    from bittorch_amd import _C
+    g = torch.Generator().manual_seed(rows + k)
+    fp, kr = (f + 15) // 16 * 16, (k + 7) // 8 * 8
+    G = torch.randn(rows, 2 * fp, generator=g).to(dt).cuda()
+    x = torch.randn(rows, kr, generator=g).to(dt).cuda()
+    for scale in (torch.rand(2 * fp, generator=g).cuda() + 0.01, torch.full((1,), 2.0 ** -6).cuda()):
+        got = _C.gated_grad_masters(G, x, scale, f, k, wt if wt == torch.float32 else dt)
+        each = scale.double().expand(2 * fp)
+        full, size = (G.double().t() @ x.double()) * each[:, None], (G.double().abs().t() @ x.double().abs()) * each[:, None]
+        pick = torch.cat((torch.arange(f), torch.arange(f) + fp)).cuda()
+        want, size = full[pick, :k], size[pick, :k]
+        half = U if wt == torch.float32 else torch.finfo(dt).eps / 2
+        assert bool(((got.double() - want).abs() <= U * 2 * (3 * rows / 32 + 80) * size + half * want.abs() + 2.0 ** -25 * (wt != torch.float32)).all())
+
+
+def test_masters_gradient_refusals():
+    from bittorch_amd import _C, _lib
+    lib, at = _lib.load(), 4096
+    grad = lambda G=at, X=at, dt=2, s=at, n_s=1, out=at, odt=2, B=4, F=8, K=16, ws=None, n=0: lib.bt_gated_grad_masters(
+        G, X, dt, s, n_s, out, odt, B, F, K, ws, n, None)
+    for bad in (dict(G=None), dict(X=None), dict(s=None), dict(out=None), dict(B=0), dict(F=0), dict(K=0), dict(F=1 << 23), dict(K=1 << 23), dict(dt=0),
+                dict(odt=1), dict(G=4100), dict(X=4100), dict(out=4100, F=16), dict(out=4097, K=15), dict(n_s=0), dict(n_s=16), dict(n_s=33)):
+        assert grad(**bad) == -1, bad
+        assert "bt_gated_grad_masters" in _lib.last_error()
+    need = lib.bt_linear_grad_weight_16_workspace_bytes(4096, 32, 16)
+    assert need > 0 and grad(B=4096, F=16) == grad(B=4096, F=16, ws=4096, n=need - 1) == grad(B=4096, F=16, ws=4100, n=need) == -2
+    with pytest.raises(RuntimeError, match="16-bit"):
+        _C.gated_grad_masters(torch.zeros(4, 32), torch.zeros(4, 16), torch.zeros(32), 16, 16, torch.float32)
