@@ -892,10 +892,9 @@ def gated_masters_serves(rows: int, masters: Tensor, per_channel: bool = True, a
 
 
 def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, up_bias: Optional[Tensor] = None,
-                  threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, back: bool = False, ranged: bool = False):
+                  threshold_factor: float = 0.05, per_channel: bool = True, as_half: bool = False, back: bool = False):
     """The operands of the gated pair, of two masters ``[F, K]`` quantized as :func:`ternary_quantize_pack` does: ``(W_pairs, W_back,
-    scale, bias)`` as ``bt_gated_quantize`` makes them; ``back``: with the copy for the input's gradient (otherwise None); ``ranged``: with
-    ``bt_gated_range``, for the gradient of fp16 rows."""
+    scale, bias)`` as ``bt_gated_quantize`` makes them; ``back``: with the copy for the input's gradient (otherwise None)."""
     masters, wdt, biases, bdt = _gated_operands(gate, up, gate_bias, up_bias, as_half)
     (F, K), dev = gate.shape, gate.device
     Fp = (F + 15) // 16 * 16
@@ -908,9 +907,35 @@ def gated_weights(gate: Tensor, up: Tensor, gate_bias: Optional[Tensor] = None, 
         _status(_L.bt_gated_quantize(masters[0].data_ptr(), masters[1].data_ptr(), wdt, F, K, float(threshold_factor), int(bool(per_channel)),
                                      _ptr(biases[0]), _ptr(biases[1]), bdt, w.data_ptr(), _ptr(w_back), scale.data_ptr(), _ptr(bias), _ptr(ws),
                                      0 if ws is None else ws.numel(), _stream(gate)))
-        if ranged:
-            _status(_L.bt_gated_range(scale.data_ptr(), F, _stream(gate)))
     return w, w_back, scale, bias
+
+
+def gated_split(scale: Tensor, out_features: int) -> Tensor:
+    """The scales of :func:`gated_weights` taken apart for the gradient of fp16 rows, as ``bt_gated_split`` lays them out (fp32 and, at the end,
+    fp16); ``scale``'s last entry becomes the power of two above all of them."""
+    n = 2 * ((out_features + 15) // 16 * 16)
+    _check(scale.is_cuda and scale.dtype == torch.float32 and scale.numel() == n + 1 and scale.is_contiguous(), "scale must be that of gated_weights")
+    split = torch.empty((_L.bt_gated_split_bytes(out_features) // 4,), dtype=torch.float32, device=scale.device)
+    with _on(scale):
+        _status(_L.bt_gated_split(scale.data_ptr(), out_features, split.data_ptr(), _stream(scale)))
+    return split
+
+
+def gated_grad_input(G: Tensor, W_back: Tensor, split: Tensor, out_features: int, in_features: int) -> Tensor:
+    """``[B, K]``: the gradient of fp16 rows, of :func:`gated_grad`'s ``G`` with ``split[:2 Fp + 1]`` in the place of the scales."""
+    F, K, Fp = out_features, in_features, (out_features + 15) // 16 * 16
+    _check(G.dim() == 2 and G.dtype == torch.float16 and G.shape[1] == 2 * Fp and G.numel() > 0, "G must be fp16, [B, 2 F] as gated_grad pads it")
+    _check(W_back.dtype == torch.uint8 and W_back.dim() == 1 and W_back.is_contiguous() and W_back.numel() == _L.bt_tiled_weights_bytes(K, 2 * Fp),
+           "W_back size doesn't match in_features x out_features")
+    _check(split.dtype == torch.float32 and split.is_contiguous() and 4 * split.numel() == _L.bt_gated_split_bytes(F), "split must be that of gated_split")
+    _check(_all_cuda(G, W_back, split), "All tensors must be CUDA")
+    G = G.contiguous()
+    out = torch.empty((G.shape[0], K), dtype=G.dtype, device=G.device)
+    with _on(G):
+        ws = _workspace(_L.bt_gated_grad_input_workspace_bytes(G.shape[0], F, K), G.device)
+        _status(_L.bt_gated_grad_input(G.data_ptr(), W_back.data_ptr(), split.data_ptr(), out.data_ptr(), G.shape[0], F, K, _ptr(ws),
+                                       0 if ws is None else ws.numel(), _stream(G)))
+    return out
 
 
 def ternary_gated_forward(X: Tensor, W_pairs: Tensor, scale: Tensor, bias: Optional[Tensor], out_features: int,

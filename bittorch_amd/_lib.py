@@ -81,6 +81,10 @@ SIGNATURES = {
     "bt_gated_quantize_workspace_bytes": (_sz, [_i64, _i64, _int]),
     "bt_gated_quantize": (_int, [_vp, _vp, _int, _i64, _i64, ctypes.c_double, _int, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "bt_gated_range": (_int, [_vp, _i64, _vp]),
+    "bt_gated_split_bytes": (_sz, [_i64]),
+    "bt_gated_split": (_int, [_vp, _i64, _vp, _vp]),
+    "bt_gated_grad_input_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "bt_gated_grad_input": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
     "bt_ternary_gated_forward": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "bt_gated_masters_serves": (_int, [_i64, _i64, _int, _int]),
     "bt_gated_masters_forward": (_int, [_vp, _int, _vp, _vp, _int, ctypes.c_double, _vp, _vp, _int, _vp, _i64, _i64, _vp]),

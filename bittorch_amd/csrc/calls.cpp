@@ -41,7 +41,7 @@ namespace {
     X(bt_ternary_linear_tensor_core_forward) X(bt_quantize_pack) X(bt_ternary_linear_grad_input) X(bt_linear_grad_weight)      \
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
     X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
-    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_range)                     \
+    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_split) X(bt_gated_split_bytes) X(bt_gated_grad_input) X(bt_gated_grad_input_workspace_bytes) \
     X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_masters) X(bt_gated_grad_workspace_bytes)                     \
     X(bt_gated_masters_serves) X(bt_gated_masters_forward)
 struct Library {
@@ -693,7 +693,7 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 struct GatedOut {
-    at::Tensor h, rows, pre, w_back, scale;  // rows: x, or the copy of it that the kernels read
+    at::Tensor h, rows, pre, w_back, scale;  // rows: x, or the copy of it that the kernels read; scale: for the gradient of fp16 rows its parts
 };
 // fp32 rows: K >= 4.  All tensors contiguous.
 GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up, const MaybeTensor& gate_bias, const MaybeTensor& up_bias,
@@ -723,7 +723,6 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
              data_of(gate_bias), data_of(up_bias), gate_bias ? tag_of(gate_bias) : tag_of(up_bias), (uint8_t*)w.data_ptr(),
              want_back ? (uint8_t*)o.w_back.data_ptr() : nullptr, scale_at, bias_at, ws.ptr(), ws.size(), st);
     }
-    if (keep && x.scalar_type() == at::kHalf) call(lib.bt_gated_range, scale_at, F, st);
     o.h = output(with_last(x, F), x.scalar_type(), x);
     if (fp32) o.pre = output({B, 2 * Fp}, at::kFloat, x);
     else if (keep) o.pre = output({B, Fp / 2 * 3}, at::kInt, x);
@@ -735,6 +734,11 @@ GatedOut gated_run(const at::Tensor& x, const at::Tensor& gate, const at::Tensor
         }
         call(lib.bt_ternary_gated_forward, x.const_data_ptr(), dt, padded, (const uint8_t*)w.const_data_ptr(), scale_at, bias_at, o.h.data_ptr(),
              keep ? o.pre.data_ptr() : nullptr, B, F, K, st);
+        if (keep && x.scalar_type() == at::kHalf) {
+            const at::Tensor split = output({(int64_t)lib.bt_gated_split_bytes(F) / 4}, at::kFloat, x);
+            call(lib.bt_gated_split, scale_at, F, (float*)split.data_ptr(), st);
+            o.scale = split;  // (the scales are the stream's until the kernels that read them have ended)
+        }
         return o;
     }
     const Scratch ws(lib.bt_tiled_forward_workspace_bytes(B, 2 * Fp, K, dt), x);
@@ -767,7 +771,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         const at::NoGradGuard no_grad;
         const c10::DeviceGuard guard(x.device());
         const int64_t F = shape[0], K = shape[1], Kr = x.size(-1), B = x.numel() / Kr;  // (a padded copy has longer rows)
-        const bool fp32 = x.scalar_type() == at::kFloat;
+        const bool fp32 = x.scalar_type() == at::kFloat, split = x.scalar_type() == at::kHalf;  // (split: scale is bt_gated_split's)
         const int64_t Fp = (F + 15) / 16 * 16;
         const int dt = tag(x.scalar_type());
         const bool want_w = w.want[1] || w.want[2], want_b = w.want[3] || w.want[4];
@@ -781,7 +785,12 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
             check_status(lib.bt_gated_grad(dh.const_data_ptr(), dt, pre.const_data_ptr(), scale_at, g.data_ptr(), want_b ? db.data_ptr() : nullptr,
                                            want_b ? tag(b_dtype) : 0, B, F, ws.ptr(), ws.size(), st));
         }
-        if (w.want[0]) {
+        if (w.want[0] && split) {
+            w.grads[0] = output(with_last(incoming[0], K), x.scalar_type(), x);
+            const Scratch ws(lib.bt_gated_grad_input_workspace_bytes(B, F, K), x);
+            check_status(lib.bt_gated_grad_input(g.const_data_ptr(), (const uint8_t*)w_back.const_data_ptr(), scale_at, w.grads[0].data_ptr(), B, F, K,
+                                                 ws.ptr(), ws.size(), st));
+        } else if (w.want[0]) {
             w.grads[0] = output(with_last(incoming[0], K), x.scalar_type(), x);
             const Scratch ws(lib.bt_tiled_forward_workspace_bytes(B, K, 2 * Fp, dt), x);
             check_status(lib.bt_ternary_linear_tiled_forward(g.const_data_ptr(), 2 * Fp, dt, 0, nullptr, 0, 0.0f, (const uint8_t*)w_back.const_data_ptr(), one,
@@ -797,8 +806,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
                                                        nullptr, B, 2 * Fp, K, ws.ptr(), ws.size(), st));
             } else {
                 const Scratch ws(lib.bt_linear_grad_weight_16_workspace_bytes(B, 2 * Fp, Kr), x);
-                check_status(lib.bt_gated_grad_masters(g.const_data_ptr(), x.const_data_ptr(), dt, one, 1, dw.data_ptr(), tag(dtype), B, F, K, ws.ptr(),
-                                                       ws.size(), st));
+                check_status(lib.bt_gated_grad_masters(g.const_data_ptr(), x.const_data_ptr(), dt, split ? scale_at + 2 * Fp + 16 : one, split ? 2 * Fp : 1,
+                                                       dw.data_ptr(), tag(dtype), B, F, K, ws.ptr(), ws.size(), st));
             }
             for (int i = 0; i < 2; i++)
                 if (w.want[1 + i]) w.grads[1 + i] = dw.narrow(0, i * rows, F).to(w_dtype);

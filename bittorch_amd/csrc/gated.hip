@@ -12,10 +12,12 @@
 // 16-bit rows: one product forms both projections and h in its output stage (gemm_f16.hip, OUT_GATED) on the tiled copy in pair
 // order.  One pass (gated_grad_kernel) makes G = [a_g dg | a_u du] of dh and the kept projections, rounded once to 16 bits as an operand
 // of the matrix cores; it serves both products behind it: dx = G [T_g; T_u] on a second tiled copy of the codes, in which the contraction
-// runs over the output features, by the forward's kernel, and dW = G^T x by the weight gradient's (grad_w16.hip).  a times dg, not
-// dg, is what is rounded, so that neither product has a scale for each feature.  For fp16 both are divided by a power of two above every a
-// (gated_range_kernel), which the products multiply their sums by: fp16 has no range for a (0.01 where dg is 1e-4 would leave 4 bits of it),
-// and so G keeps what fp16 keeps of dg.
+// runs over the output features, by the forward's kernel, and dW = G^T x by the weight gradient's (grad_w16.hip).  For bf16 a times
+// dg, not dg, is what is rounded, so that neither product has a scale for each feature.  fp16 has no range for a (0.01 where dg is 1e-4 would
+// leave 4 bits of it), and none for the ratio of two features' a either (one entry of 0.5 among masters of 0.003 is 40 of them): there a is
+// taken apart feature by feature (gated_range_kernel), a = m 2^f with m in [1/2, 1), and G = [m_g dg | m_u du] keeps what fp16 keeps of dg and
+// half of it.  dW's rows are multiplied by their 2^f in fp32, as they are stored; in dx's product, which sums over the features, 2^f goes with
+// the codes as they are decoded, over the power of two above all of them, which is the output's scale.
 // fp32 rows: the same steps on the fp32 kernels and the same copies, the projections stored in fp32 and h by the SwiGLU row kernel.  (On the
 // packed bytes as rows the fp32 products take longer: 4096 x 4096 x 768 forward 74 us, 68 on the copy, its transpose 89 and 77.)
 //
@@ -26,6 +28,9 @@ namespace bt {
 
 int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const Epilogue& epi, void* Y, uint32_t* pre, int64_t H, int64_t M,
                           int64_t N, int64_t K, hipStream_t st);
+int launch_gemm_f16_factors(const void* X, const uint8_t* W_tiled, const uint16_t* factors, const float* scale, void* Y, int64_t M, int64_t N, int64_t K,
+                            void* workspace, hipStream_t st);
+size_t gemm_f16_factors_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int launch_pad_rows(const void* X, int64_t B, int64_t K, void* P, hipStream_t st);
 float quantize_clamp_min(int w_dtype);
 bool gemm_f16_supported(int64_t N, int64_t K, const void* X, const void* W_T, const void* Y, bool tiled);
@@ -42,7 +47,7 @@ struct GatedWeightsParams {
     int64_t F, Fp, K, Kb;
     uint8_t* pairs;           // forward: tiled copy in pair order of [gate | up], 2 Fp columns
     uint8_t* back;            // backward: tiled copy of the transpose: K columns, contraction over 2 Fp
-    float* scale;             // [2 Fp + 1], the last one what products of G multiply by: 1, or gated_range_kernel's
+    float* scale;             // [2 Fp + 1], the last one 1
     float* bias;              // [2 Fp] or null
     uint32_t n_pairs, n_back;          // workgroups of each part, in this order; behind them those of the vectors
     uint32_t steps, back_steps;        // 64-wide steps of the two tiled copies
@@ -270,19 +275,40 @@ static void launch_gated_quantize(const GatedQuantizeParams& p, hipStream_t st) 
 // Rows that a wave holds, with a scale each; the others are quantized by bt_quantize_pack and their bytes put in place
 static bool gated_quantizes(int64_t K, bool per_channel) { return per_channel && K >= 8 && K <= (K % 8 == 0 ? 8192 : 4096); }
 
-// scale[n] = the least power of two 2^e with scale[i] < 2^e for all i < n, within 2^-24 .. 2^15.  One workgroup, its time is its launch.
-__global__ __launch_bounds__(1024) void gated_range_kernel(float* scale, int n) {
+// scale[n] = the least power of two 2^e with scale[i] < 2^e for all i < n, within 2^-24 .. 2^15.  With `split` (bt_gated_split) each scale
+// is also taken apart, into a power of two of its own 2^f, scale[i] / 2^f in [1/2, 1), and what is left.  One workgroup: its time is its
+// launch.  f stays within 24 below and 15 above e, where 2^(f - e) is an fp16 number (a power of two among the subnormal ones too); beyond
+// that what is left is smaller than a half, or not below 1.
+__global__ __launch_bounds__(1024) void gated_range_kernel(float* scale, int n, float* split) {
     __shared__ float part[16];
     float m = 0.0f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, scale[i]);
     m = wave_max(m);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x != 0) return;
+#pragma unroll
     for (int i = 0; i < 16; i++) m = fmaxf(m, part[i]);
-    // the exponent above m's, among those of fp16 (the weight gradient's kernel takes its scale in the rows' type)
-    const int e = (int)(__builtin_bit_cast(uint32_t, m) >> 23) - 126;
-    scale[n] = __builtin_bit_cast(float, (uint32_t)(127 + (e < -24 ? -24 : e > 15 ? 15 : e)) << 23);
+    // the exponent above v's
+    auto above = [](float v) { return (int)(__builtin_bit_cast(uint32_t, v) >> 23) - 126; };
+    auto power = [](int e) { return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23); };
+    const int e = max(-24, min(15, above(m)));
+    if (threadIdx.x == 0) scale[n] = power(e);
+    if (!split) return;
+    float* const rows = split + n + 16;
+    uint16_t* const factors = (uint16_t*)(split + 2 * n + 16);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        const int f = max(e - 24, min(e + 15, above(scale[i]))), d = f - e;
+        split[i] = scale[i] * power(-f);
+        rows[i] = power(f);
+        factors[i] = (uint16_t)(d >= -14 ? (15 + d) << 10 : 1 << (24 + d));
+    }
+    if ((n & 63) && threadIdx.x < 32) factors[n + threadIdx.x] = 0;  // (n is a multiple of 32)
+    if (threadIdx.x == 0) {
+        split[n] = 1.0f;
+        split[n + 1] = power(e);
+    }
 }
 
 // ---- one row on the masters, without a copy of them -------------------------------------------------------------------------
@@ -404,7 +430,7 @@ static bool masters_serve(int64_t B, int64_t K, int w_dtype, bool per_channel) {
 struct GatedGradParams {
     const void* dH;       // [B, F]
     const void* pre;      // 16-bit rows: [B, 3 Fp / 2] dwords, column pairs of gate and up in turn in 24 bits; fp32 rows: [B, 2 Fp], gate | up
-    const float* scale;   // [2 Fp + 1], the last one a power of two
+    const float* scale;   // [2 Fp + 1]: what dg | du are multiplied by, over the last one
     void* G;              // [B, 2 Fp]
     float* parts;         // [gridDim.y, 2 F] sums of dg | du, or null
     int64_t B, rows;      // rows: of a workgroup
@@ -594,8 +620,48 @@ extern "C" int bt_gated_range(float* scale, int64_t F, void* stream) {
         set_error("%s: null pointer, or F not between 1 and 2^23", who);
         return BT_ERR_INVALID;
     }
-    hipLaunchKernelGGL(gated_range_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, scale, (int)(2 * padded(F)));
+    hipLaunchKernelGGL(gated_range_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, scale, (int)(2 * padded(F)), nullptr);
     return check_launch(who);
+}
+
+extern "C" size_t bt_gated_split_bytes(int64_t F) {
+    return F > 0 && F < (1ll << 23) ? (size_t)(4 * (4 * padded(F) + 16) + 128 * ceil_div(2 * padded(F), 64)) : 0;
+}
+
+extern "C" int bt_gated_split(float* scale, int64_t F, float* split, void* stream) {
+    const char* who = "bt_gated_split";
+    if (!scale || !split || F <= 0 || F >= (1ll << 23) || ((uintptr_t)split) % 16 != 0) {
+        set_error("%s: null pointer, split not 16-byte aligned, or F not between 1 and 2^23", who);
+        return BT_ERR_INVALID;
+    }
+    hipLaunchKernelGGL(gated_range_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, scale, (int)(2 * padded(F)), split);
+    return check_launch(who);
+}
+
+extern "C" size_t bt_gated_grad_input_workspace_bytes(int64_t B, int64_t F, int64_t K) {
+    return B > 0 && F > 0 && K > 0 ? gemm_f16_factors_workspace_bytes(B, K, 2 * padded(F)) : 0;
+}
+
+extern "C" int bt_gated_grad_input(const void* G, const uint8_t* W_back, const float* split, void* dX, int64_t B, int64_t F, int64_t K, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+    const char* who = "bt_gated_grad_input";
+    if (!G || !W_back || !split || !dX || B <= 0 || F <= 0 || K <= 0) {
+        set_error("%s: null pointer or empty shape", who);
+        return BT_ERR_INVALID;
+    }
+    const int64_t n = 2 * padded(F);  // (below 2^24: 32-bit byte offsets span 128 rows of G)
+    if (F >= (1ll << 23) || K >= (1ll << 23) || B >= (1ll << 31) || n >= (1ll << 24) || bt_tiled_weights_bytes(K, n) >= (1ull << 32) ||
+        ((uintptr_t)W_back) % 256 != 0 || (((uintptr_t)G) | ((uintptr_t)split) | ((uintptr_t)dX)) % 16 != 0) {
+        set_error("%s: F and K below 2^23, B below 2^31, buffers 16-byte and the copy 256-byte aligned and below 4 GiB (F=%lld, K=%lld)", who,
+                  (long long)F, (long long)K);
+        return BT_ERR_INVALID;
+    }
+    const size_t need = bt_gated_grad_input_workspace_bytes(B, F, K);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace) % 256 != 0)) {
+        set_error("%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, need, workspace_bytes);
+        return BT_ERR_WORKSPACE;
+    }
+    return launch_gemm_f16_factors(G, W_back, (const uint16_t*)(split + 2 * n + 16), split + n + 1, dX, B, K, n, workspace, (hipStream_t)stream);
 }
 
 extern "C" int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,

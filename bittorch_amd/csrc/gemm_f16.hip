@@ -50,16 +50,22 @@ struct GemmFParams {
     Epilogue epi;
     uint32_t* pre;        // OUT_GATED: [M, 3 N / 4] the two projections in 24 bits each, column pairs of gate and up in turn, or null
     int64_t H;            // OUT_GATED: columns of Y, at most N / 2
+    const uint16_t* factors;  // OUT_FACTORS: [64 wstages] fp16,
+    float* parts;             // [gridDim.y, M, N rounded up to 4] the sums of so many runs of the stages, or null (one run, to Y)
+    int part_stages;          // stages of a run
 };
 // What becomes of a tile's sums: the linear layer's output; the SwiGLU of a layer whose columns are [gate | up], of the projections
-// rounded to the output's type; or the same of the projections as they are, in fp32, with a copy of them for the gradient.
-enum { OUT_LINEAR = 0, OUT_SWIGLU = 1, OUT_GATED = 2 };
+// rounded to the output's type; the same of the projections as they are, in fp32, with a copy of them for the gradient; or the linear
+// layer's output of weights that are multiplied by a factor for each k (fp16; powers of two, so that the products are exact).
+enum { OUT_LINEAR = 0, OUT_SWIGLU = 1, OUT_GATED = 2, OUT_FACTORS = 3 };
 static_assert(offsetof(GemmFParams, Y) == 64, "first argument line as laid out above");
 
 // Stages of activations in LDS; of weights one fewer, since a wave has its own in registers half a stage before it needs them.
-// NB: 32 rows of them.  One group of four waves: 56, 44, 36 KiB; two groups: 64 (NB = 2), 56 (NB = 1).
+// NB: 32 rows of them.  One group of four waves: 56, 44, 36 KiB; two groups: 64 (NB = 2), 56 (NB = 1).  A stage's factors lie behind its
+// weights, a copy for each wave (a wave waits for its own loads only): another KiB a stage, one group of waves.
 constexpr int fd_stages(int NB, int KG) { return NB == 4 || (NB == 2 && KG == 2) ? 3 : NB == 2 || KG == 2 ? 4 : 5; }
-constexpr int fd_group_bytes(int NB, int KG) { return fd_stages(NB, KG) * NB * 4096 + (fd_stages(NB, KG) - 1) * 4096; }
+constexpr int fd_weight_bytes(int OUT) { return OUT == OUT_FACTORS ? 5120 : 4096; }
+constexpr int fd_group_bytes(int NB, int KG, int OUT) { return fd_stages(NB, KG) * NB * 4096 + (fd_stages(NB, KG) - 1) * fd_weight_bytes(OUT); }
 
 // Piece q of row r of a stage lies at place q ^ fd_place(r / 2).  A 16-byte read from LDS takes its lanes in groups that hold
 // rows 0 .. 3 and 12 .. 15 of one pair of pieces with rows 4 .. 11 of the next pair: those must differ.  (With r / 2 itself every
@@ -220,19 +226,23 @@ __device__ __forceinline__ void fd_epilogue_gated(const GemmFParams& p, const v4
 template <int MODE, int SRC, int NR, int KG, bool TAIL, bool RN, int OUT>
 __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_t m0, const int tile_n, uint8_t* lds_all) {
     constexpr int NB = (NR + 1) / 2, BM = 16 * NR, A_BYTES = NB * 4096, NST = fd_stages(NB, KG), W_AT = NST * A_BYTES;
-    constexpr int A_LOADS = NB, W_LOADS = SRC == W_ROWS ? 4 : 1, LOADS = A_LOADS + W_LOADS;
-    constexpr bool SW = OUT != OUT_LINEAR;
+    constexpr int W_BYTES = fd_weight_bytes(OUT), GROUP_BYTES = fd_group_bytes(NB, KG, OUT);
+    constexpr bool SW = OUT == OUT_SWIGLU || OUT == OUT_GATED, FACTORS = OUT == OUT_FACTORS;
+    static_assert(!FACTORS || (MODE == MODE_F16 && SRC == W_TILES), "factors are fp16 and the copy's");
+    static_assert(KG * GROUP_BYTES <= 65536, "the loads into LDS have 16 bits for their place");
+    constexpr int A_LOADS = NB, W_LOADS = SRC == W_ROWS ? 4 : FACTORS ? 2 : 1, LOADS = A_LOADS + W_LOADS;
     const int lane = threadIdx.x & 63;
     const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wave_all & 3, group = KG == 1 ? 0 : wave_all >> 2;
-    uint8_t* const lds = lds_all + group * fd_group_bytes(NB, KG);
+    uint8_t* const lds = lds_all + group * GROUP_BYTES;
     const int j = lane & 15, g = lane >> 4;
     const int64_t ncol = (int64_t)tile_n * F_BN + 64 * wave + 4 * j;
     const bool col_ok = ncol < p.N;
     const int nst = (int)((p.K + F_BK - 1) / F_BK);
     const int64_t k_last = (int64_t)(nst - 1) * F_BK;
     // this group's stages: st0 .. st0 + mine - 1 (every group meets `rounds` barriers in the loop; mine >= 1)
-    const int rounds = KG == 1 ? nst : (nst + 1) / 2, st0 = group * rounds, mine = KG == 1 ? nst : min(rounds, nst - st0);
-    const int st_tail = group == KG - 1 ? mine - 1 : rounds;  // TAIL: the partial stage, if it is this group's
+    const int rounds = FACTORS ? p.part_stages : KG == 1 ? nst : (nst + 1) / 2, st0 = (FACTORS ? (int)blockIdx.y : group) * rounds;
+    const int mine = KG == 1 && !FACTORS ? nst : min(rounds, nst - st0);
+    const int st_tail = FACTORS ? nst - 1 - st0 : group == KG - 1 ? mine - 1 : rounds;  // TAIL: the partial stage, if it is this group's
 
     // A stage's row is 128 bytes of LDS, eight pieces of 16 at the places fd_place gives them.  A wave loads whole rows, eight
     // lanes each: lanes of a load that each have a row of their own take the cache four times as long.  Wave w loads rows
@@ -275,6 +285,7 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
     const int64_t w_step = SRC == W_TILES ? 256 : 16 * p.N;
     const uint8_t* a_next = (const uint8_t*)(p.X + m0 * p.K + (int64_t)st0 * F_BK);
     const uint8_t* w_next = p.W_T + st0 * w_step;
+    const uint16_t* f_next = FACTORS ? p.factors + (int64_t)st0 * F_BK : nullptr;  // (64 lanes load a stage's 128 bytes twice)
     uint32_t into = 0, w_into = W_AT;
     int st_next = 0;
     auto issue_a = [&](int b) {
@@ -284,16 +295,18 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
     auto issue_w = [&](int r) {
         const bool last = TAIL && st_next >= st_tail;
         const uint32_t wd = lds0 + w_into + (uint32_t)wave * 1024u;
-        if constexpr (SRC == W_TILES) dma16(wd, w_off[0], w_next);
+        if (FACTORS && r == 1) dma4(lds0 + w_into + 4096u + (uint32_t)wave * 256u, 4u * (lane & 31), f_next);
+        else if constexpr (SRC == W_TILES) dma16(wd, w_off[0], w_next);
         else if constexpr (SRC == W_ROWS16) dma16(wd, last ? w_tail[0] : w_off[0], w_next);
         else dma4(wd + 256u * r, last ? w_tail[r] : w_off[r], w_next);
     };
     auto next_buf = [](uint32_t b) { return b + A_BYTES == W_AT ? 0u : b + A_BYTES; };
-    auto next_wbuf = [](uint32_t b) { return b + 4096 == fd_group_bytes(NB, KG) ? (uint32_t)W_AT : b + 4096; };
+    auto next_wbuf = [](uint32_t b) { return b + W_BYTES == GROUP_BYTES ? (uint32_t)W_AT : b + W_BYTES; };
     auto advance = [&]() {  // past the end: the last stage again, never read
         st_next++;
         a_next += st_next < mine ? 2 * F_BK : 0;
         w_next += st_next < mine ? w_step : 0;
+        if constexpr (FACTORS) f_next += st_next < mine ? F_BK : 0;
         into = next_buf(into);
         w_into = next_wbuf(w_into);
     };
@@ -308,11 +321,16 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
     constexpr int RB = NB == 4 ? 4 : NR;
     u32x4 a_x[RB], a_y[RB], b0[4], b1[4];
     uint32_t raw[4];
+    u32x4 fac[2];  // FACTORS: of this lane's 16 k, two halves to a dword
     // lane (j, g): k = 16 g + 8 sub .. +7 of row 16 mb + j
     const uint32_t at_j = fd_place(j >> 1), frag_at[2] = {128u * j + 16u * ((2u * g) ^ at_j), 128u * j + 16u * ((2u * g + 1) ^ at_j)};
     auto frag = [&](uint32_t buf, int sub, int mb) { return *(const u32x4*)(lds + (buf + frag_at[sub]) + 2048 * mb); };
     auto read_raw = [&](uint32_t wbuf) {
         const uint8_t* src = lds + wbuf + wave * 1024;
+        if constexpr (FACTORS) {
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++) fac[sub] = *(const u32x4*)(lds + wbuf + 4096 + wave * 256 + 32 * g + 16 * sub);
+        }
         if constexpr (SRC == W_TILES) {
             if constexpr (SW) {  // lane (j, g)'s 16 bytes are those of columns 4 (j % 4) .. +3 of stored tile j / 4
                 const uint8_t* at = src + 256 * g + 128 * (j >> 3) + 8 * (j & 7);
@@ -340,6 +358,11 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
         const int t = e >> 2, d = e & 3, r = 2 * sub + (d >> 1), h = d & 1;
         const int q = SRC == W_TILES ? t : r, byte = SRC == W_TILES ? r : t;
         out[t][d] = perm(hi[q][2 * h + 1], hi[q][2 * h], ((uint32_t)(4 + byte) << 24) | (0x0Cu << 16) | ((uint32_t)byte << 8) | 0x0Cu);
+        if constexpr (FACTORS) {  // (the dword's codes are those of k = 8 sub + 2 d and the next one)
+            typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+            const uint32_t codes = out[t][d], by = fac[sub][d];
+            out[t][d] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, codes) * __builtin_bit_cast(half2_t, by));
+        }
     };
     // The first sub-step's tables are all of them (the copy) or those of raw[0] and raw[1] (rows).
     constexpr int T0 = SRC == W_TILES ? 16 : 8;
@@ -508,6 +531,18 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
         else if (p.epi.residual) fd_epilogue<MODE, true, RN>(p, sums, row0, g, ncol, left, ws, bs);
         else fd_epilogue<MODE, false, RN>(p, sums, row0, g, ncol, left, ws, bs);
     };
+    if (FACTORS && p.parts) {  // (uniform)
+        const int64_t pitch = (p.N + 3) / 4 * 4;
+        float* const out = p.parts + ((int64_t)blockIdx.y * p.M + m0) * pitch + ncol;
+#pragma unroll
+        for (int mb = 0; mb < NR; mb++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * mb + 4 * g + r;
+                if (stores && row < rows_left) *(v4f*)(out + row * pitch) = v4f{acc[mb][0][r], acc[mb][1][r], acc[mb][2][r], acc[mb][3][r]};
+            }
+        return;
+    }
     if constexpr (KG == 1) {
         if (stores) store(acc, m0, (int)rows_left);
     } else {
@@ -537,7 +572,7 @@ __device__ __forceinline__ void gemm_f16_tile(const GemmFParams& p, const int64_
 // NR: tiles of 16 NR rows.  NF > 0: an XCD's tiles from p.fine_from on are computed in tiles of 16 NF rows.
 template <int MODE, int SRC, int NR, int NF, int KG, bool TAIL, bool RN, int OUT>
 __global__ __launch_bounds__(256 * KG, KG == 2 || NR == 8 ? 2 : NR == 4 ? 3 : 4) void gemm_f16_kernel(GemmFParams p) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[KG * fd_group_bytes((NR + 1) / 2, KG)];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[KG * fd_group_bytes((NR + 1) / 2, KG, OUT)];
     // XCD-aware tile order: the 8 XCDs each take a contiguous run of tiles, walked in groups of four row tiles, so that one
     // XCD's L2 holds a compact block of rows and columns
     const uint32_t idx = blockIdx.x >> 3;
@@ -628,7 +663,7 @@ double gemm_f16_cost(int64_t M, int64_t N, int64_t K) {
 
 template <int MODE, int SRC, int NR, bool TAIL, bool RN = false, int OUT = OUT_LINEAR>
 static int launch_gemm_f16_cfg(GemmFParams p, hipStream_t st) {
-    const char* who = OUT == OUT_GATED ? "bt_ternary_gated_forward" : SRC == W_TILES ? "bt_ternary_linear_tiled_forward" : "bt_ternary_linear_packed_forward";
+    const char* who = OUT == OUT_FACTORS ? "bt_gated_grad_input" : OUT == OUT_GATED ? "bt_ternary_gated_forward" : SRC == W_TILES ? "bt_ternary_linear_tiled_forward" : "bt_ternary_linear_packed_forward";
     p.tiles_n = (int)ceil_div(p.N, F_BN);
     p.tiles_m = (int)ceil_div(p.M, 16 * NR);
     const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
@@ -649,7 +684,7 @@ static int launch_gemm_f16_cfg(GemmFParams p, hipStream_t st) {
             return check_launch(who);
         }
     }
-    if constexpr (NR != 8) {
+    if constexpr (NR != 8 && OUT != OUT_FACTORS) {
         if (NR == 3 || (total <= gemm_compute_units() && f16_splits_k(p.wstages))) {
             hipLaunchKernelGGL((gemm_f16_kernel<MODE, SRC, NR, 0, 2, TAIL, RN, OUT>), dim3((unsigned)(8 * p.per_xcd)), dim3(512), 0, st, p);
             return check_launch(who);
@@ -707,6 +742,91 @@ int launch_gemm_f16_gated(int mode, const void* X, const uint8_t* W_tiled, const
     double us;
     const int rows = gemm_f16_plan(M, N, K, &us);
     return mode == MODE_F16 ? launch_gemm_f16_rows<MODE_F16>(p, rows, W_TILES, 0, st) : launch_gemm_f16_rows<MODE_BF16>(p, rows, W_TILES, 0, st);
+}
+
+// ---- fp16 X [M, K] on a tiled copy whose weights of each k are multiplied by a factor ------------------------------------------
+
+// The sums of the parts, in order, and the output stage: a thread four columns
+__global__ __launch_bounds__(256) void gemm_f16_parts_kernel(const float* __restrict__ parts, int n, int64_t M, int64_t N, const float* scale, uint16_t* Y) {
+    const int64_t quads = (N + 3) / 4, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= M * quads) return;
+    const int64_t row = at / quads, col = 4 * (at - row * quads);
+    v4f sum = ((const v4f*)parts)[at];
+#pragma unroll 4
+    for (int i = 1; i < n; i++) sum += ((const v4f*)parts)[at + i * M * quads];
+    const float s = *scale;
+    uint16_t* const y = Y + row * N + col;
+    uint16_t h[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) h[t] = f32_to_f16_bits(epi_float(sum[t], s, 0.0f));
+    if (N % 4 == 0) {  // (uniform)
+        *(uint2*)y = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            if (col + t < N) y[t] = h[t];
+    }
+}
+
+// Rows of the tiles in units of 16 and runs of the stages.  A stage takes a workgroup 0.4 us however few there are, so a launch that would
+// leave compute units idle is cut along the contraction, into runs of eight stages and more, as many workgroups as run side by side at most; the
+// sums go through memory.  Priced in microseconds by a fit to 60 sizes (the choice takes 1.03 times as long as the best one, 1.2 at most).
+// One run / the choice (tiles of 16 rows x runs): 1 x 2560 x 13824 97 / 13 (2 x 27), 64 rows 97 / 20, 500 x 1100 x 5472 47 / 22 (4 x 6),
+// 1000 x 2560 x 13824 112 / 69 (8 x 3), 2048 rows 171 / 124 (8 x 3); 4096 rows 222 in one.
+struct F16FactorsPlan { int rows, parts, part_stages; };
+static F16FactorsPlan gemm_f16_factors_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t C = gemm_compute_units();
+    const int stages = (int)ceil_div(K, F_BK);
+    F16FactorsPlan best = {8, 1, stages};
+    if (gemm_whole_tiles()) return best;
+    const double least[3] = {4.5, 4.9, 4.1}, sums[3] = {2.2, 2.3, 4.1}, alone[3] = {0.20, 0.19, 0.21}, beside[3] = {0.24, 0.32, 0.49};
+    double us = 4.0 + (double)stages * (0.35 + 0.5 * f16_tail(ceil_div(M, 128) * ceil_div(N, F_BN)).rounds);
+    for (int i = 0; i < 3; i++) {
+        const int64_t tiles = ceil_div(M, 32 << i) * ceil_div(N, F_BN), slots = (4 - i) * C;  // (workgroups of 2, 4, 8 blocks of rows a compute unit)
+        for (int64_t want = i == 2 ? 2 : 1; want == 1 || (want <= stages / 8 && tiles * want <= slots); want++) {
+            const int64_t each = ceil_div(stages, want), parts = ceil_div(stages, each);
+            const double t = least[i] + (double)each * (alone[i] + beside[i] * (double)ceil_div(tiles * parts, C)) +
+                             (parts > 1 ? sums[i] + 1.5e-6 * (double)(parts * M * N) : 0.0);
+            if (t < us) { us = t; best = {2 << i, (int)parts, (int)each}; }
+        }
+    }
+    return best;
+}
+size_t gemm_f16_factors_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    const F16FactorsPlan plan = gemm_f16_factors_plan(M, N, K);
+    return plan.parts > 1 ? (size_t)plan.parts * (size_t)M * (size_t)(ceil_div(N, 4) * 4) * 4 : 0;
+}
+template <int NR>
+static int launch_gemm_f16_factors_rows(GemmFParams p, const F16FactorsPlan& plan, hipStream_t st) {
+    // (two instances: whole stages and rows of four columns, or any)
+    const bool any = p.K % F_BK != 0 || p.N % 4 != 0;
+    if (plan.parts == 1)
+        return any ? launch_gemm_f16_cfg<MODE_F16, W_TILES, NR, true, true, OUT_FACTORS>(p, st) : launch_gemm_f16_cfg<MODE_F16, W_TILES, NR, false, false, OUT_FACTORS>(p, st);
+    p.tiles_n = (int)ceil_div(p.N, F_BN);
+    p.tiles_m = (int)ceil_div(p.M, 16 * NR);
+    p.per_xcd = p.fine_from = (int)ceil_div((int64_t)p.tiles_m * p.tiles_n, 8);
+    const dim3 grid((unsigned)(8 * p.per_xcd), (unsigned)plan.parts), block(256);
+    if (any) hipLaunchKernelGGL((gemm_f16_kernel<MODE_F16, W_TILES, NR, 0, 1, true, true, OUT_FACTORS>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((gemm_f16_kernel<MODE_F16, W_TILES, NR, 0, 1, false, false, OUT_FACTORS>), grid, block, 0, st, p);
+    if (int rc = check_launch("bt_gated_grad_input")) return rc;
+    const int64_t quads = p.M * ceil_div(p.N, 4);
+    hipLaunchKernelGGL(gemm_f16_parts_kernel, dim3((unsigned)ceil_div(quads, 256)), dim3(256), 0, st, p.parts, plan.parts, p.M, p.N, (const float*)p.epi.scale, (uint16_t*)p.Y);
+    return check_launch("bt_gated_grad_input");
+}
+// factors [K rounded up to 64], zeros behind K; scale: of the output, one entry; workspace as above
+int launch_gemm_f16_factors(const void* X, const uint8_t* W_tiled, const uint16_t* factors, const float* scale, void* Y, int64_t M, int64_t N, int64_t K,
+                            void* workspace, hipStream_t st) {
+    const F16FactorsPlan plan = gemm_f16_factors_plan(M, N, K);
+    GemmFParams p = {};
+    p.X = (const uint16_t*)X; p.W_T = W_tiled; p.factors = factors; p.Y = Y;
+    p.epi.scale = scale; p.epi.scale_dtype = BT_F32; p.epi.scale_bcast = 1;
+    p.M = M; p.N = N; p.K = K; p.Kb = ceil_div(K, 4);
+    p.wstages = (int)ceil_div(K, F_BK);
+    p.tiles16 = tiles16_arg(N, W_LAYOUT_TILED);
+    p.parts = plan.parts > 1 ? (float*)workspace : nullptr;
+    p.part_stages = plan.part_stages;
+    return plan.rows == 8 ? launch_gemm_f16_factors_rows<8>(p, plan, st) : plan.rows == 4 ? launch_gemm_f16_factors_rows<4>(p, plan, st)
+                                                                         : launch_gemm_f16_factors_rows<2>(p, plan, st);
 }
 
 }  // namespace bt

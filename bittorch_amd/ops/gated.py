@@ -46,7 +46,7 @@ class _GatedLinear(torch.autograd.Function):
             h = _C.gated_masters_forward(x2, gate, up, gate_bias, up_bias, threshold_factor, as_half)
             return h.reshape(*x.shape[:-1], f)
         w, w_back, scale, bias = _C.gated_weights(gate, up, gate_bias, up_bias, threshold_factor, per_channel, as_half,
-                                                  back=keep and ctx.needs_input_grad[0], ranged=keep and x.dtype == torch.float16)
+                                                  back=keep and ctx.needs_input_grad[0])
         if x.dtype == torch.float32:
             # (the fp32 kernel of the masters' gradient takes four columns and more)
             x2 = F.pad(x2, (0, 4 - k)) if k < 4 else x2.contiguous()
@@ -56,7 +56,7 @@ class _GatedLinear(torch.autograd.Function):
         else:
             h, pre, x2 = _C.ternary_gated_forward(x2, w, scale, bias, f, keep)
         if keep:
-            ctx.save_for_backward(x2, pre, w_back, scale)
+            ctx.save_for_backward(x2, pre, w_back, _C.gated_split(scale, f) if x.dtype == torch.float16 else scale)
             ctx.shape = f, k
         return h.reshape(*x.shape[:-1], f)
 
@@ -77,16 +77,18 @@ class _GatedLinear(torch.autograd.Function):
         dx = dg = du = dgb = dub = None
         want_w, want_b = want_g or want_u, want_gb or want_ub
         b_dtype = (gb_dtype if gb_dtype == ub_dtype or not want_ub else ub_dtype if not want_gb else torch.float32) if want_b else None
-        g, db = _C.gated_grad(dh, pre, scale, b_dtype)
-        fp = g.shape[1] // 2
-        one = scale[2 * fp:]
-        if want_x:
+        fp, split = (f + 15) // 16 * 16, dh.dtype == torch.float16  # (split: scale is that of gated_split)
+        g, db = _C.gated_grad(dh, pre, scale[:2 * fp + 1], b_dtype)
+        one = scale[2 * fp:2 * fp + 1]
+        if want_x and split:
+            dx = _C.gated_grad_input(g, w_back, scale, f, k).reshape(*lead, k).to(ctx.x_dtype)
+        elif want_x:
             dx = _C.ternary_linear_tiled_forward(g, w_back, one, None, 2 * fp, k).reshape(*lead, k).to(ctx.x_dtype)
         if want_w and dh.dtype == torch.float32:
             dw, _ = _C.linear_grad_weight(g, x2, one)
             dg, du = (t.to(w_dtype).contiguous() for t in (dw[:f, :k], dw[fp:fp + f, :k]))
         elif want_w:
-            dw = _C.gated_grad_masters(g, x2, one, f, k, dh.dtype if w_dtype == dh.dtype else torch.float32)
+            dw = _C.gated_grad_masters(g, x2, scale[2 * fp + 16:4 * fp + 16] if split else one, f, k, dh.dtype if w_dtype == dh.dtype else torch.float32)
             dg, du = dw[:f].to(w_dtype), dw[f:].to(w_dtype)
         if want_b:
             dgb, dub = db[:f].to(gb_dtype) if want_gb else None, db[f:].to(ub_dtype) if want_ub else None

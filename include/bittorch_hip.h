@@ -255,6 +255,10 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *                and 2 Fp inputs, for bt_ternary_linear_tiled_forward on the gradient G;
  *       scale    [2 Fp + 1]: both layers' scales, zeros behind each, and a 1; bias [2 Fp] or NULL.
  *     bt_gated_range puts a power of two that no scale exceeds (within 2^-24 .. 2^15) in the place of that 1.
+ *     bt_gated_split does so and takes each scale apart for the gradient of fp16 rows, scale = m 2^f with m in [1/2, 1) (f within 24 below and
+ *     15 above the exponent of that power of two): split, bt_gated_split_bytes(F) bytes, holds the m [2 Fp], a 1, that power of two, from
+ *     entry 2 Fp + 16 on the 2^f [2 Fp], and from entry 4 Fp + 16 on in fp16 the 2^f over that power of two [2 Fp rounded up to 64], zeros
+ *     behind them.
  *     fp32 rows read W_pairs through bt_ternary_linear_tiled_forward (BT_EPI_NATURAL_FROM_PAIRS) and bt_swiglu.
  *     workspace: at least bt_gated_quantize_workspace_bytes(F,K,per_channel) bytes.
  *   bt_ternary_gated_forward: fp16 / bf16 rows X [B,K]; where K % 8 != 0 or X is not 16-byte aligned, X_padded [B, K rounded up to 8] takes
@@ -263,10 +267,11 @@ int bt_add_rmsnorm_backward(const void* sum, int r_dtype, const float* rstd, con
  *     of g's columns 2 i and 2 i + 1 and u's, low bits first.
  *   bt_gated_masters_forward: H [F] of one row X [K] (any x_dtype) straight from the masters, quantized as they are read, with a scale for
  *     each feature; bt_gated_masters_serves says whether a call of B rows is one of those.
- *   bt_gated_grad: G [B, 2 Fp] in dtype = d(H . dH)/d[g | u], each half times its scale over scale[2 Fp], which both products of G
- *     multiply by (fp16: with bt_gated_range, so that G has fp16's range for the gradient alone).  16-bit dtype: pre as above; BT_F32: [g | u]
- *     [B, 2 Fp] fp32.  dBias (optional) [2 F] in bias_dtype: the sums over the rows without scales; with it a workspace of
- *     bt_gated_grad_workspace_bytes(B,F).
+ *   bt_gated_grad: G [B, 2 Fp] in dtype = d(H . dH)/d[g | u], each half times its scale over scale[2 Fp] (fp16: split in the place of
+ *     scale, so that G has fp16's range for each feature's gradient).  16-bit dtype: pre as above; BT_F32: [g | u] [B, 2 Fp] fp32.  dBias
+ *     (optional) [2 F] in bias_dtype: the sums over the rows without scales; with it a workspace of bt_gated_grad_workspace_bytes(B,F).
+ *   bt_gated_grad_input: dX [B,K] fp16 of fp16 G made with split, on W_back whose weights are multiplied by split's powers of two.
+ *     workspace: at least bt_gated_grad_input_workspace_bytes(B,F,K) bytes.
  *   bt_gated_grad_weight: dW [2 F, K] (out_dtype: dtype or BT_F32), the masters' gradients one behind the other, = G^T X times the scalar
  *     factor (scale + 2 Fp): fp16 / bf16 G and rows X [B, K rounded up to 8] (values behind K are read, not used); sums and workspace
  *     as in bt_linear_grad_weight_16(B, 2 Fp, K rounded up to 8).  Each sum is rounded to dtype before the factor and after it.
@@ -278,11 +283,16 @@ int bt_gated_quantize(const void* gate, const void* up, int w_dtype, int64_t F, 
                       const void* gate_bias, const void* up_bias, int bias_dtype, uint8_t* W_pairs, uint8_t* W_back,
                       float* scale, float* bias, void* workspace, size_t workspace_bytes, void* stream);
 int bt_gated_range(float* scale, int64_t F, void* stream);
+size_t bt_gated_split_bytes(int64_t F);
+int bt_gated_split(float* scale, int64_t F, float* split, void* stream);
 int bt_ternary_gated_forward(const void* X, int x_dtype, void* X_padded, const uint8_t* W_pairs, const float* scale, const float* bias, void* H,
                              void* pre, int64_t B, int64_t F, int64_t K, void* stream);
 int bt_gated_masters_serves(int64_t B, int64_t K, int w_dtype, int per_channel);
 int bt_gated_masters_forward(const void* X, int x_dtype, const void* gate, const void* up, int w_dtype, double threshold_factor,
                              const void* gate_bias, const void* up_bias, int bias_dtype, void* H, int64_t F, int64_t K, void* stream);
+size_t bt_gated_grad_input_workspace_bytes(int64_t B, int64_t F, int64_t K);
+int bt_gated_grad_input(const void* G, const uint8_t* W_back, const float* split, void* dX, int64_t B, int64_t F, int64_t K, void* workspace,
+                        size_t workspace_bytes, void* stream);
 int bt_gated_grad_weight(const void* G, const void* X, int dtype, const float* factor, void* dW, int out_dtype, int64_t B, int64_t F,
                          int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 int bt_gated_grad_masters(const void* G, const void* X, int dtype, const float* scale, int64_t scale_len, void* dW, int out_dtype, int64_t B,

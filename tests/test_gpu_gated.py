@@ -686,3 +686,105 @@ def test_masters_gradient_refusals():
     assert need > 0 and grad(B=4096, F=16) == grad(B=4096, F=16, ws=4096, n=need - 1) == grad(B=4096, F=16, ws=4100, n=need) == -2
     with pytest.raises(RuntimeError, match="16-bit"):
         _C.gated_grad_masters(torch.zeros(4, 32), torch.zeros(4, 16), torch.zeros(32), 16, 16, torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masters", ["fp16", "autocast", "fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["one entry", "rows", "halves"])
+@pytest.mark.parametrize("rows,k,f", [(3, 96, 5), (70, 512, 340), (65, 333, 200), (300, 512, 256)])
+def test_scales_far_apart_in_fp16(rows, k, f, kind, masters):
+    """One large entry among masters of 0.003, features from 1e-4 to 1 (a spread of 1e4), one half 1000 times the other: every feature keeps
+    what fp16 keeps of its gradient."""
+    announce("gated scales apart", rows, k, f, kind, masters)
+    g = torch.Generator().manual_seed(rows + f)
+    x, dh = torch.randn(rows, k, generator=g).half().cuda(), (torch.randn(rows, f, generator=g) * 2.0 ** -12).half().cuda()
+    wg, wu = (torch.randn(f, k, generator=g) * 0.003 for _ in range(2))
+    if kind == "one entry":
+        wu[f // 2, k // 3] = 4.0
+    elif kind == "rows":
+        wg, wu = (w / 0.003 * 0.25 * 10.0 ** -(4 * torch.rand(f, 1, generator=g)) for w in (wg, wu))
+    else:
+        wu = wu * 1000
+    wt = {"fp16": torch.float16, "autocast": torch.float16, "fp32": torch.float32, "bf16": torch.bfloat16}[masters]
+    wg, wu = wg.to(wt).cuda(), wu.to(wt).cuda()
+    ref = _Reference(x, wg, wu, None, None, dh)
+    leaves = [(t.float() if masters == "autocast" else t).requires_grad_() for t in (x, wg, wu)]
+    with torch.autocast("cuda", enabled=masters == "autocast"):
+        h = _gated(*leaves)
+    assert h.dtype == torch.float16
+    _assert_fp16_gradients(leaves, h, dh, ref, rows, f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f,largest,spread", [(1, 0.7, 0), (16, 1.0, 3), (5000, 0.011, 30), (40, 3e-9, 20), (40, 1e-30, 5), (40, 3e38, 90), (8, 2.0 ** 15, 40)])
+def test_scales_taken_apart(f, largest, spread):
+    from bittorch_amd import _C
+    n = 2 * ((f + 15) // 16 * 16)
+    g = torch.Generator().manual_seed(f)
+    scale = torch.cat((largest * 2.0 ** -(spread * torch.rand(n, generator=g)), torch.tensor([1.0]))).cuda()
+    scale[n // 4], scale[n - 1] = largest, 0
+    before = scale.cpu()
+    split = _C.gated_split(scale, f)
+    scale, split = scale.cpu(), split.cpu()
+    assert split.numel() * 4 == _C._L.bt_gated_split_bytes(f) and torch.equal(scale[:n], before[:n])
+    top = min(15, max(-24, math.frexp(float(before[n // 4]))[1]))
+    own = [max(top - 24, min(top + 15, math.frexp(v)[1])) if v else top - 24 for v in before[:n].tolist()]
+    power = torch.tensor([2.0 ** e for e in own], dtype=torch.float64)
+    assert float(scale[n]) == float(split[n + 1]) == 2.0 ** top and float(split[n]) == 1
+    assert torch.equal(split[n + 16:2 * n + 16].double(), power)
+    assert torch.equal(split[:n], (before[:n].double() / power).float())
+    factors = split[2 * n + 16:].view(torch.float16)
+    assert torch.equal(factors[:n].double(), power / 2.0 ** top) and not factors[n:].any() and factors.numel() == (n + 63) // 64 * 64
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,f", [(1, 1, 1), (1, 640, 48), (7, 8, 2), (33, 264, 48), (63, 129, 90), (70, 2560, 688), (300, 1100, 546), (500, 1100, 2730), (600, 2560, 1040),
+                                      (1000, 2560, 2736), (129, 13824, 100), (2100, 4096, 520), (3000, 4098, 1030), (4096, 2560, 3456), (1300, 8192, 200)])
+def test_input_gradient_with_a_power_of_two_for_each_feature(rows, k, f):
+    """The product on its own, over factors from 2^-24 to 2^0 and a few above, in tiles of every height: against 64 bits, and the same bits again."""
+    announce("gated grad input", rows, k, f)
+    from bittorch_amd import _C
+    g = torch.Generator().manual_seed(rows + k + f)
+    fp = (f + 15) // 16 * 16
+    wg, wu = ((torch.randn(f, k, generator=g) * 0.05).half().cuda() for _ in range(2))
+    _, w_back, scale, _ = _C.gated_weights(wg, wu, back=True)
+    scale[:2 * fp] = 0.4 * 2.0 ** -(torch.rand(2 * fp, generator=g) * 22).cuda()
+    scale[f // 2] = 60000  # (a power of two of its own beyond the largest that the others are held against)
+    split = _C.gated_split(scale, f)
+    G = torch.randn(rows, 2 * fp, generator=g).half().cuda()
+    by = split[2 * fp + 16:4 * fp + 16].double()
+    codes = torch.zeros(2 * fp, k, dtype=torch.float64, device="cuda")
+    codes[:f], codes[fp:fp + f] = _ternary(wg)[0], _ternary(wu)[0]
+    got = _C.gated_grad_input(G, w_back, split, f, k)
+    terms = G.double() * by
+    want, size = terms @ codes, terms.abs() @ codes.abs()
+    bound = U * 2 * (2 * fp / 32 + 80) * size
+    bound = bound + 2.0 ** -11 * (want.abs() + bound) + 2.0 ** -25
+    fits = want.abs() + bound < 65504
+    assert bool((((got.double() - want).abs() <= bound) | ~fits).all()), float(((got.double() - want).abs() / bound)[fits].max())
+    assert torch.equal(got, _C.gated_grad_input(G, w_back, split, f, k))
+    guard = torch.full((rows * k + 64,), 7.0, dtype=torch.float16, device="cuda")
+    ws = _C._workspace(_C._L.bt_gated_grad_input_workspace_bytes(rows, f, k), G.device)
+    _C._status(_C._L.bt_gated_grad_input(G.data_ptr(), w_back.data_ptr(), split.data_ptr(), guard[32:].data_ptr(), rows, f, k,
+                                          _C._ptr(ws), 0 if ws is None else ws.numel(), _C._stream(G)))
+    assert bool((guard[:32] == 7).all()) and bool((guard[32 + rows * k:] == 7).all()) and torch.equal(guard[32:32 + rows * k].view(rows, k), got)
+
+
+def test_split_and_input_gradient_refusals():
+    from bittorch_amd import _C, _lib
+    lib, at = _lib.load(), 4096
+    assert lib.bt_gated_split_bytes(0) == lib.bt_gated_split_bytes(1 << 23) == 0 and lib.bt_gated_split_bytes(8) == 4 * (64 + 16) + 128
+    for args in ((None, 8, at), (at, 8, None), (at, 0, at), (at, 1 << 23, at), (at, 8, at + 4)):
+        assert lib.bt_gated_split(*args, None) == -1 and "bt_gated_split" in _lib.last_error()
+    grad = lambda G=at, W=at, s=at, dx=at, B=4, F=8, K=16, ws=None, n=0: lib.bt_gated_grad_input(
+        G, W, s, dx, B, F, K, ws, n, None)
+    for bad in (dict(G=None), dict(W=None), dict(s=None), dict(dx=None), dict(B=0), dict(F=0), dict(K=0), dict(F=1 << 23), dict(K=1 << 23), dict(B=1 << 31),
+                dict(F=(1 << 23) - 1), dict(F=1 << 20, K=1 << 20), dict(G=at + 8), dict(W=at + 128), dict(s=at + 4), dict(dx=at + 8)):
+        assert grad(**bad) == -1, bad
+        assert "bt_gated_grad_input" in _lib.last_error()
+    need = lib.bt_gated_grad_input_workspace_bytes(4, 1024, 16)
+    assert need > 0 and grad(F=1024) == grad(F=1024, ws=at, n=need - 1) == grad(F=1024, ws=at + 16, n=need) == -2
+    assert lib.bt_gated_grad_input_workspace_bytes(0, 8, 16) == 0
+    for call in (lambda: _C.gated_split(torch.ones(33), 16), lambda: _C.gated_grad_input(torch.zeros(4, 32), torch.zeros(1, dtype=torch.uint8), torch.zeros(8), 16, 16)):
+        with pytest.raises(RuntimeError):
+            call()
