@@ -56,13 +56,22 @@ class PackedWeightCache:
         self.key, self.value = None, None
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the current stream of that device is being captured into a graph."""
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _state(weight: Tensor) -> tuple:
     return weight._version, weight.data_ptr(), weight.dtype, weight.device
 
 
 class GatedWeightCache:
     """The packed weights of a gated pair (``_C.gated_weights``: both layers in one tiled copy, tiles of gate and up in turn), kept by the
-    same rules.  Another stream than the one that packed them waits for it; what a graph being captured packs is the graph's own and not kept."""
+    same rules.  Another stream than the one that packed them waits for it.  A graph being captured packs for itself, whether anything is kept
+    or not, and nothing of that is kept: its replays follow the masters, and read no memory that a later evaluation gives back."""
 
     __slots__ = ("key", "value", "stream", "packed")
 
@@ -72,28 +81,36 @@ class GatedWeightCache:
     def __reduce__(self):  # (a copy packs for itself)
         return GatedWeightCache, ()
 
+    @staticmethod
+    def _pack(gate, up):
+        from .. import _C
+
+        with torch.no_grad():
+            w, _, scale, bias = _C.gated_weights(gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)
+        return w, scale[:-1], bias
+
     def get(self, gate, up):
         from .. import _C
 
+        device = gate.weight.device
+        if _capturing(device):
+            return self._pack(gate, up)
         given = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
         key = (*(_state(t) for t in given), gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel))
         stream = _C._stream(gate.weight)
         if key == self.key:
-            if stream != self.stream and not torch.cuda.is_current_stream_capturing():  # (a capture starts behind a synchronization)
-                here = torch.cuda.current_stream(gate.weight.device)
+            if stream != self.stream:
+                here = torch.cuda.current_stream(device)
                 here.wait_event(self.packed)
                 for t in self.value:
                     if t is not None:
                         t.record_stream(here)
             return self.value
-        with torch.no_grad():
-            w, _, scale, bias = _C.gated_weights(gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)
-        value = w, scale[:-1], bias
-        if not torch.cuda.is_current_stream_capturing():
-            with torch.cuda.device(gate.weight.device):
-                packed = torch.cuda.Event()
-                packed.record()
-            self.key, self.value, self.stream, self.packed = key, value, stream, packed
+        value = self._pack(gate, up)
+        with torch.cuda.device(device):
+            packed = torch.cuda.Event()
+            packed.record()
+        self.key, self.value, self.stream, self.packed = key, value, stream, packed
         return value
 
     def forward(self, x: Tensor, gate, up) -> Tensor:

@@ -225,3 +225,39 @@ def test_kept_weights_on_other_streams_and_in_graphs():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want) and torch.equal(mlp(x), want)
+
+
+def _rewritten(device):
+    """Memory that was given back, taken again and overwritten."""
+    torch.cuda.synchronize()
+    return [torch.full((n,), 255, dtype=torch.uint8, device=device) for n in (512, 4096, 1 << 16, 1 << 18, 1 << 20, 3 << 20, 1 << 22) for _ in range(8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_graph_captured_on_kept_weights_follows_the_masters(bias, dt):
+    """Evaluated, captured, the masters changed, evaluated again and the memory of the first packing written over: the graph's replays are
+    the module's values."""
+    announce("gated mlp, captured warm", bias, dt)
+    mlp = _mlp(512, 768, seed=9, bias=bias).to(dt).cuda()
+    x = torch.randn(33, 512, generator=torch.Generator().manual_seed(8)).cuda().to(dt)
+    with torch.no_grad():
+        mlp.hidden(x)
+        assert mlp._packed.key is not None
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mlp.hidden(x)
+        for n in range(3):
+            for p in mlp.parameters():
+                p.mul_(-1.25)
+            if n == 1:
+                mlp.invalidate_packed_cache()
+            want = mlp.hidden(x).clone()
+            held = _rewritten(x.device)
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(mlp.hidden(x), want)
+            del held
