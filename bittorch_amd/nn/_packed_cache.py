@@ -28,34 +28,6 @@ import torch
 from torch import Tensor
 
 
-class PackedWeightCache:
-    __slots__ = ("key", "value")
-
-    def __init__(self) -> None:
-        self.key = None
-        self.value: Optional[Tuple[Tensor, Tensor, Optional[Tensor]]] = None
-
-    def get(self, weight: Tensor, threshold_factor: float, per_channel: bool) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
-        """``(packed_T uint8 [ceil(K/4), N], scale fp32 [N] or 0-dim, tiled)`` of the current weights; ``tiled`` is
-        the decode-tiled copy of ``packed_T`` (``_C.retile_weights``), or None where the tiled kernels' 32-bit
-        offsets do not reach."""
-        from .. import _C
-
-        key = (weight._version, weight.data_ptr(), weight.dtype, weight.device, float(threshold_factor),
-               bool(per_channel))
-        if key != self.key:
-            with torch.no_grad():
-                packed, scale, _ = _C.ternary_quantize_pack(weight.detach(), threshold_factor, per_channel)
-                n, k = weight.shape
-                tiled_bytes = ((n + 15) // 16) * ((((k + 3) // 4) + 15) // 16) * 256
-                tiled = _C.retile_weights(packed, k) if tiled_bytes < 2 ** 32 else None
-            self.key, self.value = key, (packed, scale, tiled)
-        return self.value
-
-    def clear(self) -> None:
-        self.key, self.value = None, None
-
-
 def _capturing(device: torch.device) -> bool:
     """Whether the current stream of that device is being captured into a graph."""
     if device.index == torch.cuda.current_device():
@@ -68,10 +40,10 @@ def _state(weight: Tensor) -> tuple:
     return weight._version, weight.data_ptr(), weight.dtype, weight.device
 
 
-class GatedWeightCache:
-    """The packed weights of a gated pair (``_C.gated_weights``: both layers in one tiled copy, tiles of gate and up in turn), kept by the
-    same rules.  Another stream than the one that packed them waits for it.  A graph being captured packs for itself, whether anything is kept
-    or not, and nothing of that is kept: its replays follow the masters, and read no memory that a later evaluation gives back."""
+class _KeptWeights:
+    """Packed weights and what they were packed of.  Another stream than the one that packed them waits for it.  A graph being captured
+    packs for itself, whether anything is kept or not, and nothing of that is kept: its replays follow the masters, and read no memory that a
+    later evaluation gives back."""
 
     __slots__ = ("key", "value", "stream", "packed")
 
@@ -79,7 +51,59 @@ class GatedWeightCache:
         self.clear()
 
     def __reduce__(self):  # (a copy packs for itself)
-        return GatedWeightCache, ()
+        return type(self), ()
+
+    def clear(self) -> None:
+        self.key, self.value, self.stream, self.packed = None, None, None, None
+
+    def _kept(self, weight: Tensor, key: tuple, pack):
+        from .. import _C
+
+        device, stream = weight.device, _C._stream(weight)
+        if key == self.key:
+            if stream != self.stream:
+                here = torch.cuda.current_stream(device)
+                here.wait_event(self.packed)
+                for t in self.value:
+                    if t is not None:
+                        t.record_stream(here)
+            return self.value
+        value = pack()
+        with torch.cuda.device(device):
+            packed = torch.cuda.Event()
+            packed.record()
+        self.key, self.value, self.stream, self.packed = key, value, stream, packed
+        return value
+
+
+class PackedWeightCache(_KeptWeights):
+    __slots__ = ()
+
+    @staticmethod
+    def _pack(weight: Tensor, threshold_factor: float, per_channel: bool) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
+        from .. import _C
+
+        with torch.no_grad():
+            packed, scale, _ = _C.ternary_quantize_pack(weight.detach(), threshold_factor, per_channel)
+            n, k = weight.shape
+            tiled_bytes = ((n + 15) // 16) * ((((k + 3) // 4) + 15) // 16) * 256
+            return packed, scale, _C.retile_weights(packed, k) if tiled_bytes < 2 ** 32 else None
+
+    def get(self, weight: Tensor, threshold_factor: float, per_channel: bool) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
+        """``(packed_T uint8 [ceil(K/4), N], scale fp32 [N] or 0-dim, tiled)`` of the current weights; ``tiled`` is
+        the decode-tiled copy of ``packed_T`` (``_C.retile_weights``), or None where the tiled kernels' 32-bit
+        offsets do not reach."""
+        pack = lambda: self._pack(weight, threshold_factor, per_channel)
+        if _capturing(weight.device):
+            return pack()
+        return self._kept(weight, (*_state(weight), float(threshold_factor), bool(per_channel)), pack)
+
+
+class GatedWeightCache(_KeptWeights):
+    """The packed weights of a gated pair (``_C.gated_weights``: both layers in one tiled copy, tiles of gate and up in turn), kept by the
+    same rules."""
+
+    __slots__ = ()
 
     @staticmethod
     def _pack(gate, up):
@@ -90,28 +114,12 @@ class GatedWeightCache:
         return w, scale[:-1], bias
 
     def get(self, gate, up):
-        from .. import _C
-
-        device = gate.weight.device
-        if _capturing(device):
-            return self._pack(gate, up)
+        pack = lambda: self._pack(gate, up)
+        if _capturing(gate.weight.device):
+            return pack()
         given = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
         key = (*(_state(t) for t in given), gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel))
-        stream = _C._stream(gate.weight)
-        if key == self.key:
-            if stream != self.stream:
-                here = torch.cuda.current_stream(device)
-                here.wait_event(self.packed)
-                for t in self.value:
-                    if t is not None:
-                        t.record_stream(here)
-            return self.value
-        value = self._pack(gate, up)
-        with torch.cuda.device(device):
-            packed = torch.cuda.Event()
-            packed.record()
-        self.key, self.value, self.stream, self.packed = key, value, stream, packed
-        return value
+        return self._kept(gate.weight, key, pack)
 
     def forward(self, x: Tensor, gate, up) -> Tensor:
         """``silu(gate(x)) * up(x)`` as ``TernarySwiGLU`` computes it."""
@@ -121,9 +129,6 @@ class GatedWeightCache:
         f = gate.out_features
         h = _C.ternary_linear_tiled_forward(x.contiguous(), w, scale, bias, gate.in_features, scale.numel(), swiglu_pairs=True)
         return h if h.shape[-1] == f else h[..., :f].contiguous()
-
-    def clear(self) -> None:
-        self.key, self.value, self.stream, self.packed = None, None, None, None
 
 
 def cache_usable(x: Tensor, weight: Tensor) -> bool:

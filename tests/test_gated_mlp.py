@@ -261,3 +261,56 @@ def test_a_graph_captured_on_kept_weights_follows_the_masters(bias, dt):
             torch.cuda.synchronize()
             assert torch.equal(out, want) and torch.equal(mlp.hidden(x), want)
             del held
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("warm", [False, True])
+@pytest.mark.parametrize("cls", [bt.nn.TernaryLinear, bt.nn.TernaryLinearCUDA])
+def test_a_layer_captured_in_evaluation_follows_its_master(cls, warm):
+    """As above for a single layer, captured with its packed weights kept and without: what the capture packed is written by its replays
+    only, so an evaluation behind the capture does not read it."""
+    announce("layer captured", cls.__name__, warm)
+    torch.manual_seed(10)
+    layer = cls(512, 768).bfloat16().cuda()
+    x = torch.randn(40, 512, generator=torch.Generator().manual_seed(8)).cuda().bfloat16()
+    with torch.no_grad():
+        want = layer(x).clone()
+        if not warm:
+            layer.invalidate_packed_cache()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer(x)
+        assert (layer._packed.key is not None) == warm and torch.equal(layer(x), want)
+        for n in range(3):
+            layer.weight.mul_(-1.25)
+            want = layer(x).clone()
+            held = _rewritten(x.device)
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(layer(x), want)
+            del held
+
+
+@pytest.mark.gpu
+def test_a_layers_kept_weights_on_another_stream():
+    announce("layer, kept weights on another stream")
+    torch.manual_seed(11)
+    layer = bt.nn.TernaryLinear(512, 768).bfloat16().cuda()
+    x = torch.randn(40, 512, generator=torch.Generator().manual_seed(8)).cuda().bfloat16()
+    busy = torch.randn(4096, 4096, device="cuda")
+    with torch.no_grad():
+        want = layer(x).clone()
+        layer.weight.mul_(1.0)  # (the same values, packed anew)
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                busy = busy @ busy * 1e-3
+            first = layer(x)  # packs behind all of that
+        second = layer(x)  # this stream has not waited for it
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want)
+        copied = copy.deepcopy(layer)
+        assert copied._packed.key is None and torch.equal(copied(x), want)
