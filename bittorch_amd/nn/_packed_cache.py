@@ -5,7 +5,8 @@ The reference re-runs ``ternary_quantize`` on the master weights in every forwar
 The result depends on the weights only, so a forward that cannot be a training step (gradient
 mode off, or frozen weights) keeps it until the weights change: the key is the parameter's
 version counter (every tracked in-place update, ``load_state_dict`` or optimizer step bumps it),
-its storage address, dtype and device, and the quantizer's two settings.  Such a forward then
+its storage address, dtype and device, and the quantizer's two settings, and the tensor has to be the
+one that was packed (another may lie at its address; a parametrized weight is another at every reading).  Such a forward then
 reads K*N/4 bytes of packed weights instead of 4*K*N bytes of masters -- and reads them from a decode-tiled copy
 built next to the packed bytes (``_C.retile_weights``; whole-cache-line loads: what ``TernaryLinearInference`` runs
 on), which such a module then holds as well, another K*N/4 bytes.  Up to 32 rows the output is the training forward's
@@ -22,7 +23,8 @@ write, e.g. ``with torch.no_grad(): w.copy_(...)``) makes the next forward re-qu
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import weakref
+from typing import Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -45,7 +47,7 @@ class _KeptWeights:
     packs for itself, whether anything is kept or not, and nothing of that is kept: its replays follow the masters, and read no memory that a
     later evaluation gives back."""
 
-    __slots__ = ("key", "value", "stream", "packed")
+    __slots__ = ("key", "of", "value", "stream", "packed")
 
     def __init__(self) -> None:
         self.clear()
@@ -54,13 +56,14 @@ class _KeptWeights:
         return type(self), ()
 
     def clear(self) -> None:
-        self.key, self.value, self.stream, self.packed = None, None, None, None
+        self.key, self.of, self.value, self.stream, self.packed = None, (), None, None, None
 
-    def _kept(self, weight: Tensor, key: tuple, pack):
+    def _kept(self, of: Sequence[Tensor], settings: tuple, pack):
         from .. import _C
 
-        device, stream = weight.device, _C._stream(weight)
-        if key == self.key:
+        key = (*(_state(t) for t in of), *settings)
+        device, stream = of[0].device, _C._stream(of[0])
+        if key == self.key and all(r() is t for r, t in zip(self.of, of)):
             if stream != self.stream:
                 here = torch.cuda.current_stream(device)
                 here.wait_event(self.packed)
@@ -72,7 +75,7 @@ class _KeptWeights:
         with torch.cuda.device(device):
             packed = torch.cuda.Event()
             packed.record()
-        self.key, self.value, self.stream, self.packed = key, value, stream, packed
+        self.key, self.of, self.value, self.stream, self.packed = key, tuple(weakref.ref(t) for t in of), value, stream, packed
         return value
 
 
@@ -96,7 +99,7 @@ class PackedWeightCache(_KeptWeights):
         pack = lambda: self._pack(weight, threshold_factor, per_channel)
         if _capturing(weight.device):
             return pack()
-        return self._kept(weight, (*_state(weight), float(threshold_factor), bool(per_channel)), pack)
+        return self._kept((weight,), (float(threshold_factor), bool(per_channel)), pack)
 
 
 class GatedWeightCache(_KeptWeights):
@@ -117,9 +120,8 @@ class GatedWeightCache(_KeptWeights):
         pack = lambda: self._pack(gate, up)
         if _capturing(gate.weight.device):
             return pack()
-        given = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
-        key = (*(_state(t) for t in given), gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel))
-        return self._kept(gate.weight, key, pack)
+        of = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
+        return self._kept(of, (gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel)), pack)
 
     def forward(self, x: Tensor, gate, up) -> Tensor:
         """``silu(gate(x)) * up(x)`` as ``TernarySwiGLU`` computes it."""

@@ -314,3 +314,47 @@ def test_a_layers_kept_weights_on_another_stream():
         assert torch.equal(first, want) and torch.equal(second, want)
         copied = copy.deepcopy(layer)
         assert copied._packed.key is None and torch.equal(copied(x), want)
+
+
+class _Sign(torch.nn.Module):
+    """A parametrization with a state of its own: the weight is a new tensor, without a history, at every reading."""
+
+    def __init__(self):
+        super().__init__()
+        self.by = torch.nn.Parameter(torch.ones(()))
+
+    def forward(self, w):
+        return w * self.by
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cls", [bt.nn.TernaryLinear, bt.nn.TernaryLinearCUDA])
+def test_kept_weights_of_a_weight_that_is_computed(cls):
+    """A new tensor at the address of one that is gone, of the same version, is not what was packed."""
+    announce("kept weights, computed weight", cls.__name__)
+    torch.manual_seed(12)
+    layer = cls(64, 48, bias=False).cuda()
+    torch.nn.utils.parametrize.register_parametrization(layer, "weight", _Sign())
+    x = torch.randn(5, 64, device="cuda")
+    with torch.no_grad():
+        for _ in range(3):
+            before = layer(x).clone()
+            layer.parametrizations.weight[0].by.neg_()
+            assert torch.equal(layer(x), -before) and before.any()
+
+
+@pytest.mark.gpu
+def test_kept_weights_of_a_parameter_put_in_the_place_of_another():
+    announce("kept weights, parameter replaced")
+    torch.manual_seed(13)
+    mlp, other = _mlp(512, 768).cuda(), None
+    x = torch.randn(33, 512, device="cuda")
+    with torch.no_grad():
+        for layer in (mlp.gate, mlp.down):
+            mlp(x)
+            at, version, values = layer.weight.data_ptr(), layer.weight._version, -layer.weight.cpu()
+            del layer.weight
+            layer.weight = torch.nn.Parameter(values.cuda())
+            while layer.weight._version < version:
+                layer.weight.mul_(1.0)
+            assert torch.equal(mlp(x), copy.deepcopy(mlp)(x)), (at == layer.weight.data_ptr(), version)
