@@ -133,10 +133,12 @@ class GatedWeightCache(_KeptWeights):
         return h if h.shape[-1] == f else h[..., :f].contiguous()
 
 
-def cache_usable(x: Tensor, weight: Tensor) -> bool:
-    """The cache holds the quantization of the stored weights in their own dtype.  A training forward
-    re-quantizes (see above).  Under autocast the autograd function quantizes an fp16 copy instead
-    (reference semantics), and float64 runs on the dense entry point, so neither uses it."""
-    if torch.is_grad_enabled() and weight.requires_grad:
+def cache_usable(x: Tensor, *of: Tensor) -> bool:
+    """The cache holds the quantization of the stored weights (``of``, with the biases where those are kept too) in their own dtype.  A
+    training forward re-quantizes (see above).  Under autocast the autograd function quantizes an fp16 copy instead
+    (reference semantics), and float64 runs on the dense entry point, so neither uses it.  A tensor made in inference
+    mode has no version counter."""
+    learning = torch.is_grad_enabled()
+    if any((learning and t.requires_grad) or t.is_inference() or t.dtype == torch.float64 for t in of):
         return False
-    return (not torch.is_autocast_enabled() and weight.dtype != torch.float64 and x.dtype != torch.float64)
+    return not torch.is_autocast_enabled() and x.dtype != torch.float64

@@ -46,8 +46,8 @@ class TernaryGatedMLP(nn.Module):
                  and gate.threshold_factor == up.threshold_factor and gate.per_channel == up.per_channel and h.dtype != torch.float64)
         if not alike or not gate._should_use_cuda_kernel(h):
             return F.silu(gate(h)) * up(h)
-        learns = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, gate.bias, up.bias))
-        if not learns and cache_usable(h, gate.weight) and cache_usable(h, up.weight):
+        of = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
+        if cache_usable(h, *of) and not (torch.is_grad_enabled() and h.requires_grad):
             return self._packed.forward(h, gate, up)
         from ..ops.gated import ternary_gated_linear
         return ternary_gated_linear(h, gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)

@@ -358,3 +358,18 @@ def test_kept_weights_of_a_parameter_put_in_the_place_of_another():
             while layer.weight._version < version:
                 layer.weight.mul_(1.0)
             assert torch.equal(mlp(x), copy.deepcopy(mlp)(x)), (at == layer.weight.data_ptr(), version)
+
+
+@pytest.mark.gpu
+def test_modules_made_in_inference_mode():
+    """Their parameters have no version counter: nothing is kept, and they are evaluated all the same."""
+    announce("kept weights, inference tensors")
+    with torch.inference_mode():
+        mlp = _mlp(64, 48, seed=14, bias=True).cuda()
+        x = torch.randn(5, 64, generator=torch.Generator().manual_seed(8)).cuda()
+        got = mlp(x)
+    other = _mlp(64, 48, seed=14, bias=True).cuda()
+    with torch.no_grad():
+        # (the pair without kept weights: silu and the projections rounded to fp32 at other places)
+        assert _norm_error(got, other(x.clone())) <= 1e-6
+    assert mlp._packed.key is None and mlp.down._packed.key is None
