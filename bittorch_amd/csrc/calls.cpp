@@ -643,6 +643,12 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
     }
 };
 
+// (a tangent, made for forward-mode derivatives, is left to Python, whose functions refuse it)
+bool has_tangent(std::initializer_list<const at::Tensor*> ts) {
+    for (const at::Tensor* t : ts)
+        if (t && t->_fw_grad(0).defined()) return true;
+    return false;
+}
 bool differentiated(std::initializer_list<const at::Tensor*> ts) {
     if (!at::GradMode::is_enabled()) return false;
     for (const at::Tensor* t : ts)
@@ -681,6 +687,7 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         weight = plain(a[2], device);
         ORDINARY(weight && weight->dim() == 1 && weight->size(0) == K && (weight->scalar_type() == x->scalar_type() || weight->scalar_type() == at::kFloat));
     }
+    ORDINARY(!has_tangent({x, residual, weight}));
     if (differentiated({x, residual, weight}))
         return tuple_of(AddRMSNorm::apply(*x, maybe(residual), maybe(weight), f.eps, f.store, f.quantize, f.operand_order, f.rowsum),
                         residual ? nullptr : a[0]);
@@ -833,6 +840,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     ORDINARY(x->size(-1) == K && (x->scalar_type() != at::kFloat || K >= 4));
     if (a[3] != Py_None) ORDINARY((gate_bias = vec(a[3], F, false, device)));
     if (a[4] != Py_None) ORDINARY((up_bias = vec(a[4], F, false, device)) && (!gate_bias || gate_bias->scalar_type() == up_bias->scalar_type()));
+    ORDINARY(!has_tangent({x, gate, up, gate_bias, up_bias}));
     if (differentiated({x, gate, up, gate_bias, up_bias}))
         return THPVariable_Wrap(GatedLinear::apply(*x, *gate, *up, maybe(gate_bias), maybe(up_bias), threshold, per_channel));
     return THPVariable_Wrap(gated_run(*x, *gate, *up, maybe(gate_bias), maybe(up_bias), threshold, per_channel, false, false).h);

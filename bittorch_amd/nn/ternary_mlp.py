@@ -19,6 +19,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
+from ..ops._autograd import differentiated
 from ._packed_cache import GatedWeightCache, cache_usable
 from .ternary_linear import BackendType, TernaryLinear
 from .ternary_linear_infer import TernaryLinearInference
@@ -47,7 +48,7 @@ class TernaryGatedMLP(nn.Module):
         if not alike or not gate._should_use_cuda_kernel(h):
             return F.silu(gate(h)) * up(h)
         of = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
-        if cache_usable(h, *of) and not (torch.is_grad_enabled() and h.requires_grad):
+        if cache_usable(h, *of) and not differentiated(h, *of):
             return self._packed.forward(h, gate, up)
         from ..ops.gated import ternary_gated_linear
         return ternary_gated_linear(h, gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)

@@ -23,6 +23,8 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
+from ._autograd import differentiated
+
 
 def swiglu(gate: Tensor, up: Tensor, store: bool = True, quantize: bool = False, operand_order: bool = False,
            return_rowsum: bool = False):
@@ -76,13 +78,14 @@ def add_rmsnorm(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor] 
     ``s`` is ``x``.  With ``quantize`` the per-row int8 form of ``y`` follows, ``(s, y, q, s_x)``, or takes its place,
     ``store=False``: ``(s, q, s_x)``; ``operand_order`` and ``return_rowsum`` as in :func:`act_quant_int8`.  The results are those of
     the addition, :func:`rmsnorm` and :func:`act_quant_int8` one after the other, bit for bit.  Differentiable in ``x``, ``residual``
-    and ``weight`` through ``s`` and ``y`` (once: no graph of the backward pass is kept); ``q`` carries no gradient."""
+    and ``weight`` through ``s`` and ``y`` (once: no graph of the backward pass is kept); ``q`` carries no gradient.  Forward-mode
+    derivatives are refused."""
     from .. import _C
 
     out = _C._N.add_rmsnorm(x, residual, weight, eps, store, quantize, operand_order, return_rowsum)
     if out is not None:
         return out
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+    if differentiated(x, residual, weight):
         out = _AddRMSNorm.apply(x, residual, weight, eps, store, quantize, operand_order, return_rowsum)
         return out if residual is not None else (x, *out)
     return _C.add_rmsnorm(x, residual, weight, eps, store, quantize, operand_order, return_rowsum)

@@ -16,6 +16,7 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from ..quant.ternary import ternary_quantize_ste
+from ._autograd import differentiated
 
 
 def _half(t: Optional[Tensor]) -> Optional[Tensor]:
@@ -124,7 +125,7 @@ def ternary_gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate
 
     On the GPU ``x`` and the masters are fp32, fp16 or bf16, in any combination; 16-bit results are rounded once, from fp32 projections.
     Differentiable (once) in all five tensors with the straight-through gradient of ``TernaryLinear``; the gradients of the masters and
-    biases have their dtype.  Under autocast it runs in fp16, as ``TernaryLinear``.  On the CPU: the same in plain torch operations."""
+    biases have their dtype.  Forward-mode derivatives are refused on the GPU.  Under autocast it runs in fp16, as ``TernaryLinear``.  On the CPU: the same in plain torch operations."""
     if x.is_cuda:
         from .. import _C
 
@@ -142,5 +143,5 @@ def ternary_gated_linear(x: Tensor, gate_weight: Tensor, up_weight: Tensor, gate
     kinds = (torch.float32, torch.float16, torch.bfloat16)
     if x.dtype not in kinds or gate_weight.dtype not in kinds or any(b is not None and b.dtype not in kinds for b in (gate_bias, up_bias)):
         raise RuntimeError("x, weights and biases must be float32, float16 or bfloat16")
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate_weight, up_weight, gate_bias, up_bias))
+    keep = differentiated(x, gate_weight, up_weight, gate_bias, up_bias)
     return _GatedLinear.apply(x, gate_weight, up_weight, gate_bias, up_bias, threshold_factor, per_channel, keep)

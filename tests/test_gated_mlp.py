@@ -373,3 +373,27 @@ def test_modules_made_in_inference_mode():
         # (the pair without kept weights: silu and the projections rounded to fp32 at other places)
         assert _norm_error(got, other(x.clone())) <= 1e-6
     assert mlp._packed.key is None and mlp.down._packed.key is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(grad):
+    """A tangent is refused, whichever argument has it and whatever the gradient mode; it is never dropped.  Calls without one go on."""
+    announce("forward mode", grad)
+    import torch.autograd.forward_ad as fa
+    mk = lambda *shape: torch.randn(*shape, device="cuda")
+    x, r, w, wg, wu, bg, bu = mk(4, 64), mk(4, 64), mk(64), mk(48, 64), mk(48, 64), mk(48), mk(48)
+    mlp = _mlp(64, 48, seed=15, bias=True).cuda().requires_grad_(False)
+    norm = lambda *a: bt.ops.add_rmsnorm(*a)
+    codes = lambda *a: bt.ops.add_rmsnorm(*a, store=False, quantize=True)
+    pair = lambda *a: bt.ops.ternary_gated_linear(*a)
+    biases = lambda a, g, u, b, c: torch.func.functional_call(mlp, {"gate.weight": g, "up.weight": u, "gate.bias": b, "up.bias": c}, (a,))
+    with fa.dual_level(), torch.set_grad_enabled(grad):
+        for call, args in ((norm, (x, r, w)), (norm, (x, None, w)), (codes, (x, r, w)), (pair, (x, wg, wu, bg, bu)), (pair, (x[:1], wg, wu)), (mlp, (x,)),
+                           (biases, (x, wg, wu, bg, bu))):
+            call(*args)
+            for n, t in enumerate(args):
+                if t is not None:
+                    with pytest.raises((NotImplementedError, RuntimeError), match="jvp"):
+                        call(*args[:n], fa.make_dual(t, torch.ones_like(t)), *args[n + 1:])
+            call(*args)
