@@ -25,13 +25,21 @@ from .ternary_linear import BackendType, TernaryLinear
 from .ternary_linear_infer import TernaryLinearInference
 
 
+def _called_as_it_is(layer: nn.Module) -> bool:
+    """Whether calling the layer is its forward and nothing else: no hooks, no forward of the instance's own."""
+    return not (layer._forward_pre_hooks or layer._forward_hooks or layer._backward_pre_hooks or layer._backward_hooks
+                or nn.modules.module._has_any_global_hook() or "forward" in layer.__dict__)
+
+
 class TernaryGatedMLP(nn.Module):
     """``down(silu(gate(h)) * up(h))`` of three ``TernaryLinear`` layers (``gate``, ``up``, ``down``: the keys of the state dict), for
     training: on the GPU the gated pair is one operator (``ops.ternary_gated_linear``: both masters ternarised in one pass, one product
     forward, two backward) and the residual connection and norm in front of it another (``ops.add_rmsnorm``).
 
     Without a gradient (evaluation) the packed weights are kept until the masters change, as in ``TernaryLinear``, and the values are
-    those of the converted module.  ``to_inference()`` gives that module, a ``TernarySwiGLU``."""
+    those of the converted module.  ``to_inference()`` gives that module, a ``TernarySwiGLU``.
+
+    Where ``gate`` or ``up`` has hooks, is a subclass or parametrized, or the two differ, they are called one by one."""
 
     def __init__(self, d_model: int, ffn: int, bias: bool = False, threshold_factor: float = 0.05, per_channel: bool = True,
                  backend: BackendType = "auto") -> None:
@@ -44,7 +52,8 @@ class TernaryGatedMLP(nn.Module):
         """``silu(gate(h)) * up(h)``."""
         gate, up = self.gate, self.up
         alike = (type(gate) is TernaryLinear and type(up) is TernaryLinear and gate.quantize and up.quantize
-                 and gate.threshold_factor == up.threshold_factor and gate.per_channel == up.per_channel and h.dtype != torch.float64)
+                 and gate.threshold_factor == up.threshold_factor and gate.per_channel == up.per_channel and h.dtype != torch.float64
+                 and _called_as_it_is(gate) and _called_as_it_is(up))
         if not alike or not gate._should_use_cuda_kernel(h):
             return F.silu(gate(h)) * up(h)
         of = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]

@@ -397,3 +397,68 @@ def test_forward_mode_derivatives_are_refused(grad):
                     with pytest.raises((NotImplementedError, RuntimeError), match="jvp"):
                         call(*args[:n], fa.make_dual(t, torch.ones_like(t)), *args[n + 1:])
             call(*args)
+
+
+def _layer_by_layer(mlp, h):
+    return F.silu(mlp.gate(h)) * mlp.up(h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("kind", ["forward", "pre", "backward", "backward pre", "global", "instance"])
+def test_hooks_of_both_layers_run(kind, grad):
+    """A layer with a hook is called, not read: the pair is then the two layers, as on the CPU."""
+    announce("gated mlp, hooks", kind, grad)
+    for which in ("gate", "up"):
+        mlp, seen = _mlp(64, 48, seed=16, bias=True).cuda(), []
+        layer, x = getattr(mlp, which), torch.randn(9, 64, device="cuda", requires_grad=True)
+        note = lambda m, *rest: seen.append(m)
+        handle = None
+        if kind == "forward":
+            handle = layer.register_forward_hook(lambda m, args, out: note(m) or out * 0)
+        elif kind == "pre":
+            handle = layer.register_forward_pre_hook(lambda m, args: note(m) or (args[0] * 2,))
+        elif kind == "backward":
+            handle = layer.register_full_backward_hook(note)
+        elif kind == "backward pre":
+            handle = layer.register_full_backward_pre_hook(note)
+        elif kind == "global":
+            handle = torch.nn.modules.module.register_module_forward_hook(note)
+        else:
+            inner = layer.forward
+            layer.forward = lambda h: note(layer) or inner(h) * 3
+        try:
+            with torch.set_grad_enabled(grad):
+                want = _layer_by_layer(mlp, x)
+                seen.clear()
+                got = mlp.hidden(x)
+                if grad:
+                    got.sum().backward()
+            assert torch.equal(got, want)
+            assert layer in seen or (not grad and kind.startswith("backward"))
+        finally:
+            if handle is not None:
+                handle.remove()
+
+
+@pytest.mark.gpu
+def test_weights_that_a_hook_computes():
+    """weight_norm and pruning set the weight in front of each call: two training steps, and an evaluation behind each."""
+    announce("gated mlp, weights computed in front of the call")
+    import torch.nn.utils.prune as prune
+    for change in (lambda m: torch.nn.utils.weight_norm(m), lambda m: prune.random_unstructured(m, "weight", 0.5)):
+        torch.manual_seed(17)
+        mlp = _mlp(64, 48, seed=17).cuda()
+        change(mlp.gate)
+        change(mlp.up)
+        x = torch.randn(9, 64, device="cuda")
+        opt = torch.optim.SGD(mlp.parameters(), lr=1.0)
+        for _ in range(2):
+            opt.zero_grad()
+            got, want = mlp.hidden(x), _layer_by_layer(mlp, x)
+            assert torch.equal(got, want)
+            got.square().sum().backward()
+            assert all(p.grad is not None for n, p in mlp.named_parameters() if not n.startswith("down"))
+            opt.step()
+            with torch.no_grad():
+                assert torch.equal(mlp.hidden(x), _layer_by_layer(mlp, x))
