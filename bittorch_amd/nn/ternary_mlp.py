@@ -54,9 +54,11 @@ class TernaryGatedMLP(nn.Module):
         alike = (type(gate) is TernaryLinear and type(up) is TernaryLinear and gate.quantize and up.quantize
                  and gate.threshold_factor == up.threshold_factor and gate.per_channel == up.per_channel and h.dtype != torch.float64
                  and _called_as_it_is(gate) and _called_as_it_is(up))
-        if not alike or not gate._should_use_cuda_kernel(h):
+        if not alike or not (gate._should_use_cuda_kernel(h) and up._should_use_cuda_kernel(h)):
             return F.silu(gate(h)) * up(h)
         of = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
+        if gate.weight.dtype != up.weight.dtype or any(t.dtype == torch.float64 for t in of):
+            return F.silu(gate(h)) * up(h)
         if cache_usable(h, *of) and not differentiated(h, *of):
             return self._packed.forward(h, gate, up)
         from ..ops.gated import ternary_gated_linear

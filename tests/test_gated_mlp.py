@@ -462,3 +462,26 @@ def test_weights_that_a_hook_computes():
             opt.step()
             with torch.no_grad():
                 assert torch.equal(mlp.hidden(x), _layer_by_layer(mlp, x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["gate", "up"])
+def test_layers_that_differ_in_backend_or_dtype(which):
+    announce("gated mlp, layers that differ", which)
+    x = torch.randn(9, 64, device="cuda")
+    mlp = _mlp(64, 48, seed=18, bias=True).cuda()
+    getattr(mlp, which).backend = "python"
+    assert torch.equal(mlp.hidden(x), _layer_by_layer(mlp, x))
+    with torch.no_grad():
+        assert torch.equal(mlp.hidden(x), _layer_by_layer(mlp, x))
+    for part, dtype in (("weight", torch.bfloat16), ("bias", torch.float64)):
+        mlp = _mlp(64, 48, seed=18, bias=True).cuda()
+        layer = getattr(mlp, which)
+        setattr(layer, part, torch.nn.Parameter(getattr(layer, part).detach().to(dtype)))
+        y = x.clone().requires_grad_()
+        out = mlp.hidden(y)
+        assert torch.equal(out, _layer_by_layer(mlp, y))
+        out.square().sum().backward()
+        assert getattr(layer, part).grad.dtype == dtype and y.grad is not None
+        with torch.no_grad():
+            assert torch.equal(mlp.hidden(x), _layer_by_layer(mlp, x))
