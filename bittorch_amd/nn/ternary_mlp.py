@@ -68,7 +68,7 @@ class TernaryGatedMLP(nn.Module):
         """``down(silu(gate(h)) * up(h)) [+ residual]`` with ``h = rmsnorm(x, norm_weight, eps)`` when ``eps`` is given and ``h = x``
         otherwise (the signature of ``TernarySwiGLU``)."""
         if eps is not None:
-            if x.is_cuda:
+            if x.is_cuda and x.dtype != torch.float64 and (norm_weight is None or norm_weight.dtype in (x.dtype, torch.float32)):
                 from ..ops.fused import add_rmsnorm
                 x = add_rmsnorm(x, None, norm_weight, eps)[1]
             else:

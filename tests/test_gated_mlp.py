@@ -485,3 +485,13 @@ def test_layers_that_differ_in_backend_or_dtype(which):
         assert getattr(layer, part).grad.dtype == dtype and y.grad is not None
         with torch.no_grad():
             assert torch.equal(mlp.hidden(x), _layer_by_layer(mlp, x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,wt", [(torch.float64, torch.float64), (torch.float64, None), (torch.float32, torch.bfloat16), (torch.float32, torch.float64)])
+def test_norms_that_the_kernel_does_not_take(dt, wt):
+    announce("gated mlp, norm", dt, wt)
+    mlp = _mlp(64, 48, seed=19).cuda()
+    x = torch.randn(5, 64, device="cuda", dtype=dt)
+    w = None if wt is None else (1 + 0.1 * torch.randn(64, device="cuda")).to(wt)
+    assert torch.equal(mlp(x, w, EPS), mlp(F.rms_norm(x, (64,), w, EPS)))
