@@ -22,7 +22,7 @@ from torch import Tensor
 from ..ops._autograd import differentiated
 from ._packed_cache import GatedWeightCache, cache_usable
 from .ternary_linear import BackendType, TernaryLinear
-from .ternary_linear_infer import TernaryLinearInference
+from .ternary_linear_infer import TernaryLinearInference, _generic_kernel_asked
 
 
 def _called_as_it_is(layer: nn.Module) -> bool:
@@ -59,7 +59,7 @@ class TernaryGatedMLP(nn.Module):
         of = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
         if gate.weight.dtype != up.weight.dtype or any(t.dtype == torch.float64 for t in of):
             return F.silu(gate(h)) * up(h)
-        if cache_usable(h, *of) and not differentiated(h, *of):
+        if cache_usable(h, *of) and not differentiated(h, *of) and not _generic_kernel_asked():  # (the kept copy is the tiled kernels')
             return self._packed.forward(h, gate, up)
         from ..ops.gated import ternary_gated_linear
         return ternary_gated_linear(h, gate.weight, up.weight, gate.bias, up.bias, gate.threshold_factor, gate.per_channel)

@@ -495,3 +495,18 @@ def test_norms_that_the_kernel_does_not_take(dt, wt):
     x = torch.randn(5, 64, device="cuda", dtype=dt)
     w = None if wt is None else (1 + 0.1 * torch.randn(64, device="cuda")).to(wt)
     assert torch.equal(mlp(x, w, EPS), mlp(F.rms_norm(x, (64,), w, EPS)))
+
+
+@pytest.mark.gpu
+def test_generic_kernels_in_evaluation(monkeypatch):
+    """BITTORCH_KERNEL=generic: the layers one by one, kept weights or not."""
+    announce("gated mlp, generic kernels")
+    mlp = _mlp(64, 48, seed=20, bias=True).cuda()
+    x = torch.randn(5, 64, device="cuda")
+    with torch.no_grad():
+        kept = mlp.hidden(x)
+        monkeypatch.setenv("BITTORCH_KERNEL", "generic")
+        from bittorch_amd import _C
+        monkeypatch.setattr(_C, "ternary_linear_tiled_forward", None)
+        got = mlp.hidden(x)
+        assert torch.equal(got, F.silu(mlp.gate(x)) * mlp.up(x)) and _norm_error(got, kept) <= 1e-5
