@@ -32,6 +32,10 @@ struct AddNormParams {
     int q_layout;
 };
 
+// HIP takes fewer than 2^32 threads along x and wraps beyond: workgroups that there may be 2^22 and more of go over x and y.
+static dim3 wide_grid(int64_t n) { return dim3((unsigned)std::min<int64_t>(n, 1 << 20), (unsigned)ceil_div(n, 1 << 20)); }
+__device__ __forceinline__ int64_t wide_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // WPR waves to a row (4: a workgroup per row; 1: four rows to a workgroup, without LDS or barriers), ITERS pieces of eight values a
 // lane: K <= 512 ITERS WPR.  All loads go out before the first value is used.
 template <int DT, int RT, int ITERS, int WPR, bool QUANT, bool RAG>
@@ -41,8 +45,8 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(AddNormParams p, int64
     __shared__ int part_i[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = WPR == 1 ? lane : (int)threadIdx.x;
     const int K = p.K;
-    const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + (WPR == 1 ? wave : 0);
-    if (row >= B) return;  // (WPR = 1: whole waves, and no barrier below; 4: never)
+    const int64_t row = wide_block() * (4 / WPR) + (WPR == 1 ? wave : 0);
+    if (row >= B) return;  // (WPR = 1: whole waves, and no barrier below; 4: whole workgroups)
     auto at = [&](int i) { return (i * 64 * WPR + t) * 8; };
     float v[ITERS][8];
     Raw8<DT> x[ITERS], w16[ITERS];
@@ -159,12 +163,13 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(AddNormParams p, int64
 
 // Rows below 8 or above 16384 values: a workgroup per row, element by element; the passes behind the first read the stored sum again.
 template <int DT, int RT>
-__global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(AddNormParams p) {
+__global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(AddNormParams p, int64_t B) {
     __shared__ double part_d[4];
     __shared__ float part_f[4];
     __shared__ int part_i[4];
     const int tid = threadIdx.x, K = p.K;
-    const int64_t row = blockIdx.x;
+    const int64_t row = wide_block();
+    if (row >= B) return;  // (whole workgroups)
     auto sum = [&](int k) {
         const float x = load_elem<DT>(p.X, row * p.ldx + k);
         return p.R ? round_to_dtype(__fadd_rn(x, load_elem<RT>(p.R, row * p.ldr + k)), RT) : x;
@@ -214,7 +219,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(AddNormParams p) {
 
 template <int DT, int RT, int ITERS, int WPR>
 static void launch_add_rmsnorm_cfg(const AddNormParams& p, int64_t B, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div(B, 4 / WPR)), block(256);
+    const dim3 grid = wide_grid(ceil_div(B, 4 / WPR)), block(256);
     if (p.K % 8 == 0) {
         if (p.Q) hipLaunchKernelGGL((add_rmsnorm_kernel<DT, RT, ITERS, WPR, true, false>), grid, block, 0, st, p, B);
         else hipLaunchKernelGGL((add_rmsnorm_kernel<DT, RT, ITERS, WPR, false, false>), grid, block, 0, st, p, B);
@@ -226,7 +231,7 @@ static void launch_add_rmsnorm_cfg(const AddNormParams& p, int64_t B, hipStream_
 template <int DT, int RT>
 static void launch_add_rmsnorm_dt(const AddNormParams& p, int64_t B, hipStream_t st) {
     if (p.K < 8 || p.K > 16384 || option(OPT_ROWOP_GENERIC)) {
-        hipLaunchKernelGGL((add_rmsnorm_any_kernel<DT, RT>), dim3((unsigned)B), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((add_rmsnorm_any_kernel<DT, RT>), wide_grid(B), dim3(256), 0, st, p, B);
         return;
     }
     // A wave to a row where there are rows for all of them and it holds the row in few registers; a workgroup's barriers and idle lanes
@@ -386,7 +391,8 @@ template <int DT, int RT>
 __global__ __launch_bounds__(256) void add_rmsnorm_grad_any_kernel(AddNormGradParams p) {
     __shared__ float part[4];
     const int tid = threadIdx.x, K = p.K;
-    const int64_t row = blockIdx.x, at = row * (int64_t)K;
+    const int64_t row = wide_block(), at = row * (int64_t)K;
+    if (row >= p.B) return;  // (whole workgroups)
     const float r = p.rstd[row];
     auto weighted = [&](int k) { return load_elem<DT>(p.dY, at + k) * (p.W ? load_elem_rt(p.W, p.w_f32 ? BT_F32 : DT, k) : 1.0f); };
     float dot = 0.0f;
@@ -419,7 +425,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_gradw_any_kernel(AddNormGradP
 __global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ parts, int64_t n, int64_t K, void* out, int dtype) {
     __shared__ float sums[16][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t k = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t k = wide_block() * 64 + lane;
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (four loads in flight)
     if (k < K) {
         int64_t i = wave;
@@ -440,7 +446,7 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restric
     }
 }
 int launch_column_sum(const float* parts, int64_t n, int64_t K, void* out, int out_dtype, hipStream_t st, const char* who) {
-    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)ceil_div(K, 64)), dim3(1024), 0, st, parts, n, K, out, out_dtype);
+    hipLaunchKernelGGL(column_sum_kernel, wide_grid(ceil_div(K, 64)), dim3(1024), 0, st, parts, n, K, out, out_dtype);
     return check_launch(who);
 }
 
@@ -464,7 +470,7 @@ template <int DT, int RT>
 static void launch_add_rmsnorm_grad(const AddNormGradParams& p, int64_t n, hipStream_t st) {
     const int K = p.K;
     if (grad_any(K)) {
-        hipLaunchKernelGGL((add_rmsnorm_grad_any_kernel<DT, RT>), dim3((unsigned)p.B), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((add_rmsnorm_grad_any_kernel<DT, RT>), wide_grid(p.B), dim3(256), 0, st, p);
         if (p.parts) hipLaunchKernelGGL((add_rmsnorm_gradw_any_kernel<DT, RT>), dim3((unsigned)ceil_div(K, 256), (unsigned)n), dim3(256), 0, st, p, ceil_div(p.B, n));
         return;
     }

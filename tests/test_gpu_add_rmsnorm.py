@@ -386,3 +386,55 @@ def test_refusals():
     assert need > 0 and back(dw=addr, ws=addr, n=need - 1) == -2 and back(dw=addr, ws=addr + 8, n=need) == -2
     assert lib.bt_add_rmsnorm_backward_workspace_bytes(0, 16) == 0
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k", [((1 << 24) + 5, 4), ((1 << 26) + 3, 8)])
+def test_more_rows_than_one_dimension_of_a_grid_has_threads(rows, k):
+    """A workgroup, or a wave, of its own for each of that many rows passes 2^32 threads."""
+    announce("add_rmsnorm", rows, k)
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    mk = lambda: torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    x, res, dy, w = mk(), mk(), mk(), (1 + 0.2 * torch.randn(k, generator=g, device="cuda")).bfloat16()
+    ends = [0, 1, 2, (1 << 20) - 1, 1 << 20, (1 << 22) - 1, 1 << 22, rows // 2, rows - 3, rows - 2, rows - 1]
+    got = ops.add_rmsnorm(x, res, w, EPS, quantize=True, return_rowsum=True)
+    assert torch.equal(got[0], (x.float() + res.float()).bfloat16())
+    for a, b in zip(got, ops.add_rmsnorm(x[ends], res[ends], w, EPS, quantize=True, return_rowsum=True)):
+        assert torch.equal(a[ends], b)
+    s, y = got[0], got[1]
+    # (each row on its own, in 32 bits: a wrong row is off by more than two steps of bf16)
+    want = s.float() * (s.float().square().mean(-1, keepdim=True) + EPS).rsqrt() * w.float()
+    assert float(((y.float() - want).abs() - 2.0 ** -7 * want.abs()).max()) <= 1e-30
+    del got, want, y
+    leaves = [t.requires_grad_() for t in (x, w)]
+    dx, dw = torch.autograd.grad(ops.add_rmsnorm(x, res, w, EPS)[1], leaves, dy)
+    few = x.detach()[ends].requires_grad_()
+    few_dx, = torch.autograd.grad(ops.add_rmsnorm(few, res[ends], w, EPS)[1], few, dy[ends])
+    assert torch.equal(dx[ends], few_dx) and bool(dx.isfinite().all())
+    terms, size = torch.zeros(k, dtype=torch.float64, device="cuda"), torch.zeros(k, dtype=torch.float64, device="cuda")
+    for a, b in zip(s.split(1 << 22), dy.split(1 << 22)):
+        t = a.double()
+        t = b.double() * t * (t.square().mean(-1, keepdim=True) + EPS).rsqrt()
+        terms += t.sum(0)
+        size += t.abs().sum(0)
+    # a chain of rows / 64 additions, each rounded by half a step of the sum so far, and bf16's own
+    bound = 2.0 ** -24 * (rows / 64 + 80) * size
+    assert bool(((dw.double() - terms).abs() <= bound + 2.0 ** -8 * terms.abs()).all())
+
+
+@pytest.mark.gpu
+def test_a_weight_of_more_columns_than_one_dimension_of_a_grid_has_threads():
+    announce("column sum", (1 << 28) + 70)
+    ops = _ops()
+    k = (1 << 28) + 70
+    x = torch.randn(1, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    w = torch.ones(k, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    dy = torch.ones(1, k, device="cuda", dtype=torch.bfloat16)
+    dw, = torch.autograd.grad(ops.add_rmsnorm(x, None, w, EPS)[1], w, dy)
+    r = 1 / (x.double().square().mean() + EPS).sqrt()
+    off = 0.0
+    for a, b in zip(dw.split(1 << 26), x[0].split(1 << 26)):
+        want = b.double() * r
+        off = max(off, float(((a.double() - want).abs() - (2.0 ** -8 + 1e-6) * want.abs()).max()))
+    assert off <= 1e-30
