@@ -25,6 +25,14 @@ enum { MODE_I8 = 0, MODE_F16 = 1, MODE_BF16 = 2 };
 // ---- host side: error text + launch check --------------------------------
 void set_error(const char* fmt, ...);
 int check_launch(const char* what);
+// HIP takes fewer than 2^32 threads along a dimension of a grid and wraps beyond, without an error (of 2^24 + 5 workgroups of 256 threads five
+// were launched): such a launch is not made, and the call's check_launch says so.
+bool launch_fits(const dim3& grid, const dim3& block);
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...)                                       \
+    do {                                                                                                \
+        if (bt::launch_fits(grid, block)) (kernel)<<<(grid), (block), (lds), (stream)>>>(__VA_ARGS__);  \
+    } while (0)
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

@@ -20,8 +20,23 @@ void set_error(const char* fmt, ...) {
     va_end(ap);
 }
 
+static thread_local bool g_too_large = false;
+
+bool launch_fits(const dim3& grid, const dim3& block) {
+    const uint64_t most = 1ull << 32;
+    const bool fits = (uint64_t)grid.x * block.x < most && (uint64_t)grid.y * block.y < most && (uint64_t)grid.z * block.z < most;
+    g_too_large = g_too_large || !fits;
+    return fits;
+}
+
 int check_launch(const char* what) {
     const hipError_t e = hipGetLastError();
+    const bool too_large = g_too_large;
+    g_too_large = false;
+    if (too_large) {
+        set_error("%s: more rows or columns than a launch has threads (2^32)", what);
+        return BT_ERR_LAUNCH;
+    }
     if (e != hipSuccess) {
         set_error("%s: HIP launch failed: %s", what, hipGetErrorString(e));
         return BT_ERR_LAUNCH;

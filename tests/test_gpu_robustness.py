@@ -213,3 +213,16 @@ def test_operands_that_start_inside_a_buffer(dtype):
         qa, sa = _C.act_quant_int8(xs)
         qb, sb = _C.act_quant_int8(xs.contiguous())
         assert torch.equal(qa, qb) and torch.equal(sa, sb)
+
+
+@pytest.mark.gpu
+def test_launches_of_too_many_threads_are_refused():
+    """HIP wraps a grid of 2^32 threads and computes a few rows of such a call; the library refuses it, and serves the next one."""
+    from bittorch_amd import ops
+    rows = (1 << 24) + 5
+    announce("rows beyond a launch", rows)
+    x = torch.ones(rows, 4, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda t: ops.rmsnorm(t), lambda t: ops.swiglu(t, t)):
+        with pytest.raises(RuntimeError, match="than a launch has threads"):
+            call(x)
+        assert call(x[:9]).shape == (9, 4)
