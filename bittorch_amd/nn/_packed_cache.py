@@ -30,10 +30,10 @@ import torch
 from torch import Tensor
 
 
-def _capturing(device: torch.device) -> bool:
-    """Whether the current stream of that device is being captured into a graph."""
-    if device.index == torch.cuda.current_device():
-        return torch.cuda.is_current_stream_capturing()
+def _capturing(device: torch.device, stream: int) -> bool:
+    """Whether `stream`, that device's current one, is being captured into a graph (the default stream cannot be)."""
+    if stream == 0:
+        return False
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
 
@@ -47,7 +47,7 @@ class _KeptWeights:
     packs for itself, whether anything is kept or not, and nothing of that is kept: its replays follow the masters, and read no memory that a
     later evaluation gives back."""
 
-    __slots__ = ("key", "of", "value", "stream", "packed")
+    __slots__ = ("held",)  # (one tuple, so that a call of another thread finds weights and what they are of together)
 
     def __init__(self) -> None:
         self.clear()
@@ -56,26 +56,30 @@ class _KeptWeights:
         return type(self), ()
 
     def clear(self) -> None:
-        self.key, self.of, self.value, self.stream, self.packed = None, (), None, None, None
+        self.held = None, (), None, None, None  # key, of, value, stream, packed
 
-    def _kept(self, of: Sequence[Tensor], settings: tuple, pack):
-        from .. import _C
+    @property
+    def key(self):
+        return self.held[0]
 
-        key = (*(_state(t) for t in of), *settings)
-        device, stream = of[0].device, _C._stream(of[0])
-        if key == self.key and all(r() is t for r, t in zip(self.of, of)):
-            if stream != self.stream:
-                here = torch.cuda.current_stream(device)
-                here.wait_event(self.packed)
-                for t in self.value:
-                    if t is not None:
-                        t.record_stream(here)
-            return self.value
-        value = pack()
-        with torch.cuda.device(device):
-            packed = torch.cuda.Event()
-            packed.record()
-        self.key, self.of, self.value, self.stream, self.packed = key, tuple(weakref.ref(t) for t in of), value, stream, packed
+    @property
+    def value(self):
+        return self.held[2]
+
+    def _kept(self, stream: int, of: Sequence[Tensor], key: tuple, pack):
+        held, refs, value, of_stream, packed = self.held
+        if key != held or any([r() is not t for r, t in zip(refs, of)]):
+            value = pack()
+            with torch.cuda.device(of[0].device):
+                packed = torch.cuda.Event()
+                packed.record()
+            self.held = key, tuple(weakref.ref(t) for t in of), value, stream, packed
+        elif stream != of_stream:
+            here = torch.cuda.current_stream(of[0].device)
+            here.wait_event(packed)
+            for t in value:
+                if t is not None:
+                    t.record_stream(here)
         return value
 
 
@@ -96,10 +100,13 @@ class PackedWeightCache(_KeptWeights):
         """``(packed_T uint8 [ceil(K/4), N], scale fp32 [N] or 0-dim, tiled)`` of the current weights; ``tiled`` is
         the decode-tiled copy of ``packed_T`` (``_C.retile_weights``), or None where the tiled kernels' 32-bit
         offsets do not reach."""
-        pack = lambda: self._pack(weight, threshold_factor, per_channel)
-        if _capturing(weight.device):
-            return pack()
-        return self._kept((weight,), (float(threshold_factor), bool(per_channel)), pack)
+        from .. import _C
+
+        stream = _C._stream(weight)
+        if _capturing(weight.device, stream):
+            return self._pack(weight, threshold_factor, per_channel)
+        key = *_state(weight), float(threshold_factor), bool(per_channel)
+        return self._kept(stream, (weight,), key, lambda: self._pack(weight, threshold_factor, per_channel))
 
 
 class GatedWeightCache(_KeptWeights):
@@ -117,11 +124,14 @@ class GatedWeightCache(_KeptWeights):
         return w, scale[:-1], bias
 
     def get(self, gate, up):
-        pack = lambda: self._pack(gate, up)
-        if _capturing(gate.weight.device):
-            return pack()
+        from .. import _C
+
+        stream = _C._stream(gate.weight)
+        if _capturing(gate.weight.device, stream):
+            return self._pack(gate, up)
         of = [t for t in (gate.weight, up.weight, gate.bias, up.bias) if t is not None]
-        return self._kept(of, (gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel)), pack)
+        key = *map(_state, of), gate.bias is None, up.bias is None, float(gate.threshold_factor), bool(gate.per_channel)
+        return self._kept(stream, of, key, lambda: self._pack(gate, up))
 
     def forward(self, x: Tensor, gate, up) -> Tensor:
         """``silu(gate(x)) * up(x)`` as ``TernarySwiGLU`` computes it."""

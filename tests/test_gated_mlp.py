@@ -510,3 +510,29 @@ def test_generic_kernels_in_evaluation(monkeypatch):
         monkeypatch.setattr(_C, "ternary_linear_tiled_forward", None)
         got = mlp.hidden(x)
         assert torch.equal(got, F.silu(mlp.gate(x)) * mlp.up(x)) and _norm_error(got, kept) <= 1e-5
+
+
+@pytest.mark.gpu
+def test_kept_weights_are_replaced_as_one():
+    """Whatever another thread reads in between, the weights it finds kept are those that the key beside them stands for."""
+    announce("kept weights, replaced as one")
+    from bittorch_amd.nn._packed_cache import PackedWeightCache
+    values = {}
+
+    class Watched(PackedWeightCache):
+        __slots__ = ()
+
+        def __setattr__(self, name, value):
+            super().__setattr__(name, value)
+            if getattr(self, "key", None) is not None:
+                assert self.value is values[self.key[0]]  # (by the weight's version)
+
+        def _pack(self, weight, *settings):
+            values[weight._version] = super()._pack(weight, *settings)
+            return values[weight._version]
+
+    cache, weight = Watched(), torch.nn.Parameter(torch.randn(48, 64, device="cuda"))
+    for n in range(3):
+        with torch.no_grad():
+            weight.mul_(-1.0)
+        assert cache.get(weight, 0.05, True) is cache.get(weight, 0.05, True) is values[weight._version]
