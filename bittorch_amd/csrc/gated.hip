@@ -15,8 +15,8 @@
 // runs over the output features, by the forward's kernel, and dW = G^T x by the weight gradient's (grad_w16.hip).  For bf16 a times
 // dg, not dg, is what is rounded, so that neither product has a scale for each feature.  fp16 has no range for a (0.01 where dg is 1e-4 would
 // leave 4 bits of it), and none for the ratio of two features' a either (one entry of 0.5 among masters of 0.003 is 40 of them): there a is
-// taken apart feature by feature (gated_range_kernel), a = m 2^f with m in [1/2, 1), and G = [m_g dg | m_u du] keeps what fp16 keeps of dg and
-// half of it.  dW's rows are multiplied by their 2^f in fp32, as they are stored; in dx's product, which sums over the features, 2^f goes with
+// taken apart feature by feature (gated_range_kernel), a = m 2^f with m in [1/2, 1), and G = [m_g dg | m_u du] has fp16's full
+// precision down to dg of 2^-13.  dW's rows are multiplied by their 2^f in fp32, as they are stored; in dx's product, which sums over the features, 2^f goes with
 // the codes as they are decoded, over the power of two above all of them, which is the output's scale.
 // fp32 rows: the same steps on the fp32 kernels and the same copies, the projections stored in fp32 and h by the SwiGLU row kernel.  (On the
 // packed bytes as rows the fp32 products take longer: 4096 x 4096 x 768 forward 74 us, 68 on the copy, its transpose 89 and 77.)

@@ -34,10 +34,11 @@ def _called_as_it_is(layer: nn.Module) -> bool:
 class TernaryGatedMLP(nn.Module):
     """``down(silu(gate(h)) * up(h))`` of three ``TernaryLinear`` layers (``gate``, ``up``, ``down``: the keys of the state dict), for
     training: on the GPU the gated pair is one operator (``ops.ternary_gated_linear``: both masters ternarised in one pass, one product
-    forward, two backward) and the residual connection and norm in front of it another (``ops.add_rmsnorm``).
+    forward, two backward; differentiable once) and the norm in front of it another (``ops.add_rmsnorm``, which a program can call itself
+    with the residual connection in front).
 
     Without a gradient (evaluation) the packed weights are kept until the masters change, as in ``TernaryLinear``, and the values are
-    those of the converted module.  ``to_inference()`` gives that module, a ``TernarySwiGLU``.
+    those of the converted module; a graph being captured packs for itself.  ``to_inference()`` gives that module, a ``TernarySwiGLU``.
 
     Where ``gate`` or ``up`` has hooks, is a subclass or parametrized, or the two differ, they are called one by one."""
 
