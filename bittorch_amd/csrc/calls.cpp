@@ -41,7 +41,8 @@ namespace {
     X(bt_ternary_linear_tensor_core_forward) X(bt_quantize_pack) X(bt_ternary_linear_grad_input) X(bt_linear_grad_weight)      \
     X(bt_linear_grad_weight_16) X(bt_unpack_dequant) X(bt_swiglu) X(bt_rmsnorm) X(bt_ternary_gemm_i8_tiled) \
     X(bt_ternary_swiglu_i8_tiled) X(bt_act_quant_i8_layout) X(bt_add_rmsnorm) X(bt_add_rmsnorm_backward)                       \
-    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_split) X(bt_gated_split_bytes) X(bt_gated_grad_input) X(bt_gated_grad_input_workspace_bytes) \
+    X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_split)     \
+    X(bt_gated_split_bytes) X(bt_gated_grad_input) X(bt_gated_grad_input_workspace_bytes)                                      \
     X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_masters) X(bt_gated_grad_workspace_bytes)                     \
     X(bt_gated_masters_serves) X(bt_gated_masters_forward)
 struct Library {
