@@ -1121,3 +1121,166 @@ def scale_grad_weight(G: Tensor, scale: Tensor) -> Tensor:
         _status(_L.bt_scale_grad_weight(G.data_ptr(), _DT[G.dtype], scale.data_ptr(), scale.numel(), out.data_ptr(),
                                         G.shape[0], G.shape[1], _stream(G)))
     return out
+
+
+def _token_rows(x: Tensor) -> Tensor:
+    """``(*, heads, D)`` as ``[tokens, heads, D]`` whose last dimension is contiguous: a view wherever one stride fits all tokens."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    return x if x.dim() == 3 else x.flatten(0, -3) if x.dim() > 3 else x.unsqueeze(0)
+
+
+def _rotary_checks(dim: int, inv_freq: Optional[Tensor], device) -> int:
+    if inv_freq is None:
+        return 0
+    _check(inv_freq.dim() == 1 and inv_freq.dtype in (torch.float32, torch.float64), "inv_freq must be 1D, float32 or float64")
+    _check(2 * inv_freq.shape[0] <= dim, f"inv_freq turns {2 * inv_freq.shape[0]} features, a head has {dim}")
+    _check(inv_freq.device == device, "All tensors must be on one device")
+    return 2 * inv_freq.shape[0]
+
+
+def rotary_args(q: Tensor, k: Optional[Tensor], positions: Tensor, inv_freq: Tensor) -> None:
+    _check(q.dim() >= 2, "q must be (*, heads, head_dim)")
+    _check(q.is_floating_point(), "q must be a floating-point tensor")
+    if k is not None:
+        _check(k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == q.shape[-1], "k must be (*, kv_heads, head_dim) of q's tokens")
+        _check(k.dtype == q.dtype and k.device == q.device, "k must match q's dtype and device")
+    _check(positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64")
+    _check(positions.device == q.device, "All tensors must be on one device")
+    _rotary_checks(q.shape[-1], inv_freq, q.device)
+
+
+def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, inv_freq: Tensor, interleaved: bool = False, amplitude: float = 1.0,
+           backward: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """``q`` and ``k`` ``(*, heads, D)`` turned by their positions (any shape that broadcasts to ``*``); ``backward``: by the opposite angles."""
+    rotary_args(q, k, positions, inv_freq)
+    _check(q.is_cuda, "All tensors must be CUDA")
+    dt = _dt(q, "q")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if k is not None and k.numel() == 0:
+        return rotary(q, None, positions, inv_freq, interleaved, amplitude, backward)[0], out[1]
+    if q.numel() == 0:
+        return out if k is None else (out[0], rotary(k, None, positions, inv_freq, interleaved, amplitude, backward)[0])
+    lead = q.shape[:-2]
+    pos = positions if positions.shape == lead else positions.expand(lead)
+    pos, freq = pos.contiguous(), inv_freq.contiguous()
+    q3, k3 = _token_rows(q), None if k is None else _token_rows(k)
+    with _on(q):
+        _status(_L.bt_rotary(
+            q3.data_ptr(), q3.stride(0), q3.stride(1), _ptr(k3), 0 if k3 is None else k3.stride(0), 0 if k3 is None else k3.stride(1), dt,
+            pos.data_ptr(), int(pos.dtype == torch.int64), _ptr(freq), int(freq.dtype == torch.float64), int(interleaved), float(amplitude),
+            int(backward), q3.shape[0], q3.shape[1], 0 if k3 is None else k3.shape[1], q3.shape[2], 2 * freq.shape[0], out[0].data_ptr(),
+            _ptr(out[1]), _stream(q)))
+    return out
+
+
+def cache_head_dim(dtype: torch.dtype, head_dim: int) -> int:
+    """Features that a cache keeps of a head: ``head_dim`` rounded up to 64 bytes."""
+    _check(dtype in _DT, "the cache must be float32, float16 or bfloat16")
+    _check(0 < head_dim <= 256, f"head_dim must be 1 .. 256, got {head_dim}")
+    return _L.bt_cache_head_dim(_DT[dtype], head_dim)
+
+
+def cache_args(rows: Tensor, kv_heads: Optional[int], k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor,
+               q_starts: Optional[Tensor]) -> None:
+    """What every call on the cache has to hold; ``rows``: the new tokens' ``[tokens, heads, D]``."""
+    _check(rows.dim() == 3, "k, v and q must be 3D [tokens, heads, head_dim]")
+    _check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "the caches must match, 4D [pages, kv_heads, page_size, features]")
+    _check(k_cache.dtype == rows.dtype == v_cache.dtype, "the caches must have the rows' dtype")
+    _check(k_cache.is_contiguous() and v_cache.is_contiguous(), "the caches must be contiguous")
+    _check(k_cache.shape[3] == cache_head_dim(rows.dtype, rows.shape[2]),
+           f"the caches keep {k_cache.shape[3]} features, a head of {rows.shape[2]} wants {cache_head_dim(rows.dtype, rows.shape[2])}")
+    _check(kv_heads is None or k_cache.shape[1] == kv_heads, "kv_heads don't match the caches")
+    page = k_cache.shape[2]
+    _check(page >= 32 and page & (page - 1) == 0 and k_cache.shape[0] > 0, "page_size must be a power of two from 32 on")
+    index = [t for t in (block_table, lengths, q_starts) if t is not None]
+    _check(all(t.dtype == torch.int32 for t in index), "block_table, lengths and q_starts must be int32")
+    _check(block_table.dim() == 2 and lengths.dim() == 1 and block_table.shape[0] == lengths.shape[0], "block_table must be 2D [sequences, width], lengths 1D")
+    _check(q_starts is None or (q_starts.dim() == 1 and q_starts.shape[0] == lengths.shape[0] + 1), "q_starts must be 1D [sequences + 1]")
+    _check(q_starts is not None or lengths.shape[0] == rows.shape[0], "without q_starts every sequence has one token")
+    _check(all(t.device == rows.device for t in (k_cache, v_cache, *index)), "All tensors must be on one device")
+    _check(rows.shape[0] == 0 or (lengths.shape[0] > 0 and block_table.shape[1] > 0), "there are tokens and no sequences")
+
+
+def append_args(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor, q_starts: Optional[Tensor],
+                q: Optional[Tensor], inv_freq: Optional[Tensor]) -> None:
+    cache_args(k, k.shape[1] if k.dim() == 3 else None, k_cache, v_cache, block_table, lengths, q_starts)
+    _check(v.shape == k.shape and v.dtype == k.dtype and v.device == k.device, "k and v must match")
+    if q is not None:
+        _check(q.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2] and q.dtype == k.dtype and q.device == k.device,
+               "q must be [tokens, heads, head_dim] of k's tokens and dtype")
+        _check(inv_freq is not None, "q is turned by inv_freq, which is not given")
+    _rotary_checks(k.shape[2], inv_freq, k.device)
+    a, b, size = k_cache.data_ptr(), v_cache.data_ptr(), k_cache.numel() * k_cache.element_size()
+    _check(a + size <= b or b + size <= a, "the caches share memory")
+
+
+def cache_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor, q_starts: Optional[Tensor],
+                 q: Optional[Tensor], inv_freq: Optional[Tensor], interleaved: bool, amplitude: float, first_position: int) -> Optional[Tensor]:
+    """The new tokens' keys (turned) and values to their pages; ``q`` turned, or None."""
+    append_args(k, v, k_cache, v_cache, block_table, lengths, q_starts, q, inv_freq)
+    _check(k.is_cuda, "All tensors must be CUDA")
+    dt = _dt(k, "k")
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k.numel() == 0:
+        return out
+    if q is not None and q.numel() == 0:
+        q = None
+    k, v = _token_rows(k), _token_rows(v)
+    q = None if q is None else _token_rows(q)
+    table, lengths = block_table.contiguous(), lengths.contiguous()
+    starts = None if q_starts is None else q_starts.contiguous()
+    freq = None if inv_freq is None else inv_freq.contiguous()
+    for cache in (k_cache, v_cache):
+        if not cache.is_inference():
+            torch.autograd.graph.increment_version(cache)
+    with _on(k):
+        _status(_L.bt_cache_append(
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _ptr(q), 0 if q is None else q.stride(0),
+            0 if q is None else q.stride(1), dt, _ptr(freq), int(freq is not None and freq.dtype == torch.float64), int(interleaved), float(amplitude),
+            int(first_position), k.shape[0], 0 if q is None else q.shape[1], k.shape[1], k.shape[2], 0 if freq is None else 2 * freq.shape[0],
+            k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], k_cache.shape[2], table.data_ptr(), table.shape[1], lengths.data_ptr(),
+            _ptr(starts), lengths.shape[0], _ptr(out), _stream(k)))
+    return out
+
+
+def attention_args(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor, q_starts: Optional[Tensor],
+                   scale: Optional[float], prefix_table: Optional[Tensor], prefix_length: int, max_length: Optional[int]) -> Tuple[float, int]:
+    """The checked call's scale and its bound of a sequence's length."""
+    cache_args(q, None, k_cache, v_cache, block_table, lengths, q_starts)
+    _check(k_cache.shape[1] > 0 and q.shape[1] % k_cache.shape[1] == 0, "heads must be a multiple of kv_heads")
+    page, most = k_cache.shape[2], block_table.shape[1] * k_cache.shape[2]
+    _check(prefix_length >= 0, "prefix_length is negative")
+    if prefix_length:
+        _check(prefix_table is not None and prefix_table.dim() == 1 and prefix_table.dtype == torch.int32 and prefix_table.device == q.device,
+               "prefix_table must be 1D int32 on q's device")
+        _check(prefix_length <= prefix_table.shape[0] * page, "prefix_length is beyond prefix_table")
+    if max_length is None:
+        max_length = most
+    _check(0 <= max_length <= most, f"max_length must be 0 .. {most}, what block_table holds")
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    _check(0.0 < scale < 3.0e38, "scale must be a positive number")
+    return scale, max_length
+
+
+def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor, q_starts: Optional[Tensor],
+                     scale: Optional[float], prefix_table: Optional[Tensor], prefix_length: int, return_lse: bool, max_length: Optional[int]):
+    """``out`` ``[tokens, heads, D]``, with ``return_lse`` also fp32 ``[tokens, heads]``."""
+    scale, longest = attention_args(q, k_cache, v_cache, block_table, lengths, q_starts, scale, prefix_table, prefix_length, max_length)
+    _check(q.is_cuda, "All tensors must be CUDA")
+    dt = _dt(q, "q")
+    (tokens, heads, dim), (pages, kv_heads, page, _), (n_seq, width) = q.shape, k_cache.shape, block_table.shape
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if q.numel():
+        q, table, lengths = _token_rows(q), block_table.contiguous(), lengths.contiguous()
+        starts = None if q_starts is None else q_starts.contiguous()
+        prefix = prefix_table.contiguous() if prefix_length else None
+        with _on(q):
+            ws = _workspace(_L.bt_cached_attention_workspace_bytes(tokens, heads, kv_heads, dim, page, width, longest, int(starts is not None), n_seq,
+                                                                   prefix_length), q.device)
+            _status(_L.bt_cached_attention(
+                q.data_ptr(), q.stride(0), q.stride(1), dt, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, table.data_ptr(), width, longest,
+                lengths.data_ptr(), _ptr(starts), n_seq, _ptr(prefix), prefix_length, scale, tokens, heads, kv_heads, dim, out.data_ptr(), _ptr(lse),
+                _ptr(ws), 0 if ws is None else ws.numel(), _stream(q)))
+    return (out, lse) if return_lse else out

@@ -23,6 +23,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
@@ -44,7 +45,8 @@ namespace {
     X(bt_add_rmsnorm_backward_workspace_bytes) X(bt_gated_quantize) X(bt_gated_quantize_workspace_bytes) X(bt_gated_split)     \
     X(bt_gated_split_bytes) X(bt_gated_grad_input) X(bt_gated_grad_input_workspace_bytes)                                      \
     X(bt_ternary_gated_forward) X(bt_gated_grad) X(bt_gated_grad_masters) X(bt_gated_grad_workspace_bytes)                     \
-    X(bt_gated_masters_serves) X(bt_gated_masters_forward)
+    X(bt_gated_masters_serves) X(bt_gated_masters_forward) X(bt_rotary) X(bt_cache_head_dim) X(bt_cache_append)                  \
+    X(bt_cached_attention_workspace_bytes) X(bt_cached_attention)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     BT_FUNCTIONS(X)
@@ -848,6 +850,221 @@ PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- positions, the paged cache and the attention over it ------------------------------------------------------------------
+
+// [tokens][heads][dim] with a stride for each of the first two
+struct HeadRows {
+    const void* data = nullptr;
+    int64_t tokens = 0, heads = 0, dim = 0, token = 0, head = 0;
+};
+bool head_rows(const at::Tensor& t, HeadRows* r) {
+    const int64_t d = t.dim();
+    if (d < 2 || tag(t.scalar_type()) < 0 || (t.stride(-1) != 1 && t.size(-1) != 1)) return false;
+    *r = {t.const_data_ptr(), 1, t.size(-2), t.size(-1), d > 2 ? t.stride(-3) : 0, t.stride(-2)};
+    for (int64_t i = d - 3; i >= 0; i--) {
+        if (i < d - 3 && t.stride(i) != t.stride(i + 1) * t.size(i + 1)) return false;
+        r->tokens *= t.size(i);
+    }
+    return true;
+}
+const at::Tensor* head_rows_of(PyObject* o, int device, HeadRows* r) {
+    const at::Tensor* t = on_device(o, device);
+    return t && head_rows(*t, r) ? t : nullptr;
+}
+// Frequencies as the library reads them
+const at::Tensor* frequencies(PyObject* o, int64_t dim, int device) {
+    const at::Tensor* f = plain(o, device);
+    return f && f->dim() == 1 && (f->scalar_type() == at::kFloat || f->scalar_type() == at::kDouble) && 2 * f->size(0) <= dim && !f->requires_grad() ? f : nullptr;
+}
+
+struct Turned {
+    at::Tensor q, k;
+};
+// LOCKED: the calling thread holds the interpreter lock, and lets go of it around the call
+template <bool LOCKED>
+Turned rotary_run(const at::Tensor& q, const HeadRows& qr, const at::Tensor* k, const HeadRows& kr, const at::Tensor& positions, const at::Tensor& freq,
+                  bool interleaved, double amplitude, bool backward) {
+    Turned o;
+    o.q = output(q.sizes(), q.scalar_type(), q);
+    if (k) o.k = output(k->sizes(), k->scalar_type(), *k);
+    void* st = stream_of(q.get_device());
+    const int dt = tag(q.scalar_type()), wide = positions.scalar_type() == at::kLong, f64 = freq.scalar_type() == at::kDouble;
+    const void *pos = positions.const_data_ptr(), *f = freq.const_data_ptr();
+    void *q_out = o.q.data_ptr(), *k_out = k ? o.k.data_ptr() : nullptr;
+    const int64_t rot = 2 * freq.size(0);
+    if constexpr (LOCKED)
+        call(lib.bt_rotary, qr.data, qr.token, qr.head, kr.data, kr.token, kr.head, dt, pos, wide, f, f64, interleaved ? 1 : 0, (float)amplitude, backward ? 1 : 0,
+             qr.tokens, qr.heads, kr.heads, qr.dim, rot, q_out, k_out, st);
+    else
+        check_status(lib.bt_rotary(qr.data, qr.token, qr.head, kr.data, kr.token, kr.head, dt, pos, wide, f, f64, interleaved ? 1 : 0, (float)amplitude,
+                                   backward ? 1 : 0, qr.tokens, qr.heads, kr.heads, qr.dim, rot, q_out, k_out, st));
+    return o;
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const MaybeTensor& k, const at::Tensor& positions, const at::Tensor& freq,
+                                 bool interleaved, double amplitude) {
+        HeadRows qr, kr;
+        head_rows(q, &qr);
+        if (k) head_rows(*k, &kr);
+        Turned o = rotary_run<true>(q, qr, k ? &*k : nullptr, kr, positions, freq, interleaved, amplitude, false);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({positions, freq});
+        ctx->saved_data["k"] = k.has_value();
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["amplitude"] = amplitude;
+        variable_list out{o.q};
+        if (k) out.push_back(o.k);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        const variable_list saved = ctx->get_saved_variables();
+        const bool has_k = ctx->saved_data["k"].toBool(), interleaved = ctx->saved_data["interleaved"].toBool();
+        const double amplitude = ctx->saved_data["amplitude"].toDouble();
+        Wanted w(ctx, 6, {true, has_k});
+        const bool graph = at::GradMode::is_enabled();
+        const at::NoGradGuard no_grad;
+        at::Tensor d[2];
+        for (int i = 0; i < (has_k ? 2 : 1); i++)
+            if (w.want[i] && incoming[i].defined()) d[i] = incoming[i];
+        const int first = d[0].defined() ? 0 : 1;
+        if (d[first].defined()) {
+            const c10::DeviceGuard guard(d[first].device());
+            HeadRows r[2];
+            for (int i = first; i < 2; i++)
+                if (d[i].defined() && !head_rows(d[i], &r[i])) {
+                    d[i] = d[i].contiguous();
+                    head_rows(d[i], &r[i]);
+                }
+            const bool both = first == 0 && d[1].defined();
+            Turned o = rotary_run<false>(d[first], r[first], both ? &d[1] : nullptr, both ? r[1] : HeadRows(), saved[0], saved[1], interleaved, amplitude, true);
+            w.grads[first] = o.q;
+            if (both) w.grads[1] = o.k;
+        }
+        return once("rotary", graph, std::move(w.grads), incoming);
+    }
+};
+
+// rotary(q, k, positions, inv_freq, interleaved, amplitude) -> (q, k), or q without k
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    int device;
+    bool interleaved;
+    double amplitude;
+    HeadRows qr, kr;
+    ORDINARY(n_args == 6 && here(a[0], &device) && as_bool(a[4], &interleaved) && as_float(a[5], &amplitude));
+    const at::Tensor *q = head_rows_of(a[0], device, &qr), *k = nullptr;
+    ORDINARY(q);
+    if (a[1] != Py_None) {
+        k = head_rows_of(a[1], device, &kr);
+        ORDINARY(k && k->dim() == q->dim() && k->scalar_type() == q->scalar_type() && kr.dim == qr.dim &&
+                 k->sizes().slice(0, k->dim() - 2) == q->sizes().slice(0, q->dim() - 2));
+    }
+    const at::Tensor *positions = plain(a[2], device), *freq = frequencies(a[3], qr.dim, device);
+    ORDINARY(positions && freq && (positions->scalar_type() == at::kLong || positions->scalar_type() == at::kInt) &&
+             positions->sizes() == q->sizes().slice(0, q->dim() - 2));
+    ORDINARY(!has_tangent({q, k}));
+    variable_list out;
+    if (differentiated({q, k})) out = Rotary::apply(*q, maybe(k), *positions, *freq, interleaved, amplitude);
+    else {
+        Turned o = rotary_run<true>(*q, qr, k, kr, *positions, *freq, interleaved, amplitude, false);
+        out = {std::move(o.q), std::move(o.k)};
+    }
+    if (!k) return THPVariable_Wrap(std::move(out[0]));
+    return tuple_of(out, nullptr);
+    END_HANDLE_TH_ERRORS
+}
+
+// What both calls on the cache share, as the library reads it
+struct CacheArgs {
+    const at::Tensor *k = nullptr, *v = nullptr, *table = nullptr, *lengths = nullptr, *starts = nullptr;
+    int64_t pages, kv_heads, page, width, sequences;
+};
+const at::Tensor* int32_of(PyObject* o, int64_t dim, int device) {
+    const at::Tensor* t = plain(o, device);
+    return t && t->dim() == dim && t->scalar_type() == at::kInt ? t : nullptr;
+}
+// a: k_cache, v_cache, block_table, lengths, q_starts; like: the rows
+bool cache_of(PyObject* const* a, const at::Tensor& like, const HeadRows& rows, int device, CacheArgs* c) {
+    c->k = plain(a[0], device), c->v = plain(a[1], device);
+    if (!c->k || !c->v || c->k->dim() != 4 || c->k->sizes() != c->v->sizes() || c->k->scalar_type() != like.scalar_type() ||
+        c->v->scalar_type() != like.scalar_type() || like.dim() != 3 || !aligned(*c->k, 16) || !aligned(*c->v, 16))
+        return false;
+    c->pages = c->k->size(0), c->kv_heads = c->k->size(1), c->page = c->k->size(2);
+    if (c->page < 32 || (c->page & (c->page - 1)) || c->k->size(3) != lib.bt_cache_head_dim(tag(like.scalar_type()), rows.dim)) return false;
+    c->table = int32_of(a[2], 2, device), c->lengths = int32_of(a[3], 1, device);
+    if (!c->table || !c->lengths || c->table->size(0) != c->lengths->size(0)) return false;
+    c->width = c->table->size(1), c->sequences = c->lengths->size(0);
+    if (a[4] == Py_None) return c->sequences == rows.tokens;
+    c->starts = int32_of(a[4], 1, device);
+    return c->starts && c->starts->size(0) == c->sequences + 1;
+}
+
+// cache_append(k, v, k_cache, v_cache, block_table, lengths, q_starts, q, inv_freq, interleaved, amplitude, first_position) -> q turned
+// (for a call without q Python's None is the answer and also says that the call was not ordinary: those are left to Python)
+PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    int device;
+    bool interleaved;
+    double amplitude;
+    int64_t first;
+    HeadRows kr, vr, qr;
+    CacheArgs c;
+    ORDINARY(n_args == 12 && here(a[0], &device) && as_bool(a[9], &interleaved) && as_float(a[10], &amplitude) && as_int(a[11], &first));
+    const at::Tensor *k = head_rows_of(a[0], device, &kr), *v = head_rows_of(a[1], device, &vr), *q = head_rows_of(a[7], device, &qr);
+    ORDINARY(k && v && q && cache_of(a + 2, *k, kr, device, &c) && v->sizes() == k->sizes() && v->scalar_type() == k->scalar_type() && q->dim() == 3 &&
+             qr.tokens == kr.tokens && qr.dim == kr.dim && q->scalar_type() == k->scalar_type() && c.kv_heads == kr.heads);
+    const at::Tensor* freq = frequencies(a[8], kr.dim, device);
+    ORDINARY(freq && !differentiated({k, v, q, c.k, c.v}) && !has_tangent({k, v, q, c.k, c.v}));
+    const char *kc = (const char*)c.k->data_ptr(), *vc = (const char*)c.v->data_ptr();
+    ORDINARY(kc + c.k->nbytes() <= vc || vc + c.v->nbytes() <= kc);
+    at::Tensor out = output(q->sizes(), q->scalar_type(), *q);
+    for (const at::Tensor* t : {c.k, c.v})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    void* st = stream_of(device);
+    call(lib.bt_cache_append, kr.data, kr.token, kr.head, vr.data, vr.token, vr.head, qr.data, qr.token, qr.head, tag(k->scalar_type()), freq->const_data_ptr(),
+         freq->scalar_type() == at::kDouble ? 1 : 0, interleaved ? 1 : 0, (float)amplitude, first, kr.tokens, qr.heads, kr.heads, kr.dim, 2 * freq->size(0),
+         c.k->data_ptr(), c.v->data_ptr(), c.pages, c.page, (const int32_t*)c.table->const_data_ptr(), c.width, (const int32_t*)c.lengths->const_data_ptr(),
+         c.starts ? (const int32_t*)c.starts->const_data_ptr() : nullptr, c.sequences, out.data_ptr(), st);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// cached_attention(q, k_cache, v_cache, block_table, lengths, q_starts, scale, prefix_table, prefix_length, return_lse, max_length) -> out or (out, lse)
+PyObject* cached_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    int device;
+    bool want_lse;
+    int64_t prefix, longest;
+    HeadRows qr;
+    CacheArgs c;
+    ORDINARY(n_args == 11 && here(a[0], &device) && as_int(a[8], &prefix) && as_bool(a[9], &want_lse) && prefix >= 0);
+    const at::Tensor *q = head_rows_of(a[0], device, &qr), *shared = nullptr;
+    ORDINARY(q && cache_of(a + 1, *q, qr, device, &c) && qr.heads % c.kv_heads == 0 && !differentiated({q, c.k, c.v}) && !has_tangent({q, c.k, c.v}));
+    double scale = 1.0 / std::sqrt((double)qr.dim);
+    if (a[6] != Py_None) ORDINARY(as_float(a[6], &scale));
+    ORDINARY(scale > 0.0 && scale < 3.0e38);
+    const int64_t most = c.width * c.page;
+    longest = most;
+    if (a[10] != Py_None) ORDINARY(as_int(a[10], &longest) && longest >= 0 && longest <= most);
+    if (prefix) {
+        shared = int32_of(a[7], 1, device);
+        ORDINARY(shared && prefix <= shared->size(0) * c.page);
+    }
+    const int64_t T = qr.tokens;
+    at::Tensor out = output(q->sizes(), q->scalar_type(), *q), lse;
+    if (want_lse) lse = output({T, qr.heads}, at::kFloat, *q);
+    const Scratch ws(lib.bt_cached_attention_workspace_bytes(T, qr.heads, c.kv_heads, qr.dim, c.page, c.width, longest, c.starts ? 1 : 0, c.sequences, prefix), *q);
+    void* st = stream_of(device);
+    call(lib.bt_cached_attention, qr.data, qr.token, qr.head, tag(q->scalar_type()), c.k->const_data_ptr(), c.v->const_data_ptr(), c.pages, c.page,
+         (const int32_t*)c.table->const_data_ptr(), c.width, longest, (const int32_t*)c.lengths->const_data_ptr(),
+         c.starts ? (const int32_t*)c.starts->const_data_ptr() : nullptr, c.sequences, shared ? (const int32_t*)shared->const_data_ptr() : nullptr, prefix,
+         (float)scale, T, qr.heads, c.kv_heads, qr.dim, out.data_ptr(), want_lse ? (float*)lse.data_ptr() : nullptr, ws.ptr(), ws.size(), st);
+    if (!want_lse) return THPVariable_Wrap(std::move(out));
+    return tuple_of({std::move(out), std::move(lse)}, nullptr);
+    END_HANDLE_TH_ERRORS
+}
+
 // generic_kernel_asked(): whether BITTORCH_KERNEL=generic, read now
 PyObject* generic_kernel_asked(PyObject*, PyObject* const*, Py_ssize_t) {
     const char* env = std::getenv("BITTORCH_KERNEL");
@@ -900,6 +1117,7 @@ PyObject* names(PyObject*, PyObject* const*, Py_ssize_t) {
 PyMethodDef methods[] = {METHOD(bind), METHOD(names), METHOD(stamp), METHOD(tiled_forward), METHOD(packed_forward), METHOD(tensor_core_forward),
                          METHOD(quantize_pack), METHOD(grad_input), METHOD(grad_weight),
                          METHOD(grad_weight_16), METHOD(unpack_dequant), METHOD(rmsnorm_int8), METHOD(swiglu_int8), METHOD(gemm_i8_tiled), METHOD(swiglu_i8_tiled), METHOD(act_quant_int8), METHOD(add_rmsnorm), METHOD(gated_linear),
+                         METHOD(rotary), METHOD(cache_append), METHOD(cached_attention),
                          METHOD(generic_kernel_asked), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Native host side of small calls (csrc/calls.cpp)", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

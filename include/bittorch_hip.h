@@ -537,6 +537,52 @@ int bt_scale_grad_weight(const void* G, int dtype, const float* scale, int64_t s
  */
 int bt_pack_ternary_i8(const int8_t* W_tern, int64_t N, int64_t K, uint8_t* packed_T, void* stream);
 
+/*
+ * The attention half of a block around its projections (no counterpart in the reference).
+ *
+ * Rotary positions: of every head's head_dim features the first rotary_dim (even) are pairs (a, b), neighbours (interleaved) or a
+ * half apart, that are turned by angle = position * inv_freq[pair]:
+ *   a' = amplitude (a cos - b sin),  b' = amplitude (b cos + a sin);  backward: by the opposite angle (the gradient of the former).
+ * Tensors are [tokens][heads][head_dim] of `dtype` with element strides for the first two (head_dim contiguous); outputs are contiguous.
+ * positions [tokens]: int32, or int64 with positions_64; inv_freq [rotary_dim / 2] in radians a position: fp32, or fp64 with freq_64.
+ * Angles are formed in 64 bits.  k may be NULL.  head_dim <= 1024.
+ */
+int bt_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head, int dtype, const void* positions,
+              int positions_64, const void* inv_freq, int freq_64, int interleaved, float amplitude, int backward, int64_t tokens, int64_t heads,
+              int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, void* q_out, void* k_out, void* stream);
+
+/*
+ * The paged cache: k_cache and v_cache are [pages][kv_heads][page_size][Dp] each, Dp = bt_cache_head_dim(dtype, head_dim): head_dim <= 256
+ * rounded up to 64 bytes (0: bad arguments); page_size a power of two from 32 on; 16-byte aligned.  With E elements in 16 bytes, a head's
+ * page holds tiles of 4 E places in the order of the matrix cores' operands (place and feature within the tile):
+ *   keys    [feature / 4E][place % E / 4][feature % 4E / E][place / E][place % 4][feature % E]
+ *   values  [feature / 16][place / E][feature % 16][place % E]
+ * Sequence s owns the pages block_table[s][0 .. table_width) (int32) and lengths[s] places in them, its new tokens included, which are the
+ * last; they are the rows q_starts[s] .. q_starts[s + 1] - 1 of k, v and q.  q_starts (sequences + 1 entries, from 0, ascending) NULL: one
+ * token a sequence.  Entries of the table behind the places in use are not read.
+ *   bt_cache_append: writes the new tokens' keys, turned as bt_rotary does at position first_position + place, and values; q (or NULL)
+ *     turned likewise goes to q_out, contiguous; rows of q_out behind the last sequence are cleared.  rotary_dim 0: as they are.  Places
+ *     below 0, behind the table and on pages that the cache does not have are not written.
+ *   bt_cached_attention: out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j with head h reading key head h / (heads / kv_heads), over the
+ *     prefix_length places of the pages prefix_table (0: none) and the places of its sequence up to the token's own; lse (or NULL)
+ *     [tokens][heads]: the logarithm of the sum of exponentials.  No places at all, and rows behind the last sequence: zeros, and -inf.  The rows of
+ *     sequences with more than max_length (<= table_width * page_size) places, and rows that see a page outside the cache (others of the
+ *     sequence may be), are not a number.
+ *     Places that a row does not see do not change it, whatever they hold.  workspace: bt_cached_attention_workspace_bytes.
+ */
+int bt_cache_head_dim(int dtype, int64_t head_dim);
+int bt_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* q, int64_t q_token,
+                    int64_t q_head, int dtype, const void* inv_freq, int freq_64, int interleaved, float amplitude, int64_t first_position,
+                    int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, void* k_cache, void* v_cache, int64_t pages,
+                    int64_t page_size, const int32_t* block_table, int64_t table_width, const int32_t* lengths, const int32_t* q_starts,
+                    int64_t sequences, void* q_out, void* stream);
+size_t bt_cached_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t table_width,
+                                           int64_t max_length, int has_starts, int64_t sequences, int64_t prefix_length);
+int bt_cached_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const void* k_cache, const void* v_cache, int64_t pages, int64_t page_size,
+                        const int32_t* block_table, int64_t table_width, int64_t max_length, const int32_t* lengths, const int32_t* q_starts,
+                        int64_t sequences, const int32_t* prefix_table, int64_t prefix_length, float scale, int64_t tokens, int64_t heads,
+                        int64_t kv_heads, int64_t head_dim, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
