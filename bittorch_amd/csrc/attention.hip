@@ -7,25 +7,36 @@
 // order of the keys.  The rows of every sequence together are the rows of the prefix, whose keys are thus read once for all.
 //
 // At few rows the launch is bound by the cache's bytes, at many by the matrix cores and the exponentials.
+#include "lds_dma.h"
 #include "paged_cache.h"
 
 namespace bt {
 
+// What workgroups leave for attend_join_kernel: [row][chunk], rows by (sequence, key head, row of it) of attend_rows_kernel's sequences and by
+// (token, head) otherwise.
+struct Parts {
+    float* o;    // part_stride(dim) floats each
+    float2* ml;
+};
 struct AttendParams {
     const void *q, *k_cache, *v_cache;
     const int32_t *table, *lengths, *starts, *prefix_table;
     int64_t q_token, q_head, tokens;
     void* out;
     float* lse;          // may be null
-    float* part_o;       // [row][part][dim], row = token * heads + head; null: a workgroup sees all keys of its rows
-    float2* part_ml;     // [row][part]
     int heads, kv_heads, group, dim, dp, n_seq, width, page_shift, pages, prefix;
-    int chunk, prefix_chunk, chunks, prefix_chunks;  // places of a chunk; chunks of the longest sequence and of the prefix
-    int units, prefix_units;                         // row tiles
-    int seq_tiles;                                   // of a sequence's one token
     int longest, wide_q;
+    int few_rows;        // sequences of up to so many rows are attend_rows_kernel's, others attend_tiles_kernel's
+    // of the two kernels: places of a chunk of a sequence, chunks of the longest, and row tiles (few: of each sequence, wide: of all of them)
+    int chunk, chunks, tiles, wide_chunk, wide_chunks, wide_tiles;
+    int prefix_chunk, prefix_chunks, prefix_tiles, prefix_wide;  // the prefix, whose rows are tiled by one of them
+    Parts few_parts, wide_parts, prefix_parts;       // without: the workgroup sees all keys of its rows
+    int few_slots;       // rows of a sequence and key head in few_parts
+    int join_few;        // attend_join_kernel goes over few_parts' rows alone
     float scale2;                                    // scale / ln 2
 };
+
+__host__ __device__ __forceinline__ int part_stride(int dim) { return (dim + 3) / 4 * 4; }
 
 template <int DT>
 struct Half8;  // an operand of 16-bit elements
@@ -74,18 +85,34 @@ __device__ __forceinline__ u32x4 first_places(u32x4 v, int live) {
     }
     return v;
 }
+// Values that are infinite or not a number, where some rows' weights are zero because they do not see them (zero times such a value is not
+// zero): `v` without them, and ones in their places.  A row that sees one is not a number; the others' sums are what they are without them.
 template <int DT>
-__device__ __forceinline__ bool any_special(u32x4 v) {  // infinite or not a number
-    bool s = false;
+__device__ __forceinline__ bool take_specials(u32x4& v, u32x4& where) {
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if constexpr (DT == BT_F32) s |= (v[i] & 0x7f800000u) == 0x7f800000u;
-        else {
-            constexpr uint32_t e = DT == BT_F16 ? 0x7c00u : 0x7f80u;
-            s |= (v[i] & e) == e || (v[i] >> 16 & e) == e;
+        if constexpr (DT == BT_F32) {
+            const bool s = (v[i] & 0x7f800000u) == 0x7f800000u;
+            where[i] = s ? 0x3f800000u : 0u;
+            v[i] = s ? 0u : v[i];
+            any |= s;
+        } else {
+            constexpr uint32_t e = DT == BT_F16 ? 0x7c00u : 0x7f80u, one = DT == BT_F16 ? 0x3c00u : 0x3f80u;
+            const bool lo = (v[i] & e) == e, hi = (v[i] >> 16 & e) == e;
+            where[i] = (lo ? one : 0u) | (hi ? one << 16 : 0u);
+            v[i] = (lo ? 0u : v[i] & 0xffffu) | (hi ? 0u : v[i] & 0xffff0000u);
+            any |= lo || hi;
         }
     }
-    return s;
+    return any;
+}
+template <int DT>
+__device__ __forceinline__ v4f add_specials(v4f o, u32x4 where, u32x4 weights) {
+    const v4f seen = step<DT>(where, weights, v4f{0, 0, 0, 0});
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = seen[i] > 0.0f ? __builtin_nanf("") : o[i];
+    return o;
 }
 __device__ __forceinline__ float over_groups_max(float x) {  // over the four lanes of a row
     x = fmaxf(x, __shfl_xor(x, 16));
@@ -105,138 +132,173 @@ struct Job {
     int limit0;          // row r sees the places below limit0 + (row0 + r) / G (own) or limit0 (prefix)
     bool causal, bad;    // bad: the length is beyond the table
     int begin, end;      // the chunk's places
-    int part;
+    int part, kv, slots;  // slots: parts of a row
+    int64_t few_slot;     // >= 0: of row 0 in few_parts
+    Parts parts;
 };
 __device__ __forceinline__ int limit_of(const AttendParams& p, const Job& j, int r) { return j.causal ? j.limit0 + (int)((j.row0 + r) / p.group) : j.limit0; }
 
 // A sequence's tokens [t0, t0 + n) and its length, as far as the table goes; whether it goes beyond
 __device__ __forceinline__ bool sequence_of(const AttendParams& p, int s, int64_t* t0, int* n, int* length) {
     *t0 = p.starts ? std::max(p.starts[s], 0) : s;
-    *n = p.starts ? (int)(std::min<int64_t>(p.starts[s + 1], p.tokens) - *t0) : 1;
+    *n = p.starts ? (int)std::max<int64_t>(0, std::min<int64_t>(p.starts[s + 1], p.tokens) - *t0) : 1;  // (0 <= t0, t0 + n <= tokens where n > 0)
     const int got = p.lengths[s];
-    *length = std::min(got, p.longest);
+    *length = std::max(0, std::min(got, p.longest));
     return got > p.longest;
 }
 
-// False: nothing to do.
-__device__ __forceinline__ bool job_of(const AttendParams& p, int R, int64_t block, Job* j, int* kv) {
-    const int64_t prefix_blocks = (int64_t)p.prefix_units * p.kv_heads * p.prefix_chunks;
-    if (block < prefix_blocks) {
-        const int c = (int)(block % p.prefix_chunks);
-        *kv = (int)(block / p.prefix_chunks % p.kv_heads);
-        j->row0 = block / p.prefix_chunks / p.kv_heads * R;
-        j->token0 = 0;
-        j->rows = (int)std::min<int64_t>(R, p.tokens * p.group - j->row0);
-        j->table = p.prefix_table;
-        j->limit0 = p.prefix;
-        j->causal = j->bad = false;
-        j->begin = c * p.prefix_chunk;
-        j->end = std::min(j->begin + p.prefix_chunk, p.prefix);
-        j->part = c;
-        return j->rows > 0 && j->begin < j->end;
-    }
-    block -= prefix_blocks;
-    const int c = (int)(block % p.chunks);
-    *kv = (int)(block / p.chunks % p.kv_heads);
-    const int64_t unit = block / p.chunks / p.kv_heads;
-    int s = (int)(unit / p.seq_tiles);
-    int64_t tile = unit % p.seq_tiles;
-    if (p.starts) {
-        // sequence s has the tiles floor(starts[s] G / R) + s and on: n tokens have n G / R + 1 tiles at most
-        const int lane = threadIdx.x & 63;
-        int found = 0;
-        for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
-            const int i = s0 + lane;
-            const uint64_t hit = __ballot(i < p.n_seq && (int64_t)std::max(p.starts[i < p.n_seq ? i : 0], 0) * p.group / R + i <= unit);
-            found += __popcll(hit);
-            if (hit != ~0ull) break;
-        }
-        s = found - 1;
-        if (s < 0) return false;
-        tile = unit - ((int64_t)std::max(p.starts[s], 0) * p.group / R + s);
-    }
+// Block `block` of the prefix: row tile, key head, chunk.
+__device__ __forceinline__ bool prefix_job(const AttendParams& p, int R, int64_t block, Job* j) {
+    const int c = (int)(block % p.prefix_chunks);
+    j->kv = (int)(block / p.prefix_chunks % p.kv_heads);
+    j->row0 = block / p.prefix_chunks / p.kv_heads * R;
+    j->token0 = 0;
+    j->rows = (int)std::min<int64_t>(R, p.tokens * p.group - j->row0);
+    j->table = p.prefix_table;
+    j->limit0 = p.prefix;
+    j->causal = j->bad = false;
+    j->begin = c * p.prefix_chunk;
+    j->end = std::min(j->begin + p.prefix_chunk, p.prefix);
+    j->part = c;
+    j->slots = p.prefix_chunks;
+    j->few_slot = -1;
+    j->parts = p.prefix_parts;
+    return j->rows > 0;
+}
+// The tile of rows [tile * R, ...) of sequence s and chunk c of its places.  False: nothing to do.
+__device__ __forceinline__ bool own_job(const AttendParams& p, int R, int s, int64_t tile, int c, int chunk, bool wide, Job* j) {
     int n, length;
     j->bad = sequence_of(p, s, &j->token0, &n, &length);
     j->row0 = tile * R;
-    if (n <= 0 || j->row0 >= (int64_t)n * p.group) return false;
-    j->rows = (int)std::min<int64_t>(R, (int64_t)n * p.group - j->row0);
+    const int64_t rows = (int64_t)n * p.group;
+    if (n <= 0 || j->row0 >= rows || (rows > p.few_rows) != wide) return false;
+    j->rows = (int)std::min<int64_t>(R, rows - j->row0);
     j->table = p.table + (int64_t)s * p.width;
     j->limit0 = length - n + 1;
     j->causal = true;
-    j->begin = c * p.chunk;
-    j->end = std::min(j->begin + p.chunk, limit_of(p, *j, j->rows - 1));
-    j->part = p.prefix_chunks + c;
-    return j->begin < j->end || (!p.part_o && c == 0);
+    j->begin = c * chunk;
+    j->end = std::min(j->begin + chunk, limit_of(p, *j, j->rows - 1));
+    j->part = c;
+    j->slots = wide ? p.wide_chunks : p.chunks;
+    j->few_slot = wide ? -1 : ((int64_t)s * p.kv_heads + j->kv) * p.few_slots + j->row0;
+    j->parts = wide ? p.wide_parts : p.few_parts;
+    return j->begin < j->end || (!j->parts.o && c == 0);
 }
-
-// o += V^T P where values among the masked places are infinite or not a number: row by row, with the places that the row does not see set to
-// zero (0 times such a value is not zero).
-template <int DT, int B>
-__device__ __forceinline__ void add_row_by_row(v4f (&o)[2 * B], const u32x4 (&v)[2 * B], u32x4 hi, u32x4 lo, int my_limit, int place) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll 1
-    for (int r = 0; r < 16; r++) {
-        const int live = __shfl(my_limit, r) - (place + lane / 16 * CacheOrder<DT>::E);
-#pragma unroll
-        for (int b = 0; b < 2 * B; b++) {
-            const u32x4 seen = first_places<DT>(v[b], live);
-            v4f x = step<DT>(seen, hi, o[b]);  // (the same sums as without it: the row's bits do not depend on what it does not see)
-            if constexpr (DT != BT_F32) x = step<DT>(seen, lo, x);
-            if (lane % 16 == r) o[b] = x;
-        }
+// Where row `r` of the job is written: row of the result
+__device__ __forceinline__ int64_t out_row_of(const AttendParams& p, const Job& j, int r) {
+    const int64_t rw = j.row0 + r;
+    return (j.token0 + rw / p.group) * p.heads + j.kv * p.group + rw % p.group;
+}
+// The chunk's pages, one a lane, 64 at a time.
+struct PageWindow {
+    int first, last, page;  // numbers of the window's first page and of the chunk's last
+    bool bad;
+    __device__ __forceinline__ PageWindow(const AttendParams& p, const Job& j) : bad(j.bad) {
+        last = (j.end - 1) >> p.page_shift;
+        load(p, j, j.begin >> p.page_shift);
     }
+    __device__ __forceinline__ void load(const AttendParams& p, const Job& j, int from) {
+        const int at = from + (int)(threadIdx.x & 63);
+        first = from;
+        page = j.end > j.begin && at <= last ? j.table[at] : 0;
+        const bool wrong = (uint32_t)page >= (uint32_t)p.pages;
+        bad |= __ballot(wrong) != 0;
+        if (wrong) page = 0;
+    }
+    __device__ __forceinline__ int64_t of(const AttendParams& p, const Job& j, int place) {  // place: not below those asked for before
+        const int number = place >> p.page_shift;
+        if (number >= first + 64) load(p, j, first + (number - first) / 64 * 64);
+        return __builtin_amdgcn_readlane(page, number - first);
+    }
+};
+// The rows behind the last sequence, where no job sees to them
+template <int DT>
+__device__ __forceinline__ void clear_rows_behind(const AttendParams& p) {
+    const int64_t n = (int64_t)p.heads * p.dim, behind = std::max<int64_t>(0, std::min<int64_t>(p.starts[p.n_seq], p.tokens));
+    for (int64_t i = behind * n + threadIdx.x; i < p.tokens * n; i += blockDim.x) store_elem<DT>(p.out, i, 0.0f);
+    for (int64_t i = behind * p.heads + threadIdx.x; p.lse && i < p.tokens * p.heads; i += blockDim.x) p.lse[i] = -__builtin_inff();
+}
+// Piece c of a row of q (E features from c TK + g E) as an operand; features behind the head are zero
+template <int DT>
+__device__ __forceinline__ u32x4 q_piece(const AttendParams& p, int64_t row_at, int f) {
+    constexpr int E = CacheOrder<DT>::E;
+    u32x4 q = {0, 0, 0, 0};
+    if (f >= p.dim) return q;
+    if (p.wide_q) return *(const u32x4*)((const char*)p.q + (row_at + f) * CacheOrder<DT>::SIZE);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (f + e >= p.dim) break;
+        if constexpr (DT == BT_F32) q[e] = ((const uint32_t*)p.q)[row_at + f + e];
+        else q[e / 2] |= (uint32_t)((const uint16_t*)p.q)[row_at + f + e] << (e % 2 * 16);
+    }
+    return q;
+}
+// Four features of row r of the job, finished or for attend_join_kernel; top: the row's maximum, in powers of two
+template <int DT>
+__device__ __forceinline__ void put_row(const AttendParams& p, const Job& j, int r, int f, v4f acc, float top, float sum) {
+    const int64_t out_row = out_row_of(p, j, r);
+    if (j.parts.o) {
+        const int64_t at = (j.few_slot >= 0 ? j.few_slot + r : out_row) * j.slots + j.part;
+        if (f == 0) j.parts.ml[at] = make_float2(top, sum);
+        *(v4f*)(j.parts.o + at * part_stride(p.dim) + f) = acc;  // (what lies behind the head is not read)
+        return;
+    }
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (p.dim % 4 == 0) {
+        if constexpr (DT == BT_F32) *(v4f*)((float*)p.out + out_row * p.dim + f) = acc * inverse;
+        else {
+            u32x2 w;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float a = acc[2 * i] * inverse, b = acc[2 * i + 1] * inverse;
+                w[i] = DT == BT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16 : f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16;
+            }
+            *(u32x2*)((uint16_t*)p.out + out_row * p.dim + f) = w;
+        }
+    } else {
+        for (int i = 0; i < 4; i++)
+            if (f + i < p.dim) store_elem<DT>(p.out, out_row * p.dim + f + i, acc[i] * inverse);
+    }
+    if (f == 0 && p.lse) p.lse[out_row] = sum == 0.0f ? -__builtin_inff() : top * 0.69314718055994530942f + __logf(sum);
 }
 
-// B: blocks of 32 features that a head has at most.  Four waves take the chunk's tiles of TK places in turn, each with all rows.
+// B: blocks of 32 features, the last one maybe in part (the first FULL groups of TK features are whole).  Four waves take the chunk's tiles of TK places in turn, each with all rows.
 template <int DT, int B>
 __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
     using Order = CacheOrder<DT>;
-    constexpr int E = Order::E, TK = Order::TK, C = 32 * B / TK, V = 2 * B, R = 16;
+    constexpr int E = Order::E, TK = Order::TK, C = 32 * B / TK, V = 2 * B, FULL = 32 * (B - 1) / TK, R = 16;
     constexpr int JB = B < 4 ? B : 4, LD = 32 * JB + 4;  // blocks that are joined at a time (LDS)
     __shared__ __attribute__((aligned(16))) float o_all[4][R * LD];
     __shared__ float m_all[4][R], l_all[4][R];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int64_t job_blocks = ((int64_t)p.prefix_units * p.prefix_chunks + (int64_t)p.units * p.chunks) * p.kv_heads;
-    if ((int64_t)blockIdx.x >= job_blocks) {  // the rows behind the last sequence, where no other kernel sees to them
-        const int64_t n = (int64_t)p.heads * p.dim, behind = std::max<int64_t>(0, std::min<int64_t>(p.starts[p.n_seq], p.tokens));
-        for (int64_t i = behind * n + threadIdx.x; i < p.tokens * n; i += 256) store_elem<DT>(p.out, i, 0.0f);
-        for (int64_t i = behind * p.heads + threadIdx.x; p.lse && i < p.tokens * p.heads; i += 256) p.lse[i] = -__builtin_inff();
-        return;
-    }
     Job j;
-    int kv;
-    if (!job_of(p, R, blockIdx.x, &j, &kv)) return;
+    {
+        int64_t block = blockIdx.x;
+        const int64_t prefix_blocks = p.prefix_wide ? 0 : (int64_t)p.prefix_tiles * p.kv_heads * p.prefix_chunks;
+        if (block < prefix_blocks) {
+            if (!prefix_job(p, R, block, &j)) return;
+        } else {
+            block -= prefix_blocks;
+            const int c = (int)(block % p.chunks);
+            block /= p.chunks;
+            j.kv = (int)(block % p.kv_heads);
+            block /= p.kv_heads;
+            if (block / p.tiles >= p.n_seq) return clear_rows_behind<DT>(p);
+            if (!own_job(p, R, (int)(block / p.tiles), block % p.tiles, c, p.chunk, false, &j)) return;
+        }
+    }
+    const int kv = j.kv;
 
-    // the chunk's pages, one a lane (at most 64)
-    const int page0 = j.begin >> p.page_shift, tiles = j.end > j.begin ? (j.end - j.begin + TK - 1) / TK : 0;
-    const int n_pages = j.end > j.begin ? ((j.end - 1) >> p.page_shift) - page0 + 1 : 0;
-    int page = lane < n_pages ? j.table[page0 + lane] : 0;
-    const bool bad_page = (uint32_t)page >= (uint32_t)p.pages;
-    const bool bad = __ballot(bad_page) != 0 || j.bad;
-    if (bad_page) page = 0;
+    PageWindow pages(p, j);
+    const int tiles = j.end > j.begin ? (j.end - j.begin + TK - 1) / TK : 0;
 
     // this lane's row as an operand
     const int64_t row = j.row0 + r;
-    const int64_t token = j.token0 + row / p.group;
-    const int head = kv * p.group + (int)(row % p.group);
+    const int64_t q_at = (j.token0 + row / p.group) * p.q_token + (kv * p.group + (int)(row % p.group)) * p.q_head;
     const int limit = r < j.rows ? limit_of(p, j, r) : 0, lowest = limit_of(p, j, 0);
     u32x4 q[C];
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-        q[c] = u32x4{0, 0, 0, 0};
-        const int f = c * TK + g * E;
-        if (r < j.rows && f < p.dim) {
-            const int64_t at = token * p.q_token + head * p.q_head + f;
-            if (p.wide_q) q[c] = *(const u32x4*)((const char*)p.q + at * Order::SIZE);
-            else {
-                for (int e = 0; e < E; e++) {
-                    if (f + e >= p.dim) break;
-                    if constexpr (DT == BT_F32) q[c][e] = ((const uint32_t*)p.q)[at + e];
-                    else q[c][e / 2] |= (uint32_t)((const uint16_t*)p.q)[at + e] << (e % 2 * 16);
-                }
-            }
-        }
-    }
+    for (int c = 0; c < C; c++) q[c] = r < j.rows ? q_piece<DT>(p, q_at, c * TK + g * E) : u32x4{0, 0, 0, 0};
 
     float m = -__builtin_inff(), l = 0.0f;  // of the row; l: of this lane's places
     v4f o[V];
@@ -245,7 +307,7 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
     const int64_t page_elements = (int64_t)p.dp << p.page_shift;
     for (int tile = wave; tile < tiles; tile += 4) {
         const int place = j.begin + tile * TK;
-        const int64_t pg = __builtin_amdgcn_readlane(page, (place >> p.page_shift) - page0);
+        const int64_t pg = pages.of(p, j, place);
         const int64_t at = (pg * p.kv_heads + kv) * page_elements + (int64_t)(place & ((1 << p.page_shift) - 1)) * p.dp + lane * E;
         const char* kp = (const char*)p.k_cache + at * Order::SIZE;
         const char* vp = (const char*)p.v_cache + at * Order::SIZE;
@@ -255,12 +317,12 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
 #pragma unroll
             for (int t = 0; t < E / 4; t++) {
                 k[c][t] = u32x4{0, 0, 0, 0};
-                if (c * TK + g * E < p.dim) k[c][t] = *(const u32x4*)(kp + (c * (E / 4) + t) * 1024);
+                if (c < FULL || c * TK + g * E < p.dim) k[c][t] = *(const u32x4*)(kp + (c * (E / 4) + t) * 1024);
             }
 #pragma unroll
         for (int b = 0; b < V; b++) {
             v[b] = u32x4{0, 0, 0, 0};
-            if (b * 16 < p.dim) v[b] = *(const u32x4*)(vp + b * 1024);
+            if (b < V - 1 || b * 16 < p.dim) v[b] = *(const u32x4*)(vp + b * 1024);
         }
         float x[E];
 #pragma unroll
@@ -299,26 +361,23 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
         }
         u32x4 lo;
         const u32x4 hi = operand<DT>(w, &lo);
-        bool special = false;
         if (masked) {
 #pragma unroll
-            for (int b = 0; b < V; b++) special |= any_special<DT>(v[b]);
-        }
-        if (masked && __any(special)) {
-            add_row_by_row<DT, B>(o, v, hi, lo, limit, place);
-        } else {
-#pragma unroll
             for (int b = 0; b < V; b++) {
-                o[b] = step<DT>(v[b], hi, o[b]);
-                if constexpr (DT != BT_F32) o[b] = step<DT>(v[b], lo, o[b]);
+                u32x4 where;
+                if (__any(take_specials<DT>(v[b], where))) o[b] = add_specials<DT>(o[b], where, hi);
             }
+        }
+#pragma unroll
+        for (int b = 0; b < V; b++) {
+            o[b] = step<DT>(v[b], hi, o[b]);
+            if constexpr (DT != BT_F32) o[b] = step<DT>(v[b], lo, o[b]);
         }
     }
     l = over_groups_sum(l);
 
     // the four waves' shares of every row
     if (g == 0) m_all[wave][r] = m, l_all[wave][r] = l;
-    const int64_t parts = p.prefix_chunks + p.chunks;
 #pragma unroll
     for (int b0 = 0; b0 < B; b0 += JB) {
         if (b0) __syncthreads();
@@ -342,103 +401,360 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
                 const v4f ow = *(const v4f*)&o_all[w][row_at * LD + at];
                 acc += ow * share;
             }
-            if (bad) sum = __builtin_nanf("");
-            const int64_t rw = j.row0 + row_at, t = j.token0 + rw / p.group;
-            const int64_t out_row = t * p.heads + kv * p.group + rw % p.group;
-            if (p.part_o) {
-                if (f == 0) p.part_ml[out_row * parts + j.part] = make_float2(top, sum);
-                float* to = p.part_o + (out_row * parts + j.part) * p.dim;
-                for (int i = 0; i < 4; i++)
-                    if (f + i < p.dim) to[f + i] = acc[i];
-            } else {
-                const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-                for (int i = 0; i < 4; i++)
-                    if (f + i < p.dim) store_elem<DT>(p.out, out_row * p.dim + f + i, acc[i] * inverse);
-                if (f == 0 && p.lse) p.lse[out_row] = sum == 0.0f ? -__builtin_inff() : top * 0.69314718055994530942f + __logf(sum);
-            }
+            put_row<DT>(p, j, row_at, f, acc, top, pages.bad ? __builtin_nanf("") : sum);
         }
     }
 }
 
-// A wave to a row: the parts' weights, a lane each, then the sum of the parts in the order of their keys.
-template <int DT>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendParams p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= p.tokens * p.heads) return;
-    const int64_t token = row / p.heads;
-    const int s = p.starts ? owner_of(p.starts, p.n_seq, token) : (int)token;
-    int own = 0;
-    bool bad = false;
-    if (s >= 0) {
-        int64_t t0;
-        int n, length;
-        bad = sequence_of(p, s, &t0, &n, &length);
-        const int64_t limit = length - n + 1 + (token - t0);
-        own = limit > 0 ? (int)((limit + p.chunk - 1) / p.chunk) : 0;
+// RT row tiles of 16 a wave and four waves: 128 rows (64 of more than 128 features, whose sums take twice the registers), whose keys and values pass through LDS once for all of them, two stages of ST tiles of TK
+// places.  A stage is read from memory straight into LDS, in the order in which the waves take it from there (16 bytes a lane in a row: no bank
+// is asked twice), while the one before is worked on.
+//
+// The exponentials are the other half of the work: per 32 places and 16 rows the matrix cores need 16 x 16 cycles (128 features) and the 8
+// weights of a lane about as many, so the instructions around them are few.  The maximum is that of the products before they are
+// scaled, and one multiply-add and the exponential make a weight.  It is raised only where a weight would pass 2^8: it needs to be near the true maximum, not to be it.
+// 16-bit weights are rounded once (the rows kernel's two halves would be half as many matrix instructions again): results are 1.4 times
+// as far from 64 bits as by their own rounding.  Their sum is that of the weights before they are rounded, as lse wants it.
+template <int DT, int B>
+__global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
+    using Order = CacheOrder<DT>;
+    constexpr int E = Order::E, TK = Order::TK, C = 32 * B / TK, V = 2 * B, FULL = 32 * (B - 1) / TK, RT = B <= 4 ? 2 : 1, R = 64 * RT;
+    constexpr int ST = B <= 4 ? 2 : 1, TILE = 2048 * B, STAGE = 2 * ST * TILE;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];  // (from offset 0: loads into LDS reach 64 KiB)
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    Job j;
+    {
+        int64_t block = blockIdx.x;
+        const int64_t prefix_blocks = p.prefix_wide ? (int64_t)p.prefix_tiles * p.kv_heads * p.prefix_chunks : 0;
+        if (block < prefix_blocks) {
+            if (!prefix_job(p, R, block, &j)) return;
+        } else {
+            block -= prefix_blocks;
+            const int c = (int)(block % p.wide_chunks);
+            block /= p.wide_chunks;
+            j.kv = (int)(block % p.kv_heads);
+            const int64_t unit = block / p.kv_heads;
+            int s;
+            int64_t tile;
+            if (p.starts) {
+                // sequence s has the tiles floor(starts[s] G / R) + s and on: n tokens have n G / R + 1 tiles at most
+                int found = 0;
+                for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
+                    const int i = s0 + lane;
+                    const uint64_t hit = __ballot(i < p.n_seq && (int64_t)std::max(p.starts[i < p.n_seq ? i : 0], 0) * p.group / R + i <= unit);
+                    found += __popcll(hit);
+                    if (hit != ~0ull) break;
+                }
+                s = found - 1;
+                if (s < 0) return;
+                tile = unit - ((int64_t)std::max(p.starts[s], 0) * p.group / R + s);
+                if (tile < 0) return;  // (starts that do not ascend)
+            } else {
+                const int each = (p.group + R - 1) / R;
+                s = (int)(unit / each);
+                tile = unit % each;
+            }
+            if (!own_job(p, R, s, tile, c, p.wide_chunk, true, &j)) return;
+        }
     }
-    const int64_t parts = p.prefix_chunks + p.chunks;
-    const int count = s < 0 ? 0 : p.prefix_chunks + own;
-    const float2* ml = p.part_ml + row * parts;
+    PageWindow pages(p, j);
+    const int tiles = j.end > j.begin ? (j.end - j.begin + TK - 1) / TK : 0;
+    const int mine = wave * RT * 16;  // this wave's first row
+    u32x4 q[RT][C];
+    int limit[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int at = mine + t * 16 + r;
+        const int64_t row = j.row0 + at;
+        const int64_t q_at = (j.token0 + row / p.group) * p.q_token + (j.kv * p.group + (int)(row % p.group)) * p.q_head;
+        limit[t] = at < j.rows ? limit_of(p, j, at) : 0;
+#pragma unroll
+        for (int c = 0; c < C; c++) q[t][c] = at < j.rows ? q_piece<DT>(p, q_at, c * TK + g * E) : u32x4{0, 0, 0, 0};
+    }
+    // the places that some row of the wave sees, and those that all see
+    const int reach = mine < j.rows ? limit_of(p, j, std::min(mine + 16 * RT, j.rows) - 1) : 0;
+    const int lowest = mine < j.rows ? limit_of(p, j, mine) : 0;
+
+    const int64_t page_elements = (int64_t)p.dp << p.page_shift;
+    const int pieces = p.dp * TK * Order::SIZE / 1024;  // KiB of a tile's keys
+    auto fetch = [&](int stage) {
+#pragma unroll
+        for (int u = 0; u < ST; u++) {
+            const int tile = stage * ST + u, place = j.begin + tile * TK;
+            if (tile >= tiles) break;
+            const int64_t at = ((pages.of(p, j, place) * p.kv_heads + j.kv) * page_elements + (int64_t)(place & ((1 << p.page_shift) - 1)) * p.dp) * Order::SIZE;
+            const uint32_t to = lds0 + (uint32_t)(stage & 1) * STAGE + u * 2 * TILE;
+#pragma unroll
+            for (int i0 = 0; i0 < V; i0 += 4) {
+                const int i = i0 + wave;
+                if (i < pieces) {
+                    dma16(to + i * 1024, i * 1024 + lane * 16, (const char*)p.k_cache + at);
+                    dma16(to + TILE + i * 1024, i * 1024 + lane * 16, (const char*)p.v_cache + at);
+                }
+            }
+        }
+    };
+
+    v4f o[RT][V];
+    float m[RT], l[RT];  // the rows' maxima (of the products before they are scaled) and sums (of this lane's places)
+    const float slack = 8.0f / p.scale2;
+    // The multiply-add rounds once, the base alone too: logits of a size at which that is more than a part of one are rounded alike first.
+    bool large = false;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        m[t] = -__builtin_inff(), l[t] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < V; b++) o[t][b] = v4f{0, 0, 0, 0};
+    }
+    auto work = [&](const uint8_t* from, int place, auto masked_c) {
+        constexpr bool MASKED = decltype(masked_c)::value;
+        v4f s[RT][E / 4];
+#pragma unroll
+        for (int h = 0; h < E / 4; h++) {
+#pragma unroll
+            for (int t = 0; t < RT; t++) s[t][h] = v4f{0, 0, 0, 0};
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                u32x4 k = *(const u32x4*)(from + (c * (E / 4) + h) * 1024 + lane * 16);
+                if (c >= FULL && c * TK + g * E >= p.dim) k = u32x4{0, 0, 0, 0};  // (what lies behind the head was never written)
+#pragma unroll
+                for (int t = 0; t < RT; t++) s[t][h] = step<DT>(k, q[t][c], s[t][h]);
+            }
+        }
+        // (the three parts' operands together would not fit the registers)
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 w[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                x[e] = s[t][e / 4][e % 4];
+                if constexpr (MASKED) x[e] = place + g * E + e < limit[t] ? x[e] : -__builtin_inff();
+            }
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < E; e++) top = fmaxf(top, x[e]);
+            if (__any(top > m[t] + slack)) {
+                const float next = fmaxf(m[t], over_groups_max(top));
+                const float shrink = __builtin_amdgcn_exp2f(m[t] == next ? 0.0f : (m[t] - next) * p.scale2);
+                m[t] = next;
+                large |= __any(fabsf(next) * p.scale2 > 65536.0f);
+                l[t] *= shrink;
+#pragma unroll
+                for (int b = 0; b < V; b++) o[t][b] *= shrink;
+            }
+            const float base = m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2;
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = __builtin_amdgcn_exp2f(large ? x[e] * p.scale2 + base : __builtin_fmaf(x[e], p.scale2, base));
+            w[t] = operand<DT>(x, nullptr);
+            float sum = x[0] + x[1];
+#pragma unroll
+            for (int e = 2; e < E; e += 2) sum += x[e] + x[e + 1];
+            l[t] += sum;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t* vf = from + TILE + lane * 16;
+        const int live = MASKED ? j.end - (place + g * E) : E;  // no row sees what lies behind: whatever it is
+#pragma unroll
+        for (int b = 0; b < V; b++) {
+            u32x4 v = *(const u32x4*)(vf + b * 1024);
+            if constexpr (MASKED) {
+                u32x4 where;
+                v = first_places<DT>(v, live);
+                if (__any(take_specials<DT>(v, where))) {
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][b] = add_specials<DT>(o[t][b], where, w[t]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) o[t][b] = step<DT>(v, w[t], o[t][b]);
+        }
+    };
+
+    const int stages = (tiles + ST - 1) / ST;
+    if (stages) fetch(0);
+    for (int stage = 0; stage < stages; stage++) {
+        // this stage has arrived, and all waves are done with the one before
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (stage + 1 < stages) fetch(stage + 1);
+#pragma unroll 1
+        for (int u = 0; u < ST; u++) {
+            const int place = j.begin + (stage * ST + u) * TK;
+            const uint8_t* from = lds + (stage & 1) * STAGE + u * 2 * TILE;
+            if (place >= reach || stage * ST + u >= tiles) break;
+            if (place + TK > lowest) work(from, place, std::true_type());
+            else work(from, place, std::false_type());
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int at = mine + t * 16 + r;
+        const float sum = over_groups_sum(l[t]);
+        if (at >= j.rows) continue;
+        const float top = m[t] == -__builtin_inff() ? m[t] : m[t] * p.scale2;
+#pragma unroll
+        for (int b = 0; b < V; b++)
+            if (b * 16 + g * 4 < p.dim) put_row<DT>(p, j, at, b * 16 + g * 4, o[t][b], top, pages.bad ? __builtin_nanf("") : sum);
+    }
+}
+
+// W waves to a row.  Each forms the parts' common maximum and sum; then a lane has four features and every (64 W / lanes of a row)th part,
+// and the lanes' sums are added in LDS, in an order that depends on the shape alone.
+template <int DT, int W>
+__global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void attend_join_kernel(AttendParams p) {
+    constexpr int ROWS = W < 4 ? 4 / W : 1;
+    __shared__ __attribute__((aligned(16))) float sums[ROWS * 64 * W * 4];
+    const int lane = threadIdx.x & 63, in_row = threadIdx.x % (64 * W);
+    int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / (64 * W), few_slot = row;
+    const int stride = part_stride(p.dim);
+    // the row's parts: `shared` of the prefix, then its sequence's
+    int shared = 0, count = 0;
+    bool there, bad = false;
+    const float2 *pml = nullptr, *ml = nullptr;
+    const float *po = nullptr, *o = nullptr;
+    int s = -1, n = 0, length = 0;
+    int64_t token = 0, t0 = 0;
+    if (p.join_few) {
+        const int64_t of = row / p.few_slots, r = row % p.few_slots;
+        there = of < (int64_t)p.n_seq * p.kv_heads;
+        if (there) {
+            s = (int)(of / p.kv_heads);
+            bad = sequence_of(p, s, &t0, &n, &length);
+            there = r < (int64_t)n * p.group && (int64_t)n * p.group <= p.few_rows;
+            token = t0 + r / p.group;
+            row = token * p.heads + of % p.kv_heads * p.group + r % p.group;
+        }
+    } else {
+        there = row < p.tokens * p.heads;
+        if (there) {
+            token = row / p.heads;
+            s = p.starts ? owner_of(p.starts, p.n_seq, token) : (int)token;
+            if (s >= 0) {
+                bad = sequence_of(p, s, &t0, &n, &length);
+                if (token < t0 || token - t0 >= n) s = -1, bad = false;  // (starts that do not ascend)
+                few_slot = ((int64_t)s * p.kv_heads + row % p.heads / p.group) * p.few_slots + (token - t0) * p.group + row % p.heads % p.group;
+            }
+        }
+    }
+    if (there && s >= 0) {
+        const bool wide = (int64_t)n * p.group > p.few_rows;
+        const int64_t limit = length - n + 1 + (token - t0);
+        const int chunk = wide ? p.wide_chunk : p.chunk, own = limit > 0 ? (int)((limit + chunk - 1) / chunk) : 0;
+        const int64_t at = wide ? row * p.wide_chunks : few_slot * p.chunks;
+        const Parts& mine = wide ? p.wide_parts : p.few_parts;
+        ml = mine.ml + at, o = mine.o + at * stride;
+        shared = p.prefix_chunks;
+        pml = p.prefix_parts.ml + row * shared, po = p.prefix_parts.o + row * shared * stride;
+        count = shared + own;
+    }
+    auto ml_of = [&](int i) { return i < shared ? pml[i] : ml[i - shared]; };
     float top = -__builtin_inff(), sum = 0.0f;
-    for (int i = lane; i < count; i += 64) top = fmaxf(top, ml[i].x);
+    for (int i = lane; i < count; i += 64) top = fmaxf(top, ml_of(i).x);
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float base = top == -__builtin_inff() ? 0.0f : top;
-    for (int i = lane; i < count; i += 64) sum += __builtin_amdgcn_exp2f(ml[i].x - base) * ml[i].y;
+    for (int i = lane; i < count; i += 64) sum += __builtin_amdgcn_exp2f(ml_of(i).x - base) * ml_of(i).y;
     for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
     if (bad) sum = __builtin_nanf("");
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    for (int f = lane; f < p.dim; f += 64) {
-        const float* o = p.part_o + row * parts * p.dim + f;
-        float acc = 0.0f;
-        for (int i = 0; i < count; i++) acc = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[i].x - base), o[(int64_t)i * p.dim], acc);
-        store_elem<DT>(p.out, row * p.dim + f, acc * inverse);
+
+    const int lanes = stride / 4, step = 64 * W / lanes;  // (lanes <= 64)
+    const int first = in_row / lanes, f = in_row % lanes * 4;
+    v4f acc = {0, 0, 0, 0};
+    if (first < step) {
+#pragma unroll 4
+        for (int i = first; i < count; i += step) {
+            const float* from = i < shared ? po + (int64_t)i * stride : o + (int64_t)(i - shared) * stride;
+            acc += *(const v4f*)(from + f) * __builtin_amdgcn_exp2f(ml_of(i).x - base);
+        }
     }
-    if (lane == 0 && p.lse) p.lse[row] = sum == 0.0f ? -__builtin_inff() : top * 0.69314718055994530942f + __logf(sum);
+    *(v4f*)&sums[threadIdx.x * 4] = acc;
+    __syncthreads();
+    if (first != 0 || !there) return;
+    for (int i = 1; i < step; i++) acc += *(const v4f*)&sums[(threadIdx.x + i * lanes) * 4];
+    for (int i = 0; i < 4; i++)
+        if (f + i < p.dim) store_elem<DT>(p.out, row * p.dim + f + i, acc[i] * inverse);
+    if (in_row == 0 && p.lse) p.lse[row] = sum == 0.0f ? -__builtin_inff() : top * 0.69314718055994530942f + __logf(sum);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 
-struct AttendPlan {
-    int64_t chunk, chunks, prefix_chunk, prefix_chunks, units, prefix_units;
-    bool parts;  // rows are joined from parts
-    size_t ml_bytes, bytes;
+struct Region {
+    int64_t rows, slots;
+    size_t ml, o;  // byte offsets in the workspace
 };
+struct AttendPlan {
+    int64_t chunk, chunks, tiles, few_slots, wide_chunk, wide_chunks, wide_tiles, prefix_chunk, prefix_chunks, prefix_tiles;
+    bool few, wide, prefix_wide;              // kernels that have work
+    bool few_parts, wide_parts, join_few;
+    Region few_region, wide_region, prefix_region;
+    size_t bytes;
+};
+constexpr int64_t FEW_ROWS = 32;
+static int64_t wide_tile(int64_t dim) { return dim <= 128 ? 128 : 64; }
 static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
-// Chunks of `places` for `tiles` of rows: workgroups for every compute unit, no more than 64 pages each
-static int64_t chunk_of(int64_t places, int64_t tiles, int64_t page) {
-    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, tiles));
-    int64_t c = round_up(ceil_div(std::max<int64_t>(places, 1), want), 128);
-    return std::max<int64_t>(128, std::min<int64_t>({c, 2048, 64 * page / 128 * 128}));
+// Chunks of `places` for `tiles` of rows, so that there are `want` workgroups
+static int64_t chunk_of(int64_t places, int64_t tiles, int64_t want, int64_t least, int64_t most) {
+    const int64_t n = std::max<int64_t>(1, want / std::max<int64_t>(1, tiles));
+    return std::max(least, std::min(most, round_up(ceil_div(std::max<int64_t>(places, 1), n), 128)));
 }
-static AttendPlan attend_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page, int64_t longest, bool starts, int64_t sequences, int64_t prefix) {
-    AttendPlan a;
-    const int64_t group = heads / kv_heads, R = 16;
-    a.units = starts ? tokens * group / R + sequences : sequences * ceil_div(group, R);
-    a.prefix_units = prefix ? ceil_div(tokens * group, R) : 0;
-    a.chunk = chunk_of(longest, a.units * kv_heads, page);
+static AttendPlan attend_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, bool starts, int64_t sequences, int64_t prefix) {
+    AttendPlan a = {};
+    const int64_t group = heads / kv_heads, most_rows = starts ? tokens * group : group;
+    a.few = starts || group <= FEW_ROWS;
+    a.wide = most_rows > FEW_ROWS;
+    a.few_slots = std::min(most_rows, FEW_ROWS);
+    a.tiles = ceil_div(a.few_slots, 16);
+    a.wide_tiles = starts ? tokens * group / wide_tile(dim) + sequences : sequences * ceil_div(group, wide_tile(dim));
+    a.chunk = chunk_of(longest, sequences * a.tiles * kv_heads, 1024, 128, 4096);
     a.chunks = std::max<int64_t>(1, ceil_div(longest, a.chunk));
-    a.prefix_chunk = prefix ? chunk_of(prefix, a.prefix_units * kv_heads, page) : 128;
-    a.prefix_chunks = prefix ? ceil_div(prefix, a.prefix_chunk) : 0;
-    a.parts = a.chunks + a.prefix_chunks > 1;
-    const int64_t parts = a.chunks + a.prefix_chunks;
-    a.ml_bytes = a.parts ? (size_t)round_up(tokens * heads * parts * 8, 256) : 0;
-    a.bytes = a.parts ? a.ml_bytes + (size_t)(tokens * heads * parts * dim * 4) : 0;
+    a.wide_chunk = chunk_of(longest, a.wide_tiles * kv_heads, 512, 256, 1 << 30);
+    a.wide_chunks = std::max<int64_t>(1, ceil_div(longest, a.wide_chunk));
+    if (prefix) {
+        a.prefix_wide = tokens * group > FEW_ROWS;
+        a.prefix_tiles = ceil_div(tokens * group, a.prefix_wide ? wide_tile(dim) : 16);
+        a.prefix_chunk = a.prefix_wide ? chunk_of(prefix, a.prefix_tiles * kv_heads, 512, 256, 1 << 30) : chunk_of(prefix, a.prefix_tiles * kv_heads, 1024, 128, 4096);
+        a.prefix_chunks = ceil_div(prefix, a.prefix_chunk);
+    }
+    a.few_parts = a.few && (a.chunks > 1 || prefix);
+    a.wide_parts = a.wide && (a.wide_chunks > 1 || prefix);
+    a.join_few = a.few_parts && a.wide && !a.wide_parts;
+    auto region = [&](bool there, int64_t rows, int64_t slots) {
+        Region r = {there ? rows : 0, slots, 0, 0};
+        r.ml = a.bytes, a.bytes += (size_t)round_up(r.rows * slots * 8, 256);
+        r.o = a.bytes, a.bytes += (size_t)round_up(r.rows * slots * part_stride((int)dim) * 4, 256);
+        return r;
+    };
+    a.few_region = region(a.few_parts, sequences * kv_heads * a.few_slots, a.chunks);
+    a.wide_region = region(a.wide_parts, tokens * heads, a.wide_chunks);
+    a.prefix_region = region(prefix > 0, tokens * heads, a.prefix_chunks);
     return a;
 }
 
+template <int DT, int B>
+static void launch_attend_cfg(const AttendParams& p, int64_t few_blocks, int64_t wide_blocks, hipStream_t st) {
+    if (wide_blocks) hipLaunchKernelGGL((attend_tiles_kernel<DT, B>), dim3((unsigned)wide_blocks), dim3(256), 0, st, p);
+    if (few_blocks) hipLaunchKernelGGL((attend_rows_kernel<DT, B>), dim3((unsigned)few_blocks), dim3(256), 0, st, p);
+}
 template <int DT>
-static void launch_attend(const AttendParams& p, int64_t blocks, hipStream_t st) {
-    const dim3 grid((unsigned)blocks), block(256);
+static void launch_attend(const AttendParams& p, int64_t few_blocks, int64_t wide_blocks, int64_t join_rows, hipStream_t st) {
     switch (ceil_div(p.dim, 32)) {
-        case 1: hipLaunchKernelGGL((attend_rows_kernel<DT, 1>), grid, block, 0, st, p); break;
-        case 2: hipLaunchKernelGGL((attend_rows_kernel<DT, 2>), grid, block, 0, st, p); break;
-        case 3: hipLaunchKernelGGL((attend_rows_kernel<DT, 3>), grid, block, 0, st, p); break;
-        case 4: hipLaunchKernelGGL((attend_rows_kernel<DT, 4>), grid, block, 0, st, p); break;
-        case 5: case 6: hipLaunchKernelGGL((attend_rows_kernel<DT, 6>), grid, block, 0, st, p); break;
-        default: hipLaunchKernelGGL((attend_rows_kernel<DT, 8>), grid, block, 0, st, p); break;
+        case 1: launch_attend_cfg<DT, 1>(p, few_blocks, wide_blocks, st); break;
+        case 2: launch_attend_cfg<DT, 2>(p, few_blocks, wide_blocks, st); break;
+        case 3: launch_attend_cfg<DT, 3>(p, few_blocks, wide_blocks, st); break;
+        case 4: launch_attend_cfg<DT, 4>(p, few_blocks, wide_blocks, st); break;
+        case 5: launch_attend_cfg<DT, 5>(p, few_blocks, wide_blocks, st); break;
+        case 6: launch_attend_cfg<DT, 6>(p, few_blocks, wide_blocks, st); break;
+        case 7: launch_attend_cfg<DT, 7>(p, few_blocks, wide_blocks, st); break;
+        default: launch_attend_cfg<DT, 8>(p, few_blocks, wide_blocks, st); break;
     }
-    if (p.part_o) hipLaunchKernelGGL((attend_join_kernel<DT>), dim3((unsigned)ceil_div(p.tokens * p.heads, 4)), block, 0, st, p);
+    if (!join_rows) return;
+    const int64_t parts = p.prefix_chunks + std::max(p.few_parts.o ? p.chunks : 0, p.wide_parts.o ? p.wide_chunks : 0);
+    if (parts <= 8) hipLaunchKernelGGL((attend_join_kernel<DT, 1>), dim3((unsigned)ceil_div(join_rows, 4)), dim3(256), 0, st, p);
+    else if (parts <= 32) hipLaunchKernelGGL((attend_join_kernel<DT, 4>), dim3((unsigned)join_rows), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((attend_join_kernel<DT, 16>), dim3((unsigned)join_rows), dim3(1024), 0, st, p);
 }
 
 static bool shape_ok(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page, int64_t width, int64_t longest, bool starts, int64_t sequences,
@@ -455,7 +771,7 @@ using namespace bt;
 extern "C" size_t bt_cached_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t table_width,
                                                       int64_t max_length, int has_starts, int64_t sequences, int64_t prefix_length) {
     if (!shape_ok(tokens, heads, kv_heads, head_dim, page_size, table_width, max_length, has_starts != 0, sequences, prefix_length)) return 0;
-    return attend_plan(tokens, heads, kv_heads, head_dim, page_size, max_length, has_starts != 0, sequences, prefix_length).bytes;
+    return attend_plan(tokens, heads, kv_heads, head_dim, max_length, has_starts != 0, sequences, prefix_length).bytes;
 }
 
 extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const void* k_cache, const void* v_cache, int64_t pages,
@@ -483,7 +799,7 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
         set_error("%s: the cache has to be 16-byte aligned", who);
         return BT_ERR_INVALID;
     }
-    const AttendPlan a = attend_plan(tokens, heads, kv_heads, head_dim, page_size, max_length, q_starts != nullptr, sequences, prefix_length);
+    const AttendPlan a = attend_plan(tokens, heads, kv_heads, head_dim, max_length, q_starts != nullptr, sequences, prefix_length);
     if (a.bytes && (!workspace || workspace_bytes < a.bytes || ((uintptr_t)workspace) % 256 != 0)) {
         set_error("%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, a.bytes, workspace_bytes);
         return BT_ERR_WORKSPACE;
@@ -491,24 +807,30 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
     AttendParams p = {};
     p.q = q, p.k_cache = k_cache, p.v_cache = v_cache, p.table = block_table, p.lengths = lengths, p.starts = q_starts, p.prefix_table = prefix_table;
     p.q_token = q_token, p.q_head = q_head, p.tokens = tokens, p.out = out, p.lse = lse;
-    p.part_ml = a.parts ? (float2*)workspace : nullptr;
-    p.part_o = a.parts ? (float*)((char*)workspace + a.ml_bytes) : nullptr;
+    auto parts = [&](const Region& r) { return r.rows ? Parts{(float*)((char*)workspace + r.o), (float2*)((char*)workspace + r.ml)} : Parts{nullptr, nullptr}; };
+    p.few_parts = parts(a.few_region), p.wide_parts = parts(a.wide_region), p.prefix_parts = parts(a.prefix_region);
     p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads), p.dim = (int)head_dim, p.dp = cache_head_dim(dtype, head_dim);
     p.n_seq = (int)sequences, p.width = (int)table_width, p.page_shift = __builtin_ctzll((unsigned long long)page_size), p.pages = (int)pages;
     p.prefix = (int)prefix_length;
-    p.chunk = (int)a.chunk, p.prefix_chunk = (int)a.prefix_chunk, p.chunks = (int)a.chunks, p.prefix_chunks = (int)a.prefix_chunks;
-    p.units = (int)a.units, p.prefix_units = (int)a.prefix_units, p.seq_tiles = (int)ceil_div(p.group, 16), p.longest = (int)max_length;
+    p.longest = (int)max_length, p.few_rows = (int)FEW_ROWS, p.few_slots = (int)a.few_slots, p.join_few = a.join_few;
+    p.chunk = (int)a.chunk, p.chunks = (int)a.chunks, p.tiles = (int)a.tiles;
+    p.wide_chunk = (int)a.wide_chunk, p.wide_chunks = (int)a.wide_chunks, p.wide_tiles = (int)a.wide_tiles;
+    p.prefix_chunk = (int)a.prefix_chunk, p.prefix_chunks = (int)a.prefix_chunks, p.prefix_tiles = (int)a.prefix_tiles, p.prefix_wide = a.prefix_wide;
     const int e = 16 / dtype_size(dtype);
     p.wide_q = head_dim % e == 0 && q_token % e == 0 && q_head % e == 0 && ((uintptr_t)q) % 16 == 0;
     p.scale2 = (float)((double)scale * 1.4426950408889634074);
-    const int64_t blocks = (a.units * a.chunks + a.prefix_units * a.prefix_chunks) * kv_heads + (q_starts && !a.parts ? 1 : 0);
-    if (blocks >= (1 << 24) || a.units > 0x7fffffff || a.prefix_units > 0x7fffffff) {
-        set_error("%s: %lld workgroups are beyond one launch", who, (long long)blocks);
+    const int64_t prefix_blocks = a.prefix_tiles * a.prefix_chunks * kv_heads;
+    const bool clear = q_starts && (a.join_few || (!a.few_parts && !a.wide_parts));  // (attend_join_kernel sees to the rows behind otherwise)
+    const int64_t few_blocks = (a.few ? sequences * a.tiles * a.chunks * kv_heads : 0) + (a.prefix_wide ? 0 : prefix_blocks) + (clear ? 1 : 0);
+    const int64_t wide_blocks = (a.wide ? a.wide_tiles * a.wide_chunks * kv_heads : 0) + (a.prefix_wide ? prefix_blocks : 0);
+    const int64_t join_rows = a.join_few ? a.few_region.rows : a.few_parts || a.wide_parts ? tokens * heads : 0;
+    if (std::max({few_blocks, wide_blocks, join_rows / 4}) >= (1 << 22) || a.wide_tiles > 0x7fffffff || a.prefix_tiles > 0x7fffffff) {
+        set_error("%s: %lld workgroups are beyond one launch", who, (long long)std::max(few_blocks, wide_blocks));
         return BT_ERR_INVALID;
     }
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == BT_F32) launch_attend<BT_F32>(p, blocks, st);
-    else if (dtype == BT_F16) launch_attend<BT_F16>(p, blocks, st);
-    else launch_attend<BT_BF16>(p, blocks, st);
+    if (dtype == BT_F32) launch_attend<BT_F32>(p, few_blocks, wide_blocks, join_rows, st);
+    else if (dtype == BT_F16) launch_attend<BT_F16>(p, few_blocks, wide_blocks, join_rows, st);
+    else launch_attend<BT_BF16>(p, few_blocks, wide_blocks, join_rows, st);
     return check_launch(who);
 }

@@ -164,7 +164,7 @@ __global__ __launch_bounds__(TURN_THREADS) void cache_append_kernel(TurnParams p
         s = found - 1;
         if (s < 0) return;
         t0 = std::max(p.starts[s], 0);
-        n = (int)(std::min<int64_t>(p.starts[s + 1], p.tokens) - t0);
+        n = (int)std::max<int64_t>(0, std::min<int64_t>(p.starts[s + 1], p.tokens) - t0);
         group = (int64_t)blockIdx.x - (t0 / E + 2 * (int64_t)s);
     }
     if (n <= 0) return;
