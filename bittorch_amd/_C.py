@@ -1277,7 +1277,9 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: T
         starts = None if q_starts is None else q_starts.contiguous()
         prefix = prefix_table.contiguous() if prefix_length else None
         with _on(q):
-            ws = _workspace(_L.bt_cached_attention_workspace_bytes(tokens, heads, kv_heads, dim, page, width, longest, int(starts is not None), n_seq,
+            per = 16 // q.element_size()
+            in_place = all(n % per == 0 for n in (dim, q.stride(0), q.stride(1))) and q.data_ptr() % 16 == 0
+            ws = _workspace(_L.bt_cached_attention_workspace_bytes(dt, int(in_place), tokens, heads, kv_heads, dim, page, width, longest, int(starts is not None), n_seq,
                                                                    prefix_length), q.device)
             _status(_L.bt_cached_attention(
                 q.data_ptr(), q.stride(0), q.stride(1), dt, k_cache.data_ptr(), v_cache.data_ptr(), pages, page, table.data_ptr(), width, longest,

@@ -103,7 +103,7 @@ SIGNATURES = {
     "bt_cache_head_dim": (_int, [_int, _i64]),
     "bt_cache_append": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _int, _int, ctypes.c_float, _i64, _i64, _i64, _i64,
                                _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp]),
-    "bt_cached_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64]),
+    "bt_cached_attention_workspace_bytes": (_sz, [_int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64]),
     "bt_cached_attention": (_int, [_vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, ctypes.c_float, _i64,
                                    _i64, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
 }

@@ -10,6 +10,8 @@
 #include "lds_dma.h"
 #include "paged_cache.h"
 
+#include <utility>
+
 namespace bt {
 
 // What workgroups leave for attend_join_kernel: [row][chunk], rows by (sequence, key head, row of it) of attend_rows_kernel's sequences and by
@@ -21,11 +23,11 @@ struct Parts {
 struct AttendParams {
     const void *q, *k_cache, *v_cache;
     const int32_t *table, *lengths, *starts, *prefix_table;
-    int64_t q_token, q_head, tokens;
+    int64_t q_token, q_head;
     void* out;
     float* lse;          // may be null
-    int heads, kv_heads, group, dim, dp, n_seq, width, page_shift, pages, prefix;
-    int longest, wide_q;
+    int tokens, heads, kv_heads, group, dim, q_dim, dp, n_seq, width, page_shift, pages, prefix;  // q_dim: features that q's rows have in memory
+    int longest;
     int few_rows;        // sequences of up to so many rows are attend_rows_kernel's, others attend_tiles_kernel's
     // of the two kernels: places of a chunk of a sequence, chunks of the longest, and row tiles (few: of each sequence, wide: of all of them)
     int chunk, chunks, tiles, wide_chunk, wide_chunks, wide_tiles;
@@ -107,13 +109,6 @@ __device__ __forceinline__ bool take_specials(u32x4& v, u32x4& where) {
     }
     return any;
 }
-template <int DT>
-__device__ __forceinline__ v4f add_specials(v4f o, u32x4 where, u32x4 weights) {
-    const v4f seen = step<DT>(where, weights, v4f{0, 0, 0, 0});
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = seen[i] > 0.0f ? __builtin_nanf("") : o[i];
-    return o;
-}
 __device__ __forceinline__ float over_groups_max(float x) {  // over the four lanes of a row
     x = fmaxf(x, __shfl_xor(x, 16));
     return fmaxf(x, __shfl_xor(x, 32));
@@ -126,53 +121,54 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 // What a workgroup works on: up to R rows of one key head and a chunk of their keys.
 struct Job {
     const int32_t* table;
-    int rows;            // of the tile
-    int64_t token0;      // row r is token token0 + (row0 + r) / G, head kv * G + (row0 + r) % G
-    int64_t row0;
-    int limit0;          // row r sees the places below limit0 + (row0 + r) / G (own) or limit0 (prefix)
-    bool causal, bad;    // bad: the length is beyond the table
-    int begin, end;      // the chunk's places
-    int part, kv, slots;  // slots: parts of a row
+    int rows, row0;       // row r of the tile is token token0 + (row0 + r) / G, head kv * G + (row0 + r) % G
+    int token0, kv;
+    int limit0;           // row r sees the places below limit0 + (row0 + r) / G (own) or limit0 (prefix)
+    bool causal, bad;     // bad: the length is beyond the table
+    int begin, end;       // the chunk's places
+    int part, slots;      // slots: parts of a row
     int64_t few_slot;     // >= 0: of row 0 in few_parts
     Parts parts;
 };
-__device__ __forceinline__ int limit_of(const AttendParams& p, const Job& j, int r) { return j.causal ? j.limit0 + (int)((j.row0 + r) / p.group) : j.limit0; }
+__device__ __forceinline__ int group_row(const AttendParams& p, const Job& j, int r) { return (int)((uint32_t)(j.row0 + r) / (uint32_t)p.group); }
+__device__ __forceinline__ int limit_of(const AttendParams& p, const Job& j, int r) { return j.limit0 + (j.causal ? group_row(p, j, r) : 0); }
 
 // A sequence's tokens [t0, t0 + n) and its length, as far as the table goes; whether it goes beyond
-__device__ __forceinline__ bool sequence_of(const AttendParams& p, int s, int64_t* t0, int* n, int* length) {
-    *t0 = p.starts ? std::max(p.starts[s], 0) : s;
-    *n = p.starts ? (int)std::max<int64_t>(0, std::min<int64_t>(p.starts[s + 1], p.tokens) - *t0) : 1;  // (0 <= t0, t0 + n <= tokens where n > 0)
+__device__ __forceinline__ bool sequence_of(const AttendParams& p, int s, int* t0, int* n, int* length) {
+    const int64_t first = p.starts ? std::max(p.starts[s], 0) : s;
+    *n = p.starts ? (int)std::max<int64_t>(0, std::min<int64_t>(p.starts[s + 1], p.tokens) - first) : 1;  // (0 <= t0, t0 + n <= tokens where n > 0)
+    *t0 = (int)first;
     const int got = p.lengths[s];
     *length = std::max(0, std::min(got, p.longest));
     return got > p.longest;
 }
 
 // Block `block` of the prefix: row tile, key head, chunk.
-__device__ __forceinline__ bool prefix_job(const AttendParams& p, int R, int64_t block, Job* j) {
-    const int c = (int)(block % p.prefix_chunks);
-    j->kv = (int)(block / p.prefix_chunks % p.kv_heads);
-    j->row0 = block / p.prefix_chunks / p.kv_heads * R;
+__device__ __forceinline__ bool prefix_job(const AttendParams& p, int R, uint32_t block, Job* j) {
+    const uint32_t at = block / (uint32_t)p.prefix_chunks, c = block - at * p.prefix_chunks, tile = at / (uint32_t)p.kv_heads;
+    j->kv = (int)(at - tile * p.kv_heads);
+    j->row0 = (int)tile * R;
     j->token0 = 0;
-    j->rows = (int)std::min<int64_t>(R, p.tokens * p.group - j->row0);
+    j->rows = std::min(R, p.tokens * p.group - j->row0);
     j->table = p.prefix_table;
     j->limit0 = p.prefix;
     j->causal = j->bad = false;
-    j->begin = c * p.prefix_chunk;
+    j->begin = (int)c * p.prefix_chunk;
     j->end = std::min(j->begin + p.prefix_chunk, p.prefix);
-    j->part = c;
+    j->part = (int)c;
     j->slots = p.prefix_chunks;
     j->few_slot = -1;
     j->parts = p.prefix_parts;
     return j->rows > 0;
 }
 // The tile of rows [tile * R, ...) of sequence s and chunk c of its places.  False: nothing to do.
-__device__ __forceinline__ bool own_job(const AttendParams& p, int R, int s, int64_t tile, int c, int chunk, bool wide, Job* j) {
+__device__ __forceinline__ bool own_job(const AttendParams& p, int R, int s, int tile, int c, int chunk, bool wide, Job* j) {
     int n, length;
     j->bad = sequence_of(p, s, &j->token0, &n, &length);
     j->row0 = tile * R;
-    const int64_t rows = (int64_t)n * p.group;
+    const int rows = n * p.group;
     if (n <= 0 || j->row0 >= rows || (rows > p.few_rows) != wide) return false;
-    j->rows = (int)std::min<int64_t>(R, rows - j->row0);
+    j->rows = std::min(R, rows - j->row0);
     j->table = p.table + (int64_t)s * p.width;
     j->limit0 = length - n + 1;
     j->causal = true;
@@ -183,11 +179,6 @@ __device__ __forceinline__ bool own_job(const AttendParams& p, int R, int s, int
     j->few_slot = wide ? -1 : ((int64_t)s * p.kv_heads + j->kv) * p.few_slots + j->row0;
     j->parts = wide ? p.wide_parts : p.few_parts;
     return j->begin < j->end || (!j->parts.o && c == 0);
-}
-// Where row `r` of the job is written: row of the result
-__device__ __forceinline__ int64_t out_row_of(const AttendParams& p, const Job& j, int r) {
-    const int64_t rw = j.row0 + r;
-    return (j.token0 + rw / p.group) * p.heads + j.kv * p.group + rw % p.group;
 }
 // The chunk's pages, one a lane, 64 at a time.
 struct PageWindow {
@@ -214,52 +205,62 @@ struct PageWindow {
 // The rows behind the last sequence, where no job sees to them
 template <int DT>
 __device__ __forceinline__ void clear_rows_behind(const AttendParams& p) {
-    const int64_t n = (int64_t)p.heads * p.dim, behind = std::max<int64_t>(0, std::min<int64_t>(p.starts[p.n_seq], p.tokens));
+    const int64_t n = (int64_t)p.heads * p.dim, behind = std::max(0, std::min(p.starts[p.n_seq], p.tokens));
     for (int64_t i = behind * n + threadIdx.x; i < p.tokens * n; i += blockDim.x) store_elem<DT>(p.out, i, 0.0f);
     for (int64_t i = behind * p.heads + threadIdx.x; p.lse && i < p.tokens * p.heads; i += blockDim.x) p.lse[i] = -__builtin_inff();
 }
-// Piece c of a row of q (E features from c TK + g E) as an operand; features behind the head are zero
-template <int DT>
-__device__ __forceinline__ u32x4 q_piece(const AttendParams& p, int64_t row_at, int f) {
-    constexpr int E = CacheOrder<DT>::E;
-    u32x4 q = {0, 0, 0, 0};
-    if (f >= p.dim) return q;
-    if (p.wide_q) return *(const u32x4*)((const char*)p.q + (row_at + f) * CacheOrder<DT>::SIZE);
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        if (f + e >= p.dim) break;
-        if constexpr (DT == BT_F32) q[e] = ((const uint32_t*)p.q)[row_at + f + e];
-        else q[e / 2] |= (uint32_t)((const uint16_t*)p.q)[row_at + f + e] << (e % 2 * 16);
-    }
-    return q;
+// Of the row with group_row `in_group`: where its q starts, and E features of it from f on (zero behind the head)
+__device__ __forceinline__ int64_t q_row(const AttendParams& p, const Job& j, int r, int in_group) {
+    return (int64_t)(j.token0 + in_group) * p.q_token + (int64_t)(j.kv * p.group + j.row0 + r - in_group * p.group) * p.q_head;
 }
+template <int DT>
+__device__ __forceinline__ u32x4 q_piece(const AttendParams& p, int64_t row_at, int f, bool there) {
+    return there && f < p.q_dim ? *(const u32x4*)((const char*)p.q + (row_at + f) * CacheOrder<DT>::SIZE) : u32x4{0, 0, 0, 0};
+}
+// q in rows of dp features, zero behind the head, where its own do not start or end on 16 bytes
+template <int DT>
+__global__ __launch_bounds__(256) void attend_copy_kernel(AttendParams p, void* to) {
+    const int64_t n = (int64_t)p.tokens * p.heads * p.dp;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / p.dp, token = row / p.heads;
+        const int f = (int)(i - row * p.dp);
+        if constexpr (DT == BT_F32) ((uint32_t*)to)[i] = f < p.dim ? ((const uint32_t*)p.q)[token * p.q_token + (row - token * p.heads) * p.q_head + f] : 0u;
+        else ((uint16_t*)to)[i] = f < p.dim ? ((const uint16_t*)p.q)[token * p.q_token + (row - token * p.heads) * p.q_head + f] : (uint16_t)0;
+    }
+}
+// Four features of a row, as they are returned
+template <int DT>
+__device__ __forceinline__ void put_features(const AttendParams& p, int64_t out_row, int f, v4f acc) {
+    if (p.dim % 4 == 0) {
+        if constexpr (DT == BT_F32) *(v4f*)((float*)p.out + out_row * p.dim + f) = acc;
+        else {
+            u32x2 w;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                w[i] = DT == BT_F16 ? f32_to_f16_bits(acc[2 * i]) | (uint32_t)f32_to_f16_bits(acc[2 * i + 1]) << 16
+                                    : f32_to_bf16_bits(acc[2 * i]) | (uint32_t)f32_to_bf16_bits(acc[2 * i + 1]) << 16;
+            *(u32x2*)((uint16_t*)p.out + out_row * p.dim + f) = w;
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < 4; i++)
+        if (f + i < p.dim) store_elem<DT>(p.out, out_row * p.dim + f + i, i == 0 ? acc[0] : i == 1 ? acc[1] : i == 2 ? acc[2] : acc[3]);
+}
+__device__ __forceinline__ float lse_of(float top, float sum) { return sum == 0.0f ? -__builtin_inff() : top * 0.69314718055994530942f + __logf(sum); }
 // Four features of row r of the job, finished or for attend_join_kernel; top: the row's maximum, in powers of two
 template <int DT>
 __device__ __forceinline__ void put_row(const AttendParams& p, const Job& j, int r, int f, v4f acc, float top, float sum) {
-    const int64_t out_row = out_row_of(p, j, r);
+    const int in_group = group_row(p, j, r);
+    const int64_t out_row = (int64_t)(j.token0 + in_group) * p.heads + j.kv * p.group + j.row0 + r - in_group * p.group;
     if (j.parts.o) {
         const int64_t at = (j.few_slot >= 0 ? j.few_slot + r : out_row) * j.slots + j.part;
         if (f == 0) j.parts.ml[at] = make_float2(top, sum);
         *(v4f*)(j.parts.o + at * part_stride(p.dim) + f) = acc;  // (what lies behind the head is not read)
         return;
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (p.dim % 4 == 0) {
-        if constexpr (DT == BT_F32) *(v4f*)((float*)p.out + out_row * p.dim + f) = acc * inverse;
-        else {
-            u32x2 w;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float a = acc[2 * i] * inverse, b = acc[2 * i + 1] * inverse;
-                w[i] = DT == BT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16 : f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16;
-            }
-            *(u32x2*)((uint16_t*)p.out + out_row * p.dim + f) = w;
-        }
-    } else {
-        for (int i = 0; i < 4; i++)
-            if (f + i < p.dim) store_elem<DT>(p.out, out_row * p.dim + f + i, acc[i] * inverse);
-    }
-    if (f == 0 && p.lse) p.lse[out_row] = sum == 0.0f ? -__builtin_inff() : top * 0.69314718055994530942f + __logf(sum);
+    put_features<DT>(p, out_row, f, acc * (sum == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum)));
+    if (f == 0 && p.lse) p.lse[out_row] = lse_of(top, sum);
 }
 
 // B: blocks of 32 features, the last one maybe in part (the first FULL groups of TK features are whole).  Four waves take the chunk's tiles of TK places in turn, each with all rows.
@@ -273,18 +274,16 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     Job j;
     {
-        int64_t block = blockIdx.x;
-        const int64_t prefix_blocks = p.prefix_wide ? 0 : (int64_t)p.prefix_tiles * p.kv_heads * p.prefix_chunks;
+        uint32_t block = blockIdx.x;
+        const uint32_t prefix_blocks = p.prefix_wide ? 0 : p.prefix_tiles * p.kv_heads * p.prefix_chunks;
         if (block < prefix_blocks) {
             if (!prefix_job(p, R, block, &j)) return;
         } else {
             block -= prefix_blocks;
-            const int c = (int)(block % p.chunks);
-            block /= p.chunks;
-            j.kv = (int)(block % p.kv_heads);
-            block /= p.kv_heads;
-            if (block / p.tiles >= p.n_seq) return clear_rows_behind<DT>(p);
-            if (!own_job(p, R, (int)(block / p.tiles), block % p.tiles, c, p.chunk, false, &j)) return;
+            const uint32_t at = block / (uint32_t)p.chunks, unit = at / (uint32_t)p.kv_heads, s = unit / (uint32_t)p.tiles;
+            j.kv = (int)(at - unit * p.kv_heads);
+            if ((int)s >= p.n_seq) return clear_rows_behind<DT>(p);
+            if (!own_job(p, R, (int)s, (int)(unit - s * p.tiles), (int)(block - at * p.chunks), p.chunk, false, &j)) return;
         }
     }
     const int kv = j.kv;
@@ -293,12 +292,12 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
     const int tiles = j.end > j.begin ? (j.end - j.begin + TK - 1) / TK : 0;
 
     // this lane's row as an operand
-    const int64_t row = j.row0 + r;
-    const int64_t q_at = (j.token0 + row / p.group) * p.q_token + (kv * p.group + (int)(row % p.group)) * p.q_head;
-    const int limit = r < j.rows ? limit_of(p, j, r) : 0, lowest = limit_of(p, j, 0);
+    const bool there = r < j.rows;
+    const int in_group = group_row(p, j, r), limit = there ? j.limit0 + (j.causal ? in_group : 0) : 0, lowest = limit_of(p, j, 0);
+    const int64_t q_at = q_row(p, j, r, in_group);
     u32x4 q[C];
 #pragma unroll
-    for (int c = 0; c < C; c++) q[c] = r < j.rows ? q_piece<DT>(p, q_at, c * TK + g * E) : u32x4{0, 0, 0, 0};
+    for (int c = 0; c < C; c++) q[c] = q_piece<DT>(p, q_at, c * TK + g * E, there);
 
     float m = -__builtin_inff(), l = 0.0f;  // of the row; l: of this lane's places
     v4f o[V];
@@ -362,10 +361,17 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
         u32x4 lo;
         const u32x4 hi = operand<DT>(w, &lo);
         if (masked) {
+            bool special = false;
+            u32x4 where[V];
 #pragma unroll
-            for (int b = 0; b < V; b++) {
-                u32x4 where;
-                if (__any(take_specials<DT>(v[b], where))) o[b] = add_specials<DT>(o[b], where, hi);
+            for (int b = 0; b < V; b++) special |= take_specials<DT>(v[b], where[b]);
+            if (__any(special)) {
+#pragma unroll
+                for (int b = 0; b < V; b++) {
+                    const v4f seen = step<DT>(where[b], hi, v4f{0, 0, 0, 0});
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[b][i] = seen[i] > 0.0f ? __builtin_nanf("") : o[b][i];
+                }
             }
         }
 #pragma unroll
@@ -406,198 +412,374 @@ __global__ __launch_bounds__(256) void attend_rows_kernel(AttendParams p) {
     }
 }
 
-// RT row tiles of 16 a wave and four waves: 128 rows (64 of more than 128 features, whose sums take twice the registers), whose keys and values pass through LDS once for all of them, two stages of ST tiles of TK
-// places.  A stage is read from memory straight into LDS, in the order in which the waves take it from there (16 bytes a lane in a row: no bank
-// is asked twice), while the one before is worked on.
+// RT row tiles of 16 a wave and four waves: 128 rows (64 of more than 128 features, whose sums take twice the registers), whose keys and
+// values pass through LDS once for all of them, a tile of TK places at a time.  Tiles are read from memory straight into LDS, in the order in
+// which the waves take them from there (16 bytes a lane in a row: no bank is asked twice), up to NR tiles ahead.
 //
-// The exponentials are the other half of the work: per 32 places and 16 rows the matrix cores need 16 x 16 cycles (128 features) and the 8
-// weights of a lane about as many, so the instructions around them are few.  The maximum is that of the products before they are
-// scaled, and one multiply-add and the exponential make a weight.  It is raised only where a weight would pass 2^8: it needs to be near the true maximum, not to be it.
-// 16-bit weights are rounded once (the rows kernel's two halves would be half as many matrix instructions again): results are 1.4 times
-// as far from 64 bits as by their own rounding.  Their sum is that of the weights before they are rounded, as lse wants it.
+// What bounds it.  A tile costs a wave (128 features) 32 matrix instructions of 16 cycles, and as many cycles for its 16 exponentials a lane
+// and the three or four instructions around each; LDS gives 64 bytes a cycle, so that the 16 KiB of fragments of each of a compute unit's eight
+// waves take 2000 cycles, and that is what a tile takes (0.87 us).  One block of instructions works on three tiles, the products of tile i + 1,
+// the weights of tile i and the sums over the values of tile i - 1, none of which waits for another: one thing after the other
+// took 1.4 us.  With 64 rows a wave and one wave a SIMD, which halves the fragments, it took 1.9 us: the sums live in accumulation registers then,
+// and the moves are more than what they spare.
+//
+// The maximum is that of the products before they are scaled, and one multiply-add and the exponential make a weight.  It is raised only where a
+// weight would pass 2^8: it needs to be near the true maximum, not to be it.  16-bit weights are rounded once (the rows kernel's two halves
+// would be half as many matrix instructions again): results are 1.4 times as far from 64 bits as by their own rounding.  Their sum is that of
+// the weights before they are rounded, as lse wants it.
+template <typename Body, int... I>
+__device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, Body body) {  // body(0), body(1) ..., each with its number as a constant
+    (body(std::integral_constant<int, I>()), ...);
+}
+template <int B>
+struct WideTile {
+    static constexpr int RT = B <= 4 ? 2 : 1, R = 64 * RT;
+};
 template <int DT, int B>
 __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     using Order = CacheOrder<DT>;
-    constexpr int E = Order::E, TK = Order::TK, C = 32 * B / TK, V = 2 * B, FULL = 32 * (B - 1) / TK, RT = B <= 4 ? 2 : 1, R = 64 * RT;
-    constexpr int ST = B <= 4 ? 2 : 1, TILE = 2048 * B, STAGE = 2 * ST * TILE;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];  // (from offset 0: loads into LDS reach 64 KiB)
+    constexpr int E = Order::E, TK = Order::TK, C = 32 * B / TK, H = E / 4, V = 2 * B, RT = WideTile<B>::RT, R = WideTile<B>::R;
+    constexpr int TILE = 2048 * B;                                        // bytes of a tile's keys or values
+    constexpr int NR = 32768 / TILE < 4 ? 32768 / TILE : 4;               // of each in LDS (loads into LDS reach 64 KiB)
+    constexpr int LOADS = 2 * ((2 * B + 3) / 4);                          // of a wave for a tile
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * NR * TILE];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     Job j;
     {
-        int64_t block = blockIdx.x;
-        const int64_t prefix_blocks = p.prefix_wide ? (int64_t)p.prefix_tiles * p.kv_heads * p.prefix_chunks : 0;
+        uint32_t block = blockIdx.x;
+        const uint32_t prefix_blocks = p.prefix_wide ? p.prefix_tiles * p.kv_heads * p.prefix_chunks : 0;
         if (block < prefix_blocks) {
             if (!prefix_job(p, R, block, &j)) return;
         } else {
             block -= prefix_blocks;
-            const int c = (int)(block % p.wide_chunks);
-            block /= p.wide_chunks;
-            j.kv = (int)(block % p.kv_heads);
-            const int64_t unit = block / p.kv_heads;
-            int s;
-            int64_t tile;
+            const uint32_t at = block / (uint32_t)p.wide_chunks, unit = at / (uint32_t)p.kv_heads;
+            j.kv = (int)(at - unit * p.kv_heads);
+            int s, tile;
             if (p.starts) {
                 // sequence s has the tiles floor(starts[s] G / R) + s and on: n tokens have n G / R + 1 tiles at most
+                auto first_of = [&](int i) { return (uint32_t)((uint64_t)(uint32_t)std::max(p.starts[i], 0) * (uint32_t)p.group / R) + (uint32_t)i; };
                 int found = 0;
                 for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
                     const int i = s0 + lane;
-                    const uint64_t hit = __ballot(i < p.n_seq && (int64_t)std::max(p.starts[i < p.n_seq ? i : 0], 0) * p.group / R + i <= unit);
+                    const uint64_t hit = __ballot(i < p.n_seq && first_of(i < p.n_seq ? i : 0) <= unit);
                     found += __popcll(hit);
                     if (hit != ~0ull) break;
                 }
                 s = found - 1;
                 if (s < 0) return;
-                tile = unit - ((int64_t)std::max(p.starts[s], 0) * p.group / R + s);
-                if (tile < 0) return;  // (starts that do not ascend)
+                const uint32_t first = first_of(s);
+                if (first > unit) return;  // (starts that do not ascend)
+                tile = (int)(unit - first);
             } else {
-                const int each = (p.group + R - 1) / R;
+                const uint32_t each = (uint32_t)(p.group + R - 1) / R;
                 s = (int)(unit / each);
-                tile = unit % each;
+                tile = (int)(unit - s * each);
             }
-            if (!own_job(p, R, s, tile, c, p.wide_chunk, true, &j)) return;
+            if (!own_job(p, R, s, tile, (int)(block - at * p.wide_chunks), p.wide_chunk, true, &j)) return;
         }
     }
-    PageWindow pages(p, j);
     const int tiles = j.end > j.begin ? (j.end - j.begin + TK - 1) / TK : 0;
     const int mine = wave * RT * 16;  // this wave's first row
     u32x4 q[RT][C];
     int limit[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-        const int at = mine + t * 16 + r;
-        const int64_t row = j.row0 + at;
-        const int64_t q_at = (j.token0 + row / p.group) * p.q_token + (j.kv * p.group + (int)(row % p.group)) * p.q_head;
-        limit[t] = at < j.rows ? limit_of(p, j, at) : 0;
+        const int at = mine + t * 16 + r, in_group = group_row(p, j, at);
+        const int64_t q_at = q_row(p, j, at, in_group);
+        limit[t] = at < j.rows ? j.limit0 + (j.causal ? in_group : 0) : 0;
 #pragma unroll
-        for (int c = 0; c < C; c++) q[t][c] = at < j.rows ? q_piece<DT>(p, q_at, c * TK + g * E) : u32x4{0, 0, 0, 0};
+        for (int c = 0; c < C; c++) q[t][c] = q_piece<DT>(p, q_at, c * TK + g * E, at < j.rows);
     }
-    // the places that some row of the wave sees, and those that all see
-    const int reach = mine < j.rows ? limit_of(p, j, std::min(mine + 16 * RT, j.rows) - 1) : 0;
-    const int lowest = mine < j.rows ? limit_of(p, j, mine) : 0;
+    // the places that some row of the wave sees, and those that all see; the wave's tiles
+    const int reach = mine < j.rows ? std::min(limit_of(p, j, std::min(mine + 16 * RT, j.rows) - 1), j.end) : 0;
+    const int lowest = mine < j.rows ? std::min(limit_of(p, j, mine), j.end) : 0;
+    const int my_tiles = reach > j.begin ? (reach - j.begin + TK - 1) / TK : 0;
 
     const int64_t page_elements = (int64_t)p.dp << p.page_shift;
     const int pieces = p.dp * TK * Order::SIZE / 1024;  // KiB of a tile's keys
-    auto fetch = [&](int stage) {
+    int64_t at1 = 0, at2 = 0, at3 = 0;                  // where the last three tiles of keys came from: their values follow
+    auto load = [&](uint32_t to, const char* from) {
 #pragma unroll
-        for (int u = 0; u < ST; u++) {
-            const int tile = stage * ST + u, place = j.begin + tile * TK;
-            if (tile >= tiles) break;
-            const int64_t at = ((pages.of(p, j, place) * p.kv_heads + j.kv) * page_elements + (int64_t)(place & ((1 << p.page_shift) - 1)) * p.dp) * Order::SIZE;
-            const uint32_t to = lds0 + (uint32_t)(stage & 1) * STAGE + u * 2 * TILE;
-#pragma unroll
-            for (int i0 = 0; i0 < V; i0 += 4) {
-                const int i = i0 + wave;
-                if (i < pieces) {
-                    dma16(to + i * 1024, i * 1024 + lane * 16, (const char*)p.k_cache + at);
-                    dma16(to + TILE + i * 1024, i * 1024 + lane * 16, (const char*)p.v_cache + at);
-                }
-            }
+        for (int i0 = 0; i0 < V; i0 += 4) {
+            const int i = std::min(i0 + wave, pieces - 1);  // (every wave makes as many loads: they are counted)
+            dma16(to + i * 1024, i * 1024 + lane * 16, from);
         }
     };
+    // The page of the tile whose keys are loaded next: a scalar load each, so that no wait for it waits for the tiles on their way.
+    typedef const __attribute__((address_space(4))) int32_t* ScalarPointer;
+    const ScalarPointer table = (ScalarPointer)(uintptr_t)j.table;
+    int page = tiles ? table[j.begin >> p.page_shift] : 0;
+    bool bad = j.bad;
+    auto load_keys = [&](int tile) {  // (behind the last tile that one again, for the count)
+        const int place = j.begin + std::min(tile, tiles - 1) * TK;
+        if ((uint32_t)page >= (uint32_t)p.pages) page = 0, bad = true;
+        at3 = at2, at2 = at1;
+        at1 = (((int64_t)page * p.kv_heads + j.kv) * page_elements + (int64_t)(place & ((1 << p.page_shift) - 1)) * p.dp) * Order::SIZE;
+        load(lds0 + (uint32_t)(tile % NR) * TILE, (const char*)p.k_cache + at1);
+        page = table[(j.begin + std::min(tile + 1, tiles - 1) * TK) >> p.page_shift];
+    };
+    // (at: where the tile's keys came from)
+    auto load_values = [&](int tile, int64_t at) { load(lds0 + (uint32_t)(NR + tile % NR) * TILE, (const char*)p.v_cache + at); };
 
-    v4f o[RT][V];
-    float m[RT], l[RT];  // the rows' maxima (of the products before they are scaled) and sums (of this lane's places)
+    v4f o[RT][V], s[RT][H];       // s: products of the tile whose weights come next
+    float m[RT], l[RT], top[RT];  // the rows' maxima (of the products before they are scaled), sums and s's maxima (of this lane's places)
+    u32x4 w[RT];                  // weights of the tile before
+    std::conditional_t<(V > 8), uint64_t, uint32_t> nan[RT];  // features 16 b + 4 g + e, bit 4 b + e, that saw a value that is no number
     const float slack = 8.0f / p.scale2;
     // The multiply-add rounds once, the base alone too: logits of a size at which that is more than a part of one are rounded alike first.
     bool large = false;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-        m[t] = -__builtin_inff(), l[t] = 0.0f;
+        m[t] = -__builtin_inff(), l[t] = 0.0f, top[t] = 0.0f, nan[t] = 0;
+        w[t] = u32x4{0, 0, 0, 0};
 #pragma unroll
         for (int b = 0; b < V; b++) o[t][b] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < H; h++) s[t][h] = v4f{0, 0, 0, 0};
     }
-    auto work = [&](const uint8_t* from, int place, auto masked_c) {
-        constexpr bool MASKED = decltype(masked_c)::value;
-        v4f s[RT][E / 4];
+    auto keys_at = [&](int tile) { return lds + tile % NR * TILE + lane * 16; };
+    auto values_at = [&](int tile) { return lds + (NR + tile % NR) * TILE + lane * 16; };
+    auto products = [&](const uint8_t* kf, v4f (&s)[RT][H]) {
 #pragma unroll
-        for (int h = 0; h < E / 4; h++) {
-#pragma unroll
-            for (int t = 0; t < RT; t++) s[t][h] = v4f{0, 0, 0, 0};
-            __builtin_amdgcn_sched_barrier(0);
+        for (int h = 0; h < H; h++)
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                u32x4 k = *(const u32x4*)(from + (c * (E / 4) + h) * 1024 + lane * 16);
-                if (c >= FULL && c * TK + g * E >= p.dim) k = u32x4{0, 0, 0, 0};  // (what lies behind the head was never written)
+                u32x4 k = *(const u32x4*)(kf + (c * H + h) * 1024);
+                if (DT == BT_F32 && c == C - 1 && c * TK >= p.dp) k = u32x4{0, 0, 0, 0};  // (a tile has one group of features less)
 #pragma unroll
-                for (int t = 0; t < RT; t++) s[t][h] = step<DT>(k, q[t][c], s[t][h]);
+                for (int t = 0; t < RT; t++) s[t][h] = step<DT>(k, q[t][c], c ? s[t][h] : v4f{0, 0, 0, 0});
             }
-        }
-        // (the three parts' operands together would not fit the registers)
-        __builtin_amdgcn_sched_barrier(0);
-        u32x4 w[RT];
+    };
+    auto maxima = [&]() {
 #pragma unroll
         for (int t = 0; t < RT; t++) {
+            top[t] = s[t][0][0];
+#pragma unroll
+            for (int e = 1; e < E; e++) top[t] = fmaxf(top[t], s[t][e / 4][e % 4]);
+        }
+    };
+    auto weights = [&](float scale, auto base_of, u32x4 (&w)[RT]) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const float base = base_of(t);
             float x[E];
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                x[e] = s[t][e / 4][e % 4];
-                if constexpr (MASKED) x[e] = place + g * E + e < limit[t] ? x[e] : -__builtin_inff();
-            }
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < E; e++) top = fmaxf(top, x[e]);
-            if (__any(top > m[t] + slack)) {
-                const float next = fmaxf(m[t], over_groups_max(top));
-                const float shrink = __builtin_amdgcn_exp2f(m[t] == next ? 0.0f : (m[t] - next) * p.scale2);
-                m[t] = next;
-                large |= __any(fabsf(next) * p.scale2 > 65536.0f);
-                l[t] *= shrink;
-#pragma unroll
-                for (int b = 0; b < V; b++) o[t][b] *= shrink;
-            }
-            const float base = m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2;
-#pragma unroll
-            for (int e = 0; e < E; e++) x[e] = __builtin_amdgcn_exp2f(large ? x[e] * p.scale2 + base : __builtin_fmaf(x[e], p.scale2, base));
+            for (int e = 0; e < E; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], scale, base));
             w[t] = operand<DT>(x, nullptr);
             float sum = x[0] + x[1];
 #pragma unroll
             for (int e = 2; e < E; e += 2) sum += x[e] + x[e + 1];
             l[t] += sum;
         }
-        __builtin_amdgcn_sched_barrier(0);
-        const uint8_t* vf = from + TILE + lane * 16;
-        const int live = MASKED ? j.end - (place + g * E) : E;  // no row sees what lies behind: whatever it is
+    };
+    auto over = [&]() {
+        bool any = false;
 #pragma unroll
-        for (int b = 0; b < V; b++) {
-            u32x4 v = *(const u32x4*)(vf + b * 1024);
-            if constexpr (MASKED) {
-                u32x4 where;
-                v = first_places<DT>(v, live);
-                if (__any(take_specials<DT>(v, where))) {
+        for (int t = 0; t < RT; t++) any |= top[t] > m[t] + slack;
+        return __any(any);
+    };
+    float shrink[RT];
+    auto raise = [&]() {  // m and l; the sums over values follow once those of the tile before are in
 #pragma unroll
-                    for (int t = 0; t < RT; t++) o[t][b] = add_specials<DT>(o[t][b], where, w[t]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < RT; t++) o[t][b] = step<DT>(v, w[t], o[t][b]);
+        for (int t = 0; t < RT; t++) {
+            const float next = fmaxf(m[t], over_groups_max(top[t]));
+            shrink[t] = __builtin_amdgcn_exp2f(m[t] == next ? 0.0f : (m[t] - next) * p.scale2);
+            m[t] = next;
+            l[t] *= shrink[t];
+            large |= __any(next != -__builtin_inff() && fabsf(next) * p.scale2 > 65536.0f);
         }
     };
-
-    const int stages = (tiles + ST - 1) / ST;
-    if (stages) fetch(0);
-    for (int stage = 0; stage < stages; stage++) {
-        // this stage has arrived, and all waves are done with the one before
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (stage + 1 < stages) fetch(stage + 1);
-#pragma unroll 1
-        for (int u = 0; u < ST; u++) {
-            const int place = j.begin + (stage * ST + u) * TK;
-            const uint8_t* from = lds + (stage & 1) * STAGE + u * 2 * TILE;
-            if (place >= reach || stage * ST + u >= tiles) break;
-            if (place + TK > lowest) work(from, place, std::true_type());
-            else work(from, place, std::false_type());
+    auto shrink_sums = [&]() {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int b = 0; b < V; b++) o[t][b] *= shrink[t];
+    };
+    // Iteration i loads the keys of tile i + NR and the values of tile i - 2 + NR into the places that iteration i - 1 read last, and reads
+    // what iteration i + 1 - NR loaded: what the last NR - 2 iterations loaded may still be on its way.
+    auto turn = [&](int i) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NR - 2) * LOADS) : "memory");
+        if (i < tiles) {
+            load_keys(i + NR);
+            load_values(i + NR - 2, at3);
         }
+    };
+    if (tiles) {
+        load_keys(0);
+#pragma unroll
+        for (int i = 1 - NR; i < 0; i++) {
+            load_keys(i + NR);
+            load_values(std::max(i + NR - 2, 0), i + NR >= 2 ? at3 : at2);
+        }
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NR - 1) * LOADS) : "memory");
+        if (my_tiles) products(keys_at(0), s);
     }
+    // tiles that all rows of the wave see as a whole
+    const int whole = lowest > j.begin ? (lowest - j.begin) / TK : 0;
+    for (int i = 0; i <= tiles && tiles;) {
+        if (i > 0 && i < whole && !large) {
+            maxima();
+            for (; i < whole && !large; i++) {
+                turn(i);
+                const bool raised = over();
+                if (raised) raise();
+                // F fragments, each with its matrix instructions and a share of the other pipe's work; loads run AHEAD fragments in front
+                constexpr int F = C * H + V, N = RT * E, AHEAD = 3;
+                const uint8_t *kf = keys_at(i + 1), *vf = values_at(i - 1);
+                u32x4 frag[F], w2[RT];
+                v4f s2[RT][H];
+                float x[RT][E], sum[RT], next_top[RT];
+                auto fetch = [&](int f) { frag[f] = *(const u32x4*)(f < C * H ? kf + (f % C * H + f / C) * 1024 : vf + (f - C * H) * 1024); };
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int at = mine + t * 16 + r;
-        const float sum = over_groups_sum(l[t]);
-        if (at >= j.rows) continue;
-        const float top = m[t] == -__builtin_inff() ? m[t] : m[t] * p.scale2;
+                for (int f = 0; f < AHEAD; f++) fetch(f);
+                unrolled(std::make_integer_sequence<int, F>(), [&](auto number) {
+                    constexpr int f = decltype(number)::value;
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (f + AHEAD < F) fetch(f + AHEAD);
+                    if constexpr (f < C * H) {
+                        constexpr int h = f / C, c = f % C;
+                        if (DT == BT_F32 && c == C - 1 && c * TK >= p.dp) frag[f] = u32x4{0, 0, 0, 0};  // (a tile has one group of features less)
 #pragma unroll
-        for (int b = 0; b < V; b++)
-            if (b * 16 + g * 4 < p.dim) put_row<DT>(p, j, at, b * 16 + g * 4, o[t][b], top, pages.bad ? __builtin_nanf("") : sum);
+                        for (int t = 0; t < RT; t++) s2[t][h] = step<DT>(frag[f], q[t][c], c ? s2[t][h] : v4f{0, 0, 0, 0});
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < RT; t++) o[t][f - C * H] = step<DT>(frag[f], w[t], o[t][f - C * H]);
+                    }
+#pragma unroll
+                    for (int n = f * N / F; n < (f + 1) * N / F; n++) {  // weights
+                        const int t = n / E, e = n % E;
+                        x[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], p.scale2, -m[t] * p.scale2));
+                        sum[t] = e ? sum[t] + x[t][e] : x[t][e];
+                        if (e == E - 1) {
+                            l[t] += sum[t];
+                            w2[t] = operand<DT>(x[t], nullptr);
+                        }
+                    }
+                    if constexpr (f >= C * H) {  // maxima of the products
+#pragma unroll
+                        for (int n = (f - C * H) * N / V; n < (f + 1 - C * H) * N / V; n++) {
+                            const int t = n / E, e = n % E;
+                            next_top[t] = e ? fmaxf(next_top[t], s2[t][e / 4][e % 4]) : s2[t][0][0];
+                        }
+                    }
+                });
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    top[t] = next_top[t], w[t] = w2[t];
+#pragma unroll
+                    for (int h = 0; h < H; h++) s[t][h] = s2[t][h];
+                    for (int h = 0; h < H; h++) asm volatile("" : "+v"(s[t][h]));
+                    asm volatile("" : "+v"(w[t]), "+v"(l[t]), "+v"(top[t]));  // (all of it here, not behind the branch)
+                }
+                if (raised) shrink_sums();
+            }
+            continue;
+        }
+        // any other: one thing after the other
+        turn(i);
+        const int place = j.begin + i * TK;
+        if (i > 0 && i <= my_tiles) {
+            const uint8_t* vf = values_at(i - 1);
+            // values that are no numbers, behind the end or where some row does not look, would make all rows such
+            bool special = false;
+#pragma unroll 1
+            for (int b = 0; b < V; b++) {
+                u32x4 v = *(const u32x4*)(vf + b * 1024), where;
+                special |= take_specials<DT>(v, where);
+            }
+            if (__any(special)) {
+                const int live = j.end - (place - TK + g * E);  // no row sees what lies behind
+#pragma unroll 1
+                for (int b = 0; b < V; b++) {
+                    u32x4 v = first_places<DT>(*(const u32x4*)(vf + b * 1024), live), where;
+                    take_specials<DT>(v, where);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        const v4f seen = step<DT>(where, w[t], v4f{0, 0, 0, 0});
+#pragma unroll
+                        for (int e = 0; e < 4; e++) nan[t] |= (decltype(nan[t] + 0))(seen[e] > 0.0f) << (4 * b + e);
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < V; b++) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    u32x4 v = first_places<DT>(*(const u32x4*)(vf + b * 1024), live), where;
+                    take_specials<DT>(v, where);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][b] = step<DT>(v, w[t], o[t][b]);
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < V; b++) {
+                    const u32x4 v = *(const u32x4*)(vf + b * 1024);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][b] = step<DT>(v, w[t], o[t][b]);
+                }
+            }
+        }
+        if (i < my_tiles) {
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int e = 0; e < E; e++) s[t][e / 4][e % 4] = place + g * E + e < limit[t] ? s[t][e / 4][e % 4] : -__builtin_inff();
+            maxima();
+            if (over()) {
+                raise();
+                if (i) shrink_sums();
+            }
+            auto base_of = [&](int t) { return m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2; };
+            if (large) {
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) s[t][e / 4][e % 4] = s[t][e / 4][e % 4] * p.scale2 + base_of(t);
+            }
+            weights(large ? 1.0f : p.scale2, [&](int t) { return large ? 0.0f : base_of(t); }, w);
+            products(keys_at(i + 1), s);
+        }
+        i++;
+    }
+    // (no load may reach LDS that is used for something else by then)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // Some of the wave's rows at a time through its quarter of LDS: whole lines to memory, and a loop where the registers would take a program
+    // longer than all the rest, which every workgroup runs once, from memory (1.2 us a KiB: it took 60 us).
+    constexpr int LD = 32 * B, TS = std::min(RT, (int)(sizeof(lds) / 4 / (16 * LD * 4)));
+    float* mine_lds = (float*)lds + wave * (int)(sizeof(lds) / 16);
+#pragma unroll
+    for (int t0 = 0; t0 < RT; t0 += TS) {
+        if (mine + t0 * 16 >= j.rows) break;
+        float sum[TS], most[TS];
+#pragma unroll
+        for (int t = 0; t < TS; t++) {
+            sum[t] = bad ? __builtin_nanf("") : over_groups_sum(l[t0 + t]);
+            most[t] = m[t0 + t] == -__builtin_inff() ? m[t0 + t] : m[t0 + t] * p.scale2;
+            // (columns of four are turned by the row, so that 16 rows are in 16 places)
+#pragma unroll
+            for (int b = 0; b < V; b++) *(v4f*)&mine_lds[(t * 16 + r) * LD + ((b * 4 + g) ^ (r & 7)) * 4] = o[t0 + t][b];
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int i = lane; i < TS * 16 * 8 * B; i += 64) {
+            const int row = i / (8 * B), f = i % (8 * B) * 4, from = row % 16;
+            v4f acc = *(const v4f*)&mine_lds[row * LD + ((f / 4) ^ (row & 7)) * 4];
+            auto bits = __shfl(nan[t0], from + f % 16 / 4 * 16);
+            float row_sum = __shfl(sum[0], from), row_most = __shfl(most[0], from);
+#pragma unroll
+            for (int t = 1; t < TS; t++) {
+                const auto b1 = __shfl(nan[t0 + t], from + f % 16 / 4 * 16);
+                const float s1 = __shfl(sum[t], from), m1 = __shfl(most[t], from);
+                if (row >= t * 16) bits = b1, row_sum = s1, row_most = m1;
+            }
+            bits >>= f / 16 * 4;
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] = bits >> e & 1 ? __builtin_nanf("") : acc[e];
+            const int at = mine + t0 * 16 + row;
+            if (at < j.rows && f < p.dim) put_row<DT>(p, j, at, f, acc, row_most, row_sum);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -615,8 +797,8 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void attend_join_kernel(Atten
     bool there, bad = false;
     const float2 *pml = nullptr, *ml = nullptr;
     const float *po = nullptr, *o = nullptr;
-    int s = -1, n = 0, length = 0;
-    int64_t token = 0, t0 = 0;
+    int s = -1, n = 0, length = 0, t0 = 0;
+    int64_t token = 0;
     if (p.join_few) {
         const int64_t of = row / p.few_slots, r = row % p.few_slots;
         there = of < (int64_t)p.n_seq * p.kv_heads;
@@ -628,7 +810,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void attend_join_kernel(Atten
             row = token * p.heads + of % p.kv_heads * p.group + r % p.group;
         }
     } else {
-        there = row < p.tokens * p.heads;
+        there = row < (int64_t)p.tokens * p.heads;
         if (there) {
             token = row / p.heads;
             s = p.starts ? owner_of(p.starts, p.n_seq, token) : (int)token;
@@ -674,9 +856,8 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void attend_join_kernel(Atten
     __syncthreads();
     if (first != 0 || !there) return;
     for (int i = 1; i < step; i++) acc += *(const v4f*)&sums[(threadIdx.x + i * lanes) * 4];
-    for (int i = 0; i < 4; i++)
-        if (f + i < p.dim) store_elem<DT>(p.out, row * p.dim + f + i, acc[i] * inverse);
-    if (in_row == 0 && p.lse) p.lse[row] = sum == 0.0f ? -__builtin_inff() : top * 0.69314718055994530942f + __logf(sum);
+    put_features<DT>(p, row, f, acc * inverse);
+    if (in_row == 0 && p.lse) p.lse[row] = lse_of(top, sum);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -690,17 +871,19 @@ struct AttendPlan {
     bool few, wide, prefix_wide;              // kernels that have work
     bool few_parts, wide_parts, join_few;
     Region few_region, wide_region, prefix_region;
+    size_t q_copy;  // byte offset
     size_t bytes;
 };
 constexpr int64_t FEW_ROWS = 32;
-static int64_t wide_tile(int64_t dim) { return dim <= 128 ? 128 : 64; }
+static int64_t wide_tile(int64_t dim) { return dim <= 128 ? WideTile<4>::R : WideTile<8>::R; }
 static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // Chunks of `places` for `tiles` of rows, so that there are `want` workgroups
 static int64_t chunk_of(int64_t places, int64_t tiles, int64_t want, int64_t least, int64_t most) {
     const int64_t n = std::max<int64_t>(1, want / std::max<int64_t>(1, tiles));
     return std::max(least, std::min(most, round_up(ceil_div(std::max<int64_t>(places, 1), n), 128)));
 }
-static AttendPlan attend_plan(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, bool starts, int64_t sequences, int64_t prefix) {
+static AttendPlan attend_plan(int dt, bool q_in_place, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, bool starts, int64_t sequences,
+                              int64_t prefix) {
     AttendPlan a = {};
     const int64_t group = heads / kv_heads, most_rows = starts ? tokens * group : group;
     a.few = starts || group <= FEW_ROWS;
@@ -730,6 +913,8 @@ static AttendPlan attend_plan(int64_t tokens, int64_t heads, int64_t kv_heads, i
     a.few_region = region(a.few_parts, sequences * kv_heads * a.few_slots, a.chunks);
     a.wide_region = region(a.wide_parts, tokens * heads, a.wide_chunks);
     a.prefix_region = region(prefix > 0, tokens * heads, a.prefix_chunks);
+    a.q_copy = a.bytes;
+    if (!q_in_place) a.bytes += (size_t)round_up(tokens * heads * cache_head_dim(dt, dim) * dtype_size(dt), 256);
     return a;
 }
 
@@ -739,7 +924,11 @@ static void launch_attend_cfg(const AttendParams& p, int64_t few_blocks, int64_t
     if (few_blocks) hipLaunchKernelGGL((attend_rows_kernel<DT, B>), dim3((unsigned)few_blocks), dim3(256), 0, st, p);
 }
 template <int DT>
-static void launch_attend(const AttendParams& p, int64_t few_blocks, int64_t wide_blocks, int64_t join_rows, hipStream_t st) {
+static void launch_attend(AttendParams& p, void* q_copy, int64_t few_blocks, int64_t wide_blocks, int64_t join_rows, hipStream_t st) {
+    if (q_copy) {
+        hipLaunchKernelGGL((attend_copy_kernel<DT>), dim3((unsigned)std::min<int64_t>(ceil_div((int64_t)p.tokens * p.heads * p.dp, 1024), 4096)), dim3(256), 0, st, p, q_copy);
+        p.q = q_copy, p.q_head = p.q_dim = p.dp, p.q_token = (int64_t)p.heads * p.dp;
+    }
     switch (ceil_div(p.dim, 32)) {
         case 1: launch_attend_cfg<DT, 1>(p, few_blocks, wide_blocks, st); break;
         case 2: launch_attend_cfg<DT, 2>(p, few_blocks, wide_blocks, st); break;
@@ -757,9 +946,9 @@ static void launch_attend(const AttendParams& p, int64_t few_blocks, int64_t wid
     else hipLaunchKernelGGL((attend_join_kernel<DT, 16>), dim3((unsigned)join_rows), dim3(1024), 0, st, p);
 }
 
-static bool shape_ok(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page, int64_t width, int64_t longest, bool starts, int64_t sequences,
+static bool shape_ok(int dt, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page, int64_t width, int64_t longest, bool starts, int64_t sequences,
                      int64_t prefix) {
-    return tokens > 0 && tokens <= 0x7fffffff && kv_heads > 0 && heads > 0 && heads <= 16384 && heads % kv_heads == 0 && dim > 0 && dim <= 256 && page >= 32 &&
+    return dt >= BT_F32 && dt <= BT_BF16 && tokens > 0 && tokens <= 0x7fffffff && kv_heads > 0 && heads > 0 && heads <= 16384 && tokens * heads <= 0x7fffffff && heads % kv_heads == 0 && dim > 0 && dim <= 256 && page >= 32 &&
            page <= 65536 && (page & (page - 1)) == 0 && width > 0 && width * page <= 0x7fffff00 && longest >= 0 && longest <= width * page && sequences > 0 &&
            sequences <= (1 << 24) && (starts || sequences == tokens) && prefix >= 0 && prefix <= 0x7fffff00;
 }
@@ -768,10 +957,10 @@ static bool shape_ok(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t di
 
 using namespace bt;
 
-extern "C" size_t bt_cached_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t table_width,
+extern "C" size_t bt_cached_attention_workspace_bytes(int dtype, int q_in_place, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t table_width,
                                                       int64_t max_length, int has_starts, int64_t sequences, int64_t prefix_length) {
-    if (!shape_ok(tokens, heads, kv_heads, head_dim, page_size, table_width, max_length, has_starts != 0, sequences, prefix_length)) return 0;
-    return attend_plan(tokens, heads, kv_heads, head_dim, max_length, has_starts != 0, sequences, prefix_length).bytes;
+    if (!shape_ok(dtype, tokens, heads, kv_heads, head_dim, page_size, table_width, max_length, has_starts != 0, sequences, prefix_length)) return 0;
+    return attend_plan(dtype, q_in_place != 0, tokens, heads, kv_heads, head_dim, max_length, has_starts != 0, sequences, prefix_length).bytes;
 }
 
 extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const void* k_cache, const void* v_cache, int64_t pages,
@@ -783,7 +972,7 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
         set_error("%s: null pointer or bad dtype", who);
         return BT_ERR_INVALID;
     }
-    if (!shape_ok(tokens, heads, kv_heads, head_dim, page_size, table_width, max_length, q_starts != nullptr, sequences, prefix_length) || pages <= 0 ||
+    if (!shape_ok(dtype, tokens, heads, kv_heads, head_dim, page_size, table_width, max_length, q_starts != nullptr, sequences, prefix_length) || pages <= 0 ||
         pages > 0x7fffffff) {
         set_error("%s: head_dim at most 256, heads a multiple of kv_heads, page_size a power of two from 32 on, places of a sequence below 2^31, one token a "
                   "sequence without q_starts (head_dim=%lld heads=%lld/%lld page_size=%lld width=%lld sequences=%lld tokens=%lld)",
@@ -799,25 +988,25 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
         set_error("%s: the cache has to be 16-byte aligned", who);
         return BT_ERR_INVALID;
     }
-    const AttendPlan a = attend_plan(tokens, heads, kv_heads, head_dim, max_length, q_starts != nullptr, sequences, prefix_length);
+    const int e = 16 / dtype_size(dtype);
+    const bool in_place = head_dim % e == 0 && q_token % e == 0 && q_head % e == 0 && ((uintptr_t)q) % 16 == 0;
+    const AttendPlan a = attend_plan(dtype, in_place, tokens, heads, kv_heads, head_dim, max_length, q_starts != nullptr, sequences, prefix_length);
     if (a.bytes && (!workspace || workspace_bytes < a.bytes || ((uintptr_t)workspace) % 256 != 0)) {
         set_error("%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who, a.bytes, workspace_bytes);
         return BT_ERR_WORKSPACE;
     }
     AttendParams p = {};
     p.q = q, p.k_cache = k_cache, p.v_cache = v_cache, p.table = block_table, p.lengths = lengths, p.starts = q_starts, p.prefix_table = prefix_table;
-    p.q_token = q_token, p.q_head = q_head, p.tokens = tokens, p.out = out, p.lse = lse;
+    p.q_token = q_token, p.q_head = q_head, p.tokens = (int)tokens, p.out = out, p.lse = lse;
     auto parts = [&](const Region& r) { return r.rows ? Parts{(float*)((char*)workspace + r.o), (float2*)((char*)workspace + r.ml)} : Parts{nullptr, nullptr}; };
     p.few_parts = parts(a.few_region), p.wide_parts = parts(a.wide_region), p.prefix_parts = parts(a.prefix_region);
-    p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads), p.dim = (int)head_dim, p.dp = cache_head_dim(dtype, head_dim);
+    p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads), p.dim = p.q_dim = (int)head_dim, p.dp = cache_head_dim(dtype, head_dim);
     p.n_seq = (int)sequences, p.width = (int)table_width, p.page_shift = __builtin_ctzll((unsigned long long)page_size), p.pages = (int)pages;
     p.prefix = (int)prefix_length;
     p.longest = (int)max_length, p.few_rows = (int)FEW_ROWS, p.few_slots = (int)a.few_slots, p.join_few = a.join_few;
     p.chunk = (int)a.chunk, p.chunks = (int)a.chunks, p.tiles = (int)a.tiles;
     p.wide_chunk = (int)a.wide_chunk, p.wide_chunks = (int)a.wide_chunks, p.wide_tiles = (int)a.wide_tiles;
     p.prefix_chunk = (int)a.prefix_chunk, p.prefix_chunks = (int)a.prefix_chunks, p.prefix_tiles = (int)a.prefix_tiles, p.prefix_wide = a.prefix_wide;
-    const int e = 16 / dtype_size(dtype);
-    p.wide_q = head_dim % e == 0 && q_token % e == 0 && q_head % e == 0 && ((uintptr_t)q) % 16 == 0;
     p.scale2 = (float)((double)scale * 1.4426950408889634074);
     const int64_t prefix_blocks = a.prefix_tiles * a.prefix_chunks * kv_heads;
     const bool clear = q_starts && (a.join_few || (!a.few_parts && !a.wide_parts));  // (attend_join_kernel sees to the rows behind otherwise)
@@ -829,8 +1018,8 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
         return BT_ERR_INVALID;
     }
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == BT_F32) launch_attend<BT_F32>(p, few_blocks, wide_blocks, join_rows, st);
-    else if (dtype == BT_F16) launch_attend<BT_F16>(p, few_blocks, wide_blocks, join_rows, st);
-    else launch_attend<BT_BF16>(p, few_blocks, wide_blocks, join_rows, st);
+    if (dtype == BT_F32) launch_attend<BT_F32>(p, in_place ? nullptr : (char*)workspace + a.q_copy, few_blocks, wide_blocks, join_rows, st);
+    else if (dtype == BT_F16) launch_attend<BT_F16>(p, in_place ? nullptr : (char*)workspace + a.q_copy, few_blocks, wide_blocks, join_rows, st);
+    else launch_attend<BT_BF16>(p, in_place ? nullptr : (char*)workspace + a.q_copy, few_blocks, wide_blocks, join_rows, st);
     return check_launch(who);
 }

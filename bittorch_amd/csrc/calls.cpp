@@ -1054,7 +1054,9 @@ PyObject* cached_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t T = qr.tokens;
     at::Tensor out = output(q->sizes(), q->scalar_type(), *q), lse;
     if (want_lse) lse = output({T, qr.heads}, at::kFloat, *q);
-    const Scratch ws(lib.bt_cached_attention_workspace_bytes(T, qr.heads, c.kv_heads, qr.dim, c.page, c.width, longest, c.starts ? 1 : 0, c.sequences, prefix), *q);
+    const int64_t per = 16 / (int64_t)q->element_size();
+    const int in_place = qr.dim % per == 0 && qr.token % per == 0 && qr.head % per == 0 && aligned(*q, 16) ? 1 : 0;
+    const Scratch ws(lib.bt_cached_attention_workspace_bytes(tag(q->scalar_type()), in_place, T, qr.heads, c.kv_heads, qr.dim, c.page, c.width, longest, c.starts ? 1 : 0, c.sequences, prefix), *q);
     void* st = stream_of(device);
     call(lib.bt_cached_attention, qr.data, qr.token, qr.head, tag(q->scalar_type()), c.k->const_data_ptr(), c.v->const_data_ptr(), c.pages, c.page,
          (const int32_t*)c.table->const_data_ptr(), c.width, longest, (const int32_t*)c.lengths->const_data_ptr(),

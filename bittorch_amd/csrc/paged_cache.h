@@ -5,6 +5,7 @@
 // matrix cores, so that every load of the attention is 1 KiB in a row, straight into registers or LDS, and no value is moved again:
 //   keys    [Dp / 4E][E / 4][g 4][m 16][E features]:  feature = 4E c + E g + e,  place = E (m / 4) + 4 t + m % 4
 //   values  [Dp / 16][g 4][m 16][E places]:           feature = 16 b + m,        place = E g + e
+// Features of a key behind D are zero, whatever the array held before.
 // The scores of keys in that order leave the matrix cores with lane (m, g) holding places E g .. E g + E - 1 of row m, which is the operand
 // that the second product takes beside the values.
 #pragma once

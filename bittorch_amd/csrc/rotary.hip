@@ -267,8 +267,8 @@ template <int DT>
 static void launch_cache_append(TurnParams& p, hipStream_t st) {
     constexpr int E = CacheOrder<DT>::E;
     const bool vec = whole_pieces(p, E);
-    const int pv = vec ? E : 1, pad = (int)ceil_div(p.dim, E) * E;
-    p.per_head = divider((uint32_t)(p.rot / 2 / pv + (pad - p.rot) / pv));
+    const int pv = vec ? E : 1;
+    p.per_head = divider((uint32_t)(p.rot / 2 / pv + (p.dp - p.rot) / pv));  // (keys are written to the end of their pad)
     p.slots = divider((uint32_t)(p.hk + (p.q ? p.hq : 0)));
     p.by_dim = divider((uint32_t)p.dim);
     p.units = (int)(p.starts ? p.tokens / E + 2 * (int64_t)p.n_seq : p.n_seq);

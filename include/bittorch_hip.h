@@ -557,6 +557,7 @@ int bt_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int
  * page holds tiles of 4 E places in the order of the matrix cores' operands (place and feature within the tile):
  *   keys    [feature / 4E][place % E / 4][feature % 4E / E][place / E][place % 4][feature % E]
  *   values  [feature / 16][place / E][feature % 16][place % E]
+ * features of the keys behind head_dim are zero (bt_cache_append writes them too).
  * Sequence s owns the pages block_table[s][0 .. table_width) (int32) and lengths[s] places in them, its new tokens included, which are the
  * last; they are the rows q_starts[s] .. q_starts[s + 1] - 1 of k, v and q.  q_starts (sequences + 1 entries, from 0, ascending) NULL: one
  * token a sequence.  Entries of the table behind the places in use are not read.
@@ -568,7 +569,8 @@ int bt_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int
  *     [tokens][heads]: the logarithm of the sum of exponentials.  No places at all, and rows behind the last sequence: zeros, and -inf.  The rows of
  *     sequences with more than max_length (<= table_width * page_size) places, and rows that see a page outside the cache (others of the
  *     sequence may be), are not a number.
- *     Places that a row does not see do not change it, whatever they hold.  workspace: bt_cached_attention_workspace_bytes.
+ *     Places that a row does not see do not change it, whatever they hold.  workspace: bt_cached_attention_workspace_bytes, where q_in_place
+ *     says that q, its strides and its heads start and end on 16 bytes (its rows are copied otherwise).
  */
 int bt_cache_head_dim(int dtype, int64_t head_dim);
 int bt_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* q, int64_t q_token,
@@ -576,7 +578,7 @@ int bt_cache_append(const void* k, int64_t k_token, int64_t k_head, const void* 
                     int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, void* k_cache, void* v_cache, int64_t pages,
                     int64_t page_size, const int32_t* block_table, int64_t table_width, const int32_t* lengths, const int32_t* q_starts,
                     int64_t sequences, void* q_out, void* stream);
-size_t bt_cached_attention_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t table_width,
+size_t bt_cached_attention_workspace_bytes(int dtype, int q_in_place, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t table_width,
                                            int64_t max_length, int has_starts, int64_t sequences, int64_t prefix_length);
 int bt_cached_attention(const void* q, int64_t q_token, int64_t q_head, int dtype, const void* k_cache, const void* v_cache, int64_t pages, int64_t page_size,
                         const int32_t* block_table, int64_t table_width, int64_t max_length, const int32_t* lengths, const int32_t* q_starts,

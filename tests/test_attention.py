@@ -199,9 +199,9 @@ def test_library_refuses_without_a_gpu():
     for bad in (dict(page=33), dict(width=0), dict(longest=33), dict(n_seq=2), dict(dim=300), dict(heads=3, kv=2), dict(scale=0.0), dict(scale=math.nan), dict(cache=at + 8),
                 dict(prefix=4)):
         assert attend(**bad) == -1 and "bt_cached_attention" in _lib.last_error(), bad
-    need = lib.bt_cached_attention_workspace_bytes(1, 2, 1, 8, 32, 1024, 32768, 0, 1, 0)
+    need = lib.bt_cached_attention_workspace_bytes(0, 1, 1, 2, 1, 8, 32, 1024, 32768, 0, 1, 0)
     assert need > 0 and attend(width=1024, longest=32768) == -2 and attend(width=1024, longest=32768, ws=256, size=need - 1) == -2
-    assert lib.bt_cached_attention_workspace_bytes(0, 2, 1, 8, 32, 1024, 32768, 0, 1, 0) == 0
+    assert lib.bt_cached_attention_workspace_bytes(0, 1, 0, 2, 1, 8, 32, 1024, 32768, 0, 1, 0) == 0
     assert [lib.bt_cache_head_dim(d, n) for d, n in ((0, 1), (0, 80), (1, 80), (2, 128), (2, 257), (3, 8), (0, 0))] == [16, 80, 96, 128, 0, 0, 0]
 
 
