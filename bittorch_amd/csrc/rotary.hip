@@ -12,6 +12,7 @@ namespace bt {
 
 constexpr int TURN_ANGLES = 1024;  // of a workgroup: tokens x pairs
 constexpr int TURN_THREADS = 256;
+constexpr int64_t APPEND_BLOCKS = 2048;
 
 struct TurnParams {
     const void *q, *k, *v;
@@ -133,9 +134,9 @@ __global__ __launch_bounds__(TURN_THREADS) void rotary_kernel(TurnParams p) {
 }
 
 // The new tokens of one sequence whose places share a 16-byte group of the values (E places): their keys and queries are turned, their
-// values transposed by the way they are read (a lane owns a feature, the group's tokens are its registers).  grid (units, shares of a
+// values transposed by the way they are read (a lane owns FV features, the group's tokens are its registers).  grid (units, shares of a
 // unit's pieces); units beyond p.units clear the queries behind the last sequence.
-template <int DT, int PV>
+template <int DT, int PV, int FV>
 __global__ __launch_bounds__(TURN_THREADS) void cache_append_kernel(TurnParams p) {
     using Order = CacheOrder<DT>;
     constexpr int E = Order::E;
@@ -185,16 +186,27 @@ __global__ __launch_bounds__(TURN_THREADS) void cache_append_kernel(TurnParams p
     const int inside = (int)(aligned * E & ((1 << p.page_shift) - 1));  // of the page
     const int64_t page_elements = (int64_t)p.dp << p.page_shift;
 
+    // Pieces of a whole group: four tokens side by side, whose 16 bytes are neighbours in the keys' order, then the pieces, then the other four
+    // (16 bytes a store each on a line of their own took the prompts of 8 x 512 tokens 41 us)
+    const bool whole = count == E;
     const uint32_t turned = (uint32_t)count * p.slots.d * p.per_head.d;                 // slots: the keys' heads, then the queries'
-    const uint32_t items = turned + (uint32_t)p.hk * p.dim;
+    const uint32_t items = turned + (uint32_t)p.hk * p.by_dim.d;
     for (uint32_t idx = blockIdx.y * TURN_THREADS + threadIdx.x; idx < items; idx += gridDim.y * TURN_THREADS) {
         if (idx < turned) {
-            const uint32_t row = divide(idx, p.per_head), i = divide(row, p.slots);
-            const int piece = (int)(idx - row * p.per_head.d), slot = (int)(row - i * p.slots.d);
+            int i, piece, slot;
+            if (whole) {
+                const uint32_t rest = idx / 4, row = divide(rest, p.per_head);
+                piece = (int)(rest - row * p.per_head.d);
+                slot = (int)(row / (E / 4));
+                i = (int)(idx % 4 + row % (E / 4) * 4);
+            } else {
+                const uint32_t row = divide(idx, p.per_head), at = divide(row, p.slots);
+                piece = (int)(idx - row * p.per_head.d), slot = (int)(row - at * p.slots.d), i = (int)at;
+            }
             const int64_t t = first + i;
             if (slot < p.hk) {
                 if (page < 0) continue;
-                const int place = inside + (int)(low - aligned * E) + (int)i;
+                const int place = inside + (int)(low - aligned * E) + i;
                 const int64_t base = (page * p.hk + slot) * page_elements;
                 turn_piece<DT, PV>(p, turn + i * (p.rot / 2), p.k, t * p.k_token + slot * p.k_head, piece, [&](int f, const float (&v)[PV]) {
                     store_piece<DT, PV>(p.k_cache, base + Order::key(place, f, p.dp), v);
@@ -209,17 +221,34 @@ __global__ __launch_bounds__(TURN_THREADS) void cache_append_kernel(TurnParams p
         }
         if (page < 0) continue;
         const uint32_t head = divide(idx - turned, p.by_dim);
-        const int f = (int)(idx - turned - head * p.by_dim.d);
+        const int f = (int)(idx - turned - head * p.by_dim.d) * FV;
         const int64_t from = first * p.v_token + head * p.v_head + f;
         const int64_t to = (page * p.hk + head) * page_elements + Order::value(inside, f, p.dp);
-        if (count == E) {
+        if (FV == 2 && whole) {  // two features a lane: 4 bytes of each token, 16 of each feature
+            u32x4 even, odd;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t a = *(const uint32_t*)((const uint16_t*)p.v + from + 2 * i * p.v_token), b = *(const uint32_t*)((const uint16_t*)p.v + from + (2 * i + 1) * p.v_token);
+                even[i] = (a & 0xffffu) | b << 16, odd[i] = a >> 16 | (b & 0xffff0000u);
+            }
+            *(u32x4*)((uint16_t*)p.v_cache + to) = even;
+            *(u32x4*)((uint16_t*)p.v_cache + to + E) = odd;
+        } else if (FV == 1 && whole) {
             float v[E];
 #pragma unroll
             for (int i = 0; i < E; i++) v[i] = load_elem<DT>(p.v, from + i * p.v_token);
             store_piece<DT, E>(p.v_cache, to, v);
         } else {
             const int skip = (int)(low - aligned * E);
-            for (int i = 0; i < count; i++) store_elem<DT>(p.v_cache, to + skip + i, load_elem<DT>(p.v, from + i * p.v_token));
+#pragma unroll
+            for (int e = 0; e < FV; e++) {
+                float v[E];  // (all on their way before the first is stored)
+#pragma unroll
+                for (int i = 0; i < E; i++) v[i] = i < count ? load_elem<DT>(p.v, from + e + i * p.v_token) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < E; i++)
+                    if (i < count) store_elem<DT>(p.v_cache, to + e * E + skip + i, v[i]);
+            }
         }
     }
 }
@@ -270,13 +299,16 @@ static void launch_cache_append(TurnParams& p, hipStream_t st) {
     const int pv = vec ? E : 1;
     p.per_head = divider((uint32_t)(p.rot / 2 / pv + (p.dp - p.rot) / pv));  // (keys are written to the end of their pad)
     p.slots = divider((uint32_t)(p.hk + (p.q ? p.hq : 0)));
-    p.by_dim = divider((uint32_t)p.dim);
+    // two features of 16 bits a lane where they are 4 bytes together
+    const bool two = vec && DT != BT_F32 && (p.v_token | p.v_head) % 2 == 0 && !misaligned(p.v, 4);
+    p.by_dim = divider((uint32_t)(two ? p.dim / 2 : p.dim));
     p.units = (int)(p.starts ? p.tokens / E + 2 * (int64_t)p.n_seq : p.n_seq);
-    const int64_t per_unit = (p.starts ? std::min<int64_t>(E, ceil_div(p.tokens, p.n_seq)) : 1) * (int64_t)p.slots.d * p.per_head.d + (int64_t)p.hk * p.dim;
-    const int64_t shares = std::min<int64_t>(ceil_div(per_unit, TURN_THREADS), std::max<int64_t>(1, 2048 / p.units));
+    const int64_t per_unit = (p.starts ? std::min<int64_t>(E, ceil_div(p.tokens, p.n_seq)) : 1) * (int64_t)p.slots.d * p.per_head.d + (int64_t)p.hk * p.by_dim.d;
+    const int64_t shares = std::min<int64_t>(ceil_div(per_unit, TURN_THREADS), std::max<int64_t>(1, APPEND_BLOCKS / p.units));
     const dim3 grid((unsigned)(p.units + (p.starts ? 1 : 0)), (unsigned)std::min<int64_t>(shares, 65535));
-    if (vec) hipLaunchKernelGGL((cache_append_kernel<DT, E>), grid, dim3(TURN_THREADS), 0, st, p);
-    else hipLaunchKernelGGL((cache_append_kernel<DT, 1>), grid, dim3(TURN_THREADS), 0, st, p);
+    if (two) hipLaunchKernelGGL((cache_append_kernel<DT, E, DT == BT_F32 ? 1 : 2>), grid, dim3(TURN_THREADS), 0, st, p);
+    else if (vec) hipLaunchKernelGGL((cache_append_kernel<DT, E, 1>), grid, dim3(TURN_THREADS), 0, st, p);
+    else hipLaunchKernelGGL((cache_append_kernel<DT, 1, 1>), grid, dim3(TURN_THREADS), 0, st, p);
 }
 
 }  // namespace bt
