@@ -3,7 +3,8 @@
 Not a model zoo entry: the workload the benchmark times and the GPU tests compare, in every variant of the ternary
 path (training modules, converted inference modules, inference modules with the block glue fused, the int8 path).
 Block structure of the reference's JS runtime (js/src/models/TernaryTransformer.ts:366-423, :489-521): pre-norm,
-causal attention, SwiGLU MLP; attention, norms and the embedding stay in PyTorch.
+causal attention, SwiGLU MLP; attention, norms and the embedding stay in PyTorch, except where the stack decodes with a cache
+(``start_cache``, ``forward_cached``): there the attention half of a block is this package's too.
 """
 
 from __future__ import annotations
@@ -19,12 +20,13 @@ class BlockStack:
     modules, inference modules with the glue fused, and the int8 path."""
 
     def __init__(self, dev, layers=30, d_model=2560, heads=20, ffn=6912, batch=8, seq=512, vocab=32000,
-                 backend="auto", act_dtype=None, fake_quant=False, attn_scale=None, master_std=0.02):
+                 backend="auto", act_dtype=None, fake_quant=False, attn_scale=None, master_std=0.02, rotary_dim=0):
         """``attn_scale``: the softmax scale of the attention (default 1/sqrt(head_dim)).  ``master_std``: standard
         deviation of the random master weights, one number or a dict by projection name (``q k v o gate up down``;
         missing names take 0.02).  With the defaults (N(0, 0.02) masters everywhere) the attention logits of a block
         have a standard deviation near 15 and the MLP branch is some 70 times the residual stream; a test that wants
-        every branch of order one, so that element-wise bounds bite, passes smaller values."""
+        every branch of order one, so that element-wise bounds bite, passes smaller values.  ``rotary_dim``: features of a head that
+        ``ops.rotary`` turns by the token's position, in every variant (0: no positions)."""
         import torch.nn as nn
         import torch.nn.functional as F
         import bittorch_amd as bt
@@ -36,6 +38,9 @@ class BlockStack:
         self.d_model, self.heads, self.ffn = d_model, heads, ffn
         act_dtype = act_dtype or torch.bfloat16
         self.act_dtype = act_dtype
+        self.inv_freq = bt.ops.rotary_frequencies(rotary_dim, device=dev)[0] if rotary_dim else None
+        self.cache = None
+        turned = self._turned
 
         def fq(t):
             """fake_quant: the int8 path's per-token activation quantizer (whole-row absmax / 127, halves away
@@ -60,8 +65,7 @@ class BlockStack:
             def forward(self, x):
                 b, t, _ = x.shape
                 h = fq(self.n1(x))
-                q = self.q(h).view(b, t, heads, -1).transpose(1, 2)
-                k = self.k(h).view(b, t, heads, -1).transpose(1, 2)
+                q, k = (z.transpose(1, 2) for z in turned(self.q(h).view(b, t, heads, -1), self.k(h).view(b, t, heads, -1)))
                 v = self.v(h).view(b, t, heads, -1).transpose(1, 2)
                 a = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=attn_scale).transpose(1, 2).reshape(b, t, -1)
                 x = x + self.o(fq(a))
@@ -83,6 +87,12 @@ class BlockStack:
         self.n_tern = sum(m.weight.numel() for m in self.blocks.modules() if isinstance(m, bt.nn.TernaryLinear))
         self.infer = None
 
+    def _turned(self, q, k):
+        """Queries and keys (batch, seq, heads, head_dim) by their places in the sequence."""
+        if self.inv_freq is None:
+            return q, k
+        return self.bt.ops.rotary(q, k, self.torch.arange(q.shape[1], device=q.device), self.inv_freq)
+
     def forward(self, stack=None):
         """Unfused forward of `stack` (the training modules by default, or the converted modules)."""
         torch = self.torch
@@ -94,14 +104,15 @@ class BlockStack:
 
     def forward_train(self):
         """The training modules with the glue between their layers fused, differentiable: the residual connections with the norms behind
-        them (``ops.add_rmsnorm``), gate and up with the SwiGLU between them (``ops.ternary_gated_linear``)."""
+        them (``ops.add_rmsnorm``), gate and up with the SwiGLU between them (``ops.ternary_gated_linear``), positions (``ops.rotary``)."""
         F, ops = self.F, self.bt.ops
         eps_of = lambda norm: self.torch.finfo(self.act_dtype).eps if norm.eps is None else norm.eps
         x, branch = self.emb(self.tokens), None
         for blk in self.blocks:
             x, h = ops.add_rmsnorm(x, None, blk.n1.weight, eps_of(blk.n1)) if branch is None else ops.add_rmsnorm(branch, x, blk.n1.weight, eps_of(blk.n1))
             b, t, _ = h.shape
-            q, k, v = (m(h).view(b, t, self.heads, -1).transpose(1, 2) for m in (blk.q, blk.k, blk.v))
+            q, k, v = (m(h).view(b, t, self.heads, -1) for m in (blk.q, blk.k, blk.v))
+            q, k, v = (z.transpose(1, 2) for z in (*self._turned(q, k), v))
             a = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=self.attn_scale).transpose(1, 2).reshape(b, t, -1)
             x, h = ops.add_rmsnorm(blk.o(a), x, blk.n2.weight, eps_of(blk.n2))
             branch = blk.down(ops.ternary_gated_linear(h, blk.gate.weight, blk.up.weight))
@@ -126,12 +137,13 @@ class BlockStack:
             blk.qkv = bt.utils.fuse_ternary_linear_inference(blk.q, blk.k, blk.v)
             blk.mlp = bt.nn.TernarySwiGLU(blk.gate, blk.up, blk.down, compute="float", fuse_gate_up=True)
 
-    def _fused_block(self, blk, x, int8):
+    def _fused_block(self, blk, x, int8, attend=None):
+        """``attend``: the attention of q, k, v (tokens, heads, head_dim) -> (tokens, d_model), x then being (tokens, d_model); default: causal in
+        every sequence of x (batch, seq, d_model)."""
         torch, F, bt = self.torch, self.F, self.bt
         from bittorch_amd.ops import fused
         heads, d_model = self.heads, self.d_model
-        b, s, _ = x.shape
-        heads_of = lambda t: t.view(b, s, heads, -1).transpose(1, 2)
+        lead = x.shape[:-1]
         if int8:  # BitNet-style: every projection on the int8 matrix cores from activations that leave the
             # norm / SwiGLU kernels already quantized per token
             # (row sums of the quantized rows ride along where the layers hold a prefill copy: prepare_prefill)
@@ -141,12 +153,15 @@ class BlockStack:
             qkv = blk.qkv.forward_int8(qh, sh, x.dtype, None, True, rs[0] if rs else None)
         else:
             qkv = blk.qkv(fused.rmsnorm(x, blk.n1.weight, blk.n1.eps or torch.finfo(x.dtype).eps))
-        q, k, v = qkv.split(d_model, dim=-1)  # one GEMM over the concatenated q|k|v columns
-        a = F.scaled_dot_product_attention(heads_of(q), heads_of(k), heads_of(v), is_causal=True, scale=self.attn_scale)
-        a = a.transpose(1, 2).reshape(b, s, -1)
+        q, k, v = (t.view(*lead, heads, -1) for t in qkv.split(d_model, dim=-1))  # one GEMM over the concatenated q|k|v columns
+        if attend is None:
+            q, k, v = (t.transpose(1, 2) for t in (*self._turned(q, k), v))
+            a = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=self.attn_scale).transpose(1, 2).reshape(*lead, -1)
+        else:
+            a = attend(q, k, v)
         if int8:
-            qa, sa, *rs = bt._C.act_quant_int8(a.reshape(b * s, -1), True, self.prefill_copy)
-            x = blk.o.forward_int8(qa, sa, x.dtype, x.reshape(b * s, -1), True, rs[0] if rs else None).view(b, s, -1)
+            qa, sa, *rs = bt._C.act_quant_int8(a.reshape(-1, d_model), True, self.prefill_copy)
+            x = blk.o.forward_int8(qa, sa, x.dtype, x.reshape(-1, d_model), True, rs[0] if rs else None).view(*lead, -1)
         else:
             x = blk.o(a, x)
         return blk.mlp(x, blk.n2.weight, blk.n2.eps or torch.finfo(x.dtype).eps, residual=x)
@@ -174,4 +189,48 @@ class BlockStack:
                 x = self._fused_block(blk, x, int8)
             return self.final(x)
 
+    def start_cache(self, sequences, places, prefix=0, page_size=64):
+        """Empty caches of every layer for ``sequences`` sequences of up to ``places`` tokens, behind a prefix of up to ``prefix`` tokens that
+        all of them share."""
+        torch, ops = self.torch, self.bt.ops
+        width, shared = -(-places // page_size), -(-prefix // page_size)
+        dev = self.tokens.device
+        make = lambda: ops.paged_cache(sequences * width + shared, self.heads, self.d_model // self.heads, page_size, self.act_dtype, dev)  # noqa: E731
+        pages = torch.arange(sequences * width + shared, dtype=torch.int32, device=dev)
+        self.cache = dict(layers=[make() for _ in self.infer], prefix_table=pages[:shared], prefix_length=0,
+                          table=pages[shared:].view(sequences, width), lengths=torch.zeros(sequences, dtype=torch.int32, device=dev))
 
+    def _cached(self, tokens, table, lengths, q_starts, int8, first, **prefix):
+        torch, ops = self.torch, self.bt.ops
+        for blk in self.infer:
+            blk.mlp.compute = "int8" if int8 else "float"
+
+        def attention(layer):
+            def attend(q, k, v):
+                turned = ops.cache_append(k, v, *layer, table, lengths, q_starts, None if self.inv_freq is None else q, self.inv_freq, first_position=first)
+                return ops.cached_attention(q if turned is None else turned, *layer, table, lengths, q_starts, scale=self.attn_scale, **prefix).flatten(1)
+            return attend
+
+        with torch.no_grad():
+            x = self.emb(tokens)
+            for blk, layer in zip(self.infer, self.cache["layers"]):
+                x = self._fused_block(blk, x, int8, attention(layer))
+            return self.final(x)
+
+    def forward_prefix(self, tokens, int8=False):
+        """The tokens (1D) that all sequences share, once, at the start of the caches; their hidden states."""
+        c, n = self.cache, tokens.numel()
+        if c["prefix_length"] or n > c["prefix_table"].numel() * c["layers"][0][0].shape[2]:
+            raise RuntimeError("the prefix is there already, or longer than start_cache was told")
+        c["prefix_length"] = n
+        at = lambda *v: self.torch.tensor(v, dtype=self.torch.int32, device=tokens.device)  # noqa: E731
+        return self._cached(tokens, c["prefix_table"][None], at(n), at(0, n), int8, 0)
+
+    def forward_cached(self, tokens, q_starts=None, int8=False):
+        """The converted, fused stack on the sequences' next tokens (1D): one each, or ``q_starts[s] .. q_starts[s + 1] - 1`` of sequence s (int32);
+        hidden states (tokens, d_model).  The caches' lengths follow on the GPU, so that a step of one token each can be captured; more tokens than
+        ``start_cache`` was told are not stored, and their sequences are not a number from then on."""
+        c = self.cache
+        c["lengths"] += 1 if q_starts is None else q_starts[1:] - q_starts[:-1]
+        return self._cached(tokens, c["table"], c["lengths"], q_starts, int8, c["prefix_length"],
+                            prefix_table=c["prefix_table"] if c["prefix_length"] else None, prefix_length=c["prefix_length"])
