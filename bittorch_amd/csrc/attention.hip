@@ -480,6 +480,28 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
 // weight would pass 2^8: it needs to be near the true maximum, not to be it.  16-bit weights are rounded once (the rows kernel's two halves
 // would be half as many matrix instructions again): results are 1.4 times as far from 64 bits as by their own rounding.  Their sum is that of
 // the weights before they are rounded, as lse wants it.
+// The tile of the unit'th workgroup of a key head: sequences by their length, their last rows first, and of the first 2 x CUs workgroups, two of
+// which share a compute unit and its LDS, the second ones from the light end (4 x 512 tokens on 1600 to 4000 places 138 -> 120 us).
+__device__ __forceinline__ bool heaviest_first(const AttendParams& p, int R, uint32_t unit, int* s, int* tile) {
+    const int lane = threadIdx.x & 63;
+    int t0, n = 0, length = 0;
+    if (lane < p.n_seq) sequence_of(p, lane, &t0, &n, &length);
+    const int rows = n * p.group, mine = rows > p.few_rows ? (rows + R - 1) / R : 0;
+    int before = 0, total = 0;  // tiles of heavier sequences, and of all
+    for (int i = 0; i < p.n_seq; i++) {
+        const int tiles = __builtin_amdgcn_readlane(mine, i), its = __builtin_amdgcn_readlane(length, i);
+        if (its > length || (its == length && i < lane)) before += tiles;
+        total += tiles;
+    }
+    if ((int)unit >= total) return false;
+    const int first = std::max(1, 256 / p.kv_heads), at = (int)unit;
+    const int rank = at < first || total <= first ? at : at < 2 * first && at < total ? total - 1 - (at - first) : at - first;
+    const uint64_t hit = __ballot(before <= rank && rank < before + mine);
+    if (!hit) return false;
+    *s = __builtin_ctzll(hit);
+    *tile = __builtin_amdgcn_readlane(mine, *s) - 1 - (rank - __builtin_amdgcn_readlane(before, *s));
+    return true;
+}
 template <typename Body, int... I>
 __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, Body body) {  // body(0), body(1) ..., each with its number as a constant
     (body(std::integral_constant<int, I>()), ...);
@@ -509,7 +531,9 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
             const uint32_t at = block / (uint32_t)p.wide_chunks, unit = at / (uint32_t)p.kv_heads;
             j.kv = (int)(at - unit * p.kv_heads);
             int s, tile;
-            if (p.starts) {
+            if (p.starts && p.n_seq <= 64) {
+                if (!heaviest_first(p, R, unit, &s, &tile)) return;
+            } else if (p.starts) {
                 // sequence s has the tiles floor(starts[s] G / R) + s and on: n tokens have n G / R + 1 tiles at most
                 auto first_of = [&](int i) { return (uint32_t)((uint64_t)(uint32_t)std::max(p.starts[i], 0) * (uint32_t)p.group / R) + (uint32_t)i; };
                 int found = 0;
