@@ -1039,8 +1039,8 @@ static void launch_attend(AttendParams& p, void* q_copy, int64_t few_blocks, int
 static bool shape_ok(int dt, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page, int64_t width, int64_t longest, bool starts, int64_t sequences,
                      int64_t prefix) {
     return dt >= BT_F32 && dt <= BT_BF16 && tokens > 0 && tokens <= 0x7fffffff && kv_heads > 0 && heads > 0 && heads <= 16384 && tokens * heads <= 0x7fffffff && heads % kv_heads == 0 && dim > 0 && dim <= 256 && page >= 32 &&
-           page <= 65536 && (page & (page - 1)) == 0 && width > 0 && width * page <= 0x7fffff00 && longest >= 0 && longest <= width * page && sequences > 0 &&
-           sequences <= (1 << 24) && (starts || sequences == tokens) && prefix >= 0 && prefix <= 0x7fffff00;
+           page <= 65536 && (page & (page - 1)) == 0 && width > 0 && width * page <= (1 << 30) && longest >= 0 && longest <= width * page && sequences > 0 &&
+           sequences <= (1 << 24) && (starts || sequences == tokens) && prefix >= 0 && prefix <= (1 << 30);
 }
 
 }  // namespace bt
@@ -1064,7 +1064,7 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
     }
     if (!shape_ok(dtype, tokens, heads, kv_heads, head_dim, page_size, table_width, max_length, q_starts != nullptr, sequences, prefix_length) || pages <= 0 ||
         pages > 0x7fffffff) {
-        set_error("%s: head_dim at most 256, heads a multiple of kv_heads, page_size a power of two from 32 on, places of a sequence below 2^31, one token a "
+        set_error("%s: head_dim at most 256, heads a multiple of kv_heads, page_size a power of two from 32 on, up to 2^30 places of a sequence, one token a "
                   "sequence without q_starts (head_dim=%lld heads=%lld/%lld page_size=%lld width=%lld sequences=%lld tokens=%lld)",
                   who, (long long)head_dim, (long long)heads, (long long)kv_heads, (long long)page_size, (long long)table_width, (long long)sequences,
                   (long long)tokens);
@@ -1103,7 +1103,7 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
     const int64_t few_blocks = (a.few ? sequences * a.tiles * a.chunks * kv_heads : 0) + (a.prefix_wide ? 0 : prefix_blocks) + (clear ? 1 : 0);
     const int64_t wide_blocks = (a.wide ? a.wide_tiles * a.wide_chunks * kv_heads : 0) + (a.prefix_wide ? prefix_blocks : 0);
     const int64_t join_rows = a.join_few ? a.few_region.rows : a.few_parts || a.wide_parts ? tokens * heads : 0;
-    if (std::max({few_blocks, wide_blocks, join_rows / 4}) >= (1 << 22) || a.wide_tiles > 0x7fffffff || a.prefix_tiles > 0x7fffffff) {
+    if (std::max({few_blocks, wide_blocks, join_rows / 4}) >= (1 << 24) || a.wide_tiles > 0x7fffffff || a.prefix_tiles > 0x7fffffff) {
         set_error("%s: %lld workgroups are beyond one launch", who, (long long)std::max(few_blocks, wide_blocks));
         return BT_ERR_INVALID;
     }

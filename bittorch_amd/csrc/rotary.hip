@@ -353,8 +353,8 @@ extern "C" int bt_cache_append(const void* k, int64_t k_token, int64_t k_head, c
     }
     if (int rc = turn_checks(who, dtype, tokens, heads, kv_heads, head_dim, rotary_dim, freq_64, inv_freq)) return rc;
     if (head_dim > 256 || page_size < 32 || page_size > 65536 || (page_size & (page_size - 1)) || pages <= 0 || pages > 0x7fffffff || table_width <= 0 ||
-        table_width * page_size > 0x7fffffff || sequences <= 0 || sequences > (1 << 24) || (!q_starts && sequences != tokens)) {
-        set_error("%s: head_dim at most 256, page_size a power of two from 32 on, places of a sequence below 2^31, one token a sequence without q_starts "
+        table_width * page_size > (1 << 30) || sequences <= 0 || sequences > (1 << 24) || (!q_starts && sequences != tokens)) {
+        set_error("%s: head_dim at most 256, page_size a power of two from 32 on, up to 2^30 places of a sequence, one token a sequence without q_starts "
                   "(head_dim=%lld page_size=%lld width=%lld sequences=%lld tokens=%lld)",
                   who, (long long)head_dim, (long long)page_size, (long long)table_width, (long long)sequences, (long long)tokens);
         return BT_ERR_INVALID;

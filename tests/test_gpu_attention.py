@@ -146,6 +146,58 @@ def test_several_tokens_each(dt, held, new, heads, kv, dim, page, prefix):
     b.check(*b.attend(return_lse=True, scale=0.3), scale=0.3)
 
 
+# every number of 32-feature blocks with many rows, odd heads; more than 64 sequences, some of them of many rows; many heads to a key head
+WIDE = [([90, 70], [80, 64], 4, 2, d, 64, 33) for d in (1, 8, 31, 33, 64, 65, 96, 100, 129, 160, 161, 192, 200, 224, 225, 256)] + [
+    ([50, 3, 200, 9] * 20, [50, 1, 90, 9] * 20, 4, 2, 64, 32, 0), ([50, 3, 200, 9] * 17, [50, 1, 90, 0] * 17, 6, 2, 40, 32, 21), ([6000, 300], [300, 40], 2, 1, 64, 64, 0),
+    ([3000], [40], 2, 2, 128, 64, 0), ([700, 2500, 40, 5], [129, 65, 33, 1], 3, 3, 128, 32, 0)]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("held,new,heads,kv,dim,page,prefix", WIDE)
+def test_many_rows(dt, held, new, heads, kv, dim, page, prefix):
+    announce("attend many", held[:5], new[:5], heads, kv, dim, page, prefix, dt)
+    b = Batch(held, new, heads, kv, dim, page, dt, prefix)
+    b.check(*b.attend(return_lse=True))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("held,heads,kv,dim,page,prefix", [([300, 90], 80, 2, 64, 32, 0), ([70], 200, 1, 128, 64, 40), ([5, 0, 600], 33, 1, 256, 64, 0), ([4200] * 97, 8, 8, 16, 32, 0),
+                                                          ([9000, 8000], 2, 2, 24, 32, 0)])
+def test_many_heads_and_many_pages(dt, held, heads, kv, dim, page, prefix):
+    """More heads to a key head than a tile of rows, one token each; more pages in a chunk than a wave has lanes."""
+    announce("attend heads", held[:5], heads, kv, dim, page, prefix, dt)
+    b = Batch(held, [1] * len(held), heads, kv, dim, page, dt, prefix)
+    b.check(*b.attend(starts=False, return_lse=True))
+    b.check(*b.attend(return_lse=True))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_logits_of_any_size(dt):
+    """Rows of many tokens whose logits are in the thousands and in the hundred thousands: the weights are those of their differences.  Keys and queries
+    are whole numbers, so that products are exact; a key's weight is one or none."""
+    ops = _ops()
+    for size in (16, 256):
+        b = Batch([300], [120], 2, 1, 32, 32, dt)
+        kn = torch.zeros(b.k_cache.shape)
+        ids = torch.randperm(300, generator=torch.Generator().manual_seed(size))
+        number = b.table[0].cpu().long()
+        for place in range(300):
+            kn[number[place // 32], 0, place % 32, 0] = float(ids[place] % 61) * size / 8
+        from bittorch_amd.ops.attention import _tiled
+        kc = _tiled(kn.to(dt), kn.to(dt))[0].contiguous().cuda()
+        q = torch.zeros_like(b.q)
+        q[..., 0] = 8 * size
+        out = ops.cached_attention(q, kc, b.v_cache, b.table, b.lengths, b.q_starts, scale=1.0)
+        assert kn.to(dt).float().equal(kn)
+        for i in (0, 50, 119):
+            seen = torch.stack([kn[number[p // 32], 0, p % 32, 0] for p in range(181 + i)])
+            best = (seen == seen.max()).nonzero()[:, 0]
+            want = b.values[0][best.cuda()].mean(0)  # equal logits share
+            off = (out[i].double() - want).abs()
+            # (equal weights of exact logits; rounded once, their sum and their values as always)
+            assert bool((off <= (_half(dt) * 2 + 64 * U) * b.values[0][best.cuda()].abs().mean(0) + 1e-30).all()), (size, i)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_long_contexts_and_large_logits(dt):
     announce("attend long", dt)
@@ -222,6 +274,42 @@ def test_lengths_pages_and_rows_that_are_not_there():
         kc, vc = b.k_cache.clone(), b.v_cache.clone()
         ops.cache_append(b.q[:, :2].contiguous(), b.q[:, :2].contiguous(), kc, vc, b.table, b.lengths, torch.tensor(starts, dtype=torch.int32, device="cuda"))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("prefix", [0, 70])
+def test_rows_behind_the_last_sequence_among_many(prefix):
+    """With rows of both kernels, finished and joined from parts."""
+    for held, new in (([700, 2500, 40, 5], [129, 65, 33, 1]), ([300, 200], [130, 3]), ([90], [90])):
+        b = Batch(held, new, 4, 2, 64, 32, torch.float16, prefix)
+        more = torch.cat((b.q, torch.full((77, 4, 64), math.nan, device="cuda").half()))
+        out, lse = b.attend(more, return_lse=True)
+        assert not out[b.tokens:].any() and bool((lse[b.tokens:] == -math.inf).all())
+        b.check(out, lse)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_caches_of_more_than_2_to_the_31_elements(dt):
+    """Pages at both ends of the cache, written and read by both kernels."""
+    ops, page, dim = _ops(), 64, 128
+    pages = 2 ** 31 // (page * dim) + 9
+    announce("large cache", pages, dt)
+    kc, vc = (torch.empty(pages, 1, page, dim, dtype=dt, device="cuda") for _ in range(2))
+    order = torch.tensor([pages - 1, 0, pages - 5, 3, pages - 2, pages - 7], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(300, h, dim, generator=g).to(dt).cuda() for h in (2, 1, 1))
+    starts = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    lengths = starts[1:]
+    ops.cache_append(k, v, kc, vc, order[None], lengths, starts)
+    small = [torch.zeros(6, 1, page, dim, dtype=dt, device="cuda") for _ in range(2)]
+    ops.cache_append(k, v, *small, torch.arange(6, dtype=torch.int32, device="cuda")[None], lengths, starts)
+    for big, own in zip((kc, vc), small):
+        got = big[order.long()]
+        assert torch.equal(got[:4], own[:4])  # (the fifth page is whole up to place 300)
+    own = torch.arange(6, dtype=torch.int32, device="cuda")[None]
+    for many in (True, False):
+        args = (q, starts) if many else (q[-1:], None)
+        want = ops.cached_attention(args[0], *small, own, lengths, args[1])
+        assert torch.equal(ops.cached_attention(args[0], kc, vc, order[None], lengths, args[1]), want)
 
 
 def test_views_streams_and_order():
