@@ -30,7 +30,8 @@ struct AttendParams {
     int longest;
     int few_rows;        // sequences of up to so many rows are attend_rows_kernel's, others attend_tiles_kernel's
     // of the two kernels: places of a chunk of a sequence, chunks of the longest, and row tiles (few: of each sequence, wide: of all of them)
-    int chunk, chunks, tiles, wide_chunk, wide_chunks, wide_tiles;
+    int chunk, chunks, tiles, units, wide_chunk, wide_chunks, wide_tiles;
+    int all_few;         // every sequence is attend_rows_kernel's, their tiles in units as attend_tiles_kernel's are
     int prefix_chunk, prefix_chunks, prefix_tiles, prefix_wide;  // the prefix, whose rows are tiled by one of them
     Parts few_parts, wide_parts, prefix_parts;       // without: the workgroup sees all keys of its rows
     int few_slots;       // rows of a sequence and key head in few_parts
@@ -189,9 +190,26 @@ __device__ __forceinline__ bool own_job(const AttendParams& p, int R, int s, int
     j->end = std::min(j->begin + chunk, limit_of(p, *j, j->rows - 1));
     j->part = c;
     j->slots = wide ? p.wide_chunks : p.chunks;
-    j->few_slot = wide ? -1 : ((int64_t)s * p.kv_heads + j->kv) * p.few_slots + j->row0;
+    j->few_slot = wide || p.all_few ? -1 : ((int64_t)s * p.kv_heads + j->kv) * p.few_slots + j->row0;
     j->parts = wide ? p.wide_parts : p.few_parts;
     return j->begin < j->end || (!j->parts.o && c == 0);
+}
+// Sequence and tile of R rows of unit `unit`: sequence s has the units floor(starts[s] G / R) + s and on (n tokens have n G / R + 1 tiles at most).
+__device__ __forceinline__ bool tile_of(const AttendParams& p, uint32_t R, uint32_t unit, int* s, int* tile) {
+    const int lane = threadIdx.x & 63;
+    auto first_of = [&](int i) { return (uint32_t)((uint64_t)(uint32_t)std::max(p.starts[i], 0) * (uint32_t)p.group / R) + (uint32_t)i; };
+    int found = 0;
+    for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
+        const int i = s0 + lane;
+        const uint64_t hit = __ballot(i < p.n_seq && first_of(i < p.n_seq ? i : 0) <= unit);
+        found += __popcll(hit);
+        if (hit != ~0ull) break;
+    }
+    *s = found - 1;
+    if (*s < 0) return false;
+    const uint32_t first = first_of(*s);
+    *tile = (int)(unit - first);
+    return first <= unit;  // (starts that do not ascend)
 }
 // The chunk's pages, one a lane, 64 at a time.  The first ones are asked for before the length is known.
 struct PageWindow {
@@ -301,12 +319,14 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
             asked = PageWindow::ask(j.table, ((j.end - 1) >> p.page_shift) + 1, j.begin >> p.page_shift);
         } else {
             block -= prefix_blocks;
-            const uint32_t at = block / (uint32_t)p.chunks, unit = at / (uint32_t)p.kv_heads, s = unit / (uint32_t)p.tiles;
-            j.kv = (int)(at - unit * p.kv_heads);
-            if ((int)s >= p.n_seq) return clear_rows_behind<DT>(p);
+            const uint32_t at = block / (uint32_t)p.chunks, unit = at / (uint32_t)p.kv_heads;
             const int c = (int)(block - at * p.chunks);
+            j.kv = (int)(at - unit * p.kv_heads);
+            if ((int)unit >= p.units) return clear_rows_behind<DT>(p);
+            int s = (int)(unit / (uint32_t)p.tiles), tile = (int)unit - s * p.tiles;
+            if (p.all_few && !tile_of(p, R, unit, &s, &tile)) return;
             asked = PageWindow::ask(p.table + (int64_t)s * p.width, p.width, (c * p.chunk) >> p.page_shift);
-            if (!own_job(p, R, (int)s, (int)(unit - s * p.tiles), c, p.chunk, false, &j)) return;
+            if (!own_job(p, R, s, tile, c, p.chunk, false, &j)) return;
         }
     }
     const int kv = j.kv;
@@ -534,20 +554,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
             if (p.starts && p.n_seq <= 64) {
                 if (!heaviest_first(p, R, unit, &s, &tile)) return;
             } else if (p.starts) {
-                // sequence s has the tiles floor(starts[s] G / R) + s and on: n tokens have n G / R + 1 tiles at most
-                auto first_of = [&](int i) { return (uint32_t)((uint64_t)(uint32_t)std::max(p.starts[i], 0) * (uint32_t)p.group / R) + (uint32_t)i; };
-                int found = 0;
-                for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
-                    const int i = s0 + lane;
-                    const uint64_t hit = __ballot(i < p.n_seq && first_of(i < p.n_seq ? i : 0) <= unit);
-                    found += __popcll(hit);
-                    if (hit != ~0ull) break;
-                }
-                s = found - 1;
-                if (s < 0) return;
-                const uint32_t first = first_of(s);
-                if (first > unit) return;  // (starts that do not ascend)
-                tile = (int)(unit - first);
+                if (!tile_of(p, R, unit, &s, &tile)) return;
             } else {
                 const uint32_t each = (uint32_t)(p.group + R - 1) / R;
                 s = (int)(unit / each);
@@ -907,7 +914,7 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void attend_join_kernel(Atten
     if (there && s >= 0) {
         const bool wide = n * p.group > p.few_rows;
         const int slots = wide ? p.wide_chunks : p.chunks, chunk = wide ? p.wide_chunk : p.chunk;
-        const int64_t at = wide ? (int64_t)row * slots : few_slot * slots;
+        const int64_t at = wide || p.all_few ? (int64_t)row * slots : few_slot * slots;
         const Parts& mine = wide ? p.wide_parts : p.few_parts;
         there = mine.o != nullptr;  // (the other kernel's rows may be finished)
         if (there) {
@@ -955,13 +962,21 @@ struct Region {
     size_t ml, o;  // byte offsets in the workspace
 };
 struct AttendPlan {
-    int64_t chunk, chunks, tiles, few_slots, wide_chunk, wide_chunks, wide_tiles, prefix_chunk, prefix_chunks, prefix_tiles;
-    bool few, wide, prefix_wide;              // kernels that have work
+    int64_t chunk, chunks, tiles, few_rows, few_slots, wide_chunk, wide_chunks, wide_tiles, prefix_chunk, prefix_chunks, prefix_tiles;
+    bool few, wide, prefix_wide, all_few;     // kernels that have work
+    int64_t units;
     bool few_parts, wide_parts, join_few;
     Region few_region, wide_region, prefix_region;
     size_t q_copy;  // byte offset
     size_t bytes;
 };
+// Which kernel takes what.  A launch of attend_tiles_kernel takes 14 us before its rows pay (a long program, read from memory by every compute
+// unit; partly filled tiles) and asks for attend_rows_kernel beside it, which takes the sequences of few rows; then it forms 2.5 times as many
+// products a microsecond as attend_rows_kernel, which reads the keys again for every 16 rows.  All of a call, rows / tiles kernel, 32 heads on 8 key heads
+// of 128, sequences x tokens at places: 1 x 512 at 512 18 / 44 us, 4 x 64 at 1000 22 / 44, 16 x 40 at 600 34 / 44, 4 x 16 at 4096 35 / 36, 8 x 16
+// at 4096 63 / 53, 16 x 16 at 2000 69 / 49, 4 x 64 at 2000 44 / 41; the prefix of 512 rows x 8 key heads x 1000 places 51 / 57, of 128 x 4000
+// 31 / 38, of 128 x 16000 70 / 54.
+constexpr double TILES_PAY = 3 << 29;  // features of products: rows x places x key heads x dim
 constexpr int64_t FEW_ROWS = 32;
 static int64_t wide_tile(int64_t dim) { return dim <= 128 ? WideTile<4>::R : WideTile<8>::R; }
 static int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
@@ -974,18 +989,22 @@ static AttendPlan attend_plan(int dt, bool q_in_place, int64_t tokens, int64_t h
                               int64_t prefix) {
     AttendPlan a = {};
     const int64_t group = heads / kv_heads, most_rows = starts ? tokens * group : group;
-    a.few = starts || group <= FEW_ROWS;
-    a.wide = most_rows > FEW_ROWS;
-    a.few_slots = std::min(most_rows, FEW_ROWS);
+    auto pays = [&](int64_t places) { return (double)tokens * heads * places * dim > TILES_PAY; };
+    a.all_few = starts && !pays(longest);
+    a.few_rows = a.all_few ? 0x7fffffff : FEW_ROWS;
+    a.few = starts || group <= a.few_rows;
+    a.wide = most_rows > a.few_rows;
+    a.few_slots = std::min(most_rows, a.few_rows);
     a.tiles = ceil_div(a.few_slots, 16);
+    a.units = a.all_few ? tokens * group / 16 + sequences : sequences * a.tiles;
     a.wide_tiles = starts ? tokens * group / wide_tile(dim) + sequences : sequences * ceil_div(group, wide_tile(dim));
     // Up to 512 places in one workgroup, without parts: a row of 500 places 8.2 us, 5.9 and 5.3 and a launch in parts
-    a.chunk = longest <= 512 && !prefix ? 512 : chunk_of(longest, sequences * a.tiles * kv_heads, 768, 128, 4096);
+    a.chunk = longest <= 512 && !prefix ? 512 : chunk_of(longest, (a.all_few ? std::max(sequences, ceil_div(tokens * group, 16)) : a.units) * kv_heads, 768, 128, 4096);
     a.chunks = std::max<int64_t>(1, ceil_div(longest, a.chunk));
     a.wide_chunk = chunk_of(longest, a.wide_tiles * kv_heads, 512, 256, 1 << 30);
     a.wide_chunks = std::max<int64_t>(1, ceil_div(longest, a.wide_chunk));
     if (prefix) {
-        a.prefix_wide = tokens * group > FEW_ROWS;
+        a.prefix_wide = tokens * group > FEW_ROWS && pays(prefix);
         a.prefix_tiles = ceil_div(tokens * group, a.prefix_wide ? wide_tile(dim) : 16);
         a.prefix_chunk = a.prefix_wide ? chunk_of(prefix, a.prefix_tiles * kv_heads, 512, 256, 1 << 30) : chunk_of(prefix, a.prefix_tiles * kv_heads, 1024, 128, 4096);
         a.prefix_chunks = ceil_div(prefix, a.prefix_chunk);
@@ -999,7 +1018,7 @@ static AttendPlan attend_plan(int dt, bool q_in_place, int64_t tokens, int64_t h
         r.o = a.bytes, a.bytes += (size_t)round_up(r.rows * slots * part_stride((int)dim) * 4, 256);
         return r;
     };
-    a.few_region = region(a.few_parts, sequences * kv_heads * a.few_slots, a.chunks);
+    a.few_region = region(a.few_parts, a.all_few ? tokens * heads : sequences * kv_heads * a.few_slots, a.chunks);
     a.wide_region = region(a.wide_parts, tokens * heads, a.wide_chunks);
     a.prefix_region = region(prefix > 0, tokens * heads, a.prefix_chunks);
     a.q_copy = a.bytes;
@@ -1093,17 +1112,17 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
     p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads), p.dim = p.q_dim = (int)head_dim, p.dp = cache_head_dim(dtype, head_dim);
     p.n_seq = (int)sequences, p.width = (int)table_width, p.page_shift = __builtin_ctzll((unsigned long long)page_size), p.pages = (int)pages;
     p.prefix = (int)prefix_length;
-    p.longest = (int)max_length, p.few_rows = (int)FEW_ROWS, p.few_slots = (int)a.few_slots, p.join_few = a.join_few;
-    p.chunk = (int)a.chunk, p.chunks = (int)a.chunks, p.tiles = (int)a.tiles;
+    p.longest = (int)max_length, p.few_rows = (int)a.few_rows, p.few_slots = (int)a.few_slots, p.join_few = a.join_few;
+    p.chunk = (int)a.chunk, p.chunks = (int)a.chunks, p.tiles = (int)a.tiles, p.units = (int)a.units, p.all_few = a.all_few;
     p.wide_chunk = (int)a.wide_chunk, p.wide_chunks = (int)a.wide_chunks, p.wide_tiles = (int)a.wide_tiles;
     p.prefix_chunk = (int)a.prefix_chunk, p.prefix_chunks = (int)a.prefix_chunks, p.prefix_tiles = (int)a.prefix_tiles, p.prefix_wide = a.prefix_wide;
     p.scale2 = (float)((double)scale * 1.4426950408889634074);
     const int64_t prefix_blocks = a.prefix_tiles * a.prefix_chunks * kv_heads;
     const bool clear = q_starts && (a.join_few || (!a.few_parts && !a.wide_parts));  // (attend_join_kernel sees to the rows behind otherwise)
-    const int64_t few_blocks = (a.few ? sequences * a.tiles * a.chunks * kv_heads : 0) + (a.prefix_wide ? 0 : prefix_blocks) + (clear ? 1 : 0);
+    const int64_t few_blocks = (a.few ? a.units * a.chunks * kv_heads : 0) + (a.prefix_wide ? 0 : prefix_blocks) + (clear ? 1 : 0);
     const int64_t wide_blocks = (a.wide ? a.wide_tiles * a.wide_chunks * kv_heads : 0) + (a.prefix_wide ? prefix_blocks : 0);
     const int64_t join_rows = a.join_few ? a.few_region.rows : a.few_parts || a.wide_parts ? tokens * heads : 0;
-    if (std::max({few_blocks, wide_blocks, join_rows / 4}) >= (1 << 24) || a.wide_tiles > 0x7fffffff || a.prefix_tiles > 0x7fffffff) {
+    if (std::max({few_blocks, wide_blocks, join_rows / 4}) >= (1 << 24) || a.units > 0x7fffffff || a.wide_tiles > 0x7fffffff || a.prefix_tiles > 0x7fffffff) {
         set_error("%s: %lld workgroups are beyond one launch", who, (long long)std::max(few_blocks, wide_blocks));
         return BT_ERR_INVALID;
     }

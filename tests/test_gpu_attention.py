@@ -71,6 +71,15 @@ class Batch:
         self.prefix_table = order[:pages(prefix)].cuda() if prefix else None
         self.q = torch.randn(self.tokens, heads, dim, generator=g).to(dt).cuda()
 
+    def widened(self, wide=True):
+        """Tables that may hold so many places that sequences of many rows are taken as such."""
+        if wide:
+            width = max(self.width, -(-2 ** 31 // (self.tokens * self.heads * self.dim * self.page)))
+            table = torch.full((len(self.held), width), -7, dtype=torch.int32, device="cuda")
+            table[:, :self.width] = self.table
+            self.table, self.width = table, width
+        return self
+
     def attend(self, q=None, starts=True, **more):
         return _ops().cached_attention(self.q if q is None else q, self.k_cache, self.v_cache, self.table, self.lengths, self.q_starts if starts else None,
                                        prefix_table=self.prefix_table, prefix_length=self.prefix, **more)
@@ -137,11 +146,12 @@ def test_one_token_each(dt, held, new, heads, kv, dim, page, prefix):
     assert torch.equal(b.attend(starts=False), out)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("held,new,heads,kv,dim,page,prefix", RAGGED)
-def test_several_tokens_each(dt, held, new, heads, kv, dim, page, prefix):
-    announce("attend several", held[:9], new[:9], heads, kv, dim, page, prefix, dt)
-    b = Batch(held, new, heads, kv, dim, page, dt, prefix)
+def test_several_tokens_each(dt, held, new, heads, kv, dim, page, prefix, wide):
+    announce("attend several", held[:9], new[:9], heads, kv, dim, page, prefix, dt, wide)
+    b = Batch(held, new, heads, kv, dim, page, dt, prefix).widened(wide)
     b.check(*b.attend(return_lse=True))
     b.check(*b.attend(return_lse=True, scale=0.3), scale=0.3)
 
@@ -149,15 +159,28 @@ def test_several_tokens_each(dt, held, new, heads, kv, dim, page, prefix):
 # every number of 32-feature blocks with many rows, odd heads; more than 64 sequences, some of them of many rows; many heads to a key head
 WIDE = [([90, 70], [80, 64], 4, 2, d, 64, 33) for d in (1, 8, 31, 33, 64, 65, 96, 100, 129, 160, 161, 192, 200, 224, 225, 256)] + [
     ([50, 3, 200, 9] * 20, [50, 1, 90, 9] * 20, 4, 2, 64, 32, 0), ([50, 3, 200, 9] * 17, [50, 1, 90, 0] * 17, 6, 2, 40, 32, 21), ([6000, 300], [300, 40], 2, 1, 64, 64, 0),
-    ([3000], [40], 2, 2, 128, 64, 0), ([700, 2500, 40, 5], [129, 65, 33, 1], 3, 3, 128, 32, 0)]
+    ([3000], [40], 2, 2, 128, 64, 0), ([700, 2500, 40, 5], [129, 65, 33, 1], 3, 3, 128, 32, 0), ([50, 3, 200, 9] * 80, [50, 1, 90, 9] * 80, 4, 2, 64, 32, 0),
+    ([700, 350] * 10, [300, 350] * 10, 8, 8, 64, 64, 0)]
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("held,new,heads,kv,dim,page,prefix", WIDE)
+def test_many_rows(dt, held, new, heads, kv, dim, page, prefix, wide):
+    announce("attend many", held[:5], new[:5], heads, kv, dim, page, prefix, dt, wide)
+    b = Batch(held, new, heads, kv, dim, page, dt, prefix).widened(wide)
+    b.check(*b.attend(return_lse=True))
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("held,new,heads,kv,dim,page,prefix", WIDE)
-def test_many_rows(dt, held, new, heads, kv, dim, page, prefix):
-    announce("attend many", held[:5], new[:5], heads, kv, dim, page, prefix, dt)
+@pytest.mark.parametrize("held,new,heads,kv,dim,page,prefix", [([600, 300], [500, 260], 8, 2, 64, 64, 4200), ([300], [290], 8, 2, 128, 64, 5633), ([200, 90], [190, 60], 8, 2, 256, 32, 3300),
+                                                              ([400, 500], [390, 500], 10, 5, 40, 128, 4700), ([20, 0, 90] * 35, [1] * 105, 32, 4, 64, 64, 8000)])
+def test_long_prefixes_of_many_rows(dt, held, new, heads, kv, dim, page, prefix):
+    announce("attend prefix", held[:5], new[:5], heads, kv, dim, page, prefix, dt)
     b = Batch(held, new, heads, kv, dim, page, dt, prefix)
     b.check(*b.attend(return_lse=True))
+    if max(new) == 1:
+        b.check(*b.attend(starts=False, return_lse=True))
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -171,13 +194,14 @@ def test_many_heads_and_many_pages(dt, held, heads, kv, dim, page, prefix):
     b.check(*b.attend(return_lse=True))
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dt", TYPES)
-def test_logits_of_any_size(dt):
+def test_logits_of_any_size(dt, wide):
     """Rows of many tokens whose logits are in the thousands and in the hundred thousands: the weights are those of their differences.  Keys and queries
     are whole numbers, so that products are exact; a key's weight is one or none."""
     ops = _ops()
     for size in (16, 256):
-        b = Batch([300], [120], 2, 1, 32, 32, dt)
+        b = Batch([300], [120], 2, 1, 32, 32, dt).widened(wide)
         kn = torch.zeros(b.k_cache.shape)
         ids = torch.randperm(300, generator=torch.Generator().manual_seed(size))
         number = b.table[0].cpu().long()
@@ -204,15 +228,16 @@ def test_long_contexts_and_large_logits(dt):
     b = Batch([20011, 70000], [1, 1], 8, 2, 128, 64, dt, std=2.0)
     b.check(*b.attend(starts=False, return_lse=True))
     b = Batch([9000], [40], 8, 2, 64, 64, dt, 5000, std=3.0)
-    b.check(*b.attend(return_lse=True))
+    for wide in (False, True):
+        b.check(*b.widened(wide).attend(return_lse=True))
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("new", [1, 9, 200])
-def test_what_a_row_does_not_see_does_not_matter(dt, new):
+@pytest.mark.parametrize("new,wide", [(1, False), (9, False), (200, False), (40, True), (200, True)])
+def test_what_a_row_does_not_see_does_not_matter(dt, new, wide):
     """Later tokens of the same chunk whose keys and values are infinite or not a number, in the tile where the mask runs."""
     ops = _ops()
-    b = Batch([new + 45], [new], 4, 2, 64, 32, dt)
+    b = Batch([new + 45], [new], 4, 2, 64, 32, dt).widened(wide)
     clean = b.attend(return_lse=True)
     place = new + 44  # the last token's own
     number, at = int(b.table[0, place // 32]), place % 32
@@ -268,6 +293,26 @@ def test_lengths_pages_and_rows_that_are_not_there():
         assert not out[3:].any() and bool((lse[3:] == -math.inf).all())
         ref = ops.cached_attention(b.q, b.k_cache, b.v_cache, b.table[:, :width], lengths)
         assert bool(((out[:3] - ref).abs() <= 4 * _half(torch.bfloat16) * 4).all())
+    # pages outside the cache and lengths beyond the table among many rows: that sequence alone
+    for wide in (False, True):
+        many = Batch([200, 90, 70], [100, 70, 3], 4, 2, 64, 32, torch.bfloat16).widened(wide)
+        want, want_lse = many.attend(return_lse=True)
+        good, good_lengths = many.table, many.lengths
+        for wrong in (-1, many.k_cache.shape[0], 2 ** 31 - 1, -2 ** 31):
+            many.table = good.clone()
+            many.table[0, 1] = wrong
+            out, lse = many.attend(return_lse=True)
+            assert out[:100].isnan().all() and lse[:100].isnan().all() and torch.equal(out[100:], want[100:]) and torch.equal(lse[100:], want_lse[100:])
+        many.table, many.lengths = good, torch.tensor([200, many.width * 32 + 1, 70], dtype=torch.int32, device="cuda")
+        out = many.attend()
+        assert out[100:170].isnan().all() and torch.equal(out[:100], want[:100]) and torch.equal(out[170:], want[170:])
+        many.lengths = good_lengths
+        many.q_starts = torch.tensor([0, 100, 100, 173], dtype=torch.int32, device="cuda")
+        out, lse = many.attend(return_lse=True)  # the third's 73 tokens on 70 places: three that see nothing
+        assert torch.equal(out[:100], want[:100]) and not out[100:103].any() and bool((lse[100:103] == -math.inf).all()) and bool(out[103:].isfinite().all())
+        for starts in ([0, 900, 100, 173], [-4, 100, 50, 173], [173, 90, 1, 0], [0, 2 ** 31 - 1, -2 ** 31, 173], [0, 0, 0, 0]):
+            many.q_starts = torch.tensor(starts, dtype=torch.int32, device="cuda")
+            many.attend()
     # starts that make no sense stay inside the tensors
     for starts in ([0, 900, 2, 3], [-4, 1, 2, 3], [3, 2, 1, 0], [0, 2 ** 31 - 1, -2 ** 31, 3]):
         ops.cached_attention(b.q, b.k_cache, b.v_cache, b.table, b.lengths, torch.tensor(starts, dtype=torch.int32, device="cuda"))
@@ -276,11 +321,12 @@ def test_lengths_pages_and_rows_that_are_not_there():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("prefix", [0, 70])
-def test_rows_behind_the_last_sequence_among_many(prefix):
+def test_rows_behind_the_last_sequence_among_many(prefix, wide):
     """With rows of both kernels, finished and joined from parts."""
     for held, new in (([700, 2500, 40, 5], [129, 65, 33, 1]), ([300, 200], [130, 3]), ([90], [90])):
-        b = Batch(held, new, 4, 2, 64, 32, torch.float16, prefix)
+        b = Batch(held, new, 4, 2, 64, 32, torch.float16, prefix).widened(wide)
         more = torch.cat((b.q, torch.full((77, 4, 64), math.nan, device="cuda").half()))
         out, lse = b.attend(more, return_lse=True)
         assert not out[b.tokens:].any() and bool((lse[b.tokens:] == -math.inf).all())
@@ -306,10 +352,11 @@ def test_caches_of_more_than_2_to_the_31_elements(dt):
         got = big[order.long()]
         assert torch.equal(got[:4], own[:4])  # (the fifth page is whole up to place 300)
     own = torch.arange(6, dtype=torch.int32, device="cuda")[None]
-    for many in (True, False):
-        args = (q, starts) if many else (q[-1:], None)
-        want = ops.cached_attention(args[0], *small, own, lengths, args[1])
-        assert torch.equal(ops.cached_attention(args[0], kc, vc, order[None], lengths, args[1]), want)
+    wide = torch.cat((own, torch.full((1, 500), -7, dtype=torch.int32, device="cuda")), 1)  # (so many places that 300 rows are taken as many)
+    for args, tables in (((q, starts), own), ((q, starts), wide), ((q[-1:], None), own)):
+        want = ops.cached_attention(args[0], *small, tables, lengths, args[1])
+        there = torch.cat((order[None], tables[:, 6:]), 1)
+        assert torch.equal(ops.cached_attention(args[0], kc, vc, there, lengths, args[1]), want)
 
 
 def test_views_streams_and_order():
