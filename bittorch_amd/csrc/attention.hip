@@ -41,6 +41,7 @@ struct AttendParams {
 
 __host__ __device__ __forceinline__ int part_stride(int dim) { return (dim + 3) / 4 * 4; }
 
+typedef float v16f __attribute__((ext_vector_type(16)));
 template <int DT>
 struct Half8;  // an operand of 16-bit elements
 template <>
@@ -58,6 +59,12 @@ __device__ __forceinline__ v4f step(u32x4 a, u32x4 b, v4f c) {
         for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(v4f, a)[e], __builtin_bit_cast(v4f, b)[e], c, 0, 0, 0);
         return c;
     }
+}
+// Two lanes' groups of 8: 32 rows, 32 columns
+template <int DT>
+__device__ __forceinline__ v16f step(u32x4 a, u32x4 b, v16f c) {
+    if constexpr (DT == BT_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 // E weights as an operand; what rounding took from them in `rest`
 template <int DT>
@@ -130,6 +137,12 @@ __device__ __forceinline__ float over_groups_max(float x) {  // over the four la
 __device__ __forceinline__ float over_groups_sum(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
+}
+
+template <int ROWS, typename F>
+__device__ __forceinline__ float over_rows_lanes(float x, F join) {  // over the lanes of a row, of which there are 64 / ROWS
+    if (ROWS == 16) x = join(x, __shfl_xor(x, 16));
+    return join(x, __shfl_xor(x, 32));
 }
 
 // What a workgroup works on: up to R rows of one key head and a chunk of their keys.
@@ -487,14 +500,16 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
 
 // RT row tiles of 16 a wave and four waves: 128 rows (64 of more than 128 features, whose sums take twice the registers), whose keys and
 // values pass through LDS once for all of them, a tile of TK places at a time.  Tiles are read from memory straight into LDS, in the order in
-// which the waves take them from there (16 bytes a lane in a row: no bank is asked twice), up to NR tiles ahead.
+// which they lie there, up to NR tiles ahead.
 //
-// What bounds it.  A tile costs a wave (128 features) 32 matrix instructions of 16 cycles, and as many cycles for its 16 exponentials a lane
-// and the three or four instructions around each; LDS gives 64 bytes a cycle, so that the 16 KiB of fragments of each of a compute unit's eight
-// waves take 2000 cycles, and that is what a tile takes (0.87 us).  One block of instructions works on three tiles, the products of tile i + 1,
-// the weights of tile i and the sums over the values of tile i - 1, none of which waits for another: one thing after the other
-// took 1.4 us.  With 64 rows a wave and one wave a SIMD, which halves the fragments, it took 1.9 us: the sums live in accumulation registers then,
-// and the moves are more than what they spare.
+// What bounds it.  One block of instructions works on three tiles, the products of tile i + 1, the weights of tile i and the sums over the values of
+// tile i - 1, none of which waits for another (one thing after the other took 1.6 times as long).  A tile costs a wave (128 features, 16 bits) 16 matrix
+// instructions of 32 cycles, and about 95 others: 16 exponentials, three or four instructions around each, the rows' maxima.  The matrix unit is busy for 47%
+// of a long call's cycles and the vector unit for 47%, at the 2.0 GHz that such a load leaves; 2 x 1024 tokens of 32 heads see 4096 places
+// more in 126 us, 1.09 PFLOP/s where a large matrix product of a library reaches 1.22.  Matrix instructions of 16 rows take as many cycles and leave the
+// vector instructions less of them (4 x 512 tokens on 2048 places 79 -> 76 us).  LDS is not the bound (its fragments take a fifth of the cycles, and without
+// their reads a tile takes as long); one wait and barrier for two tiles was slower (280 us where this takes 263: half as far ahead), and more
+// fragments ahead make no difference.  64 rows a wave and one wave a SIMD took twice as long: the sums live in accumulation registers then.
 //
 // The maximum is that of the products before they are scaled, and one multiply-add and the exponential make a weight.  It is raised only where a
 // weight would pass 2^8: it needs to be near the true maximum, not to be it.  16-bit weights are rounded once (the rows kernel's two halves
@@ -526,6 +541,21 @@ template <typename Body, int... I>
 __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, Body body) {  // body(0), body(1) ..., each with its number as a constant
     (body(std::integral_constant<int, I>()), ...);
 }
+// N KiB of consecutive memory to LDS, 16 bytes a lane
+template <int N>
+__device__ __forceinline__ void dma_run(uint32_t lds_off, uint32_t voff, const void* sbase) {
+    static_assert(N >= 1 && N <= 4);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_off);
+    if constexpr (N == 1) dma16(to, voff, sbase);
+    if constexpr (N == 2)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" ::"s"(to), "v"(voff), "s"(sbase) : "memory");
+    if constexpr (N == 3)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %1, %2 offset:2048" ::"s"(to), "v"(voff), "s"(sbase) : "memory");
+    if constexpr (N == 4)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %1, %2 offset:2048\n\tglobal_load_lds_dwordx4 %1, %2 offset:3072" ::"s"(to), "v"(voff), "s"(sbase) : "memory");
+}
 template <int B>
 struct WideTile {
     static constexpr int RT = B <= 4 ? 2 : 1, R = 64 * RT;
@@ -534,12 +564,17 @@ template <int DT, int B>
 __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     using Order = CacheOrder<DT>;
     constexpr int E = Order::E, TK = Order::TK, C = 32 * B / TK, H = E / 4, V = 2 * B, RT = WideTile<B>::RT, R = WideTile<B>::R;
+    // 16-bit types with up to 128 features: 32 rows to a matrix instruction; others 16.  A lane has sums of T rows: EL products of each, in SA
+    // accumulators of AE, that make W operands of weights, and OA accumulators of sums; KF and V fragments of keys and values make a tile.
+    constexpr bool BIG = DT != BT_F32 && B <= 4;
+    constexpr int ROWS = BIG ? 32 : 16, T = RT * 16 / ROWS, AE = BIG ? 16 : 4, SA = BIG ? 1 : H, EL = SA * AE, W = EL / E, OA = BIG ? B : V, QC = BIG ? V : C, KF = QC * SA;
+    using Acc = std::conditional_t<BIG, v16f, v4f>;
     constexpr int TILE = 2048 * B;                                        // bytes of a tile's keys or values
     constexpr int NR = 32768 / TILE < 4 ? 32768 / TILE : 4;               // of each in LDS (loads into LDS reach 64 KiB)
     constexpr int LOADS = 2 * ((2 * B + 3) / 4);                          // of a wave for a tile
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * NR * TILE];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane % ROWS, g = lane / ROWS;
     Job j;
     {
         uint32_t block = blockIdx.x;
@@ -565,109 +600,132 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     }
     const int tiles = j.end > j.begin ? (j.end - j.begin + TK - 1) / TK : 0;
     const int mine = wave * RT * 16;  // this wave's first row
-    u32x4 q[RT][C];
-    int limit[RT];
+    u32x4 q[T][QC];
+    int limit[T];
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int at = mine + t * 16 + r, in_group = group_row(p, j, at);
+    for (int t = 0; t < T; t++) {
+        const int at = mine + t * ROWS + r, in_group = group_row(p, j, at);
         const int64_t q_at = q_row(p, j, at, in_group);
         limit[t] = at < j.rows ? j.limit0 + (j.causal ? in_group : 0) : 0;
 #pragma unroll
-        for (int c = 0; c < C; c++) q[t][c] = q_piece<DT>(p, q_at, c * TK + g * E, at < j.rows);
+        for (int c = 0; c < QC; c++) q[t][c] = q_piece<DT>(p, q_at, (c * (64 / ROWS) + g) * E, at < j.rows);
     }
     // the places that some row of the wave sees, and those that all see; the wave's tiles
     const int reach = mine < j.rows ? std::min(limit_of(p, j, std::min(mine + 16 * RT, j.rows) - 1), j.end) : 0;
     const int lowest = mine < j.rows ? std::min(limit_of(p, j, mine), j.end) : 0;
     const int my_tiles = reach > j.begin ? (reach - j.begin + TK - 1) / TK : 0;
 
-    const int64_t page_elements = (int64_t)p.dp << p.page_shift;
-    const int pieces = p.dp * TK * Order::SIZE / 1024;  // KiB of a tile's keys
-    int64_t at1 = 0, at2 = 0, at3 = 0;                  // where the last three tiles of keys came from: their values follow
-    auto load = [&](uint32_t to, const char* from) {
-#pragma unroll
-        for (int i0 = 0; i0 < V; i0 += 4) {
-            const int i = std::min(i0 + wave, pieces - 1);  // (every wave makes as many loads: they are counted)
-            dma16(to + i * 1024, i * 1024 + lane * 16, from);
-        }
-    };
-    // The page of the tile whose keys are loaded next: a scalar load each, so that no wait for it waits for the tiles on their way.
-    typedef const __attribute__((address_space(4))) int32_t* ScalarPointer;
-    const ScalarPointer table = (ScalarPointer)(uintptr_t)j.table;
-    int page = tiles ? table[j.begin >> p.page_shift] : 0;
+    // Fragments: where a lane's piece of them is in the tile, and the places of the tile that a lane's products and pieces of values have.  The rows
+    // of a fragment of keys are such places that a lane's products are the weights it brings to the values.
+    const int key_lane = BIG ? (r >> 3 & 1) * 1024 + g * 256 + ((r >> 4) * 2 + (r >> 2 & 1)) * 64 + (r & 3) * 16 : lane * 16;
+    const int value_lane = BIG ? (r >> 4) * 1024 + g * 256 + (r & 15) * 16 : lane * 16;
+    auto key_piece = [](int f) { return BIG ? f / 2 * 2048 + f % 2 * 512 : (f % QC * SA + f / QC) * 1024; };
+    auto value_piece = [](int f) { return BIG ? f % OA * 2048 + f / OA * 512 : f * 1024; };
+    auto place_of = [](int g, int e) { return e / E * (E * (64 / ROWS)) + g * E + e % E; };
+
+    // A tile's KiB are split over the waves, as many to each (some twice where they are not a multiple of four: the loads are counted)
+    const int piece = std::min(LOADS / 2 * wave, p.dp * TK * Order::SIZE / 1024 - LOADS / 2);
+    auto load = [&](uint32_t to, const char* from) { dma_run<LOADS / 2>(to + piece * 1024, piece * 1024 + lane * 16, from); };
+    // The chunk's pages, 64 at a time, one a lane (a scalar load for each would be waited for together with the first fragments), and the tile whose keys
+    // are loaded next: behind the last one that one again, for the count of loads.
+    const int64_t head_bytes = ((int64_t)p.dp << p.page_shift) * Order::SIZE;
+    const int page_bytes = (int)std::min<int64_t>(head_bytes, 0x7fffffff), tile_bytes = TK * p.dp * Order::SIZE;  // (at most 2^26)
+    int numbers = 0, first_number = 0, number = j.begin >> p.page_shift, offset = (j.begin & ((1 << p.page_shift) - 1)) * p.dp * Order::SIZE, left = tiles;
+    int64_t page_at = 0, at1 = 0, at2 = 0, at3 = 0;  // at: where the last three tiles of keys came from; their values follow
     bool bad = j.bad;
-    auto load_keys = [&](int tile) {  // (behind the last tile that one again, for the count)
-        const int place = j.begin + std::min(tile, tiles - 1) * TK;
+    auto find_page = [&]() {
+        if (number >= first_number + 64 || left == tiles) {
+            first_number = number;
+            numbers = j.table[std::min(number + lane, (j.end - 1) >> p.page_shift)];
+            asm volatile("" : "+v"(numbers));  // (waited for here, not at every tile)
+        }
+        int page = __builtin_amdgcn_readlane(numbers, number - first_number);
         if ((uint32_t)page >= (uint32_t)p.pages) page = 0, bad = true;
-        at3 = at2, at2 = at1;
-        at1 = (((int64_t)page * p.kv_heads + j.kv) * page_elements + (int64_t)(place & ((1 << p.page_shift) - 1)) * p.dp) * Order::SIZE;
+        page_at = ((int64_t)page * p.kv_heads + j.kv) * head_bytes;
+    };
+    auto load_keys = [&](int tile) {
+        at3 = at2, at2 = at1, at1 = page_at + offset;
         load(lds0 + (uint32_t)(tile % NR) * TILE, (const char*)p.k_cache + at1);
-        page = table[(j.begin + std::min(tile + 1, tiles - 1) * TK) >> p.page_shift];
+        left--;
+        offset += left > 0 ? tile_bytes : 0;
+    };
+    auto next_page = [&]() {
+        if (offset == page_bytes) offset = 0, number++, find_page();
     };
     // (at: where the tile's keys came from)
     auto load_values = [&](int tile, int64_t at) { load(lds0 + (uint32_t)(NR + tile % NR) * TILE, (const char*)p.v_cache + at); };
 
-    v4f o[RT][V], s[RT][H];       // s: products of the tile whose weights come next
-    float m[RT], l[RT], top[RT];  // the rows' maxima (of the products before they are scaled), sums and s's maxima (of this lane's places)
-    u32x4 w[RT];                  // weights of the tile before
-    std::conditional_t<(V > 8), uint64_t, uint32_t> nan[RT];  // features 16 b + 4 g + e, bit 4 b + e, that saw a value that is no number
+    Acc o[T][OA], s[T][SA];     // s: products of the tile whose weights come next
+    float m[T], l[T], top[T];   // the rows' maxima (of the products before they are scaled), sums and s's maxima (of this lane's places)
+    u32x4 w[T][W];              // weights of the tile before
+    std::conditional_t<(BIG || V > 8), uint64_t, uint32_t> nan[T];  // elements e of accumulator b of the sums, bit AE b + e, that saw a value that is no number
     const float slack = 8.0f / p.scale2;
     // The multiply-add rounds once, the base alone too: logits of a size at which that is more than a part of one are rounded alike first.
     bool large = false;
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
+    for (int t = 0; t < T; t++) {
         m[t] = -__builtin_inff(), l[t] = 0.0f, top[t] = 0.0f, nan[t] = 0;
-        w[t] = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < V; b++) o[t][b] = v4f{0, 0, 0, 0};
+        for (int i = 0; i < W; i++) w[t][i] = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < H; h++) s[t][h] = v4f{0, 0, 0, 0};
+        for (int b = 0; b < OA; b++) o[t][b] = Acc{};
+#pragma unroll
+        for (int h = 0; h < SA; h++) s[t][h] = Acc{};
     }
-    auto keys_at = [&](int tile) { return lds + tile % NR * TILE + lane * 16; };
-    auto values_at = [&](int tile) { return lds + (NR + tile % NR) * TILE + lane * 16; };
-    auto products = [&](const uint8_t* kf, v4f (&s)[RT][H]) {
+    auto keys_at = [&](int tile) { return lds + tile % NR * TILE + key_lane; };
+    auto values_at = [&](int tile) { return lds + (NR + tile % NR) * TILE + value_lane; };
+    // fragment f of keys with the queries; of values with the weights
+    auto multiply_keys = [&](auto number, u32x4 k, Acc (&s)[T][SA]) {
+        constexpr int f = decltype(number)::value, h = f / QC, c = f % QC;
+        if (DT == BT_F32 && c == QC - 1 && c * TK >= p.dp) k = u32x4{0, 0, 0, 0};  // (a tile has one group of features less)
 #pragma unroll
-        for (int h = 0; h < H; h++)
+        for (int t = 0; t < T; t++) s[t][h] = step<DT>(k, q[t][c], c ? s[t][h] : Acc{});
+    };
+    auto multiply_values = [&](auto number, u32x4 v) {
+        constexpr int f = decltype(number)::value;
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                u32x4 k = *(const u32x4*)(kf + (c * H + h) * 1024);
-                if (DT == BT_F32 && c == C - 1 && c * TK >= p.dp) k = u32x4{0, 0, 0, 0};  // (a tile has one group of features less)
-#pragma unroll
-                for (int t = 0; t < RT; t++) s[t][h] = step<DT>(k, q[t][c], c ? s[t][h] : v4f{0, 0, 0, 0});
-            }
+        for (int t = 0; t < T; t++) o[t][f % OA] = step<DT>(v, w[t][f / OA], o[t][f % OA]);
+    };
+    auto products = [&](const uint8_t* kf, Acc (&s)[T][SA]) {
+        unrolled(std::make_integer_sequence<int, KF>(), [&](auto number) { multiply_keys(number, *(const u32x4*)(kf + key_piece(decltype(number)::value)), s); });
     };
     auto maxima = [&]() {
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
+        for (int t = 0; t < T; t++) {
             top[t] = s[t][0][0];
 #pragma unroll
-            for (int e = 1; e < E; e++) top[t] = fmaxf(top[t], s[t][e / 4][e % 4]);
+            for (int e = 1; e < EL; e++) top[t] = fmaxf(top[t], s[t][e / AE][e % AE]);
         }
     };
-    auto weights = [&](float scale, auto base_of, u32x4 (&w)[RT]) {
+    auto weights = [&](float scale, auto base_of) {
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
+        for (int t = 0; t < T; t++) {
             const float base = base_of(t);
-            float x[E];
+            float sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], scale, base));
-            w[t] = operand<DT>(x, nullptr);
-            float sum = x[0] + x[1];
+            for (int i = 0; i < W; i++) {
+                float x[E];
 #pragma unroll
-            for (int e = 2; e < E; e += 2) sum += x[e] + x[e + 1];
+                for (int e = 0; e < E; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][(i * E + e) / AE][(i * E + e) % AE], scale, base));
+                w[t][i] = operand<DT>(x, nullptr);
+#pragma unroll
+                for (int e = 0; e < E; e++) sum = i || e ? sum + x[e] : x[0];
+            }
             l[t] += sum;
         }
     };
     auto over = [&]() {
         bool any = false;
 #pragma unroll
-        for (int t = 0; t < RT; t++) any |= top[t] > m[t] + slack;
+        for (int t = 0; t < T; t++) any |= top[t] > m[t] + slack;
         return __any(any);
     };
-    float shrink[RT];
+    float shrink[T];
+    bool raised = false;  // m and l are, the sums are not yet
     auto raise = [&]() {  // m and l; the sums over values follow once those of the tile before are in
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const float next = fmaxf(m[t], over_groups_max(top[t]));
+        for (int t = 0; t < T; t++) {
+            const float next = fmaxf(m[t], over_rows_lanes<ROWS>(top[t], [](float a, float b) { return fmaxf(a, b); }));
             shrink[t] = __builtin_amdgcn_exp2f(m[t] == next ? 0.0f : (m[t] - next) * p.scale2);
             m[t] = next;
             l[t] *= shrink[t];
@@ -676,23 +734,19 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     };
     auto shrink_sums = [&]() {
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int t = 0; t < T; t++)
 #pragma unroll
-            for (int b = 0; b < V; b++) o[t][b] *= shrink[t];
+            for (int b = 0; b < OA; b++) o[t][b] *= shrink[t];
     };
     // Iteration i loads the keys of tile i + NR and the values of tile i - 2 + NR into the places that iteration i - 1 read last, and reads
     // what iteration i + 1 - NR loaded: what the last NR - 2 iterations loaded may still be on its way.
-    auto turn = [&](int i) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NR - 2) * LOADS) : "memory");
-        if (i < tiles) {
-            load_keys(i + NR);
-            load_values(i + NR - 2, at3);
-        }
-    };
+    auto turn = [&]() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NR - 2) * LOADS) : "memory"); };
     if (tiles) {
+        find_page();
         load_keys(0);
 #pragma unroll
         for (int i = 1 - NR; i < 0; i++) {
+            next_page();
             load_keys(i + NR);
             load_values(std::max(i + NR - 2, 0), i + NR >= 2 ? at3 : at2);
         }
@@ -704,123 +758,146 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     for (int i = 0; i <= tiles && tiles;) {
         if (i > 0 && i < whole && !large) {
             maxima();
-            for (; i < whole && !large; i++) {
-                turn(i);
-                const bool raised = over();
+            for (; i < whole; i++) {
+                raised = over();
                 if (raised) raise();
+                if (large) break;  // (before this tile's weights)
+                turn();
                 // F fragments, each with its matrix instructions and a share of the other pipe's work; loads run AHEAD fragments in front
-                constexpr int F = C * H + V, N = RT * E, AHEAD = 3;
+                constexpr int F = KF + V, N = T * EL, AHEAD = 3;
                 const uint8_t *kf = keys_at(i + 1), *vf = values_at(i - 1);
-                u32x4 frag[F], w2[RT];
-                v4f s2[RT][H];
-                float x[RT][E], sum[RT], next_top[RT];
-                auto fetch = [&](int f) { frag[f] = *(const u32x4*)(f < C * H ? kf + (f % C * H + f / C) * 1024 : vf + (f - C * H) * 1024); };
+                u32x4 frag[F], w2[T][W];
+                Acc s2[T][SA];
+                float x[T][W][E], sum[T], next_top[T], base[T];
+                auto fetch = [&](int f) { frag[f] = *(const u32x4*)(f < KF ? kf + key_piece(f) : vf + value_piece(f - KF)); };
 #pragma unroll
                 for (int f = 0; f < AHEAD; f++) fetch(f);
+                __builtin_amdgcn_sched_barrier(0);
+                next_page();
+#pragma unroll
+                for (int t = 0; t < T; t++) base[t] = -m[t] * p.scale2;
                 unrolled(std::make_integer_sequence<int, F>(), [&](auto number) {
                     constexpr int f = decltype(number)::value;
                     __builtin_amdgcn_sched_barrier(0);
                     if constexpr (f + AHEAD < F) fetch(f + AHEAD);
-                    if constexpr (f < C * H) {
-                        constexpr int h = f / C, c = f % C;
-                        if (DT == BT_F32 && c == C - 1 && c * TK >= p.dp) frag[f] = u32x4{0, 0, 0, 0};  // (a tile has one group of features less)
-#pragma unroll
-                        for (int t = 0; t < RT; t++) s2[t][h] = step<DT>(frag[f], q[t][c], c ? s2[t][h] : v4f{0, 0, 0, 0});
-                    } else {
-#pragma unroll
-                        for (int t = 0; t < RT; t++) o[t][f - C * H] = step<DT>(frag[f], w[t], o[t][f - C * H]);
-                    }
+                    if constexpr (f < KF) multiply_keys(number, frag[f], s2);
+                    else multiply_values(std::integral_constant<int, f - KF>(), frag[f]);
 #pragma unroll
                     for (int n = f * N / F; n < (f + 1) * N / F; n++) {  // weights
-                        const int t = n / E, e = n % E;
-                        x[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / 4][e % 4], p.scale2, -m[t] * p.scale2));
-                        sum[t] = e ? sum[t] + x[t][e] : x[t][e];
-                        if (e == E - 1) {
-                            l[t] += sum[t];
-                            w2[t] = operand<DT>(x[t], nullptr);
-                        }
+                        const int t = n / EL, e = n % EL;
+                        float& weight = x[t][e / E][e % E];
+                        weight = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e / AE][e % AE], p.scale2, base[t]));
+                        sum[t] = e ? sum[t] + weight : weight;
+                        asm volatile("" : "+v"(sum[t]));
+                        if (e % E == E - 1) w2[t][e / E] = operand<DT>(x[t][e / E], nullptr);
+                        if (e == EL - 1) l[t] += sum[t];
                     }
-                    if constexpr (f >= C * H) {  // maxima of the products
+                    if constexpr (f == F / 8) load_keys(i + NR);  // (scalar work and loads while the matrix instructions run)
+                    if constexpr (f == F / 8 + 1) load_values(i + NR - 2, at3);
+                    if constexpr (f >= KF) {  // maxima of the products
 #pragma unroll
-                        for (int n = (f - C * H) * N / V; n < (f + 1 - C * H) * N / V; n++) {
-                            const int t = n / E, e = n % E;
-                            next_top[t] = e ? fmaxf(next_top[t], s2[t][e / 4][e % 4]) : s2[t][0][0];
+                        for (int n = (f - KF) * N / V; n < (f + 1 - KF) * N / V; n++) {
+                            const int t = n / EL, e = n % EL;
+                            next_top[t] = e ? fmaxf(next_top[t], s2[t][e / AE][e % AE]) : s2[t][0][0];
                         }
+#pragma unroll
+                        for (int t = 0; t < T; t++) if (t <= ((f + 1 - KF) * N / V - 1) / EL) asm volatile("" : "+v"(next_top[t]));  // (here, not behind the last one)
                     }
                 });
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    top[t] = next_top[t], w[t] = w2[t];
+                for (int t = 0; t < T; t++) {
+                    top[t] = next_top[t];
 #pragma unroll
-                    for (int h = 0; h < H; h++) s[t][h] = s2[t][h];
-                    for (int h = 0; h < H; h++) asm volatile("" : "+v"(s[t][h]));
-                    asm volatile("" : "+v"(w[t]), "+v"(l[t]), "+v"(top[t]));  // (all of it here, not behind the branch)
+                    for (int h = 0; h < W; h++) {
+                        w[t][h] = w2[t][h];
+                        asm volatile("" : "+v"(w[t][h]));
+                    }
+#pragma unroll
+                    for (int h = 0; h < SA; h++) {
+                        s[t][h] = s2[t][h];
+                        asm volatile("" : "+v"(s[t][h]));
+                    }
+                    asm volatile("" : "+v"(l[t]), "+v"(top[t]));  // (all of it here, not behind the branch)
                 }
                 if (raised) shrink_sums();
+                raised = false;
             }
-            continue;
+            if (!large) continue;
         }
         // any other: one thing after the other
-        turn(i);
+        turn();
+        if (i < tiles) {
+            next_page();
+            load_keys(i + NR);
+            load_values(i + NR - 2, at3);
+        }
         const int place = j.begin + i * TK;
+        int here = g;  // (what is made of it and of the limits is made here: kept across the loop above it takes the registers that the loop's loads need)
+        asm volatile("" : "+v"(here));
         if (i > 0 && i <= my_tiles) {
             const uint8_t* vf = values_at(i - 1);
+            auto values = [&](int f) { return *(const u32x4*)(vf + value_piece(f)); };
             // values that are no numbers, behind the end or where some row does not look, would make all rows such
             bool special = false;
 #pragma unroll 1
-            for (int b = 0; b < V; b++) {
-                u32x4 v = *(const u32x4*)(vf + b * 1024), where;
+            for (int f = 0; f < V; f++) {
+                u32x4 v = values(f), where;
                 special |= take_specials<DT>(v, where);
             }
-            if (__any(special)) {
-                const int live = j.end - (place - TK + g * E);  // no row sees what lies behind
+            special = __any(special);
+            auto live = [&](int f) { return j.end - (place - TK) - place_of(here, f / OA * E); };  // no row sees what lies behind
+            if (special) {
 #pragma unroll 1
-                for (int b = 0; b < V; b++) {
-                    u32x4 v = first_places<DT>(*(const u32x4*)(vf + b * 1024), live), where;
+                for (int f = 0; f < V; f++) {
+                    u32x4 v = first_places<DT>(values(f), live(f)), where;
                     take_specials<DT>(v, where);
 #pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        const v4f seen = step<DT>(where, w[t], v4f{0, 0, 0, 0});
+                    for (int t = 0; t < T; t++) {
+                        u32x4 by = w[t][0];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) nan[t] |= (decltype(nan[t] + 0))(seen[e] > 0.0f) << (4 * b + e);
+                        for (int e = 0; e < 4; e++) by[e] = f < OA ? by[e] : w[t][W - 1][e];
+                        const Acc seen = step<DT>(where, by, Acc{});
+#pragma unroll
+                        for (int e = 0; e < AE; e++) nan[t] |= (decltype(nan[t] + 0))(seen[e] > 0.0f) << (AE * (f % OA) + e);
                     }
                 }
-#pragma unroll
-                for (int b = 0; b < V; b++) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    u32x4 v = first_places<DT>(*(const u32x4*)(vf + b * 1024), live), where;
-                    take_specials<DT>(v, where);
-#pragma unroll
-                    for (int t = 0; t < RT; t++) o[t][b] = step<DT>(v, w[t], o[t][b]);
-                }
-            } else {
-#pragma unroll
-                for (int b = 0; b < V; b++) {
-                    const u32x4 v = *(const u32x4*)(vf + b * 1024);
-#pragma unroll
-                    for (int t = 0; t < RT; t++) o[t][b] = step<DT>(v, w[t], o[t][b]);
-                }
             }
+            unrolled(std::make_integer_sequence<int, V>(), [&](auto number) {
+                __builtin_amdgcn_sched_barrier(0);
+                u32x4 v = values(decltype(number)::value);
+                if (special) {
+                    u32x4 where;
+                    v = first_places<DT>(v, live(decltype(number)::value));
+                    take_specials<DT>(v, where);
+                }
+                multiply_values(number, v);
+            });
         }
         if (i < my_tiles) {
 #pragma unroll
-            for (int t = 0; t < RT; t++)
+            for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int e = 0; e < E; e++) s[t][e / 4][e % 4] = place + g * E + e < limit[t] ? s[t][e / 4][e % 4] : -__builtin_inff();
+                for (int e = 0; e < EL; e++) s[t][e / AE][e % AE] = place + place_of(here, e) < limit[t] ? s[t][e / AE][e % AE] : -__builtin_inff();
             maxima();
-            if (over()) {
+            float owed[T];
+#pragma unroll
+            for (int t = 0; t < T; t++) owed[t] = raised ? shrink[t] : 1.0f;
+            if (over() || raised) {
                 raise();
+#pragma unroll
+                for (int t = 0; t < T; t++) shrink[t] *= owed[t];
                 if (i) shrink_sums();
             }
+            raised = false;
             auto base_of = [&](int t) { return m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2; };
             if (large) {
 #pragma unroll
-                for (int t = 0; t < RT; t++)
+                for (int t = 0; t < T; t++)
 #pragma unroll
-                    for (int e = 0; e < E; e++) s[t][e / 4][e % 4] = s[t][e / 4][e % 4] * p.scale2 + base_of(t);
+                    for (int e = 0; e < EL; e++) s[t][e / AE][e % AE] = s[t][e / AE][e % AE] * p.scale2 + base_of(t);
             }
-            weights(large ? 1.0f : p.scale2, [&](int t) { return large ? 0.0f : base_of(t); }, w);
+            weights(large ? 1.0f : p.scale2, [&](int t) { return large ? 0.0f : base_of(t); });
             products(keys_at(i + 1), s);
         }
         i++;
@@ -829,38 +906,45 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     // Some of the wave's rows at a time through its quarter of LDS: whole lines to memory, and a loop where the registers would take a program
     // longer than all the rest, which every workgroup runs once, from memory (1.2 us a KiB: it took 60 us).
-    constexpr int LD = 32 * B, TS = std::min(RT, (int)(sizeof(lds) / 4 / (16 * LD * 4)));
+    constexpr int LD = 32 * B, TS = std::min(T, (int)(sizeof(lds) / 4 / (ROWS * LD * 4)));
+    static_assert(TS >= 1);
     float* mine_lds = (float*)lds + wave * (int)(sizeof(lds) / 16);
 #pragma unroll
-    for (int t0 = 0; t0 < RT; t0 += TS) {
-        if (mine + t0 * 16 >= j.rows) break;
+    for (int t0 = 0; t0 < T; t0 += TS) {
+        if (mine + t0 * ROWS >= j.rows) break;
         float sum[TS], most[TS];
 #pragma unroll
         for (int t = 0; t < TS; t++) {
-            sum[t] = bad ? __builtin_nanf("") : over_groups_sum(l[t0 + t]);
+            sum[t] = bad ? __builtin_nanf("") : over_rows_lanes<ROWS>(l[t0 + t], [](float a, float b) { return a + b; });
             most[t] = m[t0 + t] == -__builtin_inff() ? m[t0 + t] : m[t0 + t] * p.scale2;
             // (columns of four are turned by the row, so that 16 rows are in 16 places)
 #pragma unroll
-            for (int b = 0; b < V; b++) *(v4f*)&mine_lds[(t * 16 + r) * LD + ((b * 4 + g) ^ (r & 7)) * 4] = o[t0 + t][b];
+            for (int b = 0; b < (BIG ? 4 * B : V); b++) {
+                const int column = BIG ? b * 2 + g : b * 4 + g, e = BIG ? b % 4 * 4 : 0;
+                const Acc& from = o[t0 + t][BIG ? b / 4 : b];
+                *(v4f*)&mine_lds[(t * ROWS + r) * LD + (column ^ (r & 7)) * 4] = v4f{from[e], from[e + 1], from[e + 2], from[e + 3]};
+            }
         }
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-        for (int i = lane; i < TS * 16 * 8 * B; i += 64) {
-            const int row = i / (8 * B), f = i % (8 * B) * 4, from = row % 16;
+        for (int i = lane; i < TS * ROWS * 8 * B; i += 64) {
+            const int row = i / (8 * B), f = i % (8 * B) * 4, from = row % ROWS;
             v4f acc = *(const v4f*)&mine_lds[row * LD + ((f / 4) ^ (row & 7)) * 4];
-            auto bits = __shfl(nan[t0], from + f % 16 / 4 * 16);
+            // (the lane and the bits of the row's features f to f + 3)
+            const int lane_of = from + f / 4 % (64 / ROWS) * ROWS, bit = BIG ? f / 8 * 4 : f / 16 * 4;
+            auto bits = __shfl(nan[t0], lane_of);
             float row_sum = __shfl(sum[0], from), row_most = __shfl(most[0], from);
 #pragma unroll
             for (int t = 1; t < TS; t++) {
-                const auto b1 = __shfl(nan[t0 + t], from + f % 16 / 4 * 16);
+                const auto b1 = __shfl(nan[t0 + t], lane_of);
                 const float s1 = __shfl(sum[t], from), m1 = __shfl(most[t], from);
-                if (row >= t * 16) bits = b1, row_sum = s1, row_most = m1;
+                if (row >= t * ROWS) bits = b1, row_sum = s1, row_most = m1;
             }
-            bits >>= f / 16 * 4;
+            bits >>= bit;
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] = bits >> e & 1 ? __builtin_nanf("") : acc[e];
-            const int at = mine + t0 * 16 + row;
+            const int at = mine + t0 * ROWS + row;
             if (at < j.rows && f < p.dim) put_row<DT>(p, j, at, f, acc, row_most, row_sum);
         }
         __builtin_amdgcn_wave_barrier();

@@ -194,11 +194,12 @@ def test_many_heads_and_many_pages(dt, held, heads, kv, dim, page, prefix):
     b.check(*b.attend(return_lse=True))
 
 
+@pytest.mark.parametrize("quiet", [0, 100])
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dt", TYPES)
-def test_logits_of_any_size(dt, wide):
-    """Rows of many tokens whose logits are in the thousands and in the hundred thousands: the weights are those of their differences.  Keys and queries
-    are whole numbers, so that products are exact; a key's weight is one or none."""
+def test_logits_of_any_size(dt, wide, quiet):
+    """Rows of many tokens whose logits are in the thousands and in the hundred thousands, behind `quiet` places whose are zero: the weights are those of
+    their differences.  Keys and queries are whole numbers, so that products are exact; a key's weight is one or none."""
     ops = _ops()
     for size in (16, 256):
         b = Batch([300], [120], 2, 1, 32, 32, dt).widened(wide)
@@ -206,7 +207,7 @@ def test_logits_of_any_size(dt, wide):
         ids = torch.randperm(300, generator=torch.Generator().manual_seed(size))
         number = b.table[0].cpu().long()
         for place in range(300):
-            kn[number[place // 32], 0, place % 32, 0] = float(ids[place] % 61) * size / 8
+            kn[number[place // 32], 0, place % 32, 0] = float(ids[place] % 61) * size / 8 if place >= quiet else 0.0
         from bittorch_amd.ops.attention import _tiled
         kc = _tiled(kn.to(dt), kn.to(dt))[0].contiguous().cuda()
         q = torch.zeros_like(b.q)
