@@ -1083,14 +1083,18 @@ static AttendPlan attend_plan(int dt, bool q_in_place, int64_t tokens, int64_t h
     a.units = a.all_few ? tokens * group / 16 + sequences : sequences * a.tiles;
     a.wide_tiles = starts ? tokens * group / wide_tile(dim) + sequences : sequences * ceil_div(group, wide_tile(dim));
     // Up to 512 places in one workgroup, without parts: a row of 500 places 8.2 us, 5.9 and 5.3 and a launch in parts
-    a.chunk = longest <= 512 && !prefix ? 512 : chunk_of(longest, (a.all_few ? std::max(sequences, ceil_div(tokens * group, 16)) : a.units) * kv_heads, 768, 128, 4096);
+    // Three workgroups to a compute unit where the caches are large, else one, with fewer parts to join (37 sequences of up to 7 tokens x 900 places behind 1000
+    // 25 / 19 us, 8 x 12 tokens on 1000 22 / 15; 3 x 50000 places 98 / 117)
+    const bool little = (double)sequences * kv_heads * longest * dim * 2 * dtype_size(dt) < (64 << 20);
+    a.chunk = longest <= 512 && !prefix ? 512
+                                        : chunk_of(longest, (a.all_few ? std::max(sequences, ceil_div(tokens * group, 16)) : a.units) * kv_heads, little ? 256 : 768, 128, 4096);
     a.chunks = std::max<int64_t>(1, ceil_div(longest, a.chunk));
     a.wide_chunk = chunk_of(longest, a.wide_tiles * kv_heads, 512, 256, 1 << 30);
     a.wide_chunks = std::max<int64_t>(1, ceil_div(longest, a.wide_chunk));
     if (prefix) {
         a.prefix_wide = tokens * group > FEW_ROWS && pays(prefix);
         a.prefix_tiles = ceil_div(tokens * group, a.prefix_wide ? wide_tile(dim) : 16);
-        a.prefix_chunk = a.prefix_wide ? chunk_of(prefix, a.prefix_tiles * kv_heads, 512, 256, 1 << 30) : chunk_of(prefix, a.prefix_tiles * kv_heads, 1024, 128, 4096);
+        a.prefix_chunk = a.prefix_wide ? chunk_of(prefix, a.prefix_tiles * kv_heads, 512, 256, 1 << 30) : chunk_of(prefix, a.prefix_tiles * kv_heads, 384, 128, 4096);
         a.prefix_chunks = ceil_div(prefix, a.prefix_chunk);
     }
     a.few_parts = a.few && (a.chunks > 1 || prefix);
