@@ -50,7 +50,8 @@ typedef enum {
  * and their row scales), bt_ternary_linear_packed_forward uses one for small
  * batches of fp32 activations (three bf16 planes), its fused and tiled forms also
  * one for a prologue that runs as its own kernel, and bt_linear_grad_weight,
- * bt_linear_grad_weight_16 and bt_add_rmsnorm_backward one for partial sums; bt_ternary_gemm_i8 keeps the argument so that a kernel that needs
+ * bt_linear_grad_weight_16 and bt_add_rmsnorm_backward one for partial sums, bt_cached_attention
+ * one for the parts of rows whose keys several workgroups share; bt_ternary_gemm_i8 keeps the argument so that a kernel that needs
  * scratch can be introduced without an ABI change.
  */
 /* ABI version of the loaded library (BT_ABI_VERSION at build time). */
