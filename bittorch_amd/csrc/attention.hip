@@ -775,7 +775,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
                 __builtin_amdgcn_sched_barrier(0);
                 next_page();
 #pragma unroll
-                for (int t = 0; t < T; t++) base[t] = -m[t] * p.scale2;
+                for (int t = 0; t < T; t++) base[t] = m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2;  // (all its logits may be, of infinite keys)
                 unrolled(std::make_integer_sequence<int, F>(), [&](auto number) {
                     constexpr int f = decltype(number)::value;
                     __builtin_amdgcn_sched_barrier(0);

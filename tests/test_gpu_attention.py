@@ -262,6 +262,29 @@ def test_what_a_row_does_not_see_does_not_matter(dt, new, wide):
     assert bool(out[fits].isfinite().all()) and bool(fits.any())
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("new,wide", [(1, False), (200, False), (200, True)])
+def test_places_whose_logits_are_minus_infinity(dt, new, wide):
+    """Whole tiles of keys of -inf at the start, seen by all rows: their weights are zero."""
+    from bittorch_amd.ops.attention import _tiled
+    b = Batch([400], [new], 4, 2, 64, 32, dt).widened(wide)
+    kn, vn = (t.clone() for t in natural(b.k_cache, b.v_cache))
+    for place in range(130):
+        kn[int(b.table[0, place // 32]), :, place % 32, 0] = -math.inf
+    kc, vc = (t.contiguous() for t in _tiled(kn, vn))
+    q = b.q.clone()
+    q[..., 0] = q[..., 0].abs() + 0.5
+    out, lse = _ops().cached_attention(q, kc, vc, b.table, b.lengths, b.q_starts, return_lse=True)
+    k, v = (t[0][130:].repeat_interleave(2, 1) for t in (b.keys, b.values))
+    x = torch.matmul(q.double().transpose(0, 1), k.permute(1, 2, 0)) / 8
+    x = x.masked_fill(torch.arange(130, 400, device="cuda")[None] > torch.arange(400 - new, 400, device="cuda")[:, None], -math.inf)
+    p = x.softmax(-1)
+    want, spread = (torch.matmul(p, t.transpose(0, 1)).transpose(0, 1) for t in (v, v.abs()))
+    # (as Batch.check: weights and results rounded to the type once each, 256 u for the 32-bit sums and exponentials of logits below 16)
+    assert bool(((out.double() - want).abs() <= (_half(dt) * 2 + 256 * 16 * U) * spread + _half(dt) * want.abs()).all())
+    assert bool(((lse.double() - x.logsumexp(-1).T).abs() <= 256 * 16 * U).all())
+
+
 def test_lengths_pages_and_rows_that_are_not_there():
     ops = _ops()
     b = Batch([70, 10, 33], [1, 1, 1], 4, 2, 64, 32, torch.bfloat16, width=4)
