@@ -185,7 +185,8 @@ def cache_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block_t
     ``inv_freq`` the keys are turned as in :func:`rotary`, at position ``first_position`` (a shared prefix's length) plus their place, and so is ``q``
     ``[tokens, heads, D]``, which is returned (None without).  ``k``, ``v`` and ``q`` may be views of one projection's output.
 
-    Places below 0, behind ``block_table`` and on pages outside the cache are not written; rows of the result behind the last sequence are zero.  No gradient.
+    Places below 0, behind ``block_table`` and on pages outside the cache are not written; of two tokens that the tables send to one place
+    either stays; rows of the result behind the last sequence are zero.  No gradient.
     On the CPU: the same in plain torch operations."""
     from .. import _C
 

@@ -198,7 +198,7 @@ class BlockStack:
         make = lambda: ops.paged_cache(sequences * width + shared, self.heads, self.d_model // self.heads, page_size, self.act_dtype, dev)  # noqa: E731
         pages = torch.arange(sequences * width + shared, dtype=torch.int32, device=dev)
         self.cache = dict(layers=[make() for _ in self.infer], prefix_table=pages[:shared], prefix_length=0,
-                          table=pages[shared:].view(sequences, width), lengths=torch.zeros(sequences, dtype=torch.int32, device=dev))
+                          table=pages[shared:].view(sequences, width), lengths=torch.zeros(sequences, dtype=torch.int32, device=dev), begun=False)
 
     def _cached(self, tokens, table, lengths, q_starts, int8, first, **prefix):
         torch, ops = self.torch, self.bt.ops
@@ -220,8 +220,10 @@ class BlockStack:
     def forward_prefix(self, tokens, int8=False):
         """The tokens (1D) that all sequences share, once, at the start of the caches; their hidden states."""
         c, n = self.cache, tokens.numel()
-        if c["prefix_length"] or n > c["prefix_table"].numel() * c["layers"][0][0].shape[2]:
-            raise RuntimeError("the prefix is there already, or longer than start_cache was told")
+        if c is None:
+            raise RuntimeError("start_cache comes first")
+        if c["prefix_length"] or c["begun"] or n > c["prefix_table"].numel() * c["layers"][0][0].shape[2]:
+            raise RuntimeError("the prefix or tokens behind it are there already, or it is longer than start_cache was told")
         c["prefix_length"] = n
         at = lambda *v: self.torch.tensor(v, dtype=self.torch.int32, device=tokens.device)  # noqa: E731
         return self._cached(tokens, c["prefix_table"][None], at(n), at(0, n), int8, 0)
@@ -231,6 +233,12 @@ class BlockStack:
         hidden states (tokens, d_model).  The caches' lengths follow on the GPU, so that a step of one token each can be captured; more tokens than
         ``start_cache`` was told are not stored, and their sequences are not a number from then on."""
         c = self.cache
+        if c is None:
+            raise RuntimeError("start_cache comes first")
+        n = c["lengths"].numel()
+        if tokens.numel() != n if q_starts is None else q_starts.shape != (n + 1,):
+            raise RuntimeError(f"{n} sequences need a token each, or {n + 1} q_starts")
+        c["begun"] = True
         c["lengths"] += 1 if q_starts is None else q_starts[1:] - q_starts[:-1]
         return self._cached(tokens, c["table"], c["lengths"], q_starts, int8, c["prefix_length"],
                             prefix_table=c["prefix_table"] if c["prefix_length"] else None, prefix_length=c["prefix_length"])

@@ -561,7 +561,7 @@ int bt_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int
  * features of the keys behind head_dim are zero (bt_cache_append writes them too).
  * Sequence s owns the pages block_table[s][0 .. table_width) (int32) and lengths[s] places in them, its new tokens included, which are the
  * last; they are the rows q_starts[s] .. q_starts[s + 1] - 1 of k, v and q.  q_starts (sequences + 1 entries, from 0, ascending) NULL: one
- * token a sequence.  Entries of the table behind the places in use are not read.
+ * token a sequence.  Entries of the table behind the places in use do not matter.
  *   bt_cache_append: writes the new tokens' keys, turned as bt_rotary does at position first_position + place, and values; q (or NULL)
  *     turned likewise goes to q_out, contiguous; rows of q_out behind the last sequence are cleared.  rotary_dim 0: as they are.  Places
  *     below 0, behind the table and on pages that the cache does not have are not written.

@@ -117,3 +117,22 @@ def test_training_variants_agree(rotary_dim):
     c5.convert(inplace=False)
     c5.fuse()
     assert _rel(c5.forward_fused(False), plain) < 1e-4
+
+
+def test_refused_steps_leave_the_caches_as_they_are():
+    c5 = _stack(32)
+    c5.convert()
+    c5.fuse()
+    for call in (c5.forward_prefix, c5.forward_cached):
+        with pytest.raises(RuntimeError, match="start_cache"):
+            call(c5.tokens[:, 0].contiguous())
+    c5.start_cache(3, 15, prefix=25, page_size=32)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for args in ((c5.tokens[:2, 0].contiguous(),), (c5.tokens[0, :2].contiguous(), starts)):
+        with pytest.raises(RuntimeError, match="3 sequences"):
+            c5.forward_cached(*args)
+    assert not c5.cache["lengths"].any()
+    c5.forward_cached(c5.tokens[:, 0].contiguous())
+    with pytest.raises(RuntimeError, match="prefix"):  # (the tokens behind it would move)
+        c5.forward_prefix(c5.tokens[0, :9])
+    assert c5.cache["lengths"].tolist() == [1, 1, 1]
