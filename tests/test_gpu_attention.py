@@ -564,6 +564,50 @@ def test_captured_calls_follow_lengths_and_tables():
             lengths += 1
 
 
+@pytest.mark.parametrize("wide", [False, True])
+def test_captured_prompts_follow_tokens_and_lengths(wide):
+    """Rows of both kernels, a prefix and its parts in two graphs, replayed in turn and on two streams at once, eager calls between."""
+    b = Batch([300, 90, 200, 33], [150, 70, 3, 1], 4, 2, 64, 32, torch.bfloat16, 70).widened(wide)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        b.attend(return_lse=True)
+    torch.cuda.current_stream().wait_stream(warm)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(b.attend(return_lse=True))
+    for i in range(5):
+        b.q.copy_(torch.randn(b.q.shape, device="cuda"))
+        if i == 2:
+            b.lengths -= 30  # (the third sequence's tokens move up, the last has fewer places than a tile)
+        want = b.attend(return_lse=True)
+        if i < 4:
+            graphs[i % 2].replay()
+            got = [outs[i % 2]]
+        else:
+            warm.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(warm):
+                graphs[0].replay()
+            graphs[1].replay()
+            torch.cuda.current_stream().wait_stream(warm)
+            got = outs
+        torch.cuda.synchronize()
+        for g in got:
+            assert torch.equal(g[0], want[0]) and torch.equal(g[1], want[1]), i
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("page", [4096, 65536])
+def test_pages_longer_than_chunks(dt, page, wide):
+    announce("attend long pages", dt, page, wide)
+    b = Batch([5000, 300], [150, 40], 4, 2, 64, page, dt, 4500).widened(wide)
+    b.check(*b.attend(return_lse=True))
+    one = Batch([70000, 300], [1, 1], 8, 2, 64, page, dt, 100)
+    one.check(*one.attend(starts=False, return_lse=True))
+
+
 def test_calls_made_in_python_give_the_same(monkeypatch):
     """The native host side and the Python functions it stands in for."""
     from bittorch_amd import _C, _lib
