@@ -1093,6 +1093,9 @@ static AttendPlan attend_plan(int dt, bool q_in_place, int64_t tokens, int64_t h
     const bool little = (double)sequences * kv_heads * longest * dim * 2 * dtype_size(dt) < (64 << 20);
     a.chunk = longest <= 512 && !prefix ? 512
                                         : chunk_of(longest, (a.all_few ? std::max(sequences, ceil_div(tokens * group, 16)) : a.units) * kv_heads, little ? 256 : 768, 128, 4096);
+    // (parts of a GiB at most: so many rows fill the chip with longer chunks as well)
+    const int64_t few_rows_all = a.all_few ? tokens * heads : sequences * kv_heads * a.few_slots;
+    while (a.chunk < longest && (double)few_rows_all * ceil_div(longest, a.chunk) * part_stride((int)dim) * 4 > (1 << 30)) a.chunk *= 2;
     a.chunks = std::max<int64_t>(1, ceil_div(longest, a.chunk));
     a.wide_chunk = chunk_of(longest, a.wide_tiles * kv_heads, 512, 256, 1 << 30);
     a.wide_chunks = std::max<int64_t>(1, ceil_div(longest, a.wide_chunk));
@@ -1111,7 +1114,7 @@ static AttendPlan attend_plan(int dt, bool q_in_place, int64_t tokens, int64_t h
         r.o = a.bytes, a.bytes += (size_t)round_up(r.rows * slots * part_stride((int)dim) * 4, 256);
         return r;
     };
-    a.few_region = region(a.few_parts, a.all_few ? tokens * heads : sequences * kv_heads * a.few_slots, a.chunks);
+    a.few_region = region(a.few_parts, few_rows_all, a.chunks);
     a.wide_region = region(a.wide_parts, tokens * heads, a.wide_chunks);
     a.prefix_region = region(prefix > 0, tokens * heads, a.prefix_chunks);
     a.q_copy = a.bytes;

@@ -213,3 +213,13 @@ def test_native_calls_leave_cpu_tensors_to_python():
     assert n.cached_attention(a["q"], *a["cache"], a["table"], a["lengths"], None, None, None, 0, False, None) is None
     for f in (n.rotary, n.cache_append, n.cached_attention):
         assert f() is None and f(*(None,) * 6) is None
+
+
+def test_workspaces_of_many_sequences_on_wide_tables():
+    """Parts that few rows leave take a GiB at most, however many places the table may hold."""
+    lib = _lib.load()
+    for sequences in (1, 100, 3000, 50000):
+        for starts, tokens in ((0, sequences), (1, 2 * sequences)):
+            need = lib.bt_cached_attention_workspace_bytes(_C._DT[torch.bfloat16], 1, tokens, 32, 8, 128, 64, 4096, 4096 * 64, starts, sequences, 0)
+            many = tokens * 32 * (128 * 4 + 8) * 2  # (those of rows by token and head: two chunks of the least workgroups)
+            assert need <= 2 ** 30 * 1.02 + max(many, 2 ** 27), (sequences, starts, need)

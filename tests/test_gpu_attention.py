@@ -597,6 +597,14 @@ def test_captured_prompts_follow_tokens_and_lengths(wide):
             assert torch.equal(g[0], want[0]) and torch.equal(g[1], want[1]), i
 
 
+def test_many_sequences_on_a_wide_table():
+    """So many that their parts would take more than a GiB in chunks of the usual length."""
+    held = [20, 1, 32, 7] * 600
+    held[5], held[2399] = 20000, 9000
+    b = Batch(held, [1] * 2400, 2, 2, 128, 32, torch.bfloat16, width=4096)
+    b.check(*b.attend(return_lse=True))
+
+
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("page", [4096, 65536])
