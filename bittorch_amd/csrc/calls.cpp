@@ -852,7 +852,7 @@ PyObject* gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 
 // ---- positions, the paged cache and the attention over it ------------------------------------------------------------------
 
-// [tokens][heads][dim] with a stride for each of the first two
+// [tokens][heads][dim] with a stride for each of the first two.  A dimension of one entry may have any stride, in contiguous memory too.
 struct HeadRows {
     const void* data = nullptr;
     int64_t tokens = 0, heads = 0, dim = 0, token = 0, head = 0;
@@ -860,9 +860,11 @@ struct HeadRows {
 bool head_rows(const at::Tensor& t, HeadRows* r) {
     const int64_t d = t.dim();
     if (d < 2 || tag(t.scalar_type()) < 0 || (t.stride(-1) != 1 && t.size(-1) != 1)) return false;
-    *r = {t.const_data_ptr(), 1, t.size(-2), t.size(-1), d > 2 ? t.stride(-3) : 0, t.stride(-2)};
+    *r = {t.const_data_ptr(), 1, t.size(-2), t.size(-1), 0, t.stride(-2)};
     for (int64_t i = d - 3; i >= 0; i--) {
-        if (i < d - 3 && t.stride(i) != t.stride(i + 1) * t.size(i + 1)) return false;
+        if (t.size(i) == 1) continue;
+        if (r->tokens == 1) r->token = t.stride(i);
+        else if (t.stride(i) != r->token * r->tokens) return false;
         r->tokens *= t.size(i);
     }
     return true;
@@ -934,7 +936,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
             for (int i = first; i < 2; i++)
                 if (d[i].defined() && !head_rows(d[i], &r[i])) {
                     d[i] = d[i].contiguous();
-                    head_rows(d[i], &r[i]);
+                    TORCH_CHECK(head_rows(d[i], &r[i]), "rotary: a gradient of ", d[i].sizes(), " is not rows of heads");
                 }
             const bool both = first == 0 && d[1].defined();
             Turned o = rotary_run<false>(d[first], r[first], both ? &d[1] : nullptr, both ? r[1] : HeadRows(), saved[0], saved[1], interleaved, amplitude, true);
