@@ -472,6 +472,7 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
             for (int e = 0; e < 4; e++) o[b][e] = nan >> (4 * b + e) & 1 ? __builtin_nanf("") : o[b][e];
     }
     l = over_groups_sum(l);
+    if (pages.bad) l = __builtin_nanf("");  // (a wave knows of the pages that it had a tile on: the sum over the waves tells all)
 
     // the four waves' shares of every row
     if (g == 0) m_all[wave][r] = m, l_all[wave][r] = l;
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
                 const v4f ow = *(const v4f*)&o_all[w][row_at * LD + at];
                 acc += ow * share;
             }
-            put_row<DT>(p, j, row_at, f, acc, top, pages.bad ? __builtin_nanf("") : sum);
+            put_row<DT>(p, j, row_at, f, acc, top, sum);
         }
     }
 }

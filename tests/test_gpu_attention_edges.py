@@ -1,0 +1,47 @@
+"""``ops.cached_attention`` on the GPU where a rule of its kernels ends: pages outside the cache behind many others, weights far below a row's
+largest, logits and scales at the ends of 32 bits."""
+import math
+
+import pytest
+import torch
+
+from conftest import announce
+from test_gpu_attention import Batch, _ops
+from test_gpu_rotary import U, _half
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("held", [2049, 2090, 2120, 2140])
+def test_a_page_outside_the_cache_behind_64_others(dt, held):
+    """The 65th page of a chunk and the 66th, with so few tiles behind the 64th that not every wave of a workgroup has one: all of the sequence's rows are not a
+    number, the other sequences' as they were.  (101 sequences of 8 key heads: a chunk holds a whole sequence.)"""
+    announce("bad page", held, dt)
+    b = Batch([held] + [5, 40] * 50, [1] * 101, 32, 8, 128, 32, dt, width=72)
+    want, want_lse = b.attend(starts=False, return_lse=True)
+    b.check(want, want_lse)
+    good = b.table
+    for column in range(64, -(-held // 32)):
+        for wrong in (-1, b.k_cache.shape[0]):
+            b.table = good.clone()
+            b.table[0, column] = wrong
+            for starts in (False, True):
+                out, lse = b.attend(starts=starts, return_lse=True)
+                assert out[0].isnan().all() and lse[0].isnan().all(), (column, starts)
+                assert torch.equal(out[1:], want[1:]) and torch.equal(lse[1:], want_lse[1:])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("prefix", [2049, 2090])
+def test_a_prefix_page_outside_the_cache_behind_64_others(dt, prefix):
+    """200 rows tokens of 4 heads a group and 8 key heads: a workgroup sees the whole prefix."""
+    announce("bad prefix page", prefix, dt)
+    b = Batch([30] * 200, [1] * 200, 32, 8, 64, 32, dt, prefix)
+    b.check(*b.attend(starts=False, return_lse=True))
+    b.prefix_table = b.prefix_table.clone()
+    b.prefix_table[64] = -1
+    for starts in (False, True):
+        out, lse = b.attend(starts=starts, return_lse=True)
+        assert out.isnan().all() and lse.isnan().all()
