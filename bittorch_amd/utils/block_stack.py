@@ -38,9 +38,17 @@ class BlockStack:
         self.d_model, self.heads, self.ffn = d_model, heads, ffn
         act_dtype = act_dtype or torch.bfloat16
         self.act_dtype = act_dtype
-        self.inv_freq = bt.ops.rotary_frequencies(rotary_dim, device=dev)[0] if rotary_dim else None
+        self.inv_freq = inv_freq = bt.ops.rotary_frequencies(rotary_dim, device=dev)[0] if rotary_dim else None
         self.cache = None
-        turned = self._turned
+
+        def turned(q, k):
+            """Queries and keys (batch, seq, heads, head_dim) by their places in the sequence.  (It knows nothing of the stack: the blocks hold
+            it, and a stack that they held would outlive its last reference with all of its weights.)"""
+            if inv_freq is None:
+                return q, k
+            return bt.ops.rotary(q, k, torch.arange(q.shape[1], device=q.device), inv_freq)
+
+        self._turned = turned
 
         def fq(t):
             """fake_quant: the int8 path's per-token activation quantizer (whole-row absmax / 127, halves away
@@ -86,12 +94,6 @@ class BlockStack:
         self.tokens = torch.randint(0, vocab, (batch, seq), generator=torch.Generator().manual_seed(0)).to(dev)
         self.n_tern = sum(m.weight.numel() for m in self.blocks.modules() if isinstance(m, bt.nn.TernaryLinear))
         self.infer = None
-
-    def _turned(self, q, k):
-        """Queries and keys (batch, seq, heads, head_dim) by their places in the sequence."""
-        if self.inv_freq is None:
-            return q, k
-        return self.bt.ops.rotary(q, k, self.torch.arange(q.shape[1], device=q.device), self.inv_freq)
 
     def forward(self, stack=None):
         """Unfused forward of `stack` (the training modules by default, or the converted modules)."""
