@@ -226,9 +226,12 @@ class BlockStack:
             raise RuntimeError("start_cache comes first")
         if c["prefix_length"] or c["begun"] or n > c["prefix_table"].numel() * c["layers"][0][0].shape[2]:
             raise RuntimeError("the prefix or tokens behind it are there already, or it is longer than start_cache was told")
-        c["prefix_length"] = n
+        if not n:
+            raise RuntimeError("a prefix has tokens")
         at = lambda *v: self.torch.tensor(v, dtype=self.torch.int32, device=tokens.device)  # noqa: E731
-        return self._cached(tokens, c["prefix_table"][None], at(n), at(0, n), int8, 0)
+        out = self._cached(tokens, c["prefix_table"][None], at(n), at(0, n), int8, 0)
+        c["prefix_length"] = n
+        return out
 
     def forward_cached(self, tokens, q_starts=None, int8=False):
         """The converted, fused stack on the sequences' next tokens (1D): one each, or ``q_starts[s] .. q_starts[s + 1] - 1`` of sequence s (int32);
@@ -240,7 +243,10 @@ class BlockStack:
         n = c["lengths"].numel()
         if tokens.numel() != n if q_starts is None else q_starts.shape != (n + 1,):
             raise RuntimeError(f"{n} sequences need a token each, or {n + 1} q_starts")
+        # (the counts follow the step: one that is refused can be made again, put right)
+        lengths = c["lengths"] + (1 if q_starts is None else q_starts[1:] - q_starts[:-1])
+        out = self._cached(tokens, c["table"], lengths, q_starts, int8, c["prefix_length"],
+                           prefix_table=c["prefix_table"] if c["prefix_length"] else None, prefix_length=c["prefix_length"])
+        c["lengths"].copy_(lengths)
         c["begun"] = True
-        c["lengths"] += 1 if q_starts is None else q_starts[1:] - q_starts[:-1]
-        return self._cached(tokens, c["table"], c["lengths"], q_starts, int8, c["prefix_length"],
-                            prefix_table=c["prefix_table"] if c["prefix_length"] else None, prefix_length=c["prefix_length"])
+        return out

@@ -31,3 +31,52 @@ def test_a_stack_is_freed_without_the_collector(rotary_dim, converted):
         assert not any(r() is not None for r in alive)
     finally:
         gc.enable()
+
+
+def test_a_step_that_fails_leaves_the_caches_as_they_are(monkeypatch):
+    """Whatever it fails of, behind the checks of its arguments."""
+    stack = _stack(rotary_dim=8)
+    stack.convert()
+    stack.fuse()
+    stack.start_cache(2, 8, prefix=4)
+    seen = []
+
+    def fails(tokens, table, lengths, *more, **prefix):
+        seen.append(lengths.tolist())
+        raise RuntimeError("refused")
+
+    def passes(tokens, table, lengths, *more, **prefix):
+        seen.append(lengths.tolist())
+        return torch.zeros(tokens.numel(), 32)
+
+    state = lambda: (stack.cache["lengths"].tolist(), stack.cache["prefix_length"], stack.cache["begun"])  # noqa: E731
+    counts = stack.cache["lengths"]
+    starts = torch.tensor([0, 2, 3], dtype=torch.int32)
+    for _ in range(2):
+        monkeypatch.setattr(stack, "_cached", fails)
+        with pytest.raises(RuntimeError, match="refused"):
+            stack.forward_prefix(torch.zeros(3, dtype=torch.int64))
+        assert state() == ([0, 0], 0, False)
+        with pytest.raises(RuntimeError, match="refused"):
+            stack.forward_cached(torch.zeros(2, dtype=torch.int64))
+        assert state() == ([0, 0], 0, False)
+    monkeypatch.setattr(stack, "_cached", passes)
+    stack.forward_prefix(torch.zeros(3, dtype=torch.int64))
+    assert state() == ([0, 0], 3, False)
+    stack.forward_cached(torch.zeros(3, dtype=torch.int64), starts)
+    assert state() == ([2, 1], 3, True) and stack.cache["lengths"] is counts
+    monkeypatch.setattr(stack, "_cached", fails)
+    with pytest.raises(RuntimeError, match="refused"):
+        stack.forward_cached(torch.zeros(3, dtype=torch.int64), starts)
+    assert state() == ([2, 1], 3, True)
+    assert seen == [[3], [1, 1]] * 2 + [[3], [2, 1], [4, 2]]
+
+
+def test_a_prefix_has_tokens():
+    stack = _stack()
+    stack.convert()
+    stack.fuse()
+    stack.start_cache(2, 8, prefix=4)
+    with pytest.raises(RuntimeError, match="prefix"):
+        stack.forward_prefix(torch.zeros(0, dtype=torch.int64))
+    assert stack.cache["prefix_length"] == 0
