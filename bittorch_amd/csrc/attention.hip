@@ -665,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     float m[T], l[T], top[T];   // the rows' maxima (of the products before they are scaled), sums and s's maxima (of this lane's places)
     u32x4 w[T][W];              // weights of the tile before
     std::conditional_t<(BIG || V > 8), uint64_t, uint32_t> nan[T];  // elements e of accumulator b of the sums, bit AE b + e, that saw a value that is no number
-    const float slack = 8.0f / p.scale2;
+    const float slack = std::min(8.0f / p.scale2, 3.4e38f);  // (infinite, the maximum would never leave minus infinity)
     // The multiply-add rounds once, the base alone too: logits of a size at which that is more than a part of one are rounded alike first.
     bool large = false;
 #pragma unroll

@@ -45,3 +45,14 @@ def test_a_prefix_page_outside_the_cache_behind_64_others(dt, prefix):
     for starts in (False, True):
         out, lse = b.attend(starts=starts, return_lse=True)
         assert out.isnan().all() and lse.isnan().all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("new,wide", [(1, False), (40, True)])
+def test_the_smallest_scales(dt, new, wide):
+    """All logits next to zero: means of the values, and the logarithm of the number of places."""
+    announce("smallest scale", new, wide, dt)
+    b = Batch([400], [new], 2, 1, 32, 32, dt).widened(wide)
+    for scale in (1e-30, 1e-38):
+        out, lse = b.attend(return_lse=True, scale=scale)
+        b.check(out, lse, scale=scale)
