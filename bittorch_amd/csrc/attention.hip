@@ -720,10 +720,10 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
             l[t] += sum;
         }
     };
-    auto over = [&]() {
+    auto over = [&](float by) {
         bool any = false;
 #pragma unroll
-        for (int t = 0; t < T; t++) any |= top[t] > m[t] + slack;
+        for (int t = 0; t < T; t++) any |= top[t] > m[t] + by;
         return __any(any);
     };
     float shrink[T];
@@ -765,7 +765,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
         if (i > 0 && i < whole && !large) {
             maxima();
             for (; i < whole; i++) {
-                raised = over();
+                raised = over(slack);
                 if (raised) raise();
                 if (large) break;  // (before this tile's weights)
                 turn();
@@ -889,7 +889,8 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
             float owed[T];
 #pragma unroll
             for (int t = 0; t < T; t++) owed[t] = raised ? shrink[t] : 1.0f;
-            if (over() || raised) {
+            // (large logits step by more than the slack: a weight one step above it could pass what fp16 holds)
+            if (over(large ? 0.0f : slack) || raised) {
                 raise();
 #pragma unroll
                 for (int t = 0; t < T; t++) shrink[t] *= owed[t];

@@ -13,6 +13,18 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 
+def _set_keys(b, keys, values=None):
+    """The one sequence's keys [places, dim] of every key head (and values), in the caches' order."""
+    from bittorch_amd.ops.attention import _natural, _tiled
+    kn, vn = (t.clone() for t in _natural(b.k_cache, b.v_cache))
+    places = torch.arange(keys.shape[0], device="cuda")
+    number, at = b.table[0][places // b.page].long(), places % b.page
+    kn[number, :, at, :b.dim] = keys.to(b.dt)[:, None]
+    if values is not None:
+        vn[number, :, at, :b.dim] = values.to(b.dt)[:, None]
+    b.k_cache, b.v_cache = (t.contiguous() for t in _tiled(kn, vn))
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("held", [2049, 2090, 2120, 2140])
 def test_a_page_outside_the_cache_behind_64_others(dt, held):
@@ -56,3 +68,21 @@ def test_the_smallest_scales(dt, new, wide):
     for scale in (1e-30, 1e-38):
         out, lse = b.attend(return_lse=True, scale=scale)
         b.check(out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("new,wide", [(1, False), (40, False), (40, True), (300, True)])
+def test_logits_beyond_10_to_the_8(dt, new, wide):
+    """Logits near 1.2e8, where 32 bits step by 8 and a weight's exponent by 16: what they make of it, results are means of the values."""
+    announce("large logits", new, wide, dt)
+    b = Batch([400], [new], 2, 1, 32, 32, dt).widened(wide)
+    keys = torch.zeros(400, 32, device="cuda")
+    keys[:, 0] = 58000.0 if dt != torch.bfloat16 else 57344.0
+    keys[50:, 1] = 8.0
+    values = torch.ones(400, 32, device="cuda")
+    _set_keys(b, keys, values)
+    b.q.zero_()
+    b.q[..., 0], b.q[..., 1] = 2048.0, 1.0
+    out = b.attend(scale=1.0)
+    # (equal values: weights over their sum, whatever they are, rounded once each)
+    assert bool(((out.double() - 1).abs() <= 3 * _half(dt) + 512 * U).all()), out.double().flatten()[:3]
