@@ -95,6 +95,13 @@ __device__ __forceinline__ u32x4 first_places(u32x4 v, int live) {
     }
     return v;
 }
+// fp16 weights are kept times 2^LIFT until they are summed up: as they are, those below 2^-14 of a row's largest would lose bits to fp16's
+// exponent and those below 2^-25 everything, and 65536 of them have a share of 2 / 1000.  SLACK: a weight is 2^SLACK at most before.
+template <int DT, int SLACK>
+struct Lift {
+    static constexpr int LIFT = DT == BT_F16 ? 15 - SLACK : 0;
+    static constexpr float DOWN = 1.0f / (1 << LIFT);
+};
 template <int DT>
 __device__ __forceinline__ bool any_special(u32x4 v) {  // infinite or not a number
     bool s = false;
@@ -435,7 +442,9 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
         float w[E];
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            w[e] = __builtin_amdgcn_exp2f(x[e] - base);
+            float exponent = x[e] - base;  // (the difference first: it is exact where logits are large)
+            if constexpr (Lift<DT, 0>::LIFT != 0) exponent += (float)Lift<DT, 0>::LIFT;
+            w[e] = __builtin_amdgcn_exp2f(exponent);
             l += w[e];
         }
         u32x4 lo;
@@ -494,7 +503,7 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
             v4f acc = {0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-                const float share = __builtin_amdgcn_exp2f(m_all[w][row_at] - base);
+                const float share = __builtin_amdgcn_exp2f(m_all[w][row_at] - base) * Lift<DT, 0>::DOWN;
                 sum += share * l_all[w][row_at];
                 const v4f ow = *(const v4f*)&o_all[w][row_at * LD + at];
                 acc += ow * share;
@@ -519,8 +528,9 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
 //
 // The maximum is that of the products before they are scaled, and one multiply-add and the exponential make a weight.  It is raised only where a
 // weight would pass 2^8: it needs to be near the true maximum, not to be it.  16-bit weights are rounded once (the rows kernel's two halves
-// would be half as many matrix instructions again): results are 1.4 times as far from 64 bits as by their own rounding.  Their sum is that of
-// the weights before they are rounded, as lse wants it.
+// would be half as many matrix instructions again): results are 1.4 times as far from 64 bits as by their own rounding, and fp16 ones by up to
+// 2^-32 of the row's largest value a place besides (struct Lift; the rows kernel 2^-40).  Their sum is that of the weights before they are
+// rounded, as lse wants it.
 // The tile of the unit'th workgroup of a key head: sequences by their length, their last rows first, and of the first 2 x CUs workgroups, two of
 // which share a compute unit and its LDS, the second ones from the light end (4 x 512 tokens on 1600 to 4000 places 138 -> 120 us).
 __device__ __forceinline__ bool heaviest_first(const AttendParams& p, int R, uint32_t unit, int* s, int* tile) {
@@ -665,7 +675,9 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
     float m[T], l[T], top[T];   // the rows' maxima (of the products before they are scaled), sums and s's maxima (of this lane's places)
     u32x4 w[T][W];              // weights of the tile before
     std::conditional_t<(BIG || V > 8), uint64_t, uint32_t> nan[T];  // elements e of accumulator b of the sums, bit AE b + e, that saw a value that is no number
-    const float slack = std::min(8.0f / p.scale2, 3.4e38f);  // (infinite, the maximum would never leave minus infinity)
+    constexpr int SLACK = 8;
+    using Lifted = Lift<DT, SLACK>;
+    const float slack = std::min((float)SLACK / p.scale2, 3.4e38f);  // (infinite, the maximum would never leave minus infinity)
     // The multiply-add rounds once, the base alone too: logits of a size at which that is more than a part of one are rounded alike first.
     bool large = false;
 #pragma unroll
@@ -719,6 +731,11 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
             }
             l[t] += sum;
         }
+    };
+    // of the row's weights as exponents; all its logits may be minus infinity, of infinite keys
+    auto base_of = [&](int t) {
+        if constexpr (Lifted::LIFT) return __builtin_fmaf(m[t] == -__builtin_inff() ? 0.0f : -m[t], p.scale2, (float)Lifted::LIFT);
+        else return m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2;
     };
     auto over = [&](float by) {
         bool any = false;
@@ -781,7 +798,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
                 __builtin_amdgcn_sched_barrier(0);
                 next_page();
 #pragma unroll
-                for (int t = 0; t < T; t++) base[t] = m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2;  // (all its logits may be, of infinite keys)
+                for (int t = 0; t < T; t++) base[t] = base_of(t);
                 unrolled(std::make_integer_sequence<int, F>(), [&](auto number) {
                     constexpr int f = decltype(number)::value;
                     __builtin_amdgcn_sched_barrier(0);
@@ -897,14 +914,13 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
                 if (i) shrink_sums();
             }
             raised = false;
-            auto base_of = [&](int t) { return m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2; };
             if (large) {
 #pragma unroll
                 for (int t = 0; t < T; t++)
 #pragma unroll
-                    for (int e = 0; e < EL; e++) s[t][e / AE][e % AE] = s[t][e / AE][e % AE] * p.scale2 + base_of(t);
+                    for (int e = 0; e < EL; e++) s[t][e / AE][e % AE] = s[t][e / AE][e % AE] * p.scale2 + (m[t] == -__builtin_inff() ? 0.0f : -m[t] * p.scale2);
             }
-            weights(large ? 1.0f : p.scale2, [&](int t) { return large ? 0.0f : base_of(t); });
+            weights(large ? 1.0f : p.scale2, [&](int t) { return large ? (float)Lifted::LIFT : base_of(t); });
             products(keys_at(i + 1), s);
         }
         i++;
@@ -952,7 +968,7 @@ __global__ __launch_bounds__(256, 2) void attend_tiles_kernel(AttendParams p) {
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] = bits >> e & 1 ? __builtin_nanf("") : acc[e];
             const int at = mine + t0 * ROWS + row;
-            if (at < j.rows && f < p.dim) put_row<DT>(p, j, at, f, acc, row_most, row_sum);
+            if (at < j.rows && f < p.dim) put_row<DT>(p, j, at, f, acc * Lifted::DOWN, row_most, row_sum * Lifted::DOWN);
         }
         __builtin_amdgcn_wave_barrier();
     }

@@ -86,3 +86,32 @@ def test_logits_beyond_10_to_the_8(dt, new, wide):
     out = b.attend(scale=1.0)
     # (equal values: weights over their sum, whatever they are, rounded once each)
     assert bool(((out.double() - 1).abs() <= 3 * _half(dt) + 512 * U).all()), out.double().flatten()[:3]
+
+
+@pytest.mark.parametrize("above", [15.0, 17.5])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("new,wide", [(1, False), (40, False), (40, True), (300, True)])
+def test_one_key_far_above_many(dt, new, wide, above):
+    """One key 15 or 17.5 above 20000 others, whose weights of 2^-21.6 or 2^-25.2 have 6e-3 or 5e-4 of the sum together: a value that they alone hold comes out
+    to the type's precision.  The logits are exact, so every weight is the exponential of one number: 4 u, its argument of up to 26 rounds twice (52 u), and the
+    sums have as many additions as there are keys and a few dozen where parts are joined; weights and result are rounded to the type once each, fp16 weights by
+    2^-32 of a row's largest at least where rows are taken as many, by 2^-40 where they are not."""
+    announce("far above", new, wide, above, dt)
+    held = 20000
+    b = Batch([held], [new], 2, 1, 32, 64, dt).widened(wide)
+    keys, values = torch.zeros(held, 32, device="cuda"), torch.zeros(held, 32, device="cuda")
+    keys[0, 0] = above
+    values[0, 1], values[1:, 0], values[1:, 2] = 1, 1, torch.arange(1, held, device="cuda") % 2
+    _set_keys(b, keys, values)
+    b.q.zero_()
+    b.q[..., 0] = 1
+    out, lse = b.attend(return_lse=True, scale=1.0)
+    others = (held - new + torch.arange(new, device="cuda")).double()[:, None]     # seen besides the first
+    total = math.exp(above) + others
+    off = (held + 64 + 56) * U
+    for f, want in ((0, others / total), (1, math.exp(above) / total), (2, (others / 2).ceil() / total)):
+        floor = held * 2.0 ** (-32 if wide else -40) if dt == torch.float16 else 0.0
+        bound = (want * (2 * off + _half(dt)) + floor) * (1 + _half(dt)) + want * _half(dt)
+        assert bool(((out[..., f].double() - want).abs() <= bound).all()), (f, float(((out[..., f].double() - want).abs() / want).max()))
+    assert not out[..., 3:].any()
+    assert bool(((lse.double() - total.log()).abs() <= off + 4 * U * 18).all())
