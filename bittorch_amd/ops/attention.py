@@ -221,8 +221,9 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: T
     all sequences share, and over the places of their own sequence up to their own; head ``h`` reads key head ``h // (heads / kv_heads)``.  ``scale``:
     ``D ** -0.5``.  The result is ``[tokens, heads, D]``; with ``return_lse`` the logarithms of the sums of exponentials follow, fp32 ``[tokens, heads]``.
 
-    Tokens without a place to see, and rows behind the last sequence, are zero (``-inf``).  Places that a token does not see do not change its result, whatever
-    they hold.  ``max_length``, if given, bounds the sequences' lengths on the host, where ``block_table`` is much wider than they are; tokens of longer sequences, and
+    Tokens without a place to see, and rows behind the last sequence, are zero (``-inf``), and so are heads whose logits are all minus infinity; a logit of plus
+    infinity, or one that is no number, makes the head not a number, an infinite value that it sees that feature infinite or not a number.  Places that a token does
+    not see do not change its result, whatever they hold.  ``max_length``, if given, bounds the sequences' lengths on the host, where ``block_table`` is much wider than they are; tokens of longer sequences, and
     tokens that see a page outside the cache (others of that sequence may be), are not a number.  All sums in 32 bits.  No gradient.  On the CPU: the same in plain torch operations."""
     from .. import _C
 
@@ -252,6 +253,8 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: T
                 continue
             k, v = (t[:seen].float().repeat_interleave(heads // kv_heads, 1) for t in own)
             x = torch.einsum("hd,khd->hk", q[begin + i].float(), k) * scale
-            lse[begin + i] = math.nan if bad else x.logsumexp(-1)
-            out[begin + i] = math.nan if bad else torch.einsum("hk,khd->hd", x.softmax(-1), v).to(q.dtype)
+            sums = x.logsumexp(-1).masked_fill((x == math.inf).any(-1), math.nan)
+            weights = x.softmax(-1).masked_fill((sums == -math.inf)[:, None], 0.0)
+            lse[begin + i] = math.nan if bad else sums
+            out[begin + i] = math.nan if bad else torch.einsum("hk,khd->hd", weights, v).to(q.dtype)
     return (out, lse) if return_lse else out

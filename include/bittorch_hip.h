@@ -570,7 +570,9 @@ int bt_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int
  *     [tokens][heads]: the logarithm of the sum of exponentials.  No places at all, and rows behind the last sequence: zeros, and -inf.  The rows of
  *     sequences with more than max_length (<= table_width * page_size) places, and rows that see a page outside the cache (others of the
  *     sequence may be), are not a number.
- *     Places that a row does not see do not change it, whatever they hold.  workspace: bt_cached_attention_workspace_bytes, where q_in_place
+ *     Places that a row does not see do not change it, whatever they hold.  Logits that are all minus infinity make a row of zeros, and -inf; one
+ *     of plus infinity, or that is no number, one that is not a number; an infinite value that a row sees makes its feature infinite or not a
+ *     number.  workspace: bt_cached_attention_workspace_bytes, where q_in_place
  *     says that q, its strides and its heads start and end on 16 bytes (its rows are copied otherwise).
  */
 int bt_cache_head_dim(int dtype, int64_t head_dim);

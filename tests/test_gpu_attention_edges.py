@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from conftest import announce
+from test_attention_infinities import KINDS, check, filled
 from test_gpu_attention import Batch, _ops
 from test_gpu_rotary import U, _half
 
@@ -115,3 +116,19 @@ def test_one_key_far_above_many(dt, new, wide, above):
         assert bool(((out[..., f].double() - want).abs() <= bound).all()), (f, float(((out[..., f].double() - want).abs() / want).max()))
     assert not out[..., 3:].any()
     assert bool(((lse.double() - total.log()).abs() <= off + 4 * U * 18).all())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("kind", KINDS)
+def test_infinite_keys_and_values(kind, dt):
+    """As on the CPU, in both kernels: also with 23 tokens of the sequence in question, of which two that see the places are asked."""
+    announce("infinite", kind, dt)
+    q, kc, vc, table, lengths = filled(kind, dt, "cuda")
+    check(kind, *_ops().cached_attention(q, kc, vc, table, lengths, return_lse=True))
+    starts = torch.tensor([0, 1, 24, 25], dtype=torch.int32, device="cuda")
+    rows = torch.cat((q[:1], q[1:2].expand(23, 2, 16), q[2:]))
+    for width in (2, 1 << 21):  # (so many places that rows are taken as many)
+        wide = torch.cat((table, torch.full((3, width - 2), -7, dtype=torch.int32, device="cuda")), 1)
+        out, lse = _ops().cached_attention(rows, kc, vc, wide, lengths, starts, return_lse=True)
+        for i in (10, 23):  # (their places are the 27th and the last: both see the 21st and 22nd)
+            check(kind, *(torch.stack((t[0], t[i], t[24])) for t in (out, lse)))
