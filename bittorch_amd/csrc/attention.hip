@@ -29,8 +29,8 @@ struct AttendParams {
     int tokens, heads, kv_heads, group, dim, q_dim, dp, n_seq, width, page_shift, pages, prefix;  // q_dim: features that q's rows have in memory
     int longest;
     int few_rows;        // sequences of up to so many rows are attend_rows_kernel's, others attend_tiles_kernel's
-    // of the two kernels: places of a chunk of a sequence, chunks of the longest, and row tiles (few: of each sequence, wide: of all of them)
-    int chunk, chunks, tiles, units, wide_chunk, wide_chunks, wide_tiles;
+    // of the two kernels: places of a chunk of a sequence, chunks of the longest, and row tiles of each sequence of few rows
+    int chunk, chunks, tiles, units, wide_chunk, wide_chunks;
     int all_few;         // every sequence is attend_rows_kernel's, their tiles in units as attend_tiles_kernel's are
     int prefix_chunk, prefix_chunks, prefix_tiles, prefix_wide;  // the prefix, whose rows are tiled by one of them
     Parts few_parts, wide_parts, prefix_parts;       // without: the workgroup sees all keys of its rows
@@ -519,8 +519,8 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
 //
 // What bounds it.  One block of instructions works on three tiles, the products of tile i + 1, the weights of tile i and the sums over the values of
 // tile i - 1, none of which waits for another (one thing after the other took 1.6 times as long).  A tile costs a wave (128 features, 16 bits) 16 matrix
-// instructions of 32 cycles, and about 95 others: 16 exponentials, three or four instructions around each, the rows' maxima.  The matrix unit is busy for 47%
-// of a long call's cycles and the vector unit for 47%, at the 2.0 GHz that such a load leaves; 2 x 1024 tokens of 32 heads see 4096 places
+// instructions of 32 cycles, and about 95 others: 16 exponentials, three or four instructions around each, the rows' maxima.  The matrix unit is busy for 48%
+// of a long call's cycles and the vector unit for 47%, at the 1.9 GHz that such a load leaves; 2 x 1024 tokens of 32 heads see 4096 places
 // more in 126 us, 1.09 PFLOP/s where a large matrix product of a library reaches 1.22.  Matrix instructions of 16 rows take as many cycles and leave the
 // vector instructions less of them (4 x 512 tokens on 2048 places 79 -> 76 us).  LDS is not the bound (its fragments take a fifth of the cycles, and without
 // their reads a tile takes as long); one wait and barrier for two tiles was slower (280 us where this takes 263: half as far ahead), and more
@@ -1228,7 +1228,7 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
     p.prefix = (int)prefix_length;
     p.longest = (int)max_length, p.few_rows = (int)a.few_rows, p.few_slots = (int)a.few_slots, p.join_few = a.join_few;
     p.chunk = (int)a.chunk, p.chunks = (int)a.chunks, p.tiles = (int)a.tiles, p.units = (int)a.units, p.all_few = a.all_few;
-    p.wide_chunk = (int)a.wide_chunk, p.wide_chunks = (int)a.wide_chunks, p.wide_tiles = (int)a.wide_tiles;
+    p.wide_chunk = (int)a.wide_chunk, p.wide_chunks = (int)a.wide_chunks;
     p.prefix_chunk = (int)a.prefix_chunk, p.prefix_chunks = (int)a.prefix_chunks, p.prefix_tiles = (int)a.prefix_tiles, p.prefix_wide = a.prefix_wide;
     p.scale2 = (float)((double)scale * 1.4426950408889634074);
     const int64_t prefix_blocks = a.prefix_tiles * a.prefix_chunks * kv_heads;

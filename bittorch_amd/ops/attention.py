@@ -10,7 +10,7 @@ and values, and the attention of new tokens over it.
 The cache is two tensors ``[pages, kv_heads, page_size, features]`` in an order of its own (the one in which the matrix cores take its values,
 ``include/bittorch_hip.h``); a page can be copied, shared and handed on as a whole.  ``features`` is the head dimension rounded up to 64 bytes.
 Sequence ``s`` owns the pages ``block_table[s]`` and ``lengths[s]`` places in them, its new tokens included: those are the last, and the rows
-``q_starts[s] .. q_starts[s + 1] - 1`` of the call's tokens (without ``q_starts``: one token a sequence).  All three are int32 on the GPU and are read
+``q_starts[s] .. q_starts[s + 1] - 1`` of the call's tokens (ascending from 0; without ``q_starts``: one token a sequence).  All three are int32 on the GPU and are read
 there, so that a captured call follows them.
 """
 
@@ -224,7 +224,11 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: T
     Tokens without a place to see, and rows behind the last sequence, are zero (``-inf``), and so are heads whose logits are all minus infinity; a logit of plus
     infinity, or one that is no number, makes the head not a number, an infinite value that it sees that feature infinite or not a number.  Places that a token does
     not see do not change its result, whatever they hold.  ``max_length``, if given, bounds the sequences' lengths on the host, where ``block_table`` is much wider than they are; tokens of longer sequences, and
-    tokens that see a page outside the cache (others of that sequence may be), are not a number.  All sums in 32 bits.  No gradient.  On the CPU: the same in plain torch operations."""
+    tokens that see a page outside the cache (others of that sequence may be), are not a number.
+
+    Logits, sums and ``lse`` in 32 bits.  16-bit types: the weights are multiplied with the values in two halves of 16 bits where a call has few rows, and rounded to
+    the type once where it has many (results are then 1.4 times as far from 64 bits as by their own rounding).  No gradient.  On the CPU: the same in plain
+    torch operations."""
     from .. import _C
 
     out = _C._N.cached_attention(q, k_cache, v_cache, block_table, lengths, q_starts, scale, prefix_table, prefix_length, return_lse, max_length)
