@@ -132,3 +132,14 @@ def test_infinite_keys_and_values(kind, dt):
         out, lse = _ops().cached_attention(rows, kc, vc, wide, lengths, starts, return_lse=True)
         for i in (10, 23):  # (their places are the 27th and the last: both see the 21st and 22nd)
             check(kind, *(torch.stack((t[0], t[i], t[24])) for t in (out, lse)))
+
+
+def test_the_same_bits_on_every_call():
+    """Both kernels and every join, called again between other work."""
+    for held, new, prefix in (([2000] * 20, [1] * 20, 5000), ([1500, 900, 700, 1200], [256] * 4, 0), ([30000], [1], 0), ([700, 300, 5], [200, 9, 1], 2500)):
+        b = Batch(held, new, 8, 2, 128, 64, torch.bfloat16, prefix)
+        for wide in (False, True):
+            first = b.widened(wide).attend(return_lse=True)
+            for _ in range(8):
+                torch.randn(1 << 22, device="cuda").sort()
+                assert all(torch.equal(x, y) for x, y in zip(first, b.attend(return_lse=True)))
