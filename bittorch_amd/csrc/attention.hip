@@ -259,12 +259,13 @@ struct PageWindow {
         return __builtin_amdgcn_readlane(page, number - first);
     }
 };
-// The rows behind the last sequence, where no job sees to them
+// The rows behind the last sequence, where no job sees to them: the share of workgroup `block` of `blocks`
 template <int DT>
-__device__ __forceinline__ void clear_rows_behind(const AttendParams& p) {
-    const int64_t n = (int64_t)p.heads * p.dim, behind = std::max(0, std::min(p.starts[p.n_seq], p.tokens));
-    for (int64_t i = behind * n + threadIdx.x; i < p.tokens * n; i += blockDim.x) store_elem<DT>(p.out, i, 0.0f);
-    for (int64_t i = behind * p.heads + threadIdx.x; p.lse && i < p.tokens * p.heads; i += blockDim.x) p.lse[i] = -__builtin_inff();
+__device__ __forceinline__ void clear_rows_behind(const AttendParams& p, uint32_t block, uint32_t blocks) {
+    const int64_t n = (int64_t)p.heads * p.dim, behind = std::max(0, std::min(p.starts[p.n_seq], p.tokens)), at = (int64_t)block * blockDim.x + threadIdx.x,
+                  step = (int64_t)blocks * blockDim.x;
+    for (int64_t i = behind * n + at; i < p.tokens * n; i += step) store_elem<DT>(p.out, i, 0.0f);
+    for (int64_t i = behind * p.heads + at; p.lse && i < (int64_t)p.tokens * p.heads; i += step) p.lse[i] = -__builtin_inff();
 }
 // Of the row with group_row `in_group`: where its q starts, and E features of it from f on (zero behind the head)
 __device__ __forceinline__ int64_t q_row(const AttendParams& p, const Job& j, int r, int in_group) {
@@ -347,7 +348,10 @@ __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(Attend
             const uint32_t at = block / (uint32_t)p.chunks, unit = at / (uint32_t)p.kv_heads;
             const int c = (int)(block - at * p.chunks);
             j.kv = (int)(at - unit * p.kv_heads);
-            if ((int)unit >= p.units) return clear_rows_behind<DT>(p);
+            if ((int)unit >= p.units) {
+                const uint32_t jobs = prefix_blocks + (uint32_t)p.units * p.kv_heads * p.chunks;
+                return clear_rows_behind<DT>(p, blockIdx.x - jobs, gridDim.x - jobs);
+            }
             int s = (int)(unit / (uint32_t)p.tiles), tile = (int)unit - s * p.tiles;
             if (p.all_few && !tile_of(p, R, unit, &s, &tile)) return;
             asked = PageWindow::ask(p.table + (int64_t)s * p.width, p.width, (c * p.chunk) >> p.page_shift);
@@ -1233,7 +1237,7 @@ extern "C" int bt_cached_attention(const void* q, int64_t q_token, int64_t q_hea
     p.scale2 = (float)((double)scale * 1.4426950408889634074);
     const int64_t prefix_blocks = a.prefix_tiles * a.prefix_chunks * kv_heads;
     const bool clear = q_starts && (a.join_few || (!a.few_parts && !a.wide_parts));  // (attend_join_kernel sees to the rows behind otherwise)
-    const int64_t few_blocks = (a.few ? a.units * a.chunks * kv_heads : 0) + (a.prefix_wide ? 0 : prefix_blocks) + (clear ? 1 : 0);
+    const int64_t few_blocks = (a.few ? a.units * a.chunks * kv_heads : 0) + (a.prefix_wide ? 0 : prefix_blocks) + (clear ? clearing_blocks(tokens * heads * head_dim) : 0);
     const int64_t wide_blocks = (a.wide ? a.wide_tiles * a.wide_chunks * kv_heads : 0) + (a.prefix_wide ? prefix_blocks : 0);
     const int64_t join_rows = a.join_few ? a.few_region.rows : a.few_parts || a.wide_parts ? tokens * heads : 0;
     if (std::max({few_blocks, wide_blocks, join_rows / 4}) >= (1 << 24) || a.units > 0x7fffffff || a.wide_tiles > 0x7fffffff || a.prefix_tiles > 0x7fffffff) {

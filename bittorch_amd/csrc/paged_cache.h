@@ -35,6 +35,13 @@ static inline int cache_head_dim(int dt, int64_t d) {
     return (int)(ceil_div(d, unit) * unit);
 }
 
+// Workgroups that clear the rows behind the last sequence, of so many elements if there is no sequence at all (8128 of 8192 tokens of 32 heads of
+// 128: the attention takes 67 us, the append 19; with one workgroup for all of them 3.3 and 4.1 ms)
+static inline int64_t clearing_blocks(int64_t elements) {
+    const int64_t n = ceil_div(elements, 8192);
+    return n < 1 ? 1 : n > 256 ? 256 : n;
+}
+
 // Which sequence token t belongs to: starts[s] <= t < starts[s + 1], or -1.  All lanes of a wave; one load for 64 sequences.
 __device__ __forceinline__ int owner_of(const int32_t* starts, int n_seq, int64_t t) {
     const int lane = threadIdx.x & 63;

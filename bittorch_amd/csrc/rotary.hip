@@ -143,7 +143,6 @@ __global__ __launch_bounds__(TURN_THREADS) void cache_append_kernel(TurnParams p
     constexpr int E = Order::E;
     __shared__ float2 turn[TURN_ANGLES];
     if ((int)blockIdx.x >= p.units) {
-        if (!p.q || !p.starts) return;
         const int64_t n = (int64_t)p.hq * p.dim, behind = std::max<int64_t>(0, std::min<int64_t>(p.starts[p.n_seq], p.tokens));
         const int64_t step = (int64_t)(gridDim.x - p.units) * gridDim.y * TURN_THREADS;
         for (int64_t i = behind * n + ((int64_t)(blockIdx.x - p.units) * gridDim.y + blockIdx.y) * TURN_THREADS + threadIdx.x; i < p.tokens * n; i += step)
@@ -306,7 +305,8 @@ static void launch_cache_append(TurnParams& p, hipStream_t st) {
     p.units = (int)(p.starts ? p.tokens / E + 2 * (int64_t)p.n_seq : p.n_seq);
     const int64_t per_unit = (p.starts ? std::min<int64_t>(E, ceil_div(p.tokens, p.n_seq)) : 1) * (int64_t)p.slots.d * p.per_head.d + (int64_t)p.hk * p.by_dim.d;
     const int64_t shares = std::min<int64_t>(ceil_div(per_unit, TURN_THREADS), std::max<int64_t>(1, APPEND_BLOCKS / p.units));
-    const dim3 grid((unsigned)(p.units + (p.starts ? 1 : 0)), (unsigned)std::min<int64_t>(shares, 65535));
+    const int64_t clearing = p.starts && p.q ? ceil_div(clearing_blocks(p.tokens * p.hq * p.dim), shares) : 0;
+    const dim3 grid((unsigned)(p.units + clearing), (unsigned)std::min<int64_t>(shares, 65535));
     if (two) hipLaunchKernelGGL((cache_append_kernel<DT, E, DT == BT_F32 ? 1 : 2>), grid, dim3(TURN_THREADS), 0, st, p);
     else if (vec) hipLaunchKernelGGL((cache_append_kernel<DT, E, 1>), grid, dim3(TURN_THREADS), 0, st, p);
     else hipLaunchKernelGGL((cache_append_kernel<DT, 1, 1>), grid, dim3(TURN_THREADS), 0, st, p);

@@ -143,3 +143,27 @@ def test_the_same_bits_on_every_call():
             for _ in range(8):
                 torch.randn(1 << 22, device="cuda").sort()
                 assert all(torch.equal(x, y) for x, y in zip(first, b.attend(return_lse=True)))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("tokens", [70, 4001, 70000])
+def test_a_batch_that_is_mostly_padding(dt, tokens):
+    """Rows behind the last sequence: up to many times the batch, all of them cleared, whatever they held."""
+    announce("padding", tokens, dt)
+    ops = _ops()
+    b = Batch([40, 10, 33], [1, 9, 2], 3, 1, 33, 32, dt)
+    want, want_lse = b.attend(return_lse=True)
+    f = ops.rotary_frequencies(32, device="cuda")[0]
+    q = torch.full((tokens, 3, 33), math.nan, dtype=dt, device="cuda")
+    q[:12] = b.q
+    k, v = (torch.randn(tokens, 1, 33, device="cuda").to(dt) for _ in range(2))
+    for _ in range(2):
+        held = [torch.full((tokens, 3, 33), math.nan, dtype=dt, device="cuda") for _ in range(3)]  # (what the results' memory holds)
+        del held
+        out, lse = b.attend(q, return_lse=True)
+        assert not out[12:].any() and bool((lse[12:] == -math.inf).all())
+        b.check(out, lse)
+        assert torch.equal(out[:12], want) and torch.equal(lse[:12], want_lse)
+        kc, vc = b.k_cache.clone(), b.v_cache.clone()
+        turned = ops.cache_append(k, v, kc, vc, b.table, b.lengths, b.q_starts, q, f)
+        assert not turned[12:].any() and bool(turned[:12].isfinite().all())
