@@ -326,7 +326,7 @@ __device__ __forceinline__ void put_row(const AttendParams& p, const Job& j, int
 // Bound by the cache's bytes: keys and values go straight to registers, past the caches (no other workgroup wants them), the next tile's while this
 // one is worked on, three workgroups to a compute unit (64 sequences of 1046 to 4022 places, 32 heads on 8, 118 us, 5.7 TB/s; without the two 133; one
 // of 100000 places 64 us, 6.4 TB/s).  At little work it is the chain of loads, products and joins: 500 places of one sequence 8.2 us, 120 places 5.5
-// (eight waves: 7.6, 5.6).
+// (eight waves: 7.6, 5.6).  fp32 heads of 97 to 128 features keep 7 of their registers in scratch memory.
 template <int DT, int B>
 __global__ __launch_bounds__(256, B <= 4 ? 3 : 1) void attend_rows_kernel(AttendParams p) {
     using Order = CacheOrder<DT>;

@@ -6,7 +6,7 @@
 //
 // Both kernels are bound by memory (5 operations an element) if the angles are not formed for every head anew: a workgroup takes a few
 // tokens, forms their cosines and sines once in LDS and walks the pieces (16 bytes of either half of the pairs) of all their heads.  bf16: 4096
-// tokens x 40 heads of 128 17 to 18 us (4.6 to 4.9 TB/s), the prompts of 8 x 512 tokens, 20 + 20 heads, to the cache 31 us (4.1 TB/s).
+// tokens x 40 heads of 128 17 to 18 us (4.6 to 4.9 TB/s), the prompts of 8 x 512 tokens, 20 + 20 heads, to the cache 28 us (4.4 TB/s).
 #include "paged_cache.h"
 
 namespace bt {
