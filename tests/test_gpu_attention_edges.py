@@ -49,7 +49,7 @@ def test_a_page_outside_the_cache_behind_64_others(dt, held):
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("prefix", [2049, 2090])
 def test_a_prefix_page_outside_the_cache_behind_64_others(dt, prefix):
-    """200 rows tokens of 4 heads a group and 8 key heads: a workgroup sees the whole prefix."""
+    """200 tokens of 4 heads to each of 8 key heads: a workgroup sees the whole prefix."""
     announce("bad prefix page", prefix, dt)
     b = Batch([30] * 200, [1] * 200, 32, 8, 64, 32, dt, prefix)
     b.check(*b.attend(starts=False, return_lse=True))
