@@ -157,12 +157,15 @@ def _tiled(k: Tensor, v: Tensor) -> Tuple[Tensor, Tensor]:
 
 
 def cache_read(k_cache: Tensor, v_cache: Tensor, pages: Tensor, length: int, head_dim: int) -> Tuple[Tensor, Tensor]:
-    """What the first ``length`` places of ``pages`` (a row of a block table) hold: keys and values ``[length, kv_heads, head_dim]``."""
+    """What the first ``length`` places of ``pages`` (a row of a block table) hold: keys and values ``[length, kv_heads, head_dim]``.  Places on pages outside
+    the cache are not a number."""
     page = k_cache.shape[2]
     if not 0 <= length <= pages.numel() * page or not 0 < head_dim <= k_cache.shape[3]:
         raise RuntimeError("length or head_dim is beyond the pages")
-    index = pages[:(length + page - 1) // page].long()
-    return tuple(t.transpose(1, 2).flatten(0, 1)[:length, :, :head_dim] for t in _natural(k_cache[index], v_cache[index]))
+    index, last = pages[:(length + page - 1) // page].long(), k_cache.shape[0] - 1
+    wrong, index = ((index < 0) | (index > last))[:, None, None, None], index.clamp(0, last)
+    k, v = _natural(*(t[index].masked_fill(wrong, math.nan) for t in (k_cache, v_cache)))
+    return tuple(t.transpose(1, 2).flatten(0, 1)[:length, :, :head_dim] for t in (k, v))
 
 
 def _refuse_gradients(*tensors: Optional[Tensor]) -> None:
